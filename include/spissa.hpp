@@ -181,6 +181,15 @@ class KvCache {
     if (r.is_err()) return r.error();
     return KvCache(h);
   }
+  // A cache held in 4 bits (spissa_kv_cache_q4_new): read by the fused steps and
+  // the append-first attention, which the calls with current rows refuse.
+  static Result<KvCache> create_q4(size_t num_heads, size_t head_dim, size_t max_seq_len) {
+    spissa_kv_cache *h = nullptr;
+    auto r = detail::check(spissa_kv_cache_q4_new(num_heads, head_dim, max_seq_len, &h));
+    if (r.is_err()) return r.error();
+    return KvCache(h);
+  }
+  bool is_q4() const { return spissa_kv_cache_is_q4(h_) != 0; }
   KvCache() = default;
   KvCache(KvCache &&o) noexcept : h_(o.h_) { o.h_ = nullptr; }
   KvCache &operator=(KvCache &&o) noexcept {
@@ -222,6 +231,10 @@ class KvCache {
   // Device tier: token_count rows [token_count, H, d] already on the device.
   Result<void> append_device(const float *d_keys, const float *d_values, size_t token_count) {
     return detail::check(spissa_kv_cache_append_device(h_, d_keys, d_values, token_count));
+  }
+  // Rows [first, first + count) as f32 into device buffers (either may be null).
+  Result<void> rows_device(size_t first, size_t count, float *d_keys, float *d_values) const {
+    return detail::check(spissa_kv_cache_rows_device(h_, first, count, d_keys, d_values));
   }
 
  private:
@@ -543,6 +556,20 @@ class Session {
     auto r = detail::check(spissa_kv_cache_new_in(s_, num_heads, head_dim, max_seq_len, &h));
     if (r.is_err()) return r.error();
     return KvCache(h);
+  }
+  Result<KvCache> kv_cache_q4(size_t num_heads, size_t head_dim, size_t max_seq_len) const {
+    spissa_kv_cache *h = nullptr;
+    auto r = detail::check(spissa_kv_cache_q4_new_in(s_, num_heads, head_dim, max_seq_len, &h));
+    if (r.is_err()) return r.error();
+    return KvCache(h);
+  }
+  // Append-first attention of one token of each sequence over 4-bit caches.
+  Result<void> attention_cached_batch(const float *d_q, const std::vector<const KvCache *> &caches,
+                                      const KvAttentionConfig &config, float *d_out) {
+    std::vector<const spissa_kv_cache *> raw;
+    for (const KvCache *c : caches) raw.push_back(c->raw());
+    const spissa_kv_attention_config c = config.c();
+    return detail::check(spissa_attention_cached_batch_device(s_, d_q, raw.data(), raw.size(), &c, d_out));
   }
   // freq_scale: Llama per-pair scales (nullptr = None); position_divisor: Gemma only.
   Result<RopeTable> rope_table(RopeKind kind, size_t rotary_dim, float base, size_t max_positions,

@@ -107,6 +107,47 @@ int spissa_kv_cache_read_values(const spissa_kv_cache *c, float *dst, size_t dst
 /* Device base pointers of the resident buffers (fast path, no reference counterpart). */
 const float *spissa_kv_cache_device_keys(const spissa_kv_cache *c);
 const float *spissa_kv_cache_device_values(const spissa_kv_cache *c);
+/* Rows [first, first + count) of the cache as f32 [count, num_heads, head_dim]
+ * device buffers (either may be NULL), asynchronous on the stream of the
+ * cache's session. No reference counterpart. */
+int spissa_kv_cache_rows_device(const spissa_kv_cache *c, size_t first, size_t count, float *d_keys,
+                                float *d_values);
+
+/* A KV cache held in 4 bits: 0.625 bytes a channel against four, so a decode
+ * step reads 6.4 times less and a device holds as many more tokens. No
+ * reference counterpart. Of each token and head, every 32 channels of a key or
+ * value row have a minimum and a step of their own in binary16:
+ *   min = half(lo), step = half((hi - lo) * (1/15)),
+ *   code = clamp(rne((x - min) * (1 / step)), 0, 15)  (0 where step is 0),
+ *   value = min + step * code,
+ * each operation rounded to f32. head_dim 64, 128 or 256, max_seq_len up to
+ * 2^24 (SHAPE otherwise).
+ *
+ * The handle is a spissa_kv_cache: append, append_device, clear, truncate,
+ * clone, the accessors, read_keys / read_values and rows_device (which give the
+ * values back that the codes stand for) take it; device_keys and device_values
+ * are NULL. A value that is not finite or beyond 65504 is INVALID_TENSOR_DATA:
+ * spissa_kv_cache_append refuses the rows, the device calls append them with
+ * that value replaced by a finite one and the next spissa_session_sync()
+ * reports it.
+ *
+ * Attention reads every key as the cache holds it, the new rows included
+ * (append first), so a prompt's results do not depend on its chunks beyond
+ * rounding: spissa_attention_cached_device (from one query on),
+ * spissa_attention_cached_batch_device, the fused spissa_{,gemma_}decode_step_device
+ * and spissa_{,gemma_}prefill_step_device, and spissa_attention_sublayer_device.
+ * In the Gemma steps the QK-norm's sums of squares are taken as a tree. Sums,
+ * products and softmax are f32 (prefill precision does not matter here). The
+ * calls that take current rows beside the cache (spissa_attention_device,
+ * spissa_attention_decode_batch_device,
+ * spissa_scaled_dot_product_attention_with_cache) and
+ * spissa_decode_step_device_noalloc refuse it (ARGUMENT). Device buffers are
+ * 16-byte aligned (ARGUMENT otherwise). spissa_plan_attention describes f32
+ * caches. */
+int spissa_kv_cache_q4_new(size_t num_heads, size_t head_dim, size_t max_seq_len, spissa_kv_cache **out);
+int spissa_kv_cache_q4_new_in(spissa_session *s, size_t num_heads, size_t head_dim, size_t max_seq_len,
+                              spissa_kv_cache **out);
+int spissa_kv_cache_is_q4(const spissa_kv_cache *c);
 
 /* ------------------------------------------------------------------------ */
 /* RoPE: rotary.rs:6-193                                                    */
@@ -331,9 +372,18 @@ int spissa_gemma_prefill_step_device(spissa_session *s, const spissa_rope_table 
  * spissa_attention_device(q, k, v, cache truncated to len - S, cfg) with the
  * chunk's k/v passed as current rows; this is the fused prefill step's
  * attention launch on its own. query_len > 1, bf16 prefill at head_dim 64,
- * 128 or 256 (SHAPE otherwise); len >= query_len. */
+ * 128 or 256 (SHAPE otherwise); len >= query_len. A 4-bit cache takes
+ * query_len 1 too. */
 int spissa_attention_cached_device(spissa_session *s, const float *d_q, spissa_kv_cache *cache,
                                    const spissa_kv_attention_config *cfg, float *d_out);
+
+/* The same for one token of each of `batch` sequences (cfg->query_len == 1)
+ * over 4-bit caches: d_q [batch, Hq, D], sequence b's own row is the last of
+ * caches[b]. A cache may be listed several times (queries that share a
+ * context). f32 caches are refused (ARGUMENT): spissa_decode_step_device and
+ * spissa_attention_decode_batch_device are their calls. */
+int spissa_attention_cached_batch_device(spissa_session *s, const float *d_q, const spissa_kv_cache *const *caches,
+                                         size_t batch, const spissa_kv_attention_config *cfg, float *d_out);
 
 /* ops.rs:237-291 scaled_dot_product_attention (cacheless MHA, f32). */
 int spissa_scaled_dot_product_attention(const float *q, size_t q_len, const float *k,

@@ -186,6 +186,13 @@ pub mod sys {
         pub fn spissa_kv_cache_read_values(c: *const spissa_kv_cache, dst: *mut f32, dst_len: usize) -> c_int;
         pub fn spissa_kv_cache_device_keys(c: *const spissa_kv_cache) -> *const f32;
         pub fn spissa_kv_cache_device_values(c: *const spissa_kv_cache) -> *const f32;
+        pub fn spissa_kv_cache_rows_device(c: *const spissa_kv_cache, first: usize, count: usize, d_keys: *mut f32,
+                                           d_values: *mut f32) -> c_int;
+        pub fn spissa_kv_cache_q4_new(num_heads: usize, head_dim: usize, max_seq_len: usize,
+                                      out: *mut *mut spissa_kv_cache) -> c_int;
+        pub fn spissa_kv_cache_q4_new_in(s: *mut spissa_session, num_heads: usize, head_dim: usize, max_seq_len: usize,
+                                         out: *mut *mut spissa_kv_cache) -> c_int;
+        pub fn spissa_kv_cache_is_q4(c: *const spissa_kv_cache) -> c_int;
 
         // RoPE (rotary.rs:6-193)
         pub fn spissa_gpt_neox_rotary_dim(head_dim: usize, rotary_pct: f32, out: *mut usize) -> c_int;
@@ -259,6 +266,9 @@ pub mod sys {
                                                 cfg: *const spissa_kv_attention_config, d_q_norm: *const f32,
                                                 d_k_norm: *const f32, eps: f32, q_prescale: f32,
                                                 d_out: *mut f32) -> c_int;
+        pub fn spissa_attention_cached_batch_device(s: *mut spissa_session, d_q: *const f32,
+                                                    caches: *const *const spissa_kv_cache, batch: usize,
+                                                    cfg: *const spissa_kv_attention_config, d_out: *mut f32) -> c_int;
         pub fn spissa_attention_cached_device(s: *mut spissa_session, d_q: *const f32, cache: *mut spissa_kv_cache,
                                               cfg: *const spissa_kv_attention_config, d_out: *mut f32) -> c_int;
         pub fn spissa_scaled_dot_product_attention(q: *const f32, q_len: usize, k: *const f32, k_len: usize,
@@ -459,6 +469,30 @@ impl DeviceKvCache {
         let mut h = std::ptr::null_mut();
         check(unsafe { sys::spissa_kv_cache_new_in(session.raw, num_heads, head_dim, max_seq_len, &mut h) })?;
         Ok(Self(h))
+    }
+    /// A cache held in 4 bits (0.625 bytes a channel; head_dim 64, 128 or 256).
+    /// Attention reads it append first: the fused steps,
+    /// `attention_cached_batch` and `spissa_attention_cached_device`.
+    pub fn new_q4(num_heads: usize, head_dim: usize, max_seq_len: usize) -> Result<Self> {
+        let mut h = std::ptr::null_mut();
+        check(unsafe { sys::spissa_kv_cache_q4_new(num_heads, head_dim, max_seq_len, &mut h) })?;
+        Ok(Self(h))
+    }
+    /// The same, bound to `session` (for the device tier).
+    pub fn new_q4_in(session: &Session, num_heads: usize, head_dim: usize, max_seq_len: usize) -> Result<Self> {
+        let mut h = std::ptr::null_mut();
+        check(unsafe { sys::spissa_kv_cache_q4_new_in(session.raw, num_heads, head_dim, max_seq_len, &mut h) })?;
+        Ok(Self(h))
+    }
+    pub fn is_q4(&self) -> bool {
+        unsafe { sys::spissa_kv_cache_is_q4(self.0) != 0 }
+    }
+    /// Rows [first, first + count) as f32, on the stream of the cache's session.
+    ///
+    /// # Safety
+    /// Each pointer is null or device memory of count * num_heads * head_dim floats.
+    pub unsafe fn rows_device(&self, first: usize, count: usize, d_keys: *mut f32, d_values: *mut f32) -> Result<()> {
+        check(sys::spissa_kv_cache_rows_device(self.0, first, count, d_keys, d_values))
     }
     /// rotary.rs:226-256 KvCache::append (validates before mutating).
     pub fn append(&mut self, keys: &[f32], values: &[f32], token_count: usize) -> Result<()> {
@@ -765,6 +799,17 @@ pub unsafe fn attention_device(session: &Session, d_q: *const f32, d_k: *const f
                                cache: Option<&DeviceKvCache>, cfg: &AttnConfigC, d_out: *mut f32) -> Result<()> {
     check(sys::spissa_attention_device(session.raw, d_q, d_k, d_v, cache.map_or(std::ptr::null(), |c| c.raw()), cfg,
                                        d_out))
+}
+
+/// Append-first attention of one token of each of `caches.len()` sequences over
+/// 4-bit caches (the token's own row is the cache's last).
+///
+/// # Safety
+/// d_q and d_out [caches.len(), Hq, d] device buffers, 16-byte aligned.
+pub unsafe fn attention_cached_batch(session: &Session, d_q: *const f32, caches: &[&DeviceKvCache], cfg: &AttnConfigC,
+                                     d_out: *mut f32) -> Result<()> {
+    let ptrs: Vec<*const sys::spissa_kv_cache> = caches.iter().map(|c| c.raw()).collect();
+    check(sys::spissa_attention_cached_batch_device(session.raw, d_q, ptrs.as_ptr(), ptrs.len(), cfg, d_out))
 }
 
 // ---- projections, LM head and sampling ----

@@ -13,7 +13,7 @@ from .linear import (LinearModel, LinearWeight, StreamingLinearConfig,  # noqa: 
 from .ops import is_global_layer, rms_norm, scaled_dot_product_attention  # noqa: F401
 from .sampling import (lm_head_logits_parallel, lm_head_logits_parallel_bf16,  # noqa: F401
                        sample_argmax, sample_argmax_excluding)
-from .rotary import (KvAttentionConfig, KvCache, RotaryEmbeddingConfig,  # noqa: F401
+from .rotary import (KvAttentionConfig, KvCache, Q4KvCache, RotaryEmbeddingConfig,  # noqa: F401
                      apply_gemma_rotary_inplace, apply_gpt_neox_rotary_inplace,
                      apply_llama_rotary_inplace, gpt_neox_rotary_dim,
                      scaled_dot_product_attention_with_cache)

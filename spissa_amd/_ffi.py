@@ -137,6 +137,10 @@ SIGNATURES = {
     "spissa_kv_cache_read_values": (C.c_int, [c_void_p, c_float_p, c_size]),
     "spissa_kv_cache_device_keys": (c_void_p, [c_void_p]),
     "spissa_kv_cache_device_values": (c_void_p, [c_void_p]),
+    "spissa_kv_cache_rows_device": (C.c_int, [c_void_p, c_size, c_size, c_void_p, c_void_p]),
+    "spissa_kv_cache_q4_new": (C.c_int, [c_size, c_size, c_size, C.POINTER(c_void_p)]),
+    "spissa_kv_cache_q4_new_in": (C.c_int, [c_void_p, c_size, c_size, c_size, C.POINTER(c_void_p)]),
+    "spissa_kv_cache_is_q4": (C.c_int, [c_void_p]),
     "spissa_gpt_neox_rotary_dim": (C.c_int, [c_size, C.c_float, C.POINTER(c_size)]),
     "spissa_apply_gpt_neox_rotary_inplace": (
         C.c_int, [c_float_p, c_size, c_float_p, c_size, C.POINTER(RotaryConfigC)]),
@@ -200,6 +204,8 @@ SIGNATURES = {
         C.c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, C.POINTER(AttnConfigC), c_void_p]),
     "spissa_attention_cached_device": (
         C.c_int, [c_void_p, c_void_p, c_void_p, C.POINTER(AttnConfigC), c_void_p]),
+    "spissa_attention_cached_batch_device": (
+        C.c_int, [c_void_p, c_void_p, C.POINTER(c_void_p), c_size, C.POINTER(AttnConfigC), c_void_p]),
     "spissa_scaled_dot_product_attention": (
         C.c_int,
         [c_float_p, c_size, c_float_p, c_size, c_float_p, c_size, c_size, c_size, c_size, C.c_int,

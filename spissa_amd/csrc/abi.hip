@@ -115,6 +115,7 @@ struct spissa_session {
   DevBuf sub;       // attention sublayer intermediates (normed x, q, k, v, attention, projection)
   DevBuf amax;      // argmax partials
   DevBuf qstage;    // fused prefill step: bf16 Q operand
+  DevBuf q4q;       // fused steps on a 4-bit cache: the rotated queries
   float *lin = nullptr;  // partial sums of projections whose K is split over workgroups (linear_partials)
   std::mutex lin_mutex;  // held over the launches that write and read them
   float *scratch = nullptr;  // this device's copy of `scratch` (kScratchBytes)
@@ -138,7 +139,16 @@ struct spissa_kv_cache {
   bf16 *kb = nullptr;       // bf16 shadow [H, cap, D], allocated at first prefill use
   bf16 *vt = nullptr;       // bf16 shadow [H, D, cap]
   size_t shadow_cap = 0;
+  // Held in 4 bits (then none of the above): codes, and each 32 channels' step
+  // and minimum, of keys and values (q4_cache.hip), one allocation at kc.
+  bool q4 = false;
+  unsigned char *kc = nullptr, *vc = nullptr;
+  unsigned *kp = nullptr, *vp = nullptr;
+  float *vmax = nullptr;    // [H]
   size_t width() const { return num_heads * head_dim; }
+  // bytes of keys or values that `rows` rows take in 4 bits
+  size_t q4_codes(size_t rows) const { return rows * num_heads * (head_dim / 2); }
+  size_t q4_params(size_t rows) const { return rows * num_heads * (head_dim / 32) * sizeof(unsigned); }
 };
 
 struct spissa_rope_table {
@@ -219,6 +229,7 @@ static void session_free(spissa_session *s) {
   free_buf(s->sub);
   free_buf(s->amax);
   free_buf(s->qstage);
+  free_buf(s->q4q);
   for (void *p : s->retired) (void)hipFree(p);
   if (s->d_err) (void)hipFree(s->d_err);
   if (s->lin) (void)hipFree(s->lin);
@@ -273,6 +284,9 @@ extern "C" int spissa_session_sync(spissa_session *s) {
     HIP_TRY(hipStreamSynchronize(s->stream));
     if (flag & kDevErrSoftmaxDenominator)
       return set_err(SPISSA_ERR_INVALID_TENSOR_DATA, "softmax produced invalid denominator");
+    if (flag & kDevErrCacheValue)
+      return set_err(SPISSA_ERR_INVALID_TENSOR_DATA,
+                     "a key or value appended to a 4-bit cache is not finite or beyond 65504");
     return set_err(SPISSA_ERR_DEVICE, "device error flag 0x%x", flag);
   }
   return SPISSA_OK;
@@ -411,6 +425,77 @@ extern "C" int spissa_kv_cache_new(size_t num_heads, size_t head_dim, size_t max
   GUARD_END
 }
 
+// Rows a head of a 4-bit cache may have: the byte offset of a row within its
+// head stays far below 2^32, and tokens of one append within the grid.
+constexpr size_t kQ4MaxRows = (size_t)1 << 24;
+
+static int kv_q4_validate(size_t num_heads, size_t head_dim, size_t max_seq_len) {
+  ST_TRY(kv_validate_new(num_heads, head_dim, max_seq_len));
+  if (!q4_supported(head_dim))
+    return set_err(SPISSA_ERR_SHAPE, "a 4-bit cache holds heads of 64, 128 or 256 channels, got %zu", head_dim);
+  if (max_seq_len > kQ4MaxRows || num_heads > 65535)
+    return set_err(SPISSA_ERR_SHAPE, "a 4-bit cache holds up to %zu rows of up to 65535 heads, got %zu of %zu", kQ4MaxRows,
+                   max_seq_len, num_heads);
+  return SPISSA_OK;
+}
+
+static int kv_q4_new_impl(spissa_session *s, size_t num_heads, size_t head_dim, size_t max_seq_len,
+                          spissa_kv_cache **out) {
+  std::unique_ptr<spissa_kv_cache> c(new spissa_kv_cache());
+  c->session = s;
+  c->num_heads = num_heads;
+  c->head_dim = head_dim;
+  c->max_seq_len = max_seq_len;
+  c->q4 = true;
+  const size_t codes = c->q4_codes(max_seq_len), params = c->q4_params(max_seq_len);
+  const size_t bytes = 2 * (codes + params) + num_heads * sizeof(float);
+  HIP_TRY(hipSetDevice(s->device));
+  ST_TRY(no_capture(s->stream, "a 4-bit cache", bytes));
+  HIP_TRY(hipMalloc(&c->kc, bytes));
+  c->vc = c->kc + codes;
+  c->kp = (unsigned *)(c->vc + codes);  // (codes are whole 32-byte rows)
+  c->vp = (unsigned *)((char *)c->kp + params);
+  c->vmax = (float *)((char *)c->vp + params);
+  hipError_t e = hipMemsetAsync(c->vmax, 0, num_heads * sizeof(float), s->stream);
+  if (e == hipSuccess) e = hipStreamSynchronize(s->stream);
+  if (e != hipSuccess) {
+    (void)hipFree(c->kc);
+    return set_err(SPISSA_ERR_DEVICE, "clearing a 4-bit cache failed: %s", hipGetErrorString(e));
+  }
+  *out = c.release();
+  session_retain(s);
+  return SPISSA_OK;
+}
+
+extern "C" int spissa_kv_cache_q4_new_in(spissa_session *s, size_t num_heads, size_t head_dim, size_t max_seq_len,
+                                         spissa_kv_cache **out) {
+  GUARD_BEGIN
+  if (!s || !out) return set_err(SPISSA_ERR_ARGUMENT, "null argument");
+  *out = nullptr;
+  ST_TRY(kv_q4_validate(num_heads, head_dim, max_seq_len));
+  return kv_q4_new_impl(s, num_heads, head_dim, max_seq_len, out);
+  GUARD_END
+}
+
+extern "C" int spissa_kv_cache_q4_new(size_t num_heads, size_t head_dim, size_t max_seq_len, spissa_kv_cache **out) {
+  GUARD_BEGIN
+  if (!out) return set_err(SPISSA_ERR_ARGUMENT, "out is null");
+  *out = nullptr;
+  ST_TRY(kv_q4_validate(num_heads, head_dim, max_seq_len));
+  spissa_session *s = nullptr;
+  ST_TRY(spissa_default_session(&s));
+  return kv_q4_new_impl(s, num_heads, head_dim, max_seq_len, out);
+  GUARD_END
+}
+
+extern "C" int spissa_kv_cache_is_q4(const spissa_kv_cache *c) { return c && c->q4 ? 1 : 0; }
+
+static Q4Rows q4_rows(const spissa_kv_cache *c, size_t first) {
+  return Q4Rows{c->kc, c->vc, c->kp, c->vp, c->vmax, (long)c->max_seq_len, (int)first, 0};
+}
+
+static bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
 static void kv_release(spissa_kv_cache *c) {
   (void)hipSetDevice(c->session->device);
   (void)hipStreamSynchronize(c->session->stream);
@@ -418,6 +503,7 @@ static void kv_release(spissa_kv_cache *c) {
   if (c->values) (void)hipFree(c->values);
   if (c->kb) (void)hipFree(c->kb);
   if (c->vt) (void)hipFree(c->vt);
+  if (c->kc) (void)hipFree(c->kc);
 }
 
 extern "C" void spissa_kv_cache_free(spissa_kv_cache *c) {
@@ -475,6 +561,46 @@ static int kv_validate_append(const spissa_kv_cache *c, size_t keys_len, size_t 
   return SPISSA_OK;
 }
 
+// The QK-norm of the fused Gemma steps.
+struct GemmaQkNorm {
+  const float *q_norm, *k_norm;
+  float eps, q_prescale;
+};
+
+// Appends S rows to each of B 4-bit caches (several: S is 1), from q (null:
+// none), k and v as Q4AppendArgs has them. The lengths are the caller's to move.
+static int q4_append(spissa_session *s, spissa_kv_cache *const *caches, size_t B, size_t S, const float *q, size_t Hq,
+                     const float *k, const float *v, const spissa_rope_table *table, const GemmaQkNorm *norm,
+                     float *q_out) {
+  const size_t H = caches[0]->num_heads, D = caches[0]->head_dim;
+  const size_t per = (q ? Hq : 0) + 2 * H;
+  const size_t most = std::max<size_t>(1, ((size_t)1 << 29) / per);  // tokens of a launch
+  for (size_t b0 = 0; b0 < B; b0 += kMaxDecodeBatch)
+    for (size_t t0 = 0; t0 < S; t0 += most) {
+      const size_t nb = std::min<size_t>(kMaxDecodeBatch, B - b0), at = b0 * S + t0;
+      Q4AppendArgs a{};
+      a.q = q ? q + at * Hq * D : nullptr;
+      a.k = k + at * H * D;
+      a.v = v + at * H * D;
+      a.q_out = q ? q_out + at * Hq * D : nullptr;
+      a.cos = table ? table->cos : nullptr;
+      a.sin = table ? table->sin : nullptr;
+      if (norm) {
+        a.q_norm = norm->q_norm;
+        a.k_norm = norm->k_norm;
+        a.eps = norm->eps;
+        a.prescale = norm->q_prescale;
+      }
+      a.S = (int)std::min(most, S - t0);
+      a.Hq = q ? (int)Hq : 0;
+      a.Hkv = (int)H;
+      a.err = s->d_err;
+      for (size_t b = 0; b < nb; ++b) a.seq[b] = q4_rows(caches[b0 + b], caches[b0 + b]->len + t0);
+      HIP_TRY(launch_q4_append(s->stream, a, (int)D, (int)nb));
+    }
+  return SPISSA_OK;
+}
+
 extern "C" int spissa_kv_cache_append(spissa_kv_cache *c, const float *keys, size_t keys_len,
                                       const float *values, size_t values_len, size_t token_count) {
   GUARD_BEGIN
@@ -483,6 +609,21 @@ extern "C" int spissa_kv_cache_append(spissa_kv_cache *c, const float *keys, siz
   ST_TRY(kv_validate_append(c, keys_len, values_len, token_count, true, &n, &nl));
   if (!keys || !values) return set_err(SPISSA_ERR_ARGUMENT, "keys/values are null");
   spissa_session *s = c->session;
+  if (c->q4) {
+    for (size_t i = 0; i < n; ++i)
+      if (!(std::fabs(keys[i]) <= 65504.0f) || !(std::fabs(values[i]) <= 65504.0f))
+        return set_err(SPISSA_ERR_INVALID_TENSOR_DATA,
+                       "a key or value appended to a 4-bit cache is not finite or beyond 65504");
+    float *r[2];
+    ST_TRY(io_regions(s, {n, n}, r));
+    HIP_TRY(hipSetDevice(s->device));
+    ST_TRY(h2d(s, r[0], keys, n * sizeof(float)));
+    ST_TRY(h2d(s, r[1], values, n * sizeof(float)));
+    ST_TRY(q4_append(s, &c, 1, token_count, nullptr, 0, r[0], r[1], nullptr, nullptr, nullptr));
+    ST_TRY(sync_stream(s));
+    c->len = nl;
+    return SPISSA_OK;
+  }
   HIP_TRY(hipSetDevice(s->device));
   const size_t off = c->len * c->width();
   ST_TRY(h2d(s, c->keys + off, keys, n * sizeof(float)));
@@ -502,7 +643,14 @@ extern "C" int spissa_kv_cache_append_device(spissa_kv_cache *c, const float *d_
   ST_TRY(kv_validate_append(c, 0, 0, token_count, false, &n, &nl));
   if (!d_keys || !d_values) return set_err(SPISSA_ERR_ARGUMENT, "keys/values are null");
   spissa_session *s = c->session;
+  if (c->q4 && !(aligned16(d_keys) && aligned16(d_values)))
+    return set_err(SPISSA_ERR_ARGUMENT, "a 4-bit cache takes 16-byte aligned rows");
   HIP_TRY(hipSetDevice(s->device));
+  if (c->q4) {
+    ST_TRY(q4_append(s, &c, 1, token_count, nullptr, 0, d_keys, d_values, nullptr, nullptr, nullptr));
+    c->len = nl;
+    return SPISSA_OK;
+  }
   const size_t off = c->len * c->width();
   HIP_TRY(hipMemcpyAsync(c->keys + off, d_keys, n * sizeof(float), hipMemcpyDeviceToDevice, s->stream));
   HIP_TRY(hipMemcpyAsync(c->values + off, d_values, n * sizeof(float), hipMemcpyDeviceToDevice, s->stream));
@@ -536,12 +684,13 @@ extern "C" size_t spissa_kv_cache_head_dim(const spissa_kv_cache *c) { return c 
 extern "C" size_t spissa_kv_cache_resident_bytes(const spissa_kv_cache *c) {
   if (!c) return 0;
   size_t r;
+  if (c->q4) return 2 * (c->q4_codes(c->len) + c->q4_params(c->len));
   if (mul_ovf(c->len, c->width(), &r) || mul_ovf(r, 2, &r) || mul_ovf(r, sizeof(float), &r))
     return (size_t)-1;
   return r;
 }
 
-static int kv_read(const spissa_kv_cache *c, const float *src, float *dst, size_t dst_len) {
+static int kv_read(const spissa_kv_cache *c, bool values, float *dst, size_t dst_len) {
   if (!c) return set_err(SPISSA_ERR_ARGUMENT, "cache is null");
   const size_t n = c->len * c->width();
   if (dst_len < n) return set_err(SPISSA_ERR_SHAPE, "destination holds %zu floats, cache has %zu", dst_len, n);
@@ -549,18 +698,47 @@ static int kv_read(const spissa_kv_cache *c, const float *src, float *dst, size_
   if (!dst) return set_err(SPISSA_ERR_ARGUMENT, "dst is null");
   spissa_session *s = c->session;
   HIP_TRY(hipSetDevice(s->device));
+  const float *src = values ? c->values : c->keys;
+  if (c->q4) {
+    float *r[1];
+    ST_TRY(io_regions(s, {n}, r));
+    HIP_TRY(launch_q4_rows(s->stream, q4_rows(c, 0), c->len, c->num_heads, c->head_dim, values ? nullptr : r[0],
+                           values ? r[0] : nullptr));
+    src = r[0];
+  }
   ST_TRY(d2h(s, dst, src, n * sizeof(float)));
   return sync_stream(s);
 }
 
 extern "C" int spissa_kv_cache_read_keys(const spissa_kv_cache *c, float *dst, size_t dst_len) {
   GUARD_BEGIN
-  return kv_read(c, c ? c->keys : nullptr, dst, dst_len);
+  return kv_read(c, false, dst, dst_len);
   GUARD_END
 }
 extern "C" int spissa_kv_cache_read_values(const spissa_kv_cache *c, float *dst, size_t dst_len) {
   GUARD_BEGIN
-  return kv_read(c, c ? c->values : nullptr, dst, dst_len);
+  return kv_read(c, true, dst, dst_len);
+  GUARD_END
+}
+extern "C" int spissa_kv_cache_rows_device(const spissa_kv_cache *c, size_t first, size_t count, float *d_keys,
+                                           float *d_values) {
+  GUARD_BEGIN
+  if (!c) return set_err(SPISSA_ERR_ARGUMENT, "cache is null");
+  if (first > c->len || count > c->len - first)
+    return set_err(SPISSA_ERR_SHAPE, "rows %zu..+%zu of a cache that holds %zu", first, count, c->len);
+  if (count == 0 || (!d_keys && !d_values)) return SPISSA_OK;
+  spissa_session *s = c->session;
+  if (c->q4 && !(aligned16(d_keys) && aligned16(d_values)))
+    return set_err(SPISSA_ERR_ARGUMENT, "a 4-bit cache gives its rows back to 16-byte aligned buffers");
+  HIP_TRY(hipSetDevice(s->device));
+  if (c->q4) {
+    HIP_TRY(launch_q4_rows(s->stream, q4_rows(c, first), count, c->num_heads, c->head_dim, d_keys, d_values));
+    return SPISSA_OK;
+  }
+  const size_t off = first * c->width(), bytes = count * c->width() * sizeof(float);
+  if (d_keys) HIP_TRY(hipMemcpyAsync(d_keys, c->keys + off, bytes, hipMemcpyDeviceToDevice, s->stream));
+  if (d_values) HIP_TRY(hipMemcpyAsync(d_values, c->values + off, bytes, hipMemcpyDeviceToDevice, s->stream));
+  return SPISSA_OK;
   GUARD_END
 }
 extern "C" const float *spissa_kv_cache_device_keys(const spissa_kv_cache *c) { return c ? c->keys : nullptr; }
@@ -570,11 +748,19 @@ extern "C" int spissa_kv_cache_clone(const spissa_kv_cache *c, spissa_kv_cache *
   GUARD_BEGIN
   if (!c || !out) return set_err(SPISSA_ERR_ARGUMENT, "null argument");
   spissa_kv_cache *n = nullptr;
-  ST_TRY(kv_new_impl(c->session, c->num_heads, c->head_dim, c->max_seq_len, &n));
   spissa_session *s = c->session;
+  *out = nullptr;
+  if (c->q4)
+    ST_TRY(kv_q4_new_impl(s, c->num_heads, c->head_dim, c->max_seq_len, &n));
+  else
+    ST_TRY(kv_new_impl(s, c->num_heads, c->head_dim, c->max_seq_len, &n));
   const size_t bytes = c->len * c->width() * sizeof(float);
   hipError_t e = hipSuccess;
-  if (bytes) {
+  if (c->q4) {
+    // (whole: a head's rows are apart, so the first rows of all are not one range)
+    const size_t all = 2 * (c->q4_codes(c->max_seq_len) + c->q4_params(c->max_seq_len)) + c->num_heads * sizeof(float);
+    e = hipMemcpyAsync(n->kc, c->kc, all, hipMemcpyDeviceToDevice, s->stream);
+  } else if (bytes) {
     e = hipMemcpyAsync(n->keys, c->keys, bytes, hipMemcpyDeviceToDevice, s->stream);
     if (e == hipSuccess) e = hipMemcpyAsync(n->values, c->values, bytes, hipMemcpyDeviceToDevice, s->stream);
   }
@@ -1027,11 +1213,6 @@ static bool plan_decode(int D, int Hq, int Hkv, size_t window, const int *past, 
 // capacity when `append` is set. The partials go to the session workspace,
 // or, with `fixed` set, to the fixed_bytes at `fixed` (splits are coarsened
 // to fit; the caller has checked that one split per group fits).
-struct GemmaQkNorm {  // fused QK-norm of the Gemma decode step
-  const float *q_norm, *k_norm;
-  float eps, q_prescale;
-};
-
 static int run_decode(spissa_session *s, const float *d_q, const float *d_k, const float *d_v,
                       const spissa_kv_cache *const *caches, size_t batch, const spissa_kv_attention_config *c,
                       float *d_out, const spissa_rope_table *table, bool append, float *fixed = nullptr,
@@ -1261,6 +1442,153 @@ static int run_prefill(spissa_session *s, const float *d_q, const float *d_k, co
   return SPISSA_OK;
 }
 
+// The calls that take the current rows beside the cache, or must not allocate, read f32 caches.
+static int refuse_q4(const spissa_kv_cache *c, const char *what) {
+  if (c && c->q4)
+    return set_err(SPISSA_ERR_ARGUMENT,
+                   "%s does not read a 4-bit cache: append the rows and call the attention over the cache, or a fused step",
+                   what);
+  return SPISSA_OK;
+}
+
+// ---- attention over 4-bit caches (q4_cache.hip) ----
+// The partials of a launch over n queries: enough for any lengths, so that a
+// call prepares the workspace of every later one of its batch and heads.
+static size_t q4_partial_bytes(size_t n, size_t Hq, size_t D, const Q4AttnPlan &p, size_t Hkv) {
+  const size_t groups = Hkv * p.HB;
+  return n * (groups + kDecodeGridWorkgroups) * (size_t)p.RB * (D + 2) * sizeof(float);
+}
+
+// One query of each of B sequences, whose own row is its cache's last.
+// extra: rows that the caches hold beyond their lengths (1 in a fused step).
+static int q4_attend_batch(spissa_session *s, const float *q, const spissa_kv_cache *const *caches, size_t batch,
+                           const spissa_kv_attention_config *c, float *out, size_t extra) {
+  const int D = (int)c->head_dim, Hq = (int)c->num_heads, Hkv = (int)c->kv_heads, R = Hq / Hkv;
+  for (size_t b0 = 0; b0 < batch; b0 += kMaxDecodeBatch) {
+    const int B = (int)std::min<size_t>(kMaxDecodeBatch, batch - b0);
+    Q4AttnArgs a{};
+    int keys[kMaxDecodeBatch];
+    for (int b = 0; b < B; ++b) {
+      a.seq[b].rows = q4_rows(caches[b0 + b], 0);
+      a.seq[b].len = (int)(caches[b0 + b]->len + extra);
+      keys[b] = c->window ? (int)std::min<size_t>(a.seq[b].len, c->window) : a.seq[b].len;
+    }
+    const Q4AttnPlan p = q4_attend_plan(D, R, Hkv, keys, B, 1, (size_t)1 << 40);
+    ST_TRY(ensure_buf(s, s->partial, q4_partial_bytes(B, Hq, D, p, Hkv)));
+    a.q = q + b0 * (size_t)Hq * D;
+    a.out = out + b0 * (size_t)Hq * D;
+    a.partial = (float *)s->partial.p;
+    a.err = s->d_err;
+    a.Hq = Hq;
+    a.Hkv = Hkv;
+    a.R = R;
+    a.HB = p.HB;
+    a.window = (int)c->window;
+    a.causal = c->causal ? 1 : 0;
+    a.kps = p.kps;
+    a.max_splits = p.splits;
+    a.qscale = (1.0f / sqrtf((float)D)) * 1.4426950408889634f;
+    HIP_TRY(launch_q4_attend(s->stream, a, D, p.RB, B));
+  }
+  return SPISSA_OK;
+}
+
+// The queries of the cache's last S rows; its length is `len`, those rows included.
+static int q4_attend_chunk(spissa_session *s, const float *q, const spissa_kv_cache *cache, size_t len,
+                           const spissa_kv_attention_config *c, float *out) {
+  const int D = (int)c->head_dim, Hq = (int)c->num_heads, Hkv = (int)c->kv_heads, R = Hq / Hkv;
+  const size_t S = c->query_len;
+  constexpr size_t kMost = 1024;  // queries of a launch
+  for (size_t t0 = 0; t0 < S; t0 += kMost) {
+    const int n = (int)std::min(kMost, S - t0);
+    Q4AttnArgs a{};
+    a.seq[0].rows = q4_rows(cache, 0);
+    a.seq[0].len = (int)len;
+    const int keys = (int)(c->window && c->causal ? std::min<size_t>(len, c->window) : len);
+    const Q4AttnPlan p = q4_attend_plan(D, R, Hkv, &keys, 1, n, (size_t)64 << 20);
+    ST_TRY(ensure_buf(s, s->partial, p.partial_bytes));
+    a.q = q;
+    a.out = out;
+    a.partial = (float *)s->partial.p;
+    a.err = s->d_err;
+    a.Hq = Hq;
+    a.Hkv = Hkv;
+    a.R = R;
+    a.HB = p.HB;
+    a.window = (int)c->window;
+    a.causal = c->causal ? 1 : 0;
+    a.kps = p.kps;
+    a.max_splits = p.splits;
+    a.queries = (int)S;
+    a.query0 = (int)t0;
+    a.qscale = (1.0f / sqrtf((float)D)) * 1.4426950408889634f;
+    HIP_TRY(launch_q4_attend(s->stream, a, D, p.RB, n));
+  }
+  return SPISSA_OK;
+}
+
+// Every check of a fused step of S tokens on each of `batch` 4-bit caches.
+static int q4_validate_step(spissa_session *s, const spissa_rope_table *table, const float *d_q, const float *d_k,
+                            const float *d_v, spissa_kv_cache *const *caches, size_t batch,
+                            const spissa_kv_attention_config *cfg, const float *d_out) {
+  for (size_t b = 0; b < batch; ++b) {
+    if (!caches[b]->q4) return set_err(SPISSA_ERR_ARGUMENT, "a step takes f32 caches or 4-bit caches, not both");
+    ST_TRY(validate_attention(0, 0, 0, caches[b], cfg, false));
+    size_t n, nl;  // rotary.rs:227-251: the append must fit before anything runs
+    ST_TRY(kv_validate_append(caches[b], 0, 0, cfg->query_len, false, &n, &nl));
+    if (caches[b]->session->device != s->device)
+      return set_err(SPISSA_ERR_ARGUMENT, "cache %zu lives on another device", b);
+    if (table && nl > table->max_positions)
+      return set_err(SPISSA_ERR_SHAPE, "positions up to %zu exceed the rope table (%zu positions)", nl,
+                     table->max_positions);
+  }
+  std::vector<const spissa_kv_cache *> seen(caches, caches + batch);
+  std::sort(seen.begin(), seen.end());
+  if (std::adjacent_find(seen.begin(), seen.end()) != seen.end())
+    return set_err(SPISSA_ERR_ARGUMENT, "a cache appears more than once in one decode step");
+  if (table && (table->kind == SPISSA_ROPE_NEOX || table->rotary_dim != cfg->head_dim))
+    return set_err(SPISSA_ERR_SHAPE, "a fused step needs a llama or gemma table over the whole head");
+  if (table && table->device != s->device) return set_err(SPISSA_ERR_ARGUMENT, "the rope table lives on another device");
+  if (!d_q || !d_k || !d_v || !d_out) return set_err(SPISSA_ERR_ARGUMENT, "null buffer");
+  if (!(aligned16(d_q) && aligned16(d_k) && aligned16(d_v) && aligned16(d_out)))
+    return set_err(SPISSA_ERR_ARGUMENT, "a step on a 4-bit cache takes 16-byte aligned buffers");
+  return SPISSA_OK;
+}
+
+// The fused step: (QK-norm, RoPE of q and k,) append, attention of the new
+// tokens over the rows as the cache then holds them. One token of each of
+// `batch` caches, or cfg->query_len tokens of one.
+static int q4_step(spissa_session *s, const spissa_rope_table *table, const float *d_q, const float *d_k,
+                   const float *d_v, spissa_kv_cache *const *caches, size_t batch, const spissa_kv_attention_config *cfg,
+                   float *d_out, const GemmaQkNorm *norm) {
+  ST_TRY(q4_validate_step(s, table, d_q, d_k, d_v, caches, batch, cfg, d_out));
+  if (norm && !(aligned16(norm->q_norm) && aligned16(norm->k_norm)))
+    return set_err(SPISSA_ERR_ARGUMENT, "a step on a 4-bit cache takes 16-byte aligned norms");
+  HIP_TRY(hipSetDevice(s->device));
+  const size_t S = cfg->query_len;
+  const float *q = d_q;
+  if (table || norm) {
+    ST_TRY(ensure_buf(s, s->q4q, batch * S * cfg->num_heads * cfg->head_dim * sizeof(float)));
+    q = (const float *)s->q4q.p;
+  }
+  // (workspaces before the first launch: nothing is appended by a call that fails for want of them)
+  if (S == 1) {
+    const int one = 1;
+    const Q4AttnPlan p = q4_attend_plan((int)cfg->head_dim, (int)(cfg->num_heads / cfg->kv_heads), (int)cfg->kv_heads, &one, 1,
+                                        1, (size_t)1 << 40);
+    ST_TRY(ensure_buf(s, s->partial,
+                      q4_partial_bytes(std::min<size_t>(batch, kMaxDecodeBatch), cfg->num_heads, cfg->head_dim, p, cfg->kv_heads)));
+  }
+  ST_TRY(q4_append(s, caches, batch, S, q == d_q ? nullptr : d_q, cfg->num_heads, d_k, d_v, table, norm,
+                   const_cast<float *>(q)));
+  if (S == 1)
+    ST_TRY(q4_attend_batch(s, q, caches, batch, cfg, d_out, 1));
+  else
+    ST_TRY(q4_attend_chunk(s, q, caches[0], caches[0]->len + S, cfg, d_out));
+  for (size_t b = 0; b < batch; ++b) caches[b]->len += S;
+  return SPISSA_OK;
+}
+
 static int attention_device_impl(spissa_session *s, const float *d_q, const float *d_k, const float *d_v,
                                  const spissa_kv_cache *cache, const spissa_kv_attention_config *c, float *d_out) {
   HIP_TRY(hipSetDevice(s->device));
@@ -1279,6 +1607,7 @@ extern "C" int spissa_attention_device(spissa_session *s, const float *d_q, cons
   GUARD_BEGIN
   if (!s || !cfg) return set_err(SPISSA_ERR_ARGUMENT, "null argument");
   ST_TRY(validate_attention(0, 0, 0, cache, cfg, false));
+  ST_TRY(refuse_q4(cache, "spissa_attention_device"));
   if (cache && cache->session->device != s->device)
     return set_err(SPISSA_ERR_ARGUMENT, "cache lives on device %d, session on %d", cache->session->device, s->device);
   return attention_device_impl(s, d_q, d_k, d_v, cache, cfg, d_out);
@@ -1293,6 +1622,7 @@ extern "C" int spissa_attention_decode_batch_device(spissa_session *s, const flo
   if (!s || !cfg) return set_err(SPISSA_ERR_ARGUMENT, "null argument");
   if (cfg->query_len != 1) return set_err(SPISSA_ERR_SHAPE, "batched decode needs query_len == 1, got %zu", cfg->query_len);
   for (size_t b = 0; b < batch; ++b) ST_TRY(validate_attention(0, 0, 0, caches ? caches[b] : nullptr, cfg, false));
+  for (size_t b = 0; b < batch; ++b) ST_TRY(refuse_q4(caches ? caches[b] : nullptr, "spissa_attention_decode_batch_device"));
   if (batch == 0) return SPISSA_OK;
   HIP_TRY(hipSetDevice(s->device));
   const int D = (int)cfg->head_dim;
@@ -1343,10 +1673,27 @@ static int validate_decode_step(spissa_session *s, const spissa_rope_table *tabl
   return SPISSA_OK;
 }
 
+static bool any_q4(spissa_kv_cache *const *caches, size_t batch) {
+  for (size_t b = 0; caches && b < batch; ++b)
+    if (caches[b] && caches[b]->q4) return true;
+  return false;
+}
+static int check_step_caches(spissa_kv_cache *const *caches, size_t batch, const spissa_kv_attention_config *cfg) {
+  if (cfg->query_len != 1) return set_err(SPISSA_ERR_SHAPE, "a decode step needs query_len == 1, got %zu", cfg->query_len);
+  for (size_t b = 0; b < batch; ++b)
+    if (!caches[b]) return set_err(SPISSA_ERR_ARGUMENT, "cache %zu is null", b);
+  return SPISSA_OK;
+}
+
 extern "C" int spissa_decode_step_device(spissa_session *s, const spissa_rope_table *table, const float *d_q,
                                          const float *d_k, const float *d_v, spissa_kv_cache *const *caches,
                                          size_t batch, const spissa_kv_attention_config *cfg, float *d_out) {
   GUARD_BEGIN
+  if (any_q4(caches, batch)) {
+    if (!s || !cfg) return set_err(SPISSA_ERR_ARGUMENT, "null argument");
+    ST_TRY(check_step_caches(caches, batch, cfg));
+    return q4_step(s, table, d_q, d_k, d_v, caches, batch, cfg, d_out, nullptr);
+  }
   ST_TRY(validate_decode_step(s, table, caches, batch, cfg));
   if (batch == 0) return SPISSA_OK;
   HIP_TRY(hipSetDevice(s->device));
@@ -1365,6 +1712,12 @@ extern "C" int spissa_gemma_decode_step_device(spissa_session *s, const spissa_r
   if (!table || !d_q_norm || !d_k_norm) return set_err(SPISSA_ERR_ARGUMENT, "null argument");
   if (table->kind != SPISSA_ROPE_GEMMA)
     return set_err(SPISSA_ERR_ARGUMENT, "the gemma decode step needs a gemma rope table");
+  if (any_q4(caches, batch)) {
+    if (!s || !cfg) return set_err(SPISSA_ERR_ARGUMENT, "null argument");
+    ST_TRY(check_step_caches(caches, batch, cfg));
+    const GemmaQkNorm norm{d_q_norm, d_k_norm, eps, q_prescale};
+    return q4_step(s, table, d_q, d_k, d_v, caches, batch, cfg, d_out, &norm);
+  }
   ST_TRY(validate_decode_step(s, table, caches, batch, cfg));
   if (batch == 0) return SPISSA_OK;
   HIP_TRY(hipSetDevice(s->device));
@@ -1380,6 +1733,7 @@ extern "C" int spissa_decode_step_device_noalloc(spissa_session *s, const spissa
                                                  spissa_kv_cache *const *caches, size_t batch,
                                                  const spissa_kv_attention_config *cfg, float *d_out) {
   GUARD_BEGIN
+  for (size_t b = 0; caches && b < batch; ++b) ST_TRY(refuse_q4(caches[b], "spissa_decode_step_device_noalloc"));
   ST_TRY(validate_decode_step(s, table, caches, batch, cfg));
   if (!s->scratch) return set_err(SPISSA_ERR_DEVICE, "the session has no scratch array");
   // One split per (sequence, KV head, head block) must fit; run_decode
@@ -1494,6 +1848,7 @@ extern "C" int spissa_prefill_step_device(spissa_session *s, const spissa_rope_t
   GUARD_BEGIN
   if (!s || !cfg || !cache) return set_err(SPISSA_ERR_ARGUMENT, "null argument");
   if (cfg->query_len == 1) return spissa_decode_step_device(s, table, d_q, d_k, d_v, &cache, 1, cfg, d_out);
+  if (cache->q4) return q4_step(s, table, d_q, d_k, d_v, &cache, 1, cfg, d_out, nullptr);
   return run_prefill_step(s, table, d_q, d_k, d_v, cache, cfg, d_out, nullptr);
   GUARD_END
 }
@@ -1510,6 +1865,7 @@ extern "C" int spissa_gemma_prefill_step_device(spissa_session *s, const spissa_
     return spissa_gemma_decode_step_device(s, table, d_q, d_k, d_v, &cache, 1, cfg, d_q_norm, d_k_norm, eps,
                                            q_prescale, d_out);
   const GemmaQkNorm norm{d_q_norm, d_k_norm, eps, q_prescale};
+  if (cache->q4) return q4_step(s, table, d_q, d_k, d_v, &cache, 1, cfg, d_out, &norm);
   return run_prefill_step(s, table, d_q, d_k, d_v, cache, cfg, d_out, &norm);
   GUARD_END
 }
@@ -1518,7 +1874,7 @@ extern "C" int spissa_attention_cached_device(spissa_session *s, const float *d_
                                               const spissa_kv_attention_config *cfg, float *d_out) {
   GUARD_BEGIN
   if (!s || !cfg || !cache) return set_err(SPISSA_ERR_ARGUMENT, "null argument");
-  if (cfg->query_len < 2)
+  if (cfg->query_len < (cache->q4 ? 1 : 2))
     return set_err(SPISSA_ERR_SHAPE, "append-first attention needs query_len > 1, got %zu", cfg->query_len);
   if (cache->len < cfg->query_len)
     return set_err(SPISSA_ERR_SHAPE, "the cache holds %zu rows, fewer than the chunk's %zu", cache->len,
@@ -1532,6 +1888,13 @@ extern "C" int spissa_attention_cached_device(spissa_session *s, const float *d_
   }
   if (cache->session->device != s->device)
     return set_err(SPISSA_ERR_ARGUMENT, "cache lives on device %d, session on %d", cache->session->device, s->device);
+  if (cache->q4) {
+    if (!d_q || !d_out) return set_err(SPISSA_ERR_ARGUMENT, "null buffer");
+    if (!(aligned16(d_q) && aligned16(d_out)))
+      return set_err(SPISSA_ERR_ARGUMENT, "attention over a 4-bit cache takes 16-byte aligned buffers");
+    HIP_TRY(hipSetDevice(s->device));
+    return S == 1 ? q4_attend_batch(s, d_q, &cache, 1, cfg, d_out, 0) : q4_attend_chunk(s, d_q, cache, cache->len, cfg, d_out);
+  }
   const int D = (int)cfg->head_dim;
   if (!prefill_supported(D) || s->prefill_precision != SPISSA_PREFILL_BF16)
     return set_err(SPISSA_ERR_SHAPE, "append-first attention runs the bf16 prefill at head_dim 64, 128 or 256, got %d",
@@ -1550,6 +1913,32 @@ extern "C" int spissa_attention_cached_device(spissa_session *s, const float *d_
     HIP_TRY(launch_stage_bf16(s->stream, nullptr, nullptr, 0, pad_end - (P + S), cache->num_heads, cache->head_dim,
                               cache->kb, cache->vt, P + S, cache->shadow_cap));
   return launch_prefill_from_shadow(s, a, cache, d_q, nullptr, d_out, D);
+  GUARD_END
+}
+
+extern "C" int spissa_attention_cached_batch_device(spissa_session *s, const float *d_q,
+                                                    const spissa_kv_cache *const *caches, size_t batch,
+                                                    const spissa_kv_attention_config *cfg, float *d_out) {
+  GUARD_BEGIN
+  if (!s || !cfg || (batch && !caches)) return set_err(SPISSA_ERR_ARGUMENT, "null argument");
+  if (cfg->query_len != 1) return set_err(SPISSA_ERR_SHAPE, "batched decode needs query_len == 1, got %zu", cfg->query_len);
+  for (size_t b = 0; b < batch; ++b) {
+    if (!caches[b]) return set_err(SPISSA_ERR_ARGUMENT, "cache %zu is null", b);
+    if (!caches[b]->q4)
+      return set_err(SPISSA_ERR_ARGUMENT, "append-first attention of single tokens reads 4-bit caches; cache %zu is f32", b);
+    if (caches[b]->len == 0) return set_err(SPISSA_ERR_SHAPE, "cache %zu is empty: the token's own row is its last", b);
+    spissa_kv_cache before = *caches[b];
+    before.len -= 1;
+    ST_TRY(validate_attention(0, 0, 0, &before, cfg, false));
+    if (caches[b]->session->device != s->device)
+      return set_err(SPISSA_ERR_ARGUMENT, "cache %zu lives on another device", b);
+  }
+  if (batch == 0) return SPISSA_OK;
+  if (!d_q || !d_out) return set_err(SPISSA_ERR_ARGUMENT, "null buffer");
+  if (!(aligned16(d_q) && aligned16(d_out)))
+    return set_err(SPISSA_ERR_ARGUMENT, "attention over a 4-bit cache takes 16-byte aligned buffers");
+  HIP_TRY(hipSetDevice(s->device));
+  return q4_attend_batch(s, d_q, caches, batch, cfg, d_out, 0);
   GUARD_END
 }
 
@@ -1625,6 +2014,7 @@ extern "C" int spissa_scaled_dot_product_attention_with_cache(const float *q, si
   GUARD_BEGIN
   if (!cfg) return set_err(SPISSA_ERR_ARGUMENT, "config is null");
   ST_TRY(validate_attention(q_len, k_len, v_len, cache, cfg, true));
+  ST_TRY(refuse_q4(cache, "spissa_scaled_dot_product_attention_with_cache"));
   if (out_len != q_len) return set_err(SPISSA_ERR_SHAPE, "output holds %zu floats, need %zu", out_len, q_len);
   if (!q || !current_k || !current_v || !out) return set_err(SPISSA_ERR_ARGUMENT, "null buffer");
   spissa_session *s = nullptr;
@@ -2099,7 +2489,7 @@ extern "C" int spissa_attention_sublayer_device(spissa_session *s, const spissa_
     float *const oqkv[3] = {q, k, v};
     ST_TRY(linear_launch_multi(s, wqkv, xn, S, oqkv, 3, fold, L->eps));
   }
-  if (S == 1 && cache && decode_supported((int)D, (int)(Hq / Hkv)) && decode_cache_fits(cache)) {
+  if (S == 1 && cache && (cache->q4 || (decode_supported((int)D, (int)(Hq / Hkv)) && decode_cache_fits(cache)))) {
     // (QK-norm,) RoPE, attention and append in the fused decode step
     spissa_kv_cache *caches[1] = {cache};
     if (qk_norm)
@@ -2107,7 +2497,8 @@ extern "C" int spissa_attention_sublayer_device(spissa_session *s, const spissa_
                                              L->q_prescale, att));
     else
       ST_TRY(spissa_decode_step_device(s, L->rope, q, k, v, caches, 1, &cfg, att));
-  } else if (S > 1 && cache && prefill_supported((int)D) && s->prefill_precision == SPISSA_PREFILL_BF16) {
+  } else if (S > 1 && cache &&
+             (cache->q4 || (prefill_supported((int)D) && s->prefill_precision == SPISSA_PREFILL_BF16))) {
     // (QK-norm,) RoPE, append and attention in the fused prefill step
     if (qk_norm)
       ST_TRY(spissa_gemma_prefill_step_device(s, L->rope, q, k, v, cache, &cfg, L->d_q_norm, L->d_k_norm, L->eps,

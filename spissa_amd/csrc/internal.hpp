@@ -14,7 +14,7 @@ namespace spissa {
 typedef __bf16 bf16;
 
 // Device-side error bits reported through spissa_session_sync().
-enum : int { kDevErrSoftmaxDenominator = 1 };
+enum : int { kDevErrSoftmaxDenominator = 1, kDevErrCacheValue = 2 };
 
 // Largest batch a single decode launch carries in its kernel arguments.
 constexpr int kMaxDecodeBatch = 16;
@@ -298,5 +298,63 @@ int decode_keys_per_split(int D, int RB, const int *keys, int nseq, long heads, 
 bool decode_single(int D, int B, int Hq, int Hkv, int max_keys, int cus);
 bool decode_supported(int D, int R);
 bool prefill_supported(int D);
+
+// ---- the KV cache held in 4 bits (q4_cache.hip) ----
+// One cache's buffers, keys and values: codes [Hkv][cap][D / 2], steps and
+// minima [Hkv][cap][D / 32].
+struct Q4Rows {
+  unsigned char *k, *v;
+  unsigned *kp, *vp;
+  float *vmax;  // [Hkv]: a bound on the head's |values|
+  long cap;
+  int first;    // the first row to write or to give back
+  int pad;
+};
+// Rows of S tokens of each of up to kMaxDecodeBatch sequences, token-major as
+// the callers have them: q [B * S, Hq, D] (Hq 0: none), k and v [B * S, Hkv, D].
+// S * (Hq + 2 Hkv) < 2^30.
+struct Q4AppendArgs {
+  const float *q, *k, *v;
+  float *q_out;             // the normed, rotated, prescaled query rows
+  const float *cos, *sin;   // RoPE table rows by position, or null
+  const float *q_norm, *k_norm;  // QK-norm, null: none
+  float eps, prescale;
+  int S, Hq, Hkv;
+  int *err;
+  Q4Rows seq[kMaxDecodeBatch];
+};
+hipError_t launch_q4_append(hipStream_t st, const Q4AppendArgs &a, int D, int B);
+// Rows [s.first, s.first + n) as f32 [n, Hkv, D]; either output may be null.
+hipError_t launch_q4_rows(hipStream_t st, const Q4Rows &s, size_t n, size_t Hkv, size_t D, float *k_out, float *v_out);
+
+// Attention of single queries: the last token of each sequence of a batch
+// (queries 0), or the last `queries` rows' queries of one sequence, of which a
+// launch takes those from query0 on.
+struct Q4AttnBase {
+  const float *q;   // [B or queries, Hq, D]
+  float *out;
+  float *partial;   // [B or queries, Hkv, HB, max_splits] entries of RB * (D + 2) floats
+  int *err;
+  int Hq, Hkv, R, HB, window, causal, kps, max_splits, queries, query0;
+  float qscale;     // softmax scale * log2(e)
+};
+struct Q4Seq {
+  Q4Rows rows;
+  int len;          // rows, the queries' own included
+  int pad;
+};
+template <int MB>
+struct Q4AttnArgsOf : Q4AttnBase {
+  Q4Seq seq[MB];
+};
+typedef Q4AttnArgsOf<kMaxDecodeBatch> Q4AttnArgs;
+struct Q4AttnPlan {
+  int RB, HB, kps, splits;
+  size_t partial_bytes;
+};
+// keys[i]: visible keys of the n queries of a launch (times `copies`: queries alike).
+Q4AttnPlan q4_attend_plan(int D, int R, int Hkv, const int *keys, int n, long copies, size_t partial_cap);
+hipError_t launch_q4_attend(hipStream_t st, const Q4AttnArgs &a, int D, int RB, int nz);
+bool q4_supported(size_t D);
 
 }  // namespace spissa

@@ -14,7 +14,7 @@ from typing import Optional, Sequence
 
 from . import _ffi
 from .errors import ArgumentError, check
-from .rotary import KvAttentionConfig, KvCache
+from .rotary import KvAttentionConfig, KvCache, Q4KvCache
 
 
 _f32 = None  # torch.float32, once a device tensor has been seen
@@ -207,6 +207,10 @@ class Session:
     def kv_cache(self, num_heads: int, head_dim: int, max_seq_len: int) -> KvCache:
         return KvCache(num_heads, head_dim, max_seq_len, session=self)
 
+    def q4_kv_cache(self, num_heads: int, head_dim: int, max_seq_len: int) -> Q4KvCache:
+        """A cache held in 4 bits (see spissa_amd.rotary.Q4KvCache)."""
+        return Q4KvCache(num_heads, head_dim, max_seq_len, session=self)
+
     def rope_table(self, kind: int, rotary_dim: int, base: float, position_divisor: float = 1.0,
                    freq_scale=None, max_positions: int = 8192) -> RopeTable:
         return RopeTable(self, kind, rotary_dim, base, position_divisor, freq_scale, max_positions)
@@ -302,6 +306,15 @@ class Session:
         check(self._lib.spissa_attention_cached_device(self.handle, _dev(q, "q"), cache.handle, C.byref(cfg),
                                                        _dev(out, "out")))
 
+    def attention_cached_batch(self, q, caches: Sequence[Q4KvCache], config: KvAttentionConfig, out) -> None:
+        """Append-first attention of one token of each of `len(caches)` sequences over 4-bit
+        caches (spissa_attention_cached_batch_device): q [B, Hq, D], sequence b's own row is
+        the last of caches[b]."""
+        arr = _cache_array(caches)
+        cfg = config._c()
+        check(self._lib.spissa_attention_cached_batch_device(self.handle, _dev(q, "q"), arr, len(caches), C.byref(cfg),
+                                                             _dev(out, "out")))
+
     def hbm_read_probe(self, buf, sink) -> None:
         """Reads every byte of the device tensor `buf` once (the streaming-read
         ceiling kernel); `sink` is a float32 device tensor of one element."""
@@ -319,6 +332,16 @@ class Session:
 
     def append(self, cache: KvCache, k, v, token_count: int) -> None:
         cache.append_device(_dev(k, "k"), _dev(v, "v"), token_count)
+
+    def cache_rows(self, cache: KvCache, first: int, count: int, keys, values) -> None:
+        """Rows [first, first + count) of a cache into the f32 device tensors keys and values
+        [count, heads, head_dim] (either may be None): spissa_kv_cache_rows_device."""
+        need = count * cache.num_heads() * cache.head_dim()
+        for t, name in ((keys, "keys"), (values, "values")):
+            if t is not None and t.numel() < need:
+                raise TypeError(f"{name} holds {t.numel()} values, {count} rows need {need}")
+        check(self._lib.spissa_kv_cache_rows_device(cache.handle, first, count, _dev(keys, "keys"),
+                                                    _dev(values, "values")))
 
     def attention_sublayer(self, layer: AttentionLayer, x, seq_len: int, cache: Optional[KvCache], out) -> None:
         """x [seq_len, hidden] -> out [seq_len, hidden]: norm, projections, QK-norm, RoPE at the

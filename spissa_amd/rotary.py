@@ -115,6 +115,8 @@ class KvCache:
     device and stream; by default it uses the calling thread's default session.
     """
 
+    _NEW, _NEW_IN = "spissa_kv_cache_new", "spissa_kv_cache_new_in"
+
     def __init__(self, num_heads: int, head_dim: int, max_seq_len: int, session=None,
                  _handle: Optional[int] = None):
         lib = _ffi.load()
@@ -125,9 +127,9 @@ class KvCache:
             return
         h = _ffi.c_void_p()
         if session is None:
-            check(lib.spissa_kv_cache_new(num_heads, head_dim, max_seq_len, C.byref(h)))
+            check(getattr(lib, self._NEW)(num_heads, head_dim, max_seq_len, C.byref(h)))
         else:
-            check(lib.spissa_kv_cache_new_in(session.handle, num_heads, head_dim, max_seq_len,
+            check(getattr(lib, self._NEW_IN)(session.handle, num_heads, head_dim, max_seq_len,
                                              C.byref(h)))
         self._h = h
 
@@ -156,7 +158,7 @@ class KvCache:
     def clone(self) -> "KvCache":
         out = _ffi.c_void_p()
         check(self._lib.spissa_kv_cache_clone(self.handle, C.byref(out)))
-        return KvCache(0, 0, 0, self._session, _handle=out.value)
+        return type(self)(0, 0, 0, self._session, _handle=out.value)
 
     __copy__ = clone
 
@@ -217,6 +219,20 @@ class KvCache:
 
     def device_values_ptr(self) -> int:
         return self._lib.spissa_kv_cache_device_values(self.handle)
+
+
+class Q4KvCache(KvCache):
+    """A cache held in 4 bits (spissa_kv_cache_q4_new): every 32 channels of a row
+    have a binary16 minimum and step, 0.625 bytes a channel. head_dim 64, 128 or 256.
+
+    The methods are KvCache's; keys() and values() give the values that the codes
+    stand for, and the device pointers are None. Attention over it reads every row,
+    the new ones included, as the cache holds it (append first): Session.decode_step,
+    gemma_decode_step, prefill_step, gemma_prefill_step, attention_cached,
+    attention_cached_batch and attention_sublayer take it; the calls with current
+    rows beside the cache refuse it (ArgumentError)."""
+
+    _NEW, _NEW_IN = "spissa_kv_cache_q4_new", "spissa_kv_cache_q4_new_in"
 
 
 def scaled_dot_product_attention_with_cache(q: np.ndarray, current_k: np.ndarray,
