@@ -311,7 +311,7 @@ inline bool is_global_layer(size_t layer_idx, size_t sliding_window_pattern) {
 
 // ---- linear projections (streaming/linear.rs:269-576) ----
 
-enum class DType { F32 = SPISSA_DTYPE_F32, F16 = SPISSA_DTYPE_F16, Bf16 = SPISSA_DTYPE_BF16 };
+enum class DType { F32 = SPISSA_DTYPE_F32, F16 = SPISSA_DTYPE_F16, Bf16 = SPISSA_DTYPE_BF16, Q4 = SPISSA_DTYPE_Q4 };
 
 // streaming/mod.rs:511-516
 struct StreamingLinearConfig {
@@ -337,6 +337,12 @@ class LinearWeight {
   // session = nullptr: the calling thread's default session.
   static Result<LinearWeight> create(DType dtype, size_t out_features, size_t in_features, const void *data,
                                      size_t data_bytes, const Session *session = nullptr);
+  // 4-bit codes with a scale and, with zeros, a zero point for each group of
+  // input channels (spissa_linear_weight_q4_new).
+  static Result<LinearWeight> create_q4(size_t out_features, size_t in_features, size_t group, const void *codes,
+                                        size_t codes_bytes, DType scale_dtype, const void *scales, size_t scales_bytes,
+                                        const void *zeros = nullptr, size_t zeros_bytes = 0,
+                                        const Session *session = nullptr);
   LinearWeight() = default;
   LinearWeight(LinearWeight &&o) noexcept
       : w_(o.w_), dtype_(o.dtype_), out_features_(o.out_features_), in_features_(o.in_features_) {
@@ -671,6 +677,22 @@ inline Result<LinearWeight> LinearWeight::create(DType dtype, size_t out_feature
       spissa_linear_weight_new(s, static_cast<int>(dtype), out_features, in_features, data, data_bytes, &w));
   if (r.is_err()) return r.error();
   return LinearWeight(w, dtype, out_features, in_features);
+}
+
+inline Result<LinearWeight> LinearWeight::create_q4(size_t out_features, size_t in_features, size_t group,
+                                                    const void *codes, size_t codes_bytes, DType scale_dtype,
+                                                    const void *scales, size_t scales_bytes, const void *zeros,
+                                                    size_t zeros_bytes, const Session *session) {
+  spissa_session *s = session ? session->raw() : nullptr;
+  if (!s) {
+    auto r = detail::check(spissa_default_session(&s));
+    if (r.is_err()) return r.error();
+  }
+  spissa_linear_weight *w = nullptr;
+  auto r = detail::check(spissa_linear_weight_q4_new(s, out_features, in_features, group, static_cast<int>(scale_dtype),
+                                                     codes, codes_bytes, scales, scales_bytes, zeros, zeros_bytes, &w));
+  if (r.is_err()) return r.error();
+  return LinearWeight(w, DType::Q4, out_features, in_features);
 }
 
 }  // namespace spissa

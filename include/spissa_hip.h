@@ -402,7 +402,12 @@ int spissa_scaled_dot_product_attention(const float *q, size_t q_len, const floa
 
 /* Weight element types with a device kernel (spissa_container::DType Fp32,
  * Fp16, Bf16). */
-typedef enum { SPISSA_DTYPE_F32 = 0, SPISSA_DTYPE_F16 = 1, SPISSA_DTYPE_BF16 = 2 } spissa_dtype;
+typedef enum {
+    SPISSA_DTYPE_F32 = 0,
+    SPISSA_DTYPE_F16 = 1,
+    SPISSA_DTYPE_BF16 = 2,
+    SPISSA_DTYPE_Q4 = 3 /* 4-bit codes with group scales: spissa_linear_weight_q4_new alone makes these */
+} spissa_dtype;
 typedef struct spissa_linear_weight spissa_linear_weight;
 /* Uploads a row-major [out_features, in_features] weight whose little-endian
  * element bytes are `data` (what a raw chunk of the container holds).
@@ -412,6 +417,31 @@ typedef struct spissa_linear_weight spissa_linear_weight;
  * another stream must be complete before the call. */
 int spissa_linear_weight_new(spissa_session *s, int dtype, size_t out_features, size_t in_features,
                              const void *data, size_t data_bytes, spissa_linear_weight **out);
+/* A weight of 4-bit codes with a scale, and a zero point, for each group of
+ * input channels:
+ *   W[n, k] = scale[n, k / group] * (code[n, k] - zero[n, k / group]).
+ * codes: [out_features][ceil(in_features / 2)] bytes, the even channel in the
+ * low four bits; scales: [out_features][ceil(in_features / group)] of
+ * scale_dtype (F32, F16 or BF16); zeros: as many bytes of 0..15, or NULL and
+ * zeros_bytes 0 (then every zero point is 8). group: any multiple of 32 (SHAPE
+ * otherwise); in_features need not be one of group. Byte counts that do not
+ * match, or a zero point above 15: INVALID_TENSOR_DATA. Host or device memory;
+ * work that produces it on another stream must be complete before the call.
+ * The codes are laid out anew once, here. The reference keeps such tensors on
+ * its CPU path.
+ *
+ * The handle is a spissa_linear_weight: spissa_linear, spissa_linear_device (up
+ * to 1048560 tokens), the LM head calls and spissa_attention_sublayer_device
+ * take it. Activations are held to 22 bits, down to 2^-28 of the largest of
+ * their row (up to four tokens: of 256 channels of it); sums are f32. An
+ * infinite or NaN activation gives what the plain product would. Above four
+ * tokens a call uses a workspace that grows with the tokens: under graph
+ * capture it must follow a call of the same size. spissa_plan_linear describes
+ * the other types. */
+int spissa_linear_weight_q4_new(spissa_session *s, size_t out_features, size_t in_features, size_t group,
+                                int scale_dtype, const void *codes, size_t codes_bytes, const void *scales,
+                                size_t scales_bytes, const void *zeros, size_t zeros_bytes,
+                                spissa_linear_weight **out);
 /* Frees the weight after the work queued on its session. */
 void spissa_linear_weight_free(spissa_linear_weight *w);
 /* streaming/mod.rs:511-516 StreamingLinearConfig */
@@ -468,8 +498,8 @@ int spissa_plan_linear(int dtype, size_t batch, const size_t *out_features, size
 /* streaming/mod.rs:186-236 lm_head_logits_parallel (f32 table) and
  * streaming/mod.rs:238-287 lm_head_logits_parallel_bf16 (bf16 table):
  * logits[v] = sum_h last_hidden[h] * table[v, h], with the table a
- * [vocab_size, hidden] spissa_linear_weight of dtype F32 or BF16 (other
- * dtypes: InvalidTensorData). last_hidden_len must equal hidden and
+ * [vocab_size, hidden] spissa_linear_weight of dtype F32, BF16 or Q4 (F16:
+ * InvalidTensorData). last_hidden_len must equal hidden and
  * logits_len vocab_size (Shape otherwise; the reference indexes past such
  * buffers instead). Host buffers, synchronous. */
 int spissa_lm_head_logits(const spissa_linear_weight *table, const float *last_hidden,

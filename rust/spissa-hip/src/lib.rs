@@ -44,6 +44,7 @@ pub mod sys {
     pub const SPISSA_DTYPE_F32: c_int = 0;
     pub const SPISSA_DTYPE_F16: c_int = 1;
     pub const SPISSA_DTYPE_BF16: c_int = 2;
+    pub const SPISSA_DTYPE_Q4: c_int = 3;
 
     pub const SPISSA_PREFILL_BF16: c_int = 0;
     pub const SPISSA_PREFILL_F32: c_int = 1;
@@ -280,6 +281,10 @@ pub mod sys {
         pub fn spissa_linear_weight_new(s: *mut spissa_session, dtype: c_int, out_features: usize,
                                         in_features: usize, data: *const c_void, data_bytes: usize,
                                         out: *mut *mut spissa_linear_weight) -> c_int;
+        pub fn spissa_linear_weight_q4_new(s: *mut spissa_session, out_features: usize, in_features: usize, group: usize,
+                                           scale_dtype: c_int, codes: *const c_void, codes_bytes: usize,
+                                           scales: *const c_void, scales_bytes: usize, zeros: *const c_void,
+                                           zeros_bytes: usize, out: *mut *mut spissa_linear_weight) -> c_int;
         pub fn spissa_linear_weight_free(w: *mut spissa_linear_weight);
         pub fn spissa_linear(w: *const spissa_linear_weight, input: *const f32, input_len: usize,
                              bias: *const f32, bias_len: usize, cfg: *const spissa_linear_config,
@@ -829,6 +834,20 @@ impl DeviceLinearWeight {
         check(unsafe {
             sys::spissa_linear_weight_new(session.raw, dtype, out_features, in_features, raw.as_ptr() as *const c_void,
                                           raw.len(), &mut h)
+        })?;
+        Ok(Self(h))
+    }
+    /// 4-bit codes (two a byte, the even channel low) with a scale of
+    /// `scale_dtype` and, if given, a zero point for each group of input channels.
+    pub fn upload_q4(session: &Session, out_features: usize, in_features: usize, group: usize, codes: &[u8],
+                     scale_dtype: c_int, scales: &[u8], zeros: Option<&[u8]>) -> Result<Self> {
+        let mut h = std::ptr::null_mut();
+        check(unsafe {
+            sys::spissa_linear_weight_q4_new(session.raw, out_features, in_features, group, scale_dtype,
+                                             codes.as_ptr() as *const c_void, codes.len(),
+                                             scales.as_ptr() as *const c_void, scales.len(),
+                                             zeros.map_or(std::ptr::null(), |z| z.as_ptr() as *const c_void),
+                                             zeros.map_or(0, |z| z.len()), &mut h)
         })?;
         Ok(Self(h))
     }

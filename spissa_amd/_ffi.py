@@ -27,6 +27,7 @@ PREFILL_F32 = 1
 DTYPE_F32 = 0
 DTYPE_F16 = 1
 DTYPE_BF16 = 2
+DTYPE_Q4 = 3
 
 c_size = C.c_size_t
 c_float_p = C.POINTER(C.c_float)
@@ -212,6 +213,9 @@ SIGNATURES = {
          c_float_p, c_size]),
     "spissa_linear_weight_new": (
         C.c_int, [c_void_p, C.c_int, c_size, c_size, c_void_p, c_size, C.POINTER(c_void_p)]),
+    "spissa_linear_weight_q4_new": (
+        C.c_int, [c_void_p, c_size, c_size, c_size, C.c_int, c_void_p, c_size, c_void_p, c_size, c_void_p, c_size,
+                  C.POINTER(c_void_p)]),
     "spissa_linear_weight_free": (None, [c_void_p]),
     "spissa_linear": (
         C.c_int, [c_void_p, c_float_p, c_size, c_float_p, c_size, C.POINTER(LinearConfigC), c_float_p,

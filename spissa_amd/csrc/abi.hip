@@ -118,6 +118,7 @@ struct spissa_session {
   DevBuf q4q;       // fused steps on a 4-bit cache: the rotated queries
   float *lin = nullptr;  // partial sums of projections whose K is split over workgroups (linear_partials)
   std::mutex lin_mutex;  // held over the launches that write and read them
+  DevBuf q4x;       // activations' pieces of projections of 4-bit weights (under lin_mutex)
   float *scratch = nullptr;  // this device's copy of `scratch` (kScratchBytes)
   int cus = 256;    // compute units of the device
   // Buffers replaced by larger ones. They stay allocated until the session
@@ -230,6 +231,7 @@ static void session_free(spissa_session *s) {
   free_buf(s->amax);
   free_buf(s->qstage);
   free_buf(s->q4q);
+  free_buf(s->q4x);
   for (void *p : s->retired) (void)hipFree(p);
   if (s->d_err) (void)hipFree(s->d_err);
   if (s->lin) (void)hipFree(s->lin);
@@ -2060,7 +2062,15 @@ struct spissa_linear_weight {
   int dtype = SPISSA_DTYPE_BF16;
   size_t out_features = 0, in_features = 0;
   void *data = nullptr;  // [out, in] row-major in HBM
+  // kDtypeQ4 (spissa_linear_weight_q4_new): data holds the codes of
+  // linear_q4.hip's layout, then the groups' params
+  void *params = nullptr;
+  int pack_group = 0, param_type = 0;
+  int tiles = 0, blocks = 0;
 };
+constexpr int kDtypeQ4 = SPISSA_DTYPE_Q4;
+// Tokens of one projection of 4-bit weights (row tiles of 16 are a grid dimension).
+constexpr size_t kQ4MaxTokens = (size_t)16 * 65535;
 
 static size_t dtype_size(int dtype) {
   switch (dtype) {
@@ -2101,6 +2111,95 @@ extern "C" int spissa_linear_weight_new(spissa_session *s, int dtype, size_t out
   if (e != hipSuccess) {
     (void)hipFree(w->data);
     return set_err(SPISSA_ERR_DEVICE, "weight upload failed: %s", hipGetErrorString(e));
+  }
+  *out = w.release();
+  session_retain(s);
+  return SPISSA_OK;
+  GUARD_END
+}
+
+extern "C" int spissa_linear_weight_q4_new(spissa_session *s, size_t out_features, size_t in_features, size_t group,
+                                           int scale_dtype, const void *codes, size_t codes_bytes, const void *scales,
+                                           size_t scales_bytes, const void *zeros, size_t zeros_bytes,
+                                           spissa_linear_weight **out) {
+  GUARD_BEGIN
+  if (!s || !out) return set_err(SPISSA_ERR_ARGUMENT, "null argument");
+  *out = nullptr;
+  const size_t es = dtype_size(scale_dtype);
+  if (es == 0) return set_err(SPISSA_ERR_INVALID_TENSOR_DATA, "scales of dtype %d have no device kernel", scale_dtype);
+  size_t elems;
+  if (mul_ovf(out_features, in_features, &elems) || elems > (size_t)INT32_MAX * 8)
+    return set_err(SPISSA_ERR_SHAPE, "weight element count overflow");
+  // (rows and channels are padded to whole tiles within the kernels' 32-bit range)
+  if (out_features == 0 || in_features == 0 || out_features > INT32_MAX - 64 || in_features > INT32_MAX - 256)
+    return set_err(SPISSA_ERR_SHAPE, "weight shape [%zu, %zu] is empty or too large", out_features, in_features);
+  if (group == 0 || group % 32 != 0 || group > INT32_MAX)
+    return set_err(SPISSA_ERR_SHAPE, "a scale covers a multiple of 32 input channels, got %zu", group);
+  const size_t groups = (in_features + group - 1) / group;
+  const size_t want_codes = out_features * ((in_features + 1) / 2), want_scales = out_features * groups * es;
+  if (codes_bytes != want_codes || scales_bytes != want_scales)
+    return set_err(SPISSA_ERR_INVALID_TENSOR_DATA,
+                   "weight holds %zu bytes of codes and %zu of scales, shape [%zu, %zu] by groups of %zu needs %zu and %zu",
+                   codes_bytes, scales_bytes, out_features, in_features, group, want_codes, want_scales);
+  if (zeros ? zeros_bytes != out_features * groups : zeros_bytes != 0)
+    return set_err(SPISSA_ERR_INVALID_TENSOR_DATA, "weight holds %zu bytes of zero points, needs %zu", zeros_bytes,
+                   zeros ? out_features * groups : (size_t)0);
+  if (!codes || !scales) return set_err(SPISSA_ERR_ARGUMENT, "codes or scales are null");
+  std::unique_ptr<spissa_linear_weight> w(new spissa_linear_weight);
+  w->session = s;
+  w->dtype = kDtypeQ4;
+  w->out_features = out_features;
+  w->in_features = in_features;
+  w->pack_group = group % 128 == 0 ? 128 : group % 64 == 0 ? 64 : 32;
+  w->param_type = scale_dtype == SPISSA_DTYPE_F32 ? 3 : scale_dtype == SPISSA_DTYPE_BF16 ? 2 : zeros ? 1 : 0;
+  w->tiles = (int)((out_features + 15) / 16);
+  w->blocks = (int)((in_features + 127) / 128);
+  const size_t cells = (size_t)w->tiles * w->blocks;
+  const size_t code_bytes = cells * 1024, param_bytes = cells * 16 * (128 / w->pack_group) * q4_param_bytes(w->param_type);
+  // what the caller has, on the device: codes, scales, zero points, and a flag
+  const size_t at_scales = (codes_bytes + 15) & ~(size_t)15, at_zeros = at_scales + ((scales_bytes + 15) & ~(size_t)15);
+  const size_t at_flag = at_zeros + ((zeros_bytes + 15) & ~(size_t)15);
+  HIP_TRY(hipSetDevice(s->device));
+  ST_TRY(no_capture(s->stream, "a 4-bit weight", code_bytes + param_bytes));
+  char *raw = nullptr;
+  HIP_TRY(hipMalloc(&raw, at_flag + sizeof(int)));
+  hipError_t e = hipMalloc(&w->data, code_bytes + param_bytes);
+  int bad = 0;
+  if (e == hipSuccess) {
+    w->params = (char *)w->data + code_bytes;
+    const hipStream_t st = s->stream;
+    // host or device source: the runtime resolves the direction from the pointer
+    e = hipMemcpyAsync(raw, codes, codes_bytes, hipMemcpyDefault, st);
+    if (e == hipSuccess) e = hipMemcpyAsync(raw + at_scales, scales, scales_bytes, hipMemcpyDefault, st);
+    if (e == hipSuccess && zeros) e = hipMemcpyAsync(raw + at_zeros, zeros, zeros_bytes, hipMemcpyDefault, st);
+    if (e == hipSuccess) e = hipMemsetAsync(raw + at_flag, 0, sizeof(int), st);
+    if (e == hipSuccess) {
+      Q4PackArgs a{};
+      a.codes = (const unsigned char *)raw;
+      a.scales = raw + at_scales;
+      a.zeros = zeros ? (const unsigned char *)raw + at_zeros : nullptr;
+      a.out_codes = (unsigned *)w->data;
+      a.out_params = w->params;
+      a.err = (int *)(raw + at_flag);
+      a.N = (int)out_features;
+      a.K = (int)in_features;
+      a.group = (int)group;
+      a.pack_group = w->pack_group;
+      a.scale_dtype = scale_dtype;
+      a.param_type = w->param_type;
+      a.tiles = w->tiles;
+      a.blocks = w->blocks;
+      e = launch_q4_pack(st, a);
+    }
+    if (e == hipSuccess) e = hipMemcpyAsync(&bad, raw + at_flag, sizeof(int), hipMemcpyDeviceToHost, st);
+    if (e == hipSuccess) e = hipStreamSynchronize(st);
+    else (void)hipStreamSynchronize(st);
+  }
+  (void)hipFree(raw);
+  if (e != hipSuccess || bad) {
+    if (w->data) (void)hipFree(w->data);
+    if (e != hipSuccess) return set_err(SPISSA_ERR_DEVICE, "weight upload failed: %s", hipGetErrorString(e));
+    return set_err(SPISSA_ERR_INVALID_TENSOR_DATA, "a zero point is above 15");
   }
   *out = w.release();
   session_retain(s);
@@ -2220,6 +2319,33 @@ extern "C" int spissa_plan_linear(int dtype, size_t batch, const size_t *out_fea
   GUARD_END
 }
 
+// A projection of 4-bit weights. More than four tokens' activations are split
+// into a workspace first, which grows outside a capture; several threads may
+// call on one session, so the launches that write and read it stay together.
+static int linear_run_q4(spissa_session *s, const spissa_linear_weight *w, const float *d_x, const float *d_bias,
+                         size_t batch, float *d_out) {
+  Q4LinearArgs a{};
+  a.codes = w->data;
+  a.params = w->params;
+  a.x = d_x;
+  a.bias = d_bias;
+  a.out = d_out;
+  a.M = (int)batch;
+  a.N = (int)w->out_features;
+  a.K = (int)w->in_features;
+  a.tiles = w->tiles;
+  a.blocks = w->blocks;
+  HIP_TRY(hipSetDevice(s->device));
+  const size_t need = q4_linear_workspace(a.M, a.blocks);
+  std::unique_lock<std::mutex> lock(s->lin_mutex, std::defer_lock);
+  if (need) {
+    lock.lock();
+    ST_TRY(ensure_buf(s, s->q4x, need));
+  }
+  HIP_TRY(launch_q4_linear(s->stream, a, w->pack_group, w->param_type, s->q4x.p));
+  return SPISSA_OK;
+}
+
 static LinearArgs linear_args(const spissa_linear_weight *w, const float *d_x,
                               const float *d_bias, size_t batch, float *d_out) {
   LinearArgs a{};
@@ -2238,6 +2364,10 @@ static int linear_launch(spissa_session *s, const spissa_linear_weight *w, const
                          size_t batch, float *d_out) {
   if (batch == 0) return SPISSA_OK;
   if (batch > INT32_MAX) return set_err(SPISSA_ERR_SHAPE, "batch %zu too large", batch);
+  if (w->dtype == kDtypeQ4) {
+    if (batch > kQ4MaxTokens) return set_err(SPISSA_ERR_SHAPE, "batch %zu too large for 4-bit weights", batch);
+    return linear_run_q4(s, w, d_x, d_bias, batch, d_out);
+  }
   const LinearArgs a = linear_args(w, d_x, d_bias, batch, d_out);
   return linear_run(s, &a, 1);
 }
@@ -2257,6 +2387,12 @@ static int linear_launch_multi(spissa_session *s, const spissa_linear_weight *co
   if (norm_w && (reinterpret_cast<uintptr_t>(d_x) & 15))
     return set_err(SPISSA_ERR_ARGUMENT, "the folded input norm needs a 16-byte aligned input");
   LinearArgs a[kMaxLinearSegments];
+  bool q4 = false;
+  for (int i = 0; i < n; ++i) q4 = q4 || w[i]->dtype == kDtypeQ4;
+  if (q4) {  // (norm_w: not with 4-bit weights)
+    for (int i = 0; i < n; ++i) ST_TRY(linear_launch(s, w[i], d_x, nullptr, batch, d_out[i]));
+    return SPISSA_OK;
+  }
   bool same = true;
   size_t n_total = 0;
   for (int i = 0; i < n; ++i) {
@@ -2331,8 +2467,8 @@ static int argmax_launch(spissa_session *s, const float *d_x, size_t n, int64_t 
 
 static int check_lm_table(const spissa_linear_weight *t) {
   if (!t) return set_err(SPISSA_ERR_ARGUMENT, "table is null");
-  if (t->dtype != SPISSA_DTYPE_F32 && t->dtype != SPISSA_DTYPE_BF16)
-    return set_err(SPISSA_ERR_INVALID_TENSOR_DATA, "LM head table must be f32 or bf16 (dtype %d)", t->dtype);
+  if (t->dtype != SPISSA_DTYPE_F32 && t->dtype != SPISSA_DTYPE_BF16 && t->dtype != kDtypeQ4)
+    return set_err(SPISSA_ERR_INVALID_TENSOR_DATA, "LM head table must be f32, bf16 or 4-bit (dtype %d)", t->dtype);
   return SPISSA_OK;
 }
 
@@ -2474,7 +2610,7 @@ extern "C" int spissa_attention_sublayer_device(spissa_session *s, const spissa_
   if (L->d_input_norm) {
     bool gemv = S <= 4 && (reinterpret_cast<uintptr_t>(d_x) & 15) == 0;
     for (const spissa_linear_weight *w : {L->q_weight, L->k_weight, L->v_weight})
-      gemv = gemv && w->dtype == L->q_weight->dtype &&
+      gemv = gemv && w->dtype == L->q_weight->dtype && w->dtype != kDtypeQ4 &&
              linear_path(w->dtype, (long)S, (long)w->out_features, (long)H) == kLinearGemv;
     if (gemv) {
       fold = L->d_input_norm;

@@ -275,6 +275,36 @@ size_t linear_tile_partial_bytes(int cus);
 void linear_tile_dims(const LinearTilePlan &plan, int *rows, int *columns);
 hipError_t launch_linear_tile(hipStream_t st, const LinearArgs *segs, int nseg, const LinearTilePlan &plan, float *partial);
 
+// ---- weights of 4-bit codes with group scales (linear_q4.hip) ----
+// A checkpoint's codes (row-major, two a byte, the even channel low), scales and
+// zero points (null: 8) into the kernels' layout.
+struct Q4PackArgs {
+  const unsigned char *codes;
+  const void *scales;
+  const unsigned char *zeros;
+  unsigned *out_codes;  // [tiles][blocks][64 lanes][4]
+  void *out_params;     // [tiles][blocks][16][128 / pack_group] of param_type
+  int *err;             // set where a zero point is above 15
+  int N, K, group, pack_group, scale_dtype, param_type;
+  int tiles, blocks;    // 16 rows, 128 channels
+};
+hipError_t launch_q4_pack(hipStream_t st, const Q4PackArgs &a);
+size_t q4_param_bytes(int param_type);
+struct Q4LinearArgs {
+  const void *codes, *params;
+  const float *x;     // [M, K]
+  const float *bias;  // [N] or null
+  float *out;         // [M, N]
+  int M, N, K, tiles, blocks;
+  // set by the launcher
+  const void *pieces;
+  const float *inv;
+  int mtiles, wk, blocks_per_wave;
+  bool vec;
+};
+size_t q4_linear_workspace(long M, long blocks);
+hipError_t launch_q4_linear(hipStream_t st, const Q4LinearArgs &a, int group, int param_type, void *workspace);
+
 // Greedy token choice: one partial per contiguous range of the logits.
 struct ArgmaxPart {
   float v;       // first maximum of the range's non-NaN, non-excluded values

@@ -357,6 +357,13 @@ class Session:
 
         return LinearWeight(data, dtype, out_features, in_features, session=self)
 
+    def q4_linear_weight(self, codes, scales, out_features: int, in_features: int, group: int, zeros=None):
+        """A weight of 4-bit codes with group scales on this session's device (see
+        spissa_amd.linear.Q4LinearWeight)."""
+        from .linear import Q4LinearWeight
+
+        return Q4LinearWeight(codes, scales, out_features, in_features, group, zeros, session=self)
+
     def linear(self, weight, x, bias, batch: int, out) -> None:
         """out[batch, out] = x[batch, in] x W^T + bias on device tensors (bias may be None)."""
         check(self._lib.spissa_linear_device(self.handle, weight.handle, _dev(x, "x"),

@@ -25,6 +25,7 @@ from .rotary import _f32, _ptr
 DTYPE_F32 = 0
 DTYPE_F16 = 1
 DTYPE_BF16 = 2
+DTYPE_Q4 = 3
 
 
 class MissingTensorError(SpissaError):
@@ -109,6 +110,53 @@ class LinearWeight:
             self.close()
         except Exception:
             pass
+
+
+class Q4LinearWeight(LinearWeight):
+    """A [out_features, in_features] weight of 4-bit codes with a scale, and a zero
+    point, for each group of input channels (spissa_linear_weight_q4_new):
+    W[n, k] = scales[n, k // group] * (code[n, k] - zeros[n, k // group]).
+
+    codes: uint8 [out_features, ceil(in_features / 2)], the even channel in the low
+    four bits. scales: [out_features, ceil(in_features / group)], float32, float16
+    or bfloat16 (a numpy uint16 array holds bfloat16 bits). zeros: uint8 of the
+    scales' shape, 0..15, or None (8 everywhere). Each is a contiguous numpy array
+    or a contiguous device tensor (then read after the current stream's work).
+    group: a multiple of 32. Used like a LinearWeight, as an LM head table too.
+    """
+
+    def __init__(self, codes, scales, out_features: int, in_features: int, group: int, zeros=None, session=None):
+        lib = _ffi.load()
+        self._lib = lib
+        cp, cn, _ = self._bytes(codes, "codes", {"uint8": None})
+        sp, sn, scale_dtype = self._bytes(scales, "scales", {"float32": DTYPE_F32, "float16": DTYPE_F16,
+                                                             "bfloat16": DTYPE_BF16, "uint16": DTYPE_BF16})
+        zp, zn, _ = (None, 0, None) if zeros is None else self._bytes(zeros, "zeros", {"uint8": None})
+        s = session.handle if session is not None else self._default_session(lib)
+        self._session = session
+        h = _ffi.c_void_p()
+        check(lib.spissa_linear_weight_q4_new(s, out_features, in_features, group, scale_dtype, cp, cn, sp, sn, zp, zn,
+                                              C.byref(h)))
+        self._h = h
+        self.dtype, self.out_features, self.in_features, self.group = DTYPE_Q4, out_features, in_features, group
+
+    @staticmethod
+    def _bytes(data, name: str, dtypes):
+        """(pointer, bytes, what `dtypes` has for its type) of an array or device tensor."""
+        on_device = getattr(data, "is_cuda", False)
+        kind = str(data.dtype).replace("torch.", "")
+        if kind not in dtypes or not (on_device or isinstance(data, np.ndarray)):
+            raise TypeError(f"{name} must be a numpy array or device tensor of {', '.join(dtypes)}")
+        if on_device:
+            import torch
+
+            if not data.is_contiguous():
+                raise TypeError(f"{name} must be contiguous")
+            torch.cuda.current_stream(data.device).synchronize()
+            return _ffi.c_void_p(data.data_ptr()), data.numel() * data.element_size(), dtypes[kind]
+        if not data.flags.c_contiguous:
+            raise TypeError(f"{name} must be contiguous")
+        return data.ctypes.data_as(_ffi.c_void_p), data.nbytes, dtypes[kind]
 
 
 class LinearModel:

@@ -18,7 +18,7 @@ import numpy as np
 
 from . import _ffi
 from .errors import ShapeError, check
-from .linear import DTYPE_BF16, DTYPE_F32, LinearWeight
+from .linear import DTYPE_BF16, DTYPE_F32, DTYPE_Q4, LinearWeight
 from .rotary import _f32, _ptr
 
 
@@ -46,6 +46,11 @@ def lm_head_logits_parallel_bf16(last_hidden: np.ndarray, table: LinearWeight, v
                                  hidden: int) -> np.ndarray:
     """streaming/mod.rs:238-272, bf16 table."""
     return _logits(table, last_hidden, vocab_size, hidden, DTYPE_BF16)
+
+
+def lm_head_logits_q4(last_hidden: np.ndarray, table: LinearWeight, vocab_size: int, hidden: int) -> np.ndarray:
+    """The same over a table of 4-bit codes with group scales (Q4LinearWeight)."""
+    return _logits(table, last_hidden, vocab_size, hidden, DTYPE_Q4)
 
 
 def _session(session):
