@@ -1475,7 +1475,7 @@ static int q4_attend_batch(spissa_session *s, const float *q, const spissa_kv_ca
       a.seq[b].len = (int)(caches[b0 + b]->len + extra);
       keys[b] = c->window ? (int)std::min<size_t>(a.seq[b].len, c->window) : a.seq[b].len;
     }
-    const Q4AttnPlan p = q4_attend_plan(D, R, Hkv, keys, B, 1, (size_t)1 << 40);
+    const Q4AttnPlan p = q4_attend_plan(D, R, Hkv, keys, B);
     ST_TRY(ensure_buf(s, s->partial, q4_partial_bytes(B, Hq, D, p, Hkv)));
     a.q = q + b0 * (size_t)Hq * D;
     a.out = out + b0 * (size_t)Hq * D;
@@ -1486,7 +1486,6 @@ static int q4_attend_batch(spissa_session *s, const float *q, const spissa_kv_ca
     a.R = R;
     a.HB = p.HB;
     a.window = (int)c->window;
-    a.causal = c->causal ? 1 : 0;
     a.kps = p.kps;
     a.max_splits = p.splits;
     a.qscale = (1.0f / sqrtf((float)D)) * 1.4426950408889634f;
@@ -1495,36 +1494,49 @@ static int q4_attend_batch(spissa_session *s, const float *q, const spissa_kv_ca
   return SPISSA_OK;
 }
 
-// The queries of the cache's last S rows; its length is `len`, those rows included.
+// The queries of the cache's last S rows; its length is `len`, those rows
+// included. q4_chunk_prepare makes its workspace.
+static Q4ChunkPlan q4_chunk_plan_of(spissa_session *s, size_t len, const spissa_kv_attention_config *c) {
+  return q4_chunk_plan((int)c->head_dim, (int)c->query_len, (int)(c->num_heads / c->kv_heads), (int)c->kv_heads, (int)len,
+                       c->causal ? 1 : 0, (int)c->window, s->cus);
+}
+static int q4_chunk_prepare(spissa_session *s, size_t len, const spissa_kv_attention_config *c) {
+  const Q4ChunkPlan p = q4_chunk_plan_of(s, len, c);
+  return p.partial_bytes ? ensure_buf(s, s->ppart, p.partial_bytes) : SPISSA_OK;
+}
 static int q4_attend_chunk(spissa_session *s, const float *q, const spissa_kv_cache *cache, size_t len,
                            const spissa_kv_attention_config *c, float *out) {
-  const int D = (int)c->head_dim, Hq = (int)c->num_heads, Hkv = (int)c->kv_heads, R = Hq / Hkv;
-  const size_t S = c->query_len;
-  constexpr size_t kMost = 1024;  // queries of a launch
-  for (size_t t0 = 0; t0 < S; t0 += kMost) {
-    const int n = (int)std::min(kMost, S - t0);
-    Q4AttnArgs a{};
-    a.seq[0].rows = q4_rows(cache, 0);
-    a.seq[0].len = (int)len;
-    const int keys = (int)(c->window && c->causal ? std::min<size_t>(len, c->window) : len);
-    const Q4AttnPlan p = q4_attend_plan(D, R, Hkv, &keys, 1, n, (size_t)64 << 20);
-    ST_TRY(ensure_buf(s, s->partial, p.partial_bytes));
-    a.q = q;
-    a.out = out;
-    a.partial = (float *)s->partial.p;
-    a.err = s->d_err;
-    a.Hq = Hq;
-    a.Hkv = Hkv;
-    a.R = R;
-    a.HB = p.HB;
-    a.window = (int)c->window;
-    a.causal = c->causal ? 1 : 0;
-    a.kps = p.kps;
-    a.max_splits = p.splits;
-    a.queries = (int)S;
-    a.query0 = (int)t0;
-    a.qscale = (1.0f / sqrtf((float)D)) * 1.4426950408889634f;
-    HIP_TRY(launch_q4_attend(s->stream, a, D, p.RB, n));
+  const Q4ChunkPlan p = q4_chunk_plan_of(s, len, c);
+  const int D = (int)c->head_dim;
+  Q4ChunkArgs a{};
+  a.q = q;
+  a.out = out;
+  a.err = s->d_err;
+  a.rows = q4_rows(cache, 0);
+  a.len = (int)len;
+  a.S = (int)c->query_len;
+  a.Hq = (int)c->num_heads;
+  a.Hkv = (int)c->kv_heads;
+  a.R = a.Hq / a.Hkv;
+  a.causal = c->causal ? 1 : 0;
+  a.window = (int)c->window;
+  a.qscale = (1.0f / sqrtf((float)D)) * 1.4426950408889634f;
+  a.splits = p.splits;
+  a.tps = p.tps;
+  const size_t rows = c->query_len * c->num_heads;
+  a.part_o = (float *)s->ppart.p;
+  a.part_ml = a.part_o + (size_t)p.splits * rows * D;
+  HIP_TRY(launch_q4_chunk(s->stream, a, D));
+  if (p.splits > 1) {
+    PrefillArgs m{};
+    m.out = out;
+    m.S = a.S;
+    m.Hq = a.Hq;
+    m.err = a.err;
+    m.splits = p.splits;
+    m.part_o = a.part_o;
+    m.part_ml = a.part_ml;
+    HIP_TRY(launch_prefill_combine(s->stream, m, D));
   }
   return SPISSA_OK;
 }
@@ -1576,10 +1588,11 @@ static int q4_step(spissa_session *s, const spissa_rope_table *table, const floa
   // (workspaces before the first launch: nothing is appended by a call that fails for want of them)
   if (S == 1) {
     const int one = 1;
-    const Q4AttnPlan p = q4_attend_plan((int)cfg->head_dim, (int)(cfg->num_heads / cfg->kv_heads), (int)cfg->kv_heads, &one, 1,
-                                        1, (size_t)1 << 40);
+    const Q4AttnPlan p = q4_attend_plan((int)cfg->head_dim, (int)(cfg->num_heads / cfg->kv_heads), (int)cfg->kv_heads, &one, 1);
     ST_TRY(ensure_buf(s, s->partial,
                       q4_partial_bytes(std::min<size_t>(batch, kMaxDecodeBatch), cfg->num_heads, cfg->head_dim, p, cfg->kv_heads)));
+  } else {
+    ST_TRY(q4_chunk_prepare(s, caches[0]->len + S, cfg));
   }
   ST_TRY(q4_append(s, caches, batch, S, q == d_q ? nullptr : d_q, cfg->num_heads, d_k, d_v, table, norm,
                    const_cast<float *>(q)));
@@ -1895,7 +1908,9 @@ extern "C" int spissa_attention_cached_device(spissa_session *s, const float *d_
     if (!(aligned16(d_q) && aligned16(d_out)))
       return set_err(SPISSA_ERR_ARGUMENT, "attention over a 4-bit cache takes 16-byte aligned buffers");
     HIP_TRY(hipSetDevice(s->device));
-    return S == 1 ? q4_attend_batch(s, d_q, &cache, 1, cfg, d_out, 0) : q4_attend_chunk(s, d_q, cache, cache->len, cfg, d_out);
+    if (S == 1) return q4_attend_batch(s, d_q, &cache, 1, cfg, d_out, 0);
+    ST_TRY(q4_chunk_prepare(s, cache->len, cfg));
+    return q4_attend_chunk(s, d_q, cache, cache->len, cfg, d_out);
   }
   const int D = (int)cfg->head_dim;
   if (!prefill_supported(D) || s->prefill_precision != SPISSA_PREFILL_BF16)

@@ -357,15 +357,13 @@ hipError_t launch_q4_append(hipStream_t st, const Q4AppendArgs &a, int D, int B)
 // Rows [s.first, s.first + n) as f32 [n, Hkv, D]; either output may be null.
 hipError_t launch_q4_rows(hipStream_t st, const Q4Rows &s, size_t n, size_t Hkv, size_t D, float *k_out, float *v_out);
 
-// Attention of single queries: the last token of each sequence of a batch
-// (queries 0), or the last `queries` rows' queries of one sequence, of which a
-// launch takes those from query0 on.
+// Attention of the last token of each sequence of a batch.
 struct Q4AttnBase {
-  const float *q;   // [B or queries, Hq, D]
+  const float *q;   // [B, Hq, D]
   float *out;
-  float *partial;   // [B or queries, Hkv, HB, max_splits] entries of RB * (D + 2) floats
+  float *partial;   // [B, Hkv, HB, max_splits] entries of RB * (D + 2) floats
   int *err;
-  int Hq, Hkv, R, HB, window, causal, kps, max_splits, queries, query0;
+  int Hq, Hkv, R, HB, window, kps, max_splits;
   float qscale;     // softmax scale * log2(e)
 };
 struct Q4Seq {
@@ -380,11 +378,31 @@ struct Q4AttnArgsOf : Q4AttnBase {
 typedef Q4AttnArgsOf<kMaxDecodeBatch> Q4AttnArgs;
 struct Q4AttnPlan {
   int RB, HB, kps, splits;
-  size_t partial_bytes;
 };
-// keys[i]: visible keys of the n queries of a launch (times `copies`: queries alike).
-Q4AttnPlan q4_attend_plan(int D, int R, int Hkv, const int *keys, int n, long copies, size_t partial_cap);
+// keys[i]: visible keys of the n sequences of a launch.
+Q4AttnPlan q4_attend_plan(int D, int R, int Hkv, const int *keys, int n);
 hipError_t launch_q4_attend(hipStream_t st, const Q4AttnArgs &a, int D, int RB, int nz);
 bool q4_supported(size_t D);
+
+// Attention of the queries of a cache's last S rows (q4_chunk.hip).
+struct Q4ChunkArgs {
+  const float *q;  // [S, Hq, D]
+  float *out;
+  int *err;
+  Q4Rows rows;
+  int len, S, Hq, Hkv, R, causal, window;
+  float qscale;    // softmax scale * log2(e)
+  // With splits > 1, split j takes key tiles [j * tps, (j + 1) * tps) of those a
+  // workgroup sees and writes its part as PrefillArgs has it; launch_prefill_combine
+  // merges them.
+  int splits, tps;
+  float *part_o, *part_ml;
+};
+struct Q4ChunkPlan {
+  int splits = 1, tps = 0;
+  size_t partial_bytes = 0;
+};
+Q4ChunkPlan q4_chunk_plan(int D, int S, int R, int Hkv, int len, int causal, int window, int cus);
+hipError_t launch_q4_chunk(hipStream_t st, const Q4ChunkArgs &a, int D);
 
 }  // namespace spissa

@@ -190,19 +190,17 @@ __global__ __launch_bounds__(256) void q4_rows_kernel(const Q4Rows s, int n, int
 
 namespace {
 
-// The keys that query `z` of a launch sees, [lo, hi).
+// The keys that the last token of sequence z sees, [lo, hi).
 template <int MB>
 __device__ __forceinline__ void visible(const Q4AttnArgsOf<MB> &a, int z, int *lo, int *hi) {
-  const int len = a.seq[a.queries ? 0 : z].len;
-  const int pos = a.queries ? len - a.queries + a.query0 + z : len - 1;
-  *hi = a.causal ? pos + 1 : len;
-  *lo = a.window > 0 ? max(0, pos + 1 - a.window) : 0;
+  *hi = a.seq[z].len;
+  *lo = a.window > 0 ? max(0, *hi - a.window) : 0;
 }
 
 }  // namespace
 
 // One query of RB heads of a KV head (blockIdx.x) over one range of keys
-// (blockIdx.y) of sequence or chunk query blockIdx.z. A row is spread over D/16
+// (blockIdx.y) of sequence blockIdx.z. A row is spread over D/16
 // lanes of 16 channels (8 bytes of codes, half a 32-channel group):
 //   q.k = step * sum q code + min * sum q   (the lane's part), and
 //   o += (p step) code, o_min += p min,
@@ -220,8 +218,7 @@ __global__ __launch_bounds__(256) void q4_attend_kernel(const Q4AttnArgsOf<MB> a
   if (k0 >= hi) return;  // (split 0 always has a key: the query's own)
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int sub = lane % LPR, grp = wave * GPW + lane / LPR;
-  const int qrow = a.queries ? a.query0 + z : z;
-  const Q4Rows &seq_rows = a.seq[a.queries ? 0 : z].rows;
+  const Q4Rows &seq_rows = a.seq[z].rows;
   const uint2 *kc = reinterpret_cast<const uint2 *>(seq_rows.k) + (long)h * seq_rows.cap * LPR;
   const uint2 *vc = reinterpret_cast<const uint2 *>(seq_rows.v) + (long)h * seq_rows.cap * LPR;
   const unsigned *kp = seq_rows.kp + (long)h * seq_rows.cap * (D / 32);
@@ -231,7 +228,7 @@ __global__ __launch_bounds__(256) void q4_attend_kernel(const Q4AttnArgsOf<MB> a
 #pragma unroll
   for (int r = 0; r < RB; ++r) {
     const int head = h * a.R + min(hb * RB + r, a.R - 1);  // (the last block may have heads to spare)
-    const float4 *src = reinterpret_cast<const float4 *>(a.q + ((long)qrow * a.Hq + head) * D + 16 * sub);
+    const float4 *src = reinterpret_cast<const float4 *>(a.q + ((long)z * a.Hq + head) * D + 16 * sub);
     qsum[r] = 0.0f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -356,7 +353,7 @@ __global__ __launch_bounds__(256) void q4_attend_kernel(const Q4AttnArgsOf<MB> a
         dst[RB * D + 2 * r + 1] = L;
       }
     } else if (hb * RB + r < a.R) {
-      a.out[((long)qrow * a.Hq + h * a.R + hb * RB + r) * D + dim] = O / L;
+      a.out[((long)z * a.Hq + h * a.R + hb * RB + r) * D + dim] = O / L;
       if (dim == 0 && !(L > 0.0f && L < __builtin_inff())) atomicOr(a.err, kDevErrSoftmaxDenominator);
     }
   }
@@ -401,8 +398,7 @@ __global__ __launch_bounds__(256) void q4_combine_kernel(const Q4AttnArgsOf<MB> 
       L += s_l[k][out] * g;
       O += s_o[k][out] * g;
     }
-    const int qrow = a.queries ? a.query0 + z : z;
-    a.out[((long)qrow * a.Hq + h * a.R + hb * RB) * D + e] = O / L;
+    a.out[((long)z * a.Hq + h * a.R + hb * RB) * D + e] = O / L;
     if ((e % D) == 0 && !(L > 0.0f && L < __builtin_inff())) atomicOr(a.err, kDevErrSoftmaxDenominator);
   }
 }
@@ -424,7 +420,7 @@ hipError_t attend(hipStream_t st, const Q4AttnArgsOf<MB> &a, int nz) {
 
 template <int D, int RB>
 hipError_t attend_b(hipStream_t st, const Q4AttnArgs &a, int nz) {
-  if (nz == 1 || a.queries) {
+  if (nz == 1) {
     Q4AttnArgsOf<1> one;
     static_cast<Q4AttnBase &>(one) = a;
     one.seq[0] = a.seq[0];
@@ -448,7 +444,7 @@ hipError_t attend_d(hipStream_t st, const Q4AttnArgs &a, int RB, int nz) {
 
 bool q4_supported(size_t D) { return D == 64 || D == 128 || D == 256; }
 
-Q4AttnPlan q4_attend_plan(int D, int R, int Hkv, const int *keys, int n, long copies, size_t partial_cap) {
+Q4AttnPlan q4_attend_plan(int D, int R, int Hkv, const int *keys, int n) {
   Q4AttnPlan p;
   p.HB = (R + 3) / 4;
   p.RB = (R + p.HB - 1) / p.HB;
@@ -459,15 +455,13 @@ Q4AttnPlan q4_attend_plan(int D, int R, int Hkv, const int *keys, int n, long co
     total += keys[i];
     most = std::max(most, keys[i]);
   }
-  const long heads = (long)Hkv * p.HB * copies;
+  const long heads = (long)Hkv * p.HB;
   const long per = (total * heads + kDecodeGridWorkgroups - 1) / kDecodeGridWorkgroups;
   long kps = std::max<long>(1, (per + chunk - 1) / chunk) * chunk;
-  const size_t entry = (size_t)p.RB * (D + 2) * sizeof(float) * heads * n;
-  long cap = std::min<long>(kMaxDecodeSplits, std::max<long>(1, (long)(partial_cap / entry)));
-  if ((most + kps - 1) / kps > cap) kps = ((most + cap - 1) / cap + chunk - 1) / chunk * chunk;
+  if ((most + kps - 1) / kps > kMaxDecodeSplits)
+    kps = ((most + kMaxDecodeSplits - 1) / kMaxDecodeSplits + chunk - 1) / chunk * chunk;
   p.kps = (int)kps;
   p.splits = (int)((most + kps - 1) / kps);
-  p.partial_bytes = p.splits > 1 ? entry * p.splits : 0;
   return p;
 }
 
