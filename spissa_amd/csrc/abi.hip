@@ -147,7 +147,10 @@ struct spissa_kv_cache {
   unsigned *kp = nullptr, *vp = nullptr;
   float *vmax = nullptr;    // [H]
   size_t width() const { return num_heads * head_dim; }
-  // bytes of keys or values that `rows` rows take in 4 bits
+  // Bytes of keys or values that `rows` rows take in 4 bits, and that the buffers
+  // have: tiles of keys are read whole, up to 63 rows past the last.
+  size_t q4_codes_end() const { return q4_codes(max_seq_len) + 64 * (head_dim / 2); }
+  size_t q4_params_end() const { return q4_params(max_seq_len) + 64 * (head_dim / 32) * sizeof(unsigned); }
   size_t q4_codes(size_t rows) const { return rows * num_heads * (head_dim / 2); }
   size_t q4_params(size_t rows) const { return rows * num_heads * (head_dim / 32) * sizeof(unsigned); }
 };
@@ -449,7 +452,7 @@ static int kv_q4_new_impl(spissa_session *s, size_t num_heads, size_t head_dim, 
   c->head_dim = head_dim;
   c->max_seq_len = max_seq_len;
   c->q4 = true;
-  const size_t codes = c->q4_codes(max_seq_len), params = c->q4_params(max_seq_len);
+  const size_t codes = c->q4_codes_end(), params = c->q4_params_end();
   const size_t bytes = 2 * (codes + params) + num_heads * sizeof(float);
   HIP_TRY(hipSetDevice(s->device));
   ST_TRY(no_capture(s->stream, "a 4-bit cache", bytes));
@@ -760,7 +763,7 @@ extern "C" int spissa_kv_cache_clone(const spissa_kv_cache *c, spissa_kv_cache *
   hipError_t e = hipSuccess;
   if (c->q4) {
     // (whole: a head's rows are apart, so the first rows of all are not one range)
-    const size_t all = 2 * (c->q4_codes(c->max_seq_len) + c->q4_params(c->max_seq_len)) + c->num_heads * sizeof(float);
+    const size_t all = 2 * (c->q4_codes_end() + c->q4_params_end()) + c->num_heads * sizeof(float);
     e = hipMemcpyAsync(n->kc, c->kc, all, hipMemcpyDeviceToDevice, s->stream);
   } else if (bytes) {
     e = hipMemcpyAsync(n->keys, c->keys, bytes, hipMemcpyDeviceToDevice, s->stream);

@@ -9,7 +9,7 @@
 // one more instruction over the groups:
 //   s = 2^-e (sum_g step_g (code . q)_g + sum_g min_g (sum q)_g).
 // Output: the values, step * code + min scaled by a power of two from the
-// head's largest, and the probabilities, times 2^14, are two pieces each, of
+// head's largest, and the probabilities, times 2^6, are two pieces each, of
 // whose four products the three above 2^-22 are taken.
 //
 // A workgroup (four waves) takes 64 QT rows of a KV head, a row being a (query,
@@ -42,11 +42,13 @@ __device__ __forceinline__ float half_hi(unsigned w) {
 __device__ __forceinline__ half2v pieces2(float a, float b) {
   return __builtin_bit_cast(half2v, __builtin_amdgcn_cvt_pkrtz(a, b));
 }
-__device__ __forceinline__ void split8(const float (&v)[8], half8 *hi, half8 *lo) {
+// (minus_one: -1 as the compiler does not know it, so that the difference is one
+// mixed-precision FMA and not a conversion and a subtraction)
+__device__ __forceinline__ void split8(const float (&v)[8], float minus_one, half8 *hi, half8 *lo) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const half2v h = pieces2(v[2 * i], v[2 * i + 1]);
-    const half2v l = pieces2(v[2 * i] - (float)h.x, v[2 * i + 1] - (float)h.y);
+    const half2v l = pieces2(fmaf((float)h.x, minus_one, v[2 * i]), fmaf((float)h.y, minus_one, v[2 * i + 1]));
     (*hi)[2 * i] = h.x;
     (*hi)[2 * i + 1] = h.y;
     (*lo)[2 * i] = l.x;
@@ -61,11 +63,12 @@ __device__ __forceinline__ float inverse_scale(unsigned bits) { return __uint_as
 
 // A key row's eight codes of a word in the order in which weights of a pair
 // come off it: 0, 4, 1, 5, 2, 6, 3, 7 (queries are put in that order too).
-__device__ __forceinline__ half8 codes8h(unsigned w) {
+// (base: 0x64006400, 1024 twice, in a register: an and-or takes one constant)
+__device__ __forceinline__ half8 codes8h(unsigned w, unsigned base) {
   half8 r;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const half2v p = __builtin_bit_cast(half2v, ((w >> (4 * i)) & 0x000f000fu) | 0x64006400u) -
+    const half2v p = __builtin_bit_cast(half2v, ((w >> (4 * i)) & 0x000f000fu) | base) -
                      (half2v){(_Float16)1024.0f, (_Float16)1024.0f};
     r[2 * i] = p.x;
     r[2 * i + 1] = p.y;
@@ -84,8 +87,13 @@ __global__ __launch_bounds__(256, 2) void q4_chunk_kernel(const Q4ChunkArgs a) {
   __shared__ __attribute__((aligned(16))) half8 v_lds[2][VB * DT * 64];
   __shared__ __attribute__((aligned(16))) float step_lds[KT * G * 16];
   __shared__ __attribute__((aligned(16))) _Float16 min_lds[BN][8];
-  __shared__ unsigned vp_lds[2][BN * G];  // the values' steps and minima, of this tile and the next
+  constexpr int CB = BN * D / 2, PB = BN * G * 4, RAW = 2 * (CB + PB);  // bytes of a tile's codes and params
+  __shared__ __attribute__((aligned(16))) char raw_lds[RAW];
 
+  float minus_one = -1.0f;
+  unsigned base1024 = 0x64006400u;
+  asm volatile("" : "+s"(minus_one));
+  asm volatile("" : "+v"(base1024));
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, kq = lane >> 4;
   // Blocks of rows, the last (longest) first; key splits of each.
@@ -137,18 +145,18 @@ __global__ __launch_bounds__(256, 2) void q4_chunk_kernel(const Q4ChunkArgs a) {
         v[g][i] *= scale;
         sums[g] += v[g][i];
       }
-      split8(v[g], &qh[t][g], &ql[t][g]);
+      split8(v[g], minus_one, &qh[t][g], &ql[t][g]);
       sums[g] = sum32(sum16(sums[g]));
     }
     // the sums' three pieces, one for each of the first three quarters of K
     half8 s0, s1, s2;
     float rest[8];
-    split8(sums, &s0, &s1);
+    split8(sums, minus_one, &s0, &s1);
 #pragma unroll
     for (int i = 0; i < 8; ++i) rest[i] = (sums[i] - (float)s0[i]) - (float)s1[i];
     {
       half8 unused;
-      split8(rest, &s2, &unused);
+      split8(rest, minus_one, &s2, &unused);
     }
     __builtin_amdgcn_sched_barrier(0);
     const half8 none{};
@@ -174,11 +182,26 @@ __global__ __launch_bounds__(256, 2) void q4_chunk_kernel(const Q4ChunkArgs a) {
     for (int d = 0; d < DT; ++d) o[t][d] = (f32x4){0.f, 0.f, 0.f, 0.f};
   }
 
-  // (a head's rows stay below 2^31 bytes: 32-bit offsets from a scalar base)
+  // A tile's codes, steps and minima come as they are, straight into LDS (1 KB a
+  // wave and instruction), while the tile before is computed. The rows past the
+  // last are read too (the buffers end 64 rows later) and may hold anything:
+  // their keys are hidden, and their values taken as zeros.
   const long head = (long)h * a.rows.cap;
-  const char *kc = reinterpret_cast<const char *>(a.rows.k) + head * (D / 2);
-  const char *vc = reinterpret_cast<const char *>(a.rows.v) + head * (D / 2);
-  const char *kp = reinterpret_cast<const char *>(a.rows.kp + head * G), *vp = reinterpret_cast<const char *>(a.rows.vp + head * G);
+  const char *src[4] = {reinterpret_cast<const char *>(a.rows.k) + head * (D / 2),
+                        reinterpret_cast<const char *>(a.rows.v) + head * (D / 2),
+                        reinterpret_cast<const char *>(a.rows.kp + head * G), reinterpret_cast<const char *>(a.rows.vp + head * G)};
+  auto fetch = [&](int tile) {
+#pragma unroll
+    for (int i = 0; i < (RAW + 4095) / 4096; ++i) {
+      const int at = i * 4096 + wave * 1024 + lane * 16;  // raw_lds: keys' codes, values' codes, keys' params, values' params
+      if (at >= RAW) continue;
+      const int part = at < CB ? 0 : at < 2 * CB ? 1 : at < 2 * CB + PB ? 2 : 3;
+      const int off = at - (part == 0 ? 0 : part == 1 ? CB : part == 2 ? 2 * CB : 2 * CB + PB);
+      const char *from = part == 0 ? src[0] : part == 1 ? src[1] : part == 2 ? src[2] : src[3];
+      __builtin_amdgcn_global_load_lds(from + (long)tile * (part < 2 ? CB : PB) + off,
+                                       (__attribute__((address_space(3))) void *)(raw_lds + i * 4096 + wave * 1024), 16, 0, 0);
+    }
+  };
   const unsigned vsb = scale_to(a.rows.vmax[h], 13);
   const float vscale = __uint_as_float(vsb);
 
@@ -188,39 +211,33 @@ __global__ __launch_bounds__(256, 2) void q4_chunk_kernel(const Q4ChunkArgs a) {
   const int kkey = (tid & 15) + 16 * (tid / (16 * G)), kg = (tid >> 4) % G;
   const bool kwork = BN * G >= 256 || tid < BN * G;
   const int vd = tid % DC * DPT, vq = tid / DC % 4, vb = tid / (4 * DC);
-  const int last = a.len - 1;  // (rows past it are not read; their keys are hidden)
-  u32x4 kw{};
-  unsigned kpw = 0, vpw = 0, vw[8];
-  auto fetch = [&](int tile) {
-    const int base = tile * BN;
-    if (kwork) {
-      const unsigned at = (unsigned)min(base + kkey, last) * G + kg;
-      kw = *reinterpret_cast<const u32x4 *>(kc + at * 16u);
-      kpw = *reinterpret_cast<const unsigned *>(kp + at * 4u);
-      vpw = *reinterpret_cast<const unsigned *>(vp + at * 4u);
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const unsigned row = min(base + 32 * vb + 4 * vq + (i & 3) + 16 * (i >> 2), last);
-      const char *src = vc + (row * (D / 2) + vd / 2);
-      if constexpr (DPT == 4) vw[i] = *reinterpret_cast<const unsigned short *>(src);
-      else vw[i] = *reinterpret_cast<const unsigned char *>(src);
-    }
-  };
-  auto widen = [&](int buf) {
+  auto widen = [&](int tile) {
     if (kwork) {
       const int kt = kkey >> 4;
+      const u32x4 kw = *reinterpret_cast<const u32x4 *>(raw_lds + (kkey * G + kg) * 16);
+      const unsigned kp = *reinterpret_cast<const unsigned *>(raw_lds + 2 * CB + (kkey * G + kg) * 4);
 #pragma unroll
-      for (int q = 0; q < 4; ++q) k_lds[(kt * G + kg) * 64 + q * 16 + (kkey & 15)] = codes8h(kw[q]);
-      step_lds[(kt * G + kg) * 16 + (kkey & 15)] = half_lo(kpw);
-      min_lds[kkey][kg] = __builtin_bit_cast(_Float16, (unsigned short)(kpw >> 16));
+      for (int q = 0; q < 4; ++q) k_lds[(kt * G + kg) * 64 + q * 16 + (kkey & 15)] = codes8h(kw[q], base1024);
+      step_lds[(kt * G + kg) * 16 + (kkey & 15)] = half_lo(kp);
+      min_lds[kkey][kg] = __builtin_bit_cast(_Float16, (unsigned short)(kp >> 16));
     }
     float st[8], mn[8];
+    unsigned vw[8];
+    const char *const params = raw_lds + 2 * CB + PB + ((32 * vb + 4 * vq) * G + vd / 32) * 4;
+    const char *const codes = raw_lds + CB + (32 * vb + 4 * vq) * (D / 2) + vd / 2;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const unsigned p = vp_lds[buf][(32 * vb + 4 * vq + (i & 3) + 16 * (i >> 2)) * G + vd / 32];
+      const unsigned p = *reinterpret_cast<const unsigned *>(params + ((i & 3) + 16 * (i >> 2)) * (G * 4));
+      const char *c = codes + ((i & 3) + 16 * (i >> 2)) * (D / 2);
+      if constexpr (DPT == 4) vw[i] = *reinterpret_cast<const unsigned short *>(c);
+      else vw[i] = *reinterpret_cast<const unsigned char *>(c);
       st[i] = half_lo(p) * vscale;
       mn[i] = half_hi(p) * vscale;
+    }
+    if ((tile + 1) * BN > a.len) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (tile * BN + 32 * vb + 4 * vq + (i & 3) + 16 * (i >> 2) >= a.len) st[i] = mn[i] = 0.0f;
     }
     const int dt = vd >> 4;
 #pragma unroll
@@ -229,7 +246,7 @@ __global__ __launch_bounds__(256, 2) void q4_chunk_kernel(const Q4ChunkArgs a) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] = fmaf(st[i], (float)((vw[i] >> (4 * j)) & 15u), mn[i]);
       half8 vh, vl;
-      split8(v, &vh, &vl);
+      split8(v, minus_one, &vh, &vl);
       // (the low bits mixed with the channel tile: the writes of a wave fall on all banks)
       const int at = (vb * DT + dt) * 64 + ((vq * 16 + (vd & 15) + j) ^ (dt & 7));
       v_lds[0][at] = vh;
@@ -241,18 +258,13 @@ __global__ __launch_bounds__(256, 2) void q4_chunk_kernel(const Q4ChunkArgs a) {
     for (int g = G; g < 8; ++g) min_lds[tid][g] = (_Float16)0.0f;
   }
 
-  auto keep_vp = [&](int buf) {
-    if (kwork) vp_lds[buf][kkey * G + kg] = vpw;
-  };
-  if (t0 < t1) {
-    fetch(t0);
-    keep_vp(t0 & 1);
-  }
+  if (t0 < t1) fetch(t0);
   for (int tile = t0; tile < t1; ++tile) {
-    __syncthreads();  // (the tile before is no longer read)
-    widen(tile & 1);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (a wave's part of the tile is in LDS)
+    __syncthreads();  // the tile before is no longer read
+    widen(tile);
     __syncthreads();
-    fetch(min(tile + 1, t1 - 1));
+    if (tile + 1 < t1) fetch(tile + 1);
     const int base = tile * BN;
     // 32 keys at a time: their scores, the rows' maximum, the weights, the output.
 #pragma unroll 1
@@ -266,18 +278,33 @@ __global__ __launch_bounds__(256, 2) void q4_chunk_kernel(const Q4ChunkArgs a) {
 #pragma unroll
         for (int t = 0; t < QT; ++t)
           s[k][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(mf, qs[t], (f32x4){0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+        // two groups' instructions side by side: those that depend on each
+        // other are 2 QT apart
 #pragma unroll
-        for (int g = 0; g < G; ++g) {
-          const half8 kf = k_lds[((2 * b + k) * G + g) * 64 + lane];
-          const f32x4 st = *reinterpret_cast<const f32x4 *>(&step_lds[((2 * b + k) * G + g) * 16 + 4 * kq]);
+        for (int g = 0; g < G; g += 2) {
+          half8 kf[2];
+          f32x4 st[2], c[2][QT];
 #pragma unroll
-          for (int t = 0; t < QT; ++t) {
-            f32x4 c = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[t][g], (f32x4){0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
-            c = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[t][g], c, 0, 0, 0);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[k][t][e] = fmaf(st[e], c[e], s[k][t][e]);
+          for (int i = 0; i < 2; ++i) {
+            kf[i] = k_lds[((2 * b + k) * G + g + i) * 64 + lane];
+            st[i] = *reinterpret_cast<const f32x4 *>(&step_lds[((2 * b + k) * G + g + i) * 16 + 4 * kq]);
           }
-          if (g % 2 == 1) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int t = 0; t < QT; ++t)
+              c[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[i], ql[t][g + i], (f32x4){0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int t = 0; t < QT; ++t) c[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[i], qh[t][g + i], c[i][t], 0, 0, 0);
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int t = 0; t < QT; ++t)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) s[k][t][e] = fmaf(st[i][e], c[i][t][e], s[k][t][e]);
+          __builtin_amdgcn_sched_barrier(0);
         }
       }
       __builtin_amdgcn_sched_barrier(0);
@@ -305,17 +332,19 @@ __global__ __launch_bounds__(256, 2) void q4_chunk_kernel(const Q4ChunkArgs a) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) top = fmaxf(top, s[k][t][e]);
         top = max32(max16(top)) * inv[t];
-        const float mnew = fmaxf(m[t], top), ms = safe_max(mnew);
-        const float alpha = fast_exp2(m[t] - ms);
-        m[t] = mnew;
-        l[t] *= alpha;
-        if (__any(alpha != 1.0f)) {
+        // The reference rises when a score passes it by 8: weights stay below
+        // 2^14, and the output is rarely scaled anew.
+        if (__any(top > m[t] + 8.0f)) {
+          const float mnew = fmaxf(m[t], top);
+          const float alpha = fast_exp2(m[t] - safe_max(mnew));
+          m[t] = mnew;
+          l[t] *= alpha;
 #pragma unroll
           for (int d = 0; d < DT; ++d)
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[t][d][e] *= alpha;
         }
-        const float shift = 14.0f - ms;
+        const float shift = 6.0f - safe_max(m[t]);
         float p[8];
 #pragma unroll
         for (int k = 0; k < 2; ++k)
@@ -324,23 +353,33 @@ __global__ __launch_bounds__(256, 2) void q4_chunk_kernel(const Q4ChunkArgs a) {
             p[4 * k + e] = fast_exp2(fmaf(s[k][t][e], inv[t], shift));
             l[t] += p[4 * k + e];
           }
-        split8(p, &ph[t], &pl[t]);
+        split8(p, minus_one, &ph[t], &pl[t]);
       }
       __builtin_amdgcn_sched_barrier(0);
+      // two channel tiles side by side, for the same reason
 #pragma unroll
-      for (int d = 0; d < DT; ++d) {
-        const half8 vh = v_lds[0][(b * DT + d) * 64 + (lane ^ (d & 7))];
-        const half8 vl = v_lds[1][(b * DT + d) * 64 + (lane ^ (d & 7))];
+      for (int d = 0; d < DT; d += 2) {
+        half8 vh[2], vl[2];
 #pragma unroll
-        for (int t = 0; t < QT; ++t) {
-          o[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, ph[t], o[t][d], 0, 0, 0);
-          o[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, pl[t], o[t][d], 0, 0, 0);
-          o[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, ph[t], o[t][d], 0, 0, 0);
+        for (int i = 0; i < 2; ++i) {
+          vh[i] = v_lds[0][(b * DT + d + i) * 64 + (lane ^ ((d + i) & 7))];
+          vl[i] = v_lds[1][(b * DT + d + i) * 64 + (lane ^ ((d + i) & 7))];
         }
-        if (d % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int t = 0; t < QT; ++t) o[t][d + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl[i], ph[t], o[t][d + i], 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int t = 0; t < QT; ++t) o[t][d + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh[i], pl[t], o[t][d + i], 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int t = 0; t < QT; ++t) o[t][d + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh[i], ph[t], o[t][d + i], 0, 0, 0);
+        if (d % 4 == 2) __builtin_amdgcn_sched_barrier(0);
       }
     }
-    keep_vp((tile + 1) & 1);
   }
 
   const float vinv = inverse_scale(vsb);
