@@ -148,9 +148,9 @@ struct spissa_kv_cache {
   float *vmax = nullptr;    // [H]
   size_t width() const { return num_heads * head_dim; }
   // Bytes of keys or values that `rows` rows take in 4 bits, and that the buffers
-  // have: tiles of keys are read whole, up to 63 rows past the last.
-  size_t q4_codes_end() const { return q4_codes(max_seq_len) + 64 * (head_dim / 2); }
-  size_t q4_params_end() const { return q4_params(max_seq_len) + 64 * (head_dim / 32) * sizeof(unsigned); }
+  // have: tiles of keys are read whole, up to 127 rows past the last.
+  size_t q4_codes_end() const { return q4_codes(max_seq_len) + 128 * (head_dim / 2); }
+  size_t q4_params_end() const { return q4_params(max_seq_len) + 128 * (head_dim / 32) * sizeof(unsigned); }
   size_t q4_codes(size_t rows) const { return rows * num_heads * (head_dim / 2); }
   size_t q4_params(size_t rows) const { return rows * num_heads * (head_dim / 32) * sizeof(unsigned); }
 };

@@ -12,10 +12,10 @@
 // head's largest, and the probabilities, times 2^6, are two pieces each, of
 // whose four products the three above 2^-22 are taken.
 //
-// A workgroup (four waves) takes 64 QT rows of a KV head, a row being a (query,
+// A workgroup takes 128 QT rows of a KV head, a row being a (query,
 // query head of the group) pair with the head fastest, so that short chunks
-// fill the instruction's 16 columns with heads. Per tile of BN keys it widens
-// the codes into LDS once for all of them: the keys as they are, in the order in
+// fill the instruction's 16 columns with heads. Per tile of keys it widens the
+// codes into LDS once for all of them: the keys as they are, in the order in
 // which lanes take the A operand, the values as two pieces of V^T. The scores
 // are formed as S^T = K Q^T, so a lane has one row (column lane % 16) and four
 // keys of each 16, and two such blocks are the B operand of O^T += V^T P^T
@@ -61,6 +61,14 @@ __device__ __forceinline__ unsigned scale_to(float most, unsigned top) {
 }
 __device__ __forceinline__ float inverse_scale(unsigned bits) { return __uint_as_float((254u << 23) - bits); }
 
+// Copies 16 bytes a lane from base + off into LDS at lds_base + 16 * lane, unknown
+// to the compiler, which would wait for it before any later LDS read: the kernel's
+// barriers wait for the copies that the next step reads.
+__device__ __forceinline__ void copy16(const char *base, unsigned off, char *lds_base) {
+  const unsigned lds = (unsigned)(uintptr_t)(__attribute__((address_space(3))) void *)lds_base;
+  asm volatile("global_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "{m0}"(lds) : "memory");
+}
+
 // A key row's eight codes of a word in the order in which weights of a pair
 // come off it: 0, 4, 1, 5, 2, 6, 3, 7 (queries are put in that order too).
 // (base: 0x64006400, 1024 twice, in a register: an and-or takes one constant)
@@ -78,17 +86,23 @@ __device__ __forceinline__ half8 codes8h(unsigned w, unsigned base) {
 
 }  // namespace
 
-template <int D, int QT, int BN>
-__global__ __launch_bounds__(256, 2) void q4_chunk_kernel(const Q4ChunkArgs a) {
-  constexpr int G = D / 32, DT = D / 16, KT = BN / 16, VB = BN / 32;
-  constexpr int DPT = D * BN / 2048;  // channels of a thread's eight keys
-  static_assert(DPT == 2 || DPT == 4, "");
-  __shared__ __attribute__((aligned(16))) half8 k_lds[KT * G * 64];
-  __shared__ __attribute__((aligned(16))) half8 v_lds[2][VB * DT * 64];
-  __shared__ __attribute__((aligned(16))) float step_lds[KT * G * 16];
-  __shared__ __attribute__((aligned(16))) _Float16 min_lds[BN][8];
+// Eight waves. A tile of 8192 / D keys is in LDS twice (this one and the next),
+// as it came and widened. Between two barriers a wave widens its part of the next
+// tile and computes its rows' part of this one, the first four waves in that
+// order and the last four in the other: a SIMD has one of each, so the
+// conversions of one run beside the matrix instructions of the other (one loop
+// body, in which the two kinds have the barrier at different places). Within a
+// wave the LDS reads run one step ahead of the instructions that need them.
+template <int D, int QT>
+__global__ __launch_bounds__(512, 2) void q4_chunk_kernel(const Q4ChunkArgs a) {
+  constexpr int BN = 8192 / D, G = D / 32, DT = D / 16, VB = BN / 32, NW = 8;
   constexpr int CB = BN * D / 2, PB = BN * G * 4, RAW = 2 * (CB + PB);  // bytes of a tile's codes and params
-  __shared__ __attribute__((aligned(16))) char raw_lds[RAW];
+  static_assert(CB == 4096 && PB == 1024, "a tile has the same bytes for every D");
+  __shared__ __attribute__((aligned(16))) half8 k_lds[2][BN * G * 4];
+  __shared__ __attribute__((aligned(16))) half8 v_lds[2][2][VB * DT * 64];
+  __shared__ __attribute__((aligned(16))) float step_lds[2][BN * G];
+  __shared__ __attribute__((aligned(16))) _Float16 min_lds[2][BN][8];
+  __shared__ __attribute__((aligned(16))) char raw_lds[2][RAW];
 
   float minus_one = -1.0f;
   unsigned base1024 = 0x64006400u;
@@ -100,14 +114,36 @@ __global__ __launch_bounds__(256, 2) void q4_chunk_kernel(const Q4ChunkArgs a) {
   const int h = blockIdx.y, split = blockIdx.z;
   const int block = gridDim.x - 1 - blockIdx.x;
   const int rows = a.S * a.R;
-  const int row0 = block * (64 * QT) + wave * (16 * QT);
+  const int row0 = block * (NW * 16 * QT) + wave * (16 * QT);
   const int P = a.len - a.S;  // the first query's position
   // keys that any row of the workgroup sees
-  const int first_q = block * (64 * QT) / a.R, last_q = min(rows - 1, block * (64 * QT) + 64 * QT - 1) / a.R;
+  const int first_q = block * (NW * 16 * QT) / a.R, last_q = min(rows - 1, (block + 1) * (NW * 16 * QT) - 1) / a.R;
   const int hi = a.causal ? P + last_q + 1 : a.len;
   const int lo = a.window > 0 ? max(0, P + first_q + 1 - a.window) : 0;
   const int t0 = lo / BN + split * a.tps;
   const int t1 = min((hi + BN - 1) / BN, t0 + a.tps);
+
+  // A tile's codes, steps and minima come as they are, straight into LDS (1 KB a
+  // wave and instruction). The rows past the last are read too (the buffers end
+  // 128 rows later) and may hold anything: their keys are hidden, and their
+  // values taken as zeros.
+  const long head = (long)h * a.rows.cap;
+  const char *src[4] = {reinterpret_cast<const char *>(a.rows.k) + head * (D / 2),
+                        reinterpret_cast<const char *>(a.rows.v) + head * (D / 2),
+                        reinterpret_cast<const char *>(a.rows.kp + head * G), reinterpret_cast<const char *>(a.rows.vp + head * G)};
+  auto fetch = [&](int tile) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int chunk = i * NW + wave;  // keys' codes 4, values' codes 4, keys' params 1, values' params 1
+      if (chunk >= RAW / 1024) continue;
+      const int part = chunk < 4 ? 0 : chunk < 8 ? 1 : chunk - 6;
+      const char *from = (part == 0 ? src[0] : part == 1 ? src[1] : part == 2 ? src[2] : src[3]) +
+                         (long)tile * (part < 2 ? CB : PB) + (part < 2 ? (chunk & 3) * 1024 : 0);
+      copy16(from, lane * 16, raw_lds[tile & 1] + chunk * 1024);
+    }
+  };
+  if (t0 < t1) fetch(t0);
+  if (t0 + 1 < t1) fetch(t0 + 1);
 
   // A lane's row, for each of its QT column tiles.
   int pos[QT];
@@ -120,11 +156,11 @@ __global__ __launch_bounds__(256, 2) void q4_chunk_kernel(const Q4ChunkArgs a) {
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
     pos[t] = P + min(row0 + 16 * t + col, rows - 1) / a.R;
-    const float *src = a.q + query_row(t) * D + 8 * kq;
+    const float *q = a.q + query_row(t) * D + 8 * kq;
     float v[G][8], most = 0.0f;
 #pragma unroll
     for (int g = 0; g < G; ++g) {
-      const float4 x = *reinterpret_cast<const float4 *>(src + 32 * g), y = *reinterpret_cast<const float4 *>(src + 32 * g + 4);
+      const float4 x = *reinterpret_cast<const float4 *>(q + 32 * g), y = *reinterpret_cast<const float4 *>(q + 32 * g + 4);
       const float u[8] = {x.x, y.x, x.y, y.y, x.z, y.z, x.w, y.w};  // channels 0, 4, 1, 5, ...
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -181,133 +217,134 @@ __global__ __launch_bounds__(256, 2) void q4_chunk_kernel(const Q4ChunkArgs a) {
 #pragma unroll
     for (int d = 0; d < DT; ++d) o[t][d] = (f32x4){0.f, 0.f, 0.f, 0.f};
   }
-
-  // A tile's codes, steps and minima come as they are, straight into LDS (1 KB a
-  // wave and instruction), while the tile before is computed. The rows past the
-  // last are read too (the buffers end 64 rows later) and may hold anything:
-  // their keys are hidden, and their values taken as zeros.
-  const long head = (long)h * a.rows.cap;
-  const char *src[4] = {reinterpret_cast<const char *>(a.rows.k) + head * (D / 2),
-                        reinterpret_cast<const char *>(a.rows.v) + head * (D / 2),
-                        reinterpret_cast<const char *>(a.rows.kp + head * G), reinterpret_cast<const char *>(a.rows.vp + head * G)};
-  auto fetch = [&](int tile) {
-#pragma unroll
-    for (int i = 0; i < (RAW + 4095) / 4096; ++i) {
-      const int at = i * 4096 + wave * 1024 + lane * 16;  // raw_lds: keys' codes, values' codes, keys' params, values' params
-      if (at >= RAW) continue;
-      const int part = at < CB ? 0 : at < 2 * CB ? 1 : at < 2 * CB + PB ? 2 : 3;
-      const int off = at - (part == 0 ? 0 : part == 1 ? CB : part == 2 ? 2 * CB : 2 * CB + PB);
-      const char *from = part == 0 ? src[0] : part == 1 ? src[1] : part == 2 ? src[2] : src[3];
-      __builtin_amdgcn_global_load_lds(from + (long)tile * (part < 2 ? CB : PB) + off,
-                                       (__attribute__((address_space(3))) void *)(raw_lds + i * 4096 + wave * 1024), 16, 0, 0);
-    }
-  };
   const unsigned vsb = scale_to(a.rows.vmax[h], 13);
   const float vscale = __uint_as_float(vsb);
 
-  // A thread's share of a tile: a key's group of 32 channels, and eight keys of
-  // DPT channels of the values (keys 4 q + 0..3 and 16 + 4 q + 0..3 of 32).
-  constexpr int DC = D / DPT;
-  const int kkey = (tid & 15) + 16 * (tid / (16 * G)), kg = (tid >> 4) % G;
-  const bool kwork = BN * G >= 256 || tid < BN * G;
-  const int vd = tid % DC * DPT, vq = tid / DC % 4, vb = tid / (4 * DC);
+  // A thread's share of a tile: half a key's group of 32 channels, and eight keys
+  // (4 q + 0..3 and 16 + 4 q + 0..3 of 32) of two channels of the values.
+  const int kkey = (tid & 15) + 16 * (tid / (32 * G)), kg = (tid >> 4) % G, khalf = tid / (16 * G) & 1;
+  const int vd = tid % (D / 2) * 2, vq = tid / (D / 2) % 4, vb = tid / (2 * D);
   auto widen = [&](int tile) {
-    if (kwork) {
-      const int kt = kkey >> 4;
-      const u32x4 kw = *reinterpret_cast<const u32x4 *>(raw_lds + (kkey * G + kg) * 16);
-      const unsigned kp = *reinterpret_cast<const unsigned *>(raw_lds + 2 * CB + (kkey * G + kg) * 4);
-#pragma unroll
-      for (int q = 0; q < 4; ++q) k_lds[(kt * G + kg) * 64 + q * 16 + (kkey & 15)] = codes8h(kw[q], base1024);
-      step_lds[(kt * G + kg) * 16 + (kkey & 15)] = half_lo(kp);
-      min_lds[kkey][kg] = __builtin_bit_cast(_Float16, (unsigned short)(kp >> 16));
-    }
-    float st[8], mn[8];
-    unsigned vw[8];
-    const char *const params = raw_lds + 2 * CB + PB + ((32 * vb + 4 * vq) * G + vd / 32) * 4;
-    const char *const codes = raw_lds + CB + (32 * vb + 4 * vq) * (D / 2) + vd / 2;
+    const int buf = tile & 1;
+    const char *const raw = raw_lds[buf];
+    const unsigned vstart = (32 * vb + 4 * vq) * G + vd / 32;
+    const char *const params = raw + 2 * CB + PB + vstart * 4;
+    const unsigned char *const codes = reinterpret_cast<const unsigned char *>(raw) + CB + (32 * vb + 4 * vq) * (D / 2) + vd / 2;
+    const uint2 kw = *reinterpret_cast<const uint2 *>(raw + (kkey * G + kg) * 16 + khalf * 8);
+    const unsigned kp = *reinterpret_cast<const unsigned *>(raw + 2 * CB + (kkey * G + kg) * 4);
+    unsigned vw[8], vp[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const unsigned p = *reinterpret_cast<const unsigned *>(params + ((i & 3) + 16 * (i >> 2)) * (G * 4));
-      const char *c = codes + ((i & 3) + 16 * (i >> 2)) * (D / 2);
-      if constexpr (DPT == 4) vw[i] = *reinterpret_cast<const unsigned short *>(c);
-      else vw[i] = *reinterpret_cast<const unsigned char *>(c);
-      st[i] = half_lo(p) * vscale;
-      mn[i] = half_hi(p) * vscale;
+      vp[i] = *reinterpret_cast<const unsigned *>(params + ((i & 3) + 16 * (i >> 2)) * (G * 4));
+      vw[i] = codes[((i & 3) + 16 * (i >> 2)) * (D / 2)];
+    }
+    {
+      half8 *const dst = &k_lds[buf][((kkey >> 4) * G + kg) * 64 + khalf * 32 + (kkey & 15)];
+      dst[0] = codes8h(kw.x, base1024);
+      dst[16] = codes8h(kw.y, base1024);
+      if (khalf == 0) {
+        step_lds[buf][((kkey >> 4) * G + kg) * 16 + (kkey & 15)] = half_lo(kp);
+        min_lds[buf][kkey][kg] = __builtin_bit_cast(_Float16, (unsigned short)(kp >> 16));
+      }
+    }
+    float st[8], mn[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      st[i] = fmaf(half_lo(vp[i]), vscale, 0.0f);  // (one mixed-precision instruction)
+      mn[i] = fmaf(half_hi(vp[i]), vscale, 0.0f);
     }
     if ((tile + 1) * BN > a.len) {
+      int left = a.len - tile * BN - 32 * vb - 4 * vq;
+      asm volatile("" : "+v"(left));
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        if (tile * BN + 32 * vb + 4 * vq + (i & 3) + 16 * (i >> 2) >= a.len) st[i] = mn[i] = 0.0f;
+        if ((i & 3) + 16 * (i >> 2) >= left) st[i] = mn[i] = 0.0f;
     }
     const int dt = vd >> 4;
 #pragma unroll
-    for (int j = 0; j < DPT; ++j) {
+    for (int j = 0; j < 2; ++j) {
       float v[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = fmaf(st[i], (float)((vw[i] >> (4 * j)) & 15u), mn[i]);
+      for (int i = 0; i < 8; ++i) v[i] = fmaf(st[i], (float)(j ? vw[i] >> 4 : vw[i] & 15u), mn[i]);
       half8 vh, vl;
       split8(v, minus_one, &vh, &vl);
       // (the low bits mixed with the channel tile: the writes of a wave fall on all banks)
       const int at = (vb * DT + dt) * 64 + ((vq * 16 + (vd & 15) + j) ^ (dt & 7));
-      v_lds[0][at] = vh;
-      v_lds[1][at] = vl;
+      v_lds[buf][0][at] = vh;
+      v_lds[buf][1][at] = vl;
     }
   };
-  if (G < 8 && tid < BN) {
-#pragma unroll
-    for (int g = G; g < 8; ++g) min_lds[tid][g] = (_Float16)0.0f;
-  }
 
-  if (t0 < t1) fetch(t0);
-  for (int tile = t0; tile < t1; ++tile) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (a wave's part of the tile is in LDS)
-    __syncthreads();  // the tile before is no longer read
-    widen(tile);
-    __syncthreads();
-    if (tile + 1 < t1) fetch(tile + 1);
-    const int base = tile * BN;
+  auto compute = [&](int tile) {
+    const int buf = tile & 1, base = tile * BN;
+    if (base >= wave_hi || base + BN <= wave_lo) return;
     // 32 keys at a time: their scores, the rows' maximum, the weights, the output.
 #pragma unroll 1
     for (int b = 0; b < VB; ++b) {
       const int key0 = base + 32 * b;
       if (key0 >= wave_hi || key0 + 32 <= wave_lo) continue;
-      f32x4 s[2][QT];
+      // Steps of two groups of one 16 keys; those instructions that depend on
+      // each other are 2 QT apart.
+      constexpr int NS = G;
+      half8 kf[2][2], mf[2];
+      f32x4 st[2][2], s[2][QT];
+      const half8 *const kl = &k_lds[buf][2 * b * G * 64 + lane];
+      const float *const sl = &step_lds[buf][2 * b * G * 16 + 4 * kq];
+      auto load_k = [&](int step) {
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const half8 mf = *reinterpret_cast<const half8 *>(min_lds[32 * b + 16 * k + col]);
-#pragma unroll
-        for (int t = 0; t < QT; ++t)
-          s[k][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(mf, qs[t], (f32x4){0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
-        // two groups' instructions side by side: those that depend on each
-        // other are 2 QT apart
-#pragma unroll
-        for (int g = 0; g < G; g += 2) {
-          half8 kf[2];
-          f32x4 st[2], c[2][QT];
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            kf[i] = k_lds[((2 * b + k) * G + g + i) * 64 + lane];
-            st[i] = *reinterpret_cast<const f32x4 *>(&step_lds[((2 * b + k) * G + g + i) * 16 + 4 * kq]);
-          }
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int t = 0; t < QT; ++t)
-              c[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[i], ql[t][g + i], (f32x4){0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int t = 0; t < QT; ++t) c[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[i], qh[t][g + i], c[i][t], 0, 0, 0);
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int t = 0; t < QT; ++t)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) s[k][t][e] = fmaf(st[i][e], c[i][t][e], s[k][t][e]);
-          __builtin_amdgcn_sched_barrier(0);
+        for (int i = 0; i < 2; ++i) {
+          kf[step & 1][i] = kl[(2 * step + i) * 64];
+          st[step & 1][i] = *reinterpret_cast<const f32x4 *>(sl + (2 * step + i) * 16);
         }
+      };
+      half8 vh[2][2], vl[2][2];
+      // (one address a tile, its low bits mixed anew for each read)
+      unsigned v_at = buf * (unsigned)sizeof v_lds[0] + b * (DT * 1024) + lane * 16;
+      asm volatile("" : "+v"(v_at));
+      auto load_v = [&](int step) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int d = 2 * step + i;
+          const char *const at = reinterpret_cast<const char *>(v_lds) + (v_at ^ ((d & 7) * 16)) + d * 1024;
+          vh[step & 1][i] = *reinterpret_cast<const half8 *>(at);
+          vl[step & 1][i] = *reinterpret_cast<const half8 *>(at + sizeof v_lds[0][0]);
+        }
+      };
+      mf[0] = *reinterpret_cast<const half8 *>(min_lds[buf][32 * b + col]);
+      mf[1] = *reinterpret_cast<const half8 *>(min_lds[buf][32 * b + 16 + col]);
+      load_k(0);
+#pragma unroll
+      for (int step = 0; step < NS; ++step) {
+        const int k = step / (G / 2), g = 2 * step % G;
+        if (step + 1 < NS) load_k(step + 1);
+        else load_v(0);
+        f32x4 c[2][QT];
+        if (g == 0) {
+#pragma unroll
+          for (int t = 0; t < QT; ++t)
+            s[k][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(mf[k], qs[t], (f32x4){0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int t = 0; t < QT; ++t)
+            c[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[step & 1][i], ql[t][g + i], (f32x4){0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int t = 0; t < QT; ++t)
+            c[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[step & 1][i], qh[t][g + i], c[i][t], 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int t = 0; t < QT; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[k][t][e] = fmaf(st[step & 1][i][e], c[i][t][e], s[k][t][e]);
+        // (the sums stay in their step: left to itself the compiler keeps every step's products until the last)
+#pragma unroll
+        for (int t = 0; t < QT; ++t) asm volatile("" : "+v"(s[k][t]));
+        __builtin_amdgcn_sched_barrier(0);
       }
-      __builtin_amdgcn_sched_barrier(0);
       half8 ph[QT], pl[QT];
 #pragma unroll
       for (int t = 0; t < QT; ++t) {
@@ -356,30 +393,51 @@ __global__ __launch_bounds__(256, 2) void q4_chunk_kernel(const Q4ChunkArgs a) {
         split8(p, minus_one, &ph[t], &pl[t]);
       }
       __builtin_amdgcn_sched_barrier(0);
-      // two channel tiles side by side, for the same reason
+      // steps of two channel tiles
 #pragma unroll
-      for (int d = 0; d < DT; d += 2) {
-        half8 vh[2], vl[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          vh[i] = v_lds[0][(b * DT + d + i) * 64 + (lane ^ ((d + i) & 7))];
-          vl[i] = v_lds[1][(b * DT + d + i) * 64 + (lane ^ ((d + i) & 7))];
-        }
+      for (int step = 0; step < DT / 2; ++step) {
+        if (step + 1 < DT / 2) load_v(step + 1);
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
-          for (int t = 0; t < QT; ++t) o[t][d + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl[i], ph[t], o[t][d + i], 0, 0, 0);
+          for (int t = 0; t < QT; ++t)
+            o[t][2 * step + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl[step & 1][i], ph[t], o[t][2 * step + i], 0, 0, 0);
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
-          for (int t = 0; t < QT; ++t) o[t][d + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh[i], pl[t], o[t][d + i], 0, 0, 0);
+          for (int t = 0; t < QT; ++t)
+            o[t][2 * step + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh[step & 1][i], pl[t], o[t][2 * step + i], 0, 0, 0);
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
-          for (int t = 0; t < QT; ++t) o[t][d + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh[i], ph[t], o[t][d + i], 0, 0, 0);
-        if (d % 4 == 2) __builtin_amdgcn_sched_barrier(0);
+          for (int t = 0; t < QT; ++t)
+            o[t][2 * step + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh[step & 1][i], ph[t], o[t][2 * step + i], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
+  };
+
+  if constexpr (G < 8) {
+    for (int i = tid; i < 2 * BN; i += 512)
+#pragma unroll
+      for (int g = G; g < 8; ++g) min_lds[i & 1][i >> 1][g] = (_Float16)0.0f;
+  }
+  // Barrier i: tile i is widened, tile i + 1 has come, and tile i - 1 is no longer
+  // read. The first waves widen tile i + 1 after it, the last ones before barrier
+  // i + 1, after computing tile i.
+  const bool ahead = wave < NW / 2;
+  auto barrier = [&](int tile) {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (tile + 2 < t1) fetch(tile + 2);
+  };
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");  // the first two tiles have come
+#pragma unroll 1
+  for (int tile = t0 - 1; tile < t1; ++tile) {
+    if (ahead && tile >= t0) barrier(tile);
+    const int next = ahead ? tile + 1 : tile;
+    if (next >= t0 && next < t1) widen(next);
+    if (!ahead && tile >= t0) barrier(tile);
+    if (tile >= t0) compute(tile);
   }
 
   const float vinv = inverse_scale(vsb);
@@ -413,16 +471,14 @@ __global__ __launch_bounds__(256, 2) void q4_chunk_kernel(const Q4ChunkArgs a) {
 
 namespace {
 
-// Keys of a tile, and column tiles of a wave.
-constexpr int chunk_keys(int D) { return D == 256 ? 32 : 64; }
-constexpr int chunk_cols(int D) { return D == 256 ? 1 : 2; }
+// Column tiles of a wave: two, where the registers hold them and the rows fill them.
+int chunk_cols(int D, long rows) { return D == 256 || rows <= 128 ? 1 : 2; }
 
-template <int D>
+template <int D, int QT>
 hipError_t chunk(hipStream_t st, const Q4ChunkArgs &a) {
-  constexpr int QT = chunk_cols(D), BN = chunk_keys(D);
   const long rows = (long)a.S * a.R;
-  const dim3 grid((unsigned)((rows + 64 * QT - 1) / (64 * QT)), (unsigned)a.Hkv, (unsigned)a.splits);
-  hipLaunchKernelGGL((q4_chunk_kernel<D, QT, BN>), grid, dim3(256), 0, st, a);
+  const dim3 grid((unsigned)((rows + 128 * QT - 1) / (128 * QT)), (unsigned)a.Hkv, (unsigned)a.splits);
+  hipLaunchKernelGGL((q4_chunk_kernel<D, QT>), grid, dim3(512), 0, st, a);
   return hipGetLastError();
 }
 
@@ -430,13 +486,13 @@ hipError_t chunk(hipStream_t st, const Q4ChunkArgs &a) {
 
 Q4ChunkPlan q4_chunk_plan(int D, int S, int R, int Hkv, int len, int causal, int window, int cus) {
   Q4ChunkPlan p;
-  const int BN = chunk_keys(D), per = 64 * chunk_cols(D);
+  const int BN = 8192 / D, per = 128 * chunk_cols(D, (long)S * R);
   const long blocks = ((long)S * R + per - 1) / per * Hkv;
   // tiles that the workgroup with the most keys visits
   long span = len;
   if (window > 0 && causal) span = std::min<long>(len, (long)window + per / R + 1);
   const long tiles = (span + BN - 1) / BN + 1;
-  long splits = std::max<long>(1, 2L * cus / blocks);
+  long splits = std::max<long>(1, cus / blocks);
   splits = std::min(splits, std::max<long>(1, tiles / 4));
   splits = std::min<long>(splits, 64);
   p.tps = (int)((tiles + splits - 1) / splits);
@@ -446,10 +502,11 @@ Q4ChunkPlan q4_chunk_plan(int D, int S, int R, int Hkv, int len, int causal, int
 }
 
 hipError_t launch_q4_chunk(hipStream_t st, const Q4ChunkArgs &a, int D) {
+  const int cols = chunk_cols(D, (long)a.S * a.R);
   switch (D) {
-    case 64: return chunk<64>(st, a);
-    case 128: return chunk<128>(st, a);
-    case 256: return chunk<256>(st, a);
+    case 64: return cols == 1 ? chunk<64, 1>(st, a) : chunk<64, 2>(st, a);
+    case 128: return cols == 1 ? chunk<128, 1>(st, a) : chunk<128, 2>(st, a);
+    case 256: return chunk<256, 1>(st, a);
     default: return hipErrorInvalidValue;
   }
 }
