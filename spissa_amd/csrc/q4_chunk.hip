@@ -21,6 +21,7 @@
 // keys of each 16, and two such blocks are the B operand of O^T += V^T P^T
 // without an exchange, the values' keys being stored in that order.
 #include <algorithm>
+#include <type_traits>
 
 #include "internal.hpp"
 #include "lanes.hpp"
@@ -93,14 +94,18 @@ __device__ __forceinline__ half8 codes8h(unsigned w, unsigned base) {
 // conversions of one run beside the matrix instructions of the other (one loop
 // body, in which the two kinds have the barrier at different places). Within a
 // wave the LDS reads run one step ahead of the instructions that need them.
-template <int D, int QT>
-__global__ __launch_bounds__(512, 2) void q4_chunk_kernel(const Q4ChunkArgs a) {
-  constexpr int BN = 8192 / D, G = D / 32, DT = D / 16, VB = BN / 32, NW = 8;
+template <int D, int NW, int QT>
+__global__ __launch_bounds__(NW * 64, NW / 4) void q4_chunk_kernel(const Q4ChunkArgs a) {
+  constexpr int BN = 8192 / D, G = D / 32, DT = D / 16, VB = BN / 32;
+  constexpr int AH = NW == 16 ? 1 : 2;  // fragments of a step in registers, or of this one and the next
   constexpr int CB = BN * D / 2, PB = BN * G * 4, RAW = 2 * (CB + PB);  // bytes of a tile's codes and params
   static_assert(CB == 4096 && PB == 1024, "a tile has the same bytes for every D");
   __shared__ __attribute__((aligned(16))) half8 k_lds[2][BN * G * 4];
   __shared__ __attribute__((aligned(16))) half8 v_lds[2][2][VB * DT * 64];
-  __shared__ __attribute__((aligned(16))) float step_lds[2][BN * G];
+  // (sixteen waves have the steps in binary16, half the LDS reads, in mixed-precision FMAs; eight in f32)
+  typedef std::conditional_t<NW == 16, _Float16, float> step_t;
+  typedef __attribute__((ext_vector_type(4))) step_t step4;
+  __shared__ __attribute__((aligned(16))) step_t step_lds[2][BN * G];
   __shared__ __attribute__((aligned(16))) _Float16 min_lds[2][BN][8];
   __shared__ __attribute__((aligned(16))) char raw_lds[2][RAW];
 
@@ -110,9 +115,9 @@ __global__ __launch_bounds__(512, 2) void q4_chunk_kernel(const Q4ChunkArgs a) {
   asm volatile("" : "+v"(base1024));
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, kq = lane >> 4;
-  // Blocks of rows, the last (longest) first; key splits of each.
-  const int h = blockIdx.y, split = blockIdx.z;
-  const int block = gridDim.x - 1 - blockIdx.x;
+  // Blocks of rows, the last (longest) ones of every head first; key splits of each.
+  const int h = blockIdx.x, split = blockIdx.z;
+  const int block = gridDim.y - 1 - blockIdx.y;
   const int rows = a.S * a.R;
   const int row0 = block * (NW * 16 * QT) + wave * (16 * QT);
   const int P = a.len - a.S;  // the first query's position
@@ -133,7 +138,7 @@ __global__ __launch_bounds__(512, 2) void q4_chunk_kernel(const Q4ChunkArgs a) {
                         reinterpret_cast<const char *>(a.rows.kp + head * G), reinterpret_cast<const char *>(a.rows.vp + head * G)};
   auto fetch = [&](int tile) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < (RAW / 1024 + NW - 1) / NW; ++i) {
       const int chunk = i * NW + wave;  // keys' codes 4, values' codes 4, keys' params 1, values' params 1
       if (chunk >= RAW / 1024) continue;
       const int part = chunk < 4 ? 0 : chunk < 8 ? 1 : chunk - 6;
@@ -222,36 +227,36 @@ __global__ __launch_bounds__(512, 2) void q4_chunk_kernel(const Q4ChunkArgs a) {
 
   // A thread's share of a tile: half a key's group of 32 channels, and eight keys
   // (4 q + 0..3 and 16 + 4 q + 0..3 of 32) of two channels of the values.
-  const int kkey = (tid & 15) + 16 * (tid / (32 * G)), kg = (tid >> 4) % G, khalf = tid / (16 * G) & 1;
-  const int vd = tid % (D / 2) * 2, vq = tid / (D / 2) % 4, vb = tid / (2 * D);
-  auto widen = [&](int tile) {
+  // (sixteen waves: the first eight have the values, the last eight the keys)
+  const int part = tid & 511;
+  const int kkey = (part & 15) + 16 * (part / (32 * G)), kg = (part >> 4) % G, khalf = part / (16 * G) & 1;
+  const int vd = part % (D / 2) * 2, vq = part / (D / 2) % 4, vb = part / (2 * D);
+  auto widen_k = [&](int tile) {
     const int buf = tile & 1;
     const char *const raw = raw_lds[buf];
-    const unsigned vstart = (32 * vb + 4 * vq) * G + vd / 32;
-    const char *const params = raw + 2 * CB + PB + vstart * 4;
-    const unsigned char *const codes = reinterpret_cast<const unsigned char *>(raw) + CB + (32 * vb + 4 * vq) * (D / 2) + vd / 2;
     const uint2 kw = *reinterpret_cast<const uint2 *>(raw + (kkey * G + kg) * 16 + khalf * 8);
     const unsigned kp = *reinterpret_cast<const unsigned *>(raw + 2 * CB + (kkey * G + kg) * 4);
-    unsigned vw[8], vp[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      vp[i] = *reinterpret_cast<const unsigned *>(params + ((i & 3) + 16 * (i >> 2)) * (G * 4));
-      vw[i] = codes[((i & 3) + 16 * (i >> 2)) * (D / 2)];
+    half8 *const dst = &k_lds[buf][((kkey >> 4) * G + kg) * 64 + khalf * 32 + (kkey & 15)];
+    dst[0] = codes8h(kw.x, base1024);
+    dst[16] = codes8h(kw.y, base1024);
+    if (khalf == 0) {
+      step_lds[buf][((kkey >> 4) * G + kg) * 16 + (kkey & 15)] = (step_t)__builtin_bit_cast(_Float16, (unsigned short)kp);
+      min_lds[buf][kkey][kg] = __builtin_bit_cast(_Float16, (unsigned short)(kp >> 16));
     }
-    {
-      half8 *const dst = &k_lds[buf][((kkey >> 4) * G + kg) * 64 + khalf * 32 + (kkey & 15)];
-      dst[0] = codes8h(kw.x, base1024);
-      dst[16] = codes8h(kw.y, base1024);
-      if (khalf == 0) {
-        step_lds[buf][((kkey >> 4) * G + kg) * 16 + (kkey & 15)] = half_lo(kp);
-        min_lds[buf][kkey][kg] = __builtin_bit_cast(_Float16, (unsigned short)(kp >> 16));
-      }
-    }
+  };
+  auto widen_v = [&](int tile) {
+    const int buf = tile & 1;
+    const char *const raw = raw_lds[buf];
+    const char *const params = raw + 2 * CB + PB + ((32 * vb + 4 * vq) * G + vd / 32) * 4;
+    const unsigned char *const codes = reinterpret_cast<const unsigned char *>(raw) + CB + (32 * vb + 4 * vq) * (D / 2) + vd / 2;
+    unsigned vw[8];
     float st[8], mn[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      st[i] = fmaf(half_lo(vp[i]), vscale, 0.0f);  // (one mixed-precision instruction)
-      mn[i] = fmaf(half_hi(vp[i]), vscale, 0.0f);
+      const unsigned p = *reinterpret_cast<const unsigned *>(params + ((i & 3) + 16 * (i >> 2)) * (G * 4));
+      vw[i] = codes[((i & 3) + 16 * (i >> 2)) * (D / 2)];
+      st[i] = fmaf(half_lo(p), vscale, 0.0f);  // (one mixed-precision instruction)
+      mn[i] = fmaf(half_hi(p), vscale, 0.0f);
     }
     if ((tile + 1) * BN > a.len) {
       int left = a.len - tile * BN - 32 * vb - 4 * vq;
@@ -274,6 +279,10 @@ __global__ __launch_bounds__(512, 2) void q4_chunk_kernel(const Q4ChunkArgs a) {
       v_lds[buf][1][at] = vl;
     }
   };
+  auto widen = [&](int tile) {
+    if (NW == 8 || wave >= 8) widen_k(tile);
+    if (NW == 8 || wave < 8) widen_v(tile);
+  };
 
   auto compute = [&](int tile) {
     const int buf = tile & 1, base = tile * BN;
@@ -286,18 +295,19 @@ __global__ __launch_bounds__(512, 2) void q4_chunk_kernel(const Q4ChunkArgs a) {
       // Steps of two groups of one 16 keys; those instructions that depend on
       // each other are 2 QT apart.
       constexpr int NS = G;
-      half8 kf[2][2], mf[2];
-      f32x4 st[2][2], s[2][QT];
+      half8 kf[AH][2], mf[2];
+      step4 st[AH][2];
+      f32x4 s[2][QT];
       const half8 *const kl = &k_lds[buf][2 * b * G * 64 + lane];
-      const float *const sl = &step_lds[buf][2 * b * G * 16 + 4 * kq];
+      const step_t *const sl = &step_lds[buf][2 * b * G * 16 + 4 * kq];
       auto load_k = [&](int step) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          kf[step & 1][i] = kl[(2 * step + i) * 64];
-          st[step & 1][i] = *reinterpret_cast<const f32x4 *>(sl + (2 * step + i) * 16);
+          kf[step % AH][i] = kl[(2 * step + i) * 64];
+          st[step % AH][i] = *reinterpret_cast<const step4 *>(sl + (2 * step + i) * 16);
         }
       };
-      half8 vh[2][2], vl[2][2];
+      half8 vh[AH][2], vl[AH][2];
       // (one address a tile, its low bits mixed anew for each read)
       unsigned v_at = buf * (unsigned)sizeof v_lds[0] + b * (DT * 1024) + lane * 16;
       asm volatile("" : "+v"(v_at));
@@ -306,17 +316,18 @@ __global__ __launch_bounds__(512, 2) void q4_chunk_kernel(const Q4ChunkArgs a) {
         for (int i = 0; i < 2; ++i) {
           const int d = 2 * step + i;
           const char *const at = reinterpret_cast<const char *>(v_lds) + (v_at ^ ((d & 7) * 16)) + d * 1024;
-          vh[step & 1][i] = *reinterpret_cast<const half8 *>(at);
-          vl[step & 1][i] = *reinterpret_cast<const half8 *>(at + sizeof v_lds[0][0]);
+          vh[step % AH][i] = *reinterpret_cast<const half8 *>(at);
+          vl[step % AH][i] = *reinterpret_cast<const half8 *>(at + sizeof v_lds[0][0]);
         }
       };
       mf[0] = *reinterpret_cast<const half8 *>(min_lds[buf][32 * b + col]);
       mf[1] = *reinterpret_cast<const half8 *>(min_lds[buf][32 * b + 16 + col]);
-      load_k(0);
+      if (AH == 2) load_k(0);
 #pragma unroll
       for (int step = 0; step < NS; ++step) {
         const int k = step / (G / 2), g = 2 * step % G;
-        if (step + 1 < NS) load_k(step + 1);
+        if (AH == 1) load_k(step);
+        else if (step + 1 < NS) load_k(step + 1);
         else load_v(0);
         f32x4 c[2][QT];
         if (g == 0) {
@@ -328,18 +339,18 @@ __global__ __launch_bounds__(512, 2) void q4_chunk_kernel(const Q4ChunkArgs a) {
         for (int i = 0; i < 2; ++i)
 #pragma unroll
           for (int t = 0; t < QT; ++t)
-            c[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[step & 1][i], ql[t][g + i], (f32x4){0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+            c[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[step % AH][i], ql[t][g + i], (f32x4){0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
           for (int t = 0; t < QT; ++t)
-            c[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[step & 1][i], qh[t][g + i], c[i][t], 0, 0, 0);
+            c[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[step % AH][i], qh[t][g + i], c[i][t], 0, 0, 0);
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
           for (int t = 0; t < QT; ++t)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[k][t][e] = fmaf(st[step & 1][i][e], c[i][t][e], s[k][t][e]);
+            for (int e = 0; e < 4; ++e) s[k][t][e] = fmaf((float)st[step % AH][i][e], c[i][t][e], s[k][t][e]);
         // (the sums stay in their step: left to itself the compiler keeps every step's products until the last)
 #pragma unroll
         for (int t = 0; t < QT; ++t) asm volatile("" : "+v"(s[k][t]));
@@ -396,36 +407,37 @@ __global__ __launch_bounds__(512, 2) void q4_chunk_kernel(const Q4ChunkArgs a) {
       // steps of two channel tiles
 #pragma unroll
       for (int step = 0; step < DT / 2; ++step) {
-        if (step + 1 < DT / 2) load_v(step + 1);
+        if (AH == 1) load_v(step);
+        else if (step + 1 < DT / 2) load_v(step + 1);
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
           for (int t = 0; t < QT; ++t)
-            o[t][2 * step + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl[step & 1][i], ph[t], o[t][2 * step + i], 0, 0, 0);
+            o[t][2 * step + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl[step % AH][i], ph[t], o[t][2 * step + i], 0, 0, 0);
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
           for (int t = 0; t < QT; ++t)
-            o[t][2 * step + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh[step & 1][i], pl[t], o[t][2 * step + i], 0, 0, 0);
+            o[t][2 * step + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh[step % AH][i], pl[t], o[t][2 * step + i], 0, 0, 0);
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
           for (int t = 0; t < QT; ++t)
-            o[t][2 * step + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh[step & 1][i], ph[t], o[t][2 * step + i], 0, 0, 0);
+            o[t][2 * step + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh[step % AH][i], ph[t], o[t][2 * step + i], 0, 0, 0);
         __builtin_amdgcn_sched_barrier(0);
       }
     }
   };
 
   if constexpr (G < 8) {
-    for (int i = tid; i < 2 * BN; i += 512)
+    for (int i = tid; i < 2 * BN; i += NW * 64)
 #pragma unroll
       for (int g = G; g < 8; ++g) min_lds[i & 1][i >> 1][g] = (_Float16)0.0f;
   }
   // Barrier i: tile i is widened, tile i + 1 has come, and tile i - 1 is no longer
   // read. The first waves widen tile i + 1 after it, the last ones before barrier
   // i + 1, after computing tile i.
-  const bool ahead = wave < NW / 2;
+  const bool ahead = (wave & 4) == 0;
   auto barrier = [&](int tile) {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     if (tile + 2 < t1) fetch(tile + 2);
@@ -471,14 +483,13 @@ __global__ __launch_bounds__(512, 2) void q4_chunk_kernel(const Q4ChunkArgs a) {
 
 namespace {
 
-// Column tiles of a wave: two, where the registers hold them and the rows fill them.
-int chunk_cols(int D, long rows) { return D == 256 || rows <= 128 ? 1 : 2; }
+int chunk_rows(int D, long rows) { return D == 256 || rows <= 128 ? 128 : 256; }
 
-template <int D, int QT>
+template <int D, int NW, int QT>
 hipError_t chunk(hipStream_t st, const Q4ChunkArgs &a) {
   const long rows = (long)a.S * a.R;
-  const dim3 grid((unsigned)((rows + 128 * QT - 1) / (128 * QT)), (unsigned)a.Hkv, (unsigned)a.splits);
-  hipLaunchKernelGGL((q4_chunk_kernel<D, QT>), grid, dim3(512), 0, st, a);
+  const dim3 grid((unsigned)a.Hkv, (unsigned)((rows + NW * 16 * QT - 1) / (NW * 16 * QT)), (unsigned)a.splits);
+  hipLaunchKernelGGL((q4_chunk_kernel<D, NW, QT>), grid, dim3(NW * 64), 0, st, a);
   return hipGetLastError();
 }
 
@@ -486,7 +497,7 @@ hipError_t chunk(hipStream_t st, const Q4ChunkArgs &a) {
 
 Q4ChunkPlan q4_chunk_plan(int D, int S, int R, int Hkv, int len, int causal, int window, int cus) {
   Q4ChunkPlan p;
-  const int BN = 8192 / D, per = 128 * chunk_cols(D, (long)S * R);
+  const int BN = 8192 / D, per = chunk_rows(D, (long)S * R);
   const long blocks = ((long)S * R + per - 1) / per * Hkv;
   // tiles that the workgroup with the most keys visits
   long span = len;
@@ -502,11 +513,11 @@ Q4ChunkPlan q4_chunk_plan(int D, int S, int R, int Hkv, int len, int causal, int
 }
 
 hipError_t launch_q4_chunk(hipStream_t st, const Q4ChunkArgs &a, int D) {
-  const int cols = chunk_cols(D, (long)a.S * a.R);
+  const bool wide = chunk_rows(D, (long)a.S * a.R) == 256;
   switch (D) {
-    case 64: return cols == 1 ? chunk<64, 1>(st, a) : chunk<64, 2>(st, a);
-    case 128: return cols == 1 ? chunk<128, 1>(st, a) : chunk<128, 2>(st, a);
-    case 256: return chunk<256, 1>(st, a);
+    case 64: return wide ? chunk<64, 16, 1>(st, a) : chunk<64, 8, 1>(st, a);
+    case 128: return wide ? chunk<128, 16, 1>(st, a) : chunk<128, 8, 1>(st, a);
+    case 256: return chunk<256, 8, 1>(st, a);
     default: return hipErrorInvalidValue;
   }
 }
