@@ -91,12 +91,19 @@ struct BlockParams {
   }
 };
 
+// 1024 twice in binary16, as a value that the compiler does not know: an and-or
+// takes one constant, so the other is in a register.
+__device__ __forceinline__ unsigned base_1024() {
+  unsigned b = 0x64006400u;
+  asm volatile("" : "+v"(b));
+  return b;
+}
 // The eight codes of a word less their zero point.
-__device__ __forceinline__ half8 weights8(unsigned w, half2v zero) {
+__device__ __forceinline__ half8 weights8(unsigned w, half2v zero, unsigned base) {
   half8 r;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const unsigned u = ((w >> (4 * i)) & 0x000f000fu) | 0x64006400u;
+    const unsigned u = ((w >> (4 * i)) & 0x000f000fu) | base;
     const half2v p = __builtin_bit_cast(half2v, u) - zero;
     r[2 * i] = p.x;
     r[2 * i + 1] = p.y;
@@ -212,17 +219,73 @@ __global__ __launch_bounds__(256) void q4_pack_kernel(const Q4PackArgs a) {
   }
 }
 
+// The weights and params of a block of NT tiles, as a lane has them.
+template <int PT, int GPB, int NT>
+struct BlockWeights {
+  u32x4 w[NT];
+  BlockParams<PT, GPB> p[NT];
+  __device__ __forceinline__ void load(const char *const (&codes)[NT], const char *const (&params)[NT], long block) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      w[t] = *reinterpret_cast<const u32x4 *>(codes[t] + block * 1024);
+      p[t].load(params[t] + block * (16 * GPB * Q4Param<PT>::BYTES));
+    }
+  }
+};
+
+// acc += the block's products with the A fragments hi, lo (rows 4 (lane / 16) + 0..3
+// of A), the first E rows of the lane's four.
+template <int PT, int GPB, int NT, int E, typename FRAGS, typename INV>
+__device__ __forceinline__ void block_products(const BlockWeights<PT, GPB, NT> &b, unsigned base, FRAGS frags, const INV &inv,
+                                               float (&acc)[NT][E]) {
+  constexpr int SPG = 4 / GPB;  // 32-deep steps of a group
+  f32x4 sum[NT];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    half8 hi, lo;
+    frags(j, &hi, &lo);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const half8 wf = weights8(b.w[t][j], b.p[t].zero(j / SPG), base);
+      if (j % SPG == 0) sum[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+      sum[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, wf, sum[t], 0, 0, 0);
+      sum[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, wf, sum[t], 0, 0, 0);
+      if (j % SPG == SPG - 1) {
+        const float s = b.p[t].scale(j / SPG);
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[t][e] = fmaf(sum[t][e], s * inv[e], acc[t][e]);
+      }
+    }
+  }
+}
+
+// A lane's tiles: where their codes and params begin. (Tiles past the last are
+// read as the last and not stored.)
+template <int PT, int GPB, int NT>
+__device__ __forceinline__ void tile_addresses(const Q4LinearArgs &a, long tile0, int lane, const char *(&codes)[NT],
+                                               const char *(&params)[NT]) {
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const long tile = min(tile0 + t, (long)a.tiles - 1);
+    codes[t] = reinterpret_cast<const char *>(a.codes) + tile * a.blocks * 1024 + lane * 16;
+    params[t] =
+        reinterpret_cast<const char *>(a.params) + (tile * a.blocks * 16 + (lane & 15)) * (GPB * Q4Param<PT>::BYTES);
+  }
+}
+
 // Up to MP (1 or 4) tokens. A wave takes NT row tiles over a range of K blocks;
-// the waves of a workgroup are wk ranges x wn runs of tiles. Per 256 channels a
+// the waves of a workgroup are wk ranges x runs of tiles. Per 512 channels a
 // wave splits its tokens' activations into LDS of its own, in the order in
 // which the lanes read them as the matrix instruction's A operand: the 16 rows
 // of A repeat the MP tokens, so every lane's accumulators are the same tokens'.
+// The codes and activations of the next 512 channels are in flight meanwhile.
 // Bound: HBM for large weights (the codes), latency for small ones.
 template <int PT, int GPB, int MP, int NT>
 __global__ __launch_bounds__(512) void q4_gemv_kernel(const Q4LinearArgs a) {
-  constexpr int KC = 2, SPG = 4 / GPB;  // blocks of a round; 32-deep steps of a group
+  constexpr int KC = 4;  // blocks of a round
   __shared__ __attribute__((aligned(16))) half8 xs[8][KC * 4 * 2 * 4 * MP];  // [wave][step][piece][quarter][token]
   __shared__ float red[8][NT * 16][MP];
+  const unsigned base = base_1024();
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wk = wave % a.wk, wn = wave / a.wk;
   const int row = lane & 15, quarter = lane >> 4;
@@ -230,13 +293,7 @@ __global__ __launch_bounds__(512) void q4_gemv_kernel(const Q4LinearArgs a) {
   const long tile0 = ((long)blockIdx.x * runs + wn) * NT;
   const int b0 = wk * a.blocks_per_wave, b1 = min(a.blocks, b0 + a.blocks_per_wave);
   const char *codes[NT], *params[NT];
-#pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    const long tile = min(tile0 + t, (long)a.tiles - 1);  // (tiles past the last are read and not stored)
-    codes[t] = reinterpret_cast<const char *>(a.codes) + tile * a.blocks * 1024 + lane * 16;
-    params[t] = reinterpret_cast<const char *>(a.params) + (tile * a.blocks * 16 + row) * (GPB * Q4Param<PT>::BYTES);
-  }
-  constexpr int PB = 16 * GPB * Q4Param<PT>::BYTES;  // bytes of a tile block's params
+  tile_addresses<PT, GPB, NT>(a, tile0, lane, codes, params);
 
   float acc[NT][MP];
 #pragma unroll
@@ -244,55 +301,55 @@ __global__ __launch_bounds__(512) void q4_gemv_kernel(const Q4LinearArgs a) {
 #pragma unroll
     for (int m = 0; m < MP; ++m) acc[t][m] = 0.0f;
 
+  BlockWeights<PT, GPB, NT> w[KC];
+  float4 xv[MP][2];
+  auto load_w = [&](int b) {
+#pragma unroll
+    for (int c = 0; c < KC; ++c) w[c].load(codes, params, min(b + c, b1 - 1));  // (blocks past the range are not used)
+  };
+  // Eight channels a lane and token: step lane / 4 (of 32 channels), quarter lane % 4.
+  auto load_x = [&](int b) {
+#pragma unroll
+    for (int m = 0; m < MP; ++m) {
+      const float *xr = a.x + (long)min(m, a.M - 1) * a.K;
+      const int k = b * 128 + 8 * lane, end = min(a.K, b1 * 128);
+      xv[m][0] = load4(xr, k, end, a.vec);
+      xv[m][1] = load4(xr, k + 4, end, a.vec);
+    }
+  };
+  if (b0 < b1) {
+    load_x(b0);
+    load_w(b0);
+  }
   for (int b = b0; b < b1; b += KC) {
-    u32x4 w[KC][NT];
-    BlockParams<PT, GPB> p[KC][NT];
-#pragma unroll
-    for (int c = 0; c < KC; ++c)
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const long bb = min(b + c, b1 - 1);  // (a block past the range is not used)
-        w[c][t] = *reinterpret_cast<const u32x4 *>(codes[t] + bb * 1024);
-        p[c][t].load(params[t] + bb * PB);
-      }
-    // Four channels a lane and token: step lane / 8 (of 32 channels), quarter
-    // (lane / 2) % 4, half lane % 2 of its eight.
     float inv[MP];
 #pragma unroll
     for (int m = 0; m < MP; ++m) {
-      const int tok = min(m, a.M - 1);
-      const float4 v = load4(a.x + (long)tok * a.K, b * 128 + 4 * lane, min(a.K, b1 * 128), a.vec);
-      const float most = wave_max(fmaxf(fmaxf(finite_abs(v.x), finite_abs(v.y)), fmaxf(finite_abs(v.z), finite_abs(v.w))));
+      const float4 u = xv[m][0], v = xv[m][1];
+      const float most =
+          wave_max(fmaxf(fmaxf(fmaxf(finite_abs(u.x), finite_abs(u.y)), fmaxf(finite_abs(u.z), finite_abs(u.w))),
+                         fmaxf(fmaxf(finite_abs(v.x), finite_abs(v.y)), fmaxf(finite_abs(v.z), finite_abs(v.w)))));
       const unsigned sb = scale_bits(most);
       inv[m] = inverse_scale(sb);
-      half4v hi, lo;
-      split4(v, __uint_as_float(sb), &hi, &lo);
-      half4v *dst = reinterpret_cast<half4v *>(&xs[wave][((lane >> 3) * 2 * 4 + ((lane >> 1) & 3)) * MP + m]) + (lane & 1);
-      dst[0] = hi;
-      dst[4 * MP * 2] = lo;
+      half4v h[2], l[2];
+      split4(u, __uint_as_float(sb), &h[0], &l[0]);
+      split4(v, __uint_as_float(sb), &h[1], &l[1]);
+      half8 *dst = &xs[wave][((lane >> 2) * 2 * 4 + (lane & 3)) * MP + m];
+      dst[0] = __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7);
+      dst[4 * MP] = __builtin_shufflevector(l[0], l[1], 0, 1, 2, 3, 4, 5, 6, 7);
     }
+    const bool more = b + KC < b1;
+    if (more) load_x(b + KC);
     wave_lds_order();
 #pragma unroll
     for (int c = 0; c < KC; ++c) {
       if (b + c >= b1) break;
-      f32x4 sum[NT];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const half8 hi = xs[wave][((c * 4 + j) * 2 * 4 + quarter) * MP + row % MP];
-        const half8 lo = xs[wave][(((c * 4 + j) * 2 + 1) * 4 + quarter) * MP + row % MP];
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          const half8 wf = weights8(w[c][t][j], p[c][t].zero(j / SPG));
-          if (j % SPG == 0) sum[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
-          sum[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, wf, sum[t], 0, 0, 0);
-          sum[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, wf, sum[t], 0, 0, 0);
-          if (j % SPG == SPG - 1) {
-            const float s = p[c][t].scale(j / SPG);
-#pragma unroll
-            for (int m = 0; m < MP; ++m) acc[t][m] = fmaf(sum[t][m], s * inv[m], acc[t][m]);
-          }
-        }
-      }
+      auto frags = [&](int j, half8 *hi, half8 *lo) {
+        *hi = xs[wave][((c * 4 + j) * 2 * 4 + quarter) * MP + row % MP];
+        *lo = xs[wave][(((c * 4 + j) * 2 + 1) * 4 + quarter) * MP + row % MP];
+      };
+      block_products<PT, GPB, NT, MP>(w[c], base, frags, inv, acc);
+      if (more) w[c].load(codes, params, min(b + KC + c, b1 - 1));
     }
     wave_lds_order();
   }
@@ -321,41 +378,124 @@ __global__ __launch_bounds__(512) void q4_gemv_kernel(const Q4LinearArgs a) {
 
 // The pieces of every token's activations in the order of the A operand,
 // [row tile][32-deep step][piece][lane], and the inverse of its scale. One
-// workgroup a token (rows past the last are zeros).
-__global__ __launch_bounds__(256) void q4_pieces_kernel(const float *x, int M, int K, int steps, bool vec, half8 *pieces,
-                                                        float *inv) {
-  __shared__ float part[4];
+// workgroup of 1024 a token (rows past the last are zeros); rows of up to 8192
+// channels are read once.
+__global__ __launch_bounds__(1024) void q4_pieces_kernel(const float *x, int M, int K, int steps, bool vec, half8 *pieces,
+                                                         float *inv) {
+  __shared__ float part[16];
   const int m = blockIdx.x, tid = threadIdx.x;
   const float *row = x + (long)min(m, M - 1) * K;
-  float most = 0.0f;
-  for (int k = 4 * tid; k < K; k += 1024) {
-    const float4 v = load4(row, k, K, vec);
-    most = fmaxf(most, fmaxf(fmaxf(finite_abs(v.x), finite_abs(v.y)), fmaxf(finite_abs(v.z), finite_abs(v.w))));
-  }
+  float4 u = load4(row, 8 * tid, K, vec), v = load4(row, 8 * tid + 4, K, vec);
+  auto most_of = [](const float4 &a, const float4 &b) {
+    return fmaxf(fmaxf(fmaxf(finite_abs(a.x), finite_abs(a.y)), fmaxf(finite_abs(a.z), finite_abs(a.w))),
+                 fmaxf(fmaxf(finite_abs(b.x), finite_abs(b.y)), fmaxf(finite_abs(b.z), finite_abs(b.w))));
+  };
+  float most = most_of(u, v);
+  for (int k = 8 * (tid + 1024); k < K; k += 8192) most = fmaxf(most, most_of(load4(row, k, K, vec), load4(row, k + 4, K, vec)));
   most = wave_max(most);
   if ((tid & 63) == 0) part[tid >> 6] = most;
   __syncthreads();
-  most = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+  most = wave_max(part[tid & 15]);
   const unsigned sb = scale_bits(most);
   if (tid == 0) inv[m] = inverse_scale(sb);
-  half8 *dst = pieces + (long)(m >> 4) * steps * 128;
-  for (int u = tid; u < steps * 4; u += 256) {  // eight channels: step u / 4, quarter u % 4
-    half8 h{}, l{};
+  half8 *dst = pieces + (long)(m >> 4) * steps * 128 + (m & 15);
+  for (int i = tid; i < steps * 4; i += 1024) {  // eight channels: step i / 4, quarter i % 4
+    if (i != tid) {
+      u = load4(row, 8 * i, K, vec);
+      v = load4(row, 8 * i + 4, K, vec);
+    }
+    half4v h[2]{}, l[2]{};
     if (m < M) {
-      half4v h0, l0, h1, l1;
-      split4(load4(row, 8 * u, K, vec), __uint_as_float(sb), &h0, &l0);
-      split4(load4(row, 8 * u + 4, K, vec), __uint_as_float(sb), &h1, &l1);
+      split4(u, __uint_as_float(sb), &h[0], &l[0]);
+      split4(v, __uint_as_float(sb), &h[1], &l[1]);
+    }
+    half8 *at = dst + (long)(i >> 2) * 128 + (i & 3) * 16;
+    at[0] = __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7);
+    at[64] = __builtin_shufflevector(l[0], l[1], 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+}
+
+// 5 to 64 tokens, MT tiles of 16. A wave takes NT row tiles of the weight and all
+// tokens over a range of K blocks; the waves of a workgroup are wk ranges x runs of
+// tiles. Codes and pieces come straight from memory, a block of codes and a step
+// of pieces ahead. Bound: latency and the pieces' reads from L2 (each workgroup
+// reads all tokens), which NT tiles a wave share.
+template <int PT, int GPB, int MT, int NT>
+__global__ __launch_bounds__(512) void q4_few_kernel(const Q4LinearArgs a) {
+  constexpr int SPG = 4 / GPB;
+  extern __shared__ __attribute__((aligned(16))) float red[];  // [wave][MT * NT][4][64]
+  const unsigned base = base_1024();
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wk = wave % a.wk, wn = wave / a.wk;
+  const int row = lane & 15, quarter = lane >> 4;
+  const int runs = (int)(blockDim.x >> 6) / a.wk;
+  const long tile0 = ((long)blockIdx.x * runs + wn) * NT;
+  const int b0 = wk * a.blocks_per_wave, b1 = min(a.blocks, b0 + a.blocks_per_wave);
+  const char *codes[NT], *params[NT];
+  tile_addresses<PT, GPB, NT>(a, tile0, lane, codes, params);
+  const half8 *xp = reinterpret_cast<const half8 *>(a.pieces) + lane;
+  const long pitch = (long)a.blocks * 512;  // a token tile's pieces
+
+  f32x4 acc[MT][NT], sum[MT][NT];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        h[i] = h0[i];
-        h[4 + i] = h1[i];
-        l[i] = l0[i];
-        l[4 + i] = l1[i];
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int t = 0; t < NT; ++t) acc[i][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  BlockWeights<PT, GPB, NT> w[2];
+  half8 hi[2][MT], lo[2][MT];
+  auto load_x = [&](int step, int slot) {
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      hi[slot][i] = xp[i * pitch + (long)step * 128];
+      lo[slot][i] = xp[i * pitch + (long)step * 128 + 64];
+    }
+  };
+  if (b0 < b1) {
+    load_x(4 * b0, 0);
+    w[0].load(codes, params, b0);
+  }
+  for (int b = b0; b < b1; ++b) {
+    w[1].load(codes, params, min(b + 1, b1 - 1));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      load_x(min(4 * b + j + 1, 4 * b1 - 1), (j + 1) & 1);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const half8 wf = weights8(w[0].w[t][j], w[0].p[t].zero(j / SPG), base);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          if (j % SPG == 0) sum[i][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+          sum[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo[j & 1][i], wf, sum[i][t], 0, 0, 0);
+          sum[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi[j & 1][i], wf, sum[i][t], 0, 0, 0);
+        }
+        if (j % SPG == SPG - 1) {
+          const float s = w[0].p[t].scale(j / SPG);
+#pragma unroll
+          for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[i][t][e] = fmaf(sum[i][t][e], s, acc[i][t][e]);
+        }
       }
     }
-    half8 *at = dst + (long)(u >> 2) * 128 + (u & 3) * 16 + (m & 15);
-    at[0] = h;
-    at[64] = l;
+    w[0] = w[1];
+  }
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) red[((wave * MT * NT + i * NT + t) * 4 + e) * 64 + lane] = acc[i][t][e];
+  __syncthreads();
+  // The ranges' sums, in range order, over all threads.
+  for (int c = threadIdx.x; c < runs * MT * NT * 256; c += blockDim.x) {
+    const int l = c & 63, e = c >> 6 & 3, it = c >> 8;  // lane, element, (run, token tile, row tile)
+    const int t = it % NT, i = it / NT % MT, r = it / (NT * MT);
+    const long n = (((long)blockIdx.x * runs + r) * NT + t) * 16 + (l & 15);
+    const int m = i * 16 + 4 * (l >> 4) + e;
+    if (n >= a.N || m >= a.M) continue;
+    float v = 0.0f;
+    for (int q = 0; q < a.wk; ++q) v += red[(((r * a.wk + q) * MT * NT + i * NT + t) * 4 + e) * 64 + l];
+    a.out[(long)m * a.N + n] = fmaf(v, a.inv[m], a.bias ? a.bias[n] : 0.0f);
   }
 }
 
@@ -365,6 +505,7 @@ __global__ __launch_bounds__(256) void q4_pieces_kernel(const float *x, int M, i
 template <int PT, int GPB, int MT, int NT>
 __global__ __launch_bounds__(256) void q4_tile_kernel(const Q4LinearArgs a) {
   constexpr int SPG = 4 / GPB, PB = 16 * GPB * Q4Param<PT>::BYTES;
+  const unsigned base = base_1024();
   extern __shared__ __attribute__((aligned(16))) float red[];  // [wave][MT * NT][4][64]
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wk = wave % a.wk, wn = wave / a.wk, runs = 4 / a.wk;
@@ -407,7 +548,7 @@ __global__ __launch_bounds__(256) void q4_tile_kernel(const Q4LinearArgs a) {
       }
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        const half8 wf = weights8(w[t][j], p[t].zero(j / SPG));
+        const half8 wf = weights8(w[t][j], p[t].zero(j / SPG), base);
         const float s = p[t].scale(j / SPG);
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
@@ -460,26 +601,32 @@ template <int PT, int GPB>
 hipError_t run(hipStream_t st, Q4LinearArgs a) {
   if (a.M <= 4) {
     // Waves of a workgroup share K while tiles are few.
-    const int rounds = (a.blocks + 1) / 2;
+    const int rounds = (a.blocks + 3) / 4;
     a.wk = 1;
     while (a.wk < 8 && a.wk < rounds && (long)a.tiles * a.wk < 2048) a.wk *= 2;
-    a.blocks_per_wave = ((rounds + a.wk - 1) / a.wk) * 2;
+    a.blocks_per_wave = ((rounds + a.wk - 1) / a.wk) * 4;
     const int waves = std::max(4, a.wk), runs = waves / a.wk;
     const dim3 grid((unsigned)((a.tiles + runs - 1) / runs));
     if (a.M == 1) hipLaunchKernelGGL((q4_gemv_kernel<PT, GPB, 1, 1>), grid, dim3(waves * 64), 0, st, a);
     else hipLaunchKernelGGL((q4_gemv_kernel<PT, GPB, 4, 1>), grid, dim3(waves * 64), 0, st, a);
     return hipGetLastError();
   }
-  hipLaunchKernelGGL(q4_pieces_kernel, dim3((unsigned)(a.mtiles * 16)), dim3(256), 0, st, a.x, a.M, a.K, a.blocks * 4, a.vec,
+  hipLaunchKernelGGL(q4_pieces_kernel, dim3((unsigned)(a.mtiles * 16)), dim3(1024), 0, st, a.x, a.M, a.K, a.blocks * 4, a.vec,
                      (half8 *)a.pieces, (float *)a.inv);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  if (a.M <= 32) {
-    a.wk = std::min(4, a.blocks >= 4 ? 4 : a.blocks >= 2 ? 2 : 1);
+  if (a.M <= 64) {
+    const int mt = a.mtiles == 3 ? 4 : a.mtiles, nt = 2;
+    const int groups = (a.tiles + nt - 1) / nt;
+    a.wk = 1;
+    while (a.wk < 8 && 2 * a.wk <= a.blocks && (long)groups * a.wk < 2048) a.wk *= 2;
     a.blocks_per_wave = (a.blocks + a.wk - 1) / a.wk;
-    const int runs = 4 / a.wk;
-    const dim3 grid((unsigned)((a.tiles + runs - 1) / runs), (unsigned)a.mtiles);
-    hipLaunchKernelGGL((q4_tile_kernel<PT, GPB, 1, 1>), grid, dim3(256), 4 * 4 * 64 * 4, st, a);
+    const int waves = 8, runs = waves / a.wk;
+    const dim3 grid((unsigned)((groups + runs - 1) / runs));
+    const unsigned lds = waves * mt * nt * 1024;
+    if (mt == 1) hipLaunchKernelGGL((q4_few_kernel<PT, GPB, 1, 2>), grid, dim3(512), lds, st, a);
+    else if (mt == 2) hipLaunchKernelGGL((q4_few_kernel<PT, GPB, 2, 2>), grid, dim3(512), lds, st, a);
+    else hipLaunchKernelGGL((q4_few_kernel<PT, GPB, 4, 2>), grid, dim3(512), lds, st, a);
   } else {
     a.wk = 1;
     a.blocks_per_wave = a.blocks;
@@ -509,16 +656,19 @@ hipError_t launch_q4_pack(hipStream_t st, const Q4PackArgs &a) {
   return hipGetLastError();
 }
 
+// Token tiles of the workspace: whole kernels' worth up to 64 tokens.
+static size_t q4_token_tiles(long M) { return M > 32 && M <= 48 ? 4 : (size_t)(M + 15) / 16; }
+
 // Bytes of the activations' pieces and inverse scales that M tokens need (0: none).
 size_t q4_linear_workspace(long M, long blocks) {
   if (M <= 4) return 0;
-  const size_t mt = (size_t)(M + 15) / 16;
+  const size_t mt = q4_token_tiles(M);
   return mt * blocks * 8192 + mt * 16 * sizeof(float);
 }
 
 hipError_t launch_q4_linear(hipStream_t st, const Q4LinearArgs &base, int group, int param_type, void *workspace) {
   Q4LinearArgs a = base;
-  a.mtiles = (a.M + 15) / 16;
+  a.mtiles = (int)q4_token_tiles(a.M);
   a.vec = a.K % 4 == 0 && (reinterpret_cast<uintptr_t>(a.x) & 15) == 0;
   a.pieces = workspace;
   a.inv = reinterpret_cast<const float *>(static_cast<char *>(workspace) + (size_t)a.mtiles * a.blocks * 8192);
