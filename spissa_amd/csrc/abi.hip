@@ -2354,7 +2354,7 @@ static int linear_run_q4(spissa_session *s, const spissa_linear_weight *w, const
   a.tiles = w->tiles;
   a.blocks = w->blocks;
   HIP_TRY(hipSetDevice(s->device));
-  const size_t need = q4_linear_workspace(a.M, a.blocks);
+  const size_t need = q4_linear_workspace(a.M, a.N, a.tiles, a.blocks, w->pack_group);
   std::unique_lock<std::mutex> lock(s->lin_mutex, std::defer_lock);
   if (need) {
     lock.lock();

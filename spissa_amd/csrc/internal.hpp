@@ -299,10 +299,11 @@ struct Q4LinearArgs {
   // set by the launcher
   const void *pieces;
   const float *inv;
-  int mtiles, wk, blocks_per_wave;
+  float *partial;
+  int mtiles, mblocks, splits, wk, blocks_per_wave;
   bool vec;
 };
-size_t q4_linear_workspace(long M, long blocks);
+size_t q4_linear_workspace(long M, long N, long tiles, long blocks, int pack_group);
 hipError_t launch_q4_linear(hipStream_t st, const Q4LinearArgs &a, int group, int param_type, void *workspace);
 
 // Greedy token choice: one partial per contiguous range of the logits.

@@ -68,6 +68,10 @@ struct BlockParams {
       w[0] = *reinterpret_cast<const unsigned *>(p);
     }
   }
+  __device__ __forceinline__ void here() {
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) asm volatile("" : "+v"(w[i]));
+  }
   __device__ __forceinline__ float scale(int g) const {
     if constexpr (PT == 0)
       return (float)__builtin_bit_cast(_Float16, (unsigned short)(w[g / 2] >> (16 * (g & 1))));
@@ -109,6 +113,14 @@ __device__ __forceinline__ half8 weights8(unsigned w, half2v zero, unsigned base
     r[2 * i + 1] = p.y;
   }
   return r;
+}
+
+// Copies 16 bytes a lane from base + off into LDS at lds_base + 16 * lane, unknown
+// to the compiler, which would wait for it before any later LDS read: the kernel's
+// barrier waits for the copies that the next step reads.
+__device__ __forceinline__ void copy16(const char *base, unsigned off, char *lds_base) {
+  const unsigned lds = (unsigned)(uintptr_t)(__attribute__((address_space(3))) void *)lds_base;
+  asm volatile("global_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "{m0}"(lds) : "memory");
 }
 
 // Power of two that takes a largest |activation| to 2^13..2^14 (as float bits),
@@ -231,6 +243,13 @@ struct BlockWeights {
       p[t].load(params[t] + block * (16 * GPB * Q4Param<PT>::BYTES));
     }
   }
+  __device__ __forceinline__ void here() {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      asm volatile("" : "+v"(w[t]));
+      p[t].here();
+    }
+  }
 };
 
 // acc += the block's products with the A fragments hi, lo (rows 4 (lane / 16) + 0..3
@@ -281,10 +300,11 @@ __device__ __forceinline__ void tile_addresses(const Q4LinearArgs &a, long tile0
 // The codes and activations of the next 512 channels are in flight meanwhile.
 // Bound: HBM for large weights (the codes), latency for small ones.
 template <int PT, int GPB, int MP, int NT>
-__global__ __launch_bounds__(512) void q4_gemv_kernel(const Q4LinearArgs a) {
+__global__ __launch_bounds__(MP == 1 ? 1024 : 512) void q4_gemv_kernel(const Q4LinearArgs a) {
   constexpr int KC = 4;  // blocks of a round
-  __shared__ __attribute__((aligned(16))) half8 xs[8][KC * 4 * 2 * 4 * MP];  // [wave][step][piece][quarter][token]
-  __shared__ float red[8][NT * 16][MP];
+  constexpr int WAVES = MP == 1 ? 16 : 8;
+  __shared__ __attribute__((aligned(16))) half8 xs[WAVES][KC * 4 * 2 * 4 * MP];  // [wave][step][piece][quarter][token]
+  __shared__ float red[WAVES][NT * 16][MP];
   const unsigned base = base_1024();
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wk = wave % a.wk, wn = wave / a.wk;
@@ -378,29 +398,34 @@ __global__ __launch_bounds__(512) void q4_gemv_kernel(const Q4LinearArgs a) {
 
 // The pieces of every token's activations in the order of the A operand,
 // [row tile][32-deep step][piece][lane], and the inverse of its scale. One
-// workgroup of 1024 a token (rows past the last are zeros); rows of up to 8192
-// channels are read once.
+// workgroup of 1024 for T tokens (rows past the last are zeros), T neighbours of a
+// row tile a 16 T byte store; the first 8192 / T channels of a row are read once.
+template <int T>
 __global__ __launch_bounds__(1024) void q4_pieces_kernel(const float *x, int M, int K, int steps, bool vec, half8 *pieces,
                                                          float *inv) {
-  __shared__ float part[16];
-  const int m = blockIdx.x, tid = threadIdx.x;
+  __shared__ float part[16][T];
+  const int tid = threadIdx.x, r = tid % T, unit = tid / T, m = blockIdx.x * T + r;
   const float *row = x + (long)min(m, M - 1) * K;
-  float4 u = load4(row, 8 * tid, K, vec), v = load4(row, 8 * tid + 4, K, vec);
+  float4 u = load4(row, 8 * unit, K, vec), v = load4(row, 8 * unit + 4, K, vec);
   auto most_of = [](const float4 &a, const float4 &b) {
     return fmaxf(fmaxf(fmaxf(finite_abs(a.x), finite_abs(a.y)), fmaxf(finite_abs(a.z), finite_abs(a.w))),
                  fmaxf(fmaxf(finite_abs(b.x), finite_abs(b.y)), fmaxf(finite_abs(b.z), finite_abs(b.w))));
   };
   float most = most_of(u, v);
-  for (int k = 8 * (tid + 1024); k < K; k += 8192) most = fmaxf(most, most_of(load4(row, k, K, vec), load4(row, k + 4, K, vec)));
-  most = wave_max(most);
-  if ((tid & 63) == 0) part[tid >> 6] = most;
+  for (int k = 8 * (unit + 1024 / T); k < K; k += 8192 / T)
+    most = fmaxf(most, most_of(load4(row, k, K, vec), load4(row, k + 4, K, vec)));
+#pragma unroll
+  for (int d = T; d < 64; d *= 2) most = fmaxf(most, __shfl_xor(most, d));
+  if ((tid & 63) < T) part[tid >> 6][r] = most;
   __syncthreads();
-  most = wave_max(part[tid & 15]);
+  most = part[0][r];
+#pragma unroll
+  for (int w = 1; w < 16; ++w) most = fmaxf(most, part[w][r]);
   const unsigned sb = scale_bits(most);
-  if (tid == 0) inv[m] = inverse_scale(sb);
+  if (unit == 0) inv[m] = inverse_scale(sb);
   half8 *dst = pieces + (long)(m >> 4) * steps * 128 + (m & 15);
-  for (int i = tid; i < steps * 4; i += 1024) {  // eight channels: step i / 4, quarter i % 4
-    if (i != tid) {
+  for (int i = unit; i < steps * 4; i += 1024 / T) {  // eight channels: step i / 4, quarter i % 4
+    if (i != unit) {
       u = load4(row, 8 * i, K, vec);
       v = load4(row, 8 * i + 4, K, vec);
     }
@@ -499,111 +524,215 @@ __global__ __launch_bounds__(512) void q4_few_kernel(const Q4LinearArgs a) {
   }
 }
 
-// More tokens: a wave takes MT x NT tiles of 16 x 16 outputs over a range of K
-// blocks (the waves of a workgroup: wk ranges x wn runs of row tiles of the
-// weight), both operands straight from memory.
+// More tokens: tiles of 32 MT tokens x 64 NT rows of the weight, eight waves (2 x 4)
+// of MT x NT products of 16 x 16 each, on one of `splits` ranges of K. The pieces
+// of a 128-channel block come straight into LDS (two buffers, the next block's in
+// flight), in the order in which they are read; codes go to the registers of the
+// wave that widens them, a block ahead. One barrier a block. Groups under 128 take
+// NT = 2 with MT = 4: their scales and zeros would not fit the registers.
+// Bound: the matrix cores (two instructions a product) beside the widening, which
+// a wave does for 16 NT rows and uses MT times, and a scaling FMA an output and group.
+// 2048 tokens x 4096 x 4096: 122 us, 1.13 PFLOP/s of binary16 products (a library
+// product of binary16 matrices of that size runs at 1.18); 512 tokens 54 us with
+// the pieces.
 template <int PT, int GPB, int MT, int NT>
-__global__ __launch_bounds__(256) void q4_tile_kernel(const Q4LinearArgs a) {
-  constexpr int SPG = 4 / GPB, PB = 16 * GPB * Q4Param<PT>::BYTES;
+__global__ __launch_bounds__(512, 2) void q4_tile_kernel(const Q4LinearArgs a) {
+  constexpr int SPG = 4 / GPB, TILE = 2 * MT * 8192;  // bytes of a block's pieces
+  __shared__ __attribute__((aligned(16))) char x_lds[2][TILE];
   const unsigned base = base_1024();
-  extern __shared__ __attribute__((aligned(16))) float red[];  // [wave][MT * NT][4][64]
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wk = wave % a.wk, wn = wave / a.wk, runs = 4 / a.wk;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int row = lane & 15, quarter = lane >> 4;
-  const long tile0 = ((long)blockIdx.x * runs + wn) * NT;
-  const int mt0 = blockIdx.y * MT;
-  const int b0 = wk * a.blocks_per_wave, b1 = min(a.blocks, b0 + a.blocks_per_wave);
-  const char *codes[NT], *params[NT];
-#pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    const long tile = min(tile0 + t, (long)a.tiles - 1);
-    codes[t] = reinterpret_cast<const char *>(a.codes) + tile * a.blocks * 1024 + lane * 16;
-    params[t] = reinterpret_cast<const char *>(a.params) + (tile * a.blocks * 16 + row) * (GPB * Q4Param<PT>::BYTES);
+  // Ids equal modulo 8 run on one XCD: each takes a contiguous run of the order,
+  // in which the tiles of the same tokens are neighbours.
+  int id = blockIdx.x;
+  {
+    const int g = gridDim.x, q = g >> 3, r = g & 7, xcd = id & 7;
+    id = xcd * q + min(xcd, r) + (id >> 3);
   }
-  const half8 *xp[MT];
+  const int nblocks = (a.tiles + 4 * NT - 1) / (4 * NT);
+  const int nb = id % nblocks, mb = id / nblocks % a.mblocks, split = id / nblocks / a.mblocks;
+  const int wm = wave >> 2, wn = wave & 3;
+  const long tile0 = (long)nb * (4 * NT) + wn * NT;
+  const int b0 = split * a.blocks_per_wave, b1 = min(a.blocks, b0 + a.blocks_per_wave);
+  const char *codes[NT], *params[NT];
+  tile_addresses<PT, GPB, NT>(a, tile0, lane, codes, params);
+
+  // 1 KB a wave and copy: 8 of a token tile's block, MT / 2 token tiles of a wave.
+  // (Token tiles past the last are read as the last and not stored.)
+  // Copies and codes are issued a few at a time: a burst would hold the waves up.
+  auto fetch = [&](int b, int part, int parts) {
+    const int buf = b & 1;
 #pragma unroll
-  for (int i = 0; i < MT; ++i)
-    xp[i] = reinterpret_cast<const half8 *>(a.pieces) + (long)min(mt0 + i, a.mtiles - 1) * a.blocks * 512 + lane;
-  f32x4 acc[MT][NT];
+    for (int i = 2 * MT * part / parts; i < 2 * MT * (part + 1) / parts; ++i) {
+      const int t = min(mb * 2 * MT + i, a.mtiles - 1);
+      const char *src = reinterpret_cast<const char *>(a.pieces) + ((long)t * a.blocks + b) * 8192 + wave * 1024;
+      copy16(src, lane * 16, x_lds[buf] + i * 8192 + wave * 1024);
+    }
+  };
+  f32x4 acc[MT][NT], sum[MT][NT];
 #pragma unroll
   for (int i = 0; i < MT; ++i)
 #pragma unroll
     for (int t = 0; t < NT; ++t) acc[i][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
-  for (int b = b0; b < b1; ++b) {
-    u32x4 w[NT];
-    BlockParams<PT, GPB> p[NT];
+  BlockWeights<PT, GPB, NT> w, next;
+  half8 hi[MT], lo[MT], wf[NT];
+  auto read = [&](int buf, int at, half8 (&to)[MT]) {
+    const half8 *const xl = reinterpret_cast<const half8 *>(x_lds[buf] + wm * MT * 8192) + lane;
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      w[t] = *reinterpret_cast<const u32x4 *>(codes[t] + (long)b * 1024);
-      p[t].load(params[t] + (long)b * PB);
-    }
-    f32x4 sum[MT][NT];
+    for (int i = 0; i < MT; ++i) to[i] = xl[i * 512 + at * 64];
+  };
+  fetch(b0, 0, 1);
+  w.load(codes, params, b0);
+  asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+  if (b0 + 1 < b1) {
+    fetch(b0 + 1, 0, 4);
+    next.load(codes, params, b0 + 1);
+  }
+  read(b0 & 1, 1, lo);
+#pragma unroll
+  for (int t = 0; t < NT; ++t) wf[t] = weights8(w.w[t][0], w.p[t].zero(0), base);
+  // Beside a tile's matrix instructions stand the vector ones of the tile before:
+  // its scaling, and its weights of the next 32 channels.
+  for (int b = b0; b < b1; ++b) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      half8 hi[MT], lo[MT];
-#pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        hi[i] = xp[i][(b * 4 + j) * 128];
-        lo[i] = xp[i][(b * 4 + j) * 128 + 64];
-      }
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const half8 wf = weights8(w[t][j], p[t].zero(j / SPG), base);
-        const float s = p[t].scale(j / SPG);
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          if (j % SPG == 0) sum[i][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
-          sum[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi[i], wf, sum[i][t], 0, 0, 0);
-          sum[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo[i], wf, sum[i][t], 0, 0, 0);
-          if (j % SPG == SPG - 1) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[i][t][e] = fmaf(sum[i][t][e], s, acc[i][t][e]);
-          }
-        }
-      }
-    }
-  }
-  if (a.wk > 1) {
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
+      read(b & 1, 2 * j, hi);
+      if (j < 2 && b + 1 < b1) fetch(b + 1, 2 * j + 1, 4);
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) red[((wave * MT * NT + i * NT + t) * 4 + e) * 64 + lane] = acc[i][t][e];
-    __syncthreads();
-    if (wk != 0) return;
-    for (int q = 1; q < a.wk; ++q)
+        for (int i = 0; i < MT; ++i) {
+          if (j % SPG == 0) sum[i][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+          sum[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo[i], wf[t], sum[i][t], 0, 0, 0);
+        }
+      __builtin_amdgcn_sched_barrier(0);
+      if (j < 3) {
+        read(b & 1, 2 * j + 3, lo);
+        if (j == 0 && b + 1 < b1) fetch(b + 1, 2, 4);
+        if (j == 1 && b > b0 && b + 1 < b1) next.load(codes, params, b + 1);
+      } else {
+        // This block's pieces are all in registers, the next block's in LDS.
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        next.here();  // (the compiler would wait at their first use, for the copies below too)
+        if (b + 2 < b1) fetch(b + 2, 0, 4);
+        if (b + 1 < b1) read((b + 1) & 1, 1, lo);
+      }
 #pragma unroll
-      for (int i = 0; i < MT; ++i)
+      for (int t = 0; t <= NT; ++t) {
+        if (t < NT)
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
+          for (int i = 0; i < MT; ++i)
+            sum[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi[i], wf[t], sum[i][t], 0, 0, 0);
+        if (t > 0) {
+          if (j % SPG == SPG - 1) {
+            const float s = w.p[t - 1].scale(j / SPG);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc[i][t][e] += red[(((wave + q) * MT * NT + i * NT + t) * 4 + e) * 64 + lane];
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) acc[i][t - 1][e] = fmaf(sum[i][t - 1][e], s, acc[i][t - 1][e]);
+          }
+          wf[t - 1] = j < 3 ? weights8(w.w[t - 1][j < 3 ? j + 1 : 0], w.p[t - 1].zero((j < 3 ? j + 1 : 0) / SPG), base)
+                            : weights8(next.w[t - 1][0], next.p[t - 1].zero(0), base);
+        }
+        if (t > 0 && t < NT)
+#pragma unroll
+          for (int i = 0; i < MT; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x002, 6, 0);
+          }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    w = next;
   }
+  const bool part = a.splits > 1;
+  float *const out = part ? a.partial + (long)split * a.M * a.N : a.out;
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     const long n = (tile0 + t) * 16 + row;
     if (n >= a.N) continue;
-    const float bias = a.bias ? a.bias[n] : 0.0f;
+    const float bias = a.bias && !part ? a.bias[n] : 0.0f;
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const long m = (long)(mt0 + i) * 16 + 4 * quarter + e;
-        if (m < a.M) a.out[m * a.N + n] = fmaf(acc[i][t][e], a.inv[m], bias);
+        const long m = (long)(mb * 2 * MT + wm * MT + i) * 16 + 4 * quarter + e;
+        if (m < a.M) out[m * a.N + n] = part ? acc[i][t][e] : fmaf(acc[i][t][e], a.inv[m], bias);
       }
   }
 }
 
+// out = (the ranges' partial sums, in range order) / the token's scale + bias.
+__global__ __launch_bounds__(256) void q4_reduce_kernel(const Q4LinearArgs a) {
+  const long n = (long)blockIdx.x * 256 + threadIdx.x, m = blockIdx.y, stride = (long)a.M * a.N;
+  if (n >= a.N) return;
+  const float *p = a.partial + m * a.N + n;
+  float v = 0.0f;
+  for (int s = 0; s < a.splits; ++s) v += p[s * stride];
+  a.out[m * a.N + n] = fmaf(v, a.inv[m], a.bias ? a.bias[n] : 0.0f);
+}
+
 namespace {
+
+template <int PT, int GPB, int MT, int NT>
+hipError_t few_n(hipStream_t st, Q4LinearArgs a) {
+  const int groups = (a.tiles + NT - 1) / NT;
+  a.wk = 1;
+  while (a.wk < 8 && 2 * a.wk <= a.blocks && (long)groups * a.wk < 2048) a.wk *= 2;
+  a.blocks_per_wave = (a.blocks + a.wk - 1) / a.wk;
+  const int runs = 8 / a.wk;
+  const dim3 grid((unsigned)((groups + runs - 1) / runs));
+  hipLaunchKernelGGL((q4_few_kernel<PT, GPB, MT, NT>), grid, dim3(512), 8 * MT * NT * 1024, st, a);
+  return hipGetLastError();
+}
+template <int PT, int GPB, int MT>
+hipError_t few(hipStream_t st, const Q4LinearArgs &a) {
+  // (One row tile a wave while that leaves a CU without a workgroup: 16 tokens,
+  // 4096 x 4096 9.4 us against 11.4 with two; 8192 x 4096 15.3 against 13.6; 64
+  // tokens 14336 x 4096 52 against 35.)
+  return a.tiles < 2 * 256 ? few_n<PT, GPB, MT, 1>(st, a) : few_n<PT, GPB, MT, 2>(st, a);
+}
+
+template <int PT, int GPB, int MT, int NT>
+hipError_t tile(hipStream_t st, Q4LinearArgs a) {
+  a.mblocks = (a.mtiles + 2 * MT - 1) / (2 * MT);
+  const long grid = (long)a.mblocks * ((a.tiles + 4 * NT - 1) / (4 * NT)) * a.splits;
+  hipLaunchKernelGGL((q4_tile_kernel<PT, GPB, MT, NT>), dim3((unsigned)grid), dim3(512), 0, st, a);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || a.splits == 1) return e;
+  hipLaunchKernelGGL(q4_reduce_kernel, dim3((unsigned)((a.N + 255) / 256), (unsigned)a.M), dim3(256), 0, st, a);
+  return hipGetLastError();
+}
+
+// Tile shape and ranges of K of a projection of more than 64 tokens; the larger
+// shape is 128 tokens x big_tiles row tiles. It wins once it fills three quarters
+// of the CUs (4096 x 4096, groups of 128: 2048 tokens 138 us against 156, 1536
+// level at 120, 1024 114 against 86); below, 64 x 8 row tiles, over ranges of K
+// while a CU stays without a workgroup (256 tokens: 49 us with one range, 39 with
+// two; 512 tokens: 54 and 57).
+struct Q4TilePlan {
+  bool big;
+  int splits;
+};
+Q4TilePlan q4_tile_plan(long M, long tiles, long blocks, int big_tiles) {
+  Q4TilePlan p{};
+  const long big = ((M + 127) / 128) * ((tiles + big_tiles - 1) / big_tiles), small = ((M + 63) / 64) * ((tiles + 7) / 8);
+  p.big = big >= 192;
+  p.splits = p.big ? 1 : (int)std::max<long>(1, std::min(256 / small, blocks / 4));
+  while ((p.splits - 1) * ((blocks + p.splits - 1) / p.splits) >= blocks) --p.splits;  // (no range empty)
+  return p;
+}
 
 template <int PT, int GPB>
 hipError_t run(hipStream_t st, Q4LinearArgs a) {
   if (a.M <= 4) {
-    // Waves of a workgroup share K while tiles are few.
+    // Waves of a workgroup share K while tiles are few. (One token: 2048 x 8192
+    // 6.2 us with up to 16 waves, 8.7 with 8. Four tokens' activations take the
+    // LDS of 8.)
     const int rounds = (a.blocks + 3) / 4;
     a.wk = 1;
-    while (a.wk < 8 && a.wk < rounds && (long)a.tiles * a.wk < 2048) a.wk *= 2;
+    const int most = a.M == 1 ? 16 : 8;
+    while (a.wk < most && a.wk < rounds && (long)a.tiles * a.wk < 2048) a.wk *= 2;
     a.blocks_per_wave = ((rounds + a.wk - 1) / a.wk) * 4;
     const int waves = std::max(4, a.wk), runs = waves / a.wk;
     const dim3 grid((unsigned)((a.tiles + runs - 1) / runs));
@@ -611,29 +740,23 @@ hipError_t run(hipStream_t st, Q4LinearArgs a) {
     else hipLaunchKernelGGL((q4_gemv_kernel<PT, GPB, 4, 1>), grid, dim3(waves * 64), 0, st, a);
     return hipGetLastError();
   }
-  hipLaunchKernelGGL(q4_pieces_kernel, dim3((unsigned)(a.mtiles * 16)), dim3(1024), 0, st, a.x, a.M, a.K, a.blocks * 4, a.vec,
-                     (half8 *)a.pieces, (float *)a.inv);
+  // (2048 tokens x 4096: 8 a workgroup 15.5 us, 1 a workgroup 30; few tokens want the
+  // workgroups.)
+  const dim3 rows((unsigned)(a.mtiles * (a.M > 64 ? 2 : 16)));
+  auto pieces = a.M > 64 ? q4_pieces_kernel<8> : q4_pieces_kernel<1>;
+  hipLaunchKernelGGL(pieces, rows, dim3(1024), 0, st, a.x, a.M, a.K, a.blocks * 4, a.vec, (half8 *)a.pieces, (float *)a.inv);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   if (a.M <= 64) {
-    const int mt = a.mtiles == 3 ? 4 : a.mtiles, nt = 2;
-    const int groups = (a.tiles + nt - 1) / nt;
-    a.wk = 1;
-    while (a.wk < 8 && 2 * a.wk <= a.blocks && (long)groups * a.wk < 2048) a.wk *= 2;
-    a.blocks_per_wave = (a.blocks + a.wk - 1) / a.wk;
-    const int waves = 8, runs = waves / a.wk;
-    const dim3 grid((unsigned)((groups + runs - 1) / runs));
-    const unsigned lds = waves * mt * nt * 1024;
-    if (mt == 1) hipLaunchKernelGGL((q4_few_kernel<PT, GPB, 1, 2>), grid, dim3(512), lds, st, a);
-    else if (mt == 2) hipLaunchKernelGGL((q4_few_kernel<PT, GPB, 2, 2>), grid, dim3(512), lds, st, a);
-    else hipLaunchKernelGGL((q4_few_kernel<PT, GPB, 4, 2>), grid, dim3(512), lds, st, a);
+    if (a.mtiles == 1) return few<PT, GPB, 1>(st, a);
+    if (a.mtiles == 2) return few<PT, GPB, 2>(st, a);
+    return few<PT, GPB, 4>(st, a);
   } else {
-    a.wk = 1;
-    a.blocks_per_wave = a.blocks;
-    const dim3 grid((unsigned)((a.tiles + 15) / 16), (unsigned)((a.mtiles + 3) / 4));
-    hipLaunchKernelGGL((q4_tile_kernel<PT, GPB, 4, 4>), grid, dim3(256), 0, st, a);
+    const Q4TilePlan p = q4_tile_plan(a.M, a.tiles, a.blocks, GPB == 1 ? 16 : 8);
+    a.splits = p.splits;
+    a.blocks_per_wave = (a.blocks + p.splits - 1) / p.splits;
+    return p.big ? tile<PT, GPB, 4, GPB == 1 ? 4 : 2>(st, a) : tile<PT, GPB, 2, 2>(st, a);
   }
-  return hipGetLastError();
 }
 
 template <int PT>
@@ -659,11 +782,12 @@ hipError_t launch_q4_pack(hipStream_t st, const Q4PackArgs &a) {
 // Token tiles of the workspace: whole kernels' worth up to 64 tokens.
 static size_t q4_token_tiles(long M) { return M > 32 && M <= 48 ? 4 : (size_t)(M + 15) / 16; }
 
-// Bytes of the activations' pieces and inverse scales that M tokens need (0: none).
-size_t q4_linear_workspace(long M, long blocks) {
+// The workspace: pieces, inverse scales, and the partial sums of split K (0 bytes: none).
+size_t q4_linear_workspace(long M, long N, long tiles, long blocks, int pack_group) {
   if (M <= 4) return 0;
   const size_t mt = q4_token_tiles(M);
-  return mt * blocks * 8192 + mt * 16 * sizeof(float);
+  const int splits = M <= 64 ? 1 : q4_tile_plan(M, tiles, blocks, pack_group == 128 ? 16 : 8).splits;
+  return mt * blocks * 8192 + mt * 16 * sizeof(float) + (splits > 1 ? (size_t)splits * M * N * sizeof(float) : 0);
 }
 
 hipError_t launch_q4_linear(hipStream_t st, const Q4LinearArgs &base, int group, int param_type, void *workspace) {
@@ -672,6 +796,7 @@ hipError_t launch_q4_linear(hipStream_t st, const Q4LinearArgs &base, int group,
   a.vec = a.K % 4 == 0 && (reinterpret_cast<uintptr_t>(a.x) & 15) == 0;
   a.pieces = workspace;
   a.inv = reinterpret_cast<const float *>(static_cast<char *>(workspace) + (size_t)a.mtiles * a.blocks * 8192);
+  a.partial = const_cast<float *>(a.inv) + a.mtiles * 16;
   switch (param_type) {
     case 0: return run_g<0>(st, a, group);
     case 1: return run_g<1>(st, a, group);

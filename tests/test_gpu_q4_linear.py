@@ -125,6 +125,16 @@ def test_large(ses, m, n, k):
     check(ses, wt, acts(rng, m, k), rng.standard_normal(n).astype(np.float32))
 
 
+@pytest.mark.parametrize("scale,zeros,group", [("f16", False, 128), ("f16", True, 64), ("f32", True, 32), ("bf16", False, 128),
+                                               ("f32", False, 128), ("f16", False, 32), ("bf16", True, 64)])
+@pytest.mark.parametrize("k", [1, 130, 257, 700])
+def test_many_tokens_and_many_rows(ses, scale, zeros, group, k):
+    """The tiles of many tokens, their last ones ragged, over one block of K and more."""
+    rng = np.random.default_rng(k + group)
+    wt = Weight(rng, 4100, k, group, scale, zeros)
+    check(ses, wt, acts(rng, 1545, k), rng.standard_normal(4100).astype(np.float32), what=f"{scale} zeros {zeros}")
+
+
 @pytest.mark.parametrize("m", [1, 4, 5, 40])
 def test_activations_of_every_size(ses, m):
     """Outliers, a row of zeros, rows at the ends of the f32 range."""
