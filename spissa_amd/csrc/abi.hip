@@ -1492,7 +1492,7 @@ static int q4_attend_batch(spissa_session *s, const float *q, const spissa_kv_ca
     a.kps = p.kps;
     a.max_splits = p.splits;
     a.qscale = (1.0f / sqrtf((float)D)) * 1.4426950408889634f;
-    HIP_TRY(launch_q4_attend(s->stream, a, D, p.RB, B));
+    HIP_TRY(launch_q4_attend(s->stream, a, D, B));
   }
   return SPISSA_OK;
 }

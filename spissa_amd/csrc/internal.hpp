@@ -382,7 +382,7 @@ struct Q4AttnPlan {
 };
 // keys[i]: visible keys of the n sequences of a launch.
 Q4AttnPlan q4_attend_plan(int D, int R, int Hkv, const int *keys, int n);
-hipError_t launch_q4_attend(hipStream_t st, const Q4AttnArgs &a, int D, int RB, int nz);
+hipError_t launch_q4_attend(hipStream_t st, const Q4AttnArgs &a, int D, int nz);
 bool q4_supported(size_t D);
 
 // Attention of the queries of a cache's last S rows (q4_chunk.hip).

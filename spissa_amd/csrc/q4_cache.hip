@@ -31,6 +31,91 @@ __device__ __forceinline__ unsigned half_bits(float v) {
   return __builtin_bit_cast(unsigned short, (_Float16)v);
 }
 
+typedef __attribute__((ext_vector_type(8))) _Float16 half8;
+typedef __attribute__((ext_vector_type(2))) _Float16 half2v;
+typedef __attribute__((ext_vector_type(4))) float f32x4;
+
+// Truncation, two at a time: the second piece takes what the first leaves.
+__device__ __forceinline__ half2v pieces2(float a, float b) {
+  return __builtin_bit_cast(half2v, __builtin_amdgcn_cvt_pkrtz(a, b));
+}
+// (minus_one: -1 as the compiler does not know it, so that the difference is one
+// mixed-precision FMA and not a conversion and a subtraction)
+__device__ __forceinline__ void split8(const float (&v)[8], float minus_one, half8 *hi, half8 *lo) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const half2v h = pieces2(v[2 * i], v[2 * i + 1]);
+    const half2v l = pieces2(fmaf((float)h.x, minus_one, v[2 * i]), fmaf((float)h.y, minus_one, v[2 * i + 1]));
+    (*hi)[2 * i] = h.x;
+    (*hi)[2 * i + 1] = h.y;
+    (*lo)[2 * i] = l.x;
+    (*lo)[2 * i + 1] = l.y;
+  }
+}
+// Power of two that takes `most` to 2^top..2^(top + 1), as float bits.
+__device__ __forceinline__ unsigned scale_to(float most, unsigned top) {
+  return min(254u + top - (__float_as_uint(most) >> 23), 253u) << 23;
+}
+__device__ __forceinline__ float inverse_scale(unsigned bits) { return __uint_as_float((254u << 23) - bits); }
+
+template <int N>
+__device__ __forceinline__ void words(const char *p, unsigned (&w)[N]) {
+  if constexpr (N == 1) {
+    w[0] = *reinterpret_cast<const unsigned *>(p);
+  } else if constexpr (N == 2) {
+    const uint2 v = *reinterpret_cast<const uint2 *>(p);
+    w[0] = v.x;
+    w[1] = v.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+      const uint4 v = reinterpret_cast<const uint4 *>(p)[i];
+      w[4 * i] = v.x;
+      w[4 * i + 1] = v.y;
+      w[4 * i + 2] = v.z;
+      w[4 * i + 3] = v.w;
+    }
+  }
+}
+
+// A key word's eight codes as slots: channels 0, 4, 1, 5, 2, 6, 3, 7, as code 2^-24
+// (0, 4, 2, 6) or code 2^-20.
+__device__ __forceinline__ half8 code_slots(unsigned w) {
+  const unsigned u = w >> 8;
+  const uint4 r = make_uint4(w & 0x000f000fu, w & 0x00f000f0u, u & 0x000f000fu, u & 0x00f000f0u);
+  return __builtin_bit_cast(half8, r);
+}
+// The codes of channel n of a lane's CH of eight rows, as code 2^-24 (n even) or
+// code 2^-20. (The compiler shares what the channels of a half word have in common.)
+template <int CH, int N>
+__device__ __forceinline__ half8 value_slots(const unsigned (&v)[8][N], int n) {
+  unsigned r[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const unsigned w0 = v[2 * i][n / 8], w1 = v[2 * i + 1][n / 8];
+    const unsigned u = __builtin_amdgcn_perm(w1, w0, n & 4 ? 0x07060302u : 0x05040100u);
+    r[i] = (n & 2 ? u >> 8 : u) & (n & 1 ? 0x00f000f0u : 0x000f000fu);
+  }
+  const uint4 q = make_uint4(r[0], r[1], r[2], r[3]);
+  return __builtin_bit_cast(half8, q);
+}
+
+// Over the 16 lanes of a row of them, the sum of the lanes NQ apart: each step leaves
+// equal values that many lanes apart, so all lanes add the same pairs.
+template <int NQ>
+__device__ __forceinline__ float groups_sum(float v) {
+  v += dpp0<0x128>(v);                         // row_ror:8
+  if constexpr (NQ <= 4) v += dpp0<0x124>(v);  // row_ror:4
+  if constexpr (NQ <= 2) v += dpp0<0x122>(v);  // row_ror:2
+  return v;
+}
+__device__ __forceinline__ float row_max(float v) {
+  v = fmaxf(v, dpp<0x128>(v));
+  v = fmaxf(v, dpp<0x124>(v));
+  v = fmaxf(v, dpp<0x122>(v));
+  return fmaxf(v, dpp<0x121>(v));
+}
+
 // The eight codes of a word as floats, in channel order.
 __device__ __forceinline__ void codes8(unsigned w, float (&c)[8]) {
   const unsigned lo = w & 0x0f0f0f0fu, hi = (w >> 4) & 0x0f0f0f0fu;
@@ -199,143 +284,200 @@ __device__ __forceinline__ void visible(const Q4AttnArgsOf<MB> &a, int z, int *l
 
 }  // namespace
 
-// One query of RB heads of a KV head (blockIdx.x) over one range of keys
-// (blockIdx.y) of sequence blockIdx.z. A row is spread over D/16
-// lanes of 16 channels (8 bytes of codes, half a 32-channel group):
-//   q.k = step * sum q code + min * sum q   (the lane's part), and
-//   o += (p step) code, o_min += p min,
-// so a code costs one conversion and one FMA a head, all in f32.
-template <int D, int RB, int RPG, int MB>
-__global__ __launch_bounds__(256) void q4_attend_kernel(const Q4AttnArgsOf<MB> a) {
-  constexpr int LPR = D / 16, GPW = 64 / LPR, NG = 4 * GPW, ENTRY = RB * (D + 2);
-  __shared__ float red_o[4][RB][D];
-  __shared__ float red_l[4][RB], wave_m[4][RB];
+// One query of NQ heads of a KV head (blockIdx.x) over one range of keys
+// (blockIdx.y) of sequence blockIdx.z, 32 keys of the range a wave and step.
+//
+// With G = D / 32 groups a row, the 16 columns of a matrix instruction are NQ =
+// 16 / G heads x G groups: column (q, g) of the queries has q's channels of group
+// g and zeros elsewhere, so one accumulator gathers sum_g-channels q code for
+// every (q, g), and a lane, whose column is one (q, g), adds its group's
+//   step * that sum + min * sum_g q
+// for its four keys of 16; the groups' lanes add up to the score. Its weights
+// times its group's steps of the values are row (q, g) of the other product
+// at once, P' V: a column holds channels of one group, and takes its output from
+// that group's rows. min p goes beside it as one sum a (q, g).
+// A lane takes codes in whole words: of a key, the k slots of its quarter are a
+// quarter of the row; of the values, a column is D / 16 consecutive channels,
+// one a product. Codes are operands as they come out of a word: a code in bits
+// 0..3 of a binary16 is code 2^-24, in bits 4..7 code 2^-20, exactly, and the
+// matrix instructions take such numbers as they are; the factor is taken off the
+// queries' slots and the output. Queries and weights are two binary16 pieces.
+// Bound: HBM for many keys, latency (one step of loads, one of sums) for few.
+template <int D, int MB>
+__global__ __launch_bounds__(256, 2) void q4_attend_kernel(const Q4AttnArgsOf<MB> a) {
+  constexpr int G = D / 32, NQ = 16 / G, CH = D / 16, ENTRY = NQ * (D + 2);
+  __shared__ float red_o[4][NQ][D];
+  __shared__ float red_l[4][NQ], wave_m[4][NQ];
 
   const int z = blockIdx.z, hb = blockIdx.x % a.HB, h = blockIdx.x / a.HB, split = blockIdx.y;
   int lo, hi;
   visible(a, z, &lo, &hi);
   const int k0 = lo + split * a.kps, k1 = min(hi, k0 + a.kps);
   if (k0 >= hi) return;  // (split 0 always has a key: the query's own)
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int sub = lane % LPR, grp = wave * GPW + lane / LPR;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 15, t = lane >> 4, g = col / NQ;
   const Q4Rows &seq_rows = a.seq[z].rows;
-  const uint2 *kc = reinterpret_cast<const uint2 *>(seq_rows.k) + (long)h * seq_rows.cap * LPR;
-  const uint2 *vc = reinterpret_cast<const uint2 *>(seq_rows.v) + (long)h * seq_rows.cap * LPR;
-  const unsigned *kp = seq_rows.kp + (long)h * seq_rows.cap * (D / 32);
-  const unsigned *vp = seq_rows.vp + (long)h * seq_rows.cap * (D / 32);
+  const char *const kc = reinterpret_cast<const char *>(seq_rows.k) + (long)h * seq_rows.cap * (D / 2);
+  const char *const vc = reinterpret_cast<const char *>(seq_rows.v) + (long)h * seq_rows.cap * (D / 2);
+  const char *const kp = reinterpret_cast<const char *>(seq_rows.kp) + (long)h * seq_rows.cap * (G * 4);
+  const char *const vp = reinterpret_cast<const char *>(seq_rows.vp) + (long)h * seq_rows.cap * (G * 4);
+  const unsigned k_at = col * (D / 2) + t * (D / 8), v_at = 4 * t * (D / 2) + col * (CH / 2);
+  const unsigned p_at = 4 * t * (G * 4) + g * 4;
 
-  float q[RB][16], qsum[RB], o[RB][16], omin[RB], m[RB], l[RB];
-#pragma unroll
-  for (int r = 0; r < RB; ++r) {
-    const int head = h * a.R + min(hb * RB + r, a.R - 1);  // (the last block may have heads to spare)
-    const float4 *src = reinterpret_cast<const float4 *>(a.q + ((long)z * a.Hq + head) * D + 16 * sub);
-    qsum[r] = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float4 t = src[i];
-      q[r][4 * i] = t.x * a.qscale;
-      q[r][4 * i + 1] = t.y * a.qscale;
-      q[r][4 * i + 2] = t.z * a.qscale;
-      q[r][4 * i + 3] = t.w * a.qscale;
-    }
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      qsum[r] += q[r][i];
-      o[r][i] = 0.0f;
-    }
-    omin[r] = l[r] = 0.0f;
-    m[r] = NEG_INF;
-  }
-
-  for (int c = k0; c < k1; c += NG * RPG) {
-    uint2 kw[RPG], vw[RPG];
-    unsigned kpw[RPG], vpw[RPG];
-    bool valid[RPG];
-#pragma unroll
-    for (int i = 0; i < RPG; ++i) {
-      const int j = c + grp + i * NG;
-      valid[i] = j < k1;
-      const int jj = valid[i] ? j : k0;  // (a row of the range, its weight 0)
-      kw[i] = kc[(long)jj * LPR + sub];
-      kpw[i] = kp[(long)jj * (D / 32) + sub / 2];
-      vw[i] = vc[(long)jj * LPR + sub];
-      vpw[i] = vp[(long)jj * (D / 32) + sub / 2];
-    }
-    float s[RPG][RB];
-#pragma unroll
-    for (int i = 0; i < RPG; ++i) {
-      float e[16];
-      codes8(kw[i].x, reinterpret_cast<float(&)[8]>(e[0]));
-      codes8(kw[i].y, reinterpret_cast<float(&)[8]>(e[8]));
-      const float step = half_lo(kpw[i]), min = half_hi(kpw[i]);
-#pragma unroll
-      for (int r = 0; r < RB; ++r) {
-        float d = 0.0f;
-#pragma unroll
-        for (int t = 0; t < 16; ++t) d = fmaf(q[r][t], e[t], d);
-        s[i][r] = group_sum<LPR>(fmaf(step, d, min * qsum[r]));
-      }
-    }
-    float alpha[RB];
-#pragma unroll
-    for (int r = 0; r < RB; ++r) {
-      float top = NEG_INF;
-#pragma unroll
-      for (int i = 0; i < RPG; ++i) top = valid[i] ? fmaxf(top, s[i][r]) : top;
-      if constexpr (LPR <= 4) top = fmaxf(top, dpp<0x124>(top));  // row_ror:4
-      top = groups_max<LPR>(top);
-      const float mnew = fmaxf(m[r], top), ms = safe_max(mnew);
-      alpha[r] = fast_exp2(m[r] - ms);
-      m[r] = mnew;
-      l[r] *= alpha[r];
-      omin[r] *= alpha[r];
-#pragma unroll
-      for (int t = 0; t < 16; ++t) o[r][t] *= alpha[r];
-#pragma unroll
-      for (int i = 0; i < RPG; ++i) {
-        s[i][r] = valid[i] ? fast_exp2(s[i][r] - ms) : 0.0f;
-        l[r] += s[i][r];
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < RPG; ++i) {
-      float e[16];
-      codes8(vw[i].x, reinterpret_cast<float(&)[8]>(e[0]));
-      codes8(vw[i].y, reinterpret_cast<float(&)[8]>(e[8]));
-      const float step = half_lo(vpw[i]), min = half_hi(vpw[i]);
-#pragma unroll
-      for (int r = 0; r < RB; ++r) {
-        const float ps = s[i][r] * step;
-        omin[r] = fmaf(s[i][r], min, omin[r]);
-#pragma unroll
-        for (int t = 0; t < 16; ++t) o[r][t] = fmaf(ps, e[t], o[r][t]);
-      }
-    }
-  }
-
-  // The row groups of a wave share m: their sums add.
-  auto add_groups = [&](float v) {
-    if constexpr (LPR <= 8) v += dpp0<0x128>(v);  // row_ror:8
-    if constexpr (LPR <= 4) v += dpp0<0x124>(v);  // row_ror:4
-    return sum32(sum16(v));
+  // Of 32 keys from c on: two rows' quarters, and of the eight keys 4 t + 0..3 and
+  // 16 + 4 t + 0..3 the values' words and both rows' params. (The buffers go on for
+  // 128 rows past the last.)
+  struct Tile {
+    unsigned k[2][G], v[8][CH / 8 + (CH < 8)], kp[8], vp[8];
   };
+  auto load = [&](Tile &x, int c) {
+    const char *const kr = kc + (long)c * (D / 2) + k_at, *const vr = vc + (long)c * (D / 2) + v_at;
+    const char *const kpr = kp + (long)c * (G * 4) + p_at, *const vpr = vp + (long)c * (G * 4) + p_at;
 #pragma unroll
-  for (int r = 0; r < RB; ++r) {
-    l[r] = add_groups(l[r]);
+    for (int i = 0; i < 2; ++i) words(kr + i * 16 * (D / 2), x.k[i]);
 #pragma unroll
-    for (int t = 0; t < 16; ++t) {
-      const float v = add_groups(o[r][t] + omin[r]);
-      if (lane < LPR) red_o[wave][r][16 * sub + t] = v;
+    for (int i = 0; i < 8; ++i) {
+      const int row = (i & 3) + 16 * (i >> 2);
+      x.kp[i] = *reinterpret_cast<const unsigned *>(kpr + row * (G * 4));
+      x.vp[i] = *reinterpret_cast<const unsigned *>(vpr + row * (G * 4));
+      if constexpr (CH < 8) x.v[i][0] = *reinterpret_cast<const unsigned short *>(vr + row * (D / 2));
+      else words(vr + row * (D / 2), x.v[i]);
     }
-    if (lane == 0) {
-      red_l[wave][r] = l[r];
-      wave_m[wave][r] = m[r];
+  };
+  int c = k0 + 32 * wave;
+  Tile x, next;
+  if (c < k1) load(next, c);
+
+  // The lane's slots of its head's row; a head past the last is the last.
+  half8 qh[G], ql[G];
+  float inv, qsum = 0.0f;
+  float minus_one = -1.0f;
+  asm volatile("" : "+v"(minus_one));
+  {
+    const int head = h * a.R + min(hb * NQ + col % NQ, a.R - 1);
+    const float *q = a.q + ((long)z * a.Hq + head) * D;
+    float v[G][8], most = 0.0f;
+#pragma unroll
+    for (int j = 0; j < G; ++j) {
+      const int ch = t * (D / 4) + 8 * j;
+      const float4 u0 = *reinterpret_cast<const float4 *>(q + ch), u1 = *reinterpret_cast<const float4 *>(q + ch + 4);
+      const float u[8] = {u0.x, u1.x, u0.y, u1.y, u0.z, u1.z, u0.w, u1.w};  // as codes come off a word
+      const bool mine = ch / 32 == g;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        v[j][i] = mine ? u[i] * a.qscale : 0.0f;
+        const float y = fabsf(v[j][i]);
+        most = fmaxf(most, y <= 3.402823466e38f ? y : 0.0f);
+      }
     }
+    most = max32(max16(most));
+#pragma unroll
+    for (int d = NQ; d < 16; d *= 2) most = fmaxf(most, __shfl_xor(most, d));
+    const unsigned sb = scale_to(most, 13);
+    inv = inverse_scale(sb);
+#pragma unroll
+    for (int j = 0; j < G; ++j) {
+      float w[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        w[i] = v[j][i] * __uint_as_float(sb);
+        qsum += w[i];
+        if (i & 2) w[i] *= 0x1p-4f;
+      }
+      split8(w, minus_one, &qh[j], &ql[j]);
+    }
+    qsum = sum32(sum16(qsum));
+  }
+  // The weights are scaled by a power of two, that their products with the steps
+  // keep two whole pieces; it leaves in the quotient. (A step is at most 2/15 of
+  // vmax, so the products are under 2^15. Steps are no less than 2^-24: a scale past
+  // 2^40 would only let the sums overflow.)
+  const int vexp = min((int)(scale_to(seq_rows.vmax[h], 16) >> 23) - 127, 40);
+
+  f32x4 o[CH];
+#pragma unroll
+  for (int n = 0; n < CH; ++n) o[n] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  float omin = 0.0f, l = 0.0f, m = NEG_INF;
+#pragma unroll 2
+  for (; c < k1; c += 128) {
+    x = next;
+    if (c + 128 < k1) load(next, c + 128);
+    f32x4 sum[2];
+#pragma unroll
+    for (int j = 0; j < G; ++j)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (j == 0) sum[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
+        const half8 kf = code_slots(x.k[i][j]);
+        sum[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[j], sum[i], 0, 0, 0);
+        sum[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[j], sum[i], 0, 0, 0);
+      }
+    float s[8], top = NEG_INF;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float y = fmaf(half_lo(x.kp[i]), sum[i >> 2][i & 3] * 0x1p24f, half_hi(x.kp[i]) * qsum);
+      s[i] = groups_sum<NQ>(y);
+    }
+    const int left = k1 - c - 4 * t;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      s[i] = (i & 3) + 16 * (i >> 2) < left ? s[i] : NEG_INF;
+      top = fmaxf(top, s[i]);
+    }
+    top = max32(max16(top));
+    if (__any(top > m)) {
+      const float mnew = fmaxf(m, top), alpha = fast_exp2((m - safe_max(mnew)) * inv);
+      m = mnew;
+      l *= alpha;
+      omin *= alpha;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float f = __shfl(alpha, 4 * t + e);
+#pragma unroll
+        for (int n = 0; n < CH; ++n) o[n][e] *= f;
+      }
+    }
+    const float shift = fmaf(-safe_max(m), inv, (float)vexp);
+    float p[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const bool valid = (i & 3) + 16 * (i >> 2) < left;
+      const float w = fast_exp2(fmaf(s[i], inv, shift));
+      l += w;
+      // (rows past the range may hold anything)
+      p[i] = valid ? w * half_lo(x.vp[i]) : 0.0f;
+      omin = valid ? fmaf(w, half_hi(x.vp[i]), omin) : omin;
+    }
+    half8 ph, pl;
+    split8(p, minus_one, &ph, &pl);
+#pragma unroll
+    for (int n = 0; n < CH; ++n) {
+      const half8 vf = value_slots<CH>(x.v, n);
+      o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl, vf, o[n], 0, 0, 0);
+      o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph, vf, o[n], 0, 0, 0);
+    }
+  }
+
+  l = sum32(sum16(l));
+  omin = sum32(sum16(omin));
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int row = 4 * t + e;
+    const float least = __shfl(omin, row);
+    if (row / NQ == g)
+#pragma unroll
+      for (int n = 0; n < CH; ++n) red_o[wave][row % NQ][col * CH + n] = fmaf(o[n][e], n & 1 ? 0x1p20f : 0x1p24f, least);
+  }
+  if (lane < NQ) {
+    red_l[wave][lane] = l;
+    wave_m[wave][lane] = m == NEG_INF ? m : m * inv;
   }
   __syncthreads();
   const long entry = (((long)z * a.Hkv + h) * a.HB + hb) * a.max_splits + split;
-  for (int e = threadIdx.x; e < RB * D; e += 256) {
+#pragma unroll
+  for (int e = threadIdx.x; e < NQ * D; e += 256) {
     const int r = e / D, dim = e % D;
+    if (hb * NQ + r >= a.R) break;
     const float M = fmaxf(fmaxf(wave_m[0][r], wave_m[1][r]), fmaxf(wave_m[2][r], wave_m[3][r]));
     const float Ms = safe_max(M);
     float O = 0.0f, L = 0.0f;
@@ -349,95 +491,94 @@ __global__ __launch_bounds__(256) void q4_attend_kernel(const Q4AttnArgsOf<MB> a
       float *dst = a.partial + entry * (long)ENTRY;
       dst[e] = O;
       if (dim == 0) {
-        dst[RB * D + 2 * r] = M;
-        dst[RB * D + 2 * r + 1] = L;
+        dst[NQ * D + 2 * r] = M;
+        dst[NQ * D + 2 * r + 1] = L;
       }
-    } else if (hb * RB + r < a.R) {
-      a.out[((long)z * a.Hq + h * a.R + hb * RB + r) * D + dim] = O / L;
+    } else {
+      a.out[((long)z * a.Hq + h * a.R + hb * NQ + r) * D + dim] = O / L;
       if (dim == 0 && !(L > 0.0f && L < __builtin_inff())) atomicOr(a.err, kDevErrSoftmaxDenominator);
     }
   }
 }
 
-// Merges the key ranges of one (query, KV head, head block). 256 threads: 32
-// consecutive outputs x 8 range lanes.
-template <int D, int RB, int MB>
-__global__ __launch_bounds__(256) void q4_combine_kernel(const Q4AttnArgsOf<MB> a) {
-  constexpr int ENTRY = RB * (D + 2), OUTS = 32, SL = 8;
-  __shared__ float s_m[SL][OUTS], s_l[SL][OUTS], s_o[SL][OUTS];
+// Merges the key ranges of one (query, KV head, head block): 32 consecutive
+// outputs x 32 range lanes. The ranges' weights come first, a thread a range, so
+// that the sums' reads depend on nothing and are all in flight at once.
+template <int D, int MB>
+__global__ __launch_bounds__(1024) void q4_combine_kernel(const Q4AttnArgsOf<MB> a) {
+  constexpr int NQ = 512 / D, ENTRY = NQ * (D + 2), OUTS = 32, SL = 32;
+  __shared__ float weight[kMaxDecodeSplits], part[SL][OUTS + 1], wave_m[16], wave_l[16];
   const int z = blockIdx.z, hb = blockIdx.x % a.HB, h = blockIdx.x / a.HB;
+  const int tid = threadIdx.x, e = blockIdx.y * OUTS + tid % OUTS, r = blockIdx.y * OUTS / D, sl = tid / OUTS;
+  if (hb * NQ + r >= a.R) return;
   int lo, hi;
   visible(a, z, &lo, &hi);
   const int nsplit = (hi - lo + a.kps - 1) / a.kps;
-  const int out = threadIdx.x % OUTS, sl = threadIdx.x / OUTS;
-  const int e = blockIdx.y * OUTS + out, r = e / D;
   const float *ents = a.partial + (((long)z * a.Hkv + h) * a.HB + hb) * a.max_splits * (long)ENTRY;
-  float m = NEG_INF, l = 0.0f, o = 0.0f;
-  for (int s = sl; s < nsplit; s += SL) {
-    const float *ent = ents + (long)s * ENTRY;
-    const float em = ent[RB * D + 2 * r], el = ent[RB * D + 2 * r + 1], eo = ent[e];
-    const float mx = fmaxf(m, em), mxs = safe_max(mx);
-    const float f = fast_exp2(m - mxs), g = fast_exp2(em - mxs);
-    l = l * f + el * g;
-    o = o * f + eo * g;
-    m = mx;
+  float em = NEG_INF, el = 0.0f;
+  if (tid < nsplit) {
+    const float2 ml = *reinterpret_cast<const float2 *>(ents + (long)tid * ENTRY + NQ * D + 2 * r);
+    em = ml.x;
+    el = ml.y;
   }
-  s_m[sl][out] = m;
-  s_l[sl][out] = l;
-  s_o[sl][out] = o;
+  float v[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int s = sl + i * SL;
+    v[i] = s < nsplit ? ents[(long)s * ENTRY + e] : 0.0f;
+  }
+  const float top = max32(max16(row_max(em)));
+  if ((tid & 63) == 0) wave_m[tid >> 6] = top;
   __syncthreads();
-  if (sl == 0 && hb * RB + r < a.R) {
-    float M = NEG_INF;
+  const float M = safe_max(row_max(wave_m[tid & 15]));
+  const float w = fast_exp2(em - M);
+  if (tid < nsplit) weight[tid] = w;
+  const float sum = group_sum<64>(tid < nsplit ? el * w : 0.0f);
+  if ((tid & 63) == 0) wave_l[tid >> 6] = sum;
+  __syncthreads();
+  float O = 0.0f;
 #pragma unroll
-    for (int k = 0; k < SL; ++k) M = fmaxf(M, s_m[k][out]);
-    const float Ms = safe_max(M);
-    float L = 0.0f, O = 0.0f;
+  for (int i = 0; i < 4; ++i) {
+    const int s = sl + i * SL;
+    if (s < nsplit) O = fmaf(v[i], weight[s], O);
+  }
+#pragma unroll 4
+  for (int s = sl + 4 * SL; s < nsplit; s += SL) O = fmaf(ents[(long)s * ENTRY + e], weight[s], O);
+  part[sl][tid % OUTS] = O;
+  __syncthreads();
+  if (tid < OUTS) {
+    float total = 0.0f, L = 0.0f;
 #pragma unroll
-    for (int k = 0; k < SL; ++k) {
-      const float g = fast_exp2(s_m[k][out] - Ms);
-      L += s_l[k][out] * g;
-      O += s_o[k][out] * g;
-    }
-    a.out[((long)z * a.Hq + h * a.R + hb * RB) * D + e] = O / L;
+    for (int k = 0; k < SL; ++k) total += part[k][tid];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) L += wave_l[k];
+    a.out[((long)z * a.Hq + h * a.R + hb * NQ) * D + e] = total / L;
     if ((e % D) == 0 && !(L > 0.0f && L < __builtin_inff())) atomicOr(a.err, kDevErrSoftmaxDenominator);
   }
 }
 
 namespace {
 
-constexpr int kQ4Rows = 2;  // rows per lane group in flight
-
-template <int D, int RB, int MB>
+template <int D, int MB>
 hipError_t attend(hipStream_t st, const Q4AttnArgsOf<MB> &a, int nz) {
   const dim3 grid((unsigned)(a.Hkv * a.HB), (unsigned)a.max_splits, (unsigned)nz);
-  hipLaunchKernelGGL((q4_attend_kernel<D, RB, kQ4Rows, MB>), grid, dim3(256), 0, st, a);
+  hipLaunchKernelGGL((q4_attend_kernel<D, MB>), grid, dim3(256), 0, st, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.max_splits == 1) return e;
-  const dim3 cgrid((unsigned)(a.Hkv * a.HB), (unsigned)(RB * D / 32), (unsigned)nz);
-  hipLaunchKernelGGL((q4_combine_kernel<D, RB, MB>), cgrid, dim3(256), 0, st, a);
+  const dim3 cgrid((unsigned)(a.Hkv * a.HB), (unsigned)(std::min(a.R, 512 / D) * D / 32), (unsigned)nz);
+  hipLaunchKernelGGL((q4_combine_kernel<D, MB>), cgrid, dim3(1024), 0, st, a);
   return hipGetLastError();
 }
 
-template <int D, int RB>
-hipError_t attend_b(hipStream_t st, const Q4AttnArgs &a, int nz) {
+template <int D>
+hipError_t attend_d(hipStream_t st, const Q4AttnArgs &a, int nz) {
   if (nz == 1) {
     Q4AttnArgsOf<1> one;
     static_cast<Q4AttnBase &>(one) = a;
     one.seq[0] = a.seq[0];
-    return attend<D, RB, 1>(st, one, nz);
+    return attend<D, 1>(st, one, nz);
   }
-  return attend<D, RB, kMaxDecodeBatch>(st, a, nz);
-}
-
-template <int D>
-hipError_t attend_d(hipStream_t st, const Q4AttnArgs &a, int RB, int nz) {
-  switch (RB) {
-    case 1: return attend_b<D, 1>(st, a, nz);
-    case 2: return attend_b<D, 2>(st, a, nz);
-    case 3: return attend_b<D, 3>(st, a, nz);
-    case 4: return attend_b<D, 4>(st, a, nz);
-    default: return hipErrorInvalidValue;
-  }
+  return attend<D, kMaxDecodeBatch>(st, a, nz);
 }
 
 }  // namespace
@@ -446,9 +587,9 @@ bool q4_supported(size_t D) { return D == 64 || D == 128 || D == 256; }
 
 Q4AttnPlan q4_attend_plan(int D, int R, int Hkv, const int *keys, int n) {
   Q4AttnPlan p;
-  p.HB = (R + 3) / 4;
-  p.RB = (R + p.HB - 1) / p.HB;
-  const int chunk = 4 * (64 / (D / 16)) * kQ4Rows;
+  p.RB = 512 / D;  // the kernel's heads
+  p.HB = (R + p.RB - 1) / p.RB;
+  const int chunk = 128;  // a step of the workgroup
   long total = 0;
   int most = 1;
   for (int i = 0; i < n; ++i) {
@@ -465,11 +606,11 @@ Q4AttnPlan q4_attend_plan(int D, int R, int Hkv, const int *keys, int n) {
   return p;
 }
 
-hipError_t launch_q4_attend(hipStream_t st, const Q4AttnArgs &a, int D, int RB, int nz) {
+hipError_t launch_q4_attend(hipStream_t st, const Q4AttnArgs &a, int D, int nz) {
   switch (D) {
-    case 64: return attend_d<64>(st, a, RB, nz);
-    case 128: return attend_d<128>(st, a, RB, nz);
-    case 256: return attend_d<256>(st, a, RB, nz);
+    case 64: return attend_d<64>(st, a, nz);
+    case 128: return attend_d<128>(st, a, nz);
+    case 256: return attend_d<256>(st, a, nz);
     default: return hipErrorInvalidValue;
   }
 }
