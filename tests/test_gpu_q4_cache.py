@@ -41,7 +41,10 @@ def dev(a):
 
 @pytest.fixture(scope="module")
 def ses(gpu):
-    return Session(0, stream=torch.cuda.current_stream())
+    # the tests' own tensors are made, filled and freed on the session's stream
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        yield Session(0, stream=stream)
 
 
 def held(ses, cache, first=0, n=None):

@@ -23,7 +23,10 @@ pytestmark = pytest.mark.gpu
 
 @pytest.fixture(scope="module")
 def ses(gpu):
-    return Session(0, stream=torch.cuda.current_stream())
+    # the tests' own tensors are made, filled and freed on the session's stream
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        yield Session(0, stream=stream)
 
 
 SCALES = {"f16": np.float16, "bf16": None, "f32": np.float32}
