@@ -1461,7 +1461,7 @@ static int refuse_q4(const spissa_kv_cache *c, const char *what) {
 // call prepares the workspace of every later one of its batch and heads.
 static size_t q4_partial_bytes(size_t n, size_t Hq, size_t D, const Q4AttnPlan &p, size_t Hkv) {
   const size_t groups = Hkv * p.HB;
-  return n * (groups + kDecodeGridWorkgroups) * (size_t)p.RB * (D + 2) * sizeof(float);
+  return n * (groups + kQ4GridWorkgroups) * (size_t)p.RB * (D + 2) * sizeof(float);
 }
 
 // One query of each of B sequences, whose own row is its cache's last.

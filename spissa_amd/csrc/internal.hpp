@@ -377,6 +377,10 @@ struct Q4AttnArgsOf : Q4AttnBase {
   Q4Seq seq[MB];
 };
 typedef Q4AttnArgsOf<kMaxDecodeBatch> Q4AttnArgs;
+// Workgroups that a decode launch over 4-bit caches aims at: one a CU. (16 sequences
+// of 4096 keys, 64 heads on 8 of 128: 36 us, aiming at 512 workgroups 60; 32768 keys
+// of one head of 256: 15 us either way.)
+constexpr int kQ4GridWorkgroups = 256;
 struct Q4AttnPlan {
   int RB, HB, kps, splits;
 };

@@ -100,6 +100,9 @@ __device__ __forceinline__ half8 value_slots(const unsigned (&v)[8][N], int n) {
   return __builtin_bit_cast(half8, q);
 }
 
+// The key of 32 in slot i of a lane's eight, above the 4 (lane / 16) that the lanes differ by.
+__device__ __forceinline__ constexpr int key_of(int i) { return (i & 3) + 16 * (i >> 2); }
+
 // Over the 16 lanes of a row of them, the sum of the lanes NQ apart: each step leaves
 // equal values that many lanes apart, so all lanes add the same pairs.
 template <int NQ>
@@ -275,6 +278,9 @@ __global__ __launch_bounds__(256) void q4_rows_kernel(const Q4Rows s, int n, int
 
 namespace {
 
+// (eight waves: a workgroup a CU holds two or three a SIMD)
+constexpr int kQ4Waves = 8, kQ4Step = 32 * kQ4Waves;  // waves of a workgroup, and the keys of a step of theirs
+
 // The keys that the last token of sequence z sees, [lo, hi).
 template <int MB>
 __device__ __forceinline__ void visible(const Q4AttnArgsOf<MB> &a, int z, int *lo, int *hi) {
@@ -303,11 +309,17 @@ __device__ __forceinline__ void visible(const Q4AttnArgsOf<MB> &a, int z, int *l
 // matrix instructions take such numbers as they are; the factor is taken off the
 // queries' slots and the output. Queries and weights are two binary16 pieces.
 // Bound: HBM for many keys, latency (one step of loads, one of sums) for few.
+// 16 sequences of 8192 keys, 24 heads on 8 of 128: 40 us, 4.1 TB/s of codes and
+// params (a copy reaches 5.1); 32768 keys of one head of 256: 12 us; 512 keys, 32
+// heads on 8 of 64: 5.6 us.
 template <int D, int MB>
-__global__ __launch_bounds__(256, 2) void q4_attend_kernel(const Q4AttnArgsOf<MB> a) {
+__global__ __launch_bounds__(64 * kQ4Waves) void q4_attend_kernel(const Q4AttnArgsOf<MB> a) {
   constexpr int G = D / 32, NQ = 16 / G, CH = D / 16, ENTRY = NQ * (D + 2);
-  __shared__ float red_o[4][NQ][D];
-  __shared__ float red_l[4][NQ], wave_m[4][NQ];
+  __shared__ float red_o[kQ4Waves][NQ][D];
+  __shared__ float red_l[kQ4Waves][NQ], wave_m[kQ4Waves][NQ];
+  __shared__ _Float16 q_lds[2][NQ][D + 8] __attribute__((aligned(16)));
+  __shared__ float q_sum[NQ][G], q_inv[NQ];
+  static_assert(NQ * D == 64 * kQ4Waves, "a thread a channel of the queries");
 
   const int z = blockIdx.z, hb = blockIdx.x % a.HB, h = blockIdx.x / a.HB, split = blockIdx.y;
   int lo, hi;
@@ -327,66 +339,65 @@ __global__ __launch_bounds__(256, 2) void q4_attend_kernel(const Q4AttnArgsOf<MB
   // Of 32 keys from c on: two rows' quarters, and of the eight keys 4 t + 0..3 and
   // 16 + 4 t + 0..3 the values' words and both rows' params. (The buffers go on for
   // 128 rows past the last.)
-  struct Tile {
-    unsigned k[2][G], v[8][CH / 8 + (CH < 8)], kp[8], vp[8];
-  };
-  auto load = [&](Tile &x, int c) {
-    const char *const kr = kc + (long)c * (D / 2) + k_at, *const vr = vc + (long)c * (D / 2) + v_at;
-    const char *const kpr = kp + (long)c * (G * 4) + p_at, *const vpr = vp + (long)c * (G * 4) + p_at;
+  unsigned kw[2][G], vw[8][CH / 8 + (CH < 8)], kpw[8], vpw[8];
+  auto load_k = [&](int c) {
+    const char *const rows = kc + (long)c * (D / 2) + k_at, *const params = kp + (long)c * (G * 4) + p_at;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) words(kr + i * 16 * (D / 2), x.k[i]);
+    for (int i = 0; i < 2; ++i) words(rows + i * 16 * (D / 2), kw[i]);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) kpw[i] = *reinterpret_cast<const unsigned *>(params + key_of(i) * (G * 4));
+  };
+  auto load_v = [&](int c) {
+    const char *const rows = vc + (long)c * (D / 2) + v_at, *const params = vp + (long)c * (G * 4) + p_at;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int row = (i & 3) + 16 * (i >> 2);
-      x.kp[i] = *reinterpret_cast<const unsigned *>(kpr + row * (G * 4));
-      x.vp[i] = *reinterpret_cast<const unsigned *>(vpr + row * (G * 4));
-      if constexpr (CH < 8) x.v[i][0] = *reinterpret_cast<const unsigned short *>(vr + row * (D / 2));
-      else words(vr + row * (D / 2), x.v[i]);
+      vpw[i] = *reinterpret_cast<const unsigned *>(params + key_of(i) * (G * 4));
+      if constexpr (CH < 8) vw[i][0] = *reinterpret_cast<const unsigned short *>(rows + key_of(i) * (D / 2));
+      else words(rows + key_of(i) * (D / 2), vw[i]);
     }
   };
   int c = k0 + 32 * wave;
-  Tile x, next;
-  if (c < k1) load(next, c);
+  if (c < k1) {
+    load_k(c);
+    load_v(c);
+  }
 
-  // The lane's slots of its head's row; a head past the last is the last.
+  // The queries' pieces, a channel a thread, as codes come off a word: 0, 4, 1, 5,
+  // 2, 6, 3, 7 of eight. (A head past the last is the last.)
+  const int r = threadIdx.x / D, ch = threadIdx.x % D;
+  float y = a.q[((long)z * a.Hq + h * a.R + min(hb * NQ + r, a.R - 1)) * D + ch] * a.qscale;
+  {
+    const float size = fabsf(y);
+    const float most = max32(max16(row_max(size <= 3.402823466e38f ? size : 0.0f)));
+    if (lane == 0) wave_m[wave][0] = most;
+  }
+  __syncthreads();
+  float most = 0.0f;
+#pragma unroll
+  for (int i = 0; i < D / 64; ++i) most = fmaxf(most, wave_m[r * (D / 64) + i][0]);
+  const unsigned sb = scale_to(most, 13);
+  y *= __uint_as_float(sb);
+  {
+    const float sum = group_sum<32>(y);
+    if (ch % 32 == 0) q_sum[r][ch / 32] = sum;
+    if (ch % D == 0) q_inv[r] = inverse_scale(sb);
+    const float slot = y * (ch & 1 ? 0x1p-4f : 1.0f);
+    const _Float16 hi_piece = pieces2(slot, 0.0f).x;
+    const int at = (ch & ~7) + (ch & 3) * 2 + (ch >> 2 & 1);
+    q_lds[0][r][at] = hi_piece;
+    q_lds[1][r][at] = pieces2(slot - (float)hi_piece, 0.0f).x;
+  }
+  __syncthreads();
   half8 qh[G], ql[G];
-  float inv, qsum = 0.0f;
+  const float inv = q_inv[col % NQ], qsum = q_sum[col % NQ][g];
   float minus_one = -1.0f;
   asm volatile("" : "+v"(minus_one));
-  {
-    const int head = h * a.R + min(hb * NQ + col % NQ, a.R - 1);
-    const float *q = a.q + ((long)z * a.Hq + head) * D;
-    float v[G][8], most = 0.0f;
 #pragma unroll
-    for (int j = 0; j < G; ++j) {
-      const int ch = t * (D / 4) + 8 * j;
-      const float4 u0 = *reinterpret_cast<const float4 *>(q + ch), u1 = *reinterpret_cast<const float4 *>(q + ch + 4);
-      const float u[8] = {u0.x, u1.x, u0.y, u1.y, u0.z, u1.z, u0.w, u1.w};  // as codes come off a word
-      const bool mine = ch / 32 == g;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        v[j][i] = mine ? u[i] * a.qscale : 0.0f;
-        const float y = fabsf(v[j][i]);
-        most = fmaxf(most, y <= 3.402823466e38f ? y : 0.0f);
-      }
-    }
-    most = max32(max16(most));
-#pragma unroll
-    for (int d = NQ; d < 16; d *= 2) most = fmaxf(most, __shfl_xor(most, d));
-    const unsigned sb = scale_to(most, 13);
-    inv = inverse_scale(sb);
-#pragma unroll
-    for (int j = 0; j < G; ++j) {
-      float w[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        w[i] = v[j][i] * __uint_as_float(sb);
-        qsum += w[i];
-        if (i & 2) w[i] *= 0x1p-4f;
-      }
-      split8(w, minus_one, &qh[j], &ql[j]);
-    }
-    qsum = sum32(sum16(qsum));
+  for (int j = 0; j < G; ++j) {
+    const int first = t * (D / 4) + 8 * j;
+    const half8 none{};
+    qh[j] = first / 32 == g ? *reinterpret_cast<const half8 *>(&q_lds[0][col % NQ][first]) : none;
+    ql[j] = first / 32 == g ? *reinterpret_cast<const half8 *>(&q_lds[1][col % NQ][first]) : none;
   }
   // The weights are scaled by a power of two, that their products with the steps
   // keep two whole pieces; it leaves in the quotient. (A step is at most 2/15 of
@@ -398,32 +409,38 @@ __global__ __launch_bounds__(256, 2) void q4_attend_kernel(const Q4AttnArgsOf<MB
 #pragma unroll
   for (int n = 0; n < CH; ++n) o[n] = (f32x4){0.f, 0.f, 0.f, 0.f};
   float omin = 0.0f, l = 0.0f, m = NEG_INF;
-#pragma unroll 2
-  for (; c < k1; c += 128) {
-    x = next;
-    if (c + 128 < k1) load(next, c + 128);
+  // (no copies of the next step's words: they are asked for when this step's are spent)
+  for (; c < k1; c += kQ4Step) {
+    const bool more = c + kQ4Step < k1;
     f32x4 sum[2];
 #pragma unroll
     for (int j = 0; j < G; ++j)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         if (j == 0) sum[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
-        const half8 kf = code_slots(x.k[i][j]);
+        const half8 kf = code_slots(kw[i][j]);
         sum[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[j], sum[i], 0, 0, 0);
         sum[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[j], sum[i], 0, 0, 0);
       }
     float s[8], top = NEG_INF;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float y = fmaf(half_lo(x.kp[i]), sum[i >> 2][i & 3] * 0x1p24f, half_hi(x.kp[i]) * qsum);
+      const float y = fmaf(half_lo(kpw[i]), sum[i >> 2][i & 3] * 0x1p24f, half_hi(kpw[i]) * qsum);
       s[i] = groups_sum<NQ>(y);
     }
-    const int left = k1 - c - 4 * t;
+    if (more) load_k(c + kQ4Step);
+    if (c + 32 > k1) {  // (rows past the range may hold anything)
+      int left = k1 - c - 4 * t;
+      asm volatile("" : "+v"(left));
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      s[i] = (i & 3) + 16 * (i >> 2) < left ? s[i] : NEG_INF;
-      top = fmaxf(top, s[i]);
+      for (int i = 0; i < 8; ++i)
+        if (key_of(i) >= left) {
+          s[i] = NEG_INF;
+          vpw[i] = 0;
+        }
     }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = fmaxf(top, s[i]);
     top = max32(max16(top));
     if (__any(top > m)) {
       const float mnew = fmaxf(m, top), alpha = fast_exp2((m - safe_max(mnew)) * inv);
@@ -441,21 +458,20 @@ __global__ __launch_bounds__(256, 2) void q4_attend_kernel(const Q4AttnArgsOf<MB
     float p[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const bool valid = (i & 3) + 16 * (i >> 2) < left;
       const float w = fast_exp2(fmaf(s[i], inv, shift));
       l += w;
-      // (rows past the range may hold anything)
-      p[i] = valid ? w * half_lo(x.vp[i]) : 0.0f;
-      omin = valid ? fmaf(w, half_hi(x.vp[i]), omin) : omin;
+      p[i] = w * half_lo(vpw[i]);
+      omin = fmaf(w, half_hi(vpw[i]), omin);
     }
     half8 ph, pl;
     split8(p, minus_one, &ph, &pl);
 #pragma unroll
     for (int n = 0; n < CH; ++n) {
-      const half8 vf = value_slots<CH>(x.v, n);
+      const half8 vf = value_slots<CH>(vw, n);
       o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl, vf, o[n], 0, 0, 0);
       o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph, vf, o[n], 0, 0, 0);
     }
+    if (more) load_v(c + kQ4Step);
   }
 
   l = sum32(sum16(l));
@@ -475,14 +491,16 @@ __global__ __launch_bounds__(256, 2) void q4_attend_kernel(const Q4AttnArgsOf<MB
   __syncthreads();
   const long entry = (((long)z * a.Hkv + h) * a.HB + hb) * a.max_splits + split;
 #pragma unroll
-  for (int e = threadIdx.x; e < NQ * D; e += 256) {
+  for (int e = threadIdx.x; e < NQ * D; e += 64 * kQ4Waves) {
     const int r = e / D, dim = e % D;
     if (hb * NQ + r >= a.R) break;
-    const float M = fmaxf(fmaxf(wave_m[0][r], wave_m[1][r]), fmaxf(wave_m[2][r], wave_m[3][r]));
+    float M = NEG_INF;
+#pragma unroll
+    for (int w = 0; w < kQ4Waves; ++w) M = fmaxf(M, wave_m[w][r]);
     const float Ms = safe_max(M);
     float O = 0.0f, L = 0.0f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < kQ4Waves; ++w) {
       const float f = fast_exp2(wave_m[w][r] - Ms);
       O = fmaf(red_o[w][r][dim], f, O);
       L = fmaf(red_l[w][r], f, L);
@@ -562,7 +580,7 @@ namespace {
 template <int D, int MB>
 hipError_t attend(hipStream_t st, const Q4AttnArgsOf<MB> &a, int nz) {
   const dim3 grid((unsigned)(a.Hkv * a.HB), (unsigned)a.max_splits, (unsigned)nz);
-  hipLaunchKernelGGL((q4_attend_kernel<D, MB>), grid, dim3(256), 0, st, a);
+  hipLaunchKernelGGL((q4_attend_kernel<D, MB>), grid, dim3(64 * kQ4Waves), 0, st, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.max_splits == 1) return e;
   const dim3 cgrid((unsigned)(a.Hkv * a.HB), (unsigned)(std::min(a.R, 512 / D) * D / 32), (unsigned)nz);
@@ -589,7 +607,7 @@ Q4AttnPlan q4_attend_plan(int D, int R, int Hkv, const int *keys, int n) {
   Q4AttnPlan p;
   p.RB = 512 / D;  // the kernel's heads
   p.HB = (R + p.RB - 1) / p.RB;
-  const int chunk = 128;  // a step of the workgroup
+  constexpr int chunk = kQ4Step;
   long total = 0;
   int most = 1;
   for (int i = 0; i < n; ++i) {
@@ -597,8 +615,12 @@ Q4AttnPlan q4_attend_plan(int D, int R, int Hkv, const int *keys, int n) {
     most = std::max(most, keys[i]);
   }
   const long heads = (long)Hkv * p.HB;
-  const long per = (total * heads + kDecodeGridWorkgroups - 1) / kDecodeGridWorkgroups;
+  const long per = (total * heads + kQ4GridWorkgroups - 1) / kQ4GridWorkgroups;
   long kps = std::max<long>(1, (per + chunk - 1) / chunk) * chunk;
+  // A second launch costs 3.3 us, a step 1.2 to 2: two steps stay one range.
+  // (512 keys, heads of 64: 6.3 us against 8.0 in two ranges; 1024: 8.7 in one,
+  // 8.0 in four.)
+  if (most <= 2 * chunk) kps = 2 * chunk;
   if ((most + kps - 1) / kps > kMaxDecodeSplits)
     kps = ((most + kMaxDecodeSplits - 1) / kMaxDecodeSplits + chunk - 1) / chunk * chunk;
   p.kps = (int)kps;
