@@ -1524,6 +1524,7 @@ static int q4_attend_chunk(spissa_session *s, const float *q, const spissa_kv_ca
   a.causal = c->causal ? 1 : 0;
   a.window = (int)c->window;
   a.qscale = (1.0f / sqrtf((float)D)) * 1.4426950408889634f;
+  a.per = p.per;
   a.splits = p.splits;
   a.tps = p.tps;
   const size_t rows = c->query_len * c->num_heads;

@@ -400,11 +400,11 @@ struct Q4ChunkArgs {
   // With splits > 1, split j takes key tiles [j * tps, (j + 1) * tps) of those a
   // workgroup sees and writes its part as PrefillArgs has it; launch_prefill_combine
   // merges them.
-  int splits, tps;
+  int per, splits, tps;  // per: rows of a workgroup, 128 or 256 (128 for heads of 256)
   float *part_o, *part_ml;
 };
 struct Q4ChunkPlan {
-  int splits = 1, tps = 0;
+  int per = 128, splits = 1, tps = 0;
   size_t partial_bytes = 0;
 };
 Q4ChunkPlan q4_chunk_plan(int D, int S, int R, int Hkv, int len, int causal, int window, int cus);

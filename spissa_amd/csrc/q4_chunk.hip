@@ -12,7 +12,7 @@
 // head's largest, and the probabilities, times 2^6, are two pieces each, of
 // whose four products the three above 2^-22 are taken.
 //
-// A workgroup takes 128 QT rows of a KV head, a row being a (query,
+// A workgroup takes 128 or 256 rows of a KV head, a row being a (query,
 // query head of the group) pair with the head fastest, so that short chunks
 // fill the instruction's 16 columns with heads. Per tile of keys it widens the
 // codes into LDS once for all of them: the keys as they are, in the order in
@@ -94,7 +94,7 @@ __device__ __forceinline__ half8 codes8h(unsigned w, unsigned base) {
 // conversions of one run beside the matrix instructions of the other (one loop
 // body, in which the two kinds have the barrier at different places). Within a
 // wave the LDS reads run one step ahead of the instructions that need them.
-template <int D, int NW, int QT>
+template <int D, int NW>
 __global__ __launch_bounds__(NW * 64, NW / 4) void q4_chunk_kernel(const Q4ChunkArgs a) {
   constexpr int BN = 8192 / D, G = D / 32, DT = D / 16, VB = BN / 32;
   constexpr int AH = NW == 16 ? 1 : 2;  // fragments of a step in registers, or of this one and the next
@@ -119,14 +119,27 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void q4_chunk_kernel(const Q4Chunk
   const int h = blockIdx.x, split = blockIdx.z;
   const int block = gridDim.y - 1 - blockIdx.y;
   const int rows = a.S * a.R;
-  const int row0 = block * (NW * 16 * QT) + wave * (16 * QT);
+  const int row0 = block * (NW * 16) + wave * 16;
   const int P = a.len - a.S;  // the first query's position
   // keys that any row of the workgroup sees
-  const int first_q = block * (NW * 16 * QT) / a.R, last_q = min(rows - 1, (block + 1) * (NW * 16 * QT) - 1) / a.R;
+  const int first_q = block * (NW * 16) / a.R, last_q = min(rows - 1, (block + 1) * (NW * 16) - 1) / a.R;
   const int hi = a.causal ? P + last_q + 1 : a.len;
   const int lo = a.window > 0 ? max(0, P + first_q + 1 - a.window) : 0;
   const int t0 = lo / BN + split * a.tps;
   const int t1 = min((hi + BN - 1) / BN, t0 + a.tps);
+
+  // A lane's row, for the column.
+  const int pos = P + min(row0 + col, rows - 1) / a.R;
+  const long orow = [&] {  // query * Hq + head
+    const int r = min(row0 + col, rows - 1), query = r / a.R;
+    return (long)query * a.Hq + h * a.R + (r - query * a.R);
+  }();
+  const long total = (long)a.S * a.Hq;
+  float *const ml = a.part_ml + ((long)split * total + orow) * 2;
+  if (t0 >= t1) {  // (a range of none of the block's tiles: with m at -inf no outputs are read)
+    if (row0 + col < rows && kq == 0) *reinterpret_cast<float2 *>(ml) = make_float2(NEG_INF, 0.0f);
+    return;
+  }
 
   // A tile's codes, steps and minima come as they are, straight into LDS (1 KB a
   // wave and instruction). The rows past the last are read too (the buffers end
@@ -147,81 +160,65 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void q4_chunk_kernel(const Q4Chunk
       copy16(from, lane * 16, raw_lds[tile & 1] + chunk * 1024);
     }
   };
-  if (t0 < t1) fetch(t0);
+  fetch(t0);
   if (t0 + 1 < t1) fetch(t0 + 1);
 
-  // A lane's row, for each of its QT column tiles.
-  int pos[QT];
-  auto query_row = [&](int t) {  // query * Hq + head
-    const int r = min(row0 + 16 * t + col, rows - 1), query = r / a.R;
-    return (long)query * a.Hq + h * a.R + (r - query * a.R);
-  };
-  half8 qh[QT][G], ql[QT][G], qs[QT];
-  float inv[QT];
+  half8 qh[G], ql[G], qs;
+  float inv;
+  const float *q = a.q + orow * D + 8 * kq;
+  float v[G][8], most = 0.0f;
 #pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    pos[t] = P + min(row0 + 16 * t + col, rows - 1) / a.R;
-    const float *q = a.q + query_row(t) * D + 8 * kq;
-    float v[G][8], most = 0.0f;
+  for (int g = 0; g < G; ++g) {
+    const float4 x = *reinterpret_cast<const float4 *>(q + 32 * g), y = *reinterpret_cast<const float4 *>(q + 32 * g + 4);
+    const float u[8] = {x.x, y.x, x.y, y.y, x.z, y.z, x.w, y.w};  // channels 0, 4, 1, 5, ...
 #pragma unroll
-    for (int g = 0; g < G; ++g) {
-      const float4 x = *reinterpret_cast<const float4 *>(q + 32 * g), y = *reinterpret_cast<const float4 *>(q + 32 * g + 4);
-      const float u[8] = {x.x, y.x, x.y, y.y, x.z, y.z, x.w, y.w};  // channels 0, 4, 1, 5, ...
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        v[g][i] = u[i] * a.qscale;
-        const float m = fabsf(v[g][i]);
-        most = fmaxf(most, m <= 3.402823466e38f ? m : 0.0f);
-      }
+    for (int i = 0; i < 8; ++i) {
+      v[g][i] = u[i] * a.qscale;
+      const float m = fabsf(v[g][i]);
+      most = fmaxf(most, m <= 3.402823466e38f ? m : 0.0f);
     }
-    most = max32(max16(most));
-    const unsigned sb = scale_to(most, 9);
-    inv[t] = inverse_scale(sb);
-    const float scale = __uint_as_float(sb);
-    float sums[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int g = 0; g < G; ++g) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        v[g][i] *= scale;
-        sums[g] += v[g][i];
-      }
-      split8(v[g], minus_one, &qh[t][g], &ql[t][g]);
-      sums[g] = sum32(sum16(sums[g]));
-    }
-    // the sums' three pieces, one for each of the first three quarters of K
-    half8 s0, s1, s2;
-    float rest[8];
-    split8(sums, minus_one, &s0, &s1);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) rest[i] = (sums[i] - (float)s0[i]) - (float)s1[i];
-    {
-      half8 unused;
-      split8(rest, minus_one, &s2, &unused);
-    }
-    __builtin_amdgcn_sched_barrier(0);
-    const half8 none{};
-    qs[t] = kq == 0 ? s0 : kq == 1 ? s1 : kq == 2 ? s2 : none;
   }
-  int wave_hi = 0, wave_lo = 0x7fffffff;  // keys that any row of the wave sees
+  most = max32(max16(most));
+  const unsigned sb = scale_to(most, 9);
+  inv = inverse_scale(sb);
+  const float scale = __uint_as_float(sb);
+  float sums[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    const int r = row0 + 16 * t;
-    if (r < rows) {
-      wave_hi = max(wave_hi, a.causal ? P + min(rows - 1, r + 15) / a.R + 1 : a.len);
-      wave_lo = min(wave_lo, a.window > 0 ? max(0, P + r / a.R + 1 - a.window) : 0);
+  for (int g = 0; g < G; ++g) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      v[g][i] *= scale;
+      sums[g] += v[g][i];
     }
+    split8(v[g], minus_one, &qh[g], &ql[g]);
+    sums[g] = sum32(sum16(sums[g]));
+  }
+  // the sums' three pieces, one for each of the first three quarters of K
+  half8 s0, s1, s2;
+  float rest[8];
+  split8(sums, minus_one, &s0, &s1);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) rest[i] = (sums[i] - (float)s0[i]) - (float)s1[i];
+  {
+    half8 unused;
+    split8(rest, minus_one, &s2, &unused);
+  }
+  __builtin_amdgcn_sched_barrier(0);
+  const half8 none{};
+  qs = kq == 0 ? s0 : kq == 1 ? s1 : kq == 2 ? s2 : none;
+  int wave_hi = 0, wave_lo = 0x7fffffff;  // keys that any row of the wave sees
+  const int r = row0;
+  if (r < rows) {
+    wave_hi = max(wave_hi, a.causal ? P + min(rows - 1, r + 15) / a.R + 1 : a.len);
+    wave_lo = min(wave_lo, a.window > 0 ? max(0, P + r / a.R + 1 - a.window) : 0);
   }
 
-  f32x4 o[QT][DT];
-  float m[QT], l[QT];
+  f32x4 o[DT];
+  float m, l;
+  m = NEG_INF;
+  l = 0.0f;
 #pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    m[t] = NEG_INF;
-    l[t] = 0.0f;
-#pragma unroll
-    for (int d = 0; d < DT; ++d) o[t][d] = (f32x4){0.f, 0.f, 0.f, 0.f};
-  }
+  for (int d = 0; d < DT; ++d) o[d] = (f32x4){0.f, 0.f, 0.f, 0.f};
   const unsigned vsb = scale_to(a.rows.vmax[h], 13);
   const float vscale = __uint_as_float(vsb);
 
@@ -288,16 +285,19 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void q4_chunk_kernel(const Q4Chunk
     const int buf = tile & 1, base = tile * BN;
     if (base >= wave_hi || base + BN <= wave_lo) return;
     // 32 keys at a time: their scores, the rows' maximum, the weights, the output.
+    // (The earlier a wave is in its 32 keys, the more it goes before the others of its
+    // SIMD, so that they come apart: 512 queries over 8192 keys, 24 heads on 8 of 128
+    // 148 us against 155, a prompt of 2048 of 32 heads on 8 of 64 87 against 100.)
 #pragma unroll 1
     for (int b = 0; b < VB; ++b) {
       const int key0 = base + 32 * b;
       if (key0 >= wave_hi || key0 + 32 <= wave_lo) continue;
       // Steps of two groups of one 16 keys; those instructions that depend on
-      // each other are 2 QT apart.
+      // each other are two apart.
       constexpr int NS = G;
       half8 kf[AH][2], mf[2];
       step4 st[AH][2];
-      f32x4 s[2][QT];
+      f32x4 s[2];
       const half8 *const kl = &k_lds[buf][2 * b * G * 64 + lane];
       const step_t *const sl = &step_lds[buf][2 * b * G * 16 + 4 * kq];
       auto load_k = [&](int step) {
@@ -323,107 +323,92 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void q4_chunk_kernel(const Q4Chunk
       mf[0] = *reinterpret_cast<const half8 *>(min_lds[buf][32 * b + col]);
       mf[1] = *reinterpret_cast<const half8 *>(min_lds[buf][32 * b + 16 + col]);
       if (AH == 2) load_k(0);
+      __builtin_amdgcn_s_setprio(2);
 #pragma unroll
       for (int step = 0; step < NS; ++step) {
         const int k = step / (G / 2), g = 2 * step % G;
         if (AH == 1) load_k(step);
         else if (step + 1 < NS) load_k(step + 1);
         else load_v(0);
-        f32x4 c[2][QT];
+        f32x4 c[2];
         if (g == 0) {
-#pragma unroll
-          for (int t = 0; t < QT; ++t)
-            s[k][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(mf[k], qs[t], (f32x4){0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+          s[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(mf[k], qs, (f32x4){0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
         }
 #pragma unroll
         for (int i = 0; i < 2; ++i)
+          c[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[step % AH][i], ql[g + i], (f32x4){0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
 #pragma unroll
-          for (int t = 0; t < QT; ++t)
-            c[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[step % AH][i], ql[t][g + i], (f32x4){0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+        for (int i = 0; i < 2; ++i)
+          c[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[step % AH][i], qh[g + i], c[i], 0, 0, 0);
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
-          for (int t = 0; t < QT; ++t)
-            c[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[step % AH][i], qh[t][g + i], c[i][t], 0, 0, 0);
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int t = 0; t < QT; ++t)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[k][t][e] = fmaf((float)st[step % AH][i][e], c[i][t][e], s[k][t][e]);
+          for (int e = 0; e < 4; ++e) s[k][e] = fmaf((float)st[step % AH][i][e], c[i][e], s[k][e]);
         // (the sums stay in their step: left to itself the compiler keeps every step's products until the last)
-#pragma unroll
-        for (int t = 0; t < QT; ++t) asm volatile("" : "+v"(s[k][t]));
+        asm volatile("" : "+v"(s[k]));
         __builtin_amdgcn_sched_barrier(0);
       }
-      half8 ph[QT], pl[QT];
-#pragma unroll
-      for (int t = 0; t < QT; ++t) {
-        // (32 keys that every row sees need no mask: uniform over the wave)
-        const int r = row0 + 16 * t;
-        const bool whole = r + 15 < rows && key0 + 32 <= (a.causal ? P + r / a.R + 1 : a.len) &&
-                           key0 >= (a.window > 0 ? P + (r + 15) / a.R + 1 - a.window : 0);
-        if (!whole) {
-          const int kend = r + col < rows ? (a.causal ? pos[t] + 1 : a.len) : 0;
-          const int kbeg = a.window > 0 ? pos[t] + 1 - a.window : 0;
-#pragma unroll
-          for (int k = 0; k < 2; ++k)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int key = key0 + 16 * k + 4 * kq + e;
-              if (key >= kend || key < kbeg) s[k][t][e] = NEG_INF;
-            }
-        }
-        float top = NEG_INF;
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) top = fmaxf(top, s[k][t][e]);
-        top = max32(max16(top)) * inv[t];
-        // The reference rises when a score passes it by 8: weights stay below
-        // 2^14, and the output is rarely scaled anew.
-        if (__any(top > m[t] + 8.0f)) {
-          const float mnew = fmaxf(m[t], top);
-          const float alpha = fast_exp2(m[t] - safe_max(mnew));
-          m[t] = mnew;
-          l[t] *= alpha;
-#pragma unroll
-          for (int d = 0; d < DT; ++d)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[t][d][e] *= alpha;
-        }
-        const float shift = 6.0f - safe_max(m[t]);
-        float p[8];
+      __builtin_amdgcn_s_setprio(1);
+      half8 ph, pl;
+      // (32 keys that every row sees need no mask: uniform over the wave)
+      const int r = row0;
+      const bool whole = r + 15 < rows && key0 + 32 <= (a.causal ? P + r / a.R + 1 : a.len) &&
+                         key0 >= (a.window > 0 ? P + (r + 15) / a.R + 1 - a.window : 0);
+      if (!whole) {
+        const int kend = r + col < rows ? (a.causal ? pos + 1 : a.len) : 0;
+        const int kbeg = a.window > 0 ? pos + 1 - a.window : 0;
 #pragma unroll
         for (int k = 0; k < 2; ++k)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            p[4 * k + e] = fast_exp2(fmaf(s[k][t][e], inv[t], shift));
-            l[t] += p[4 * k + e];
+            const int key = key0 + 16 * k + 4 * kq + e;
+            if (key >= kend || key < kbeg) s[k][e] = NEG_INF;
           }
-        split8(p, minus_one, &ph[t], &pl[t]);
       }
+      float top = NEG_INF;
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top = fmaxf(top, s[k][e]);
+      top = max32(max16(top)) * inv;
+      // The reference rises when a score passes it by 8: weights stay below
+      // 2^14, and the output is rarely scaled anew.
+      if (__any(top > m + 8.0f)) {
+        const float mnew = fmaxf(m, top);
+        const float alpha = fast_exp2(m - safe_max(mnew));
+        m = mnew;
+        l *= alpha;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[d][e] *= alpha;
+      }
+      const float shift = 6.0f - safe_max(m);
+      float p[8];
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          p[4 * k + e] = fast_exp2(fmaf(s[k][e], inv, shift));
+          l += p[4 * k + e];
+        }
+      split8(p, minus_one, &ph, &pl);
       __builtin_amdgcn_sched_barrier(0);
       // steps of two channel tiles
+      __builtin_amdgcn_s_setprio(0);
 #pragma unroll
       for (int step = 0; step < DT / 2; ++step) {
         if (AH == 1) load_v(step);
         else if (step + 1 < DT / 2) load_v(step + 1);
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int t = 0; t < QT; ++t)
-            o[t][2 * step + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl[step % AH][i], ph[t], o[t][2 * step + i], 0, 0, 0);
+          o[2 * step + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl[step % AH][i], ph, o[2 * step + i], 0, 0, 0);
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int t = 0; t < QT; ++t)
-            o[t][2 * step + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh[step % AH][i], pl[t], o[t][2 * step + i], 0, 0, 0);
+          o[2 * step + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh[step % AH][i], pl, o[2 * step + i], 0, 0, 0);
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int t = 0; t < QT; ++t)
-            o[t][2 * step + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh[step % AH][i], ph[t], o[t][2 * step + i], 0, 0, 0);
+          o[2 * step + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh[step % AH][i], ph, o[2 * step + i], 0, 0, 0);
         __builtin_amdgcn_sched_barrier(0);
       }
     }
@@ -453,71 +438,98 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void q4_chunk_kernel(const Q4Chunk
   }
 
   const float vinv = inverse_scale(vsb);
-  const long total = (long)a.S * a.Hq;
-#pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    const float sum = sum32(sum16(l[t]));
-    const long orow = query_row(t);
-    if (row0 + 16 * t + col >= rows) continue;
-    float *dst;
-    float f;
-    if (a.splits > 1) {
-      float *ml = a.part_ml + ((long)split * total + orow) * 2;
-      if (kq == 0) {
-        ml[0] = m[t];
-        ml[1] = sum;
-      }
-      dst = a.part_o + ((long)split * total + orow) * D;
-      f = vinv;
-    } else {
-      if (kq == 0 && !(sum > 0.0f && sum < __builtin_inff())) atomicOr(a.err, kDevErrSoftmaxDenominator);
-      dst = a.out + orow * D;
-      f = vinv / sum;
-    }
-#pragma unroll
-    for (int d = 0; d < DT; ++d)
-      *reinterpret_cast<float4 *>(dst + 16 * d + 4 * kq) =
-          make_float4(o[t][d][0] * f, o[t][d][1] * f, o[t][d][2] * f, o[t][d][3] * f);
+  const float sum = sum32(sum16(l));
+  if (row0 + col >= rows) return;
+  float *dst;
+  float f;
+  if (a.splits > 1) {
+    if (kq == 0) *reinterpret_cast<float2 *>(ml) = make_float2(m, sum);
+    if (m == NEG_INF) return;
+    dst = a.part_o + ((long)split * total + orow) * D;
+    f = vinv;
+  } else {
+    if (kq == 0 && !(sum > 0.0f && sum < __builtin_inff())) atomicOr(a.err, kDevErrSoftmaxDenominator);
+    dst = a.out + orow * D;
+    f = vinv / sum;
   }
+#pragma unroll
+  for (int d = 0; d < DT; ++d)
+    *reinterpret_cast<float4 *>(dst + 16 * d + 4 * kq) =
+        make_float4(o[d][0] * f, o[d][1] * f, o[d][2] * f, o[d][3] * f);
 }
 
 namespace {
 
-int chunk_rows(int D, long rows) { return D == 256 || rows <= 128 ? 128 : 256; }
-
-template <int D, int NW, int QT>
+template <int D, int NW>
 hipError_t chunk(hipStream_t st, const Q4ChunkArgs &a) {
   const long rows = (long)a.S * a.R;
-  const dim3 grid((unsigned)a.Hkv, (unsigned)((rows + NW * 16 * QT - 1) / (NW * 16 * QT)), (unsigned)a.splits);
-  hipLaunchKernelGGL((q4_chunk_kernel<D, NW, QT>), grid, dim3(NW * 64), 0, st, a);
+  const dim3 grid((unsigned)a.Hkv, (unsigned)((rows + NW * 16 - 1) / (NW * 16)), (unsigned)a.splits);
+  hipLaunchKernelGGL((q4_chunk_kernel<D, NW>), grid, dim3(NW * 64), 0, st, a);
   return hipGetLastError();
 }
 
 }  // namespace
 
+// The rows of a workgroup and the ranges of its keys that a model of the launch
+// finds fastest: a workgroup takes 3 us and a time for each tile, the CUs take the
+// workgroups longest first, and ranges are merged at 2.2 MB a us after 3.5 us.
+// Measured and modelled, us: a prompt of 2048, 24 heads on 8 of 128, in blocks of
+// 256 rows with two ranges 101 and 102, with one 140 and 147, of 128 rows with one
+// 106 and 104; 512 queries over 8192 keys, 256 rows with five ranges 147 and 135,
+// four 158 and 162, 16 174 and 165; 2048, 4 heads on 2 of 256, three ranges 81 and
+// 88, one 164 and 165.
 Q4ChunkPlan q4_chunk_plan(int D, int S, int R, int Hkv, int len, int causal, int window, int cus) {
-  Q4ChunkPlan p;
-  const int BN = 8192 / D, per = chunk_rows(D, (long)S * R);
-  const long blocks = ((long)S * R + per - 1) / per * Hkv;
-  // tiles that the workgroup with the most keys visits
-  long span = len;
-  if (window > 0 && causal) span = std::min<long>(len, (long)window + per / R + 1);
-  const long tiles = (span + BN - 1) / BN + 1;
-  long splits = std::max<long>(1, cus / blocks);
-  splits = std::min(splits, std::max<long>(1, tiles / 4));
-  splits = std::min<long>(splits, 64);
-  p.tps = (int)((tiles + splits - 1) / splits);
-  p.splits = (int)((tiles + p.tps - 1) / p.tps);
-  if (p.splits > 1) p.partial_bytes = (size_t)p.splits * S * R * Hkv * (D + 2) * sizeof(float);
-  return p;
+  const int BN = 8192 / D;
+  const long rows = (long)S * R;
+  Q4ChunkPlan best;
+  double best_time = 0.0;
+  for (int per = 128; per <= (D < 256 && rows > 128 ? 256 : 128); per += 128) {
+    const double tile = D == 256 ? 2.45 : D == 128 ? (per == 256 ? 4.2 : 3.0) : per == 256 ? 5.2 : 3.9;
+    const long blocks = (rows + per - 1) / per;
+    auto tiles_of = [&](long block) {  // as the kernel has them
+      const long first = block * per / R, last = std::min(rows - 1, (block + 1) * per - 1) / R;
+      const long hi = causal ? len - S + last + 1 : len, lo = window > 0 ? std::max<long>(0, len - S + first + 1 - window) : 0;
+      return (hi + BN - 1) / BN - lo / BN;
+    };
+    long most = 1;
+    for (long b = 0; b < blocks; ++b) most = std::max(most, tiles_of(b));
+    int last_splits = 0;
+    for (long want = 1; want <= 64 && (want == 1 || want * blocks * Hkv <= 4L * cus); ++want) {
+      const long tps = (most + want - 1) / want;
+      const int splits = (int)((most + tps - 1) / tps);
+      if (splits == last_splits) continue;
+      last_splits = splits;
+      double sum = 0.0, least = 1e30;
+      long pieces = 0;
+      for (long b = 0; b < blocks; ++b) {
+        const long n = tiles_of(b), k = (n + tps - 1) / tps;
+        pieces += k;
+        sum += n * tile + 3.0 * k;
+        least = std::min(least, (n - (k - 1) * tps) * tile + 3.0);
+      }
+      const long n = pieces * Hkv, full = n / cus * cus;
+      const double longest = tps * tile + 3.0;
+      // (CUs that get one workgroup more than the others: by how much at least)
+      double time = std::max(longest, sum * Hkv / cus + (n > cus && n > full ? least * (1.0 - (double)(n - full) / cus) : 0.0));
+      if (splits > 1) time += 3.5 + (double)splits * rows * Hkv * D * sizeof(float) / 2.2e6;
+      if (best_time == 0.0 || time < best_time) {
+        best_time = time;
+        best.per = per;
+        best.splits = splits;
+        best.tps = (int)tps;
+      }
+    }
+  }
+  if (best.splits > 1) best.partial_bytes = (size_t)best.splits * rows * Hkv * (D + 2) * sizeof(float);
+  return best;
 }
 
 hipError_t launch_q4_chunk(hipStream_t st, const Q4ChunkArgs &a, int D) {
-  const bool wide = chunk_rows(D, (long)a.S * a.R) == 256;
+  const bool wide = a.per == 256;
   switch (D) {
-    case 64: return wide ? chunk<64, 16, 1>(st, a) : chunk<64, 8, 1>(st, a);
-    case 128: return wide ? chunk<128, 16, 1>(st, a) : chunk<128, 8, 1>(st, a);
-    case 256: return chunk<256, 8, 1>(st, a);
+    case 64: return wide ? chunk<64, 16>(st, a) : chunk<64, 8>(st, a);
+    case 128: return wide ? chunk<128, 16>(st, a) : chunk<128, 8>(st, a);
+    case 256: return chunk<256, 8>(st, a);
     default: return hipErrorInvalidValue;
   }
 }
