@@ -1503,6 +1503,14 @@ static Q4ChunkPlan q4_chunk_plan_of(spissa_session *s, size_t len, const spissa_
   return q4_chunk_plan((int)c->head_dim, (int)c->query_len, (int)(c->num_heads / c->kv_heads), (int)c->kv_heads, (int)len,
                        c->causal ? 1 : 0, (int)c->window, s->cus);
 }
+// (the blocks of 128 rows of a head are the grid's second dimension)
+static int q4_chunk_limit(const spissa_kv_attention_config *c) {
+  const size_t most = 65535 * (size_t)128;
+  if (c->query_len > most / (c->num_heads / c->kv_heads))
+    return set_err(SPISSA_ERR_SHAPE, "%zu queries of %zu heads a KV head over a 4-bit cache: more than %zu rows a head",
+                   c->query_len, c->num_heads / c->kv_heads, most);
+  return SPISSA_OK;
+}
 static int q4_chunk_prepare(spissa_session *s, size_t len, const spissa_kv_attention_config *c) {
   const Q4ChunkPlan p = q4_chunk_plan_of(s, len, c);
   return p.partial_bytes ? ensure_buf(s, s->ppart, p.partial_bytes) : SPISSA_OK;
@@ -1552,6 +1560,7 @@ static int q4_validate_step(spissa_session *s, const spissa_rope_table *table, c
   for (size_t b = 0; b < batch; ++b) {
     if (!caches[b]->q4) return set_err(SPISSA_ERR_ARGUMENT, "a step takes f32 caches or 4-bit caches, not both");
     ST_TRY(validate_attention(0, 0, 0, caches[b], cfg, false));
+    ST_TRY(q4_chunk_limit(cfg));
     size_t n, nl;  // rotary.rs:227-251: the append must fit before anything runs
     ST_TRY(kv_validate_append(caches[b], 0, 0, cfg->query_len, false, &n, &nl));
     if (caches[b]->session->device != s->device)
@@ -1911,6 +1920,7 @@ extern "C" int spissa_attention_cached_device(spissa_session *s, const float *d_
     if (!d_q || !d_out) return set_err(SPISSA_ERR_ARGUMENT, "null buffer");
     if (!(aligned16(d_q) && aligned16(d_out)))
       return set_err(SPISSA_ERR_ARGUMENT, "attention over a 4-bit cache takes 16-byte aligned buffers");
+    ST_TRY(q4_chunk_limit(cfg));
     HIP_TRY(hipSetDevice(s->device));
     if (S == 1) return q4_attend_batch(s, d_q, &cache, 1, cfg, d_out, 0);
     ST_TRY(q4_chunk_prepare(s, cache->len, cfg));

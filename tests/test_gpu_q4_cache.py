@@ -503,3 +503,18 @@ def test_refusals(ses):
     assert len(c) == 10 and len(full) == 3 and len(empty) == 0
     assert not c.device_keys_ptr() and not c.device_values_ptr()
     ses.sync()
+
+
+def test_more_rows_than_a_launch_takes(ses):
+    """Refused before anything runs: the small tensors are never read."""
+    n, t = 140000, torch.zeros(64, device="cuda")
+    c = ses.q4_kv_cache(1, 64, n)
+    cfg = KvAttentionConfig(n, 64, 1, 64, True)
+    with pytest.raises(sa.ShapeError):
+        ses.prefill_step(None, t, t, t, c, cfg, t)
+    assert len(c) == 0
+    k = torch.zeros(n, 64, device="cuda")
+    ses.append(c, k, k, n)
+    with pytest.raises(sa.ShapeError):
+        ses.attention_cached(t, c, cfg, t)
+    ses.sync()
