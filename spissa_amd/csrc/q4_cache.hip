@@ -78,26 +78,43 @@ __device__ __forceinline__ void words(const char *p, unsigned (&w)[N]) {
   }
 }
 
-// A key word's eight codes as slots: channels 0, 4, 1, 5, 2, 6, 3, 7, as code 2^-24
-// (0, 4, 2, 6) or code 2^-20.
-__device__ __forceinline__ half8 code_slots(unsigned w) {
-  const unsigned u = w >> 8;
-  const uint4 r = make_uint4(w & 0x000f000fu, w & 0x00f000f0u, u & 0x000f000fu, u & 0x00f000f0u);
-  return __builtin_bit_cast(half8, r);
+// (code - 8) 2^-9 twice. A code in bits 0..3 of a binary16 is code 2^-24, in bits
+// 4..7 code 2^-20, so a packed FMA makes it an ordinary number and takes the 8 off.
+struct Slots {
+  half2v from0, from4, offset;  // (in registers: the compiler does not know them)
+  __device__ __forceinline__ Slots() {
+    unsigned a = 0x78007800u, b = 0x68006800u, c = 0xa400a400u;  // 2^15, 2^11, -2^-6
+    asm volatile("" : "+v"(a), "+v"(b), "+v"(c));
+    from0 = __builtin_bit_cast(half2v, a);
+    from4 = __builtin_bit_cast(half2v, b);
+    offset = __builtin_bit_cast(half2v, c);
+  }
+  __device__ __forceinline__ half2v low(unsigned w) const {
+    return __builtin_elementwise_fma(__builtin_bit_cast(half2v, w & 0x000f000fu), from0, offset);
+  }
+  __device__ __forceinline__ half2v high(unsigned w) const {
+    return __builtin_elementwise_fma(__builtin_bit_cast(half2v, w & 0x00f000f0u), from4, offset);
+  }
+};
+__device__ __forceinline__ half8 join(half2v a, half2v b, half2v c, half2v d) {
+  return (half8){a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
 }
-// The codes of channel n of a lane's CH of eight rows, as code 2^-24 (n even) or
-// code 2^-20. (The compiler shares what the channels of a half word have in common.)
+// A key word's eight codes as slots: channels 0, 4, 1, 5, 2, 6, 3, 7.
+__device__ __forceinline__ half8 code_slots(unsigned w, const Slots &s) {
+  return join(s.low(w), s.high(w), s.low(w >> 8), s.high(w >> 8));
+}
+// The codes of channel n of a lane's CH of eight rows. (The compiler shares what the
+// channels of a half word have in common.)
 template <int CH, int N>
-__device__ __forceinline__ half8 value_slots(const unsigned (&v)[8][N], int n) {
-  unsigned r[4];
+__device__ __forceinline__ half8 value_slots(const unsigned (&v)[8][N], int n, const Slots &s) {
+  half2v r[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const unsigned w0 = v[2 * i][n / 8], w1 = v[2 * i + 1][n / 8];
     const unsigned u = __builtin_amdgcn_perm(w1, w0, n & 4 ? 0x07060302u : 0x05040100u);
-    r[i] = (n & 2 ? u >> 8 : u) & (n & 1 ? 0x00f000f0u : 0x000f000fu);
+    r[i] = n & 1 ? s.high(n & 2 ? u >> 8 : u) : s.low(n & 2 ? u >> 8 : u);
   }
-  const uint4 q = make_uint4(r[0], r[1], r[2], r[3]);
-  return __builtin_bit_cast(half8, q);
+  return join(r[0], r[1], r[2], r[3]);
 }
 
 // The key of 32 in slot i of a lane's eight, above the 4 (lane / 16) that the lanes differ by.
@@ -297,21 +314,22 @@ __device__ __forceinline__ void visible(const Q4AttnArgsOf<MB> &a, int z, int *l
 // 16 / G heads x G groups: column (q, g) of the queries has q's channels of group
 // g and zeros elsewhere, so one accumulator gathers sum_g-channels q code for
 // every (q, g), and a lane, whose column is one (q, g), adds its group's
-//   step * that sum + min * sum_g q
+//   step * that sum + (min + 8 step) * sum_g q
 // for its four keys of 16; the groups' lanes add up to the score. Its weights
 // times its group's steps of the values are row (q, g) of the other product
 // at once, P' V: a column holds channels of one group, and takes its output from
-// that group's rows. min p goes beside it as one sum a (q, g).
+// that group's rows. (min + 8 step) p goes beside it as one sum a (q, g).
 // A lane takes codes in whole words: of a key, the k slots of its quarter are a
 // quarter of the row; of the values, a column is D / 16 consecutive channels,
-// one a product. Codes are operands as they come out of a word: a code in bits
-// 0..3 of a binary16 is code 2^-24, in bits 4..7 code 2^-20, exactly, and the
-// matrix instructions take such numbers as they are; the factor is taken off the
-// queries' slots and the output. Queries and weights are two binary16 pieces.
+// one a product. Operands are code - 8 (times 2^-9), with min + 8 step beside them:
+// with the codes as they are, the sums of many keys' values would grow, and cancel
+// against the minima's only at the end (outputs over 8192 keys were 1e-6 off).
+// Queries and weights are two binary16 pieces.
 // Bound: HBM for many keys, latency (one step of loads, one of sums) for few.
-// 16 sequences of 8192 keys, 24 heads on 8 of 128: 40 us, 4.1 TB/s of codes and
+// 16 sequences of 8192 keys, 24 heads on 8 of 128: 44 us, 3.8 TB/s of codes and
 // params (a copy reaches 5.1); 32768 keys of one head of 256: 12 us; 512 keys, 32
-// heads on 8 of 64: 5.6 us.
+// heads on 8 of 64: 6 us. Outputs are 1.2e-7 off (RMS, relative), as a plain f32
+// form's are.
 template <int D, int MB>
 __global__ __launch_bounds__(64 * kQ4Waves) void q4_attend_kernel(const Q4AttnArgsOf<MB> a) {
   constexpr int G = D / 32, NQ = 16 / G, CH = D / 16, ENTRY = NQ * (D + 2);
@@ -378,18 +396,19 @@ __global__ __launch_bounds__(64 * kQ4Waves) void q4_attend_kernel(const Q4AttnAr
   const unsigned sb = scale_to(most, 13);
   y *= __uint_as_float(sb);
   {
-    const float sum = group_sum<32>(y);
-    if (ch % 32 == 0) q_sum[r][ch / 32] = sum;
-    if (ch % D == 0) q_inv[r] = inverse_scale(sb);
-    const float slot = y * (ch & 1 ? 0x1p-4f : 1.0f);
-    const _Float16 hi_piece = pieces2(slot, 0.0f).x;
+    const _Float16 first = pieces2(y, 0.0f).x, second = pieces2(y - (float)first, 0.0f).x;
     const int at = (ch & ~7) + (ch & 3) * 2 + (ch >> 2 & 1);
-    q_lds[0][r][at] = hi_piece;
-    q_lds[1][r][at] = pieces2(slot - (float)hi_piece, 0.0f).x;
+    q_lds[0][r][at] = first;
+    q_lds[1][r][at] = second;
+    const float sum = group_sum<32>((float)first + (float)second);
+    if (ch % 32 == 0) q_sum[r][ch / 32] = sum;
+    if (ch == 0) q_inv[r] = inverse_scale(sb);
   }
   __syncthreads();
   half8 qh[G], ql[G];
-  const float inv = q_inv[col % NQ], qsum = q_sum[col % NQ][g];
+  // (scores are held as 1 / inv of what they are)
+  const float inv = q_inv[col % NQ], qsum = q_sum[col % NQ][g], qsum8 = 8.0f * qsum;
+  const Slots slots;
   float minus_one = -1.0f;
   asm volatile("" : "+v"(minus_one));
 #pragma unroll
@@ -418,14 +437,14 @@ __global__ __launch_bounds__(64 * kQ4Waves) void q4_attend_kernel(const Q4AttnAr
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         if (j == 0) sum[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
-        const half8 kf = code_slots(kw[i][j]);
+        const half8 kf = code_slots(kw[i][j], slots);
         sum[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[j], sum[i], 0, 0, 0);
         sum[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[j], sum[i], 0, 0, 0);
       }
     float s[8], top = NEG_INF;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float y = fmaf(half_lo(kpw[i]), sum[i >> 2][i & 3] * 0x1p24f, half_hi(kpw[i]) * qsum);
+      const float y = fmaf(half_lo(kpw[i]), fmaf(sum[i >> 2][i & 3], 512.0f, qsum8), half_hi(kpw[i]) * qsum);
       s[i] = groups_sum<NQ>(y);
     }
     if (more) load_k(c + kQ4Step);
@@ -461,13 +480,13 @@ __global__ __launch_bounds__(64 * kQ4Waves) void q4_attend_kernel(const Q4AttnAr
       const float w = fast_exp2(fmaf(s[i], inv, shift));
       l += w;
       p[i] = w * half_lo(vpw[i]);
-      omin = fmaf(w, half_hi(vpw[i]), omin);
+      omin = fmaf(w, fmaf(half_lo(vpw[i]), 8.0f, half_hi(vpw[i])), omin);
     }
     half8 ph, pl;
     split8(p, minus_one, &ph, &pl);
 #pragma unroll
     for (int n = 0; n < CH; ++n) {
-      const half8 vf = value_slots<CH>(vw, n);
+      const half8 vf = value_slots<CH>(vw, n, slots);
       o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl, vf, o[n], 0, 0, 0);
       o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph, vf, o[n], 0, 0, 0);
     }
@@ -482,7 +501,7 @@ __global__ __launch_bounds__(64 * kQ4Waves) void q4_attend_kernel(const Q4AttnAr
     const float least = __shfl(omin, row);
     if (row / NQ == g)
 #pragma unroll
-      for (int n = 0; n < CH; ++n) red_o[wave][row % NQ][col * CH + n] = fmaf(o[n][e], n & 1 ? 0x1p20f : 0x1p24f, least);
+      for (int n = 0; n < CH; ++n) red_o[wave][row % NQ][col * CH + n] = fmaf(o[n][e], 512.0f, least);
   }
   if (lane < NQ) {
     red_l[wave][lane] = l;
