@@ -1465,9 +1465,14 @@ static size_t q4_partial_bytes(size_t n, size_t Hq, size_t D, const Q4AttnPlan &
 }
 
 // One query of each of B sequences, whose own row is its cache's last.
-// extra: rows that the caches hold beyond their lengths (1 in a fused step).
+// With `step` (its rows k and v, table and norm) the launch appends those rows first.
+struct Q4StepRows {
+  const float *k, *v;
+  const spissa_rope_table *table;
+  const GemmaQkNorm *norm;
+};
 static int q4_attend_batch(spissa_session *s, const float *q, const spissa_kv_cache *const *caches, size_t batch,
-                           const spissa_kv_attention_config *c, float *out, size_t extra) {
+                           const spissa_kv_attention_config *c, float *out, const Q4StepRows *step) {
   const int D = (int)c->head_dim, Hq = (int)c->num_heads, Hkv = (int)c->kv_heads, R = Hq / Hkv;
   for (size_t b0 = 0; b0 < batch; b0 += kMaxDecodeBatch) {
     const int B = (int)std::min<size_t>(kMaxDecodeBatch, batch - b0);
@@ -1475,7 +1480,7 @@ static int q4_attend_batch(spissa_session *s, const float *q, const spissa_kv_ca
     int keys[kMaxDecodeBatch];
     for (int b = 0; b < B; ++b) {
       a.seq[b].rows = q4_rows(caches[b0 + b], 0);
-      a.seq[b].len = (int)(caches[b0 + b]->len + extra);
+      a.seq[b].len = (int)(caches[b0 + b]->len + (step ? 1 : 0));
       keys[b] = c->window ? (int)std::min<size_t>(a.seq[b].len, c->window) : a.seq[b].len;
     }
     const Q4AttnPlan p = q4_attend_plan(D, R, Hkv, keys, B);
@@ -1492,6 +1497,18 @@ static int q4_attend_batch(spissa_session *s, const float *q, const spissa_kv_ca
     a.kps = p.kps;
     a.max_splits = p.splits;
     a.qscale = (1.0f / sqrtf((float)D)) * 1.4426950408889634f;
+    if (step) {
+      a.k = step->k + b0 * (size_t)Hkv * D;
+      a.v = step->v + b0 * (size_t)Hkv * D;
+      a.cos = step->table ? step->table->cos : nullptr;
+      a.sin = step->table ? step->table->sin : nullptr;
+      if (step->norm) {
+        a.q_norm = step->norm->q_norm;
+        a.k_norm = step->norm->k_norm;
+        a.eps = step->norm->eps;
+        a.prescale = step->norm->q_prescale;
+      }
+    }
     HIP_TRY(launch_q4_attend(s->stream, a, D, B));
   }
   return SPISSA_OK;
@@ -1593,26 +1610,25 @@ static int q4_step(spissa_session *s, const spissa_rope_table *table, const floa
     return set_err(SPISSA_ERR_ARGUMENT, "a step on a 4-bit cache takes 16-byte aligned norms");
   HIP_TRY(hipSetDevice(s->device));
   const size_t S = cfg->query_len;
-  const float *q = d_q;
-  if (table || norm) {
-    ST_TRY(ensure_buf(s, s->q4q, batch * S * cfg->num_heads * cfg->head_dim * sizeof(float)));
-    q = (const float *)s->q4q.p;
-  }
   // (workspaces before the first launch: nothing is appended by a call that fails for want of them)
   if (S == 1) {
     const int one = 1;
     const Q4AttnPlan p = q4_attend_plan((int)cfg->head_dim, (int)(cfg->num_heads / cfg->kv_heads), (int)cfg->kv_heads, &one, 1);
     ST_TRY(ensure_buf(s, s->partial,
                       q4_partial_bytes(std::min<size_t>(batch, kMaxDecodeBatch), cfg->num_heads, cfg->head_dim, p, cfg->kv_heads)));
+    const Q4StepRows rows{d_k, d_v, table, norm};
+    ST_TRY(q4_attend_batch(s, d_q, caches, batch, cfg, d_out, &rows));
   } else {
+    const float *q = d_q;
+    if (table || norm) {
+      ST_TRY(ensure_buf(s, s->q4q, S * cfg->num_heads * cfg->head_dim * sizeof(float)));
+      q = (const float *)s->q4q.p;
+    }
     ST_TRY(q4_chunk_prepare(s, caches[0]->len + S, cfg));
-  }
-  ST_TRY(q4_append(s, caches, batch, S, q == d_q ? nullptr : d_q, cfg->num_heads, d_k, d_v, table, norm,
-                   const_cast<float *>(q)));
-  if (S == 1)
-    ST_TRY(q4_attend_batch(s, q, caches, batch, cfg, d_out, 1));
-  else
+    ST_TRY(q4_append(s, caches, 1, S, q == d_q ? nullptr : d_q, cfg->num_heads, d_k, d_v, table, norm,
+                     const_cast<float *>(q)));
     ST_TRY(q4_attend_chunk(s, q, caches[0], caches[0]->len + S, cfg, d_out));
+  }
   for (size_t b = 0; b < batch; ++b) caches[b]->len += S;
   return SPISSA_OK;
 }
@@ -1922,7 +1938,7 @@ extern "C" int spissa_attention_cached_device(spissa_session *s, const float *d_
       return set_err(SPISSA_ERR_ARGUMENT, "attention over a 4-bit cache takes 16-byte aligned buffers");
     ST_TRY(q4_chunk_limit(cfg));
     HIP_TRY(hipSetDevice(s->device));
-    if (S == 1) return q4_attend_batch(s, d_q, &cache, 1, cfg, d_out, 0);
+    if (S == 1) return q4_attend_batch(s, d_q, &cache, 1, cfg, d_out, nullptr);
     ST_TRY(q4_chunk_prepare(s, cache->len, cfg));
     return q4_attend_chunk(s, d_q, cache, cache->len, cfg, d_out);
   }
@@ -1969,7 +1985,7 @@ extern "C" int spissa_attention_cached_batch_device(spissa_session *s, const flo
   if (!(aligned16(d_q) && aligned16(d_out)))
     return set_err(SPISSA_ERR_ARGUMENT, "attention over a 4-bit cache takes 16-byte aligned buffers");
   HIP_TRY(hipSetDevice(s->device));
-  return q4_attend_batch(s, d_q, caches, batch, cfg, d_out, 0);
+  return q4_attend_batch(s, d_q, caches, batch, cfg, d_out, nullptr);
   GUARD_END
 }
 

@@ -366,6 +366,11 @@ struct Q4AttnBase {
   int *err;
   int Hq, Hkv, R, HB, window, kps, max_splits;
   float qscale;     // softmax scale * log2(e)
+  // A fused step: the tokens' rows k, v [B, Hkv, D], which the launch prepares as
+  // Q4AppendArgs has them, q too, and appends as the caches' last rows. Null k: the
+  // caches hold them, and q is as it is.
+  const float *k, *v, *cos, *sin, *q_norm, *k_norm;
+  float eps, prescale;
 };
 struct Q4Seq {
   Q4Rows rows;

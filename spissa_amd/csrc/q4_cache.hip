@@ -190,13 +190,64 @@ __device__ __forceinline__ float hold32(const float4 x, bool store, bool first, 
   return fmaxf(fabsf(min), fabsf(min + 15.0f * step));
 }
 
+// What a fused step does to query and key rows before they are used or held.
+struct RowPrep {
+  const float *cos, *sin;        // RoPE table rows by position, or null
+  const float *q_norm, *k_norm;  // QK-norm, null: none
+  float eps, prescale;
+};
+// A row over D/8 lanes, of which lane `sub` has channels [4 sub, 4 sub + 4) and
+// [D/2 + 4 sub, ...): rotate-half partners, and eight consecutive lanes hold 32
+// consecutive channels of either half.
+template <int D>
+__device__ __forceinline__ void prepare_row(const RowPrep &a, bool is_q, bool is_v, int pos, int sub, float4 &x0, float4 &x1) {
+#pragma clang fp contract(off)
+  constexpr int HALF = D / 2;
+  if (a.q_norm) {
+    float ss = (x0.x * x0.x + x0.y * x0.y) + (x0.z * x0.z + x0.w * x0.w);
+    ss += (x1.x * x1.x + x1.y * x1.y) + (x1.z * x1.z + x1.w * x1.w);
+    ss = group_sum<D / 8>(ss);
+    const float inv = 1.0f / sqrtf(ss / (float)D + a.eps);
+    const float *nw = is_q ? a.q_norm : a.k_norm;
+    const float4 w0 = *reinterpret_cast<const float4 *>(nw + 4 * sub);
+    const float4 w1 = *reinterpret_cast<const float4 *>(nw + HALF + 4 * sub);
+    if (!is_v) {
+      x0 = make_float4(x0.x * inv * w0.x, x0.y * inv * w0.y, x0.z * inv * w0.z, x0.w * inv * w0.w);
+      x1 = make_float4(x1.x * inv * w1.x, x1.y * inv * w1.y, x1.z * inv * w1.z, x1.w * inv * w1.w);
+    }
+  }
+  if (a.cos && !is_v) {
+    const float4 c = *reinterpret_cast<const float4 *>(a.cos + (long)pos * HALF + 4 * sub);
+    const float4 s = *reinterpret_cast<const float4 *>(a.sin + (long)pos * HALF + 4 * sub);
+    rotate_pair(x0.x, x1.x, c.x, s.x);
+    rotate_pair(x0.y, x1.y, c.y, s.y);
+    rotate_pair(x0.z, x1.z, c.z, s.z);
+    rotate_pair(x0.w, x1.w, c.w, s.w);
+  }
+  if (a.q_norm && is_q) {
+    x0 = make_float4(x0.x * a.prescale, x0.y * a.prescale, x0.z * a.prescale, x0.w * a.prescale);
+    x1 = make_float4(x1.x * a.prescale, x1.y * a.prescale, x1.z * a.prescale, x1.w * a.prescale);
+  }
+}
+// ... and into codes: every lane takes part in the exchanges, those with `store`
+// write. Returns the row's largest |value| in every lane (a bound).
+template <int D>
+__device__ __forceinline__ float hold_row(const float4 &x0, const float4 &x1, int sub, bool store, unsigned char *codes,
+                                          unsigned *params, bool *bad) {
+  constexpr int LPR = D / 8;
+  float big = hold32(x0, store, (sub & 7) == 0, codes + 2 * sub, params + sub / 8, bad);
+  big = fmaxf(big, hold32(x1, store, (sub & 7) == 0, codes + D / 4 + 2 * sub, params + D / 64 + sub / 8, bad));
+  big = max8(big);
+  if constexpr (LPR >= 16) big = fmaxf(big, dpp<0x140>(big));
+  if constexpr (LPR >= 32) big = max16(big);
+  return big;
+}
+
 }  // namespace
 
 // Appends the rows of S tokens of each sequence (blockIdx.z): keys QK-normed
 // and rotated, values as they are; with Hq > 0 the query rows too, normed,
-// rotated and prescaled into q_out. A row is spread over D/8 lanes, each with
-// channels [4 s, 4 s + 4) and [D/2 + 4 s, ...): rotate-half partners, and eight
-// consecutive lanes hold 32 consecutive channels of either half.
+// rotated and prescaled into q_out.
 // Bound: HBM (reads 8 bytes and writes 1.25 for a channel of K and V).
 template <int D>
 __global__ __launch_bounds__(256) void q4_append_kernel(const Q4AppendArgs a) {
@@ -217,34 +268,7 @@ __global__ __launch_bounds__(256) void q4_append_kernel(const Q4AppendArgs a) {
   const float *src = is_q ? a.q + (t * a.Hq + h) * D : (is_v ? a.v : a.k) + (t * a.Hkv + h) * D;
   float4 x0 = *reinterpret_cast<const float4 *>(src + 4 * sub);
   float4 x1 = *reinterpret_cast<const float4 *>(src + HALF + 4 * sub);
-  {
-#pragma clang fp contract(off)
-    if (a.q_norm) {
-      float ss = (x0.x * x0.x + x0.y * x0.y) + (x0.z * x0.z + x0.w * x0.w);
-      ss += (x1.x * x1.x + x1.y * x1.y) + (x1.z * x1.z + x1.w * x1.w);
-      ss = group_sum<LPR>(ss);
-      const float inv = 1.0f / sqrtf(ss / (float)D + a.eps);
-      const float *nw = is_q ? a.q_norm : a.k_norm;
-      const float4 w0 = *reinterpret_cast<const float4 *>(nw + 4 * sub);
-      const float4 w1 = *reinterpret_cast<const float4 *>(nw + HALF + 4 * sub);
-      if (!is_v) {
-        x0 = make_float4(x0.x * inv * w0.x, x0.y * inv * w0.y, x0.z * inv * w0.z, x0.w * inv * w0.w);
-        x1 = make_float4(x1.x * inv * w1.x, x1.y * inv * w1.y, x1.z * inv * w1.z, x1.w * inv * w1.w);
-      }
-    }
-    if (a.cos && !is_v) {
-      const float4 c = *reinterpret_cast<const float4 *>(a.cos + (long)pos * HALF + 4 * sub);
-      const float4 s = *reinterpret_cast<const float4 *>(a.sin + (long)pos * HALF + 4 * sub);
-      rotate_pair(x0.x, x1.x, c.x, s.x);
-      rotate_pair(x0.y, x1.y, c.y, s.y);
-      rotate_pair(x0.z, x1.z, c.z, s.z);
-      rotate_pair(x0.w, x1.w, c.w, s.w);
-    }
-    if (a.q_norm && is_q) {
-      x0 = make_float4(x0.x * a.prescale, x0.y * a.prescale, x0.z * a.prescale, x0.w * a.prescale);
-      x1 = make_float4(x1.x * a.prescale, x1.y * a.prescale, x1.z * a.prescale, x1.w * a.prescale);
-    }
-  }
+  prepare_row<D>({a.cos, a.sin, a.q_norm, a.k_norm, a.eps, a.prescale}, is_q, is_v, pos, sub, x0, x1);
   if (is_q && live) {
     float *dst = a.q_out + (t * a.Hq + h) * D;
     *reinterpret_cast<float4 *>(dst + 4 * sub) = x0;
@@ -256,14 +280,10 @@ __global__ __launch_bounds__(256) void q4_append_kernel(const Q4AppendArgs a) {
   unsigned *param = (is_v ? seq.vp : seq.kp) + at_row * (D / 32);
   const bool keep = live && !is_q;
   bool bad = false;
-  float big = hold32(x0, keep, (sub & 7) == 0, codes + 2 * sub, param + sub / 8, &bad);
-  big = fmaxf(big, hold32(x1, keep, (sub & 7) == 0, codes + HALF / 2 + 2 * sub, param + D / 64 + sub / 8, &bad));
+  const float big = hold_row<D>(x0, x1, sub, keep, codes, param, &bad);
   if (keep && bad) atomicOr(a.err, kDevErrCacheValue);
   // The head's largest |value| (a bound: it never shrinks), which scales the
-  // 16-bit pieces of the chunk attention's values. Positive floats order as integers.
-  big = max8(big);
-  if constexpr (LPR >= 16) big = fmaxf(big, dpp<0x140>(big));
-  if constexpr (LPR >= 32) big = max16(big);
+  // 16-bit pieces of the attention's values. Positive floats order as integers.
   if (keep && is_v && sub == 0 && big > seq.vmax[h])
     atomicMax(reinterpret_cast<int *>(seq.vmax + h), __float_as_int(big));
 }
@@ -330,7 +350,12 @@ __device__ __forceinline__ void visible(const Q4AttnArgsOf<MB> &a, int z, int *l
 // params (a copy reaches 5.1); 32768 keys of one head of 256: 12 us; 512 keys, 32
 // heads on 8 of 64: 6 us. Outputs are 1.2e-7 off (RMS, relative), as a plain f32
 // form's are.
-template <int D, int MB>
+// STEP: the fused step of one token. Every workgroup prepares its queries and
+// holds the sequence's new row of its head in LDS (as q4_append_kernel does, bit for
+// bit), and takes that row from there; the one with the last range and the first heads
+// writes it. A step over 512 keys, 32 heads on 8 of 64, with its rows read back: 18.2 us
+// with a launch of q4_append_kernel before, 14.7 without.
+template <int D, int MB, bool STEP>
 __global__ __launch_bounds__(64 * kQ4Waves) void q4_attend_kernel(const Q4AttnArgsOf<MB> a) {
   constexpr int G = D / 32, NQ = 16 / G, CH = D / 16, ENTRY = NQ * (D + 2);
   __shared__ float red_o[kQ4Waves][NQ][D];
@@ -338,6 +363,10 @@ __global__ __launch_bounds__(64 * kQ4Waves) void q4_attend_kernel(const Q4AttnAr
   __shared__ _Float16 q_lds[2][NQ][D + 8] __attribute__((aligned(16)));
   __shared__ float q_sum[NQ][G], q_inv[NQ];
   static_assert(NQ * D == 64 * kQ4Waves, "a thread a channel of the queries");
+  __shared__ __attribute__((aligned(16))) float q_row[STEP ? NQ : 1][D];
+  __shared__ __attribute__((aligned(16))) unsigned char new_codes[2][D / 2];
+  __shared__ unsigned new_params[2][G];
+  __shared__ float new_big;
 
   const int z = blockIdx.z, hb = blockIdx.x % a.HB, h = blockIdx.x / a.HB, split = blockIdx.y;
   int lo, hi;
@@ -380,10 +409,35 @@ __global__ __launch_bounds__(64 * kQ4Waves) void q4_attend_kernel(const Q4AttnAr
     load_v(c);
   }
 
+  if constexpr (STEP) {
+    constexpr int LPR = D / 8;
+    const int sub = lane % LPR, r = lane / LPR, pos = hi - 1;
+    const RowPrep prep{a.cos, a.sin, a.q_norm, a.k_norm, a.eps, a.prescale};
+    if (wave == 0) {  // its 64 lanes are NQ rows
+      const float *src = a.q + ((long)z * a.Hq + h * a.R + min(hb * NQ + r, a.R - 1)) * D + 4 * sub;
+      float4 x0 = *reinterpret_cast<const float4 *>(src), x1 = *reinterpret_cast<const float4 *>(src + D / 2);
+      prepare_row<D>(prep, true, false, pos, sub, x0, x1);
+      *reinterpret_cast<float4 *>(&q_row[r][4 * sub]) = x0;
+      *reinterpret_cast<float4 *>(&q_row[r][D / 2 + 4 * sub]) = x1;
+    } else if (wave == 1) {  // the key and the value
+      const bool is_v = r & 1, writes = k1 == hi && hb == 0;
+      const float *src = (is_v ? a.v : a.k) + ((long)z * a.Hkv + h) * D + 4 * sub;
+      float4 x0 = *reinterpret_cast<const float4 *>(src), x1 = *reinterpret_cast<const float4 *>(src + D / 2);
+      prepare_row<D>(prep, false, is_v, pos, sub, x0, x1);
+      bool bad = false;
+      const float big = hold_row<D>(x0, x1, sub, r < 2, new_codes[is_v], new_params[is_v], &bad);
+      if (r == 1 && sub == 0) new_big = big;
+      if (writes && bad) atomicOr(a.err, kDevErrCacheValue);
+    }
+    __syncthreads();
+  }
+
   // The queries' pieces, a channel a thread, as codes come off a word: 0, 4, 1, 5,
   // 2, 6, 3, 7 of eight. (A head past the last is the last.)
   const int r = threadIdx.x / D, ch = threadIdx.x % D;
-  float y = a.q[((long)z * a.Hq + h * a.R + min(hb * NQ + r, a.R - 1)) * D + ch] * a.qscale;
+  float y;
+  if constexpr (STEP) y = q_row[r][ch] * a.qscale;
+  else y = a.q[((long)z * a.Hq + h * a.R + min(hb * NQ + r, a.R - 1)) * D + ch] * a.qscale;
   {
     const float size = fabsf(y);
     const float most = max32(max16(row_max(size <= 3.402823466e38f ? size : 0.0f)));
@@ -422,7 +476,10 @@ __global__ __launch_bounds__(64 * kQ4Waves) void q4_attend_kernel(const Q4AttnAr
   // keep two whole pieces; it leaves in the quotient. (A step is at most 2/15 of
   // vmax, so the products are under 2^15. Steps are no less than 2^-24: a scale past
   // 2^40 would only let the sums overflow.)
-  const int vexp = min((int)(scale_to(seq_rows.vmax[h], 16) >> 23) - 127, 40);
+  // (A step takes the bound with the new row's, whether that is written yet or not.)
+  float vmax = seq_rows.vmax[h];
+  if constexpr (STEP) vmax = fmaxf(vmax, new_big);
+  const int vexp = min((int)(scale_to(vmax, 16) >> 23) - 127, 40);
 
   f32x4 o[CH];
 #pragma unroll
@@ -431,6 +488,23 @@ __global__ __launch_bounds__(64 * kQ4Waves) void q4_attend_kernel(const Q4AttnAr
   // (no copies of the next step's words: they are asked for when this step's are spent)
   for (; c < k1; c += kQ4Step) {
     const bool more = c + kQ4Step < k1;
+    if constexpr (STEP) {
+      if (c + 32 >= hi) {  // (the tile has the new row, and k1 is hi)
+        const int at = hi - 1 - c;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          if (16 * i + col == at) words(reinterpret_cast<const char *>(new_codes[0]) + t * (D / 8), kw[i]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (4 * t + key_of(i) == at) {
+            kpw[i] = new_params[0][g];
+            vpw[i] = new_params[1][g];
+            const char *const from = reinterpret_cast<const char *>(new_codes[1]) + col * (CH / 2);
+            if constexpr (CH < 8) vw[i][0] = *reinterpret_cast<const unsigned short *>(from);
+            else words(from, vw[i]);
+          }
+      }
+    }
     f32x4 sum[2];
 #pragma unroll
     for (int j = 0; j < G; ++j)
@@ -491,6 +565,23 @@ __global__ __launch_bounds__(64 * kQ4Waves) void q4_attend_kernel(const Q4AttnAr
       o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph, vf, o[n], 0, 0, 0);
     }
     if (more) load_v(c + kQ4Step);
+  }
+
+  if constexpr (STEP) {
+    if (k1 == hi && hb == 0) {
+      const long row = (long)h * seq_rows.cap + hi - 1;
+      const int i = threadIdx.x;
+      if (i < D / 4) {
+        const int which = i / (D / 8), w = i % (D / 8);
+        reinterpret_cast<unsigned *>((which ? seq_rows.v : seq_rows.k) + row * (D / 2))[w] =
+            reinterpret_cast<const unsigned *>(new_codes[which])[w];
+      } else if (i < D / 4 + 2 * G) {
+        const int which = (i - D / 4) / G, w = (i - D / 4) % G;
+        (which ? seq_rows.vp : seq_rows.kp)[row * G + w] = new_params[which][w];
+      } else if (i == D / 4 + 2 * G && new_big > seq_rows.vmax[h]) {
+        atomicMax(reinterpret_cast<int *>(seq_rows.vmax + h), __float_as_int(new_big));
+      }
+    }
   }
 
   l = sum32(sum16(l));
@@ -599,7 +690,8 @@ namespace {
 template <int D, int MB>
 hipError_t attend(hipStream_t st, const Q4AttnArgsOf<MB> &a, int nz) {
   const dim3 grid((unsigned)(a.Hkv * a.HB), (unsigned)a.max_splits, (unsigned)nz);
-  hipLaunchKernelGGL((q4_attend_kernel<D, MB>), grid, dim3(64 * kQ4Waves), 0, st, a);
+  auto kernel = a.k ? q4_attend_kernel<D, MB, true> : q4_attend_kernel<D, MB, false>;
+  hipLaunchKernelGGL(kernel, grid, dim3(64 * kQ4Waves), 0, st, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.max_splits == 1) return e;
   const dim3 cgrid((unsigned)(a.Hkv * a.HB), (unsigned)(std::min(a.R, 512 / D) * D / 32), (unsigned)nz);
