@@ -728,10 +728,11 @@ Q4AttnPlan q4_attend_plan(int D, int R, int Hkv, const int *keys, int n) {
   const long heads = (long)Hkv * p.HB;
   const long per = (total * heads + kQ4GridWorkgroups - 1) / kQ4GridWorkgroups;
   long kps = std::max<long>(1, (per + chunk - 1) / chunk) * chunk;
-  // A second launch costs 3.3 us, a step 1.2 to 2: two steps stay one range.
-  // (512 keys, heads of 64: 6.3 us against 8.0 in two ranges; 1024: 8.7 in one,
-  // 8.0 in four.)
-  if (most <= 2 * chunk) kps = 2 * chunk;
+  // Ranges cost a second launch, a step 1 to 2 us: short contexts stay one range.
+  // (768 keys, heads of 64 7.2 us in one range, 8.0 in three; of 128 9.0 and 9.0;
+  // of 256 13.2 and 11.2, 512 keys 10.5 and 11.2.)
+  const long one = (D == 256 ? 2 : 3) * chunk;
+  if (most <= one) kps = one;
   if ((most + kps - 1) / kps > kMaxDecodeSplits)
     kps = ((most + kMaxDecodeSplits - 1) / kMaxDecodeSplits + chunk - 1) / chunk * chunk;
   p.kps = (int)kps;
