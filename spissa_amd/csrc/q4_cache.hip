@@ -346,7 +346,7 @@ __device__ __forceinline__ void visible(const Q4AttnArgsOf<MB> &a, int z, int *l
 // against the minima's only at the end (outputs over 8192 keys were 1e-6 off).
 // Queries and weights are two binary16 pieces.
 // Bound: HBM for many keys, latency (one step of loads, one of sums) for few.
-// 16 sequences of 8192 keys, 24 heads on 8 of 128: 44 us, 3.8 TB/s of codes and
+// 16 sequences of 8192 keys, 24 heads on 8 of 128: 39 us, 4.3 TB/s of codes and
 // params (a copy reaches 5.1); 32768 keys of one head of 256: 12 us; 512 keys, 32
 // heads on 8 of 64: 6 us. Outputs are 1.2e-7 off (RMS, relative), as a plain f32
 // form's are.
@@ -629,13 +629,13 @@ __global__ __launch_bounds__(64 * kQ4Waves) void q4_attend_kernel(const Q4AttnAr
   }
 }
 
-// Merges the key ranges of one (query, KV head, head block): 32 consecutive
-// outputs x 32 range lanes. The ranges' weights come first, a thread a range, so
+// Merges the key ranges of one (query, KV head, head block): OUTS consecutive
+// outputs x SL range lanes. The ranges' weights come first, a thread a range, so
 // that the sums' reads depend on nothing and are all in flight at once.
-template <int D, int MB>
-__global__ __launch_bounds__(1024) void q4_combine_kernel(const Q4AttnArgsOf<MB> a) {
-  constexpr int NQ = 512 / D, ENTRY = NQ * (D + 2), OUTS = 32, SL = 32;
-  __shared__ float weight[kMaxDecodeSplits], part[SL][OUTS + 1], wave_m[16], wave_l[16];
+template <int D, int MB, int OUTS, int SL>
+__global__ __launch_bounds__(OUTS * SL) void q4_combine_kernel(const Q4AttnArgsOf<MB> a) {
+  constexpr int NQ = 512 / D, ENTRY = NQ * (D + 2), WAVES = OUTS * SL / 64;
+  __shared__ float weight[OUTS * SL], part[SL][OUTS + 1], wave_m[WAVES], wave_l[WAVES];
   const int z = blockIdx.z, hb = blockIdx.x % a.HB, h = blockIdx.x / a.HB;
   const int tid = threadIdx.x, e = blockIdx.y * OUTS + tid % OUTS, r = blockIdx.y * OUTS / D, sl = tid / OUTS;
   if (hb * NQ + r >= a.R) return;
@@ -658,7 +658,7 @@ __global__ __launch_bounds__(1024) void q4_combine_kernel(const Q4AttnArgsOf<MB>
   const float top = max32(max16(row_max(em)));
   if ((tid & 63) == 0) wave_m[tid >> 6] = top;
   __syncthreads();
-  const float M = safe_max(row_max(wave_m[tid & 15]));
+  const float M = safe_max(row_max(wave_m[tid % WAVES]));
   const float w = fast_exp2(em - M);
   if (tid < nsplit) weight[tid] = w;
   const float sum = group_sum<64>(tid < nsplit ? el * w : 0.0f);
@@ -679,7 +679,7 @@ __global__ __launch_bounds__(1024) void q4_combine_kernel(const Q4AttnArgsOf<MB>
 #pragma unroll
     for (int k = 0; k < SL; ++k) total += part[k][tid];
 #pragma unroll
-    for (int k = 0; k < 16; ++k) L += wave_l[k];
+    for (int k = 0; k < WAVES; ++k) L += wave_l[k];
     a.out[((long)z * a.Hq + h * a.R + hb * NQ) * D + e] = total / L;
     if ((e % D) == 0 && !(L > 0.0f && L < __builtin_inff())) atomicOr(a.err, kDevErrSoftmaxDenominator);
   }
@@ -694,8 +694,11 @@ hipError_t attend(hipStream_t st, const Q4AttnArgsOf<MB> &a, int nz) {
   hipLaunchKernelGGL(kernel, grid, dim3(64 * kQ4Waves), 0, st, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.max_splits == 1) return e;
-  const dim3 cgrid((unsigned)(a.Hkv * a.HB), (unsigned)(std::min(a.R, 512 / D) * D / 32), (unsigned)nz);
-  hipLaunchKernelGGL((q4_combine_kernel<D, MB>), cgrid, dim3(1024), 0, st, a);
+  // (32 range lanes for many ranges; two ranges of 16 sequences, 24 heads on 8 of 128:
+  // 8.5 us with them, 3.3 with four)
+  const unsigned outs = (unsigned)(std::min(a.R, 512 / D) * D), x = (unsigned)(a.Hkv * a.HB), z = (unsigned)nz;
+  if (a.max_splits <= 16) hipLaunchKernelGGL((q4_combine_kernel<D, MB, 64, 4>), dim3(x, outs / 64, z), dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((q4_combine_kernel<D, MB, 32, 32>), dim3(x, outs / 32, z), dim3(1024), 0, st, a);
   return hipGetLastError();
 }
 
@@ -730,7 +733,7 @@ Q4AttnPlan q4_attend_plan(int D, int R, int Hkv, const int *keys, int n) {
   long kps = std::max<long>(1, (per + chunk - 1) / chunk) * chunk;
   // Ragged lengths leave short last ranges: no more workgroups than are aimed at (or
   // one a head and sequence), which would wait for another to end. (16 sequences of
-  // 2432 to 8192 keys, 24 heads on 8 of 128: 41 us, 52 without.)
+  // 2432 to 8192 keys, 24 heads on 8 of 128: 36 us, 46 without.)
   const long limit = std::max<long>(kQ4GridWorkgroups, n * heads);
   for (;;) {
     long wgs = 0;
@@ -739,8 +742,8 @@ Q4AttnPlan q4_attend_plan(int D, int R, int Hkv, const int *keys, int n) {
     kps += std::max<long>(1, kps / chunk / 16) * chunk;
   }
   // Ranges cost a second launch, a step 1 to 2 us: short contexts stay one range.
-  // (768 keys, heads of 64 7.2 us in one range, 8.0 in three; of 128 9.0 and 9.0;
-  // of 256 13.2 and 11.2, 512 keys 10.5 and 11.2.)
+  // (768 keys, heads of 64 7.2 us in one range, 7.2 in three, with one launch more for
+  // the host; of 128 9.0 and 8.6; of 256 13.2 and 11.2, 512 keys 10.5 and 11.2.)
   const long one = (D == 256 ? 2 : 3) * chunk;
   if (most <= one) kps = one;
   if ((most + kps - 1) / kps > kMaxDecodeSplits)
