@@ -142,8 +142,8 @@ int spissa_kv_cache_rows_device(const spissa_kv_cache *c, size_t first, size_t c
  * spissa_attention_decode_batch_device,
  * spissa_scaled_dot_product_attention_with_cache) and
  * spissa_decode_step_device_noalloc refuse it (ARGUMENT). Device buffers are
- * 16-byte aligned (ARGUMENT otherwise). spissa_plan_attention describes f32
- * caches. */
+ * 16-byte aligned (ARGUMENT otherwise). Several queries a call: up to 8388480 /
+ * (Hq / Hkv) of them (SHAPE otherwise). spissa_plan_attention describes f32 caches. */
 int spissa_kv_cache_q4_new(size_t num_heads, size_t head_dim, size_t max_seq_len, spissa_kv_cache **out);
 int spissa_kv_cache_q4_new_in(spissa_session *s, size_t num_heads, size_t head_dim, size_t max_seq_len,
                               spissa_kv_cache **out);

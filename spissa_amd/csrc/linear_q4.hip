@@ -298,7 +298,9 @@ __device__ __forceinline__ void tile_addresses(const Q4LinearArgs &a, long tile0
 // which the lanes read them as the matrix instruction's A operand: the 16 rows
 // of A repeat the MP tokens, so every lane's accumulators are the same tokens'.
 // The codes and activations of the next 512 channels are in flight meanwhile.
-// Bound: HBM for large weights (the codes), latency for small ones.
+// Bound: HBM for large weights (the codes), latency for small ones. One token: 262144 x
+// 1152 39 us, 4.1 TB/s; 4096 x 4096 5.3 us; 2048 x 8192 5.7 us; two to four tokens,
+// 4096 x 4096 7.5 to 7.9 us.
 template <int PT, int GPB, int MP, int NT>
 __global__ __launch_bounds__(MP == 1 ? 1024 : 512) void q4_gemv_kernel(const Q4LinearArgs a) {
   constexpr int KC = 4;  // blocks of a round
@@ -444,7 +446,8 @@ __global__ __launch_bounds__(1024) void q4_pieces_kernel(const float *x, int M, 
 // tokens over a range of K blocks; the waves of a workgroup are wk ranges x runs of
 // tiles. Codes and pieces come straight from memory, a block of codes and a step
 // of pieces ahead. Bound: latency and the pieces' reads from L2 (each workgroup
-// reads all tokens), which NT tiles a wave share.
+// reads all tokens), which NT tiles a wave share. With the pieces' launch: 16
+// tokens, 4096 x 4096 9.4 us, 2560 x 2048 7 us; 64 tokens 22 us.
 template <int PT, int GPB, int MT, int NT>
 __global__ __launch_bounds__(512) void q4_few_kernel(const Q4LinearArgs a) {
   constexpr int SPG = 4 / GPB;
