@@ -518,3 +518,81 @@ def test_more_rows_than_a_launch_takes(ses):
     with pytest.raises(sa.ShapeError):
         ses.attention_cached(t, c, cfg, t)
     ses.sync()
+
+
+@pytest.mark.parametrize("d,hq,hkv", [(64, 32, 2), (64, 3, 3), (128, 12, 1), (128, 6, 2), (256, 8, 1), (256, 3, 1)])
+@pytest.mark.parametrize("size", [1.0, 3000.0])
+def test_steps_over_several_key_ranges(ses, d, hq, hkv, size):
+    """A ragged batch whose longest caches are split, with a new value row far beyond the held ones."""
+    rng = np.random.default_rng(d + hq)
+    lens = [0, 1, 255, 900, 2600]
+    made = [filled(ses, rng, n, hkv, d, 1) if n else
+            (ses.q4_kv_cache(hkv, d, 1), np.zeros((0, hkv, d)), np.zeros((0, hkv, d))) for n in lens]
+    b = len(lens)
+    q, k, v = rows(rng, b, hq, d), rows(rng, b, hkv, d), (rows(rng, b, hkv, d) * np.float32(size)).astype(np.float32)
+    for window in (0, 1000):
+        out = torch.full((b, hq, d), np.nan, device="cuda")
+        for m, n in zip(made, lens):
+            m[0].truncate(n)
+        ses.decode_step(None, dev(q), dev(k), dev(v), [m[0] for m in made], KvAttentionConfig(1, hq, hkv, d, True, window), out)
+        ses.sync()
+        for i, (c, k0, v0) in enumerate(made):
+            keys, values = np.concatenate([k0, hold(k[i:i + 1])]), np.concatenate([v0, hold(v[i:i + 1])])
+            gk, gv = held(ses, c)
+            assert_bitwise(gk, keys.astype(np.float32), f"keys of {lens[i]}")
+            assert_bitwise(gv, values.astype(np.float32), f"values of {lens[i]}")
+            check(out[i], attend(q[i:i + 1], keys, values, True, window)[0], values, f"step over {lens[i]} window {window}")
+
+
+def test_steps_report_values_outside_the_format(ses):
+    d, hq, hkv = 128, 4, 2
+    rng = np.random.default_rng(31)
+    for which in (0, 1):
+        c, _, _ = filled(ses, rng, 20, hkv, d, 1)
+        kv = [rows(rng, 1, hkv, d), rows(rng, 1, hkv, d)]
+        kv[which][0, 1, 77] = np.inf
+        q, out = dev(rows(rng, 1, hq, d)), torch.empty(1, hq, d, device="cuda")
+        ses.decode_step(None, q, dev(kv[0]), dev(kv[1]), [c], KvAttentionConfig(1, hq, hkv, d, True), out)
+        with pytest.raises(sa.InvalidTensorDataError):
+            ses.sync()
+        ses.sync()
+
+
+def test_two_graphs_share_the_workspaces(ses):
+    """Replays in turn, of a split step, of a chunk with ranges, and of the step's chunk form."""
+    d, hq, hkv = 128, 6, 2
+    rng = np.random.default_rng(32)
+    stream = torch.cuda.Stream()
+    own = Session(0, stream=stream)
+    with torch.cuda.stream(stream):
+        made = [filled(own, rng, n, hkv, d, 40)[0] for n in (3000, 1800)]
+        q1, k1, v1 = (dev(rows(rng, 1, h, d)) for h in (hq, hkv, hkv))
+        q2, k2, v2 = (dev(rows(rng, 40, h, d)) for h in (hq, hkv, hkv))
+        outs = [torch.zeros(1, hq, d, device="cuda"), torch.zeros(40, hq, d, device="cuda")]
+    table = own.rope_table(0, d, 10000.0, max_positions=4000)
+
+    def one():
+        made[0].truncate(3000)
+        own.decode_step(table, q1, k1, v1, [made[0]], KvAttentionConfig(1, hq, hkv, d, True), outs[0])
+
+    def many():
+        made[1].truncate(1800)
+        own.prefill_step(table, q2, k2, v2, made[1], KvAttentionConfig(40, hq, hkv, d, True), outs[1])
+
+    calls, graphs, want = (one, many), [], []
+    for call, out in zip(calls, outs):
+        call()
+        own.sync()
+        want.append(out.cpu().numpy())
+    for call in calls:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=stream):
+            call()
+    for turn in (0, 1, 0, 0, 1, 1):
+        with torch.cuda.stream(stream):
+            outs[turn].zero_()
+        torch.cuda.synchronize()
+        graphs[turn].replay()
+        torch.cuda.synchronize()
+        assert_bitwise(outs[turn].cpu().numpy(), want[turn], f"graph {turn}")
+        own.sync()
