@@ -1466,24 +1466,26 @@ static size_t q4_partial_bytes(size_t n, size_t Hq, size_t D, const Q4AttnPlan &
 
 // One query of each of B sequences, whose own row is its cache's last.
 // With `step` (its rows k and v, table and norm) the launch appends those rows first.
+// A few queries of one sequence (q4_few) likewise. extra: rows that the caches hold
+// beyond their lengths, or will.
 struct Q4StepRows {
   const float *k, *v;
   const spissa_rope_table *table;
   const GemmaQkNorm *norm;
 };
 static int q4_attend_batch(spissa_session *s, const float *q, const spissa_kv_cache *const *caches, size_t batch,
-                           const spissa_kv_attention_config *c, float *out, const Q4StepRows *step) {
-  const int D = (int)c->head_dim, Hq = (int)c->num_heads, Hkv = (int)c->kv_heads, R = Hq / Hkv;
+                           const spissa_kv_attention_config *c, float *out, const Q4StepRows *step, size_t extra) {
+  const int D = (int)c->head_dim, Hq = (int)c->num_heads, Hkv = (int)c->kv_heads, R = Hq / Hkv, S = (int)c->query_len;
   for (size_t b0 = 0; b0 < batch; b0 += kMaxDecodeBatch) {
     const int B = (int)std::min<size_t>(kMaxDecodeBatch, batch - b0);
     Q4AttnArgs a{};
     int keys[kMaxDecodeBatch];
     for (int b = 0; b < B; ++b) {
       a.seq[b].rows = q4_rows(caches[b0 + b], 0);
-      a.seq[b].len = (int)(caches[b0 + b]->len + (step ? 1 : 0));
-      keys[b] = c->window ? (int)std::min<size_t>(a.seq[b].len, c->window) : a.seq[b].len;
+      a.seq[b].len = (int)(caches[b0 + b]->len + extra);
+      keys[b] = c->window ? (int)std::min<size_t>(a.seq[b].len, c->window + S - 1) : a.seq[b].len;
     }
-    const Q4AttnPlan p = q4_attend_plan(D, R, Hkv, keys, B);
+    const Q4AttnPlan p = q4_attend_plan(D, S * R, Hkv, keys, B);
     ST_TRY(ensure_buf(s, s->partial, q4_partial_bytes(B, Hq, D, p, Hkv)));
     a.q = q + b0 * (size_t)Hq * D;
     a.out = out + b0 * (size_t)Hq * D;
@@ -1493,6 +1495,8 @@ static int q4_attend_batch(spissa_session *s, const float *q, const spissa_kv_ca
     a.Hkv = Hkv;
     a.R = R;
     a.HB = p.HB;
+    a.S = S;
+    a.causal = c->causal ? 1 : 0;
     a.window = (int)c->window;
     a.kps = p.kps;
     a.max_splits = p.splits;
@@ -1528,12 +1532,30 @@ static int q4_chunk_limit(const spissa_kv_attention_config *c) {
                    c->query_len, c->num_heads / c->kv_heads, most);
   return SPISSA_OK;
 }
+// Whether a chunk of a cache of `len` rows, the chunk's included, takes the single
+// queries' kernel, each of whose workgroups reads the keys for 512 / D rows: by the
+// two models' times. (us, single queries' kernel and chunk's, 24 heads on 8 of 128:
+// 4 queries over 100 keys 5.2 and 9.4, 32 over 1000 12.7 and 16.9, 4 over 8000 15
+// and 21, 8 over 8000 22 and 22, 16 37 and 24; 8 heads on 4 of 256, 4 over 100 6.6 and
+// 12.4, 16 over 8000 33 and 29.)
+static bool q4_few(spissa_session *s, size_t len, const spissa_kv_attention_config *c, Q4AttnPlan *plan) {
+  const size_t rows = c->query_len * (c->num_heads / c->kv_heads);
+  if (rows > 1024) return false;
+  const int keys = c->window ? (int)std::min<size_t>(len, c->window + c->query_len - 1) : (int)len;
+  *plan = q4_attend_plan((int)c->head_dim, (int)rows, (int)c->kv_heads, &keys, 1);
+  return plan->time < q4_chunk_plan_of(s, len, c).time;
+}
 static int q4_chunk_prepare(spissa_session *s, size_t len, const spissa_kv_attention_config *c) {
+  Q4AttnPlan few;
+  if (q4_few(s, len, c, &few))
+    return ensure_buf(s, s->partial, q4_partial_bytes(1, c->num_heads, c->head_dim, few, c->kv_heads));
   const Q4ChunkPlan p = q4_chunk_plan_of(s, len, c);
   return p.partial_bytes ? ensure_buf(s, s->ppart, p.partial_bytes) : SPISSA_OK;
 }
 static int q4_attend_chunk(spissa_session *s, const float *q, const spissa_kv_cache *cache, size_t len,
                            const spissa_kv_attention_config *c, float *out) {
+  Q4AttnPlan few;
+  if (q4_few(s, len, c, &few)) return q4_attend_batch(s, q, &cache, 1, c, out, nullptr, len - cache->len);
   const Q4ChunkPlan p = q4_chunk_plan_of(s, len, c);
   const int D = (int)c->head_dim;
   Q4ChunkArgs a{};
@@ -1617,7 +1639,7 @@ static int q4_step(spissa_session *s, const spissa_rope_table *table, const floa
     ST_TRY(ensure_buf(s, s->partial,
                       q4_partial_bytes(std::min<size_t>(batch, kMaxDecodeBatch), cfg->num_heads, cfg->head_dim, p, cfg->kv_heads)));
     const Q4StepRows rows{d_k, d_v, table, norm};
-    ST_TRY(q4_attend_batch(s, d_q, caches, batch, cfg, d_out, &rows));
+    ST_TRY(q4_attend_batch(s, d_q, caches, batch, cfg, d_out, &rows, 1));
   } else {
     const float *q = d_q;
     if (table || norm) {
@@ -1938,7 +1960,7 @@ extern "C" int spissa_attention_cached_device(spissa_session *s, const float *d_
       return set_err(SPISSA_ERR_ARGUMENT, "attention over a 4-bit cache takes 16-byte aligned buffers");
     ST_TRY(q4_chunk_limit(cfg));
     HIP_TRY(hipSetDevice(s->device));
-    if (S == 1) return q4_attend_batch(s, d_q, &cache, 1, cfg, d_out, nullptr);
+    if (S == 1) return q4_attend_batch(s, d_q, &cache, 1, cfg, d_out, nullptr, 0);
     ST_TRY(q4_chunk_prepare(s, cache->len, cfg));
     return q4_attend_chunk(s, d_q, cache, cache->len, cfg, d_out);
   }
@@ -1985,7 +2007,7 @@ extern "C" int spissa_attention_cached_batch_device(spissa_session *s, const flo
   if (!(aligned16(d_q) && aligned16(d_out)))
     return set_err(SPISSA_ERR_ARGUMENT, "attention over a 4-bit cache takes 16-byte aligned buffers");
   HIP_TRY(hipSetDevice(s->device));
-  return q4_attend_batch(s, d_q, caches, batch, cfg, d_out, nullptr);
+  return q4_attend_batch(s, d_q, caches, batch, cfg, d_out, nullptr, 0);
   GUARD_END
 }
 

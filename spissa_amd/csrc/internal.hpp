@@ -358,13 +358,13 @@ hipError_t launch_q4_append(hipStream_t st, const Q4AppendArgs &a, int D, int B)
 // Rows [s.first, s.first + n) as f32 [n, Hkv, D]; either output may be null.
 hipError_t launch_q4_rows(hipStream_t st, const Q4Rows &s, size_t n, size_t Hkv, size_t D, float *k_out, float *v_out);
 
-// Attention of the last token of each sequence of a batch.
+// Attention of the last token of each sequence of a batch, or of the last few of one.
 struct Q4AttnBase {
-  const float *q;   // [B, Hq, D]
+  const float *q;   // [B, Hq, D] or [S, Hq, D]
   float *out;
   float *partial;   // [B, Hkv, HB, max_splits] entries of RB * (D + 2) floats
   int *err;
-  int Hq, Hkv, R, HB, window, kps, max_splits;
+  int Hq, Hkv, R, HB, S, causal, window, kps, max_splits;  // S queries (several: one sequence); HB blocks of S * R rows
   float qscale;     // softmax scale * log2(e)
   // A fused step: the tokens' rows k, v [B, Hkv, D], which the launch prepares as
   // Q4AppendArgs has them, q too, and appends as the caches' last rows. Null k: the
@@ -388,9 +388,10 @@ typedef Q4AttnArgsOf<kMaxDecodeBatch> Q4AttnArgs;
 constexpr int kQ4GridWorkgroups = 256;
 struct Q4AttnPlan {
   int RB, HB, kps, splits;
+  double time;  // us, a model: a start, steps of 256 keys a CU, the merge
 };
-// keys[i]: visible keys of the n sequences of a launch.
-Q4AttnPlan q4_attend_plan(int D, int R, int Hkv, const int *keys, int n);
+// rows of a KV head (queries x heads); keys[i]: visible keys of the n sequences of a launch.
+Q4AttnPlan q4_attend_plan(int D, int rows, int Hkv, const int *keys, int n);
 hipError_t launch_q4_attend(hipStream_t st, const Q4AttnArgs &a, int D, int nz);
 bool q4_supported(size_t D);
 
@@ -410,6 +411,7 @@ struct Q4ChunkArgs {
 };
 struct Q4ChunkPlan {
   int per = 128, splits = 1, tps = 0;
+  double time = 0.0;  // us, the model's
   size_t partial_bytes = 0;
 };
 Q4ChunkPlan q4_chunk_plan(int D, int S, int R, int Hkv, int len, int causal, int window, int cus);

@@ -284,7 +284,7 @@ __global__ __launch_bounds__(256) void q4_append_kernel(const Q4AppendArgs a) {
   const float big = hold_row<D>(x0, x1, sub, keep, codes, param, &bad);
   if (keep && bad) atomicOr(a.err, kDevErrCacheValue);
   // The head's largest |value| (a bound: it never shrinks), which scales the
-  // 16-bit pieces of the attention's values. Positive floats order as integers.
+  // 16-bit pieces of the chunk attention's values. Positive floats order as integers.
   if (keep && is_v && sub == 0 && big > seq.vmax[h])
     atomicMax(reinterpret_cast<int *>(seq.vmax + h), __float_as_int(big));
 }
@@ -320,17 +320,25 @@ namespace {
 // (eight waves: a workgroup a CU holds two or three a SIMD)
 constexpr int kQ4Waves = 8, kQ4Step = 32 * kQ4Waves;  // waves of a workgroup, and the keys of a step of theirs
 
-// The keys that the last token of sequence z sees, [lo, hi).
+// The keys that any of the last S tokens of sequence z sees, [lo, hi).
 template <int MB>
 __device__ __forceinline__ void visible(const Q4AttnArgsOf<MB> &a, int z, int *lo, int *hi) {
   *hi = a.seq[z].len;
-  *lo = a.window > 0 ? max(0, *hi - a.window) : 0;
+  *lo = a.window > 0 ? max(0, *hi - a.S + 1 - a.window) : 0;
+}
+// Row r of a KV head h, a (query, head of the group) pair with the head fastest, among
+// the rows of the queries and outputs.
+template <int MB>
+__device__ __forceinline__ long row_of(const Q4AttnArgsOf<MB> &a, int z, int h, int r) {
+  if (a.S == 1) return (long)z * a.Hq + h * a.R + r;
+  const int query = r / a.R;
+  return (long)query * a.Hq + h * a.R + (r - query * a.R);
 }
 
 }  // namespace
 
-// One query of NQ heads of a KV head (blockIdx.x) over one range of keys
-// (blockIdx.y) of sequence blockIdx.z, 32 keys of the range a wave and step.
+// NQ rows, heads of a query or of a few, of a KV head (blockIdx.x) over one range of
+// keys (blockIdx.y) of sequence blockIdx.z, 32 keys of the range a wave and step.
 //
 // With G = D / 32 groups a row, the 16 columns of a matrix instruction are NQ =
 // 16 / G heads x G groups: column (q, g) of the queries has q's channels of group
@@ -357,7 +365,8 @@ __device__ __forceinline__ void visible(const Q4AttnArgsOf<MB> &a, int z, int *l
 // bit), and takes that row from there; the one with the last range and the first heads
 // writes it. A step over 512 keys, 32 heads on 8 of 64, with its rows read back: 18.2 us
 // with a launch of q4_append_kernel before, 14.7 without.
-template <int D, int MB, bool STEP>
+// FEW: several queries of one sequence (S > 1), whose keys end (and begin) at their own.
+template <int D, int MB, bool STEP, bool FEW>
 __global__ __launch_bounds__(64 * kQ4Waves) void q4_attend_kernel(const Q4AttnArgsOf<MB> a) {
   constexpr int G = D / 32, NQ = 16 / G, CH = D / 16, ENTRY = NQ * (D + 2);
   __shared__ float red_o[kQ4Waves][NQ][D];
@@ -384,6 +393,7 @@ __global__ __launch_bounds__(64 * kQ4Waves) void q4_attend_kernel(const Q4AttnAr
   const char *const vp = reinterpret_cast<const char *>(seq_rows.vp) + (long)h * seq_rows.cap * (G * 4);
   const unsigned k_at = col * (D / 2) + t * (D / 8), v_at = 4 * t * (D / 2) + col * (CH / 2);
   const unsigned p_at = 4 * t * (G * 4) + g * 4;
+  const int rows = FEW ? a.S * a.R : a.R;
 
   // Of 32 keys from c on: two rows' quarters, and of the eight keys 4 t + 0..3 and
   // 16 + 4 t + 0..3 the values' words and both rows' params. (The buffers go on for
@@ -416,7 +426,7 @@ __global__ __launch_bounds__(64 * kQ4Waves) void q4_attend_kernel(const Q4AttnAr
     const int sub = lane % LPR, r = lane / LPR, pos = hi - 1;
     const RowPrep prep{a.cos, a.sin, a.q_norm, a.k_norm, a.eps, a.prescale};
     if (wave == 0) {  // its 64 lanes are NQ rows
-      const float *src = a.q + ((long)z * a.Hq + h * a.R + min(hb * NQ + r, a.R - 1)) * D + 4 * sub;
+      const float *src = a.q + row_of(a, z, h, min(hb * NQ + r, rows - 1)) * D + 4 * sub;
       float4 x0 = *reinterpret_cast<const float4 *>(src), x1 = *reinterpret_cast<const float4 *>(src + D / 2);
       prepare_row<D>(prep, true, false, pos, sub, x0, x1);
       *reinterpret_cast<float4 *>(&q_row[r][4 * sub]) = x0;
@@ -439,7 +449,7 @@ __global__ __launch_bounds__(64 * kQ4Waves) void q4_attend_kernel(const Q4AttnAr
   const int r = threadIdx.x / D, ch = threadIdx.x % D;
   float y;
   if constexpr (STEP) y = q_row[r][ch] * a.qscale;
-  else y = a.q[((long)z * a.Hq + h * a.R + min(hb * NQ + r, a.R - 1)) * D + ch] * a.qscale;
+  else y = a.q[row_of(a, z, h, min(hb * NQ + r, rows - 1)) * D + ch] * a.qscale;
   {
     const float size = fabsf(y);
     const float most = max32(max16(row_max(size <= 3.402823466e38f ? size : 0.0f)));
@@ -474,19 +484,24 @@ __global__ __launch_bounds__(64 * kQ4Waves) void q4_attend_kernel(const Q4AttnAr
     qh[j] = first / 32 == g ? *reinterpret_cast<const half8 *>(&q_lds[0][col % NQ][first]) : none;
     ql[j] = first / 32 == g ? *reinterpret_cast<const half8 *>(&q_lds[1][col % NQ][first]) : none;
   }
-  // The weights are scaled by a power of two, that their products with the steps
-  // keep two whole pieces; it leaves in the quotient. (A step is at most 2/15 of
-  // vmax, so the products are under 2^15. Steps are no less than 2^-24: a scale past
-  // 2^40 would only let the sums overflow.)
-  // (A step takes the bound with the new row's, whether that is written yet or not.)
-  float vmax = seq_rows.vmax[h];
-  if constexpr (STEP) vmax = fmaxf(vmax, new_big);
-  const int vexp = min((int)(scale_to(vmax, 16) >> 23) - 127, 40);
+  // FEW: the keys of the column's query, and those that all queries see.
+  int row_end = 0, row_begin = 0, all_end = 0, all_begin = 0;
+  if constexpr (FEW) {
+    const int pos = hi - a.S + min(hb * NQ + col % NQ, rows - 1) / a.R;
+    row_end = a.causal ? pos + 1 : hi;
+    row_begin = a.window > 0 ? pos + 1 - a.window : 0;
+    all_end = a.causal ? hi - a.S + 1 : hi;
+    all_begin = a.window > 0 ? hi - a.window : 0;
+  }
 
   f32x4 o[CH];
 #pragma unroll
   for (int n = 0; n < CH; ++n) o[n] = (f32x4){0.f, 0.f, 0.f, 0.f};
-  float omin = 0.0f, l = 0.0f, m = NEG_INF;
+  // The weights are scaled by a power of two, a column's own, that their products with
+  // its group's steps keep two whole pieces: the largest step so far goes to 2^14..2^15,
+  // and one past `cap` moves the scale, as a score past m moves the reference.
+  float omin = 0.0f, l = 0.0f, m = NEG_INF, cap = -1.0f;
+  unsigned scale = 127u << 23;
   // (no copies of the next step's words: they are asked for when this step's are spent)
   for (; c < k1; c += kQ4Step) {
     const bool more = c + kQ4Step < k1;
@@ -534,12 +549,30 @@ __global__ __launch_bounds__(64 * kQ4Waves) void q4_attend_kernel(const Q4AttnAr
           vpw[i] = 0;
         }
     }
+    if constexpr (FEW) {
+      if (c + 32 > all_end || c < all_begin) {
+        int end = row_end - c - 4 * t, begin = row_begin - c - 4 * t;
+        asm volatile("" : "+v"(end), "+v"(begin));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s[i] = key_of(i) >= end || key_of(i) < begin ? NEG_INF : s[i];
+      }
+    }
 #pragma unroll
     for (int i = 0; i < 8; ++i) top = fmaxf(top, s[i]);
     top = max32(max16(top));
-    if (__any(top > m)) {
-      const float mnew = fmaxf(m, top), alpha = fast_exp2((m - safe_max(mnew)) * inv);
+    unsigned short step = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) step = max(step, (unsigned short)vpw[i]);  // (positive halves order as integers)
+    if (__any(top > m || half_lo(step) > cap)) {
+      const float mnew = fmaxf(m, top), largest = max32(max16(half_lo(step)));
+      float alpha = fast_exp2((m - safe_max(mnew)) * inv);
       m = mnew;
+      if (largest > cap) {  // (steps are no less than 2^-24: past 2^40 the sums would only overflow)
+        const unsigned to = min(scale_to(largest, 14), 167u << 23);
+        alpha *= __uint_as_float(to) * inverse_scale(scale);
+        scale = to;
+        cap = 60000.0f * inverse_scale(scale);
+      }
       l *= alpha;
       omin *= alpha;
 #pragma unroll
@@ -549,7 +582,7 @@ __global__ __launch_bounds__(64 * kQ4Waves) void q4_attend_kernel(const Q4AttnAr
         for (int n = 0; n < CH; ++n) o[n][e] *= f;
       }
     }
-    const float shift = fmaf(-safe_max(m), inv, (float)vexp);
+    const float shift = fmaf(-safe_max(m), inv, (float)((int)(scale >> 23) - 127));
     float p[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -588,16 +621,17 @@ __global__ __launch_bounds__(64 * kQ4Waves) void q4_attend_kernel(const Q4AttnAr
 
   l = sum32(sum16(l));
   omin = sum32(sum16(omin));
+  const float unscale = inverse_scale(scale);
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     const int row = 4 * t + e;
-    const float least = __shfl(omin, row);
+    const float least = __shfl(omin, row), back = __shfl(unscale, row);
     if (row / NQ == g)
 #pragma unroll
-      for (int n = 0; n < CH; ++n) red_o[wave][row % NQ][col * CH + n] = fmaf(o[n][e], 512.0f, least);
+      for (int n = 0; n < CH; ++n) red_o[wave][row % NQ][col * CH + n] = fmaf(o[n][e], 512.0f, least) * back;
   }
   if (lane < NQ) {
-    red_l[wave][lane] = l;
+    red_l[wave][lane] = l * unscale;
     wave_m[wave][lane] = m == NEG_INF ? m : m * inv;
   }
   __syncthreads();
@@ -605,7 +639,7 @@ __global__ __launch_bounds__(64 * kQ4Waves) void q4_attend_kernel(const Q4AttnAr
 #pragma unroll
   for (int e = threadIdx.x; e < NQ * D; e += 64 * kQ4Waves) {
     const int r = e / D, dim = e % D;
-    if (hb * NQ + r >= a.R) break;
+    if (hb * NQ + r >= rows) break;
     float M = NEG_INF;
 #pragma unroll
     for (int w = 0; w < kQ4Waves; ++w) M = fmaxf(M, wave_m[w][r]);
@@ -625,7 +659,7 @@ __global__ __launch_bounds__(64 * kQ4Waves) void q4_attend_kernel(const Q4AttnAr
         dst[NQ * D + 2 * r + 1] = L;
       }
     } else {
-      a.out[((long)z * a.Hq + h * a.R + hb * NQ + r) * D + dim] = O / L;
+      a.out[row_of(a, z, h, hb * NQ + r) * D + dim] = O / L;
       if (dim == 0 && !(L > 0.0f && L < __builtin_inff())) atomicOr(a.err, kDevErrSoftmaxDenominator);
     }
   }
@@ -640,7 +674,7 @@ __global__ __launch_bounds__(OUTS * SL) void q4_combine_kernel(const Q4AttnArgsO
   __shared__ float weight[OUTS * SL], part[SL][OUTS + 1], wave_m[WAVES], wave_l[WAVES];
   const int z = blockIdx.z, hb = blockIdx.x % a.HB, h = blockIdx.x / a.HB;
   const int tid = threadIdx.x, e = blockIdx.y * OUTS + tid % OUTS, r = blockIdx.y * OUTS / D, sl = tid / OUTS;
-  if (hb * NQ + r >= a.R) return;
+  if (hb * NQ + r >= a.S * a.R) return;
   int lo, hi;
   visible(a, z, &lo, &hi);
   const int nsplit = (hi - lo + a.kps - 1) / a.kps;
@@ -682,7 +716,7 @@ __global__ __launch_bounds__(OUTS * SL) void q4_combine_kernel(const Q4AttnArgsO
     for (int k = 0; k < SL; ++k) total += part[k][tid];
 #pragma unroll
     for (int k = 0; k < WAVES; ++k) L += wave_l[k];
-    a.out[((long)z * a.Hq + h * a.R + hb * NQ) * D + e] = total / L;
+    a.out[row_of(a, z, h, hb * NQ + r) * D + e % D] = total / L;
     if ((e % D) == 0 && !(L > 0.0f && L < __builtin_inff())) atomicOr(a.err, kDevErrSoftmaxDenominator);
   }
 }
@@ -692,13 +726,15 @@ namespace {
 template <int D, int MB>
 hipError_t attend(hipStream_t st, const Q4AttnArgsOf<MB> &a, int nz) {
   const dim3 grid((unsigned)(a.Hkv * a.HB), (unsigned)a.max_splits, (unsigned)nz);
-  auto kernel = a.k ? q4_attend_kernel<D, MB, true> : q4_attend_kernel<D, MB, false>;
+  auto kernel = a.k ? q4_attend_kernel<D, MB, true, false> : q4_attend_kernel<D, MB, false, false>;
+  if constexpr (MB == 1)
+    if (a.S > 1) kernel = q4_attend_kernel<D, MB, false, true>;
   hipLaunchKernelGGL(kernel, grid, dim3(64 * kQ4Waves), 0, st, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.max_splits == 1) return e;
   // (32 range lanes for many ranges; two ranges of 16 sequences, 24 heads on 8 of 128:
   // 8.5 us with them, 3.3 with four)
-  const unsigned outs = (unsigned)(std::min(a.R, 512 / D) * D), x = (unsigned)(a.Hkv * a.HB), z = (unsigned)nz;
+  const unsigned outs = (unsigned)(std::min(a.S * a.R, 512 / D) * D), x = (unsigned)(a.Hkv * a.HB), z = (unsigned)nz;
   if (a.max_splits <= 16) hipLaunchKernelGGL((q4_combine_kernel<D, MB, 64, 4>), dim3(x, outs / 64, z), dim3(256), 0, st, a);
   else hipLaunchKernelGGL((q4_combine_kernel<D, MB, 32, 32>), dim3(x, outs / 32, z), dim3(1024), 0, st, a);
   return hipGetLastError();
@@ -719,10 +755,10 @@ hipError_t attend_d(hipStream_t st, const Q4AttnArgs &a, int nz) {
 
 bool q4_supported(size_t D) { return D == 64 || D == 128 || D == 256; }
 
-Q4AttnPlan q4_attend_plan(int D, int R, int Hkv, const int *keys, int n) {
+Q4AttnPlan q4_attend_plan(int D, int rows, int Hkv, const int *keys, int n) {
   Q4AttnPlan p;
-  p.RB = 512 / D;  // the kernel's heads
-  p.HB = (R + p.RB - 1) / p.RB;
+  p.RB = 512 / D;  // the kernel's rows
+  p.HB = (rows + p.RB - 1) / p.RB;
   constexpr int chunk = kQ4Step;
   long total = 0;
   int most = 1;
@@ -752,6 +788,10 @@ Q4AttnPlan q4_attend_plan(int D, int R, int Hkv, const int *keys, int n) {
     kps = ((most + kMaxDecodeSplits - 1) / kMaxDecodeSplits + chunk - 1) / chunk * chunk;
   p.kps = (int)kps;
   p.splits = (int)((most + kps - 1) / kps);
+  long wgs = 0;
+  for (int i = 0; i < n; ++i) wgs += (keys[i] + kps - 1) / kps * heads;
+  const long steps = (wgs + kQ4GridWorkgroups - 1) / kQ4GridWorkgroups * ((std::min<long>(kps, most) + chunk - 1) / chunk);
+  p.time = (D == 64 ? 3.5 + 1.6 * steps : D == 128 ? 4.0 + 2.1 * steps : 5.0 + 3.0 * steps) + (p.splits > 1 ? 3.0 : 0.0);
   return p;
 }
 

@@ -488,7 +488,6 @@ Q4ChunkPlan q4_chunk_plan(int D, int S, int R, int Hkv, int len, int causal, int
   const int BN = 8192 / D;
   const long rows = (long)S * R;
   Q4ChunkPlan best;
-  double best_time = 0.0;
   for (int per = 128; per <= (D < 256 && rows > 128 ? 256 : 128); per += 128) {
     const double tile = D == 256 ? 2.45 : D == 128 ? (per == 256 ? 4.2 : 3.0) : per == 256 ? 5.2 : 3.9;
     const long blocks = (rows + per - 1) / per;
@@ -518,14 +517,15 @@ Q4ChunkPlan q4_chunk_plan(int D, int S, int R, int Hkv, int len, int causal, int
       // (CUs that get one workgroup more than the others: by how much at least)
       double time = std::max(longest, sum * Hkv / cus + (n > cus && n > full ? least * (1.0 - (double)(n - full) / cus) : 0.0));
       if (splits > 1) time += 3.5 + (double)splits * rows * Hkv * D * sizeof(float) / 2.2e6;
-      if (best_time == 0.0 || time < best_time) {
-        best_time = time;
+      if (best.time == 0.0 || time < best.time) {
+        best.time = time;
         best.per = per;
         best.splits = splits;
         best.tps = (int)tps;
       }
     }
   }
+  best.time += 3.0;  // (the launch)
   if (best.splits > 1) best.partial_bytes = (size_t)best.splits * rows * Hkv * (D + 2) * sizeof(float);
   return best;
 }

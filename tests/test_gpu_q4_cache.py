@@ -596,3 +596,39 @@ def test_two_graphs_share_the_workspaces(ses):
         torch.cuda.synchronize()
         assert_bitwise(outs[turn].cpu().numpy(), want[turn], f"graph {turn}")
         own.sync()
+
+
+@pytest.mark.parametrize("d,hq,hkv,s,past", [(64, 9, 3, 401, 333), (128, 5, 1, 450, 77), (256, 4, 2, 300, 513), (128, 16, 2, 129, 2000)])
+def test_chunks_of_many_rows(ses, d, hq, hkv, s, past):
+    test_chunks(ses, d, hq, hkv, s, past)
+
+
+@pytest.mark.parametrize("d,hq,hkv", [(64, 9, 3), (128, 4, 2), (256, 3, 1), (64, 5, 5)])
+@pytest.mark.parametrize("s,past", [(2, 2600), (7, 1500), (33, 800)])
+def test_a_few_queries_over_several_key_ranges(ses, d, hq, hkv, s, past):
+    test_chunks(ses, d, hq, hkv, s, past)
+
+
+@pytest.mark.parametrize("s", [1, 3])
+@pytest.mark.parametrize("scale", [1e-3, 300.0])
+def test_few_queries_of_values_of_any_size(ses, s, scale):
+    """As test_values_of_any_size, and with one row of large values among small ones."""
+    rng = np.random.default_rng(33)
+    k, v = rows(rng, 900, 2, 64), (rows(rng, 900, 2, 64) * scale).astype(np.float32)
+    c = ses.q4_kv_cache(2, 64, 900)
+    big = np.full((1, 2, 64), 60000.0, np.float32)
+    ses.append(c, dev(big), dev(big), 1)
+    c.truncate(0)
+    ses.append(c, dev(k), dev(v), 900)
+    q = rng.standard_normal((s, 4, 64)).astype(np.float32)
+    out = torch.empty(s, 4, 64, device="cuda")
+    cfg = KvAttentionConfig(s, 4, 2, 64, True)
+    ses.attention_cached(dev(q), c, cfg, out)
+    ses.sync()
+    check(out, attend(q, hold(k), hold(v)), hold(v), f"values of {scale}")
+    c.truncate(0)
+    v[400] *= np.float32(40.0)  # (the range's scale moves in the middle; 300 * 40 * 5 is within the format's 65504)
+    ses.append(c, dev(k), dev(v), 900)
+    ses.attention_cached(dev(q), c, cfg, out)
+    ses.sync()
+    check(out, attend(q, hold(k), hold(v)), hold(v), f"values of {scale}, one row far larger")
