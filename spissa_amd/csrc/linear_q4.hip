@@ -15,8 +15,9 @@
 // blocks of 128. A tile's block is 1 KB of codes in the order in which a wave's
 // lanes take them (lane l: row l % 16, quarter l / 16), 16 bytes a lane: four
 // words, word j with the eight codes of k = 32 j + 8 (l / 16) + 0..7, codes 2 i
-// and 2 i + 1 at bits 4 i and 16 + 4 i, so that a shift and one and-or make a
-// pair of binary16 numbers 1024 + code. The block's scales follow the rows:
+// and 2 i + 1 at bits 4 i and 16 + 4 i: read as binary16 numbers, those in bits 0..3
+// are code 2^-24 and those in bits 4..7 code 2^-20, so that one packed FMA makes a
+// pair of weights (code - zero) 2^-9, exactly; the 2^9 is in the tokens' factors. The block's scales follow the rows:
 // [tile][block][row][group in block], zero points beside them (Q4Param).
 #include <algorithm>
 
@@ -35,9 +36,9 @@ typedef __attribute__((ext_vector_type(4))) unsigned u32x4;
 
 // A group's scale and zero point as the kernels read them.
 //   0: binary16 scale, zero point 8            (2 bytes)
-//   1: binary16 scale, binary16 1024 + zero    (4 bytes)
-//   2: bfloat16 scale, binary16 1024 + zero    (4 bytes)
-//   3: f32 scale, binary16 1024 + zero twice   (8 bytes)
+//   1: binary16 scale, binary16 -zero / 512    (4 bytes)
+//   2: bfloat16 scale, binary16 -zero / 512    (4 bytes)
+//   3: f32 scale, binary16 -zero / 512 twice   (8 bytes)
 template <int PT>
 struct Q4Param {
   static constexpr int BYTES = PT == 0 ? 2 : PT == 3 ? 8 : 4;
@@ -82,10 +83,10 @@ struct BlockParams {
     else
       return __uint_as_float(w[2 * g]);
   }
-  // 1024 + zero, twice
+  // -zero / 512, twice
   __device__ __forceinline__ half2v zero(int g) const {
     if constexpr (PT == 0)
-      return (half2v){(_Float16)1032.0f, (_Float16)1032.0f};
+      return (half2v){(_Float16)-0x1p-6f, (_Float16)-0x1p-6f};
     else if constexpr (PT == 3)
       return __builtin_bit_cast(half2v, w[2 * g + 1]);
     else {
@@ -95,20 +96,24 @@ struct BlockParams {
   }
 };
 
-// 1024 twice in binary16, as a value that the compiler does not know: an and-or
-// takes one constant, so the other is in a register.
-__device__ __forceinline__ unsigned base_1024() {
-  unsigned b = 0x64006400u;
-  asm volatile("" : "+v"(b));
-  return b;
-}
-// The eight codes of a word less their zero point.
-__device__ __forceinline__ half8 weights8(unsigned w, half2v zero, unsigned base) {
+// The factors of codes in bits 0..3 and 4..7, 2^15 and 2^11 twice, as values that the
+// compiler does not know (it would take shifts for them).
+struct Factors {
+  half2v from0, from4;
+  __device__ __forceinline__ Factors() {
+    unsigned a = 0x78007800u, b = 0x68006800u;
+    asm volatile("" : "+v"(a), "+v"(b));
+    from0 = __builtin_bit_cast(half2v, a);
+    from4 = __builtin_bit_cast(half2v, b);
+  }
+};
+// The eight codes of a word less their zero point, times 2^-9.
+__device__ __forceinline__ half8 weights8(unsigned w, half2v zero, const Factors &f) {
   half8 r;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const unsigned u = ((w >> (4 * i)) & 0x000f000fu) | base;
-    const half2v p = __builtin_bit_cast(half2v, u) - zero;
+    const unsigned u = (i & 2 ? w >> 8 : w) & (i & 1 ? 0x00f000f0u : 0x000f000fu);
+    const half2v p = __builtin_elementwise_fma(__builtin_bit_cast(half2v, u), i & 1 ? f.from4 : f.from0, zero);
     r[2 * i] = p.x;
     r[2 * i + 1] = p.y;
   }
@@ -219,7 +224,7 @@ __global__ __launch_bounds__(256) void q4_pack_kernel(const Q4PackArgs a) {
       if (a.scale_dtype == SPISSA_DTYPE_F32) s = reinterpret_cast<const float *>(a.scales)[src];
       else sbits = reinterpret_cast<const unsigned short *>(a.scales)[src];
     }
-    const unsigned zb = __builtin_bit_cast(unsigned short, (_Float16)(1024.0f + (float)z));
+    const unsigned zb = __builtin_bit_cast(unsigned short, (_Float16)((float)z * (-1.0f / 512.0f)));
     const long at = (tb * 16 + row) * gpb + g;
     if (a.param_type == 0) {
       reinterpret_cast<unsigned short *>(a.out_params)[at] = (unsigned short)sbits;
@@ -255,7 +260,7 @@ struct BlockWeights {
 // acc += the block's products with the A fragments hi, lo (rows 4 (lane / 16) + 0..3
 // of A), the first E rows of the lane's four.
 template <int PT, int GPB, int NT, int E, typename FRAGS, typename INV>
-__device__ __forceinline__ void block_products(const BlockWeights<PT, GPB, NT> &b, unsigned base, FRAGS frags, const INV &inv,
+__device__ __forceinline__ void block_products(const BlockWeights<PT, GPB, NT> &b, const Factors &factors, FRAGS frags, const INV &inv,
                                                float (&acc)[NT][E]) {
   constexpr int SPG = 4 / GPB;  // 32-deep steps of a group
   f32x4 sum[NT];
@@ -265,7 +270,7 @@ __device__ __forceinline__ void block_products(const BlockWeights<PT, GPB, NT> &
     frags(j, &hi, &lo);
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      const half8 wf = weights8(b.w[t][j], b.p[t].zero(j / SPG), base);
+      const half8 wf = weights8(b.w[t][j], b.p[t].zero(j / SPG), factors);
       if (j % SPG == 0) sum[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
       sum[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, wf, sum[t], 0, 0, 0);
       sum[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, wf, sum[t], 0, 0, 0);
@@ -299,15 +304,15 @@ __device__ __forceinline__ void tile_addresses(const Q4LinearArgs &a, long tile0
 // of A repeat the MP tokens, so every lane's accumulators are the same tokens'.
 // The codes and activations of the next 512 channels are in flight meanwhile.
 // Bound: HBM for large weights (the codes), latency for small ones. One token: 262144 x
-// 1152 39 us, 4.1 TB/s; 4096 x 4096 5.3 us; 2048 x 8192 5.7 us; two to four tokens,
-// 4096 x 4096 7.5 to 7.9 us.
+// 1152 35 us, 4.6 TB/s; 16384 x 4096 10 us; 4096 x 4096 5.2 us; 2048 x 8192 5.9 us; two
+// to four tokens, 4096 x 4096 7.5 to 7.7 us.
 template <int PT, int GPB, int MP, int NT>
 __global__ __launch_bounds__(MP == 1 ? 1024 : 512) void q4_gemv_kernel(const Q4LinearArgs a) {
   constexpr int KC = 4;  // blocks of a round
   constexpr int WAVES = MP == 1 ? 16 : 8;
   __shared__ __attribute__((aligned(16))) half8 xs[WAVES][KC * 4 * 2 * 4 * MP];  // [wave][step][piece][quarter][token]
   __shared__ float red[WAVES][NT * 16][MP];
-  const unsigned base = base_1024();
+  const Factors factors;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wk = wave % a.wk, wn = wave / a.wk;
   const int row = lane & 15, quarter = lane >> 4;
@@ -352,7 +357,7 @@ __global__ __launch_bounds__(MP == 1 ? 1024 : 512) void q4_gemv_kernel(const Q4L
           wave_max(fmaxf(fmaxf(fmaxf(finite_abs(u.x), finite_abs(u.y)), fmaxf(finite_abs(u.z), finite_abs(u.w))),
                          fmaxf(fmaxf(finite_abs(v.x), finite_abs(v.y)), fmaxf(finite_abs(v.z), finite_abs(v.w)))));
       const unsigned sb = scale_bits(most);
-      inv[m] = inverse_scale(sb);
+      inv[m] = 512.0f * inverse_scale(sb);
       half4v h[2], l[2];
       split4(u, __uint_as_float(sb), &h[0], &l[0]);
       split4(v, __uint_as_float(sb), &h[1], &l[1]);
@@ -370,7 +375,7 @@ __global__ __launch_bounds__(MP == 1 ? 1024 : 512) void q4_gemv_kernel(const Q4L
         *hi = xs[wave][((c * 4 + j) * 2 * 4 + quarter) * MP + row % MP];
         *lo = xs[wave][(((c * 4 + j) * 2 + 1) * 4 + quarter) * MP + row % MP];
       };
-      block_products<PT, GPB, NT, MP>(w[c], base, frags, inv, acc);
+      block_products<PT, GPB, NT, MP>(w[c], factors, frags, inv, acc);
       if (more) w[c].load(codes, params, min(b + KC + c, b1 - 1));
     }
     wave_lds_order();
@@ -424,7 +429,7 @@ __global__ __launch_bounds__(1024) void q4_pieces_kernel(const float *x, int M, 
 #pragma unroll
   for (int w = 1; w < 16; ++w) most = fmaxf(most, part[w][r]);
   const unsigned sb = scale_bits(most);
-  if (unit == 0) inv[m] = inverse_scale(sb);
+  if (unit == 0) inv[m] = 512.0f * inverse_scale(sb);
   half8 *dst = pieces + (long)(m >> 4) * steps * 128 + (m & 15);
   for (int i = unit; i < steps * 4; i += 1024 / T) {  // eight channels: step i / 4, quarter i % 4
     if (i != unit) {
@@ -447,12 +452,12 @@ __global__ __launch_bounds__(1024) void q4_pieces_kernel(const float *x, int M, 
 // tiles. Codes and pieces come straight from memory, a block of codes and a step
 // of pieces ahead. Bound: latency and the pieces' reads from L2 (each workgroup
 // reads all tokens), which NT tiles a wave share. With the pieces' launch: 16
-// tokens, 4096 x 4096 9.4 us, 2560 x 2048 7 us; 64 tokens 22 us.
+// tokens, 4096 x 4096 9.8 us, 2560 x 2048 7 us; 64 tokens 22 us.
 template <int PT, int GPB, int MT, int NT>
 __global__ __launch_bounds__(512) void q4_few_kernel(const Q4LinearArgs a) {
   constexpr int SPG = 4 / GPB;
   extern __shared__ __attribute__((aligned(16))) float red[];  // [wave][MT * NT][4][64]
-  const unsigned base = base_1024();
+  const Factors factors;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wk = wave % a.wk, wn = wave / a.wk;
   const int row = lane & 15, quarter = lane >> 4;
@@ -489,7 +494,7 @@ __global__ __launch_bounds__(512) void q4_few_kernel(const Q4LinearArgs a) {
       load_x(min(4 * b + j + 1, 4 * b1 - 1), (j + 1) & 1);
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        const half8 wf = weights8(w[0].w[t][j], w[0].p[t].zero(j / SPG), base);
+        const half8 wf = weights8(w[0].w[t][j], w[0].p[t].zero(j / SPG), factors);
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
           if (j % SPG == 0) sum[i][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
@@ -535,14 +540,14 @@ __global__ __launch_bounds__(512) void q4_few_kernel(const Q4LinearArgs a) {
 // NT = 2 with MT = 4: their scales and zeros would not fit the registers.
 // Bound: the matrix cores (two instructions a product) beside the widening, which
 // a wave does for 16 NT rows and uses MT times, and a scaling FMA an output and group.
-// 2048 tokens x 4096 x 4096: 122 us, 1.13 PFLOP/s of binary16 products (a library
-// product of binary16 matrices of that size runs at 1.18); 512 tokens 54 us with
-// the pieces.
+// 2048 tokens x 4096 x 4096: 115 us, 1.2 PFLOP/s of binary16 products (a library
+// product of 4096 x 4096 binary16 matrices runs at 1.18); 512 tokens 52 us with the
+// pieces.
 template <int PT, int GPB, int MT, int NT>
 __global__ __launch_bounds__(512, 2) void q4_tile_kernel(const Q4LinearArgs a) {
   constexpr int SPG = 4 / GPB, TILE = 2 * MT * 8192;  // bytes of a block's pieces
   __shared__ __attribute__((aligned(16))) char x_lds[2][TILE];
-  const unsigned base = base_1024();
+  const Factors factors;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int row = lane & 15, quarter = lane >> 4;
   // Ids equal modulo 8 run on one XCD: each takes a contiguous run of the order,
@@ -593,7 +598,7 @@ __global__ __launch_bounds__(512, 2) void q4_tile_kernel(const Q4LinearArgs a) {
   }
   read(b0 & 1, 1, lo);
 #pragma unroll
-  for (int t = 0; t < NT; ++t) wf[t] = weights8(w.w[t][0], w.p[t].zero(0), base);
+  for (int t = 0; t < NT; ++t) wf[t] = weights8(w.w[t][0], w.p[t].zero(0), factors);
   // Beside a tile's matrix instructions stand the vector ones of the tile before:
   // its scaling, and its weights of the next 32 channels.
   for (int b = b0; b < b1; ++b) {
@@ -634,8 +639,8 @@ __global__ __launch_bounds__(512, 2) void q4_tile_kernel(const Q4LinearArgs a) {
 #pragma unroll
               for (int e = 0; e < 4; ++e) acc[i][t - 1][e] = fmaf(sum[i][t - 1][e], s, acc[i][t - 1][e]);
           }
-          wf[t - 1] = j < 3 ? weights8(w.w[t - 1][j < 3 ? j + 1 : 0], w.p[t - 1].zero((j < 3 ? j + 1 : 0) / SPG), base)
-                            : weights8(next.w[t - 1][0], next.p[t - 1].zero(0), base);
+          wf[t - 1] = j < 3 ? weights8(w.w[t - 1][j < 3 ? j + 1 : 0], w.p[t - 1].zero((j < 3 ? j + 1 : 0) / SPG), factors)
+                            : weights8(next.w[t - 1][0], next.p[t - 1].zero(0), factors);
         }
         if (t > 0 && t < NT)
 #pragma unroll
@@ -709,10 +714,10 @@ hipError_t tile(hipStream_t st, Q4LinearArgs a) {
 
 // Tile shape and ranges of K of a projection of more than 64 tokens; the larger
 // shape is 128 tokens x big_tiles row tiles. It wins once it fills three quarters
-// of the CUs (4096 x 4096, groups of 128: 2048 tokens 138 us against 156, 1536
-// level at 120, 1024 114 against 86); below, 64 x 8 row tiles, over ranges of K
-// while a CU stays without a workgroup (256 tokens: 49 us with one range, 39 with
-// two; 512 tokens: 54 and 57).
+// of the CUs (4096 x 4096, groups of 128: 2048 tokens 129 us against 144, 1536
+// level at 113, 1024 111 against 79); below, 64 x 8 row tiles, over ranges of K
+// while a CU stays without a workgroup (256 tokens: 50 us with one range, 39 with
+// two; 512 tokens: 52 and 54).
 struct Q4TilePlan {
   bool big;
   int splits;
@@ -729,17 +734,28 @@ Q4TilePlan q4_tile_plan(long M, long tiles, long blocks, int big_tiles) {
 template <int PT, int GPB>
 hipError_t run(hipStream_t st, Q4LinearArgs a) {
   if (a.M <= 4) {
-    // Waves of a workgroup share K while tiles are few. (One token: 2048 x 8192
-    // 6.2 us with up to 16 waves, 8.7 with 8. Four tokens' activations take the
-    // LDS of 8.)
+    // Waves of a workgroup share K: while tiles are few, and up to 8192 waves where the
+    // ranges come out even. (One token: 2048 x 8192 5.9 us with up to 16 waves, 8.7
+    // with 8; 16384 x 4096 10.0 with eight ranges, 15.7 with two; 65536 x 1152, three
+    // rounds, 16.9 with two, 14.4 with one. Four tokens' activations take the LDS of 8;
+    // 14336 x 4096 18 us with four ranges, 26 with two.)
     const int rounds = (a.blocks + 3) / 4;
     a.wk = 1;
     const int most = a.M == 1 ? 16 : 8;
-    while (a.wk < most && a.wk < rounds && (long)a.tiles * a.wk < 2048) a.wk *= 2;
+    auto even = [&](int wk) { return (rounds + wk - 1) / wk * wk * 4 <= rounds * 5; };
+    while (a.wk < most && a.wk < rounds &&
+           ((long)a.tiles * a.wk < 2048 || ((long)a.tiles * a.wk < 8192 && even(2 * a.wk))))
+      a.wk *= 2;
+    // Two row tiles a wave where there are thousands: its activations are split once
+    // for both. (262144 x 1152 35 us against 41, 128256 x 2048 29 against 35; 65536 x
+    // 1152 level; four spill.)
+    const bool two = a.M == 1 && a.tiles >= 6144;
+    if (two) a.wk = 1;
     a.blocks_per_wave = ((rounds + a.wk - 1) / a.wk) * 4;
-    const int waves = std::max(4, a.wk), runs = waves / a.wk;
+    const int waves = std::max(4, a.wk), runs = waves / a.wk * (two ? 2 : 1);
     const dim3 grid((unsigned)((a.tiles + runs - 1) / runs));
-    if (a.M == 1) hipLaunchKernelGGL((q4_gemv_kernel<PT, GPB, 1, 1>), grid, dim3(waves * 64), 0, st, a);
+    if (two) hipLaunchKernelGGL((q4_gemv_kernel<PT, GPB, 1, 2>), grid, dim3(waves * 64), 0, st, a);
+    else if (a.M == 1) hipLaunchKernelGGL((q4_gemv_kernel<PT, GPB, 1, 1>), grid, dim3(waves * 64), 0, st, a);
     else hipLaunchKernelGGL((q4_gemv_kernel<PT, GPB, 4, 1>), grid, dim3(waves * 64), 0, st, a);
     return hipGetLastError();
   }

@@ -128,6 +128,15 @@ def test_large(ses, m, n, k):
     check(ses, wt, acts(rng, m, k), rng.standard_normal(n).astype(np.float32))
 
 
+@pytest.mark.parametrize("n,k,group", [(98337, 200, 64), (98305, 129, 32), (99000, 640, 128), (20005, 1100, 64), (33000, 515, 32)])
+@pytest.mark.parametrize("scale,zeros", [("f16", False), ("f32", True)])
+@pytest.mark.parametrize("m", [1, 3])
+def test_one_token_of_many_rows(ses, n, k, group, scale, zeros, m):
+    rng = np.random.default_rng(n)
+    wt = Weight(rng, n, k, group, scale, zeros)
+    check(ses, wt, acts(rng, m, k), rng.standard_normal(n).astype(np.float32), what=f"{scale} zeros {zeros}")
+
+
 @pytest.mark.parametrize("scale,zeros,group", [("f16", False, 128), ("f16", True, 64), ("f32", True, 32), ("bf16", False, 128),
                                                ("f32", False, 128), ("f16", False, 32), ("bf16", True, 64)])
 @pytest.mark.parametrize("k", [1, 130, 257, 700])
