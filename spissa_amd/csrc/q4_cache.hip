@@ -729,7 +729,11 @@ hipError_t attend(hipStream_t st, const Q4AttnArgsOf<MB> &a, int nz) {
   auto kernel = a.k ? q4_attend_kernel<D, MB, true, false> : q4_attend_kernel<D, MB, false, false>;
   if constexpr (MB == 1)
     if (a.S > 1) kernel = q4_attend_kernel<D, MB, false, true>;
-  hipLaunchKernelGGL(kernel, grid, dim3(64 * kQ4Waves), 0, st, a);
+  // One workgroup a CU: two, which heads of 64 have the registers for, come together
+  // while other CUs stay empty, so LDS that nothing uses keeps them apart. (16 sequences
+  // of 2432 to 8192 keys, 32 heads on 8 of 64: 28 us, 42 without.)
+  const unsigned apart = D == 64 ? 62 * 1024 : 0;
+  hipLaunchKernelGGL(kernel, grid, dim3(64 * kQ4Waves), apart, st, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.max_splits == 1) return e;
   // (32 range lanes for many ranges; two ranges of 16 sequences, 24 heads on 8 of 128:
