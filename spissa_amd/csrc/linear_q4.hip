@@ -447,12 +447,12 @@ __global__ __launch_bounds__(1024) void q4_pieces_kernel(const float *x, int M, 
   }
 }
 
-// 5 to 64 tokens, MT tiles of 16. A wave takes NT row tiles of the weight and all
+// 5 to 32 tokens, MT tiles of 16. A wave takes NT row tiles of the weight and all
 // tokens over a range of K blocks; the waves of a workgroup are wk ranges x runs of
 // tiles. Codes and pieces come straight from memory, a block of codes and a step
 // of pieces ahead. Bound: latency and the pieces' reads from L2 (each workgroup
 // reads all tokens), which NT tiles a wave share. With the pieces' launch: 16
-// tokens, 4096 x 4096 9.8 us, 2560 x 2048 7 us; 64 tokens 22 us.
+// tokens, 4096 x 4096 9.7 us, 2560 x 2048 7.3 us; 32 tokens 14.8 and 9.9 us.
 template <int PT, int GPB, int MT, int NT>
 __global__ __launch_bounds__(512) void q4_few_kernel(const Q4LinearArgs a) {
   constexpr int SPG = 4 / GPB;
@@ -696,8 +696,8 @@ hipError_t few_n(hipStream_t st, Q4LinearArgs a) {
 template <int PT, int GPB, int MT>
 hipError_t few(hipStream_t st, const Q4LinearArgs &a) {
   // (One row tile a wave while that leaves a CU without a workgroup: 16 tokens,
-  // 4096 x 4096 9.4 us against 11.4 with two; 8192 x 4096 15.3 against 13.6; 64
-  // tokens 14336 x 4096 52 against 35.)
+  // 4096 x 4096 9.4 us against 11.4 with two; 8192 x 4096 15.3 against 13.6; 32
+  // tokens, 14336 x 4096 34 against 23.)
   return a.tiles < 2 * 256 ? few_n<PT, GPB, MT, 1>(st, a) : few_n<PT, GPB, MT, 2>(st, a);
 }
 
@@ -712,7 +712,14 @@ hipError_t tile(hipStream_t st, Q4LinearArgs a) {
   return hipGetLastError();
 }
 
-// Tile shape and ranges of K of a projection of more than 64 tokens; the larger
+// Whether tokens are few: up to 32, or 16 where K is past 8192 (each workgroup reads all
+// pieces, which its few rows do not repay). us, few and tiles: 32
+// tokens, 4096 x 4096 14.8 and 18.0, 14336 x 4096 23 and 31, 4096 x 14336 43 and 34; 16
+// of the last 27 and 33; 64, which had twice the tiles a wave, 22 and 21, 35 and 34,
+// 62 and 36.
+bool q4_few_tokens(long M, long blocks) { return M <= 16 || (M <= 32 && blocks <= 64); }
+
+// Tile shape and ranges of K of a projection of more tokens; the larger
 // shape is 128 tokens x big_tiles row tiles. It wins once it fills three quarters
 // of the CUs (4096 x 4096, groups of 128: 2048 tokens 129 us against 144, 1536
 // level at 113, 1024 111 against 79); below, 64 x 8 row tiles, over ranges of K
@@ -766,10 +773,8 @@ hipError_t run(hipStream_t st, Q4LinearArgs a) {
   hipLaunchKernelGGL(pieces, rows, dim3(1024), 0, st, a.x, a.M, a.K, a.blocks * 4, a.vec, (half8 *)a.pieces, (float *)a.inv);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  if (a.M <= 64) {
-    if (a.mtiles == 1) return few<PT, GPB, 1>(st, a);
-    if (a.mtiles == 2) return few<PT, GPB, 2>(st, a);
-    return few<PT, GPB, 4>(st, a);
+  if (q4_few_tokens(a.M, a.blocks)) {
+    return a.mtiles == 1 ? few<PT, GPB, 1>(st, a) : few<PT, GPB, 2>(st, a);
   } else {
     const Q4TilePlan p = q4_tile_plan(a.M, a.tiles, a.blocks, GPB == 1 ? 16 : 8);
     a.splits = p.splits;
@@ -798,20 +803,17 @@ hipError_t launch_q4_pack(hipStream_t st, const Q4PackArgs &a) {
   return hipGetLastError();
 }
 
-// Token tiles of the workspace: whole kernels' worth up to 64 tokens.
-static size_t q4_token_tiles(long M) { return M > 32 && M <= 48 ? 4 : (size_t)(M + 15) / 16; }
-
 // The workspace: pieces, inverse scales, and the partial sums of split K (0 bytes: none).
 size_t q4_linear_workspace(long M, long N, long tiles, long blocks, int pack_group) {
   if (M <= 4) return 0;
-  const size_t mt = q4_token_tiles(M);
-  const int splits = M <= 64 ? 1 : q4_tile_plan(M, tiles, blocks, pack_group == 128 ? 16 : 8).splits;
+  const size_t mt = (size_t)(M + 15) / 16;
+  const int splits = q4_few_tokens(M, blocks) ? 1 : q4_tile_plan(M, tiles, blocks, pack_group == 128 ? 16 : 8).splits;
   return mt * blocks * 8192 + mt * 16 * sizeof(float) + (splits > 1 ? (size_t)splits * M * N * sizeof(float) : 0);
 }
 
 hipError_t launch_q4_linear(hipStream_t st, const Q4LinearArgs &base, int group, int param_type, void *workspace) {
   Q4LinearArgs a = base;
-  a.mtiles = (int)q4_token_tiles(a.M);
+  a.mtiles = (a.M + 15) / 16;
   a.vec = a.K % 4 == 0 && (reinterpret_cast<uintptr_t>(a.x) & 15) == 0;
   a.pieces = workspace;
   a.inv = reinterpret_cast<const float *>(static_cast<char *>(workspace) + (size_t)a.mtiles * a.blocks * 8192);

@@ -128,6 +128,15 @@ def test_large(ses, m, n, k):
     check(ses, wt, acts(rng, m, k), rng.standard_normal(n).astype(np.float32))
 
 
+@pytest.mark.parametrize("m", [16, 17, 24, 32, 33, 47, 64])
+@pytest.mark.parametrize("n,k,group", [(70, 8192, 128), (130, 8200, 64), (1000, 9000, 32), (2100, 500, 128)])
+def test_some_tokens(ses, m, n, k, group):
+    """Either side of where the tiles of many tokens begin."""
+    rng = np.random.default_rng(n + m)
+    wt = Weight(rng, n, k, group, "f16", True)
+    check(ses, wt, acts(rng, m, k), rng.standard_normal(n).astype(np.float32))
+
+
 @pytest.mark.parametrize("n,k,group", [(98337, 200, 64), (98305, 129, 32), (99000, 640, 128), (20005, 1100, 64), (33000, 515, 32)])
 @pytest.mark.parametrize("scale,zeros", [("f16", False), ("f32", True)])
 @pytest.mark.parametrize("m", [1, 3])
