@@ -121,9 +121,15 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void q4_chunk_kernel(const Q4Chunk
   asm volatile("" : "+v"(base1024));
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, kq = lane >> 4;
-  // Blocks of rows, the last (longest) ones of every head first; key splits of each.
+  // Blocks of rows, the last (longest) ones of every head first; key ranges of each.
+  // Ids equal modulo 8 share an XCD: where heads do not spread a block's ranges over
+  // them, each range takes eight blocks in an order of its own. (2048 queries of 4 heads
+  // on one of 256, six ranges: 70 us, 78 without; 32 heads on 8 of 64, two ranges, would
+  // go from 85 to 94.)
   const int h = blockIdx.x, split = blockIdx.z;
-  const int block = gridDim.y - 1 - blockIdx.y;
+  int order = blockIdx.y;
+  if (a.Hkv % 8 != 0 && (order | 7) < (int)gridDim.y) order = (order & ~7) | ((order + split) & 7);
+  const int block = gridDim.y - 1 - order;
   const int rows = a.S * a.R;
   const int row0 = block * (NW * 16) + wave * 16;
   const int P = a.len - a.S;  // the first query's position
