@@ -1,5 +1,5 @@
-// lanes.hpp -- exchanges between the lanes of a wave, and the scalar pieces of
-// RoPE and the online softmax, shared by the attention kernels.
+// lanes.hpp -- exchanges between the lanes of a wave, the scalar pieces of RoPE and
+// the online softmax, and f32 numbers as two binary16 pieces, shared by the kernels.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -74,6 +74,50 @@ __device__ __forceinline__ void rotate_pair(float &first, float &second, float c
   const float b = second * c + first * s;
   first = a;
   second = b;
+}
+
+typedef __attribute__((ext_vector_type(8))) _Float16 half8;
+typedef __attribute__((ext_vector_type(2))) _Float16 half2v;
+typedef __attribute__((ext_vector_type(4))) float f32x4;
+typedef __attribute__((ext_vector_type(4))) unsigned u32x4;
+
+__device__ __forceinline__ float half_lo(unsigned w) { return (float)__builtin_bit_cast(_Float16, (unsigned short)w); }
+__device__ __forceinline__ float half_hi(unsigned w) {
+  return (float)__builtin_bit_cast(_Float16, (unsigned short)(w >> 16));
+}
+
+// Two pieces of eight numbers: the nearest binary16 number and the nearest one of what
+// that leaves, so a number within the pieces' range is off by at most 2^-23 of itself, to
+// either side. (Cut pieces would be off by up to 2^-21, and always towards zero.)
+// (minus_one: -1 as the compiler does not know it, so that the difference is one
+// mixed-precision FMA and not a conversion and a subtraction)
+__device__ __forceinline__ void split8(const float (&v)[8], float minus_one, half8 *hi, half8 *lo) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    unsigned w = __builtin_bit_cast(unsigned, (half2v){(_Float16)v[2 * i], (_Float16)v[2 * i + 1]});
+    asm("" : "+v"(w));  // (one packed conversion: the FMAs would have one each again)
+    const half2v h = __builtin_bit_cast(half2v, w);
+    float r0 = fmaf((float)h.x, minus_one, v[2 * i]), r1 = fmaf((float)h.y, minus_one, v[2 * i + 1]);
+    asm("" : "+v"(r0), "+v"(r1));  // (FMAs that write a half of a register each: chunk attention 1 to 2 % slower)
+    const half2v l = {(_Float16)r0, (_Float16)r1};
+    (*hi)[2 * i] = h.x;
+    (*hi)[2 * i + 1] = h.y;
+    (*lo)[2 * i] = l.x;
+    (*lo)[2 * i + 1] = l.y;
+  }
+}
+// Power of two that takes `most` to 2^top..2^(top + 1), as float bits.
+__device__ __forceinline__ unsigned scale_to(float most, unsigned top) {
+  return min(254u + top - (__float_as_uint(most) >> 23), 253u) << 23;
+}
+__device__ __forceinline__ float inverse_scale(unsigned bits) { return __uint_as_float((254u << 23) - bits); }
+
+// Copies 16 bytes a lane from base + off into LDS at lds_base + 16 * lane, unknown
+// to the compiler, which would wait for it before any later LDS read: the kernel's
+// barriers wait for the copies that the next step reads.
+__device__ __forceinline__ void copy16(const char *base, unsigned off, char *lds_base) {
+  const unsigned lds = (unsigned)(uintptr_t)(__attribute__((address_space(3))) void *)lds_base;
+  asm volatile("global_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "{m0}"(lds) : "memory");
 }
 
 }  // namespace

@@ -28,11 +28,7 @@ namespace spissa {
 
 namespace {
 
-typedef __attribute__((ext_vector_type(8))) _Float16 half8;
-typedef __attribute__((ext_vector_type(2))) _Float16 half2v;
 typedef __attribute__((ext_vector_type(4))) _Float16 half4v;
-typedef __attribute__((ext_vector_type(4))) float f32x4;
-typedef __attribute__((ext_vector_type(4))) unsigned u32x4;
 
 // A group's scale and zero point as the kernels read them.
 //   0: binary16 scale, zero point 8            (2 bytes)
@@ -120,20 +116,6 @@ __device__ __forceinline__ half8 weights8(unsigned w, half2v zero, const Factors
   return r;
 }
 
-// Copies 16 bytes a lane from base + off into LDS at lds_base + 16 * lane, unknown
-// to the compiler, which would wait for it before any later LDS read: the kernel's
-// barrier waits for the copies that the next step reads.
-__device__ __forceinline__ void copy16(const char *base, unsigned off, char *lds_base) {
-  const unsigned lds = (unsigned)(uintptr_t)(__attribute__((address_space(3))) void *)lds_base;
-  asm volatile("global_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "{m0}"(lds) : "memory");
-}
-
-// Power of two that takes a largest |activation| to 2^13..2^14 (as float bits),
-// and its inverse.
-__device__ __forceinline__ unsigned scale_bits(float most) {
-  return min(267u - (__float_as_uint(most) >> 23), 253u) << 23;
-}
-__device__ __forceinline__ float inverse_scale(unsigned bits) { return __uint_as_float((254u << 23) - bits); }
 __device__ __forceinline__ float finite_abs(float v) {
   const float a = fabsf(v);
   return a <= 3.402823466e38f ? a : 0.0f;
@@ -356,7 +338,7 @@ __global__ __launch_bounds__(MP == 1 ? 1024 : 512) void q4_gemv_kernel(const Q4L
       const float most =
           wave_max(fmaxf(fmaxf(fmaxf(finite_abs(u.x), finite_abs(u.y)), fmaxf(finite_abs(u.z), finite_abs(u.w))),
                          fmaxf(fmaxf(finite_abs(v.x), finite_abs(v.y)), fmaxf(finite_abs(v.z), finite_abs(v.w)))));
-      const unsigned sb = scale_bits(most);
+      const unsigned sb = scale_to(most, 13);
       inv[m] = 512.0f * inverse_scale(sb);
       half4v h[2], l[2];
       split4(u, __uint_as_float(sb), &h[0], &l[0]);
@@ -428,7 +410,7 @@ __global__ __launch_bounds__(1024) void q4_pieces_kernel(const float *x, int M, 
   most = part[0][r];
 #pragma unroll
   for (int w = 1; w < 16; ++w) most = fmaxf(most, part[w][r]);
-  const unsigned sb = scale_bits(most);
+  const unsigned sb = scale_to(most, 13);
   if (unit == 0) inv[m] = 512.0f * inverse_scale(sb);
   half8 *dst = pieces + (long)(m >> 4) * steps * 128 + (m & 15);
   for (int i = unit; i < steps * 4; i += 1024 / T) {  // eight channels: step i / 4, quarter i % 4

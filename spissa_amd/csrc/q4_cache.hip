@@ -23,40 +23,11 @@ namespace spissa {
 
 namespace {
 
-__device__ __forceinline__ float half_lo(unsigned w) { return (float)__builtin_bit_cast(_Float16, (unsigned short)w); }
-__device__ __forceinline__ float half_hi(unsigned w) {
-  return (float)__builtin_bit_cast(_Float16, (unsigned short)(w >> 16));
-}
 __device__ __forceinline__ unsigned half_bits(float v) {
   return __builtin_bit_cast(unsigned short, (_Float16)v);
 }
 
-typedef __attribute__((ext_vector_type(8))) _Float16 half8;
-typedef __attribute__((ext_vector_type(2))) _Float16 half2v;
-typedef __attribute__((ext_vector_type(4))) float f32x4;
 
-// Truncation, two at a time: the second piece takes what the first leaves.
-__device__ __forceinline__ half2v pieces2(float a, float b) {
-  return __builtin_bit_cast(half2v, __builtin_amdgcn_cvt_pkrtz(a, b));
-}
-// (minus_one: -1 as the compiler does not know it, so that the difference is one
-// mixed-precision FMA and not a conversion and a subtraction)
-__device__ __forceinline__ void split8(const float (&v)[8], float minus_one, half8 *hi, half8 *lo) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const half2v h = pieces2(v[2 * i], v[2 * i + 1]);
-    const half2v l = pieces2(fmaf((float)h.x, minus_one, v[2 * i]), fmaf((float)h.y, minus_one, v[2 * i + 1]));
-    (*hi)[2 * i] = h.x;
-    (*hi)[2 * i + 1] = h.y;
-    (*lo)[2 * i] = l.x;
-    (*lo)[2 * i + 1] = l.y;
-  }
-}
-// Power of two that takes `most` to 2^top..2^(top + 1), as float bits.
-__device__ __forceinline__ unsigned scale_to(float most, unsigned top) {
-  return min(254u + top - (__float_as_uint(most) >> 23), 253u) << 23;
-}
-__device__ __forceinline__ float inverse_scale(unsigned bits) { return __uint_as_float((254u << 23) - bits); }
 
 template <int N>
 __device__ __forceinline__ void words(const char *p, unsigned (&w)[N]) {
@@ -462,7 +433,7 @@ __global__ __launch_bounds__(64 * kQ4Waves) void q4_attend_kernel(const Q4AttnAr
   const unsigned sb = scale_to(most, 13);
   y *= __uint_as_float(sb);
   {
-    const _Float16 first = pieces2(y, 0.0f).x, second = pieces2(y - (float)first, 0.0f).x;
+    const _Float16 first = (_Float16)y, second = (_Float16)(y - (float)first);
     const int at = (ch & ~7) + (ch & 3) * 2 + (ch >> 2 & 1);
     q_lds[0][r][at] = first;
     q_lds[1][r][at] = second;

@@ -36,45 +36,7 @@ namespace spissa {
 
 namespace {
 
-typedef __attribute__((ext_vector_type(8))) _Float16 half8;
-typedef __attribute__((ext_vector_type(2))) _Float16 half2v;
-typedef __attribute__((ext_vector_type(4))) float f32x4;
-typedef __attribute__((ext_vector_type(4))) unsigned u32x4;
 
-__device__ __forceinline__ float half_lo(unsigned w) { return (float)__builtin_bit_cast(_Float16, (unsigned short)w); }
-__device__ __forceinline__ float half_hi(unsigned w) {
-  return (float)__builtin_bit_cast(_Float16, (unsigned short)(w >> 16));
-}
-// Truncation, two at a time: the second piece takes what the first leaves.
-__device__ __forceinline__ half2v pieces2(float a, float b) {
-  return __builtin_bit_cast(half2v, __builtin_amdgcn_cvt_pkrtz(a, b));
-}
-// (minus_one: -1 as the compiler does not know it, so that the difference is one
-// mixed-precision FMA and not a conversion and a subtraction)
-__device__ __forceinline__ void split8(const float (&v)[8], float minus_one, half8 *hi, half8 *lo) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const half2v h = pieces2(v[2 * i], v[2 * i + 1]);
-    const half2v l = pieces2(fmaf((float)h.x, minus_one, v[2 * i]), fmaf((float)h.y, minus_one, v[2 * i + 1]));
-    (*hi)[2 * i] = h.x;
-    (*hi)[2 * i + 1] = h.y;
-    (*lo)[2 * i] = l.x;
-    (*lo)[2 * i + 1] = l.y;
-  }
-}
-// Power of two that takes `most` to 2^top..2^(top + 1), as float bits.
-__device__ __forceinline__ unsigned scale_to(float most, unsigned top) {
-  return min(254u + top - (__float_as_uint(most) >> 23), 253u) << 23;
-}
-__device__ __forceinline__ float inverse_scale(unsigned bits) { return __uint_as_float((254u << 23) - bits); }
-
-// Copies 16 bytes a lane from base + off into LDS at lds_base + 16 * lane, unknown
-// to the compiler, which would wait for it before any later LDS read: the kernel's
-// barriers wait for the copies that the next step reads.
-__device__ __forceinline__ void copy16(const char *base, unsigned off, char *lds_base) {
-  const unsigned lds = (unsigned)(uintptr_t)(__attribute__((address_space(3))) void *)lds_base;
-  asm volatile("global_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "{m0}"(lds) : "memory");
-}
 
 // A key row's eight codes of a word in the order in which weights of a pair
 // come off it: 0, 4, 1, 5, 2, 6, 3, 7 (queries are put in that order too).

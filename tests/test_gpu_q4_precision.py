@@ -1,0 +1,95 @@
+"""How far attention over the 4-bit cache is from 64-bit sums over the same held
+rows, by the root mean square (RMS) of the errors against that of the outputs.
+
+A score takes at most 24 roundings of 2^-24 (tests/test_gpu_q4_cache.py counts
+them) of partial sums that are at most A = sum |q k| / sqrt(D). Each is off by
+at most half a step and unbiased, so of RMS 2^-24 A / sqrt(3): together sqrt(8)
+2^-24 A, which is the relative error of a weight. Weights, values and outputs
+add a few roundings of 2^-24 of their own: 2^-22 holds sixteen of them at their
+worst, or more at their RMS. An error that all outputs of a row share is at most that too.
+"""
+import numpy as np
+import pytest
+import torch
+
+from spissa_amd.device import Session
+from spissa_amd.rotary import KvAttentionConfig
+from tests.q4 import attend, hold
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ses(gpu):
+    # the tests' own tensors are made, filled and freed on the session's stream
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        yield Session(0, stream=stream)
+
+
+def dev(a):
+    return torch.from_numpy(np.ascontiguousarray(a)).cuda()
+
+
+def attention(ses, q, cache, hkv, causal=True, window=0):
+    s, hq, d = q.shape
+    out = torch.full((s, hq, d), np.nan, device="cuda")
+    ses.attention_cached(dev(q), cache, KvAttentionConfig(s, hq, hkv, d, causal, window), out)
+    ses.sync()
+    return out.cpu().numpy()
+
+
+def rms(a):
+    return float(np.sqrt(np.mean(np.square(np.asarray(a, np.float64)))))
+
+
+def score_size(q, keys):
+    """A: the largest sum |q k| / sqrt(D) of a query and a key of its KV head."""
+    hq, hkv, d = q.shape[1], keys.shape[1], q.shape[2]
+    q, keys = np.abs(q).astype(np.float64), np.abs(keys).astype(np.float64)
+    return max(np.max(q[:, h] @ keys[:, h * hkv // hq].T) for h in range(hq)) / np.sqrt(d)
+
+
+def check(got, ref, a, what, more=0.0):
+    off, tol = rms(got - ref) / rms(ref), np.sqrt(8.0) * 2.0**-24 * a + 2.0**-22 + more
+    print(f"[q4 precision] {what}: {off:.2e} of {tol:.2e}", flush=True)
+    assert off <= tol, (what, off, tol)
+
+
+@pytest.mark.parametrize("d,hq,hkv", [(64, 4, 1), (128, 6, 2), (256, 2, 1)])
+@pytest.mark.parametrize("s", [1, 5])
+@pytest.mark.parametrize("nats", [9.0, 11.0, 13.0])
+def test_a_sink(ses, d, hq, hkv, s, nats):
+    """The first key takes the weight and has no value: the output is the rest, which has little weight each."""
+    rng = np.random.default_rng(d + s)
+    n = 6000
+    k = rng.standard_normal((n, hkv, d)).astype(np.float32)
+    v = (1 + 0.3 * rng.standard_normal((n, hkv, d))).astype(np.float32)
+    q = rng.standard_normal((s, hq, d)).astype(np.float32)
+    k[:, :, 0], q[:, :, 0] = 0, 4
+    k[0], v[0] = 0, 0
+    k[0, :, 0] = nats * np.sqrt(d) / 4  # (the others' scores are about N(0, 1))
+    c = ses.q4_kv_cache(hkv, d, n)
+    ses.append(c, dev(k), dev(v), n)
+    keys, values = hold(k), hold(v)
+    check(attention(ses, q, c, hkv), attend(q, keys, values), score_size(q, keys), f"d {d} s {s} {nats} nats")
+
+
+@pytest.mark.parametrize("d,hq,hkv", [(64, 4, 4), (128, 2, 2), (256, 1, 1), (128, 8, 1)])
+@pytest.mark.parametrize("s", [40, 1100])
+def test_roundings_have_no_side(ses, d, hq, hkv, s):
+    """Queries that see one key each give its value back. Weights and values of two
+    pieces, each the nearest, are off to either side alike: over the 320 (key, group)
+    pairs or more of a case, a mean of roundings of 2^-24 at most (2^-25 in RMS) stays
+    within 2^-29, and four times that is allowed. Cut pieces are off to one side."""
+    rng = np.random.default_rng(d + s)
+    k, v = rng.standard_normal((2, s, hkv, d)).astype(np.float32)
+    q = rng.standard_normal((s, hq, d)).astype(np.float32)
+    c = ses.q4_kv_cache(hkv, d, s)
+    ses.append(c, dev(k), dev(v), s)
+    ref = np.repeat(hold(v).astype(np.float64), hq // hkv, axis=1)
+    got = attention(ses, q, c, hkv, window=1)
+    gain = float(np.sum((got - ref) * ref) / np.sum(ref * ref))
+    print(f"[q4 precision] d {d} heads {hq}/{hkv} s {s}: 1 + {gain:.2e}", flush=True)
+    assert abs(gain) <= 2.0**-27, gain
+    check(got, ref, 0.0, "one key")
