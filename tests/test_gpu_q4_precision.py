@@ -57,7 +57,7 @@ def check(got, ref, a, what, more=0.0):
 
 
 @pytest.mark.parametrize("d,hq,hkv", [(64, 4, 1), (128, 6, 2), (256, 2, 1)])
-@pytest.mark.parametrize("s", [1, 5])
+@pytest.mark.parametrize("s", [1, 5, 550])
 @pytest.mark.parametrize("nats", [9.0, 11.0, 13.0])
 def test_a_sink(ses, d, hq, hkv, s, nats):
     """The first key takes the weight and has no value: the output is the rest, which has little weight each."""
@@ -73,6 +73,33 @@ def test_a_sink(ses, d, hq, hkv, s, nats):
     ses.append(c, dev(k), dev(v), n)
     keys, values = hold(k), hold(v)
     check(attention(ses, q, c, hkv), attend(q, keys, values), score_size(q, keys), f"d {d} s {s} {nats} nats")
+
+
+@pytest.mark.parametrize("d,hq,hkv", [(64, 4, 1), (128, 6, 2), (256, 2, 1)])
+@pytest.mark.parametrize("s,past", [(1, 39), (5, 35), (550, 0)])
+@pytest.mark.parametrize("nats", [5.0, 9.0, 13.0])
+def test_a_sink_before_few_keys(ses, d, hq, hkv, s, past, nats):
+    """As test_a_sink, with each row's error against that row's output: few keys do not
+    average their weights' roundings. The weights are about e^-nats of the largest, so
+    2^-19 at the least; a second piece that ends 2^-38 below the largest is a rounding
+    of 2^-20 there: off by at most half of that, 2^-22 in RMS over two keys and more."""
+    rng = np.random.default_rng(d + s)
+    n = s + past
+    k = rng.standard_normal((n, hkv, d)).astype(np.float32)
+    v = (1 + 0.3 * rng.standard_normal((n, hkv, d))).astype(np.float32)
+    q = rng.standard_normal((s, hq, d)).astype(np.float32)
+    k[:, :, 0], q[:, :, 0] = 0, 4
+    k[0], v[0] = 0, 0
+    k[0, :, 0] = nats * np.sqrt(d) / 4
+    c = ses.q4_kv_cache(hkv, d, n)
+    ses.append(c, dev(k), dev(v), n)
+    keys, values = hold(k), hold(v)
+    got, ref = attention(ses, q, c, hkv), attend(q, keys, values)
+    if past == 0:  # (the first query sees the sink alone)
+        assert not np.any(got[0]) and not np.any(ref[0])
+        got, ref = got[1:], ref[1:]
+    size = np.sqrt(np.mean(ref * ref, axis=2, keepdims=True))
+    check(got / size, ref / size, score_size(q, keys), f"d {d} s {s} {nats} nats, few keys", 2.0**-22)
 
 
 @pytest.mark.parametrize("d,hq,hkv", [(64, 4, 4), (128, 2, 2), (256, 1, 1), (128, 8, 1)])
