@@ -136,10 +136,11 @@ int spissa_kv_cache_rows_device(const spissa_kv_cache *c, size_t first, size_t c
  * rounding: spissa_attention_cached_device (from one query on),
  * spissa_attention_cached_batch_device, the fused spissa_{,gemma_}decode_step_device
  * and spissa_{,gemma_}prefill_step_device, and spissa_attention_sublayer_device.
- * In the Gemma steps the QK-norm's sums of squares are taken as a tree. Sums,
- * products and softmax are f32 (prefill precision does not matter here); where
- * more queries take the chunk kernel, values are held down to 2^-37 of the largest
- * |value| that the head has held. The
+ * In the Gemma steps the QK-norm's sums of squares are taken as a tree. Sums and
+ * softmax are f32 (prefill precision does not matter here). Queries, softmax
+ * weights and, where more queries take the chunk kernel, values are held to 2^-23
+ * of themselves; weights and values not below 2^-38 of the largest among the keys
+ * that the call reads. The
  * calls that take current rows beside the cache (spissa_attention_device,
  * spissa_attention_decode_batch_device,
  * spissa_scaled_dot_product_attention_with_cache) and

@@ -145,7 +145,6 @@ struct spissa_kv_cache {
   bool q4 = false;
   unsigned char *kc = nullptr, *vc = nullptr;
   unsigned *kp = nullptr, *vp = nullptr;
-  float *vmax = nullptr;    // [H]
   size_t width() const { return num_heads * head_dim; }
   // Bytes of keys or values that `rows` rows take in 4 bits, and that the buffers
   // have: tiles of keys are read whole, up to 127 rows past the last.
@@ -453,20 +452,13 @@ static int kv_q4_new_impl(spissa_session *s, size_t num_heads, size_t head_dim, 
   c->max_seq_len = max_seq_len;
   c->q4 = true;
   const size_t codes = c->q4_codes_end(), params = c->q4_params_end();
-  const size_t bytes = 2 * (codes + params) + num_heads * sizeof(float);
+  const size_t bytes = 2 * (codes + params);
   HIP_TRY(hipSetDevice(s->device));
   ST_TRY(no_capture(s->stream, "a 4-bit cache", bytes));
   HIP_TRY(hipMalloc(&c->kc, bytes));
   c->vc = c->kc + codes;
   c->kp = (unsigned *)(c->vc + codes);  // (codes are whole 32-byte rows)
   c->vp = (unsigned *)((char *)c->kp + params);
-  c->vmax = (float *)((char *)c->vp + params);
-  hipError_t e = hipMemsetAsync(c->vmax, 0, num_heads * sizeof(float), s->stream);
-  if (e == hipSuccess) e = hipStreamSynchronize(s->stream);
-  if (e != hipSuccess) {
-    (void)hipFree(c->kc);
-    return set_err(SPISSA_ERR_DEVICE, "clearing a 4-bit cache failed: %s", hipGetErrorString(e));
-  }
   *out = c.release();
   session_retain(s);
   return SPISSA_OK;
@@ -496,7 +488,7 @@ extern "C" int spissa_kv_cache_q4_new(size_t num_heads, size_t head_dim, size_t 
 extern "C" int spissa_kv_cache_is_q4(const spissa_kv_cache *c) { return c && c->q4 ? 1 : 0; }
 
 static Q4Rows q4_rows(const spissa_kv_cache *c, size_t first) {
-  return Q4Rows{c->kc, c->vc, c->kp, c->vp, c->vmax, (long)c->max_seq_len, (int)first, 0};
+  return Q4Rows{c->kc, c->vc, c->kp, c->vp, (long)c->max_seq_len, (int)first, 0};
 }
 
 static bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -763,7 +755,7 @@ extern "C" int spissa_kv_cache_clone(const spissa_kv_cache *c, spissa_kv_cache *
   hipError_t e = hipSuccess;
   if (c->q4) {
     // (whole: a head's rows are apart, so the first rows of all are not one range)
-    const size_t all = 2 * (c->q4_codes_end() + c->q4_params_end()) + c->num_heads * sizeof(float);
+    const size_t all = 2 * (c->q4_codes_end() + c->q4_params_end());
     e = hipMemcpyAsync(n->kc, c->kc, all, hipMemcpyDeviceToDevice, s->stream);
   } else if (bytes) {
     e = hipMemcpyAsync(n->keys, c->keys, bytes, hipMemcpyDeviceToDevice, s->stream);

@@ -336,7 +336,6 @@ bool prefill_supported(int D);
 struct Q4Rows {
   unsigned char *k, *v;
   unsigned *kp, *vp;
-  float *vmax;  // [Hkv]: a bound on the head's |values|
   long cap;
   int first;    // the first row to write or to give back
   int pad;

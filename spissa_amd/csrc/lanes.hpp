@@ -60,6 +60,15 @@ __device__ __forceinline__ float groups_max(float v) {
   return v;
 }
 
+// Max over a wave.
+__device__ __forceinline__ float wave_max(float v) {
+  v = fmaxf(v, dpp<0xB1>(v));
+  v = fmaxf(v, dpp<0x4E>(v));
+  v = fmaxf(v, dpp<0x141>(v));
+  v = fmaxf(v, dpp<0x140>(v));
+  return max32(max16(v));
+}
+
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
 constexpr float NEG_INF = -__builtin_inff();

@@ -128,9 +128,9 @@ __device__ __forceinline__ float min8(float v) { return -max8(-v); }
 constexpr float kHalfMax = 65504.0f;
 
 // Eight lanes' 32 channels, four each, into codes; lane 0 of the eight stores
-// their step and minimum. Returns the largest |value| that the codes can stand for.
-__device__ __forceinline__ float hold32(const float4 x, bool store, bool first, unsigned char *codes, unsigned *param,
-                                        bool *bad) {
+// their step and minimum.
+__device__ __forceinline__ void hold32(const float4 x, bool store, bool first, unsigned char *codes, unsigned *param,
+                                       bool *bad) {
 #pragma clang fp contract(off)
   const float v[4] = {x.x, x.y, x.z, x.w};
   float lo = fminf(fminf(v[0], v[1]), fminf(v[2], v[3]));
@@ -158,7 +158,6 @@ __device__ __forceinline__ float hold32(const float4 x, bool store, bool first, 
     *reinterpret_cast<unsigned short *>(codes) = (unsigned short)c;
     if (first) *param = mb << 16 | sb;
   }
-  return fmaxf(fabsf(min), fabsf(min + 15.0f * step));
 }
 
 // What a fused step does to query and key rows before they are used or held.
@@ -201,17 +200,12 @@ __device__ __forceinline__ void prepare_row(const RowPrep &a, bool is_q, bool is
   }
 }
 // ... and into codes: every lane takes part in the exchanges, those with `store`
-// write. Returns the row's largest |value| in every lane (a bound).
+// write.
 template <int D>
-__device__ __forceinline__ float hold_row(const float4 &x0, const float4 &x1, int sub, bool store, unsigned char *codes,
-                                          unsigned *params, bool *bad) {
-  constexpr int LPR = D / 8;
-  float big = hold32(x0, store, (sub & 7) == 0, codes + 2 * sub, params + sub / 8, bad);
-  big = fmaxf(big, hold32(x1, store, (sub & 7) == 0, codes + D / 4 + 2 * sub, params + D / 64 + sub / 8, bad));
-  big = max8(big);
-  if constexpr (LPR >= 16) big = fmaxf(big, dpp<0x140>(big));
-  if constexpr (LPR >= 32) big = max16(big);
-  return big;
+__device__ __forceinline__ void hold_row(const float4 &x0, const float4 &x1, int sub, bool store, unsigned char *codes,
+                                         unsigned *params, bool *bad) {
+  hold32(x0, store, (sub & 7) == 0, codes + 2 * sub, params + sub / 8, bad);
+  hold32(x1, store, (sub & 7) == 0, codes + D / 4 + 2 * sub, params + D / 64 + sub / 8, bad);
 }
 
 }  // namespace
@@ -252,12 +246,8 @@ __global__ __launch_bounds__(256) void q4_append_kernel(const Q4AppendArgs a) {
   unsigned *param = (is_v ? seq.vp : seq.kp) + at_row * (D / 32);
   const bool keep = live && !is_q;
   bool bad = false;
-  const float big = hold_row<D>(x0, x1, sub, keep, codes, param, &bad);
+  hold_row<D>(x0, x1, sub, keep, codes, param, &bad);
   if (keep && bad) atomicOr(a.err, kDevErrCacheValue);
-  // The head's largest |value| (a bound: it never shrinks), which scales the
-  // 16-bit pieces of the chunk attention's values. Positive floats order as integers.
-  if (keep && is_v && sub == 0 && big > seq.vmax[h])
-    atomicMax(reinterpret_cast<int *>(seq.vmax + h), __float_as_int(big));
 }
 
 // Rows [first, first + n) of a cache as the f32 values they stand for, keys
@@ -348,7 +338,6 @@ __global__ __launch_bounds__(64 * kQ4Waves) void q4_attend_kernel(const Q4AttnAr
   __shared__ __attribute__((aligned(16))) float q_row[STEP ? NQ : 1][D];
   __shared__ __attribute__((aligned(16))) unsigned char new_codes[2][D / 2];
   __shared__ unsigned new_params[2][G];
-  __shared__ float new_big;
 
   const int z = blockIdx.z, hb = blockIdx.x % a.HB, h = blockIdx.x / a.HB, split = blockIdx.y;
   int lo, hi;
@@ -408,8 +397,7 @@ __global__ __launch_bounds__(64 * kQ4Waves) void q4_attend_kernel(const Q4AttnAr
       float4 x0 = *reinterpret_cast<const float4 *>(src), x1 = *reinterpret_cast<const float4 *>(src + D / 2);
       prepare_row<D>(prep, false, is_v, pos, sub, x0, x1);
       bool bad = false;
-      const float big = hold_row<D>(x0, x1, sub, r < 2, new_codes[is_v], new_params[is_v], &bad);
-      if (r == 1 && sub == 0) new_big = big;
+      hold_row<D>(x0, x1, sub, r < 2, new_codes[is_v], new_params[is_v], &bad);
       if (writes && bad) atomicOr(a.err, kDevErrCacheValue);
     }
     __syncthreads();
@@ -584,8 +572,6 @@ __global__ __launch_bounds__(64 * kQ4Waves) void q4_attend_kernel(const Q4AttnAr
       } else if (i < D / 4 + 2 * G) {
         const int which = (i - D / 4) / G, w = (i - D / 4) % G;
         (which ? seq_rows.vp : seq_rows.kp)[row * G + w] = new_params[which][w];
-      } else if (i == D / 4 + 2 * G && new_big > seq_rows.vmax[h]) {
-        atomicMax(reinterpret_cast<int *>(seq_rows.vmax + h), __float_as_int(new_big));
       }
     }
   }

@@ -8,9 +8,9 @@
 // step in f32, and the minima times the queries' group sums (three pieces) are
 // one more instruction over the groups:
 //   s = 2^-e (sum_g step_g (code . q)_g + sum_g min_g (sum q)_g).
-// Output: the values, step * code + min scaled by a power of two from the
-// head's largest, and the probabilities, times 2^14, are two pieces each, of
-// whose four products the three above 2^-22 are taken.
+// Output: the values, step * code + min scaled by a power of two that takes the
+// largest of the workgroup's keys to 2^13..2^14, and the probabilities, times 2^14,
+// are two pieces each, of whose four products the three above 2^-22 are taken.
 //
 // A workgroup takes 128 or 256 rows of a KV head, a row being a (query,
 // query head of the group) pair with the head fastest, so that short chunks
@@ -76,6 +76,7 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void q4_chunk_kernel(const Q4Chunk
   __shared__ __attribute__((aligned(16))) step_t step_lds[2][BN * G];
   __shared__ __attribute__((aligned(16))) _Float16 min_lds[2][BN][8];
   __shared__ __attribute__((aligned(16))) char raw_lds[2][RAW];
+  __shared__ __attribute__((aligned(16))) float most_lds[NW];
 
   float minus_one = -1.0f;
   unsigned base1024 = 0x64006400u;
@@ -136,6 +137,30 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void q4_chunk_kernel(const Q4Chunk
   };
   fetch(t0);
   if (t0 + 1 < t1) fetch(t0 + 1);
+  // The largest value of the range's rows, which their steps and minima bound, beside
+  // the first tiles on their way: 0 to 2 % of the time. (A bound kept with the cache
+  // would outlive rows that are taken back, and one of each tile takes 3 to 8 %.)
+  {
+    constexpr int AT_ONCE = 4;  // loads of a lane in flight
+    typedef u32x4 __attribute__((aligned(4))) params_t;
+    const params_t *const params = reinterpret_cast<const params_t *>(src[3] + (long)t0 * PB);
+    const int words = (min(t1 * BN, a.len) - t0 * BN) * G, vectors = (words + 3) / 4;
+    float most = 0.0f;
+    for (int i = tid; i < vectors; i += NW * 64 * AT_ONCE) {
+      u32x4 p[AT_ONCE];
+#pragma unroll
+      for (int u = 0; u < AT_ONCE; ++u) p[u] = params[min(i + u * NW * 64, vectors - 1)];
+#pragma unroll
+      for (int u = 0; u < AT_ONCE; ++u) {
+        if (G == 2 && 4 * min(i + u * NW * 64, vectors - 1) + 2 == words) p[u].z = p[u].w = 0;  // (an odd last row)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          most = fmaxf(most, fmaxf(fabsf(half_hi(p[u][j])), fabsf(fmaf(half_lo(p[u][j]), 15.0f, half_hi(p[u][j])))));
+      }
+    }
+    most = wave_max(most);
+    if (lane == 0) most_lds[wave] = most;
+  }
 
   half8 qh[G], ql[G], qs;
   float inv;
@@ -193,8 +218,8 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void q4_chunk_kernel(const Q4Chunk
   l = 0.0f;
 #pragma unroll
   for (int d = 0; d < DT; ++d) o[d] = (f32x4){0.f, 0.f, 0.f, 0.f};
-  const unsigned vsb = scale_to(a.rows.vmax[h], 13);
-  const float vscale = __uint_as_float(vsb);
+  unsigned vsb;  // the values' scale, as float bits
+  float vscale;
 
   // A thread's share of a tile: half a key's group of 32 channels, and eight keys
   // (4 q + 0..3 and 16 + 4 q + 0..3 of 32) of two channels of the values.
@@ -405,6 +430,11 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void q4_chunk_kernel(const Q4Chunk
     if (tile + 2 < t1) fetch(tile + 2);
   };
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");  // the first two tiles have come
+  float largest = 0.0f;
+#pragma unroll
+  for (int i = 0; i < NW; ++i) largest = fmaxf(largest, most_lds[i]);
+  vsb = __builtin_amdgcn_readfirstlane(scale_to(largest, 13));
+  vscale = __uint_as_float(vsb);
 #pragma unroll 1
   for (int tile = t0 - 1; tile < t1; ++tile) {
     if (ahead && tile >= t0) barrier(tile);

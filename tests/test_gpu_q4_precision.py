@@ -12,6 +12,7 @@ import numpy as np
 import pytest
 import torch
 
+from spissa_amd import InvalidTensorDataError
 from spissa_amd.device import Session
 from spissa_amd.rotary import KvAttentionConfig
 from tests.q4 import attend, hold
@@ -120,3 +121,55 @@ def test_roundings_have_no_side(ses, d, hq, hkv, s):
     print(f"[q4 precision] d {d} heads {hq}/{hkv} s {s}: 1 + {gain:.2e}", flush=True)
     assert abs(gain) <= 2.0**-27, gain
     check(got, ref, 0.0, "one key")
+
+
+@pytest.mark.parametrize("d,hq,hkv", [(64, 8, 2), (128, 6, 2), (256, 4, 1)])
+@pytest.mark.parametrize("how", ["clear", "truncate", "roll back", "not finite"])
+def test_a_used_cache_is_as_a_new_one(ses, d, hq, hkv, how):
+    """Rows that are gone leave nothing behind, bit for bit."""
+    rng = np.random.default_rng(d)
+    n, half = 700, 300
+    k, v = rng.standard_normal((2, n, hkv, d)).astype(np.float32) * np.float32(0.01)
+    q = rng.standard_normal((n, hq, d)).astype(np.float32)
+    new, used = (ses.q4_kv_cache(hkv, d, n) for _ in range(2))
+    ses.append(new, dev(k), dev(v), n)
+    at = half if how in ("roll back", "not finite") else 0
+    if at:
+        ses.append(used, dev(k[:at]), dev(v[:at]), at)
+    gone = torch.full((100, hkv, d), np.inf if how == "not finite" else 65504.0, device="cuda")
+    gone[:, :, ::2] = -65504.0
+    ses.append(used, gone, gone, 100)
+    if how == "not finite":
+        with pytest.raises(InvalidTensorDataError):
+            ses.sync()
+    if how == "clear":
+        used.clear()
+    else:
+        used.truncate(at)
+    ses.append(used, dev(k[at:]), dev(v[at:]), n - at)
+    want, got = attention(ses, q, new, hkv), attention(ses, q, used, hkv)
+    assert np.array_equal(want.view(np.uint32), got.view(np.uint32))
+    keys, values = hold(k), hold(v)
+    check(got, attend(q, keys, values), score_size(q, keys), f"d {d} {how}")
+
+
+@pytest.mark.parametrize("d,hq,hkv", [(64, 8, 2), (128, 6, 2), (256, 4, 1)])
+@pytest.mark.parametrize("s", [1, 5, 550])
+@pytest.mark.parametrize("at", [0, 333])
+def test_small_values_beside_a_large_one(ses, d, hq, hkv, s, at):
+    """A row of large values that no query looks at costs the others what the pieces
+    cannot hold: 2^-38 of the largest value, for each of the weights and the values."""
+    rng = np.random.default_rng(d + s + at)
+    n = 900
+    k, v = rng.standard_normal((2, n, hkv, d)).astype(np.float32)
+    v = 1 + np.float32(0.1) * v
+    q = rng.standard_normal((s, hq, d)).astype(np.float32)
+    k[:, :, 0], q[:, :, 0] = 0, 4
+    k[at] = 0
+    k[at, :, 0] = -10.0 * np.sqrt(d)  # 40 nats below
+    v[at] = 3000 * rng.standard_normal((hkv, d))
+    c = ses.q4_kv_cache(hkv, d, n)
+    ses.append(c, dev(k), dev(v), n)
+    keys, values = hold(k), hold(v)
+    ref = attend(q, keys, values)
+    check(attention(ses, q, c, hkv), ref, score_size(q, keys), f"d {d} s {s}, a large row", 2 * 2.0**-38 * np.max(np.abs(values)) / rms(ref))
