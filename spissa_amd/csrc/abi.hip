@@ -2397,11 +2397,13 @@ static int linear_run_q4(spissa_session *s, const spissa_linear_weight *w, const
   HIP_TRY(hipSetDevice(s->device));
   const size_t need = q4_linear_workspace(a.M, a.N, a.tiles, a.blocks, w->pack_group);
   std::unique_lock<std::mutex> lock(s->lin_mutex, std::defer_lock);
+  void *workspace = nullptr;  // (s->q4x is read and replaced under the lock alone)
   if (need) {
     lock.lock();
     ST_TRY(ensure_buf(s, s->q4x, need));
+    workspace = s->q4x.p;
   }
-  HIP_TRY(launch_q4_linear(s->stream, a, w->pack_group, w->param_type, s->q4x.p));
+  HIP_TRY(launch_q4_linear(s->stream, a, w->pack_group, w->param_type, workspace));
   return SPISSA_OK;
 }
 

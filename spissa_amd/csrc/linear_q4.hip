@@ -789,9 +789,11 @@ hipError_t launch_q4_linear(hipStream_t st, const Q4LinearArgs &base, int group,
   Q4LinearArgs a = base;
   a.mtiles = (a.M + 15) / 16;
   a.vec = a.K % 4 == 0 && (reinterpret_cast<uintptr_t>(a.x) & 15) == 0;
-  a.pieces = workspace;
-  a.inv = reinterpret_cast<const float *>(static_cast<char *>(workspace) + (size_t)a.mtiles * a.blocks * 8192);
-  a.partial = const_cast<float *>(a.inv) + a.mtiles * 16;
+  if (workspace) {
+    a.pieces = workspace;
+    a.inv = reinterpret_cast<const float *>(static_cast<char *>(workspace) + (size_t)a.mtiles * a.blocks * 8192);
+    a.partial = const_cast<float *>(a.inv) + a.mtiles * 16;
+  }
   switch (param_type) {
     case 0: return run_g<0>(st, a, group);
     case 1: return run_g<1>(st, a, group);

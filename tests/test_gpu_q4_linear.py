@@ -289,6 +289,40 @@ def test_several_threads_on_one_session(ses):
         assert np.array_equal(o.cpu().numpy(), r)
 
 
+def test_one_token_beside_a_growing_workspace(ses):
+    """One thread's calls need no workspace while another's replace it by larger ones."""
+    rng = np.random.default_rng(11)
+    own = Session(0)
+    wt = Weight(rng, 48, 512, 64)
+    w = wt.on(own)
+    one, many = acts(rng, 1, 512), acts(rng, 400, 512)
+    want = call(ses, wt.on(ses), one)
+    d_one, d_many = torch.from_numpy(one).cuda(), torch.from_numpy(many).cuda()
+    outs = [torch.zeros(1, 48, device="cuda") for _ in range(64)]
+    out = torch.zeros(400, 48, device="cuda")
+    torch.cuda.synchronize()
+    failed = []
+
+    def run(calls):
+        try:
+            for c in calls:
+                own.linear(w, *c)
+        except Exception as e:  # noqa: BLE001
+            failed.append(e)
+
+    threads = [threading.Thread(target=run, args=([(d_one, None, 1, o) for o in outs],)),
+               threading.Thread(target=run, args=([(d_many, None, m, out) for m in range(5, 401, 9)],))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    own.sync()
+    assert not failed
+    for o in outs:
+        assert np.array_equal(o.cpu().numpy(), want)
+    assert np.array_equal(out[:392].cpu().numpy(), call(ses, wt.on(ses), many[:392]))
+
+
 def test_refusals(ses):
     rng = np.random.default_rng(9)
     wt = Weight(rng, 20, 100, 32, "f16", True)
