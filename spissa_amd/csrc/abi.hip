@@ -1458,15 +1458,16 @@ static size_t q4_partial_bytes(size_t n, size_t Hq, size_t D, const Q4AttnPlan &
 
 // One query of each of B sequences, whose own row is its cache's last.
 // With `step` (its rows k and v, table and norm) the launch appends those rows first.
-// A few queries of one sequence (q4_few) likewise. extra: rows that the caches hold
-// beyond their lengths, or will.
+// A few queries of one sequence likewise, by the plan that q4_choose made. extra: rows
+// that the caches hold beyond their lengths, or will.
 struct Q4StepRows {
   const float *k, *v;
   const spissa_rope_table *table;
   const GemmaQkNorm *norm;
 };
 static int q4_attend_batch(spissa_session *s, const float *q, const spissa_kv_cache *const *caches, size_t batch,
-                           const spissa_kv_attention_config *c, float *out, const Q4StepRows *step, size_t extra) {
+                           const spissa_kv_attention_config *c, float *out, const Q4StepRows *step, size_t extra,
+                           const Q4AttnPlan *made = nullptr) {
   const int D = (int)c->head_dim, Hq = (int)c->num_heads, Hkv = (int)c->kv_heads, R = Hq / Hkv, S = (int)c->query_len;
   for (size_t b0 = 0; b0 < batch; b0 += kMaxDecodeBatch) {
     const int B = (int)std::min<size_t>(kMaxDecodeBatch, batch - b0);
@@ -1477,7 +1478,7 @@ static int q4_attend_batch(spissa_session *s, const float *q, const spissa_kv_ca
       a.seq[b].len = (int)(caches[b0 + b]->len + extra);
       keys[b] = c->window ? (int)std::min<size_t>(a.seq[b].len, c->window + S - 1) : a.seq[b].len;
     }
-    const Q4AttnPlan p = q4_attend_plan(D, S * R, Hkv, keys, B);
+    const Q4AttnPlan p = made ? *made : q4_attend_plan(D, S * R, Hkv, keys, B);
     ST_TRY(ensure_buf(s, s->partial, q4_partial_bytes(B, Hq, D, p, Hkv)));
     a.q = q + b0 * (size_t)Hq * D;
     a.out = out + b0 * (size_t)Hq * D;
@@ -1510,12 +1511,6 @@ static int q4_attend_batch(spissa_session *s, const float *q, const spissa_kv_ca
   return SPISSA_OK;
 }
 
-// The queries of the cache's last S rows; its length is `len`, those rows
-// included. q4_chunk_prepare makes its workspace.
-static Q4ChunkPlan q4_chunk_plan_of(spissa_session *s, size_t len, const spissa_kv_attention_config *c) {
-  return q4_chunk_plan((int)c->head_dim, (int)c->query_len, (int)(c->num_heads / c->kv_heads), (int)c->kv_heads, (int)len,
-                       c->causal ? 1 : 0, (int)c->window, s->cus);
-}
 // (the blocks of 128 rows of a head are the grid's second dimension)
 static int q4_chunk_limit(const spissa_kv_attention_config *c) {
   const size_t most = 65535 * (size_t)128;
@@ -1524,31 +1519,38 @@ static int q4_chunk_limit(const spissa_kv_attention_config *c) {
                    c->query_len, c->num_heads / c->kv_heads, most);
   return SPISSA_OK;
 }
-// Whether a chunk of a cache of `len` rows, the chunk's included, takes the single
-// queries' kernel, each of whose workgroups reads the keys for 512 / D rows: by the
-// two models' times. (us, single queries' kernel and chunk's, 24 heads on 8 of 128:
-// 4 queries over 100 keys 5.2 and 9.4, 32 over 1000 12.7 and 16.9, 4 over 8000 15
-// and 21, 8 over 8000 22 and 22, 16 37 and 24; 8 heads on 4 of 256, 4 over 100 6.6 and
-// 12.4, 16 over 8000 33 and 29.)
-static bool q4_few(spissa_session *s, size_t len, const spissa_kv_attention_config *c, Q4AttnPlan *plan) {
-  const size_t rows = c->query_len * (c->num_heads / c->kv_heads);
-  if (rows > 1024) return false;
-  const int keys = c->window ? (int)std::min<size_t>(len, c->window + c->query_len - 1) : (int)len;
-  *plan = q4_attend_plan((int)c->head_dim, (int)rows, (int)c->kv_heads, &keys, 1);
-  return plan->time < q4_chunk_plan_of(s, len, c).time;
+// How a chunk of a cache of `len` rows, the chunk's included, runs, decided once a
+// call. few: by the single queries' kernel, each of whose workgroups reads the keys for
+// 512 / D rows: by the two models' times. (us, single queries' kernel and chunk's, 24
+// heads on 8 of 128: 4 queries over 100 keys 5.2 and 9.4, 32 over 1000 12.7 and 16.9, 4
+// over 8000 15 and 21, 8 over 8000 22 and 22, 16 37 and 24; 8 heads on 4 of 256, 4 over
+// 100 6.6 and 12.4, 16 over 8000 33 and 29.)
+struct Q4Choice {
+  bool few = false;
+  Q4AttnPlan single{};
+  Q4ChunkPlan chunk;
+};
+static Q4Choice q4_choose(const spissa_session *s, size_t len, const spissa_kv_attention_config *c) {
+  Q4Choice p;
+  const size_t R = c->num_heads / c->kv_heads, rows = c->query_len * R;
+  p.chunk = q4_chunk_plan((int)c->head_dim, (int)c->query_len, (int)R, (int)c->kv_heads, (int)len, c->causal ? 1 : 0,
+                          (int)c->window, s->cus);
+  if (rows <= 1024) {
+    const int keys = c->window ? (int)std::min<size_t>(len, c->window + c->query_len - 1) : (int)len;
+    p.single = q4_attend_plan((int)c->head_dim, (int)rows, (int)c->kv_heads, &keys, 1);
+    p.few = p.single.time < p.chunk.time;
+  }
+  return p;
 }
-static int q4_chunk_prepare(spissa_session *s, size_t len, const spissa_kv_attention_config *c) {
-  Q4AttnPlan few;
-  if (q4_few(s, len, c, &few))
-    return ensure_buf(s, s->partial, q4_partial_bytes(1, c->num_heads, c->head_dim, few, c->kv_heads));
-  const Q4ChunkPlan p = q4_chunk_plan_of(s, len, c);
-  return p.partial_bytes ? ensure_buf(s, s->ppart, p.partial_bytes) : SPISSA_OK;
+// Its workspace; then the queries of the cache's last S rows.
+static int q4_chunk_prepare(spissa_session *s, const Q4Choice &p, const spissa_kv_attention_config *c) {
+  if (p.few) return ensure_buf(s, s->partial, q4_partial_bytes(1, c->num_heads, c->head_dim, p.single, c->kv_heads));
+  return p.chunk.partial_bytes ? ensure_buf(s, s->ppart, p.chunk.partial_bytes) : SPISSA_OK;
 }
 static int q4_attend_chunk(spissa_session *s, const float *q, const spissa_kv_cache *cache, size_t len,
-                           const spissa_kv_attention_config *c, float *out) {
-  Q4AttnPlan few;
-  if (q4_few(s, len, c, &few)) return q4_attend_batch(s, q, &cache, 1, c, out, nullptr, len - cache->len);
-  const Q4ChunkPlan p = q4_chunk_plan_of(s, len, c);
+                           const spissa_kv_attention_config *c, float *out, const Q4Choice &choice) {
+  if (choice.few) return q4_attend_batch(s, q, &cache, 1, c, out, nullptr, len - cache->len, &choice.single);
+  const Q4ChunkPlan &p = choice.chunk;
   const int D = (int)c->head_dim;
   Q4ChunkArgs a{};
   a.q = q;
@@ -1638,10 +1640,11 @@ static int q4_step(spissa_session *s, const spissa_rope_table *table, const floa
       ST_TRY(ensure_buf(s, s->q4q, S * cfg->num_heads * cfg->head_dim * sizeof(float)));
       q = (const float *)s->q4q.p;
     }
-    ST_TRY(q4_chunk_prepare(s, caches[0]->len + S, cfg));
+    const Q4Choice choice = q4_choose(s, caches[0]->len + S, cfg);
+    ST_TRY(q4_chunk_prepare(s, choice, cfg));
     ST_TRY(q4_append(s, caches, 1, S, q == d_q ? nullptr : d_q, cfg->num_heads, d_k, d_v, table, norm,
                      const_cast<float *>(q)));
-    ST_TRY(q4_attend_chunk(s, q, caches[0], caches[0]->len + S, cfg, d_out));
+    ST_TRY(q4_attend_chunk(s, q, caches[0], caches[0]->len + S, cfg, d_out, choice));
   }
   for (size_t b = 0; b < batch; ++b) caches[b]->len += S;
   return SPISSA_OK;
@@ -1953,8 +1956,9 @@ extern "C" int spissa_attention_cached_device(spissa_session *s, const float *d_
     ST_TRY(q4_chunk_limit(cfg));
     HIP_TRY(hipSetDevice(s->device));
     if (S == 1) return q4_attend_batch(s, d_q, &cache, 1, cfg, d_out, nullptr, 0);
-    ST_TRY(q4_chunk_prepare(s, cache->len, cfg));
-    return q4_attend_chunk(s, d_q, cache, cache->len, cfg, d_out);
+    const Q4Choice choice = q4_choose(s, cache->len, cfg);
+    ST_TRY(q4_chunk_prepare(s, choice, cfg));
+    return q4_attend_chunk(s, d_q, cache, cache->len, cfg, d_out, choice);
   }
   const int D = (int)cfg->head_dim;
   if (!prefill_supported(D) || s->prefill_precision != SPISSA_PREFILL_BF16)
