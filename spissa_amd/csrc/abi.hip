@@ -571,7 +571,7 @@ static int q4_append(spissa_session *s, spissa_kv_cache *const *caches, size_t B
                      float *q_out) {
   const size_t H = caches[0]->num_heads, D = caches[0]->head_dim;
   const size_t per = (q ? Hq : 0) + 2 * H;
-  const size_t most = std::max<size_t>(1, ((size_t)1 << 29) / per);  // tokens of a launch
+  const size_t most = std::max<size_t>(1, kQ4LaunchThreads / (D / 8) / per);  // tokens of a launch
   for (size_t b0 = 0; b0 < B; b0 += kMaxDecodeBatch)
     for (size_t t0 = 0; t0 < S; t0 += most) {
       const size_t nb = std::min<size_t>(kMaxDecodeBatch, B - b0), at = b0 * S + t0;

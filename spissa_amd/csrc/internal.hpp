@@ -342,7 +342,8 @@ struct Q4Rows {
 };
 // Rows of S tokens of each of up to kMaxDecodeBatch sequences, token-major as
 // the callers have them: q [B * S, Hq, D] (Hq 0: none), k and v [B * S, Hkv, D].
-// S * (Hq + 2 Hkv) < 2^30.
+// S * (Hq + 2 Hkv) rows of D / 8 threads: up to kQ4LaunchThreads.
+constexpr size_t kQ4LaunchThreads = (size_t)1 << 31;  // (HIP takes fewer than 2^32 in a grid's dimension)
 struct Q4AppendArgs {
   const float *q, *k, *v;
   float *q_out;             // the normed, rotated, prescaled query rows

@@ -778,10 +778,18 @@ hipError_t launch_q4_append(hipStream_t st, const Q4AppendArgs &a, int D, int B)
 }
 
 hipError_t launch_q4_rows(hipStream_t st, const Q4Rows &s, size_t n, size_t Hkv, size_t D, float *k_out, float *v_out) {
-  const size_t threads = n * Hkv * (D / 8);
-  const dim3 grid((unsigned)((threads + 255) / 256), 2);
-  hipLaunchKernelGGL(q4_rows_kernel, grid, dim3(256), 0, st, s, (int)n, (int)Hkv, (int)D, k_out, v_out);
-  return hipGetLastError();
+  const size_t most = std::max<size_t>(1, kQ4LaunchThreads / (Hkv * (D / 8)));  // rows of a launch
+  for (size_t at = 0; at < n; at += most) {
+    const size_t rows = std::min(most, n - at), out = at * Hkv * D;
+    Q4Rows from = s;
+    from.first += (int)at;
+    const dim3 grid((unsigned)((rows * Hkv * (D / 8) + 255) / 256), 2);
+    hipLaunchKernelGGL(q4_rows_kernel, grid, dim3(256), 0, st, from, (int)rows, (int)Hkv, (int)D, k_out ? k_out + out : nullptr,
+                       v_out ? v_out + out : nullptr);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 }  // namespace spissa

@@ -632,3 +632,26 @@ def test_few_queries_of_values_of_any_size(ses, s, scale):
     ses.attention_cached(dev(q), c, cfg, out)
     ses.sync()
     check(out, attend(q, hold(k), hold(v)), hold(v), f"values of {scale}, one row far larger")
+
+
+def test_rows_past_a_launch(ses):
+    """More rows in one append than a grid has threads for, which is under 2^32."""
+    n, h, d = 15900000, 17, 64
+    if torch.cuda.mem_get_info()[0] < 130 << 30:
+        pytest.skip("needs 130 GiB of device memory")
+    rng = np.random.default_rng(41)
+    x = torch.zeros(n, h, d, device="cuda")
+    places = [0, 7895159, 7895160, 7895161, 15790319, 15790320, 15790321, n - 1]
+    some = rows(rng, len(places), h, d)
+    x[torch.tensor(places, device="cuda")] = dev(some)
+    c = ses.q4_kv_cache(h, d, n)
+    ses.append(c, x, x, n)
+    ses.sync()
+    for i, at in enumerate(places):
+        gk, gv = held(ses, c, at, 1)
+        assert_bitwise(gk, hold(some[i:i + 1]), f"key {at}")
+        assert_bitwise(gv, hold(some[i:i + 1]), f"value {at}")
+    gk, _ = held(ses, c, 7895100, 60)
+    assert not np.any(gk[:59])
+    del x
+    torch.cuda.empty_cache()
