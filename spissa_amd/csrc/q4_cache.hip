@@ -458,7 +458,9 @@ __global__ __launch_bounds__(64 * kQ4Waves) void q4_attend_kernel(const Q4AttnAr
   for (int n = 0; n < CH; ++n) o[n] = (f32x4){0.f, 0.f, 0.f, 0.f};
   // The weights are scaled by a power of two, a column's own, that their products with
   // its group's steps keep two whole pieces: the largest step so far goes to 2^14..2^15,
-  // and one past `cap` moves the scale, as a score past m moves the reference.
+  // and one past `cap` moves the scale, as a score past m moves the reference. Beside
+  // references past 2^20, whose digits the scale's exponent would be lost in (and the
+  // weights overflow), it is 1, which no step is too large for.
   float omin = 0.0f, l = 0.0f, m = NEG_INF, cap = -1.0f;
   unsigned scale = 127u << 23;
   // (no copies of the next step's words: they are asked for when this step's are spent)
@@ -526,11 +528,13 @@ __global__ __launch_bounds__(64 * kQ4Waves) void q4_attend_kernel(const Q4AttnAr
       const float mnew = fmaxf(m, top), largest = max32(max16(half_lo(step)));
       float alpha = fast_exp2((m - safe_max(mnew)) * inv);
       m = mnew;
-      if (largest > cap) {  // (steps are no less than 2^-24: past 2^40 the sums would only overflow)
-        const unsigned to = min(scale_to(largest, 14), 167u << 23);
+      const bool far = fabsf(safe_max(m) * inv) >= 0x1p20f, was_far = cap > 0x1p100f;
+      if (far ? !was_far : was_far || largest > cap) {
+        // (steps are no less than 2^-24: past 2^40 the sums would only overflow)
+        const unsigned to = far ? 127u << 23 : min(scale_to(largest, 14), 167u << 23);
         alpha *= __uint_as_float(to) * inverse_scale(scale);
         scale = to;
-        cap = 60000.0f * inverse_scale(scale);
+        cap = far ? __builtin_inff() : 60000.0f * inverse_scale(scale);
       }
       l *= alpha;
       omin *= alpha;

@@ -370,13 +370,15 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void q4_chunk_kernel(const Q4Chunk
 #pragma unroll
         for (int e = 0; e < 4; ++e) top = fmaxf(top, s[k][e]);
       top = max32(max16(top)) * inv;
-      // The reference rises when a score passes it by 1.9, and a weight there is 2^14:
-      // weights stay below 2^15.9, in binary16's range, and the second piece, which ends
-      // at 2^-24, leaves two whole pieces down to 2^-16 of the reference's. (Keys of
-      // little weight count where the key that has most of it has no value. 3.9 and 2^12,
-      // which scale the output anew less often, take 1 % off 2048 queries.)
-      if (__any(top > m + 1.9f)) {
-        const float mnew = fmaxf(m, top);
+      // A weight is exp2(score - m), and m is set 14 below the largest score, which has
+      // the weight 2^14, and rises when a score passes it by 15.9: weights stay in
+      // binary16's range, and the second piece, which ends at 2^-24, leaves two whole
+      // pieces down to 2^-16 of the largest. (Keys of little weight count where the key
+      // that has most of it has no value. 12 and 15.9, which scale the output anew less
+      // often, take 1 % off 2048 queries.) Scores past 2^20, whose digits 14 would be
+      // lost in, are references themselves.
+      if (__any(top - m > 15.9f)) {
+        const float mnew = fmaxf(m, fabsf(top) < 0x1p20f ? top - 14.0f : top);
         const float alpha = fast_exp2(m - safe_max(mnew));
         m = mnew;
         l *= alpha;
@@ -385,7 +387,7 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void q4_chunk_kernel(const Q4Chunk
 #pragma unroll
           for (int e = 0; e < 4; ++e) o[d][e] *= alpha;
       }
-      const float shift = 14.0f - safe_max(m);
+      const float shift = -safe_max(m);
       float p[8];
 #pragma unroll
       for (int k = 0; k < 2; ++k)

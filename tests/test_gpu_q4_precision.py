@@ -173,3 +173,33 @@ def test_small_values_beside_a_large_one(ses, d, hq, hkv, s, at):
     keys, values = hold(k), hold(v)
     ref = attend(q, keys, values)
     check(attention(ses, q, c, hkv), ref, score_size(q, keys), f"d {d} s {s}, a large row", 2 * 2.0**-38 * np.max(np.abs(values)) / rms(ref))
+
+
+@pytest.mark.parametrize("d,hq,hkv", [(64, 8, 2), (128, 6, 2), (256, 4, 1)])
+@pytest.mark.parametrize("s", [1, 5, 550])
+@pytest.mark.parametrize("size", [1e5, 1e7, 1e9, 1e30])
+@pytest.mark.parametrize("value", [1.0, 0.02])
+def test_scores_of_any_size(ses, d, hq, hkv, s, size, value):
+    """Scores whose largest takes the whole weight: its value comes back, to a weight of two
+    pieces and seven roundings of the step's part, the minimum's and their sum over the
+    weight's, each at most 1.1 of the largest value: under sixteen of 2^-24 together. Where
+    two scores are within their roundings of each other the row says nothing: 24 of 2^-24 A
+    each, and 30 to make the second's weight vanish."""
+    rng = np.random.default_rng(d + s)
+    n = 600
+    k, v = rng.standard_normal((2, n, hkv, d)).astype(np.float32)
+    v *= np.float32(value)  # (and with them the scale that the weights are held at)
+    q = (rng.standard_normal((s, hq, d)) * size).astype(np.float32)
+    c = ses.q4_kv_cache(hkv, d, n)
+    ses.append(c, dev(k), dev(v), n)
+    keys, values = hold(k), hold(v)
+    got, ref = attention(ses, q, c, hkv), attend(q, keys, values)
+    assert np.isfinite(got).all()
+    sc = np.einsum("shd,nhd->shn", q.astype(np.float64), np.repeat(keys, hq // hkv, axis=1)) / np.sqrt(d)
+    pos = np.arange(n - s, n)[:, None, None]
+    sc = np.sort(np.where(np.arange(n) > pos, -np.inf, sc), axis=2)
+    clear = sc[:, :, -1] - sc[:, :, -2] > 30 + 48 * 2.0**-24 * score_size(q, keys)
+    assert clear.mean() > 0.5
+    off = np.max(np.abs(got - ref)[clear]) / np.max(np.abs(values))
+    print(f"[q4 precision] d {d} s {s} scores of {size}: {off:.2e}, {clear.mean():.2f} of the rows", flush=True)
+    assert off <= 2.0**-20, off
