@@ -690,10 +690,17 @@ hipError_t attend(hipStream_t st, const Q4AttnArgsOf<MB> &a, int nz) {
   auto kernel = a.k ? q4_attend_kernel<D, MB, true, false> : q4_attend_kernel<D, MB, false, false>;
   if constexpr (MB == 1)
     if (a.S > 1) kernel = q4_attend_kernel<D, MB, false, true>;
-  // One workgroup a CU: two, which heads of 64 have the registers for, come together
-  // while other CUs stay empty, so LDS that nothing uses keeps them apart. (16 sequences
-  // of 2432 to 8192 keys, 32 heads on 8 of 64: 28 us, 42 without.)
-  const unsigned apart = D == 64 ? 62 * 1024 : 0;
+  // One workgroup a CU where that is all there are: two, which heads of 64 have the
+  // registers for, come together while other CUs stay empty, so LDS that nothing uses
+  // keeps them apart. (16 sequences of 2432 to 8192 keys, 32 heads on 8 of 64: 28 us, 42
+  // without. More workgroups go better two a CU: 16 of 1024 keys, 32 heads on 32, 16 us,
+  // 19 with it.)
+  long live = 0;
+  for (int z = 0; z < nz; ++z) {
+    const int keys = a.window > 0 ? (int)std::min<long>(a.seq[z].len, (long)a.window + a.S - 1) : a.seq[z].len;
+    live += (keys + a.kps - 1) / a.kps * (long)grid.x;
+  }
+  const unsigned apart = D == 64 && live <= kQ4GridWorkgroups ? 62 * 1024 : 0;
   hipLaunchKernelGGL(kernel, grid, dim3(64 * kQ4Waves), apart, st, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.max_splits == 1) return e;
