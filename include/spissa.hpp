@@ -571,10 +571,10 @@ class Session {
   }
   // Append-first attention of one token of each sequence over 4-bit caches.
   Result<void> attention_cached_batch(const float *d_q, const std::vector<const KvCache *> &caches,
-                                      const KvAttentionConfig &config, float *d_out) {
-    std::vector<const spissa_kv_cache *> raw;
-    for (const KvCache *c : caches) raw.push_back(c->raw());
-    const spissa_kv_attention_config c = config.c();
+                                      const KvAttentionConfig &cfg, float *d_out) const {
+    std::vector<const spissa_kv_cache *> raw(caches.size());
+    for (size_t i = 0; i < caches.size(); ++i) raw[i] = caches[i] ? caches[i]->raw() : nullptr;
+    const auto c = cfg.c();
     return detail::check(spissa_attention_cached_batch_device(s_, d_q, raw.data(), raw.size(), &c, d_out));
   }
   // freq_scale: Llama per-pair scales (nullptr = None); position_divisor: Gemma only.

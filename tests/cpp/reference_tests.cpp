@@ -695,6 +695,92 @@ TEST(kv_cache_clone_is_independent) {
   CHECK(cache.is_empty() && copy.values() == (std::vector<float>{3, 4}));
 }
 
+// A 4-bit cache's refusals come before any device work.
+HOST_TEST(four_bit_cache_rejects_shapes) {
+  CHECK(KvCache::create_q4(2, 32, 8).error().kind == ErrorKind::Shape);
+  CHECK(KvCache::create_q4(0, 64, 8).error().kind == ErrorKind::Shape);
+  CHECK(KvCache::create_q4(2, 64, ((size_t)1 << 24) + 1).error().kind == ErrorKind::Shape);
+}
+
+// Rows of whole numbers 0..15 are what 4 bits hold exactly, so every result is too:
+// queries of zeros give the mean of the values.
+TEST(four_bit_cache_steps_on_device) {
+  const size_t Hq = 4, Hkv = 2, D = 64, P = 7;
+  auto session = ok(Session::create(0));
+  std::vector<float> k((P + 1) * Hkv * D), v(k.size());
+  for (size_t i = 0; i < k.size(); ++i) {
+    k[i] = (float)(i % 16);
+    v[i] = (float)((i * 7 + i / 64) % 16);
+  }
+  auto cache = ok(session.kv_cache_q4(Hkv, D, P + 1)), twin = ok(KvCache::create_q4(Hkv, D, P + 1));
+  CHECK(cache.is_q4() && twin.is_q4() && !ok(session.kv_cache(Hkv, D, 2)).is_q4());
+  ok(cache.append(slice(k, 0, P * Hkv * D), slice(v, 0, P * Hkv * D), P));
+  ok(twin.append(k, v, P + 1));
+  CHECK(cache.keys() == slice(k, 0, P * Hkv * D) && twin.values() == v);
+
+  float *dq = nullptr, *dk = nullptr, *dv = nullptr, *dout = nullptr, *drows = nullptr;
+  CHECK(hipMalloc(&dq, Hq * D * 4) == hipSuccess && hipMalloc(&dk, Hkv * D * 4) == hipSuccess &&
+        hipMalloc(&dv, Hkv * D * 4) == hipSuccess && hipMalloc(&dout, Hq * D * 4) == hipSuccess &&
+        hipMalloc(&drows, 2 * Hkv * D * 4) == hipSuccess);
+  CHECK(hipMemset(dq, 0, Hq * D * 4) == hipSuccess);
+  CHECK(hipMemcpy(dk, k.data() + P * Hkv * D, Hkv * D * 4, hipMemcpyHostToDevice) == hipSuccess);
+  CHECK(hipMemcpy(dv, v.data() + P * Hkv * D, Hkv * D * 4, hipMemcpyHostToDevice) == hipSuccess);
+  CHECK(hipDeviceSynchronize() == hipSuccess);
+  const KvAttentionConfig config{1, Hq, Hkv, D, true};
+  std::vector<float> expected(Hq * D), got(Hq * D), rows(2 * Hkv * D);
+  for (size_t h = 0; h < Hq; ++h)
+    for (size_t d = 0; d < D; ++d) {
+      for (size_t t = 0; t <= P; ++t) expected[h * D + d] += v[(t * Hkv + h / (Hq / Hkv)) * D + d] / (float)(P + 1);
+    }
+  auto compare = [&] {
+    ok(session.sync());
+    CHECK(hipMemcpy(got.data(), dout, got.size() * 4, hipMemcpyDeviceToHost) == hipSuccess);
+    assert_close_vec(got, expected, 15.0f * 0x1p-20f);  // sixteen roundings of 2^-24 of 15
+  };
+  ok(session.decode_step(nullptr, dq, dk, dv, {&cache}, config, dout));
+  compare();
+  CHECK(cache.len() == P + 1 && cache.keys() == k && cache.values() == v);
+  CHECK(hipMemset(dout, 0, Hq * D * 4) == hipSuccess && hipDeviceSynchronize() == hipSuccess);
+  ok(session.attention_cached_batch(dq, {&cache}, config, dout));
+  compare();
+  ok(cache.rows_device(P - 1, 2, drows, nullptr));
+  ok(session.sync());
+  CHECK(hipMemcpy(rows.data(), drows, rows.size() * 4, hipMemcpyDeviceToHost) == hipSuccess);
+  CHECK(rows == slice(k, (P - 1) * Hkv * D, (P + 1) * Hkv * D));
+  CHECK(cache.rows_device(P, 2, drows, nullptr).error().kind == ErrorKind::Shape);
+  CHECK(session.attention_cached_batch(dq, {&cache, nullptr}, config, dout).error().kind == ErrorKind::Argument);
+  CHECK(session.attention(dq, dk, dv, &cache, config, dout).error().kind == ErrorKind::Argument);
+  for (float *p : {dq, dk, dv, dout, drows}) (void)hipFree(p);
+}
+
+// Whole numbers again: every product and sum is exact.
+TEST(four_bit_weights_project_exactly) {
+  const size_t N = 19, K = 70, G = 32;
+  std::vector<uint8_t> codes(N * (K / 2)), zeros(N * 3);
+  std::vector<float> scales(N * 3), x(K);
+  for (size_t i = 0; i < codes.size(); ++i) codes[i] = (uint8_t)(i * 37 + i / 11);
+  for (size_t i = 0; i < zeros.size(); ++i) {
+    zeros[i] = (uint8_t)(i % 16);
+    scales[i] = (float)(1 + i % 3);
+  }
+  for (size_t i = 0; i < K; ++i) x[i] = (float)(int)(i % 9) - 4.0f;
+  for (bool with_zeros : {false, true}) {
+    auto w = ok(LinearWeight::create_q4(N, K, G, codes.data(), codes.size(), DType::F32, scales.data(), scales.size() * 4,
+                                        with_zeros ? zeros.data() : nullptr, with_zeros ? zeros.size() : 0));
+    auto got = ok(linear(w, x, nullptr, StreamingLinearConfig{1, K, N}));
+    for (size_t n = 0; n < N; ++n) {
+      float expected = 0.0f;
+      for (size_t i = 0; i < K; ++i) {
+        const int code = codes[n * (K / 2) + i / 2] >> (i % 2 ? 4 : 0) & 15, zero = with_zeros ? zeros[n * 3 + i / G] : 8;
+        expected += x[i] * scales[n * 3 + i / G] * (float)(code - zero);
+      }
+      CHECK(got[n] == expected);
+    }
+  }
+  CHECK(LinearWeight::create_q4(N, K, 48, codes.data(), codes.size(), DType::F32, scales.data(), scales.size() * 4).error().kind ==
+        ErrorKind::Shape);
+}
+
 // Device tier: one fused decode step (RoPE + attention + append in two
 // launches) equals the drop-in call sequence of models/llama/generate.rs:383-416
 // (RoPE, cached attention, append) at Llama-3.2-1B head geometry.
