@@ -12,7 +12,7 @@ import numpy as np
 import pytest
 import torch
 
-from spissa_amd import InvalidTensorDataError
+from spissa_amd import InvalidTensorDataError, RotaryEmbeddingConfig, apply_gemma_rotary_inplace, rms_norm
 from spissa_amd.device import Session
 from spissa_amd.rotary import KvAttentionConfig
 from tests.q4 import attend, hold
@@ -203,3 +203,74 @@ def test_scores_of_any_size(ses, d, hq, hkv, s, size, value):
     off = np.max(np.abs(got - ref)[clear]) / np.max(np.abs(values))
     print(f"[q4 precision] d {d} s {s} scores of {size}: {off:.2e}, {clear.mean():.2f} of the rows", flush=True)
     assert off <= 2.0**-20, off
+
+
+@pytest.mark.parametrize("d,hq,hkv", [(64, 8, 2), (128, 6, 2), (256, 4, 2)])
+@pytest.mark.parametrize("batch", [1, 5, 17])
+@pytest.mark.parametrize("window", [0, 64])
+def test_gemma_steps_of_a_batch(ses, d, hq, hkv, batch, window):
+    """Norm, rotation, prescale, append and attention of a token of each of several
+    sequences. The norm's sum is a tree where the plain form's is a chain: each is off by
+    at most d / 2 roundings of 2^-24, so queries and keys may differ by 2^-16 of themselves
+    (d 256) at worst, and by 2^-21 in RMS. The reference takes the keys as they were held."""
+    eps, prescale = 1e-6, 0.5
+    rng = np.random.default_rng(d + batch)
+    lens = [int(x) for x in rng.integers(0, 900, batch)]
+    lens[0] = 0
+    q, k, v = (rng.standard_normal((batch, h, d)).astype(np.float32) for h in (hq, hkv, hkv))
+    qn, kn = (1 + 0.1 * rng.standard_normal((2, d))).astype(np.float32)
+    table = ses.rope_table(1, d, 10000.0, 8.0, max_positions=max(lens) + 1)
+    caches, held = [], []
+    for n in lens:
+        pk, pv = rng.standard_normal((2, n, hkv, d)).astype(np.float32)
+        caches.append(ses.q4_kv_cache(hkv, d, n + 1))
+        if n:
+            ses.append(caches[-1], dev(pk), dev(pv), n)
+        held.append((hold(pk), hold(pv)))
+    out = torch.full((batch, hq, d), np.nan, device="cuda")
+    ses.gemma_decode_step(table, dev(q), dev(k), dev(v), caches, KvAttentionConfig(1, hq, hkv, d, True, window), dev(qn), dev(kn), eps,
+                          prescale, out)
+    ses.sync()
+    got = out.cpu().numpy()
+    for b, n in enumerate(lens):
+        qr = rms_norm(q[b].ravel(), qn, hq, d, eps)
+        kr = rms_norm(k[b].ravel(), kn, hkv, d, eps)
+        apply_gemma_rotary_inplace(qr, kr, hq, hkv, RotaryEmbeddingConfig(1, hq, d, d, 10000.0, n), 8.0)
+        assert len(caches[b]) == n + 1
+        keys, values = caches[b].keys().reshape(n + 1, hkv, d), caches[b].values().reshape(n + 1, hkv, d)
+        assert np.array_equal(keys[:n].view(np.uint32), held[b][0].view(np.uint32))
+        assert np.array_equal(values.view(np.uint32), np.concatenate([held[b][1], hold(v[b:b + 1])]).view(np.uint32))
+        near, step = hold(kr.reshape(1, hkv, d)), np.ptp(kr.reshape(-1, 32), axis=1).repeat(32).reshape(1, hkv, d) / 15
+        assert np.all(np.abs(keys[n:] - near) <= 1.01 * step + 1e-3 * np.abs(near)), f"key of sequence {b}"
+        qr = (qr * np.float32(prescale)).reshape(1, hq, d)
+        a = score_size(qr, keys)
+        check(got[b:b + 1], attend(qr, keys, values, True, window), a, f"d {d} sequence {b} of {n}", 2.0**-21 * a)
+
+
+@pytest.mark.parametrize("d,hq,hkv", [(64, 32, 8), (128, 6, 2), (256, 4, 1)])
+@pytest.mark.parametrize("s,past", [(1, 0), (1, 40), (1, 5000), (6, 700), (40, 3000), (300, 20), (530, 900)])
+def test_outputs(ses, d, hq, hkv, s, past):
+    """Ordinary rows, against the outputs' own size: a second piece left out anywhere
+    (2^-12 of a query, a weight or a value) is tens of times the tolerance."""
+    rng = np.random.default_rng(d + s + past)
+    n = s + past
+    k, v = rng.standard_normal((2, n, hkv, d)).astype(np.float32)
+    k += rng.standard_normal((hkv, d)).astype(np.float32)  # channels' own offsets
+    q = rng.standard_normal((s, hq, d)).astype(np.float32)
+    c = ses.q4_kv_cache(hkv, d, n)
+    if past:
+        ses.append(c, dev(k[:past]), dev(v[:past]), past)
+    keys, values = hold(k), hold(v)
+    a = score_size(q, keys)
+    out = torch.full((s, hq, d), np.nan, device="cuda")
+    for window in (0, 100):
+        c.truncate(past)
+        cfg = KvAttentionConfig(s, hq, hkv, d, True, window)
+        args = dev(q), dev(k[past:]), dev(v[past:])
+        ses.decode_step(None, *args, [c], cfg, out) if s == 1 else ses.prefill_step(None, *args, c, cfg, out)
+        ses.sync()
+        ref = attend(q, keys, values, True, window)
+        check(out.cpu().numpy(), ref, a, f"d {d} step {s}+{past} window {window}")
+        got = attention(ses, q, c, hkv, window=window)
+        assert np.array_equal(got.view(np.uint32), out.cpu().numpy().view(np.uint32)), "the attention alone"
+    check(attention(ses, q, c, hkv, causal=False), attend(q, keys, values, False), a, f"d {d} {s}+{past} not causal")
