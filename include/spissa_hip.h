@@ -138,9 +138,9 @@ int spissa_kv_cache_rows_device(const spissa_kv_cache *c, size_t first, size_t c
  * and spissa_{,gemma_}prefill_step_device, and spissa_attention_sublayer_device.
  * In the Gemma steps the QK-norm's sums of squares are taken as a tree. Sums and
  * softmax are f32 (prefill precision does not matter here). Queries, softmax
- * weights and, where more queries take the chunk kernel, values are held to 2^-23
- * of themselves; weights and values not below 2^-38 of the largest among the keys
- * that the call reads. The
+ * weights and, where more queries take the chunk kernel, values are rounded to
+ * 2^-23 of themselves, or to 2^-34 of the largest of their row or, weights and
+ * values, to 2^-38 of the largest of the call, where that is more. The
  * calls that take current rows beside the cache (spissa_attention_device,
  * spissa_attention_decode_batch_device,
  * spissa_scaled_dot_product_attention_with_cache) and
@@ -435,9 +435,10 @@ int spissa_linear_weight_new(spissa_session *s, int dtype, size_t out_features, 
  *
  * The handle is a spissa_linear_weight: spissa_linear, spissa_linear_device (up
  * to 1048560 tokens), the LM head calls and spissa_attention_sublayer_device
- * take it. Activations are held to 22 bits, down to 2^-28 of the largest of
- * their row (up to four tokens: of 256 channels of it); sums are f32. An
- * infinite or NaN activation gives what the plain product would. Above four
+ * take it. Activations are rounded to 2^-23 of themselves, or to 2^-38 of the
+ * largest of their row (up to four tokens: of 512 channels of it) where that is
+ * more, which it is below 2^-15 of the largest; sums are f32, and take scales up to
+ * 2^96. An infinite or NaN activation gives what the plain product would. Above four
  * tokens a call uses a workspace that grows with the tokens: under graph
  * capture it must follow a call of the same size. spissa_plan_linear describes
  * the other types. */

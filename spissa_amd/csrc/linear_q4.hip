@@ -5,11 +5,12 @@
 // Products run on v_mfma_f32_16x16x32_f16. A weight without its scale,
 // code - zero, is a whole number of at most 15 and so exact in binary16; an
 // activation is scaled by a power of two that takes the largest of its row (or
-// of 256 channels of it) to 2^13..2^14, and split into two binary16 pieces, the
-// nearest one and the nearest of what is left: 22 bits of each activation down
-// to 2^-28 of the largest, and nothing above 2^-38 of the largest is lost. The
-// products of a group are summed in f32 and scaled once, so the arithmetic is
-// that of f32 sums, at two matrix instructions for 512 weights.
+// of 512 channels of it) to 2^13..2^14, and split into two binary16 pieces, the
+// nearest one and the nearest of what is left: off by at most 2^-23 of each
+// activation down to 2^-15 of the largest, and below by at most 2^-38 of the
+// largest, where the second piece's last digit is. The products of a group are
+// summed in f32 and scaled once, so the arithmetic is that of f32 sums, at two
+// matrix instructions for 512 weights.
 //
 // HBM layout, made once when a weight is created: rows in tiles of 16, K in
 // blocks of 128. A tile's block is 1 KB of codes in the order in which a wave's

@@ -27,8 +27,6 @@ __device__ __forceinline__ unsigned half_bits(float v) {
   return __builtin_bit_cast(unsigned short, (_Float16)v);
 }
 
-
-
 template <int N>
 __device__ __forceinline__ void words(const char *p, unsigned (&w)[N]) {
   if constexpr (N == 1) {
@@ -315,12 +313,12 @@ __device__ __forceinline__ long row_of(const Q4AttnArgsOf<MB> &a, int z, int h, 
 // one a product. Operands are code - 8 (times 2^-9), with min + 8 step beside them:
 // with the codes as they are, the sums of many keys' values would grow, and cancel
 // against the minima's only at the end (outputs over 8192 keys were 1e-6 off).
-// Queries and weights are two binary16 pieces.
+// Queries and weights are two nearest binary16 pieces.
 // Bound: HBM for many keys, latency (one step of loads, one of sums) for few.
-// 16 sequences of 8192 keys, 24 heads on 8 of 128: 39 us, 4.3 TB/s of codes and
-// params (a copy reaches 5.1); 32768 keys of one head of 256: 12 us; 512 keys, 32
-// heads on 8 of 64: 6 us. Outputs are 1.2e-7 off (RMS, relative), as a plain f32
-// form's are.
+// 16 sequences of 8192 keys, 24 heads on 8 of 128: 40 us, 4.2 TB/s of codes and
+// params (a plain read reaches 6.0 to 6.6); 32768 keys of one head of 256: 13 us; 512
+// keys, 32 heads on 8 of 64: 6 us. Outputs are 1e-7 off (RMS, relative), where a plain
+// f32 form's are 1e-7 to 7e-7.
 // STEP: the fused step of one token. Every workgroup prepares its queries and
 // holds the sequence's new row of its head in LDS (as q4_append_kernel does, bit for
 // bit), and takes that row from there; the one with the last range and the first heads

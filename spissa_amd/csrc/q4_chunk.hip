@@ -3,7 +3,7 @@
 //
 // The products are f32's in all but name. Scores: a code is a whole number and
 // so exact in binary16; the queries, scaled by a power of two that takes their
-// row's largest to 2^9..2^10, are two binary16 pieces (22 bits). A 32-channel
+// row's largest to 2^9..2^10, are two nearest binary16 pieces. A 32-channel
 // group is the depth of one instruction, so its product is scaled by the key's
 // step in f32, and the minima times the queries' group sums (three pieces) are
 // one more instruction over the groups:
@@ -23,9 +23,9 @@
 //
 // Bound: the matrix cores beside the vector work of scaling, softmax, pieces and
 // widening: of a SIMD's time at 512 queries over 8192 keys (24 heads on 8 of 128,
-// 147 us with the merge, 340 TFLOP/s of the plain products) matrix instructions
+// 150 us with the merge, 330 TFLOP/s of the plain products) matrix instructions
 // take half, and vector ones' issue, in which a matrix instruction takes two
-// slots, about as much; the two overlap in part.
+// slots, three fifths; the two overlap in part.
 #include <algorithm>
 #include <type_traits>
 
@@ -35,8 +35,6 @@
 namespace spissa {
 
 namespace {
-
-
 
 // A key row's eight codes of a word in the order in which weights of a pair
 // come off it: 0, 4, 1, 5, 2, 6, 3, 7 (queries are put in that order too).
