@@ -402,3 +402,51 @@ def test_sublayer_of_4_bit_weights_over_a_4_bit_cache(ses, mixed):
         assert np.all(np.abs(values[at:].reshape(-1, 32) - v.reshape(-1, 32)) <= 0.52 * step[:, None] + 2e-3)
         at += s
     assert len(cache) == at
+
+
+def test_gemma_sublayer_of_4_bit_weights_over_a_4_bit_cache(ses):
+    """The same through a Gemma layer's: norms of queries and keys, a prescale, positions
+    divided by eight, a window, a norm behind. Scores reach A = 16 / 4 = 4 at most (rows of
+    norm 16, sqrt(256), a prescale of 1/4), off by the angles' 25 * 2^-24 and the sums' 1e-5
+    of them: under 5e-5 in a weight; the output's own sums and norms are 2e-5."""
+    hidden, hq, hkv, d, eps, prescale, window = 320, 4, 2, 256, 1e-6, 0.25, 60
+    rng = np.random.default_rng(12)
+    made = {t: Weight(rng, n, k, 32, "f16", True, size=0.02) for t, (n, k) in
+            {"q": (hq * d, hidden), "k": (hkv * d, hidden), "v": (hkv * d, hidden), "o": (hidden, hq * d)}.items()}
+    w = {t: m.on(ses) for t, m in made.items()}
+    nw, pw = (1 + 0.1 * rng.standard_normal((2, hidden))).astype(np.float32)
+    qn, kn = (1 + 0.1 * rng.standard_normal((2, d))).astype(np.float32)
+    on = lambda a: torch.from_numpy(a).cuda()  # noqa: E731
+    layer = AttentionLayer(hidden, hq, hkv, d, w["q"], w["k"], w["v"], w["o"], input_norm=on(nw), q_norm=on(qn), k_norm=on(kn),
+                           post_norm=on(pw), eps=eps, rope=ses.rope_table(1, d, 10000.0, 8.0, max_positions=200),
+                           q_prescale=prescale, window=window)
+    cache = ses.q4_kv_cache(hkv, d, 200)
+    inv = 1.0 / 10000.0 ** (np.arange(0, d, 2) / d)
+    at = 0
+
+    def rotated(y, s):
+        ang = (np.arange(at, at + s)[:, None] / 8.0 * inv)[:, None, :]
+        a, b = y[..., :d // 2], y[..., d // 2:]
+        return np.concatenate([a * np.cos(ang) - b * np.sin(ang), b * np.cos(ang) + a * np.sin(ang)], -1)
+
+    for s in (90, 1, 6, 40, 1):
+        x = acts(rng, s, hidden)
+        out = torch.empty(s, hidden, device="cuda")
+        ses.attention_sublayer(layer, on(x), s, cache, out)
+        rows = [torch.empty(at + s, hkv, d, device="cuda") for _ in range(2)]
+        ses.cache_rows(cache, 0, at + s, *rows)
+        ses.sync()
+        keys, values = (r.cpu().numpy() for r in rows)
+        xn = norm(x.astype(np.float64), nw, eps)
+        q = rotated(norm((xn @ made["q"].w.T).reshape(s, hq, d), qn, eps), s) * prescale
+        ref = norm(attend(q, keys, values, True, window).reshape(s, hq * d) @ made["o"].w.T, pw, eps)
+        err = np.max(np.abs(out.cpu().numpy() - ref)) / np.max(np.abs(ref))
+        print(f"[q4 sublayer] gemma, {s} tokens: {err:.2e}", flush=True)
+        assert err <= 1e-4, (s, err)
+        k = rotated(norm((xn @ made["k"].w.T).reshape(s, hkv, d), kn, eps), s)
+        for got, y in ((keys, k), (values, (xn @ made["v"].w.T).reshape(s, hkv, d))):
+            g = y.reshape(-1, 32)
+            step = (g.max(1) - g.min(1)) / 15
+            assert np.all(np.abs(got[at:].reshape(-1, 32) - g) <= 0.52 * step[:, None] + 2e-3 * np.max(np.abs(g), axis=1, keepdims=True))
+        at += s
+    assert len(cache) == at
