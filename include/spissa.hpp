@@ -648,6 +648,49 @@ class Session {
     return detail::check(
         spissa_lm_head_device(s_, table.raw(), d_hidden, detail::excluded_arg(excluded), d_logits, d_token));
   }
+  // One token of each row of d_logits [rows, vocab] by the settings of cfg; d_probs may be null.
+  Result<void> sample(const float *d_logits, const float *d_uniform, const spissa_sampling_config &cfg,
+                      int32_t *d_tokens, float *d_probs = nullptr) const {
+    return detail::check(spissa_sample_device(s_, d_logits, d_uniform, &cfg, d_tokens, d_probs));
+  }
+  // A tree of drafted tokens of each sequence through one layer; nodes[b] tokens of sequence b.
+  Result<void> tree_step(const RopeTable *table, const float *d_q, const float *d_k, const float *d_v,
+                         const std::vector<KvCache *> &caches, const std::vector<size_t> &nodes,
+                         const int32_t *d_parents, const KvAttentionConfig &cfg, float *d_out) const {
+    if (nodes.size() != caches.size()) return sequences_error(nodes.size(), caches.size());
+    const auto raw = handles(caches);
+    const auto c = cfg.c();
+    return detail::check(spissa_tree_step_device(s_, table ? table->raw() : nullptr, d_q, d_k, d_v, raw.data(),
+                                                 nodes.data(), raw.size(), d_parents, &c, d_out));
+  }
+  // The same for a Gemma 3 layer: QK-norm, Gemma RoPE, q prescale.
+  Result<void> gemma_tree_step(const RopeTable &table, const float *d_q, const float *d_k, const float *d_v,
+                               const std::vector<KvCache *> &caches, const std::vector<size_t> &nodes,
+                               const int32_t *d_parents, const KvAttentionConfig &cfg, const float *d_q_norm,
+                               const float *d_k_norm, float eps, float q_prescale, float *d_out) const {
+    if (nodes.size() != caches.size()) return sequences_error(nodes.size(), caches.size());
+    const auto raw = handles(caches);
+    const auto c = cfg.c();
+    return detail::check(spissa_gemma_tree_step_device(s_, table.raw(), d_q, d_k, d_v, raw.data(), nodes.data(),
+                                                       raw.size(), d_parents, &c, d_q_norm, d_k_norm, eps, q_prescale,
+                                                       d_out));
+  }
+  // The drafted tokens that the sampled ones confirm.
+  Result<void> tree_accept(const int32_t *d_parents, const int32_t *d_tokens, const int32_t *d_sampled,
+                           const std::vector<size_t> &nodes, int32_t *d_path, int32_t *d_count,
+                           int32_t *d_next) const {
+    return detail::check(spissa_tree_accept_device(s_, d_parents, d_tokens, d_sampled, nodes.data(), nodes.size(),
+                                                   d_path, d_count, d_next));
+  }
+  // Moves the accepted nodes' rows together in the caches of every layer; the lengths stay.
+  Result<void> keep_rows(const std::vector<KvCache *> &caches, const std::vector<size_t> &nodes,
+                         const int32_t *d_path, const int32_t *d_count) const {
+    if (nodes.empty() ? !caches.empty() : caches.size() % nodes.size() != 0)
+      return sequences_error(nodes.size(), caches.size());
+    const auto raw = handles(caches);
+    return detail::check(spissa_kv_cache_keep_device(s_, raw.data(), nodes.empty() ? 0 : raw.size() / nodes.size(),
+                                                     nodes.data(), nodes.size(), d_path, d_count));
+  }
   // RoPE + attention + append of one decode step of one layer (table = nullptr: no RoPE).
   Result<void> decode_step(const RopeTable *table, const float *d_q, const float *d_k, const float *d_v,
                            const std::vector<KvCache *> &caches, const KvAttentionConfig &cfg, float *d_out) const {
@@ -659,6 +702,15 @@ class Session {
   }
 
  private:
+  static std::vector<spissa_kv_cache *> handles(const std::vector<KvCache *> &caches) {
+    std::vector<spissa_kv_cache *> raw(caches.size());
+    for (size_t i = 0; i < caches.size(); ++i) raw[i] = caches[i] ? caches[i]->raw() : nullptr;
+    return raw;
+  }
+  static RuntimeError sequences_error(size_t nodes, size_t caches) {
+    return RuntimeError{ErrorKind::Shape,
+                        std::to_string(nodes) + " counts of nodes for " + std::to_string(caches) + " caches"};
+  }
   explicit Session(spissa_session *s) : s_(s) {}
   spissa_session *s_ = nullptr;
 };

@@ -2,7 +2,8 @@
  * spissa_hip.h -- C ABI of the MI355X (gfx950) attention path for the Spissa
  * runtime: RoPE, the per-layer KV cache, cached SDPA (decode and causal GQA
  * prefill), the Gemma 3 QK-norm, the linear projections either side, and
- * the LM head with greedy sampling after the last layer.
+ * the LM head with greedy sampling after the last layer; beside the runtime's
+ * items, decoding with drafted tokens and sampling.
  *
  * Every symbol here replaces one Rust item of crates/spissa-runtime; the
  * citation next to each declaration names it (paths relative to the
@@ -556,6 +557,107 @@ typedef struct {
 int spissa_attention_sublayer_device(spissa_session *s, const spissa_attention_layer *layer,
                                      const float *d_x, size_t seq_len, spissa_kv_cache *cache,
                                      float *d_out);
+
+/* ------------------------------------------------------------------------ */
+/* Sampling, and decoding with drafted tokens. No reference counterpart (the */
+/* reference takes the largest logit, one token a step).                     */
+/* ------------------------------------------------------------------------ */
+
+/* One token of each of `rows` rows of `vocab` logits. With the weights
+ * w_i = exp((x_i - max x) / temperature) and the tokens in the order of falling
+ * logits (equal ones by index): the first top_k of them are kept (0: all), of
+ * those the shortest run whose weights reach top_p of their sum (1: all), of
+ * those the ones with w_i >= min_p (0: all). temperature 0 keeps the first
+ * alone. Each setting is the struct's number, or, where the pointer is not
+ * NULL, a device array of one number a row. */
+typedef struct {
+    size_t rows;
+    size_t vocab;              /* up to 2^22 (SHAPE otherwise) */
+    float temperature;         /* finite, >= 0 */
+    size_t top_k;
+    float top_p;               /* 0..1 */
+    float min_p;               /* 0..1 */
+    const float *d_temperature; /* [rows] or NULL */
+    const int32_t *d_top_k;    /* [rows] or NULL; 0 or less: all */
+    const float *d_top_p;      /* [rows] or NULL */
+    const float *d_min_p;      /* [rows] or NULL */
+} spissa_sampling_config;
+/* d_tokens[r] = the first index at which the running sum of row r's kept
+ * weights, taken in index order, is above d_uniform[r] (0 <= u < 1) times their
+ * sum; d_probs[r] (d_probs may be NULL) = its share of that sum. d_logits
+ * [rows, vocab]. Weights are formed in 64 bits and summed as whole numbers of
+ * 2^-62 vocab (of the next power of two), so a row's token does not depend on
+ * the order of any sum, nor on the other rows; one whose weight is below that
+ * is never taken. A setting of the struct that is out of its range is
+ * INVALID_TENSOR_DATA. A row with a NaN or +infinite logit, with none above
+ * -infinity, or with a setting or uniform number out of its range gets token -1
+ * and probability 0, and the next spissa_session_sync() reports it. */
+int spissa_sample_device(spissa_session *s, const float *d_logits, const float *d_uniform,
+                         const spissa_sampling_config *cfg, int32_t *d_tokens, float *d_probs);
+
+/* One step of one layer for a tree of drafted tokens of each of `batch`
+ * sequences. Sequence b has nodes[b] tokens (host array; 0 to 256), whose rows
+ * follow those of the sequences before it: d_q [N, Hq, D], d_k and d_v
+ * [N, Hkv, D], d_parents [N] and d_out [N, Hq, D] with N = cfg->query_len, the
+ * sum of nodes. d_parents[t] is the index within the sequence of the node before
+ * it, below its own, or -1. A node's position is the cache's length plus its
+ * depth (0 without a parent); it sees the cached rows, the nodes it descends
+ * from and itself, with cfg->window W those less than W positions before it.
+ * Each cache gains nodes[b] rows, in the nodes' order: the key rotated from
+ * `table` (NULL: none) at the node's position and the value; then the nodes
+ * attend as in spissa_decode_step_device, a chain of nodes like as many decode
+ * steps. spissa_kv_cache_keep_device and spissa_kv_cache_truncate leave the
+ * accepted ones.
+ *
+ * Products are f32's in all but name: queries, keys, values and softmax weights
+ * as two nearest binary16 pieces (2^-23 of themselves, or 2^-32 of the largest
+ * of their row's, their workgroup's keys' or 1 where that is more), sums and
+ * softmax in f32.
+ * A parent out of its range counts as -1 and is reported by the next
+ * spissa_session_sync(); so is a key or value that is not finite, which makes
+ * the outputs of the nodes that see it NaN, and those alone.
+ *
+ * cfg->causal must be set, head_dim 64, 128 or 256 (SHAPE); f32 caches, each
+ * once (ARGUMENT); 16-byte aligned buffers (ARGUMENT). All checks run before any
+ * launch. The call uses workspaces that grow with its sizes: under graph capture
+ * it must follow a call of the same sizes. */
+int spissa_tree_step_device(spissa_session *s, const spissa_rope_table *table, const float *d_q, const float *d_k,
+                            const float *d_v, spissa_kv_cache *const *caches, const size_t *nodes, size_t batch,
+                            const int32_t *d_parents, const spissa_kv_attention_config *cfg, float *d_out);
+/* The same for a Gemma 3 layer: q and k are RMS-normed with the [head_dim]
+ * weights first (sums of squares as a tree), rotated from `table` (a GEMMA
+ * table), and q multiplied by q_prescale. */
+int spissa_gemma_tree_step_device(spissa_session *s, const spissa_rope_table *table, const float *d_q,
+                                  const float *d_k, const float *d_v, spissa_kv_cache *const *caches,
+                                  const size_t *nodes, size_t batch, const int32_t *d_parents,
+                                  const spissa_kv_attention_config *cfg, const float *d_q_norm,
+                                  const float *d_k_norm, float eps, float q_prescale, float *d_out);
+
+/* The drafted tokens that sampling confirms. The sequences' nodes lie one after
+ * the other as above; d_tokens[t] is the token drafted at node t, d_sampled[t]
+ * the one sampled from the logits after it. From node 0 (whose parent is -1; a
+ * sequence's last known token) the walk goes to the first child whose drafted
+ * token is the one sampled, and on. d_count[b] = nodes of the walk, node 0
+ * included; d_path: at the sequence's first count places their indices within
+ * the sequence, -1 at its others; d_next[b] = the token sampled at the last of
+ * them. Without nodes: count 0 and next -1. A sampled token below 0 confirms
+ * none. A parent out of its range counts as -1 and is reported by the next
+ * spissa_session_sync(). */
+int spissa_tree_accept_device(spissa_session *s, const int32_t *d_parents, const int32_t *d_tokens,
+                              const int32_t *d_sampled, const size_t *nodes, size_t batch, int32_t *d_path,
+                              int32_t *d_count, int32_t *d_next);
+
+/* Moves the accepted nodes' rows together, in layers * batch caches at once:
+ * caches[l * batch + b] is sequence b's of layer l, whose last nodes[b] rows are
+ * the nodes'. With P = len - nodes[b]: row P + i becomes what row P + d_path[i]
+ * was, for i below d_count[b] (d_path, d_count: as spissa_tree_accept_device
+ * writes them). The rows from P + d_count[b] on and the lengths stay as they
+ * are: once the count is known, spissa_kv_cache_truncate to P + count. Takes
+ * f32 caches (with their bf16 prefill operands) and 4-bit ones, each once
+ * (ARGUMENT). A path ends where it does not rise within the sequence's nodes, and
+ * counts end at nodes[b]; the next spissa_session_sync() reports either. */
+int spissa_kv_cache_keep_device(spissa_session *s, spissa_kv_cache *const *caches, size_t layers,
+                                const size_t *nodes, size_t batch, const int32_t *d_path, const int32_t *d_count);
 
 /* Streaming-read ceiling (no reference counterpart): reads the `bytes` bytes
  * of d_buf once with 16-byte non-temporal loads, as the decode kernels read

@@ -120,6 +120,22 @@ pub mod sys {
         pub partial_bytes: usize,
     }
 
+    /// Settings of a sampling call: numbers, or device arrays of one a row (null: the number).
+    #[repr(C)]
+    #[derive(Debug, Clone, Copy)]
+    pub struct spissa_sampling_config {
+        pub rows: usize,
+        pub vocab: usize,
+        pub temperature: f32,
+        pub top_k: usize,
+        pub top_p: f32,
+        pub min_p: f32,
+        pub d_temperature: *const f32,
+        pub d_top_k: *const i32,
+        pub d_top_p: *const f32,
+        pub d_min_p: *const f32,
+    }
+
     /// streaming/mod.rs:511-516 StreamingLinearConfig.
     #[repr(C)]
     #[derive(Debug, Clone, Copy, PartialEq, Eq)]
@@ -305,6 +321,27 @@ pub mod sys {
         pub fn spissa_lm_head_device(s: *mut spissa_session, table: *const spissa_linear_weight,
                                      d_hidden: *const f32, excluded: i64, d_logits: *mut f32,
                                      d_token: *mut i32) -> c_int;
+
+        // sampling and decoding with drafted tokens (no reference counterpart)
+        pub fn spissa_sample_device(s: *mut spissa_session, d_logits: *const f32, d_uniform: *const f32,
+                                    cfg: *const spissa_sampling_config, d_tokens: *mut i32,
+                                    d_probs: *mut f32) -> c_int;
+        pub fn spissa_tree_step_device(s: *mut spissa_session, table: *const spissa_rope_table, d_q: *const f32,
+                                       d_k: *const f32, d_v: *const f32, caches: *const *mut spissa_kv_cache,
+                                       nodes: *const usize, batch: usize, d_parents: *const i32,
+                                       cfg: *const spissa_kv_attention_config, d_out: *mut f32) -> c_int;
+        pub fn spissa_gemma_tree_step_device(s: *mut spissa_session, table: *const spissa_rope_table,
+                                             d_q: *const f32, d_k: *const f32, d_v: *const f32,
+                                             caches: *const *mut spissa_kv_cache, nodes: *const usize, batch: usize,
+                                             d_parents: *const i32, cfg: *const spissa_kv_attention_config,
+                                             d_q_norm: *const f32, d_k_norm: *const f32, eps: f32, q_prescale: f32,
+                                             d_out: *mut f32) -> c_int;
+        pub fn spissa_tree_accept_device(s: *mut spissa_session, d_parents: *const i32, d_tokens: *const i32,
+                                         d_sampled: *const i32, nodes: *const usize, batch: usize,
+                                         d_path: *mut i32, d_count: *mut i32, d_next: *mut i32) -> c_int;
+        pub fn spissa_kv_cache_keep_device(s: *mut spissa_session, caches: *const *mut spissa_kv_cache,
+                                           layers: usize, nodes: *const usize, batch: usize, d_path: *const i32,
+                                           d_count: *const i32) -> c_int;
 
         // the attention sublayer (models/gemma/generate.rs:178-312, models/llama/generate.rs:200-450)
         pub fn spissa_attention_sublayer_device(s: *mut spissa_session, layer: *const spissa_attention_layer,
@@ -817,7 +854,77 @@ pub unsafe fn attention_cached_batch(session: &Session, d_q: *const f32, caches:
     check(sys::spissa_attention_cached_batch_device(session.raw, d_q, ptrs.as_ptr(), ptrs.len(), cfg, d_out))
 }
 
+/// A tree of drafted tokens of each sequence through one layer: RoPE at the cache's
+/// length plus the node's depth, append, attention over the cached rows, the node's
+/// ancestors and itself. nodes[b] tokens of sequence b, one sequence after the other.
+///
+/// # Safety
+/// d_q [N, Hq, d], d_k and d_v [N, Hkv, d], d_parents [N], d_out [N, Hq, d] device
+/// buffers with N = cfg.query_len, 16-byte aligned.
+pub unsafe fn tree_step(session: &Session, table: Option<&RopeTable>, d_q: *const f32, d_k: *const f32,
+                        d_v: *const f32, caches: &mut [&mut DeviceKvCache], nodes: &[usize], d_parents: *const i32,
+                        cfg: &AttnConfigC, d_out: *mut f32) -> Result<()> {
+    if nodes.len() != caches.len() {
+        return Err(HipError::Shape(format!("{} counts of nodes for {} caches", nodes.len(), caches.len())));
+    }
+    let ptrs = cache_ptrs(caches);
+    check(sys::spissa_tree_step_device(session.raw, table.map_or(std::ptr::null(), |t| t.raw()), d_q, d_k, d_v,
+                                       ptrs.as_ptr(), nodes.as_ptr(), ptrs.len(), d_parents, cfg, d_out))
+}
+
+/// The same for a Gemma 3 layer: QK-norm, Gemma RoPE, q prescale.
+///
+/// # Safety
+/// As `tree_step`; d_q_norm and d_k_norm are device [head_dim] weights.
+pub unsafe fn gemma_tree_step(session: &Session, table: &RopeTable, d_q: *const f32, d_k: *const f32,
+                              d_v: *const f32, caches: &mut [&mut DeviceKvCache], nodes: &[usize],
+                              d_parents: *const i32, cfg: &AttnConfigC, d_q_norm: *const f32, d_k_norm: *const f32,
+                              eps: f32, q_prescale: f32, d_out: *mut f32) -> Result<()> {
+    if nodes.len() != caches.len() {
+        return Err(HipError::Shape(format!("{} counts of nodes for {} caches", nodes.len(), caches.len())));
+    }
+    let ptrs = cache_ptrs(caches);
+    check(sys::spissa_gemma_tree_step_device(session.raw, table.raw(), d_q, d_k, d_v, ptrs.as_ptr(), nodes.as_ptr(),
+                                             ptrs.len(), d_parents, cfg, d_q_norm, d_k_norm, eps, q_prescale, d_out))
+}
+
+/// The drafted tokens that the sampled ones confirm.
+///
+/// # Safety
+/// d_parents, d_tokens, d_sampled, d_path: device buffers of as many as all nodes;
+/// d_count, d_next: of nodes.len().
+pub unsafe fn tree_accept(session: &Session, d_parents: *const i32, d_tokens: *const i32, d_sampled: *const i32,
+                          nodes: &[usize], d_path: *mut i32, d_count: *mut i32, d_next: *mut i32) -> Result<()> {
+    check(sys::spissa_tree_accept_device(session.raw, d_parents, d_tokens, d_sampled, nodes.as_ptr(), nodes.len(),
+                                         d_path, d_count, d_next))
+}
+
+/// Moves the accepted nodes' rows together in the caches of every layer (each layer's
+/// in the order of the sequences). The lengths stay.
+///
+/// # Safety
+/// d_path and d_count as `tree_accept` writes them.
+pub unsafe fn keep_rows(session: &Session, caches: &mut [&mut DeviceKvCache], nodes: &[usize], d_path: *const i32,
+                        d_count: *const i32) -> Result<()> {
+    if (nodes.is_empty() && !caches.is_empty()) || (!nodes.is_empty() && caches.len() % nodes.len() != 0) {
+        return Err(HipError::Shape(format!("{} caches for {} sequences", caches.len(), nodes.len())));
+    }
+    let ptrs = cache_ptrs(caches);
+    check(sys::spissa_kv_cache_keep_device(session.raw, ptrs.as_ptr(), ptrs.len() / nodes.len().max(1),
+                                           nodes.as_ptr(), nodes.len(), d_path, d_count))
+}
+
 // ---- projections, LM head and sampling ----
+
+/// One token of each row of device logits [rows, vocab] by the settings of `cfg`.
+///
+/// # Safety
+/// d_logits [rows, vocab], d_uniform and d_tokens [rows], d_probs [rows] or null, and
+/// the arrays that `cfg` names: device buffers.
+pub unsafe fn sample(session: &Session, d_logits: *const f32, d_uniform: *const f32,
+                     cfg: &sys::spissa_sampling_config, d_tokens: *mut i32, d_probs: *mut f32) -> Result<()> {
+    check(sys::spissa_sample_device(session.raw, d_logits, d_uniform, cfg, d_tokens, d_probs))
+}
 
 /// A weight resident in HBM (streaming_tile_linear_from_model's weight,
 /// uploaded once), row-major [out_features, in_features].

@@ -52,6 +52,16 @@ class AttentionLayerC(C.Structure):
     ]
 
 
+class SamplingConfigC(C.Structure):
+    """spissa_sampling_config: settings of the whole call, or device arrays of one a row."""
+
+    _fields_ = [
+        ("rows", c_size), ("vocab", c_size), ("temperature", C.c_float), ("top_k", c_size), ("top_p", C.c_float),
+        ("min_p", C.c_float), ("d_temperature", c_void_p), ("d_top_k", c_void_p), ("d_top_p", c_void_p),
+        ("d_min_p", c_void_p),
+    ]
+
+
 class RotaryConfigC(C.Structure):
     """spissa_rotary_config (rotary.rs:6-14)."""
 
@@ -227,6 +237,21 @@ SIGNATURES = {
     "spissa_sample_argmax": (C.c_int, [c_void_p, c_float_p, c_size, C.c_int64, C.POINTER(c_size)]),
     "spissa_argmax_device": (C.c_int, [c_void_p, c_void_p, c_size, C.c_int64, c_void_p]),
     "spissa_lm_head_device": (C.c_int, [c_void_p, c_void_p, c_void_p, C.c_int64, c_void_p, c_void_p]),
+    "spissa_sample_device": (
+        C.c_int, [c_void_p, c_void_p, c_void_p, C.POINTER(SamplingConfigC), c_void_p, c_void_p]),
+    "spissa_tree_step_device": (
+        C.c_int,
+        [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, C.POINTER(c_void_p), C.POINTER(c_size), c_size, c_void_p,
+         C.POINTER(AttnConfigC), c_void_p]),
+    "spissa_gemma_tree_step_device": (
+        C.c_int,
+        [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, C.POINTER(c_void_p), C.POINTER(c_size), c_size, c_void_p,
+         C.POINTER(AttnConfigC), c_void_p, c_void_p, C.c_float, C.c_float, c_void_p]),
+    "spissa_tree_accept_device": (
+        C.c_int,
+        [c_void_p, c_void_p, c_void_p, c_void_p, C.POINTER(c_size), c_size, c_void_p, c_void_p, c_void_p]),
+    "spissa_kv_cache_keep_device": (
+        C.c_int, [c_void_p, C.POINTER(c_void_p), c_size, C.POINTER(c_size), c_size, c_void_p, c_void_p]),
     "spissa_attention_sublayer_device": (
         C.c_int, [c_void_p, C.POINTER(AttentionLayerC), c_void_p, c_size, c_void_p, c_void_p]),
 }

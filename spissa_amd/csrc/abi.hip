@@ -116,6 +116,7 @@ struct spissa_session {
   DevBuf amax;      // argmax partials
   DevBuf qstage;    // fused prefill step: bf16 Q operand
   DevBuf q4q;       // fused steps on a 4-bit cache: the rotated queries
+  DevBuf tree;      // tree steps: rotated queries, depths and visible nodes
   float *lin = nullptr;  // partial sums of projections whose K is split over workgroups (linear_partials)
   std::mutex lin_mutex;  // held over the launches that write and read them
   DevBuf q4x;       // activations' pieces of projections of 4-bit weights (under lin_mutex)
@@ -233,6 +234,7 @@ static void session_free(spissa_session *s) {
   free_buf(s->amax);
   free_buf(s->qstage);
   free_buf(s->q4q);
+  free_buf(s->tree);
   free_buf(s->q4x);
   for (void *p : s->retired) (void)hipFree(p);
   if (s->d_err) (void)hipFree(s->d_err);
@@ -291,6 +293,13 @@ extern "C" int spissa_session_sync(spissa_session *s) {
     if (flag & kDevErrCacheValue)
       return set_err(SPISSA_ERR_INVALID_TENSOR_DATA,
                      "a key or value appended to a 4-bit cache is not finite or beyond 65504");
+    if (flag & kDevErrTreeParent)
+      return set_err(SPISSA_ERR_INVALID_TENSOR_DATA, "a drafted node's parent is not a node before it");
+    if (flag & kDevErrTreePath)
+      return set_err(SPISSA_ERR_INVALID_TENSOR_DATA, "an accepted path does not rise within its sequence's nodes");
+    if (flag & kDevErrSampling)
+      return set_err(SPISSA_ERR_INVALID_TENSOR_DATA,
+                     "a sampled row has no finite largest logit, a NaN, or a setting or uniform number out of range");
     return set_err(SPISSA_ERR_DEVICE, "device error flag 0x%x", flag);
   }
   return SPISSA_OK;
@@ -2598,6 +2607,298 @@ extern "C" int spissa_lm_head_device(spissa_session *s, const spissa_linear_weig
     return set_err(SPISSA_ERR_SHAPE, "%zu logits exceed the device index range", table->out_features);
   ST_TRY(linear_launch(s, table, d_hidden, nullptr, 1, d_logits));
   if (d_token) ST_TRY(argmax_launch(s, d_logits, table->out_features, excluded, d_token));
+  return SPISSA_OK;
+  GUARD_END
+}
+
+// ------------------------------------------------------------------------
+// Sampling, and decoding with drafted tokens
+// ------------------------------------------------------------------------
+extern "C" int spissa_sample_device(spissa_session *s, const float *d_logits, const float *d_uniform,
+                                    const spissa_sampling_config *cfg, int32_t *d_tokens, float *d_probs) {
+  GUARD_BEGIN
+  if (!cfg) return set_err(SPISSA_ERR_ARGUMENT, "config is null");
+  if (cfg->rows && cfg->vocab == 0) return set_err(SPISSA_ERR_INVALID_TENSOR_DATA, "cannot sample from empty logits");
+  if (cfg->vocab > kSampleMaxVocab || cfg->rows > (size_t)INT32_MAX)
+    return set_err(SPISSA_ERR_SHAPE, "sampling takes up to %d rows of %zu logits, got %zu of %zu", INT32_MAX,
+                   kSampleMaxVocab, cfg->rows, cfg->vocab);
+  if (!(cfg->temperature >= 0.0f && std::isfinite(cfg->temperature)))
+    return set_err(SPISSA_ERR_INVALID_TENSOR_DATA, "temperature %g is not a finite number >= 0", (double)cfg->temperature);
+  if (!(cfg->top_p >= 0.0f && cfg->top_p <= 1.0f) || !(cfg->min_p >= 0.0f && cfg->min_p <= 1.0f))
+    return set_err(SPISSA_ERR_INVALID_TENSOR_DATA, "top_p %g and min_p %g must lie in 0..1", (double)cfg->top_p,
+                   (double)cfg->min_p);
+  if (!s) return set_err(SPISSA_ERR_ARGUMENT, "session is null");
+  if (cfg->rows == 0) return SPISSA_OK;
+  if (!d_logits || !d_uniform || !d_tokens) return set_err(SPISSA_ERR_ARGUMENT, "null buffer");
+  SampleArgs a{};
+  a.x = d_logits;
+  a.u = d_uniform;
+  a.d_temperature = cfg->d_temperature;
+  a.d_top_k = cfg->d_top_k;
+  a.d_top_p = cfg->d_top_p;
+  a.d_min_p = cfg->d_min_p;
+  a.temperature = cfg->temperature;
+  a.top_k = (int)std::min(cfg->top_k, kSampleMaxVocab);
+  a.top_p = cfg->top_p;
+  a.min_p = cfg->min_p;
+  a.rows = (int)cfg->rows;
+  a.vocab = (int)cfg->vocab;
+  a.tokens = d_tokens;
+  a.probs = d_probs;
+  a.err = s->d_err;
+  HIP_TRY(hipSetDevice(s->device));
+  HIP_TRY(launch_sample(s->stream, a));
+  return SPISSA_OK;
+  GUARD_END
+}
+
+// Every check of a tree step that needs no device, before anything runs.
+static int validate_tree_config(const size_t *nodes, size_t batch, const spissa_kv_attention_config *cfg) {
+  if (!cfg || (batch && !nodes)) return set_err(SPISSA_ERR_ARGUMENT, "null argument");
+  size_t total = 0;
+  for (size_t b = 0; b < batch; ++b) {
+    if (nodes[b] > (size_t)kTreeMaxNodes)
+      return set_err(SPISSA_ERR_SHAPE, "a tree has up to %d nodes, got %zu", kTreeMaxNodes, nodes[b]);
+    total += nodes[b];
+  }
+  if (total != cfg->query_len)
+    return set_err(SPISSA_ERR_SHAPE, "the trees have %zu nodes, query_len is %zu", total, cfg->query_len);
+  if (!cfg->causal) return set_err(SPISSA_ERR_SHAPE, "a tree step is causal");
+  if (!decode_supported((int)std::min<size_t>(cfg->head_dim, 4096), 1))
+    return set_err(SPISSA_ERR_SHAPE, "the tree step supports head_dim 64, 128 and 256, got %zu", cfg->head_dim);
+  return SPISSA_OK;
+}
+
+static int validate_tree_step(spissa_session *s, const spissa_rope_table *table, const float *d_q, const float *d_k,
+                              const float *d_v, spissa_kv_cache *const *caches, const size_t *nodes, size_t batch,
+                              const int32_t *d_parents, const spissa_kv_attention_config *cfg, const float *d_out) {
+  ST_TRY(validate_tree_config(nodes, batch, cfg));
+  if (!s || (batch && !caches)) return set_err(SPISSA_ERR_ARGUMENT, "null argument");
+  for (size_t b = 0; b < batch; ++b)
+    if (!caches[b]) return set_err(SPISSA_ERR_ARGUMENT, "cache %zu is null", b);
+  std::vector<const spissa_kv_cache *> seen(caches, caches + batch);
+  std::sort(seen.begin(), seen.end());
+  if (std::adjacent_find(seen.begin(), seen.end()) != seen.end())
+    return set_err(SPISSA_ERR_ARGUMENT, "a cache appears more than once in one tree step");
+  for (size_t b = 0; b < batch; ++b) {
+    ST_TRY(refuse_q4(caches[b], "the tree step"));
+    if (cfg->query_len) ST_TRY(validate_attention(0, 0, 0, caches[b], cfg, false));
+    size_t n, nl = caches[b]->len;
+    if (nodes[b]) ST_TRY(kv_validate_append(caches[b], 0, 0, nodes[b], false, &n, &nl));
+    if (caches[b]->session->device != s->device)
+      return set_err(SPISSA_ERR_ARGUMENT, "cache %zu lives on another device", b);
+    if (table && nl > table->max_positions)
+      return set_err(SPISSA_ERR_SHAPE, "positions up to %zu exceed the rope table (%zu positions)", nl,
+                     table->max_positions);
+  }
+  if (table && (table->kind == SPISSA_ROPE_NEOX || table->rotary_dim != cfg->head_dim))
+    return set_err(SPISSA_ERR_SHAPE, "the tree step needs a llama or gemma table over the whole head");
+  if (table && table->device != s->device) return set_err(SPISSA_ERR_ARGUMENT, "the rope table lives on another device");
+  if (cfg->query_len == 0) return SPISSA_OK;
+  if (!d_q || !d_k || !d_v || !d_out || !d_parents) return set_err(SPISSA_ERR_ARGUMENT, "null buffer");
+  if (!(aligned16(d_q) && aligned16(d_k) && aligned16(d_v) && aligned16(d_out)))
+    return set_err(SPISSA_ERR_ARGUMENT, "a tree step takes 16-byte aligned buffers");
+  return SPISSA_OK;
+}
+
+static int run_tree_step(spissa_session *s, const spissa_rope_table *table, const float *d_q, const float *d_k,
+                         const float *d_v, spissa_kv_cache *const *caches, const size_t *nodes, size_t batch,
+                         const int32_t *d_parents, const spissa_kv_attention_config *cfg, float *d_out,
+                         const GemmaQkNorm *norm) {
+  const int D = (int)cfg->head_dim, Hq = (int)cfg->num_heads, Hkv = (int)cfg->kv_heads;
+  HIP_TRY(hipSetDevice(s->device));
+  // workspace of the largest launch: queries, depths, visible nodes
+  size_t most = 0;
+  for (size_t b0 = 0; b0 < batch; b0 += kMaxDecodeBatch) {
+    size_t n = 0;
+    for (size_t b = b0; b < std::min(batch, b0 + kMaxDecodeBatch); ++b) n += nodes[b];
+    most = std::max(most, n);
+  }
+  const size_t q_bytes = most * Hq * D * sizeof(float), mask_bytes = most * (kTreeMaxNodes / 8);
+  ST_TRY(ensure_buf(s, s->tree, q_bytes + mask_bytes + most * sizeof(int)));
+  size_t at = 0;
+  for (size_t b0 = 0; b0 < batch; b0 += kMaxDecodeBatch) {
+    const int B = (int)std::min<size_t>(kMaxDecodeBatch, batch - b0);
+    TreeArgs a{};
+    int n = 0;
+    for (int b = 0; b < B; ++b) {
+      const spissa_kv_cache *c = caches[b0 + b];
+      a.seq[b] = TreeSeq{c->keys, c->values, c->kb, c->vt, (long)c->shadow_cap, (int)c->len, (int)nodes[b0 + b], n, 0};
+      n += (int)nodes[b0 + b];
+    }
+    if (n == 0) continue;
+    a.q = d_q + at * Hq * D;
+    a.k = d_k + at * Hkv * D;
+    a.v = d_v + at * Hkv * D;
+    a.out = d_out + at * Hq * D;
+    a.parents = d_parents + at;
+    at += n;
+    a.q_rot = (float *)s->tree.p;
+    a.mask = (unsigned *)((char *)s->tree.p + q_bytes);
+    a.depth = (int *)((char *)s->tree.p + q_bytes + mask_bytes);
+    a.cos = table ? table->cos : nullptr;
+    a.sin = table ? table->sin : nullptr;
+    a.prescale = 1.0f;
+    if (norm) {
+      a.q_norm = norm->q_norm;
+      a.k_norm = norm->k_norm;
+      a.eps = norm->eps;
+      a.prescale = norm->q_prescale;
+    }
+    a.err = s->d_err;
+    a.Hq = Hq;
+    a.Hkv = Hkv;
+    a.R = Hq / Hkv;
+    a.window = (int)cfg->window;
+    a.qscale = (1.0f / sqrtf((float)D)) * 1.4426950408889634f;
+    HIP_TRY(launch_tree(s->stream, a, D, B));
+  }
+  for (size_t b = 0; b < batch; ++b) caches[b]->len += nodes[b];
+  return SPISSA_OK;
+}
+
+extern "C" int spissa_tree_step_device(spissa_session *s, const spissa_rope_table *table, const float *d_q,
+                                       const float *d_k, const float *d_v, spissa_kv_cache *const *caches,
+                                       const size_t *nodes, size_t batch, const int32_t *d_parents,
+                                       const spissa_kv_attention_config *cfg, float *d_out) {
+  GUARD_BEGIN
+  ST_TRY(validate_tree_step(s, table, d_q, d_k, d_v, caches, nodes, batch, d_parents, cfg, d_out));
+  if (cfg->query_len == 0) return SPISSA_OK;
+  return run_tree_step(s, table, d_q, d_k, d_v, caches, nodes, batch, d_parents, cfg, d_out, nullptr);
+  GUARD_END
+}
+
+extern "C" int spissa_gemma_tree_step_device(spissa_session *s, const spissa_rope_table *table, const float *d_q,
+                                             const float *d_k, const float *d_v, spissa_kv_cache *const *caches,
+                                             const size_t *nodes, size_t batch, const int32_t *d_parents,
+                                             const spissa_kv_attention_config *cfg, const float *d_q_norm,
+                                             const float *d_k_norm, float eps, float q_prescale, float *d_out) {
+  GUARD_BEGIN
+  ST_TRY(validate_tree_config(nodes, batch, cfg));
+  if (!table || !d_q_norm || !d_k_norm) return set_err(SPISSA_ERR_ARGUMENT, "null argument");
+  if (table->kind != SPISSA_ROPE_GEMMA)
+    return set_err(SPISSA_ERR_ARGUMENT, "the gemma tree step needs a gemma rope table");
+  ST_TRY(validate_tree_step(s, table, d_q, d_k, d_v, caches, nodes, batch, d_parents, cfg, d_out));
+  if (!(aligned16(d_q_norm) && aligned16(d_k_norm)))
+    return set_err(SPISSA_ERR_ARGUMENT, "a tree step takes 16-byte aligned norms");
+  if (cfg->query_len == 0) return SPISSA_OK;
+  const GemmaQkNorm norm{d_q_norm, d_k_norm, eps, q_prescale};
+  return run_tree_step(s, table, d_q, d_k, d_v, caches, nodes, batch, d_parents, cfg, d_out, &norm);
+  GUARD_END
+}
+
+// The nodes of `batch` sequences, each within the tree's limit.
+static int validate_nodes(const size_t *nodes, size_t batch, size_t *total) {
+  if (batch && !nodes) return set_err(SPISSA_ERR_ARGUMENT, "null argument");
+  *total = 0;
+  for (size_t b = 0; b < batch; ++b) {
+    if (nodes[b] > (size_t)kTreeMaxNodes)
+      return set_err(SPISSA_ERR_SHAPE, "a tree has up to %d nodes, got %zu", kTreeMaxNodes, nodes[b]);
+    *total += nodes[b];
+  }
+  if (*total > (size_t)INT32_MAX) return set_err(SPISSA_ERR_SHAPE, "%zu nodes exceed the device index range", *total);
+  return SPISSA_OK;
+}
+
+extern "C" int spissa_tree_accept_device(spissa_session *s, const int32_t *d_parents, const int32_t *d_tokens,
+                                         const int32_t *d_sampled, const size_t *nodes, size_t batch,
+                                         int32_t *d_path, int32_t *d_count, int32_t *d_next) {
+  GUARD_BEGIN
+  size_t total;
+  ST_TRY(validate_nodes(nodes, batch, &total));
+  if (!s) return set_err(SPISSA_ERR_ARGUMENT, "session is null");
+  if (batch == 0) return SPISSA_OK;
+  if (!d_count || !d_next || (total && (!d_parents || !d_tokens || !d_sampled || !d_path)))
+    return set_err(SPISSA_ERR_ARGUMENT, "null buffer");
+  HIP_TRY(hipSetDevice(s->device));
+  size_t at = 0;
+  for (size_t b0 = 0; b0 < batch; b0 += kTreeAcceptBatch) {
+    const int B = (int)std::min<size_t>(kTreeAcceptBatch, batch - b0);
+    TreeAcceptArgs a{};
+    a.parents = d_parents;
+    a.tokens = d_tokens;
+    a.sampled = d_sampled;
+    a.path = d_path;
+    a.count = d_count + b0;
+    a.next = d_next + b0;
+    a.err = s->d_err;
+    for (int b = 0; b < B; ++b) {
+      a.nodes[b] = (int)nodes[b0 + b];
+      a.first[b] = (int)at;
+      at += nodes[b0 + b];
+    }
+    HIP_TRY(launch_tree_accept(s->stream, a, B));
+  }
+  return SPISSA_OK;
+  GUARD_END
+}
+
+extern "C" int spissa_kv_cache_keep_device(spissa_session *s, spissa_kv_cache *const *caches, size_t layers,
+                                           const size_t *nodes, size_t batch, const int32_t *d_path,
+                                           const int32_t *d_count) {
+  GUARD_BEGIN
+  size_t total, n;
+  ST_TRY(validate_nodes(nodes, batch, &total));
+  if (mul_ovf(layers, batch, &n)) return set_err(SPISSA_ERR_SHAPE, "layers * batch overflow");
+  if (!s || (n && !caches)) return set_err(SPISSA_ERR_ARGUMENT, "null argument");
+  for (size_t i = 0; i < n; ++i) {
+    const spissa_kv_cache *c = caches[i];
+    if (!c) return set_err(SPISSA_ERR_ARGUMENT, "cache %zu is null", i);
+    if (c->len < nodes[i % batch])
+      return set_err(SPISSA_ERR_SHAPE, "cache %zu holds %zu rows, fewer than its sequence's %zu nodes", i, c->len,
+                     nodes[i % batch]);
+    if (c->len > (size_t)INT32_MAX || c->num_heads > 65535 || c->head_dim > 65535 || c->width() > (size_t)1 << 28)
+      return set_err(SPISSA_ERR_SHAPE, "cache sizes exceed the device kernels' limits");
+    if (c->session->device != s->device) return set_err(SPISSA_ERR_ARGUMENT, "cache %zu lives on another device", i);
+  }
+  std::vector<const spissa_kv_cache *> seen(caches, caches + n);
+  std::sort(seen.begin(), seen.end());
+  if (std::adjacent_find(seen.begin(), seen.end()) != seen.end())
+    return set_err(SPISSA_ERR_ARGUMENT, "a cache appears more than once in one call");
+  if (n == 0 || total == 0) return SPISSA_OK;
+  if (!d_path || !d_count) return set_err(SPISSA_ERR_ARGUMENT, "null buffer");
+  HIP_TRY(hipSetDevice(s->device));
+  std::vector<int> first(batch);
+  for (size_t b = 0, at = 0; b < batch; at += nodes[b], ++b) first[b] = (int)at;
+  KeepArgs a{};
+  a.path = d_path;
+  a.count = d_count;
+  a.err = s->d_err;
+  int in = 0;
+  for (size_t i = 0; i < n; ++i) {
+    const spissa_kv_cache *c = caches[i];
+    const size_t b = i % batch;
+    if (nodes[b]) {
+      const size_t P = c->len - nodes[b];
+      KeepCache &k = a.cache[in++];
+      k = KeepCache{};
+      k.past = (int)P;
+      k.nodes = (int)nodes[b];
+      k.seq = (int)b;
+      k.first = first[b];
+      k.heads = (int)c->num_heads;
+      k.dim = (int)c->head_dim;
+      if (c->q4) {
+        k.kind = 2;
+        k.k = (char *)c->kc;
+        k.v = (char *)c->vc;
+        k.kp = (char *)c->kp;
+        k.vp = (char *)c->vp;
+        k.cap = (long)c->max_seq_len;
+      } else {
+        k.kind = c->kb ? 1 : 0;
+        k.k = (char *)c->keys;
+        k.v = (char *)c->values;
+        k.kp = (char *)c->kb;
+        k.vp = (char *)c->vt;
+        k.cap = (long)c->shadow_cap;
+      }
+    }
+    if (in == kKeepBatch || (i + 1 == n && in)) {
+      HIP_TRY(launch_keep(s->stream, a, in));
+      in = 0;
+    }
+  }
   return SPISSA_OK;
   GUARD_END
 }

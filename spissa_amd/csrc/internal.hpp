@@ -14,7 +14,13 @@ namespace spissa {
 typedef __bf16 bf16;
 
 // Device-side error bits reported through spissa_session_sync().
-enum : int { kDevErrSoftmaxDenominator = 1, kDevErrCacheValue = 2 };
+enum : int {
+  kDevErrSoftmaxDenominator = 1,
+  kDevErrCacheValue = 2,
+  kDevErrTreeParent = 4,
+  kDevErrTreePath = 8,
+  kDevErrSampling = 16
+};
 
 // Largest batch a single decode launch carries in its kernel arguments.
 constexpr int kMaxDecodeBatch = 16;
@@ -318,6 +324,76 @@ constexpr int kArgmaxMaxParts = 1024;  // partials one launch writes at most
 // sample_argmax_excluding(x, excl) with 0 <= excl < n and n >= 2;
 // n <= INT32_MAX - 1024.
 hipError_t launch_argmax(hipStream_t st, const float *x, int n, int excl, ArgmaxPart *parts, int *token);
+
+// One token of each row of logits (sampler.hip): spissa_sampling_config's settings,
+// a row's from the array where there is one.
+struct SampleArgs {
+  const float *x;        // [rows, vocab]
+  const float *u;        // [rows]
+  const float *d_temperature, *d_top_p, *d_min_p;
+  const int *d_top_k;
+  float temperature, top_p, min_p;
+  int top_k;             // 0: all
+  int rows, vocab;
+  int *tokens;           // [rows]
+  float *probs;          // [rows] or null
+  int *err;
+};
+constexpr size_t kSampleMaxVocab = (size_t)1 << 22;
+hipError_t launch_sample(hipStream_t st, const SampleArgs &a);
+
+// ---- trees of drafted tokens (tree.hip) ----
+constexpr int kTreeMaxNodes = 256;
+struct TreeSeq {
+  float *k, *v;      // the cache's rows
+  bf16 *kb, *vt;     // its bf16 prefill operands, or null
+  long cap;
+  int past, nodes;   // cached rows; nodes, whose rows come after them
+  int first, pad;    // the sequence's first node among the launch's
+};
+struct TreeArgs {
+  const float *q, *k, *v;        // [N, Hq, D], [N, Hkv, D]
+  const int *parents;            // [N]
+  float *out;
+  float *q_rot;                  // [N, Hq, D]: the normed, rotated, prescaled queries
+  int *depth;                    // [N]
+  unsigned *mask;                // [N][kTreeMaxNodes / 32]: the nodes that a node sees
+  const float *cos, *sin;        // RoPE table rows by position, or null
+  const float *q_norm, *k_norm;  // QK-norm, or null
+  float eps, prescale;
+  int *err;
+  int Hq, Hkv, R, window;
+  float qscale;                  // softmax scale * log2(e)
+  TreeSeq seq[kMaxDecodeBatch];
+};
+hipError_t launch_tree(hipStream_t st, const TreeArgs &a, int D, int B);
+
+struct TreeAcceptArgs {
+  const int *parents, *tokens, *sampled;
+  int *path, *count, *next;
+  int *err;
+  int nodes[64], first[64];  // of each sequence of the launch
+};
+constexpr int kTreeAcceptBatch = 64;
+hipError_t launch_tree_accept(hipStream_t st, const TreeAcceptArgs &a, int B);
+
+// A cache whose last `nodes` rows, from row `past` on, a launch moves together.
+struct KeepCache {
+  char *k, *v;          // f32 rows, or 4-bit codes
+  char *kp, *vp;        // steps and minima (4 bits), or the bf16 prefill operands
+  long cap;             // rows of a head (4 bits, bf16)
+  int past, nodes;
+  int seq, first;       // the sequence, for its count, and its path's first place
+  int heads, dim;
+  int kind, pad;        // 0: f32; 1: f32 with bf16 operands; 2: 4 bits
+};
+constexpr int kKeepBatch = 40;  // (3 KB of arguments)
+struct KeepArgs {
+  const int *path, *count;
+  int *err;
+  KeepCache cache[kKeepBatch];
+};
+hipError_t launch_keep(hipStream_t st, const KeepArgs &a, int n);
 
 // Keys per split of a decode launch: keys[b] = visible cached keys of
 // sequence b (nseq of them), heads = (KV head, head block) pairs per

@@ -62,6 +62,20 @@ def _dev_i32(t, name: str) -> int:
     return t.data_ptr()
 
 
+def _many_i32(t, count: int, name: str) -> int:
+    p = _dev_i32(t, name)
+    if t is None or t.numel() < count or not t.is_contiguous():
+        raise TypeError(f"{name} must be a contiguous int32 device tensor of {count} elements")
+    return p
+
+
+def _many_f32(t, count: int, name: str) -> int:
+    p = _dev(t, name)
+    if t is None or t.numel() < count:
+        raise TypeError(f"{name} must be a float32 device tensor of {count} elements")
+    return p
+
+
 def plan_attention(config: KvAttentionConfig, past_lens: Sequence[int], compute_units: int = 256,
                    precision: int = _ffi.PREFILL_BF16, noalloc: bool = False) -> dict:
     """The launch geometry spissa_plan_attention reports for one attention call
@@ -86,6 +100,31 @@ def plan_linear(dtype: int, batch: int, out_features, in_features: int, compute_
     check(_ffi.load().spissa_plan_linear(dtype, batch, (_ffi.c_size * max(1, len(rows)))(*rows), len(rows), in_features,
                                          compute_units, C.byref(plan)))
     return {name: getattr(plan, name) for name, _ in _ffi.LinearPlanC._fields_}
+
+
+@dataclass(frozen=True)
+class SamplingConfig:
+    """The settings of Session.sample: numbers for all rows, or device tensors of one a row
+    (float32; top_k int32). temperature 0 takes the largest logit; top_k 0, top_p 1 and
+    min_p 0 keep every token."""
+
+    temperature: object = 1.0
+    top_k: object = 0
+    top_p: object = 1.0
+    min_p: object = 0.0
+
+    def _c(self, rows: int, vocab: int) -> _ffi.SamplingConfigC:
+        c = _ffi.SamplingConfigC(rows, vocab, 1.0, 0, 1.0, 0.0, None, None, None, None)
+        for name in ("temperature", "top_k", "top_p", "min_p"):
+            value = getattr(self, name)
+            if hasattr(value, "data_ptr"):
+                many = _many_i32 if name == "top_k" else _many_f32
+                setattr(c, "d_" + name, many(value, rows, name))
+            elif name == "top_k":
+                c.top_k = max(0, int(value))
+            else:
+                setattr(c, name, float(value))
+        return c
 
 
 class RopeTable:
@@ -314,6 +353,71 @@ class Session:
         cfg = config._c()
         check(self._lib.spissa_attention_cached_batch_device(self.handle, _dev(q, "q"), arr, len(caches), C.byref(cfg),
                                                              _dev(out, "out")))
+
+    def _tree(self, fn, table, q, k, v, caches, nodes, parents, config, out, *more) -> None:
+        n, d = config.query_len, config.head_dim
+        for t, heads, name in ((q, config.num_heads, "q"), (k, config.kv_heads, "k"), (v, config.kv_heads, "v"),
+                               (out, config.num_heads, "out")):
+            _many_f32(t, n * heads * d, name)
+        if len(nodes) != len(caches):
+            raise TypeError(f"{len(nodes)} counts of nodes for {len(caches)} caches")
+        arr = _cache_array(caches)
+        cfg = config._c()
+        check(fn(self.handle, None if table is None else table.handle, _dev(q, "q"), _dev(k, "k"), _dev(v, "v"), arr,
+                 (_ffi.c_size * max(1, len(nodes)))(*nodes), len(caches), _many_i32(parents, n, "parents"),
+                 C.byref(cfg), *more, _dev(out, "out")))
+
+    def tree_step(self, table: Optional[RopeTable], q, k, v, caches: Sequence[KvCache], nodes: Sequence[int], parents,
+                  config: KvAttentionConfig, out) -> None:
+        """A tree of drafted tokens of each of `len(caches)` sequences through one layer
+        (spissa_tree_step_device): RoPE at the cache's length plus the node's depth, append,
+        attention over the cached rows, the node's ancestors and itself. q [N, Hq, D],
+        k/v [N, Hkv, D], parents [N] int32, N = config.query_len = sum(nodes); the sequences'
+        nodes lie one after the other, and caches[b] gains nodes[b] rows."""
+        self._tree(self._lib.spissa_tree_step_device, table, q, k, v, caches, nodes, parents, config, out)
+
+    def gemma_tree_step(self, table: RopeTable, q, k, v, caches: Sequence[KvCache], nodes: Sequence[int], parents,
+                        config: KvAttentionConfig, q_norm, k_norm, eps: float, q_prescale: float, out) -> None:
+        """The same for a Gemma 3 layer (spissa_gemma_tree_step_device): QK-norm with the [D]
+        weights q_norm / k_norm, Gemma RoPE, q *= q_prescale, then as tree_step."""
+        for t, name in ((q_norm, "q_norm"), (k_norm, "k_norm")):
+            _many_f32(t, config.head_dim, name)
+        self._tree(self._lib.spissa_gemma_tree_step_device, table, q, k, v, caches, nodes, parents, config, out,
+                   _dev(q_norm, "q_norm"), _dev(k_norm, "k_norm"), float(eps), float(q_prescale))
+
+    def tree_accept(self, parents, tokens, sampled, nodes: Sequence[int], path, count, next_token) -> None:
+        """The drafted tokens that the sampled ones confirm (spissa_tree_accept_device), int32
+        device tensors: path [sum(nodes)] and count, next_token [len(nodes)] from parents,
+        tokens and sampled [sum(nodes)]."""
+        n, b = sum(nodes), len(nodes)
+        ins = [_many_i32(t, n, name) if n else 0
+               for t, name in ((parents, "parents"), (tokens, "tokens"), (sampled, "sampled"), (path, "path"))]
+        check(self._lib.spissa_tree_accept_device(
+            self.handle, *ins[:3], (_ffi.c_size * max(1, b))(*nodes), b, ins[3],
+            _many_i32(count, b, "count") if b else 0, _many_i32(next_token, b, "next_token") if b else 0))
+
+    def keep_rows(self, caches: Sequence[KvCache], nodes: Sequence[int], path, count) -> None:
+        """Moves the accepted nodes' rows together (spissa_kv_cache_keep_device): caches are those
+        of every layer, each layer's in the order of the sequences nodes counts, whose last
+        nodes[b] rows are the nodes'; path and count as tree_accept wrote them. The lengths
+        stay: KvCache.truncate, once the counts are known."""
+        b, n = len(nodes), sum(nodes)
+        if len(caches) % max(1, b) != 0 or (caches and not b):
+            raise TypeError(f"{len(caches)} caches for {b} sequences")
+        check(self._lib.spissa_kv_cache_keep_device(
+            self.handle, _cache_array(caches), len(caches) // max(1, b), (_ffi.c_size * max(1, b))(*nodes), b,
+            _many_i32(path, n, "path") if n else 0, _many_i32(count, b, "count") if b else 0))
+
+    def sample(self, logits, uniform, config: SamplingConfig, tokens, probs=None) -> None:
+        """tokens[r] (int32) from each row of logits [rows, vocab] by the settings and the numbers
+        uniform [rows] in [0, 1), probs[r] (float32 or None) its probability (spissa_sample_device)."""
+        rows = uniform.numel()
+        if logits.numel() % max(1, rows) != 0:
+            raise TypeError(f"{logits.numel()} logits for {rows} rows")
+        cfg = config._c(rows, logits.numel() // max(1, rows))
+        check(self._lib.spissa_sample_device(
+            self.handle, _dev(logits, "logits"), _dev(uniform, "uniform"), C.byref(cfg),
+            _many_i32(tokens, rows, "tokens") if rows else 0, _many_f32(probs, rows, "probs") if probs is not None else None))
 
     def hbm_read_probe(self, buf, sink) -> None:
         """Reads every byte of the device tensor `buf` once (the streaming-read

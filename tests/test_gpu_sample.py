@@ -1,0 +1,252 @@
+"""Sampling on the device (spissa_sample_device) against the same in 64 bits.
+
+Tokens have to be equal: the settings' limits and the random number's place are
+compared on sums that are exact to 2^-38 of the largest weight or better, and a number
+drawn this near a border of the definition's own (64-bit) sums is left out of the
+comparison: BORDER, 2^-36 of the sum. Probabilities: one rounding to f32 (2^-24 of the
+value), and weights in steps of 2^-(62 - log2 vocab) of the largest.
+"""
+import numpy as np
+import pytest
+
+from spissa_amd import _ffi
+from tests import drafts
+
+pytestmark = pytest.mark.gpu
+
+BORDER = 2.0 ** -36
+ROWS = [  # temperature, top_k, top_p, min_p
+    (1.0, 0, 1.0, 0.0), (0.7, 0, 1.0, 0.0), (1.0, 1, 1.0, 0.0), (1.0, 20, 1.0, 0.0), (1.3, 0, 0.9, 0.0), (0.8, 50, 0.95, 0.05),
+    (1.0, 0, 1.0, 0.3), (0.0, 0, 1.0, 0.0), (0.0, 5, 0.5, 0.5), (1.0, 0, 0.0, 0.0), (1.0, 0, 0.5, 1.0), (2.5, 300, 0.99, 0.001),
+    (1e-3, 0, 0.9, 0.0), (100.0, 0, 0.5, 0.0), (1.0, 10**6, 0.8, 0.0), (1.0, 7, 0.999999, 0.0)]
+
+
+@pytest.fixture(scope="module")
+def s(gpu):
+    import torch
+
+    from spissa_amd.device import Session
+
+    stream = torch.cuda.Stream()
+    session = Session(0, stream=stream)
+    with torch.cuda.stream(stream):
+        yield session
+
+
+def run(s, x, u, rows, per_row=True):
+    """tokens, probs of logits x [n, vocab] under the settings rows [n]."""
+    import torch
+
+    from spissa_amd.device import SamplingConfig
+
+    n = len(x)
+    cols = list(zip(*rows))
+    if per_row:
+        cfg = SamplingConfig(*(torch.tensor(c, dtype=torch.int32 if i == 1 else torch.float32, device="cuda") for i, c in enumerate(cols)))
+    else:
+        cfg = SamplingConfig(*rows[0])
+    tokens = torch.full((n,), -7, dtype=torch.int32, device="cuda")
+    probs = torch.full((n,), -7.0, device="cuda")
+    s.sample(torch.as_tensor(x, device="cuda"), torch.as_tensor(np.asarray(u, np.float32), device="cuda"), cfg, tokens, probs)
+    return tokens.cpu().numpy(), probs.cpu().numpy()
+
+
+def compare(x, u, rows, got):
+    left_out = 0
+    for i, (row, setting) in enumerate(zip(x, rows)):
+        token, prob, near = drafts.sample(row, u[i], *setting)
+        if near < BORDER:
+            left_out += 1
+            continue
+        assert got[0][i] == token, (i, setting, got[0][i], token, prob)
+        unit = 2.0 ** -min(51, 62 - int(np.ceil(np.log2(max(2, len(row))))))
+        assert abs(got[1][i] - prob) <= prob * 2.0 ** -23 + 2 * unit * len(row), (i, setting)
+    assert left_out * 4 <= len(rows)
+
+
+def logits(rng, n, vocab, kind):
+    if kind == "flat":
+        return rng.normal(size=(n, vocab)).astype(np.float32) * 0.01
+    if kind == "equal":
+        return np.full((n, vocab), -3.25, np.float32)
+    x = rng.normal(size=(n, vocab)).astype(np.float32) * 3
+    if kind == "ties":  # few values, each many times; both zeros among them
+        x = np.round(x)
+        x[:, ::3] *= np.where(x[:, ::3] == 0, -1, 1).astype(np.float32)
+        x = np.where((x == 0) & (rng.random(x.shape) < 0.5), np.float32(-0.0), x)
+    if kind == "banned":
+        x[:, rng.random(vocab) < 0.7] = -np.inf
+        x[:, vocab // 2] = 0.5
+    if kind == "wide":
+        x *= 1e4
+    return x.astype(np.float32)
+
+
+@pytest.mark.parametrize("vocab", [1, 2, 3, 63, 64, 65, 255, 1000, 1023, 1024, 1025, 4099, 32003, 128256, 262144])
+@pytest.mark.parametrize("kind", ["plain", "ties", "flat", "equal", "banned", "wide"])
+def test_rows_of_settings(s, vocab, kind):
+    print(f"[case] sample vocab={vocab} {kind}", flush=True)
+    rng = np.random.default_rng(vocab * 7 + len(kind))
+    x = logits(rng, len(ROWS), vocab, kind)
+    u = rng.random(len(ROWS)).astype(np.float32)
+    u = np.minimum(u, np.float32(1 - 2.0 ** -24))
+    compare(x, u, ROWS, run(s, x, u, ROWS))
+    s.sync()
+
+
+@pytest.mark.parametrize("setting", ROWS)
+def test_one_setting_for_all_rows_gives_the_same(s, setting):
+    rng = np.random.default_rng(5)
+    x = logits(rng, 7, 5003, "plain")
+    u = rng.random(7).astype(np.float32)
+    a, b = run(s, x, u, [setting] * 7), run(s, x, u, [setting] * 7, per_row=False)
+    compare(x, u, [setting] * 7, a)
+    assert np.array_equal(a[0], b[0]) and np.array_equal(a[1], b[1])
+
+
+@pytest.mark.parametrize("vocab", [77, 5001, 128256])
+def test_uniform_numbers_at_their_ends(s, vocab):
+    rng = np.random.default_rng(3)
+    x = np.repeat(logits(rng, 1, vocab, "plain"), 2, 0)
+    rows = [(1.0, 0, 1.0, 0.0)] * 2
+    u = np.array([0.0, 1 - 2.0 ** -24], np.float32)
+    tokens, _ = run(s, x, u, rows)
+    # u = 0: the first token whose weight counts
+    w = np.exp(x[0].astype(np.float64) - x[0].max())
+    assert tokens[0] == int(np.nonzero(w >= 2.0 ** -40)[0][0])
+    assert tokens[1] == drafts.sample(x[1], u[1], *rows[1])[0]
+
+
+def test_every_token_comes_as_often_as_its_weight(s):
+    """Evenly spaced numbers: each token's count is its probability's, to one at either end of its range."""
+    rng = np.random.default_rng(11)
+    n = 4096
+    x = np.repeat(logits(rng, 1, 37, "plain"), n, 0)
+    u = ((np.arange(n) + 0.5) / n).astype(np.float32)
+    for setting in [(1.0, 0, 1.0, 0.0), (0.7, 9, 0.9, 0.0)]:
+        tokens, probs = run(s, x, u, [setting] * n)
+        for t in np.unique(tokens):
+            assert abs((tokens == t).sum() - probs[tokens == t][0] * n) <= 1 + 1e-3
+
+
+def test_rows_do_not_depend_on_their_neighbours(s):
+    rng = np.random.default_rng(2)
+    x = logits(rng, 48, 9001, "plain")
+    u = rng.random(48).astype(np.float32)
+    rows = [ROWS[i % len(ROWS)] for i in range(48)]
+    whole = run(s, x, u, rows)
+    for i in (0, 17, 47):
+        one = run(s, x[i:i + 1], u[i:i + 1], rows[i:i + 1])
+        assert one[0][0] == whole[0][i] and one[1][0] == whole[1][i]
+
+
+def test_no_probabilities_and_an_offset_buffer(s):
+    import torch
+
+    from spissa_amd.device import SamplingConfig
+
+    rng = np.random.default_rng(9)
+    x = logits(rng, 3, 4099, "plain")
+    u = rng.random(3).astype(np.float32)
+    buf = torch.empty(3 * 4099 + 1, device="cuda")
+    buf[1:] = torch.as_tensor(x.reshape(-1), device="cuda")  # rows at no multiple of 16 bytes
+    tokens = torch.full((5,), -7, dtype=torch.int32, device="cuda")
+    s.sample(buf[1:], torch.as_tensor(u, device="cuda"), SamplingConfig(0.9, 40, 0.9, 0.0), tokens)
+    s.sync()
+    assert tokens.tolist() == [drafts.sample(x[i], u[i], 0.9, 40, 0.9, 0.0)[0] for i in range(3)] + [-7, -7]
+
+
+@pytest.mark.parametrize("what", ["nan", "inf", "none", "u1", "u-", "unan", "t-", "tnan", "p", "m"])
+def test_bad_rows_are_reported_and_leave_the_others(gpu, s, what):
+    print(f"[case] bad row {what}", flush=True)
+    rng = np.random.default_rng(4)
+    x = logits(rng, 3, 3001, "plain")
+    u = rng.random(3).astype(np.float32)
+    rows = [(0.8, 50, 0.95, 0.05)] * 3
+    if what == "nan":
+        x[1, 2999] = np.nan
+    elif what == "inf":
+        x[1, 5] = np.inf
+    elif what == "none":
+        x[1] = -np.inf
+    elif what[0] == "u":
+        u[1] = {"u1": 1.0, "u-": -0.25, "unan": np.nan}[what]
+    else:
+        rows[1] = {"t-": (-1.0, 0, 1.0, 0.0), "tnan": (np.nan, 0, 1.0, 0.0), "p": (1.0, 0, 1.5, 0.0), "m": (1.0, 0, 1.0, -1.0)}[what]
+    tokens, probs = run(s, x, u, rows)
+    with pytest.raises(gpu.InvalidTensorDataError):
+        s.sync()
+    s.sync()  # reported once
+    assert tokens[1] == -1 and probs[1] == 0
+    for i in (0, 2):
+        assert tokens[i] == drafts.sample(x[i], u[i], *rows[i])[0]
+
+
+def test_no_rows(s):
+    import torch
+
+    from spissa_amd.device import SamplingConfig
+
+    none = torch.empty(0, device="cuda")
+    s.sample(none, none, SamplingConfig(), none.int())
+    s.sync()
+
+
+def test_refusals(gpu, s):
+    import torch
+
+    from spissa_amd.device import SamplingConfig
+
+    x, u, t = torch.zeros(2, 8, device="cuda"), torch.zeros(2, device="cuda"), torch.zeros(2, dtype=torch.int32, device="cuda")
+    for bad in (SamplingConfig(-1.0), SamplingConfig(top_p=2.0), SamplingConfig(min_p=-0.5)):
+        with pytest.raises(gpu.InvalidTensorDataError):
+            s.sample(x, u, bad, t)
+    with pytest.raises(TypeError):
+        s.sample(x, u, SamplingConfig(temperature=torch.ones(1, device="cuda")), t)
+    with pytest.raises(TypeError):
+        s.sample(x, u, SamplingConfig(top_k=torch.ones(2, device="cuda")), t)
+    with pytest.raises(TypeError):
+        s.sample(x, u, SamplingConfig(), t[:1])
+    with pytest.raises(TypeError):
+        s.sample(x[:, :5], u, SamplingConfig(), t)
+    assert _ffi.load().spissa_sample_device(s.handle, None, u.data_ptr(), SamplingConfig()._c(2, 8), t.data_ptr(), None) == _ffi.ERR_ARGUMENT
+
+
+def test_two_captured_calls_in_turn_with_eager_ones(gpu):
+    """Two graphs of one session share its workspace: replayed in turn, with new inputs and eager calls between."""
+    import torch
+
+    from spissa_amd.device import SamplingConfig, Session
+
+    stream = torch.cuda.Stream()
+    ses = Session(0, stream=stream)
+    rng = np.random.default_rng(8)
+    shapes, sets = [(3, 128256), (40, 5003)], []
+    with torch.cuda.stream(stream):
+        for n, vocab in shapes:
+            rows = [ROWS[i % len(ROWS)] for i in range(n)]
+            cols = list(zip(*rows))
+            cfg = SamplingConfig(*(torch.tensor(c, dtype=torch.int32 if i == 1 else torch.float32, device="cuda") for i, c in enumerate(cols)))
+            st = {"rows": rows, "cfg": cfg, "x": torch.zeros(n, vocab, device="cuda"), "u": torch.zeros(n, device="cuda"),
+                  "t": torch.zeros(n, dtype=torch.int32, device="cuda"), "p": torch.zeros(n, device="cuda")}
+            ses.sample(st["x"], st["u"], cfg, st["t"], st["p"])
+            sets.append(st)
+        ses.sync()
+        for st in sets:
+            st["graph"] = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(st["graph"], stream=stream):
+                ses.sample(st["x"], st["u"], st["cfg"], st["t"], st["p"])
+        for _ in range(3):
+            for st in sets:
+                n, vocab = st["x"].shape
+                x, u = logits(rng, n, vocab, "plain"), rng.random(n).astype(np.float32)
+                st["x"].copy_(torch.as_tensor(x, device="cuda"))
+                st["u"].copy_(torch.as_tensor(u, device="cuda"))
+                st["t"].fill_(-9)
+                st["graph"].replay()
+                got = st["t"].cpu().numpy(), st["p"].cpu().numpy()
+                compare(x, u, st["rows"], got)
+                eager = torch.zeros_like(st["t"])
+                ses.sample(st["x"], st["u"], st["cfg"], eager)
+                ses.sync()
+                assert np.array_equal(eager.cpu().numpy(), got[0])
