@@ -319,16 +319,17 @@ def _session():
 
 
 class _Rows:
-    """Rows of a cache's keys or values as the tensor library takes them, in place."""
+    """Rows of a cache's keys or values as the tensor library takes them, in place; they hold the cache."""
 
-    def __init__(self, pointer, shape):
+    def __init__(self, cache, pointer, shape):
+        self.cache = cache
         self.__cuda_array_interface__ = {"data": (pointer, False), "shape": tuple(shape), "typestr": "<f4", "version": 2}
 
 
 def _view(cache, first, count):
     """A cache's rows first..first + count: keys and values."""
     h, d = cache.num_heads(), cache.head_dim()
-    return [torch.as_tensor(_Rows(p + first * h * d * 4, (count, h, d)), device=DEV) for p in (cache.device_keys_ptr(), cache.device_values_ptr())]
+    return [torch.as_tensor(_Rows(cache, p + first * h * d * 4, (count, h, d)), device=DEV) for p in (cache.device_keys_ptr(), cache.device_values_ptr())]
 
 
 def _padded(rows, n):
