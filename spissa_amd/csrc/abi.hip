@@ -116,7 +116,7 @@ struct spissa_session {
   DevBuf amax;      // argmax partials
   DevBuf qstage;    // fused prefill step: bf16 Q operand
   DevBuf q4q;       // fused steps on a 4-bit cache: the rotated queries
-  DevBuf tree;      // tree steps: rotated queries, depths and visible nodes
+  DevBuf tree;      // tree steps: the key splits' outputs
   float *lin = nullptr;  // partial sums of projections whose K is split over workgroups (linear_partials)
   std::mutex lin_mutex;  // held over the launches that write and read them
   DevBuf q4x;       // activations' pieces of projections of 4-bit weights (under lin_mutex)
@@ -2707,15 +2707,21 @@ static int run_tree_step(spissa_session *s, const spissa_rope_table *table, cons
                          const GemmaQkNorm *norm) {
   const int D = (int)cfg->head_dim, Hq = (int)cfg->num_heads, Hkv = (int)cfg->kv_heads;
   HIP_TRY(hipSetDevice(s->device));
-  // workspace of the largest launch: queries, depths, visible nodes
-  size_t most = 0;
+  // (the workspace of every launch before the first: nothing is appended by a call that fails for want of it)
+  std::vector<TreePlan> plans;
+  size_t bytes = 0;
   for (size_t b0 = 0; b0 < batch; b0 += kMaxDecodeBatch) {
-    size_t n = 0;
-    for (size_t b = b0; b < std::min(batch, b0 + kMaxDecodeBatch); ++b) n += nodes[b];
-    most = std::max(most, n);
+    const int B = (int)std::min<size_t>(kMaxDecodeBatch, batch - b0);
+    int past[kMaxDecodeBatch], count[kMaxDecodeBatch], n = 0;
+    for (int b = 0; b < B; ++b) {
+      past[b] = (int)caches[b0 + b]->len;
+      n += count[b] = (int)nodes[b0 + b];
+    }
+    const TreePlan p = tree_plan(D, Hq / Hkv, Hkv, (int)cfg->window, past, count, B, s->cus);
+    plans.push_back(p);
+    if (p.splits > 1) bytes = std::max(bytes, (size_t)p.splits * n * Hq * (D + 4) * sizeof(float));
   }
-  const size_t q_bytes = most * Hq * D * sizeof(float), mask_bytes = most * (kTreeMaxNodes / 8);
-  ST_TRY(ensure_buf(s, s->tree, q_bytes + mask_bytes + most * sizeof(int)));
+  if (bytes) ST_TRY(ensure_buf(s, s->tree, bytes));
   size_t at = 0;
   for (size_t b0 = 0; b0 < batch; b0 += kMaxDecodeBatch) {
     const int B = (int)std::min<size_t>(kMaxDecodeBatch, batch - b0);
@@ -2733,9 +2739,7 @@ static int run_tree_step(spissa_session *s, const spissa_rope_table *table, cons
     a.out = d_out + at * Hq * D;
     a.parents = d_parents + at;
     at += n;
-    a.q_rot = (float *)s->tree.p;
-    a.mask = (unsigned *)((char *)s->tree.p + q_bytes);
-    a.depth = (int *)((char *)s->tree.p + q_bytes + mask_bytes);
+    a.part = (float *)s->tree.p;
     a.cos = table ? table->cos : nullptr;
     a.sin = table ? table->sin : nullptr;
     a.prescale = 1.0f;
@@ -2751,6 +2755,11 @@ static int run_tree_step(spissa_session *s, const spissa_rope_table *table, cons
     a.R = Hq / Hkv;
     a.window = (int)cfg->window;
     a.qscale = (1.0f / sqrtf((float)D)) * 1.4426950408889634f;
+    const TreePlan &p = plans[b0 / kMaxDecodeBatch];
+    a.splits = p.splits;
+    a.tps = p.tps;
+    a.blocks = p.blocks;
+    a.total = n * Hq;
     HIP_TRY(launch_tree(s->stream, a, D, B));
   }
   for (size_t b = 0; b < batch; ++b) caches[b]->len += nodes[b];

@@ -355,17 +355,23 @@ struct TreeArgs {
   const float *q, *k, *v;        // [N, Hq, D], [N, Hkv, D]
   const int *parents;            // [N]
   float *out;
-  float *q_rot;                  // [N, Hq, D]: the normed, rotated, prescaled queries
-  int *depth;                    // [N]
-  unsigned *mask;                // [N][kTreeMaxNodes / 32]: the nodes that a node sees
+  float *part;                   // [splits][N * Hq] entries of D + 4 floats: output, largest score, sum (splits > 1)
   const float *cos, *sin;        // RoPE table rows by position, or null
   const float *q_norm, *k_norm;  // QK-norm, or null
   float eps, prescale;
   int *err;
   int Hq, Hkv, R, window;
   float qscale;                  // softmax scale * log2(e)
+  int splits, tps, blocks;       // TreePlan
+  int total;                     // N * Hq
   TreeSeq seq[kMaxDecodeBatch];
 };
+// splits: workgroups of the longest sequence over its key tiles, each with up to tps of
+// them; blocks: of 128 rows (nodes x query heads of a KV head) of the largest tree.
+struct TreePlan {
+  int splits = 1, tps = 1, blocks = 1;
+};
+TreePlan tree_plan(int D, int R, int Hkv, int window, const int *past, const int *nodes, int B, int cus);
 hipError_t launch_tree(hipStream_t st, const TreeArgs &a, int D, int B);
 
 struct TreeAcceptArgs {

@@ -7,6 +7,7 @@
 // the nodes it descends from and itself. Its key, rotated at its position, and its
 // value become the cache's row P + t, and
 //   out_t = sum_j p_tj v_j,  p_t = softmax_j(q_t . k_j / sqrt(d)).
+#include <algorithm>
 #include <type_traits>
 
 #include "internal.hpp"
@@ -18,190 +19,526 @@ namespace {
 
 constexpr int kMaskWords = kTreeMaxNodes / 32;
 
-// Each thread's node (of up to 256): its depth and, with MASKS, the nodes that it
-// sees, by doubling: after k rounds a node knows the 2^k nodes above it. A parent
-// out of its range counts as none. For 256 threads.
+// The nodes' depths and, with MASKS, the nodes that each sees, by doubling: after k
+// rounds a node knows the 2^k nodes above it. A parent out of its range counts as
+// none. For kTreeMaxNodes threads or more; ends with the shape in LDS, after a barrier.
 struct TreeShape {
   int depth[kTreeMaxNodes];
   int above[kTreeMaxNodes];  // the node 2^k above
   unsigned mask[kTreeMaxNodes][kMaskWords];
 };
-template <bool MASKS>
-__device__ void tree_shape(const int *parents, int nodes, TreeShape &s, int *err) {
+__device__ __forceinline__ void tree_shape(const int *parents, int nodes, int window, bool masks, TreeShape &s, int *err) {
   const int t = threadIdx.x;
-  int p = t < nodes ? parents[t] : -1;
-  if (p < -1 || p >= t) {
+  const bool mine = t < nodes;
+  int p = mine ? parents[t] : -1;
+  if (mine && (p < -1 || p >= t)) {
     if (err) atomicOr(err, kDevErrTreeParent);
     p = -1;
   }
   int depth = p >= 0 ? 1 : 0;
-  unsigned m[kMaskWords] = {};
-  if constexpr (MASKS) {
-#pragma unroll
-    for (int w = 0; w < kMaskWords; ++w) m[w] = t >> 5 == w ? 1u << (t & 31) : 0u;
-  }
-  for (int span = 1;; span *= 2) {
-    s.depth[t] = depth;
-    s.above[t] = p;
-    if constexpr (MASKS) {
-#pragma unroll
-      for (int w = 0; w < kMaskWords; ++w) s.mask[t][w] = m[w];
+  const int words = (nodes + 31) / 32;
+  if (mine && masks)
+    for (int w = 0; w < words; ++w) s.mask[t][w] = t >> 5 == w ? 1u << (t & 31) : 0u;
+  for (;;) {
+    if (mine) {
+      s.depth[t] = depth;
+      s.above[t] = p;
     }
-    __syncthreads();
-    if (span >= nodes) return;
+    if (!__syncthreads_or(p >= 0)) break;
     int up = -1;
+    unsigned m[kMaskWords];
     if (p >= 0) {
       depth += s.depth[p];
       up = s.above[p];
-      if constexpr (MASKS) {
+      if (masks) {
 #pragma unroll
-        for (int w = 0; w < kMaskWords; ++w) m[w] |= s.mask[p][w];
+        for (int w = 0; w < kMaskWords; ++w)
+          if (w < words) m[w] = s.mask[t][w] | s.mask[p][w];
       }
     }
+    __syncthreads();
+    if (p >= 0 && masks) {
+#pragma unroll
+      for (int w = 0; w < kMaskWords; ++w)
+        if (w < words) s.mask[t][w] = m[w];
+    }
     p = up;
+  }
+  if (masks && window > 0) {
+    if (mine && depth >= window)
+      for (int j = 0; j < t; ++j)
+        if (depth - s.depth[j] >= window) s.mask[t][j >> 5] &= ~(1u << (j & 31));
     __syncthreads();
   }
+}
+
+__device__ __forceinline__ float unbits(unsigned b) { return __uint_as_float(b); }
+
+// Channels 4 l..4 l + 3 and their rotation's partners, half a row on, of row `row`.
+template <int D>
+__device__ __forceinline__ void load_pairs(const float *row, int l, float4 &lo, float4 &hi) {
+  lo = *reinterpret_cast<const float4 *>(row + 4 * l);
+  hi = *reinterpret_cast<const float4 *>(row + D / 2 + 4 * l);
+}
+// The norm's weights times 1 / rms on such channels.
+template <int D>
+__device__ __forceinline__ void norm_pairs(float4 &lo, float4 &hi, const float *w, int l, float inv) {
+#pragma clang fp contract(off)
+  float4 a, b;
+  load_pairs<D>(w, l, a, b);
+  lo = make_float4(lo.x * inv * a.x, lo.y * inv * a.y, lo.z * inv * a.z, lo.w * inv * a.w);
+  hi = make_float4(hi.x * inv * b.x, hi.y * inv * b.y, hi.z * inv * b.z, hi.w * inv * b.w);
+}
+__device__ __forceinline__ void rotate_pairs(float4 &lo, float4 &hi, const float *cos, const float *sin, long at) {
+  const float4 c = *reinterpret_cast<const float4 *>(cos + at), s = *reinterpret_cast<const float4 *>(sin + at);
+  rotate_pair(lo.x, hi.x, c.x, s.x);
+  rotate_pair(lo.y, hi.y, c.y, s.y);
+  rotate_pair(lo.z, hi.z, c.z, s.z);
+  rotate_pair(lo.w, hi.w, c.w, s.w);
+}
+__device__ __forceinline__ float squares(const float4 &a, const float4 &b) {
+#pragma clang fp contract(off)
+  return ((a.x * a.x + b.x * b.x) + (a.y * a.y + b.y * b.y)) + ((a.z * a.z + b.z * b.z) + (a.w * a.w + b.w * b.w));
 }
 
 }  // namespace
 
-// Queries, keys and values of the nodes: the norm, the rotation at the node's
-// position, the rows into the cache (and its bf16 operands). D / 8 threads a row,
-// each with four channels and their rotation's partners, half a row on.
-// Grid: (row blocks of the longest sequence, sequences), 256 threads.
+// Eight waves, each with 16 rows of a KV head (a row: a node and one of the head's
+// query heads) and a share of the loads. Keys go by in tiles of 8192 / D: first the
+// cached rows from the first that any node sees, then the nodes' own. A tile comes
+// into registers while the one before is computed; waves 0..3 take its values, waves
+// 4..7 its keys, and write them to LDS once for all rows as two binary16 pieces, in
+// the order in which lanes take the operands. S^T = K Q^T, so a lane has one row
+// (column lane % 16) and four keys of each 16, and two such blocks are the B operand
+// of O^T += V^T P^T without an exchange, the values' keys being stored in that order.
+// Channels of the scores' product come as 4 l..4 l + 3 beside D / 2 + 4 l..., which
+// makes a rotation's pairs neighbours in a lane.
+//
+// Scales. Pieces hold 2^-23 of a number only between 2^-3 and 2^16. Keys and values
+// are multiplied by a power of two that takes the first tile's largest to 2^11..2^12.
+// Each tile's largest is known after it is written; one that does not fit (or is not
+// finite) is loaded and written again, with the scale that it needs, the output so
+// far following, or, where a number is not finite, with zeros in its place and its key
+// noted: rows that see such a key become NaN.
+//
+// Grid: (KV heads, splits, sequences x blocks of 128 rows).
 template <int D>
-__global__ __launch_bounds__(256) void tree_prepare_kernel(const TreeArgs a) {
+__global__ __launch_bounds__(512, 2) void tree_attend_kernel(const TreeArgs a) {
+  constexpr int BN = 8192 / D, G = D / 32, DT = D / 16, VB = BN / 32, KB = BN / 16, TR = D / 8;
+  __shared__ __attribute__((aligned(16))) half8 kp_lds[2][KB * G * 64];
+  __shared__ __attribute__((aligned(16))) half8 vp_lds[2][VB * DT * 64];
   __shared__ TreeShape shape;
-  constexpr int TR = D / 8, ROWS = 256 / TR;
-  const TreeSeq &s = a.seq[blockIdx.y];
-  const int per = a.Hq + 2 * a.Hkv, total = s.nodes * per;
-  if ((int)blockIdx.x * ROWS >= total) return;
-  if (blockIdx.x == 0) {
-    tree_shape<true>(a.parents + s.first, s.nodes, shape, a.err);
-    const int t = threadIdx.x;
-    if (t < s.nodes) {
-      a.depth[s.first + t] = shape.depth[t];
-#pragma unroll
-      for (int w = 0; w < kMaskWords; ++w) a.mask[(long)(s.first + t) * kMaskWords + w] = shape.mask[t][w];
-    }
-  } else {
-    tree_shape<false>(a.parents + s.first, s.nodes, shape, nullptr);
+  __shared__ unsigned most_lds[2][8];
+  __shared__ unsigned bad_lds[VB];
+
+  float minus_one = -1.0f;
+  asm volatile("" : "+s"(minus_one));
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 15, kq = lane >> 4;
+  const int h = blockIdx.x, split = blockIdx.y, b = blockIdx.z / a.blocks, block = blockIdx.z - b * a.blocks;
+  const int past = a.seq[b].past, nodes = a.seq[b].nodes, seq_first = a.seq[b].first;
+  const int rows = nodes * a.R, row0 = block * 128 + wave * 16;
+  if (block * 128 >= rows) return;
+  const int lo = a.window > 0 ? max(0, past + 1 - a.window) : 0;
+  const int cached = (past - lo + BN - 1) / BN, tiles = cached + (nodes + BN - 1) / BN;
+  const int t0 = split * a.tps, t1 = min(tiles, t0 + a.tps);
+
+  const int r = min(row0 + col, rows - 1), node = r / a.R, hq = h * a.R + (r - node * a.R);
+  const bool live = row0 + col < rows;
+  const long orow = (long)(seq_first + node) * a.Hq + hq;
+  float *const part = a.part + ((long)split * a.total + orow) * (D + 4);
+  if (t0 >= t1) {  // (no keys: nothing of the row's part is read)
+    if (live && kq == 0) *reinterpret_cast<float2 *>(part + D) = make_float2(NEG_INF, 0.0f);
+    return;
   }
-  const int row = blockIdx.x * ROWS + threadIdx.x / TR, c = threadIdx.x % TR * 4;
-  if (row >= total) return;
-  const int node = row / per, hh = row - node * per;
-  const int kind = hh < a.Hq ? 0 : hh < a.Hq + a.Hkv ? 1 : 2;
-  const int h = kind == 0 ? hh : kind == 1 ? hh - a.Hq : hh - a.Hq - a.Hkv;
-  const float *src = kind == 0 ? a.q + ((long)(s.first + node) * a.Hq + h) * D
-                               : (kind == 1 ? a.k : a.v) + ((long)(s.first + node) * a.Hkv + h) * D;
-  const float4 x = *reinterpret_cast<const float4 *>(src + c), y = *reinterpret_cast<const float4 *>(src + D / 2 + c);
-  float lo[4] = {x.x, x.y, x.z, x.w}, hi[4] = {y.x, y.y, y.z, y.w};
-  const long at = s.past + node;
-  if (kind < 2) {
-    if (a.q_norm) {
-#pragma clang fp contract(off)
-      float sum = 0.0f;
+
+  // A thread's share of a tile: of values eight keys (4 q + 0..3 and 16 + 4 q + 0..3 of
+  // 32) of four channels; of keys, four rows' channels 4 l.. and D / 2 + 4 l...
+  const bool values = wave < 4;
+  const int part_of = tid & 255;
+  const int vl = part_of % (D / 4), vg = part_of / (D / 4), vb0 = vg >> 2, vq = vg & 3;
+  const int kl = part_of % TR, kk = part_of / TR;
+  const long stride = (long)a.Hkv * D;
+  float *const cache_rows = (values ? +a.seq[b].v : +a.seq[b].k) + h * D + (values ? 4 * vl : 4 * kl);
+  const float *const own_rows = (values ? +a.v : +a.k) + seq_first * stride + h * D + (values ? 4 * vl : 4 * kl);
+  bf16 *const kb = a.seq[b].kb, *const vt = a.seq[b].vt;
+  const long cap = a.seq[b].cap;
+  float4 raw[8];
+  auto key_of = [&](int i) __attribute__((always_inline)) { return values ? vb0 * 32 + 4 * vq + (i & 3) + 16 * (i >> 2) : kk + (i >> 1) * (256 / TR); };
+  auto load = [&](int tile) __attribute__((always_inline)) {
+    const bool own = tile >= cached;
+    const int first = own ? (tile - cached) * BN : lo + tile * BN, last = (own ? nodes : past) - 1;
+    const float *const src = own ? own_rows : +cache_rows;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sum += lo[i] * lo[i] + hi[i] * hi[i];
-      const float inv = 1.0f / sqrtf(group_sum<TR>(sum) / (float)D + a.eps);
-      const float *w = kind == 0 ? a.q_norm : a.k_norm;
+    for (int i = 0; i < 8; ++i) {
+      const float *at = src + min(first + key_of(i), last) * stride;
+      raw[i] = *reinterpret_cast<const float4 *>(values ? at : at + (i & 1) * (D / 2));
+    }
+  };
+  // The nodes' own rows: the norm and the rotation of keys, and the append.
+  auto finish = [&](int tile) __attribute__((always_inline)) {
+    const int first = (tile - cached) * BN;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        lo[i] = lo[i] * inv * w[c + i];
-        hi[i] = hi[i] * inv * w[D / 2 + c + i];
+    for (int i = 0; i < 8; i += 2) {
+      if (!values) {
+        const int t = min(first + key_of(i), nodes - 1);
+        if (a.k_norm) {
+          const float inv = 1.0f / sqrtf(group_sum<TR>(squares(raw[i], raw[i + 1])) / (float)D + a.eps);
+          norm_pairs<D>(raw[i], raw[i + 1], a.k_norm, kl, inv);
+        }
+        if (a.cos) rotate_pairs(raw[i], raw[i + 1], a.cos, a.sin, (long)(past + shape.depth[t]) * (D / 2) + 4 * kl);
       }
     }
+    if (block != 0) return;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int t = first + key_of(i);
+      if (t >= nodes) continue;
+      const long at = past + t;
+      const int half = values ? 0 : (i & 1) * (D / 2), c = (values ? 4 * vl : 4 * kl) + half;
+      *reinterpret_cast<float4 *>(cache_rows + at * stride + half) = raw[i];
+      if (!kb) continue;
+      const float x[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+      bf16 *const dst = values ? vt + ((long)h * D + c) * cap + vt_key_slot(at) : kb + ((long)h * cap + at) * D + c;
+      const long step = values ? cap : 1;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) dst[j * step] = (bf16)x[j];
+    }
+  };
+  // The wave's largest magnitude, as bits (a NaN or an infinity is above the rest).
+  auto post = [&](int slot) __attribute__((always_inline)) {
+    unsigned m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      m = max(m, max(__float_as_uint(raw[i].x) & 0x7fffffffu, __float_as_uint(raw[i].y) & 0x7fffffffu));
+      m = max(m, max(__float_as_uint(raw[i].z) & 0x7fffffffu, __float_as_uint(raw[i].w) & 0x7fffffffu));
+    }
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) m = max(m, (unsigned)__shfl_xor((int)m, d));
+    if (lane == 0) most_lds[slot][wave] = m;
+  };
+  unsigned kbits = 127u << 23, vbits = 127u << 23;  // the scales, as float bits
+  auto write = [&]() __attribute__((always_inline)) {
+    const float scale = unbits(values ? vbits : kbits);
+    if (values) {
+      const int dt = vl >> 2;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = (c == 0 ? raw[i].x : c == 1 ? raw[i].y : c == 2 ? raw[i].z : raw[i].w) * scale;
+        half8 ph, pl;
+        split8(v, minus_one, &ph, &pl);
+        // (the low bits mixed: the writes of a wave fall on all banks)
+        const int at = (vb0 * DT + dt) * 64 + vq * 16 + ((4 * (vl & 3) + c) ^ (dt & 3));
+        vp_lds[0][at] = ph;
+        vp_lds[1][at] = pl;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; i += 2) {
+        const float v[8] = {raw[i].x * scale,     raw[i].y * scale,     raw[i].z * scale,     raw[i].w * scale,
+                            raw[i + 1].x * scale, raw[i + 1].y * scale, raw[i + 1].z * scale, raw[i + 1].w * scale};
+        half8 ph, pl;
+        split8(v, minus_one, &ph, &pl);
+        const int key = key_of(i), at = ((key >> 4) * G + (kl >> 2)) * 64 + (kl & 3) * 16 + ((key ^ kl) & 15);
+        kp_lds[0][at] = ph;
+        kp_lds[1][at] = pl;
+      }
+    }
+  };
+  auto largest = [&](int slot, int from) __attribute__((always_inline)) {
+    const unsigned *m = most_lds[slot] + from;
+    return max(max(m[0], m[1]), max(m[2], m[3]));
+  };
+
+  if (t0 < cached) load(t0);
+  tree_shape(a.parents + seq_first, nodes, a.window, t1 > cached, shape, block == 0 && split == 0 && h == 0 ? a.err : nullptr);
+  if (t0 >= cached) load(t0);
+
+  // The queries of the wave's rows, as the B operand.
+  half8 qh[G], ql[G];
+  float inv_q;
+  const int pos = past + shape.depth[node], row_lo = a.window > 0 ? max(0, pos + 1 - a.window) : 0;
+  {
+    const float *q = a.q + orow * D;
+    float4 x[G], y[G];
+    float sum = 0.0f, most = 0.0f;
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      load_pairs<D>(q, 4 * g + kq, x[g], y[g]);
+      sum += squares(x[g], y[g]);
+    }
+    if (a.q_norm) {
+      const float inv = 1.0f / sqrtf(sum32(sum16(sum)) / (float)D + a.eps);
+#pragma unroll
+      for (int g = 0; g < G; ++g) norm_pairs<D>(x[g], y[g], a.q_norm, 4 * g + kq, inv);
+    }
     if (a.cos) {
-      const long pos = (s.past + shape.depth[node]) * (long)(D / 2) + c;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) rotate_pair(lo[i], hi[i], a.cos[pos + i], a.sin[pos + i]);
+      for (int g = 0; g < G; ++g) rotate_pairs(x[g], y[g], a.cos, a.sin, (long)pos * (D / 2) + 4 * (4 * g + kq));
+    }
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      float *const v[8] = {&x[g].x, &x[g].y, &x[g].z, &x[g].w, &y[g].x, &y[g].y, &y[g].z, &y[g].w};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        *v[i] = *v[i] * a.prescale * a.qscale;
+        const float m = fabsf(*v[i]);
+        most = fmaxf(most, m <= 3.402823466e38f ? m : 0.0f);
+      }
+    }
+    const unsigned bits = scale_to(max32(max16(most)), 9);
+    const float scale = unbits(bits);
+    inv_q = inverse_scale(bits);
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      const float v[8] = {x[g].x * scale, x[g].y * scale, x[g].z * scale, x[g].w * scale,
+                          y[g].x * scale, y[g].y * scale, y[g].z * scale, y[g].w * scale};
+      split8(v, minus_one, &qh[g], &ql[g]);
     }
   }
-  float *dst;
-  if (kind == 0) {
+  int wave_lo = row_lo;  // keys from here on are seen by all rows of the wave
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      lo[i] *= a.prescale;
-      hi[i] *= a.prescale;
+  for (int d = 8; d > 0; d >>= 1) wave_lo = max(wave_lo, __shfl_xor(wave_lo, d));
+
+  f32x4 o[DT];
+#pragma unroll
+  for (int d = 0; d < DT; ++d) o[d] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  float m = NEG_INF, l = 0.0f;  // m: the largest score so far, or up to 7 below it
+  bool poison = false;
+
+  auto compute = [&](int tile, bool bad) __attribute__((always_inline)) {
+    const bool own = tile >= cached;
+    const int base = lo + tile * BN;
+    f32x4 sc[KB];
+#pragma unroll
+    for (int k = 0; k < KB; ++k) sc[k] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      const int at = g * 64 + kq * 16 + ((col ^ (4 * g + kq)) & 15);
+      half8 fh[KB], fl[KB];
+#pragma unroll
+      for (int k = 0; k < KB; ++k) {
+        fh[k] = kp_lds[0][k * G * 64 + at];
+        fl[k] = kp_lds[1][k * G * 64 + at];
+      }
+#pragma unroll
+      for (int k = 0; k < KB; ++k) sc[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fh[k], qh[g], sc[k], 0, 0, 0);
+#pragma unroll
+      for (int k = 0; k < KB; ++k) sc[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fh[k], ql[g], sc[k], 0, 0, 0);
+#pragma unroll
+      for (int k = 0; k < KB; ++k) sc[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fl[k], qh[g], sc[k], 0, 0, 0);
     }
-    dst = a.q_rot + ((long)(s.first + node) * a.Hq + h) * D;
-  } else {
-    dst = (kind == 1 ? s.k : s.v) + (at * a.Hkv + h) * D;
+    // (finite and above 0: hidden scores stay -inf)
+    const float f = fminf(fmaxf(inv_q * inverse_scale(kbits), 1.1754944e-38f), 3.402823466e38f);
+    // (scores of hidden keys at -inf)
+    if (own || bad || base + BN > past || base < wave_lo) {
+#pragma unroll
+      for (int v = 0; v < VB; ++v) {
+        unsigned seen;
+        if (own) {
+          const int w = (tile - cached) * VB + v;
+          seen = w < kMaskWords && w * 32 < nodes ? shape.mask[node][w] : 0u;
+        } else {
+          const int from = max(0, row_lo - base - 32 * v), to = min(32, past - base - 32 * v);
+          seen = from >= 32 || to <= from ? 0u : (0xffffffffu << from) & (0xffffffffu >> (32 - to));
+        }
+        if (bad) poison |= (seen & bad_lds[v]) != 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (!(seen >> ((i & 3) + 4 * kq + 16 * (i >> 2)) & 1u)) sc[2 * v + (i >> 2)][i & 3] = NEG_INF;
+      }
+    }
+    float big = NEG_INF;
+#pragma unroll
+    for (int k = 0; k < KB; ++k) big = fmaxf(big, fmaxf(fmaxf(sc[k][0], sc[k][1]), fmaxf(sc[k][2], sc[k][3])));
+    big = max32(max16(big)) * f;
+    if (__any(big > m + 7.0f)) {
+      const float next = big > m + 7.0f ? big : m, keep = fast_exp2(m - safe_max(next));
+      m = next;
+      l *= keep;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) o[d] *= keep;
+    }
+    const float off = 8.0f - safe_max(m);  // weights times 2^8, up to 2^15
+    half8 ph[VB], pl[VB];
+#pragma unroll
+    for (int v = 0; v < VB; ++v) {
+      float p[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        p[i] = fast_exp2(fmaf(sc[2 * v + (i >> 2)][i & 3], f, off));
+        l += p[i];
+      }
+      split8(p, minus_one, &ph[v], &pl[v]);
+    }
+#pragma unroll
+    for (int v = 0; v < VB; ++v)
+#pragma unroll
+      for (int d = 0; d < DT; d += 4) {
+        half8 fh[4], fl[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int at = (v * DT + d + j) * 64 + kq * 16 + (col ^ j);
+          fh[j] = vp_lds[0][at];
+          fl[j] = vp_lds[1][at];
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[d + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fh[j], ph[v], o[d + j], 0, 0, 0);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[d + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fh[j], pl[v], o[d + j], 0, 0, 0);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[d + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fl[j], ph[v], o[d + j], 0, 0, 0);
+      }
+  };
+
+  constexpr unsigned kInfinite = 0x7f800000u;
+  constexpr unsigned kTop = (127u + 15u) << 23;  // 2^15
+  for (int tile = t0; tile < t1; ++tile) {
+    const int slot = tile & 1;
+    if (tile >= cached) finish(tile);
+    post(slot);
+    if (tile == t0) {
+      __syncthreads();
+      kbits = scale_to(unbits(min(largest(slot, 4), kInfinite - 1)), 11);
+      vbits = scale_to(unbits(min(largest(slot, 0), kInfinite - 1)), 11);
+    }
+    write();
+    if (tile + 1 < t1) load(tile + 1);
+    __syncthreads();
+    const unsigned km = largest(slot, 4), vm = largest(slot, 0);
+    bool bad = km >= kInfinite || vm >= kInfinite;
+    // (the largest times the scale, by exponents: bits of both less the bias)
+    if (bad || (km > kTop - kbits + (127u << 23) && km != 0) || (vm > kTop - vbits + (127u << 23) && vm != 0)) {
+      __syncthreads();
+      load(tile);
+      if (tile >= cached) finish(tile);
+      if (bad) {
+        if (tid < VB) bad_lds[tid] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          float *const x[4] = {&raw[i].x, &raw[i].y, &raw[i].z, &raw[i].w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (!(fabsf(*x[j]) < __builtin_inff())) {
+              *x[j] = 0.0f;
+              atomicOr(&bad_lds[key_of(i) >> 5], 1u << (key_of(i) & 31));
+            }
+        }
+        post(slot);
+        __syncthreads();
+      }
+      kbits = scale_to(unbits(largest(slot, 4)), 11);
+      unsigned now = scale_to(unbits(largest(slot, 0)), 11);
+      if (tile > t0) now = min(now, vbits);  // (the output so far only ever gets smaller)
+      const float keep = unbits(now) * inverse_scale(vbits);
+      vbits = now;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) o[d] *= keep;
+      write();
+      if (tile + 1 < t1) load(tile + 1);
+      __syncthreads();
+    }
+    if (row0 < rows) compute(tile, bad);
+    __syncthreads();
   }
-  *reinterpret_cast<float4 *>(dst + c) = make_float4(lo[0], lo[1], lo[2], lo[3]);
-  *reinterpret_cast<float4 *>(dst + D / 2 + c) = make_float4(hi[0], hi[1], hi[2], hi[3]);
-  if (kind == 1 && s.kb) {
-    bf16 *kb = s.kb + ((long)h * s.cap + at) * D + c;
+
+  if (row0 >= rows) return;
+  l = sum32(sum16(l));
+  if (poison) l = __builtin_nanf("");
+  const float inv = l == 0.0f ? 0.0f : inverse_scale(vbits) / l;
+  float *const out = a.splits > 1 ? part : a.out + orow * D;
+  if (live) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      kb[i] = (bf16)lo[i];
-      kb[D / 2 + i] = (bf16)hi[i];
-    }
-  } else if (kind == 2 && s.kb) {
-    bf16 *vt = s.vt + ((long)h * D + c) * s.cap + vt_key_slot(at);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      vt[i * s.cap] = (bf16)lo[i];
-      vt[(D / 2 + i) * s.cap] = (bf16)hi[i];
+    for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4 *>(out + 16 * d + 4 * kq) = o[d] * inv;
+    if (a.splits > 1) {
+      if (kq == 0) *reinterpret_cast<float2 *>(part + D) = make_float2(m, l);
+    } else if (!(l > 0.0f) || l > 3.402823466e38f) {
+      atomicOr(a.err, kDevErrSoftmaxDenominator);
     }
   }
 }
 
-// Attention of one node and query head a wave, key by key.
-// Grid: (nodes of the longest sequence, ceil(Hq / 4), sequences), 256 threads.
+// The splits' outputs, each divided by its own sum, by their sums' shares. D / 4
+// threads an output row and as many lanes over the splits as a workgroup has room for.
 template <int D>
-__global__ __launch_bounds__(256) void tree_attend_kernel(const TreeArgs a) {
-  constexpr int E = D / 64;
-  const TreeSeq &s = a.seq[blockIdx.z];
-  const int node = blockIdx.x, hq = blockIdx.y * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-  if (node >= s.nodes || hq >= a.Hq) return;
-  const int h = hq / a.R, depth = a.depth[s.first + node], pos = s.past + depth;
-  const unsigned *mask = a.mask + (long)(s.first + node) * kMaskWords;
-  const long orow = ((long)(s.first + node) * a.Hq + hq) * D + lane * E;
-  float q[E], o[E], m = NEG_INF, l = 0.0f;
-  bool wrong = false;  // a key or value that is not finite
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    q[e] = a.q_rot[orow + e] * a.qscale;
-    o[e] = 0.0f;
-  }
-  auto key = [&](int j) {
-    const long at = ((long)j * a.Hkv + h) * D + lane * E;
-    float dot = 0.0f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const float k = s.k[at + e], v = s.v[at + e];
-      wrong |= !(fabsf(k) < __builtin_inff()) || !(fabsf(v) < __builtin_inff());
-      dot = fmaf(q[e], k, dot);
-    }
-    const float x = group_sum<64>(dot), big = fmaxf(m, x);
-    const float keep = fast_exp2(m - safe_max(big)), p = fast_exp2(x - safe_max(big));
-    l = l * keep + p;
-#pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = fmaf(o[e], keep, p * s.v[at + e]);
+__global__ __launch_bounds__(256) void tree_merge_kernel(const TreeArgs a) {
+  constexpr int TR = D / 4, SL = 256 / TR;
+  __shared__ float4 acc_lds[SL][TR];
+  __shared__ float2 ml_lds[SL];
+  const int c = threadIdx.x % TR, sl = threadIdx.x / TR;
+  const long row = blockIdx.x;
+  float m = NEG_INF, l = 0.0f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i = sl; i < a.splits; i += SL) {
+    const float *const part = a.part + ((long)i * a.total + row) * (D + 4);
+    const float2 ml = *reinterpret_cast<const float2 *>(part + D);
+    if (ml.x == NEG_INF && ml.y == 0.0f) continue;
+    const float4 x = reinterpret_cast<const float4 *>(part)[c];
+    const float big = fmaxf(m, ml.x), keep = fast_exp2(m - safe_max(big)), w = ml.y * fast_exp2(ml.x - safe_max(big));
+    l = l * keep + w;
+    acc = make_float4(fmaf(x.x, w, acc.x * keep), fmaf(x.y, w, acc.y * keep), fmaf(x.z, w, acc.z * keep), fmaf(x.w, w, acc.w * keep));
     m = big;
-  };
-  for (int j = a.window > 0 ? max(0, pos + 1 - a.window) : 0; j < s.past; ++j) key(j);
-  for (int t = 0; t <= node; ++t)
-    if (mask[t >> 5] >> (t & 31) & 1u && (a.window <= 0 || depth - a.depth[s.first + t] < a.window)) key(s.past + t);
-  if (__any(wrong)) l = __builtin_nanf("");
-  if (!(l > 0.0f) || l > 3.402823466e38f) {
-    if (lane == 0) atomicOr(a.err, kDevErrSoftmaxDenominator);
   }
+  acc_lds[sl][c] = acc;
+  if (c == 0) ml_lds[sl] = make_float2(m, l);
+  __syncthreads();
+  if (sl != 0) return;
+  float big = NEG_INF;
 #pragma unroll
-  for (int e = 0; e < E; ++e) a.out[orow + e] = o[e] / l;
+  for (int i = 0; i < SL; ++i) big = fmaxf(big, ml_lds[i].x);
+  l = 0.0f;
+  acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+  for (int i = 0; i < SL; ++i) {
+    const float w = fast_exp2(ml_lds[i].x - safe_max(big));
+    const float4 x = acc_lds[i][c];
+    l = fmaf(ml_lds[i].y, w, l);
+    acc = make_float4(fmaf(x.x, w, acc.x), fmaf(x.y, w, acc.y), fmaf(x.z, w, acc.z), fmaf(x.w, w, acc.w));
+  }
+  if (c == 0 && (!(l > 0.0f) || l > 3.402823466e38f)) atomicOr(a.err, kDevErrSoftmaxDenominator);
+  const float inv = 1.0f / l;
+  *reinterpret_cast<float4 *>(a.out + row * D + 4 * c) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+}
+
+// Tiles a workgroup takes, for about a workgroup a CU; blocks of the largest tree; splits of the longest
+// sequence.
+TreePlan tree_plan(int D, int R, int Hkv, int window, const int *past, const int *nodes, int B, int cus) {
+  const int BN = 8192 / D;
+  TreePlan p;
+  long work = 0;
+  int most = 0;
+  for (int b = 0; b < B; ++b) {
+    if (!nodes[b]) continue;
+    const int lo = window > 0 ? std::max(0, past[b] + 1 - window) : 0;
+    const int tiles = (past[b] - lo + BN - 1) / BN + (nodes[b] + BN - 1) / BN, blocks = (nodes[b] * R + 127) / 128;
+    work += (long)tiles * blocks * Hkv;
+    most = std::max(most, tiles);
+    p.blocks = std::max(p.blocks, blocks);
+  }
+  p.tps = (int)std::max<long>(1, (work + cus - 1) / cus);
+  for (;; ++p.tps) {
+    long groups = 0;
+    for (int b = 0; b < B; ++b) {
+      if (!nodes[b]) continue;
+      const int lo = window > 0 ? std::max(0, past[b] + 1 - window) : 0;
+      const int tiles = (past[b] - lo + BN - 1) / BN + (nodes[b] + BN - 1) / BN;
+      groups += (long)((tiles + p.tps - 1) / p.tps) * ((nodes[b] * R + 127) / 128) * Hkv;
+    }
+    if (groups <= cus || p.tps >= most) break;
+  }
+  p.splits = (most + p.tps - 1) / p.tps;
+  return p;
 }
 
 hipError_t launch_tree(hipStream_t st, const TreeArgs &a, int D, int B) {
-  int most = 0;
-  for (int b = 0; b < B; ++b) most = a.seq[b].nodes > most ? a.seq[b].nodes : most;
-  const int rows = 256 / (D / 8);
-  const dim3 prepare((unsigned)((most * (long)(a.Hq + 2 * a.Hkv) + rows - 1) / rows), B);
-  const dim3 attend(most, (a.Hq + 3) / 4, B);
+  const dim3 grid(a.Hkv, a.splits, B * a.blocks);
   auto run = [&](auto d) {
     constexpr int DD = decltype(d)::value;
-    hipLaunchKernelGGL(tree_prepare_kernel<DD>, prepare, dim3(256), 0, st, a);
-    hipLaunchKernelGGL(tree_attend_kernel<DD>, attend, dim3(256), 0, st, a);
+    hipLaunchKernelGGL(tree_attend_kernel<DD>, grid, dim3(512), 0, st, a);
+    if (a.splits > 1) hipLaunchKernelGGL(tree_merge_kernel<DD>, dim3((unsigned)a.total), dim3(256), 0, st, a);
   };
   if (D == 64) run(std::integral_constant<int, 64>{});
   else if (D == 128) run(std::integral_constant<int, 128>{});
@@ -296,16 +633,19 @@ __global__ __launch_bounds__(256) void keep_kernel(const KeepArgs a) {
   __shared__ int path[kTreeMaxNodes], end;
   const KeepCache &c = a.cache[blockIdx.y];
   const bool values = blockIdx.z != 0;
+  const int nodes = c.nodes, first = c.first, heads = c.heads, dim = c.dim, kind = c.kind;
+  const long cap = c.cap, P = c.past, width = (long)heads * dim;
+  char *const rows = values ? +c.v : +c.k, *const more = values ? +c.vp : +c.kp;
   const int t = threadIdx.x;
   int count = a.count[c.seq];
-  bool wrong = count < 0 || count > c.nodes;
-  count = min(max(count, 0), c.nodes);
+  bool wrong = count < 0 || count > nodes;
+  count = min(max(count, 0), nodes);
   if (t == 0) end = count;
   __syncthreads();
   if (t < count) {
-    const int p = a.path[c.first + t];
+    const int p = a.path[first + t];
     path[t] = p;
-    if (p < 0 || p >= c.nodes || (t > 0 && p <= a.path[c.first + t - 1])) {
+    if (p < 0 || p >= nodes || (t > 0 && p <= a.path[first + t - 1])) {
       wrong = true;
       atomicMin(&end, t);
     }
@@ -313,41 +653,39 @@ __global__ __launch_bounds__(256) void keep_kernel(const KeepArgs a) {
   if (wrong && blockIdx.x == 0 && !values) atomicOr(a.err, kDevErrTreePath);
   __syncthreads();
   const int n = end;
-  const long width = (long)c.heads * c.dim, P = c.past;
   const long unit = (long)blockIdx.x * 256 + t;
-  char *const rows = values ? c.v : c.k;
-  if (c.kind == 2) {
+  if (kind == 2) {
     // pieces of a head's codes, then its words of step and minimum
-    const int pieces = c.dim / 32, words = c.dim / 32;
+    const int pieces = dim / 32, words = dim / 32;
     const long h = unit / (pieces + words);
     const int i = (int)(unit - h * (pieces + words));
-    if (h >= c.heads) return;
+    if (h >= heads) return;
     if (i < pieces) {
-      char *const p = rows + (h * c.cap + P) * (c.dim / 2) + i * 16;
-      move_rows<uint4>(path, n, [&](int r) { return p + (long)r * (c.dim / 2); });
+      char *const p = rows + (h * cap + P) * (dim / 2) + i * 16;
+      move_rows<u32x4>(path, n, [&](int r) __attribute__((always_inline)) { return p + (long)r * (dim / 2); });
     } else {
-      char *const p = (values ? c.vp : c.kp) + ((h * c.cap + P) * words + (i - pieces)) * 4;
-      move_rows<unsigned>(path, n, [&](int r) { return p + (long)r * words * 4; });
+      char *const p = more + ((h * cap + P) * words + (i - pieces)) * 4;
+      move_rows<unsigned>(path, n, [&](int r) __attribute__((always_inline)) { return p + (long)r * words * 4; });
     }
     return;
   }
   const bool wide = width % 4 == 0;
   if (unit < (wide ? width / 4 : width)) {
     char *const p = rows + (P * width + unit * (wide ? 4 : 1)) * 4;
-    if (wide) move_rows<uint4>(path, n, [&](int r) { return p + (long)r * width * 4; });
-    else move_rows<unsigned>(path, n, [&](int r) { return p + (long)r * width * 4; });
+    if (wide) move_rows<u32x4>(path, n, [&](int r) __attribute__((always_inline)) { return p + (long)r * width * 4; });
+    else move_rows<unsigned>(path, n, [&](int r) __attribute__((always_inline)) { return p + (long)r * width * 4; });
   }
-  if (c.kind == 0) return;
+  if (kind == 0) return;
   if (!values) {  // bf16 keys [H, cap, D], eight a thread
-    const long h = unit / (c.dim / 8);
-    const int i = (int)(unit - h * (c.dim / 8));
-    if (h >= c.heads) return;
-    char *const p = c.kp + ((h * c.cap + P) * c.dim + i * 8) * 2;
-    move_rows<uint4>(path, n, [&](int r) { return p + (long)r * c.dim * 2; });
+    const long h = unit / (dim / 8);
+    const int i = (int)(unit - h * (dim / 8));
+    if (h >= heads) return;
+    char *const p = more + ((h * cap + P) * dim + i * 8) * 2;
+    move_rows<u32x4>(path, n, [&](int r) __attribute__((always_inline)) { return p + (long)r * dim * 2; });
   } else {  // bf16 values [H, D, cap], four channels a thread
     for (long i = unit * 4; i < min(unit * 4 + 4, width); ++i) {
-      char *const p = c.vp + i * c.cap * 2;
-      move_rows<unsigned short>(path, n, [&](int r) { return p + vt_key_slot(P + r) * 2; });
+      char *const p = more + i * cap * 2;
+      move_rows<unsigned short>(path, n, [&](int r) __attribute__((always_inline)) { return p + vt_key_slot(P + r) * 2; });
     }
   }
 }
