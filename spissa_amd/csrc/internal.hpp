@@ -351,7 +351,7 @@ struct TreeSeq {
   int past, nodes;   // cached rows; nodes, whose rows come after them
   int first, pad;    // the sequence's first node among the launch's
 };
-struct TreeArgs {
+struct TreeBase {
   const float *q, *k, *v;        // [N, Hq, D], [N, Hkv, D]
   const int *parents;            // [N]
   float *out;
@@ -364,7 +364,17 @@ struct TreeArgs {
   float qscale;                  // softmax scale * log2(e)
   int splits, tps, blocks;       // TreePlan
   int total;                     // N * Hq
-  TreeSeq seq[kMaxDecodeBatch];
+};
+template <int MB>
+struct TreeArgsOf : TreeBase {
+  TreeSeq seq[MB];
+};
+typedef TreeArgsOf<kMaxDecodeBatch> TreeArgs;
+struct TreeMerge {
+  const float *part;
+  float *out;
+  int *err;
+  int splits, total;
 };
 // splits: workgroups of the longest sequence over its key tiles, each with up to tps of
 // them; blocks: of 128 rows (nodes x query heads of a KV head) of the largest tree.

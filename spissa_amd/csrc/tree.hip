@@ -27,10 +27,10 @@ struct TreeShape {
   int above[kTreeMaxNodes];  // the node 2^k above
   unsigned mask[kTreeMaxNodes][kMaskWords];
 };
-__device__ __forceinline__ void tree_shape(const int *parents, int nodes, int window, bool masks, TreeShape &s, int *err) {
+// p: the thread's node's parent.
+__device__ __forceinline__ void tree_shape(int p, int nodes, int window, bool masks, TreeShape &s, int *err) {
   const int t = threadIdx.x;
   const bool mine = t < nodes;
-  int p = mine ? parents[t] : -1;
   if (mine && (p < -1 || p >= t)) {
     if (err) atomicOr(err, kDevErrTreeParent);
     p = -1;
@@ -122,11 +122,11 @@ __device__ __forceinline__ float squares(const float4 &a, const float4 &b) {
 // noted: rows that see such a key become NaN.
 //
 // Grid: (KV heads, splits, sequences x blocks of 128 rows).
-template <int D>
-__global__ __launch_bounds__(512, 2) void tree_attend_kernel(const TreeArgs a) {
+template <int D, int MB>
+__global__ __launch_bounds__(512, 2) void tree_attend_kernel(const TreeArgsOf<MB> a) {
   constexpr int BN = 8192 / D, G = D / 32, DT = D / 16, VB = BN / 32, KB = BN / 16, TR = D / 8;
-  __shared__ __attribute__((aligned(16))) half8 kp_lds[2][KB * G * 64];
-  __shared__ __attribute__((aligned(16))) half8 vp_lds[2][VB * DT * 64];
+  __shared__ __attribute__((aligned(16))) half8 kp_lds[2][2][KB * G * 64];
+  __shared__ __attribute__((aligned(16))) half8 vp_lds[2][2][VB * DT * 64];
   __shared__ TreeShape shape;
   __shared__ unsigned most_lds[2][8];
   __shared__ unsigned bad_lds[VB];
@@ -153,35 +153,45 @@ __global__ __launch_bounds__(512, 2) void tree_attend_kernel(const TreeArgs a) {
   }
 
   // A thread's share of a tile: of values eight keys (4 q + 0..3 and 16 + 4 q + 0..3 of
-  // 32) of four channels; of keys, four rows' channels 4 l.. and D / 2 + 4 l...
+  // 32) of four channels; of keys, four rows' channels 4 l.. and D / 2 + 4 l... Load i
+  // has the key thread_key + step_key(i).
   const bool values = wave < 4;
   const int part_of = tid & 255;
-  const int vl = part_of % (D / 4), vg = part_of / (D / 4), vb0 = vg >> 2, vq = vg & 3;
-  const int kl = part_of % TR, kk = part_of / TR;
+  const int vg = part_of / (D / 4);
+  int vl = part_of % (D / 4), vb0 = vg >> 2, vq = vg & 3;
+  int kl = part_of % TR, kk = part_of / TR;
+  int thread_key = values ? vb0 * 32 + 4 * vq : kk, thread_channel = values ? 4 * vl : 4 * kl;
   const long stride = (long)a.Hkv * D;
-  float *const cache_rows = (values ? +a.seq[b].v : +a.seq[b].k) + h * D + (values ? 4 * vl : 4 * kl);
-  const float *const own_rows = (values ? +a.v : +a.k) + seq_first * stride + h * D + (values ? 4 * vl : 4 * kl);
+  float *const cache_rows = (values ? +a.seq[b].v : +a.seq[b].k) + h * D;
+  const float *const own_rows = (values ? +a.v : +a.k) + seq_first * stride + h * D;
   bf16 *const kb = a.seq[b].kb, *const vt = a.seq[b].vt;
   const long cap = a.seq[b].cap;
   float4 raw[8];
-  auto key_of = [&](int i) __attribute__((always_inline)) { return values ? vb0 * 32 + 4 * vq + (i & 3) + 16 * (i >> 2) : kk + (i >> 1) * (256 / TR); };
+  auto step_key = [&](int i) __attribute__((always_inline)) { return values ? (i & 3) + 16 * (i >> 2) : (i >> 1) * (256 / TR); };
   auto load = [&](int tile) __attribute__((always_inline)) {
     const bool own = tile >= cached;
-    const int first = own ? (tile - cached) * BN : lo + tile * BN, last = (own ? nodes : past) - 1;
-    const float *const src = own ? own_rows : +cache_rows;
+    const int first = own ? (tile - cached) * BN : lo + tile * BN, left = (own ? nodes : past) - first;
+    const char *const src = reinterpret_cast<const char *>((own ? own_rows : +cache_rows) + first * stride);
+    if (left >= BN) {
+      const unsigned off = (unsigned)(thread_key * stride + thread_channel) * 4u;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float *at = src + min(first + key_of(i), last) * stride;
-      raw[i] = *reinterpret_cast<const float4 *>(values ? at : at + (i & 1) * (D / 2));
+      for (int i = 0; i < 8; ++i)
+        raw[i] = *reinterpret_cast<const float4 *>(src + (step_key(i) * stride + (values ? 0 : (i & 1) * (D / 2))) * 4 + off);
+    } else {  // (rows past the last: that one again)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const long at = min(thread_key + step_key(i), left - 1) * stride + thread_channel + (values ? 0 : (i & 1) * (D / 2));
+        raw[i] = *reinterpret_cast<const float4 *>(src + at * 4);
+      }
     }
   };
   // The nodes' own rows: the norm and the rotation of keys, and the append.
   auto finish = [&](int tile) __attribute__((always_inline)) {
-    const int first = (tile - cached) * BN;
+    const int first = (tile - cached) * BN + thread_key;
+    if (!values) {
 #pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-      if (!values) {
-        const int t = min(first + key_of(i), nodes - 1);
+      for (int i = 0; i < 8; i += 2) {
+        const int t = min(first + step_key(i), nodes - 1);
         if (a.k_norm) {
           const float inv = 1.0f / sqrtf(group_sum<TR>(squares(raw[i], raw[i + 1])) / (float)D + a.eps);
           norm_pairs<D>(raw[i], raw[i + 1], a.k_norm, kl, inv);
@@ -192,11 +202,11 @@ __global__ __launch_bounds__(512, 2) void tree_attend_kernel(const TreeArgs a) {
     if (block != 0) return;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int t = first + key_of(i);
+      const int t = first + step_key(i);
       if (t >= nodes) continue;
       const long at = past + t;
-      const int half = values ? 0 : (i & 1) * (D / 2), c = (values ? 4 * vl : 4 * kl) + half;
-      *reinterpret_cast<float4 *>(cache_rows + at * stride + half) = raw[i];
+      const int c = thread_channel + (values ? 0 : (i & 1) * (D / 2));
+      *reinterpret_cast<float4 *>(cache_rows + at * stride + c) = raw[i];
       if (!kb) continue;
       const float x[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
       bf16 *const dst = values ? vt + ((long)h * D + c) * cap + vt_key_slot(at) : kb + ((long)h * cap + at) * D + c;
@@ -218,7 +228,7 @@ __global__ __launch_bounds__(512, 2) void tree_attend_kernel(const TreeArgs a) {
     if (lane == 0) most_lds[slot][wave] = m;
   };
   unsigned kbits = 127u << 23, vbits = 127u << 23;  // the scales, as float bits
-  auto write = [&]() __attribute__((always_inline)) {
+  auto write = [&](int buf) __attribute__((always_inline)) {
     const float scale = unbits(values ? vbits : kbits);
     if (values) {
       const int dt = vl >> 2;
@@ -231,8 +241,8 @@ __global__ __launch_bounds__(512, 2) void tree_attend_kernel(const TreeArgs a) {
         split8(v, minus_one, &ph, &pl);
         // (the low bits mixed: the writes of a wave fall on all banks)
         const int at = (vb0 * DT + dt) * 64 + vq * 16 + ((4 * (vl & 3) + c) ^ (dt & 3));
-        vp_lds[0][at] = ph;
-        vp_lds[1][at] = pl;
+        vp_lds[buf][0][at] = ph;
+        vp_lds[buf][1][at] = pl;
       }
     } else {
 #pragma unroll
@@ -241,9 +251,9 @@ __global__ __launch_bounds__(512, 2) void tree_attend_kernel(const TreeArgs a) {
                             raw[i + 1].x * scale, raw[i + 1].y * scale, raw[i + 1].z * scale, raw[i + 1].w * scale};
         half8 ph, pl;
         split8(v, minus_one, &ph, &pl);
-        const int key = key_of(i), at = ((key >> 4) * G + (kl >> 2)) * 64 + (kl & 3) * 16 + ((key ^ kl) & 15);
-        kp_lds[0][at] = ph;
-        kp_lds[1][at] = pl;
+        const int key = thread_key + step_key(i), at = ((key >> 4) * G + (kl >> 2)) * 64 + (kl & 3) * 16 + ((key ^ kl) & 15);
+        kp_lds[buf][0][at] = ph;
+        kp_lds[buf][1][at] = pl;
       }
     }
   };
@@ -252,24 +262,24 @@ __global__ __launch_bounds__(512, 2) void tree_attend_kernel(const TreeArgs a) {
     return max(max(m[0], m[1]), max(m[2], m[3]));
   };
 
-  if (t0 < cached) load(t0);
-  tree_shape(a.parents + seq_first, nodes, a.window, t1 > cached, shape, block == 0 && split == 0 && h == 0 ? a.err : nullptr);
-  if (t0 >= cached) load(t0);
+  // (all that needs no other load first: the parents, the queries, the first tiles)
+  const int parent = tid < nodes ? a.parents[seq_first + tid] : -1;
+  float4 x[G], y[G];
+#pragma unroll
+  for (int g = 0; g < G; ++g) load_pairs<D>(a.q + orow * D, 4 * g + kq, x[g], y[g]);
+  load(t0);
+  tree_shape(parent, nodes, a.window, t1 > cached, shape, block == 0 && split == 0 && h == 0 ? a.err : nullptr);
 
   // The queries of the wave's rows, as the B operand.
   half8 qh[G], ql[G];
   float inv_q;
   const int pos = past + shape.depth[node], row_lo = a.window > 0 ? max(0, pos + 1 - a.window) : 0;
   {
-    const float *q = a.q + orow * D;
-    float4 x[G], y[G];
-    float sum = 0.0f, most = 0.0f;
-#pragma unroll
-    for (int g = 0; g < G; ++g) {
-      load_pairs<D>(q, 4 * g + kq, x[g], y[g]);
-      sum += squares(x[g], y[g]);
-    }
+    float most = 0.0f;
     if (a.q_norm) {
+      float sum = 0.0f;
+#pragma unroll
+      for (int g = 0; g < G; ++g) sum += squares(x[g], y[g]);
       const float inv = 1.0f / sqrtf(sum32(sum16(sum)) / (float)D + a.eps);
 #pragma unroll
       for (int g = 0; g < G; ++g) norm_pairs<D>(x[g], y[g], a.q_norm, 4 * g + kq, inv);
@@ -309,6 +319,7 @@ __global__ __launch_bounds__(512, 2) void tree_attend_kernel(const TreeArgs a) {
   bool poison = false;
 
   auto compute = [&](int tile, bool bad) __attribute__((always_inline)) {
+    const int buf = tile & 1;
     const bool own = tile >= cached;
     const int base = lo + tile * BN;
     f32x4 sc[KB];
@@ -320,8 +331,8 @@ __global__ __launch_bounds__(512, 2) void tree_attend_kernel(const TreeArgs a) {
       half8 fh[KB], fl[KB];
 #pragma unroll
       for (int k = 0; k < KB; ++k) {
-        fh[k] = kp_lds[0][k * G * 64 + at];
-        fl[k] = kp_lds[1][k * G * 64 + at];
+        fh[k] = kp_lds[buf][0][k * G * 64 + at];
+        fl[k] = kp_lds[buf][1][k * G * 64 + at];
       }
 #pragma unroll
       for (int k = 0; k < KB; ++k) sc[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fh[k], qh[g], sc[k], 0, 0, 0);
@@ -381,8 +392,8 @@ __global__ __launch_bounds__(512, 2) void tree_attend_kernel(const TreeArgs a) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int at = (v * DT + d + j) * 64 + kq * 16 + (col ^ j);
-          fh[j] = vp_lds[0][at];
-          fl[j] = vp_lds[1][at];
+          fh[j] = vp_lds[buf][0][at];
+          fl[j] = vp_lds[buf][1][at];
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) o[d + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fh[j], ph[v], o[d + j], 0, 0, 0);
@@ -395,53 +406,77 @@ __global__ __launch_bounds__(512, 2) void tree_attend_kernel(const TreeArgs a) {
 
   constexpr unsigned kInfinite = 0x7f800000u;
   constexpr unsigned kTop = (127u + 15u) << 23;  // 2^15
-  for (int tile = t0; tile < t1; ++tile) {
-    const int slot = tile & 1;
-    if (tile >= cached) finish(tile);
-    post(slot);
-    if (tile == t0) {
-      __syncthreads();
-      kbits = scale_to(unbits(min(largest(slot, 4), kInfinite - 1)), 11);
-      vbits = scale_to(unbits(min(largest(slot, 0), kInfinite - 1)), 11);
-    }
-    write();
-    if (tile + 1 < t1) load(tile + 1);
-    __syncthreads();
-    const unsigned km = largest(slot, 4), vm = largest(slot, 0);
-    bool bad = km >= kInfinite || vm >= kInfinite;
+  // The first tile in LDS, with the scales that it sets.
+  if (t0 >= cached) finish(t0);
+  post(t0 & 1);
+  __syncthreads();
+  kbits = scale_to(unbits(min(largest(t0 & 1, 4), kInfinite - 1)), 11);
+  vbits = scale_to(unbits(min(largest(t0 & 1, 0), kInfinite - 1)), 11);
+  write(t0 & 1);
+  if (t0 + 1 < t1) load(t0 + 1);
+  __syncthreads();
+
+  // Between two barriers a wave computes its rows' part of a tile and writes its share
+  // of the next one, the first four waves in the other order: a SIMD has one of each.
+  // A tile that has to be written again takes a turn of its own, one in which something
+  // is not finite two, as the largest of the rest is not known before it is written.
+  bool bad = false, rescale = false;
+#pragma unroll 1
+  for (int tile = t0; tile < t1;) {
+    // (addresses anew each turn: kept, they would not leave room for the rest)
+    asm volatile("" : "+v"(thread_key), "+v"(thread_channel), "+v"(kl), "+v"(vl), "+v"(vb0), "+v"(vq));
+    const unsigned km = largest(tile & 1, 4), vm = largest(tile & 1, 0);
+    const bool more = km >= kInfinite || vm >= kInfinite;
     // (the largest times the scale, by exponents: bits of both less the bias)
-    if (bad || (km > kTop - kbits + (127u << 23) && km != 0) || (vm > kTop - vbits + (127u << 23) && vm != 0)) {
-      __syncthreads();
+    const bool again = more || rescale || km > kTop - kbits + (127u << 23) || vm > kTop - vbits + (127u << 23);
+    const int target = again ? tile : tile + 1;
+    if (again) {
       load(tile);
-      if (tile >= cached) finish(tile);
-      if (bad) {
+      if (more) {
+        bad = rescale = true;
         if (tid < VB) bad_lds[tid] = 0;
-        __syncthreads();
+      } else {
+        rescale = false;
+        kbits = scale_to(unbits(km), 11);
+        unsigned now = scale_to(unbits(vm), 11);
+        if (tile > t0) now = min(now, vbits);  // (the output so far only ever gets smaller)
+        const float keep = unbits(now) * inverse_scale(vbits);
+        vbits = now;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[d] *= keep;
+      }
+      __syncthreads();  // (the tile's largest is read, its bad keys cleared)
+    }
+    auto stage = [&]() __attribute__((always_inline)) {
+      if (target >= t1) return;
+      if (target >= cached) finish(target);
+      if (again && bad) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          float *const x[4] = {&raw[i].x, &raw[i].y, &raw[i].z, &raw[i].w};
+          float v[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+          bool wrong = false;
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            if (!(fabsf(*x[j]) < __builtin_inff())) {
-              *x[j] = 0.0f;
-              atomicOr(&bad_lds[key_of(i) >> 5], 1u << (key_of(i) & 31));
+            if (!(fabsf(v[j]) < __builtin_inff())) {
+              v[j] = 0.0f;
+              wrong = true;
             }
+          raw[i] = make_float4(v[0], v[1], v[2], v[3]);
+          const int key = thread_key + step_key(i);
+          if (wrong) atomicOr(&bad_lds[key >> 5], 1u << (key & 31));
         }
-        post(slot);
-        __syncthreads();
       }
-      kbits = scale_to(unbits(largest(slot, 4)), 11);
-      unsigned now = scale_to(unbits(largest(slot, 0)), 11);
-      if (tile > t0) now = min(now, vbits);  // (the output so far only ever gets smaller)
-      const float keep = unbits(now) * inverse_scale(vbits);
-      vbits = now;
-#pragma unroll
-      for (int d = 0; d < DT; ++d) o[d] *= keep;
-      write();
-      if (tile + 1 < t1) load(tile + 1);
-      __syncthreads();
+      post(target & 1);
+      write(target & 1);
+      if (target + 1 < t1) load(target + 1);
+    };
+    if (values) stage();
+    if (!again && row0 < rows) compute(tile, bad);
+    if (!values) stage();
+    if (!again) {
+      bad = false;
+      ++tile;
     }
-    if (row0 < rows) compute(tile, bad);
     __syncthreads();
   }
 
@@ -464,22 +499,39 @@ __global__ __launch_bounds__(512, 2) void tree_attend_kernel(const TreeArgs a) {
 // The splits' outputs, each divided by its own sum, by their sums' shares. D / 4
 // threads an output row and as many lanes over the splits as a workgroup has room for.
 template <int D>
-__global__ __launch_bounds__(256) void tree_merge_kernel(const TreeArgs a) {
-  constexpr int TR = D / 4, SL = 256 / TR;
+__global__ __launch_bounds__(256) void tree_merge_kernel(const TreeMerge a) {
+  constexpr int TR = D / 4, SL = 256 / TR, AT_ONCE = 8;
   __shared__ float4 acc_lds[SL][TR];
   __shared__ float2 ml_lds[SL];
   const int c = threadIdx.x % TR, sl = threadIdx.x / TR;
   const long row = blockIdx.x;
   float m = NEG_INF, l = 0.0f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i = sl; i < a.splits; i += SL) {
-    const float *const part = a.part + ((long)i * a.total + row) * (D + 4);
-    const float2 ml = *reinterpret_cast<const float2 *>(part + D);
-    if (ml.x == NEG_INF && ml.y == 0.0f) continue;
-    const float4 x = reinterpret_cast<const float4 *>(part)[c];
-    const float big = fmaxf(m, ml.x), keep = fast_exp2(m - safe_max(big)), w = ml.y * fast_exp2(ml.x - safe_max(big));
-    l = l * keep + w;
-    acc = make_float4(fmaf(x.x, w, acc.x * keep), fmaf(x.y, w, acc.y * keep), fmaf(x.z, w, acc.z * keep), fmaf(x.w, w, acc.w * keep));
+  for (int i = sl; i < a.splits; i += SL * AT_ONCE) {
+    float2 ml[AT_ONCE];
+    float4 x[AT_ONCE];
+#pragma unroll
+    for (int j = 0; j < AT_ONCE; ++j) {
+      const float *const part = a.part + ((long)min(i + j * SL, a.splits - 1) * a.total + row) * (D + 4);
+      ml[j] = *reinterpret_cast<const float2 *>(part + D);
+      x[j] = reinterpret_cast<const float4 *>(part)[c];
+    }
+    float big = m;
+#pragma unroll
+    for (int j = 0; j < AT_ONCE; ++j) {
+      if (i + j * SL >= a.splits) ml[j] = make_float2(NEG_INF, 0.0f);
+      big = fmaxf(big, ml[j].x);
+    }
+    const float keep = fast_exp2(m - safe_max(big));
+    l *= keep;
+    acc = make_float4(acc.x * keep, acc.y * keep, acc.z * keep, acc.w * keep);
+#pragma unroll
+    for (int j = 0; j < AT_ONCE; ++j) {
+      if (ml[j].x == NEG_INF && ml[j].y == 0.0f) continue;  // (a part without keys is not written)
+      const float w = ml[j].y * fast_exp2(ml[j].x - safe_max(big));
+      l += w;
+      acc = make_float4(fmaf(x[j].x, w, acc.x), fmaf(x[j].y, w, acc.y), fmaf(x[j].z, w, acc.z), fmaf(x[j].w, w, acc.w));
+    }
     m = big;
   }
   acc_lds[sl][c] = acc;
@@ -503,47 +555,64 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(const TreeArgs a) {
   *reinterpret_cast<float4 *>(a.out + row * D + 4 * c) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
 }
 
-// Tiles a workgroup takes, for about a workgroup a CU; blocks of the largest tree; splits of the longest
-// sequence.
+// The number of splits by a model of the launch: rounds of a workgroup a CU, each of a
+// start and its tiles, and the merge, which reads each split's output.
 TreePlan tree_plan(int D, int R, int Hkv, int window, const int *past, const int *nodes, int B, int cus) {
   const int BN = 8192 / D;
+  int tiles[kMaxDecodeBatch], blocks[kMaxDecodeBatch], most = 1;
+  long rows = 0;
   TreePlan p;
-  long work = 0;
-  int most = 0;
   for (int b = 0; b < B; ++b) {
+    tiles[b] = blocks[b] = 0;
     if (!nodes[b]) continue;
     const int lo = window > 0 ? std::max(0, past[b] + 1 - window) : 0;
-    const int tiles = (past[b] - lo + BN - 1) / BN + (nodes[b] + BN - 1) / BN, blocks = (nodes[b] * R + 127) / 128;
-    work += (long)tiles * blocks * Hkv;
-    most = std::max(most, tiles);
-    p.blocks = std::max(p.blocks, blocks);
+    tiles[b] = (past[b] - lo + BN - 1) / BN + (nodes[b] + BN - 1) / BN;
+    blocks[b] = (nodes[b] * R + 127) / 128;
+    most = std::max(most, tiles[b]);
+    p.blocks = std::max(p.blocks, blocks[b]);
+    rows += (long)nodes[b] * R * Hkv;
   }
-  p.tps = (int)std::max<long>(1, (work + cus - 1) / cus);
-  for (;; ++p.tps) {
+  constexpr double kStart = 6.0, kTile = 2.7;  // us
+  double best = 0.0;
+  for (int splits = 1; splits <= std::min(most, 128); ++splits) {
+    const int tps = (most + splits - 1) / splits;
+    if (splits > 1 && (most + tps - 1) / tps != splits) continue;
     long groups = 0;
-    for (int b = 0; b < B; ++b) {
-      if (!nodes[b]) continue;
-      const int lo = window > 0 ? std::max(0, past[b] + 1 - window) : 0;
-      const int tiles = (past[b] - lo + BN - 1) / BN + (nodes[b] + BN - 1) / BN;
-      groups += (long)((tiles + p.tps - 1) / p.tps) * ((nodes[b] * R + 127) / 128) * Hkv;
+    for (int b = 0; b < B; ++b) groups += (long)((tiles[b] + tps - 1) / tps) * blocks[b] * Hkv;
+    const double rounds = (double)((groups + cus - 1) / cus);
+    const double merge = splits > 1 ? 2.0 + rows * splits * D * 1.0e-6 : 0.0;  // us: a launch, 4 MB a us
+    const double time = rounds * (kStart + tps * kTile) + merge;
+    if (splits == 1 || time < best) {
+      best = time;
+      p.splits = splits;
+      p.tps = tps;
     }
-    if (groups <= cus || p.tps >= most) break;
   }
-  p.splits = (most + p.tps - 1) / p.tps;
   return p;
 }
 
-hipError_t launch_tree(hipStream_t st, const TreeArgs &a, int D, int B) {
-  const dim3 grid(a.Hkv, a.splits, B * a.blocks);
-  auto run = [&](auto d) {
-    constexpr int DD = decltype(d)::value;
-    hipLaunchKernelGGL(tree_attend_kernel<DD>, grid, dim3(512), 0, st, a);
-    if (a.splits > 1) hipLaunchKernelGGL(tree_merge_kernel<DD>, dim3((unsigned)a.total), dim3(256), 0, st, a);
-  };
-  if (D == 64) run(std::integral_constant<int, 64>{});
-  else if (D == 128) run(std::integral_constant<int, 128>{});
-  else run(std::integral_constant<int, 256>{});
+template <int D, int MB>
+static void run_tree(hipStream_t st, const TreeArgsOf<MB> &a, int B) {
+  hipLaunchKernelGGL((tree_attend_kernel<D, MB>), dim3(a.Hkv, a.splits, B * a.blocks), dim3(512), 0, st, a);
+  if (a.splits > 1)
+    hipLaunchKernelGGL(tree_merge_kernel<D>, dim3((unsigned)a.total), dim3(256), 0, st,
+                       TreeMerge{a.part, a.out, a.err, a.splits, a.total});
+}
+
+template <int MB>
+static hipError_t run_tree(hipStream_t st, const TreeArgsOf<MB> &a, int D, int B) {
+  if (D == 64) run_tree<64>(st, a, B);
+  else if (D == 128) run_tree<128>(st, a, B);
+  else run_tree<256>(st, a, B);
   return hipGetLastError();
+}
+
+hipError_t launch_tree(hipStream_t st, const TreeArgs &a, int D, int B) {
+  if (B > 1) return run_tree(st, a, D, B);
+  TreeArgsOf<1> one;  // (a launch's arguments cost the host time)
+  static_cast<TreeBase &>(one) = a;
+  one.seq[0] = a.seq[0];
+  return run_tree(st, one, D, 1);
 }
 
 // The walk along confirmed nodes: every node that holds the token sampled at its
