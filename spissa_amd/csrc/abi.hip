@@ -2759,6 +2759,7 @@ static int run_tree_step(spissa_session *s, const spissa_rope_table *table, cons
     a.splits = p.splits;
     a.tps = p.tps;
     a.blocks = p.blocks;
+    a.kw = p.kw;
     a.total = n * Hq;
     HIP_TRY(launch_tree(s->stream, a, D, B));
   }

@@ -362,7 +362,7 @@ struct TreeBase {
   int *err;
   int Hq, Hkv, R, window;
   float qscale;                  // softmax scale * log2(e)
-  int splits, tps, blocks;       // TreePlan
+  int splits, tps, blocks, kw;   // TreePlan
   int total;                     // N * Hq
 };
 template <int MB>
@@ -377,9 +377,10 @@ struct TreeMerge {
   int splits, total;
 };
 // splits: workgroups of the longest sequence over its key tiles, each with up to tps of
-// them; blocks: of 128 rows (nodes x query heads of a KV head) of the largest tree.
+// them; blocks: of 128 / kw rows (nodes x query heads of a KV head) of the largest
+// tree; kw: waves that share a tile's keys.
 struct TreePlan {
-  int splits = 1, tps = 1, blocks = 1;
+  int splits = 1, tps = 1, blocks = 1, kw = 1;
 };
 TreePlan tree_plan(int D, int R, int Hkv, int window, const int *past, const int *nodes, int B, int cus);
 hipError_t launch_tree(hipStream_t st, const TreeArgs &a, int D, int B);

@@ -19,93 +19,131 @@ namespace {
 
 constexpr int kMaskWords = kTreeMaxNodes / 32;
 
-// The nodes' depths and, with MASKS, the nodes that each sees, by doubling: after k
-// rounds a node knows the 2^k nodes above it. A parent out of its range counts as
-// none. For kTreeMaxNodes threads or more; ends with the shape in LDS, after a barrier.
+// The nodes' depths and the nodes that each sees (with a window those less than it
+// apart), by doubling: after k rounds a node knows the 2^k nodes above it. A parent out
+// of its range counts as none.
 struct TreeShape {
   int depth[kTreeMaxNodes];
   int above[kTreeMaxNodes];  // the node 2^k above
   unsigned mask[kTreeMaxNodes][kMaskWords];
 };
-// p: the thread's node's parent.
-__device__ __forceinline__ void tree_shape(int p, int nodes, int window, bool masks, TreeShape &s, int *err) {
-  const int t = threadIdx.x;
-  const bool mine = t < nodes;
-  if (mine && (p < -1 || p >= t)) {
-    if (err) atomicOr(err, kDevErrTreeParent);
+// What is further than the window above node t is not seen.
+__device__ __forceinline__ void narrow(int t, int window, TreeShape &s) {
+  const int depth = s.depth[t];
+  if (window > 0 && depth >= window)
+    for (int j = 0; j < t; ++j)
+      if (depth - s.depth[j] >= window) s.mask[t][j >> 5] &= ~(1u << (j & 31));
+}
+// Up to 64 nodes: by one wave, without a barrier. p: the lane's node's parent.
+__device__ __forceinline__ void shape_of_wave(int p, int nodes, int window, TreeShape &s, int *err) {
+  const int t = threadIdx.x & 63;
+  if (p < -1 || p >= t) {
+    if (err && t < nodes) atomicOr(err, kDevErrTreeParent);
     p = -1;
   }
   int depth = p >= 0 ? 1 : 0;
-  const int words = (nodes + 31) / 32;
-  if (mine && masks)
-    for (int w = 0; w < words; ++w) s.mask[t][w] = t >> 5 == w ? 1u << (t & 31) : 0u;
+  unsigned lo = t < 32 ? 1u << t : 0u, hi = t < 32 ? 0u : 1u << (t - 32);
+  while (__any(p >= 0)) {
+    const int from = p < 0 ? t : p;
+    const int d = __shfl(depth, from), up = __shfl(p, from);
+    const unsigned l = (unsigned)__shfl((int)lo, from), h = (unsigned)__shfl((int)hi, from);
+    if (p >= 0) {
+      depth += d;
+      lo |= l;
+      hi |= h;
+      p = up;
+    }
+  }
+  s.depth[t] = depth;
+  s.mask[t][0] = lo;
+  s.mask[t][1] = hi;
+  if (window > 0 && t < nodes) {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    narrow(t, window, s);
+  }
+}
+// More nodes: two threads a node, each with half of its words.
+__device__ __forceinline__ void shape_of_workgroup(int p, int nodes, int window, TreeShape &s, int *err) {
+  constexpr int HALF = kMaskWords / 2;
+  const int t = threadIdx.x & (kTreeMaxNodes - 1), w0 = threadIdx.x / kTreeMaxNodes * HALF;
+  if (p < -1 || p >= t) {
+    if (err && t < nodes) atomicOr(err, kDevErrTreeParent);
+    p = -1;
+  }
+  int depth = p >= 0 ? 1 : 0;
+  unsigned m[HALF];
+#pragma unroll
+  for (int w = 0; w < HALF; ++w) m[w] = t >> 5 == w0 + w ? 1u << (t & 31) : 0u;
   for (;;) {
-    if (mine) {
+    if (w0 == 0) {
       s.depth[t] = depth;
       s.above[t] = p;
     }
+#pragma unroll
+    for (int w = 0; w < HALF; ++w) s.mask[t][w0 + w] = m[w];
     if (!__syncthreads_or(p >= 0)) break;
-    int up = -1;
-    unsigned m[kMaskWords];
     if (p >= 0) {
       depth += s.depth[p];
-      up = s.above[p];
-      if (masks) {
 #pragma unroll
-        for (int w = 0; w < kMaskWords; ++w)
-          if (w < words) m[w] = s.mask[t][w] | s.mask[p][w];
-      }
+      for (int w = 0; w < HALF; ++w) m[w] |= s.mask[p][w0 + w];
+      p = s.above[p];
     }
     __syncthreads();
-    if (p >= 0 && masks) {
-#pragma unroll
-      for (int w = 0; w < kMaskWords; ++w)
-        if (w < words) s.mask[t][w] = m[w];
-    }
-    p = up;
   }
-  if (masks && window > 0) {
-    if (mine && depth >= window)
-      for (int j = 0; j < t; ++j)
-        if (depth - s.depth[j] >= window) s.mask[t][j >> 5] &= ~(1u << (j & 31));
+  if (window > 0) {
+    if (w0 == 0 && t < nodes) narrow(t, window, s);
     __syncthreads();
   }
 }
 
+__device__ __forceinline__ unsigned wave_max_bits(unsigned v) {
+  v = max(v, (unsigned)__builtin_amdgcn_update_dpp((int)v, (int)v, 0xB1, 0xf, 0xf, false));
+  v = max(v, (unsigned)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x4E, 0xf, 0xf, false));
+  v = max(v, (unsigned)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x141, 0xf, 0xf, false));
+  v = max(v, (unsigned)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x140, 0xf, 0xf, false));
+  auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = max(r[0], r[1]);
+  r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return max(r[0], r[1]);
+}
 __device__ __forceinline__ float unbits(unsigned b) { return __uint_as_float(b); }
 
 // Channels 4 l..4 l + 3 and their rotation's partners, half a row on, of row `row`.
 template <int D>
-__device__ __forceinline__ void load_pairs(const float *row, int l, float4 &lo, float4 &hi) {
-  lo = *reinterpret_cast<const float4 *>(row + 4 * l);
-  hi = *reinterpret_cast<const float4 *>(row + D / 2 + 4 * l);
+__device__ __forceinline__ void load_pairs(const float *row, int l, f32x4 &lo, f32x4 &hi) {
+  lo = *reinterpret_cast<const f32x4 *>(row + 4 * l);
+  hi = *reinterpret_cast<const f32x4 *>(row + D / 2 + 4 * l);
 }
 // The norm's weights times 1 / rms on such channels.
 template <int D>
-__device__ __forceinline__ void norm_pairs(float4 &lo, float4 &hi, const float *w, int l, float inv) {
+__device__ __forceinline__ void norm_pairs(f32x4 &lo, f32x4 &hi, const float *w, int l, float inv) {
 #pragma clang fp contract(off)
-  float4 a, b;
+  f32x4 a, b;
   load_pairs<D>(w, l, a, b);
-  lo = make_float4(lo.x * inv * a.x, lo.y * inv * a.y, lo.z * inv * a.z, lo.w * inv * a.w);
-  hi = make_float4(hi.x * inv * b.x, hi.y * inv * b.y, hi.z * inv * b.z, hi.w * inv * b.w);
+  lo = lo * inv * a;
+  hi = hi * inv * b;
 }
-__device__ __forceinline__ void rotate_pairs(float4 &lo, float4 &hi, const float *cos, const float *sin, long at) {
-  const float4 c = *reinterpret_cast<const float4 *>(cos + at), s = *reinterpret_cast<const float4 *>(sin + at);
-  rotate_pair(lo.x, hi.x, c.x, s.x);
-  rotate_pair(lo.y, hi.y, c.y, s.y);
-  rotate_pair(lo.z, hi.z, c.z, s.z);
-  rotate_pair(lo.w, hi.w, c.w, s.w);
+__device__ __forceinline__ void rotate_pairs(f32x4 &lo, f32x4 &hi, const float *cos, const float *sin, long at) {
+  const f32x4 c = *reinterpret_cast<const f32x4 *>(cos + at), s = *reinterpret_cast<const f32x4 *>(sin + at);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float x = lo[i], y = hi[i];
+    rotate_pair(x, y, c[i], s[i]);
+    lo[i] = x;
+    hi[i] = y;
+  }
 }
-__device__ __forceinline__ float squares(const float4 &a, const float4 &b) {
+__device__ __forceinline__ float squares(const f32x4 &a, const f32x4 &b) {
 #pragma clang fp contract(off)
-  return ((a.x * a.x + b.x * b.x) + (a.y * a.y + b.y * b.y)) + ((a.z * a.z + b.z * b.z) + (a.w * a.w + b.w * b.w));
+  return ((a[0] * a[0] + b[0] * b[0]) + (a[1] * a[1] + b[1] * b[1])) + ((a[2] * a[2] + b[2] * b[2]) + (a[3] * a[3] + b[3] * b[3]));
 }
 
 }  // namespace
 
-// Eight waves, each with 16 rows of a KV head (a row: a node and one of the head's
-// query heads) and a share of the loads. Keys go by in tiles of 8192 / D: first the
-// cached rows from the first that any node sees, then the nodes' own. A tile comes
+// Eight waves. A row is a node and one of the KV head's query heads; a wave has NB
+// blocks of 16 rows and, of each tile of 8192 / D keys, all (heads of 256) or half
+// (waves 0..3 the first, 4..7 the second; the halves meet at the end). Tiles are first
+// the cached rows from the first that any node sees, then the nodes' own. A tile comes
 // into registers while the one before is computed; waves 0..3 take its values, waves
 // 4..7 its keys, and write them to LDS once for all rows as two binary16 pieces, in
 // the order in which lanes take the operands. S^T = K Q^T, so a lane has one row
@@ -121,12 +159,15 @@ __device__ __forceinline__ float squares(const float4 &a, const float4 &b) {
 // far following, or, where a number is not finite, with zeros in its place and its key
 // noted: rows that see such a key become NaN.
 //
-// Grid: (KV heads, splits, sequences x blocks of 128 rows).
-template <int D, int MB>
+// Grid: (KV heads, splits, sequences x blocks of rows).
+template <int D, int KW, int MB>
 __global__ __launch_bounds__(512, 2) void tree_attend_kernel(const TreeArgsOf<MB> a) {
   constexpr int BN = 8192 / D, G = D / 32, DT = D / 16, VB = BN / 32, KB = BN / 16, TR = D / 8;
-  __shared__ __attribute__((aligned(16))) half8 kp_lds[2][2][KB * G * 64];
-  __shared__ __attribute__((aligned(16))) half8 vp_lds[2][2][VB * DT * 64];
+  constexpr int NB = 1, RW = 8 / KW, ROWS = RW * NB * 16;
+  constexpr int KBW = KB / KW, VBW = VB / KW;  // a wave's 16 and 32 keys of a tile
+  static_assert(KB * G == 16 && VB * DT == 16, "a tile has 8192 keys' and as many values' channels");
+  __shared__ __attribute__((aligned(16))) half8 pieces_lds[2][2][2][1024];  // values, buffer, piece
+  half8 (*const kp_lds)[2][1024] = pieces_lds[0], (*const vp_lds)[2][1024] = pieces_lds[1];
   __shared__ TreeShape shape;
   __shared__ unsigned most_lds[2][8];
   __shared__ unsigned bad_lds[VB];
@@ -134,27 +175,39 @@ __global__ __launch_bounds__(512, 2) void tree_attend_kernel(const TreeArgsOf<MB
   float minus_one = -1.0f;
   asm volatile("" : "+s"(minus_one));
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int col = lane & 15, kq = lane >> 4;
+  int col = lane & 15, kq = lane >> 4;
+  const int rw = wave % RW, kw = wave / RW;
   const int h = blockIdx.x, split = blockIdx.y, b = blockIdx.z / a.blocks, block = blockIdx.z - b * a.blocks;
   const int past = a.seq[b].past, nodes = a.seq[b].nodes, seq_first = a.seq[b].first;
-  const int rows = nodes * a.R, row0 = block * 128 + wave * 16;
-  if (block * 128 >= rows) return;
+  const int rows = nodes * a.R;
+  if (block * ROWS >= rows) return;
   const int lo = a.window > 0 ? max(0, past + 1 - a.window) : 0;
   const int cached = (past - lo + BN - 1) / BN, tiles = cached + (nodes + BN - 1) / BN;
   const int t0 = split * a.tps, t1 = min(tiles, t0 + a.tps);
 
-  const int r = min(row0 + col, rows - 1), node = r / a.R, hq = h * a.R + (r - node * a.R);
-  const bool live = row0 + col < rows;
-  const long orow = (long)(seq_first + node) * a.Hq + hq;
-  float *const part = a.part + ((long)split * a.total + orow) * (D + 4);
+  // Rows of the wave: blocks rw, rw + RW, ... of 16.
+  int node[NB];
+  long orow[NB];
+  bool live[NB];
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
+    const int row = block * ROWS + (n * RW + rw) * 16 + col, r = min(row, rows - 1);
+    live[n] = row < rows;
+    node[n] = r / a.R;
+    orow[n] = (long)(seq_first + node[n]) * a.Hq + h * a.R + (r - node[n] * a.R);
+  }
+  auto busy = [&](int n) __attribute__((always_inline)) { return block * ROWS + (n * RW + rw) * 16 < rows; };
+  auto part = [&](int n) __attribute__((always_inline)) { return a.part + ((long)split * a.total + orow[n]) * (D + 4); };
   if (t0 >= t1) {  // (no keys: nothing of the row's part is read)
-    if (live && kq == 0) *reinterpret_cast<float2 *>(part + D) = make_float2(NEG_INF, 0.0f);
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+      if (live[n] && kq == 0 && kw == 0) *reinterpret_cast<float2 *>(part(n) + D) = make_float2(NEG_INF, 0.0f);
     return;
   }
 
   // A thread's share of a tile: of values eight keys (4 q + 0..3 and 16 + 4 q + 0..3 of
   // 32) of four channels; of keys, four rows' channels 4 l.. and D / 2 + 4 l... Load i
-  // has the key thread_key + step_key(i).
+  // has the key thread_key + step_key(i, values).
   const bool values = wave < 4;
   const int part_of = tid & 255;
   const int vg = part_of / (D / 4);
@@ -164,11 +217,9 @@ __global__ __launch_bounds__(512, 2) void tree_attend_kernel(const TreeArgsOf<MB
   const long stride = (long)a.Hkv * D;
   float *const cache_rows = (values ? +a.seq[b].v : +a.seq[b].k) + h * D;
   const float *const own_rows = (values ? +a.v : +a.k) + seq_first * stride + h * D;
-  bf16 *const kb = a.seq[b].kb, *const vt = a.seq[b].vt;
-  const long cap = a.seq[b].cap;
-  float4 raw[8];
-  auto step_key = [&](int i) __attribute__((always_inline)) { return values ? (i & 3) + 16 * (i >> 2) : (i >> 1) * (256 / TR); };
-  auto load = [&](int tile) __attribute__((always_inline)) {
+  f32x4 raw[8];
+  auto step_key = [&](int i, auto values) __attribute__((always_inline)) { return values ? (i & 3) + 16 * (i >> 2) : (i >> 1) * (256 / TR); };
+  auto load = [&](int tile, auto values) __attribute__((always_inline)) {
     const bool own = tile >= cached;
     const int first = own ? (tile - cached) * BN : lo + tile * BN, left = (own ? nodes : past) - first;
     const char *const src = reinterpret_cast<const char *>((own ? own_rows : +cache_rows) + first * stride);
@@ -176,59 +227,50 @@ __global__ __launch_bounds__(512, 2) void tree_attend_kernel(const TreeArgsOf<MB
       const unsigned off = (unsigned)(thread_key * stride + thread_channel) * 4u;
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        raw[i] = *reinterpret_cast<const float4 *>(src + (step_key(i) * stride + (values ? 0 : (i & 1) * (D / 2))) * 4 + off);
+        raw[i] = *reinterpret_cast<const f32x4 *>(src + (step_key(i, values) * stride + (values ? 0 : (i & 1) * (D / 2))) * 4 + off);
     } else {  // (rows past the last: that one again)
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const long at = min(thread_key + step_key(i), left - 1) * stride + thread_channel + (values ? 0 : (i & 1) * (D / 2));
-        raw[i] = *reinterpret_cast<const float4 *>(src + at * 4);
+        const long at = min(thread_key + step_key(i, values), left - 1) * stride + thread_channel + (values ? 0 : (i & 1) * (D / 2));
+        raw[i] = *reinterpret_cast<const f32x4 *>(src + at * 4);
       }
     }
   };
   // The nodes' own rows: the norm and the rotation of keys, and the append.
-  auto finish = [&](int tile) __attribute__((always_inline)) {
+  auto finish = [&](int tile, auto values, f32x4 (&cur)[8]) __attribute__((always_inline)) {
     const int first = (tile - cached) * BN + thread_key;
     if (!values) {
 #pragma unroll
       for (int i = 0; i < 8; i += 2) {
-        const int t = min(first + step_key(i), nodes - 1);
+        const int t = min(first + step_key(i, values), nodes - 1);
         if (a.k_norm) {
-          const float inv = 1.0f / sqrtf(group_sum<TR>(squares(raw[i], raw[i + 1])) / (float)D + a.eps);
-          norm_pairs<D>(raw[i], raw[i + 1], a.k_norm, kl, inv);
+          const float inv = 1.0f / sqrtf(group_sum<TR>(squares(cur[i], cur[i + 1])) / (float)D + a.eps);
+          norm_pairs<D>(cur[i], cur[i + 1], a.k_norm, kl, inv);
         }
-        if (a.cos) rotate_pairs(raw[i], raw[i + 1], a.cos, a.sin, (long)(past + shape.depth[t]) * (D / 2) + 4 * kl);
+        if (a.cos) rotate_pairs(cur[i], cur[i + 1], a.cos, a.sin, (long)(past + shape.depth[t]) * (D / 2) + 4 * kl);
       }
     }
     if (block != 0) return;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int t = first + step_key(i);
-      if (t >= nodes) continue;
-      const long at = past + t;
-      const int c = thread_channel + (values ? 0 : (i & 1) * (D / 2));
-      *reinterpret_cast<float4 *>(cache_rows + at * stride + c) = raw[i];
-      if (!kb) continue;
-      const float x[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-      bf16 *const dst = values ? vt + ((long)h * D + c) * cap + vt_key_slot(at) : kb + ((long)h * cap + at) * D + c;
-      const long step = values ? cap : 1;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) dst[j * step] = (bf16)x[j];
+      const int t = first + step_key(i, values);
+      if (t < nodes)
+        *reinterpret_cast<f32x4 *>(cache_rows + (past + t) * stride + thread_channel + (values ? 0 : (i & 1) * (D / 2))) = cur[i];
     }
   };
   // The wave's largest magnitude, as bits (a NaN or an infinity is above the rest).
-  auto post = [&](int slot) __attribute__((always_inline)) {
+  auto post = [&](int slot, const f32x4 (&cur)[8]) __attribute__((always_inline)) {
     unsigned m = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      m = max(m, max(__float_as_uint(raw[i].x) & 0x7fffffffu, __float_as_uint(raw[i].y) & 0x7fffffffu));
-      m = max(m, max(__float_as_uint(raw[i].z) & 0x7fffffffu, __float_as_uint(raw[i].w) & 0x7fffffffu));
+      m = max(m, max(__float_as_uint(cur[i][0]) & 0x7fffffffu, __float_as_uint(cur[i][1]) & 0x7fffffffu));
+      m = max(m, max(__float_as_uint(cur[i][2]) & 0x7fffffffu, __float_as_uint(cur[i][3]) & 0x7fffffffu));
     }
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) m = max(m, (unsigned)__shfl_xor((int)m, d));
+    m = wave_max_bits(m);
     if (lane == 0) most_lds[slot][wave] = m;
   };
   unsigned kbits = 127u << 23, vbits = 127u << 23;  // the scales, as float bits
-  auto write = [&](int buf) __attribute__((always_inline)) {
+  auto write = [&](int buf, auto values, const f32x4 (&cur)[8]) __attribute__((always_inline)) {
     const float scale = unbits(values ? vbits : kbits);
     if (values) {
       const int dt = vl >> 2;
@@ -236,7 +278,7 @@ __global__ __launch_bounds__(512, 2) void tree_attend_kernel(const TreeArgsOf<MB
       for (int c = 0; c < 4; ++c) {
         float v[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = (c == 0 ? raw[i].x : c == 1 ? raw[i].y : c == 2 ? raw[i].z : raw[i].w) * scale;
+        for (int i = 0; i < 8; ++i) v[i] = cur[i][c] * scale;
         half8 ph, pl;
         split8(v, minus_one, &ph, &pl);
         // (the low bits mixed: the writes of a wave fall on all banks)
@@ -247,253 +289,346 @@ __global__ __launch_bounds__(512, 2) void tree_attend_kernel(const TreeArgsOf<MB
     } else {
 #pragma unroll
       for (int i = 0; i < 8; i += 2) {
-        const float v[8] = {raw[i].x * scale,     raw[i].y * scale,     raw[i].z * scale,     raw[i].w * scale,
-                            raw[i + 1].x * scale, raw[i + 1].y * scale, raw[i + 1].z * scale, raw[i + 1].w * scale};
+        const float v[8] = {cur[i][0] * scale,     cur[i][1] * scale,     cur[i][2] * scale,     cur[i][3] * scale,
+                            cur[i + 1][0] * scale, cur[i + 1][1] * scale, cur[i + 1][2] * scale, cur[i + 1][3] * scale};
         half8 ph, pl;
         split8(v, minus_one, &ph, &pl);
-        const int key = thread_key + step_key(i), at = ((key >> 4) * G + (kl >> 2)) * 64 + (kl & 3) * 16 + ((key ^ kl) & 15);
+        const int key = thread_key + step_key(i, values), at = ((key >> 4) * G + (kl >> 2)) * 64 + (kl & 3) * 16 + ((key ^ kl) & 15);
         kp_lds[buf][0][at] = ph;
         kp_lds[buf][1][at] = pl;
       }
     }
   };
   auto largest = [&](int slot, int from) __attribute__((always_inline)) {
-    const unsigned *m = most_lds[slot] + from;
-    return max(max(m[0], m[1]), max(m[2], m[3]));
+    const uint4 m = *reinterpret_cast<const uint4 *>(most_lds[slot] + from);
+    return max(max(m.x, m.y), max(m.z, m.w));
   };
 
-  // (all that needs no other load first: the parents, the queries, the first tiles)
-  const int parent = tid < nodes ? a.parents[seq_first + tid] : -1;
-  float4 x[G], y[G];
-#pragma unroll
-  for (int g = 0; g < G; ++g) load_pairs<D>(a.q + orow * D, 4 * g + kq, x[g], y[g]);
-  load(t0);
-  tree_shape(parent, nodes, a.window, t1 > cached, shape, block == 0 && split == 0 && h == 0 ? a.err : nullptr);
-
-  // The queries of the wave's rows, as the B operand.
-  half8 qh[G], ql[G];
-  float inv_q;
-  const int pos = past + shape.depth[node], row_lo = a.window > 0 ? max(0, pos + 1 - a.window) : 0;
+  // (all that needs no other load first: the parents, the queries, the first tile)
+  const int own_node = tid & (nodes > 64 ? kTreeMaxNodes - 1 : 63), parent = own_node < nodes ? a.parents[seq_first + own_node] : -1;
+  half8 qh[NB][G], ql[NB][G];
+  float inv_q[NB];
+  int row_lo[NB], wave_lo = 0;  // keys from row_lo on are seen by the row, from wave_lo on by all rows of the wave
   {
-    float most = 0.0f;
-    if (a.q_norm) {
-      float sum = 0.0f;
+    f32x4 x[NB][G], y[NB][G];
 #pragma unroll
-      for (int g = 0; g < G; ++g) sum += squares(x[g], y[g]);
-      const float inv = 1.0f / sqrtf(sum32(sum16(sum)) / (float)D + a.eps);
+    for (int n = 0; n < NB; ++n)
+      if (busy(n)) {
 #pragma unroll
-      for (int g = 0; g < G; ++g) norm_pairs<D>(x[g], y[g], a.q_norm, 4 * g + kq, inv);
+        for (int g = 0; g < G; ++g) load_pairs<D>(a.q + orow[n] * D, 4 * g + kq, x[n][g], y[n][g]);
+      }
+    load(t0, values);
+    int *const err = block == 0 && split == 0 && h == 0 ? a.err : nullptr;
+    if (nodes > 64) {
+      shape_of_workgroup(parent, nodes, a.window, shape, err);
+    } else {
+      // (a wave that is the last to have rows)
+      if (wave == 7) shape_of_wave(parent, nodes, a.window, shape, err);
+      __syncthreads();
     }
-    if (a.cos) {
+    // The queries, as the B operand.
 #pragma unroll
-      for (int g = 0; g < G; ++g) rotate_pairs(x[g], y[g], a.cos, a.sin, (long)pos * (D / 2) + 4 * (4 * g + kq));
-    }
+    for (int n = 0; n < NB; ++n) {
+      if (!busy(n)) continue;
+      const int pos = past + shape.depth[node[n]];
+      row_lo[n] = a.window > 0 ? max(0, pos + 1 - a.window) : 0;
+      int most_lo = row_lo[n];
 #pragma unroll
-    for (int g = 0; g < G; ++g) {
-      float *const v[8] = {&x[g].x, &x[g].y, &x[g].z, &x[g].w, &y[g].x, &y[g].y, &y[g].z, &y[g].w};
+      for (int d = 8; d > 0; d >>= 1) most_lo = max(most_lo, __shfl_xor(most_lo, d));
+      wave_lo = max(wave_lo, most_lo);
+      float most = 0.0f;
+      if (a.q_norm) {
+        float sum = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        *v[i] = *v[i] * a.prescale * a.qscale;
-        const float m = fabsf(*v[i]);
-        most = fmaxf(most, m <= 3.402823466e38f ? m : 0.0f);
+        for (int g = 0; g < G; ++g) sum += squares(x[n][g], y[n][g]);
+        const float inv = 1.0f / sqrtf(sum32(sum16(sum)) / (float)D + a.eps);
+#pragma unroll
+        for (int g = 0; g < G; ++g) norm_pairs<D>(x[n][g], y[n][g], a.q_norm, 4 * g + kq, inv);
+      }
+      if (a.cos) {
+#pragma unroll
+        for (int g = 0; g < G; ++g) rotate_pairs(x[n][g], y[n][g], a.cos, a.sin, (long)pos * (D / 2) + 4 * (4 * g + kq));
+      }
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+                x[n][g] = x[n][g] * a.prescale * a.qscale;
+        y[n][g] = y[n][g] * a.prescale * a.qscale;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float u = fabsf(x[n][g][i]), w = fabsf(y[n][g][i]);
+          most = fmaxf(most, fmaxf(u <= 3.402823466e38f ? u : 0.0f, w <= 3.402823466e38f ? w : 0.0f));
+        }
+      }
+      const unsigned bits = scale_to(max32(max16(most)), 9);
+      const float scale = unbits(bits);
+      inv_q[n] = inverse_scale(bits);
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        const float v[8] = {x[n][g][0] * scale, x[n][g][1] * scale, x[n][g][2] * scale, x[n][g][3] * scale,
+                            y[n][g][0] * scale, y[n][g][1] * scale, y[n][g][2] * scale, y[n][g][3] * scale};
+        split8(v, minus_one, &qh[n][g], &ql[n][g]);
       }
     }
-    const unsigned bits = scale_to(max32(max16(most)), 9);
-    const float scale = unbits(bits);
-    inv_q = inverse_scale(bits);
-#pragma unroll
-    for (int g = 0; g < G; ++g) {
-      const float v[8] = {x[g].x * scale, x[g].y * scale, x[g].z * scale, x[g].w * scale,
-                          y[g].x * scale, y[g].y * scale, y[g].z * scale, y[g].w * scale};
-      split8(v, minus_one, &qh[g], &ql[g]);
-    }
   }
-  int wave_lo = row_lo;  // keys from here on are seen by all rows of the wave
-#pragma unroll
-  for (int d = 8; d > 0; d >>= 1) wave_lo = max(wave_lo, __shfl_xor(wave_lo, d));
 
-  f32x4 o[DT];
+  f32x4 o[NB][DT];
+  float m[NB], l[NB];  // m: the largest score so far, or up to 7 below it
+  bool poison[NB];
 #pragma unroll
-  for (int d = 0; d < DT; ++d) o[d] = (f32x4){0.f, 0.f, 0.f, 0.f};
-  float m = NEG_INF, l = 0.0f;  // m: the largest score so far, or up to 7 below it
-  bool poison = false;
+  for (int n = 0; n < NB; ++n) {
+    m[n] = NEG_INF;
+    l[n] = 0.0f;
+    poison[n] = false;
+#pragma unroll
+    for (int d = 0; d < DT; ++d) o[n][d] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  }
 
   auto compute = [&](int tile, bool bad) __attribute__((always_inline)) {
     const int buf = tile & 1;
     const bool own = tile >= cached;
     const int base = lo + tile * BN;
-    f32x4 sc[KB];
+    f32x4 sc[NB][KBW];
 #pragma unroll
-    for (int k = 0; k < KB; ++k) sc[k] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int k = 0; k < KBW; ++k) sc[n][k] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int g = 0; g < G; ++g) {
-      const int at = g * 64 + kq * 16 + ((col ^ (4 * g + kq)) & 15);
-      half8 fh[KB], fl[KB];
+      const int at = (kw * KBW * G + g) * 64 + kq * 16 + ((col ^ (4 * g + kq)) & 15);
+      half8 fh[KBW], fl[KBW];
 #pragma unroll
-      for (int k = 0; k < KB; ++k) {
+      for (int k = 0; k < KBW; ++k) {
         fh[k] = kp_lds[buf][0][k * G * 64 + at];
         fl[k] = kp_lds[buf][1][k * G * 64 + at];
       }
 #pragma unroll
-      for (int k = 0; k < KB; ++k) sc[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fh[k], qh[g], sc[k], 0, 0, 0);
+      for (int n = 0; n < NB; ++n)
 #pragma unroll
-      for (int k = 0; k < KB; ++k) sc[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fh[k], ql[g], sc[k], 0, 0, 0);
+        for (int k = 0; k < KBW; ++k) sc[n][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fh[k], qh[n][g], sc[n][k], 0, 0, 0);
 #pragma unroll
-      for (int k = 0; k < KB; ++k) sc[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fl[k], qh[g], sc[k], 0, 0, 0);
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int k = 0; k < KBW; ++k) sc[n][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fh[k], ql[n][g], sc[n][k], 0, 0, 0);
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int k = 0; k < KBW; ++k) sc[n][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fl[k], qh[n][g], sc[n][k], 0, 0, 0);
     }
-    // (finite and above 0: hidden scores stay -inf)
-    const float f = fminf(fmaxf(inv_q * inverse_scale(kbits), 1.1754944e-38f), 3.402823466e38f);
-    // (scores of hidden keys at -inf)
-    if (own || bad || base + BN > past || base < wave_lo) {
+    const bool hidden = own || bad || base + BN > past || base < wave_lo;
+    half8 ph[NB][VBW], pl[NB][VBW];
 #pragma unroll
-      for (int v = 0; v < VB; ++v) {
-        unsigned seen;
-        if (own) {
-          const int w = (tile - cached) * VB + v;
-          seen = w < kMaskWords && w * 32 < nodes ? shape.mask[node][w] : 0u;
-        } else {
-          const int from = max(0, row_lo - base - 32 * v), to = min(32, past - base - 32 * v);
-          seen = from >= 32 || to <= from ? 0u : (0xffffffffu << from) & (0xffffffffu >> (32 - to));
+    for (int n = 0; n < NB; ++n) {
+      // (finite and above 0: hidden scores stay -inf)
+      const float f = fminf(fmaxf(inv_q[n] * inverse_scale(kbits), 1.1754944e-38f), 3.402823466e38f);
+      if (hidden) {
+#pragma unroll
+        for (int v = 0; v < VBW; ++v) {
+          const int first = 32 * (kw * VBW + v);  // of the tile
+          unsigned seen;
+          if (own) {
+            const int w = ((tile - cached) * BN + first) / 32;
+            seen = w < kMaskWords && w * 32 < nodes ? shape.mask[node[n]][w] : 0u;
+          } else {
+            const int from = max(0, row_lo[n] - base - first), to = min(32, past - base - first);
+            seen = from >= 32 || to <= from ? 0u : (0xffffffffu << from) & (0xffffffffu >> (32 - to));
+          }
+          if (bad) poison[n] |= (seen & bad_lds[kw * VBW + v]) != 0;
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (!(seen >> ((i & 3) + 4 * kq + 16 * (i >> 2)) & 1u)) sc[n][2 * v + (i >> 2)][i & 3] = NEG_INF;
         }
-        if (bad) poison |= (seen & bad_lds[v]) != 0;
+      }
+      float big = NEG_INF;
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (!(seen >> ((i & 3) + 4 * kq + 16 * (i >> 2)) & 1u)) sc[2 * v + (i >> 2)][i & 3] = NEG_INF;
+      for (int k = 0; k < KBW; ++k) big = fmaxf(big, fmaxf(fmaxf(sc[n][k][0], sc[n][k][1]), fmaxf(sc[n][k][2], sc[n][k][3])));
+      big = max32(max16(big)) * f;
+      if (__any(big > m[n] + 7.0f)) {
+        const float next = big > m[n] + 7.0f ? big : m[n], keep = fast_exp2(m[n] - safe_max(next));
+        m[n] = next;
+        l[n] *= keep;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[n][d] *= keep;
+      }
+      const float off = 8.0f - safe_max(m[n]);  // weights times 2^8, up to 2^15
+#pragma unroll
+      for (int v = 0; v < VBW; ++v) {
+        float p[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          p[i] = fast_exp2(fmaf(sc[n][2 * v + (i >> 2)][i & 3], f, off));
+          l[n] += p[i];
+        }
+        split8(p, minus_one, &ph[n][v], &pl[n][v]);
       }
     }
-    float big = NEG_INF;
 #pragma unroll
-    for (int k = 0; k < KB; ++k) big = fmaxf(big, fmaxf(fmaxf(sc[k][0], sc[k][1]), fmaxf(sc[k][2], sc[k][3])));
-    big = max32(max16(big)) * f;
-    if (__any(big > m + 7.0f)) {
-      const float next = big > m + 7.0f ? big : m, keep = fast_exp2(m - safe_max(next));
-      m = next;
-      l *= keep;
-#pragma unroll
-      for (int d = 0; d < DT; ++d) o[d] *= keep;
-    }
-    const float off = 8.0f - safe_max(m);  // weights times 2^8, up to 2^15
-    half8 ph[VB], pl[VB];
-#pragma unroll
-    for (int v = 0; v < VB; ++v) {
-      float p[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        p[i] = fast_exp2(fmaf(sc[2 * v + (i >> 2)][i & 3], f, off));
-        l += p[i];
-      }
-      split8(p, minus_one, &ph[v], &pl[v]);
-    }
-#pragma unroll
-    for (int v = 0; v < VB; ++v)
+    for (int v = 0; v < VBW; ++v)
 #pragma unroll
       for (int d = 0; d < DT; d += 4) {
         half8 fh[4], fl[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const int at = (v * DT + d + j) * 64 + kq * 16 + (col ^ j);
+          const int at = ((kw * VBW + v) * DT + d + j) * 64 + kq * 16 + (col ^ j);
           fh[j] = vp_lds[buf][0][at];
           fl[j] = vp_lds[buf][1][at];
         }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) o[d + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fh[j], ph[v], o[d + j], 0, 0, 0);
+        for (int n = 0; n < NB; ++n) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) o[d + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fh[j], pl[v], o[d + j], 0, 0, 0);
+          for (int j = 0; j < 4; ++j) o[n][d + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fh[j], ph[n][v], o[n][d + j], 0, 0, 0);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) o[d + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fl[j], ph[v], o[d + j], 0, 0, 0);
+          for (int j = 0; j < 4; ++j) o[n][d + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fh[j], pl[n][v], o[n][d + j], 0, 0, 0);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[n][d + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fl[j], ph[n][v], o[n][d + j], 0, 0, 0);
+        }
       }
   };
 
   constexpr unsigned kInfinite = 0x7f800000u;
   constexpr unsigned kTop = (127u + 15u) << 23;  // 2^15
-  // The first tile in LDS, with the scales that it sets.
-  if (t0 >= cached) finish(t0);
-  post(t0 & 1);
-  __syncthreads();
-  kbits = scale_to(unbits(min(largest(t0 & 1, 4), kInfinite - 1)), 11);
-  vbits = scale_to(unbits(min(largest(t0 & 1, 0), kInfinite - 1)), 11);
-  write(t0 & 1);
-  if (t0 + 1 < t1) load(t0 + 1);
-  __syncthreads();
-
-  // Between two barriers a wave computes its rows' part of a tile and writes its share
-  // of the next one, the first four waves in the other order: a SIMD has one of each.
-  // A tile that has to be written again takes a turn of its own, one in which something
-  // is not finite two, as the largest of the rest is not known before it is written.
-  bool bad = false, rescale = false;
+  // Between two barriers a wave computes its part of a tile and writes its share of the
+  // next one, the first four waves in the other order: a SIMD has one of each. A tile
+  // that has to be written again takes a turn of its own, one in which something is not
+  // finite two, as the largest of the rest is not known before it is written. In the
+  // first turn there is nothing to compute, and the scales are set between reading the
+  // tile's largest and writing it. (Two loops, one for either kind of wave: in one the
+  // registers of a tile on its way would be copied, that is waited for.)
+  auto turns = [&](auto values) __attribute__((always_inline)) {
+    constexpr bool V = decltype(values)::value;
+    bool bad = false, rescale = false;
 #pragma unroll 1
-  for (int tile = t0; tile < t1;) {
-    // (addresses anew each turn: kept, they would not leave room for the rest)
-    asm volatile("" : "+v"(thread_key), "+v"(thread_channel), "+v"(kl), "+v"(vl), "+v"(vb0), "+v"(vq));
-    const unsigned km = largest(tile & 1, 4), vm = largest(tile & 1, 0);
-    const bool more = km >= kInfinite || vm >= kInfinite;
-    // (the largest times the scale, by exponents: bits of both less the bias)
-    const bool again = more || rescale || km > kTop - kbits + (127u << 23) || vm > kTop - vbits + (127u << 23);
-    const int target = again ? tile : tile + 1;
-    if (again) {
-      load(tile);
-      if (more) {
-        bad = rescale = true;
-        if (tid < VB) bad_lds[tid] = 0;
-      } else {
-        rescale = false;
-        kbits = scale_to(unbits(km), 11);
-        unsigned now = scale_to(unbits(vm), 11);
-        if (tile > t0) now = min(now, vbits);  // (the output so far only ever gets smaller)
-        const float keep = unbits(now) * inverse_scale(vbits);
-        vbits = now;
+    for (int tile = t0 - 1; tile < t1;) {
+      // (addresses anew each time: kept, they would not leave room for the rest)
+      asm volatile("" : "+v"(thread_key), "+v"(thread_channel), "+v"(kl), "+v"(vl), "+v"(vb0), "+v"(vq), "+v"(col), "+v"(kq));
+      bool again = false;
+      if (tile >= t0) {
+        const unsigned km = largest(tile & 1, 4), vm = largest(tile & 1, 0);
+        const bool more = km >= kInfinite || vm >= kInfinite;
+        // (the largest times the scale, by exponents: bits of both less the bias)
+        again = more || rescale || km > kTop - kbits + (127u << 23) || vm > kTop - vbits + (127u << 23);
+        if (again) {
+          load(tile, values);
+          if (more) {
+            bad = rescale = true;
+            if (tid < VB) bad_lds[tid] = 0;
+          } else {
+            rescale = false;
+            kbits = scale_to(unbits(km), 11);
+            unsigned now = scale_to(unbits(vm), 11);
+            if (tile > t0) now = min(now, vbits);  // (the output so far only ever gets smaller)
+            const float keep = unbits(now) * inverse_scale(vbits);
+            vbits = now;
 #pragma unroll
-        for (int d = 0; d < DT; ++d) o[d] *= keep;
-      }
-      __syncthreads();  // (the tile's largest is read, its bad keys cleared)
-    }
-    auto stage = [&]() __attribute__((always_inline)) {
-      if (target >= t1) return;
-      if (target >= cached) finish(target);
-      if (again && bad) {
+            for (int n = 0; n < NB; ++n)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          float v[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-          bool wrong = false;
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (!(fabsf(v[j]) < __builtin_inff())) {
-              v[j] = 0.0f;
-              wrong = true;
-            }
-          raw[i] = make_float4(v[0], v[1], v[2], v[3]);
-          const int key = thread_key + step_key(i);
-          if (wrong) atomicOr(&bad_lds[key >> 5], 1u << (key & 31));
+              for (int d = 0; d < DT; ++d) o[n][d] *= keep;
+          }
+          __syncthreads();  // (the tile's largest is read, its bad keys cleared)
         }
       }
-      post(target & 1);
-      write(target & 1);
-      if (target + 1 < t1) load(target + 1);
-    };
-    if (values) stage();
-    if (!again && row0 < rows) compute(tile, bad);
-    if (!values) stage();
-    if (!again) {
-      bad = false;
-      ++tile;
-    }
-    __syncthreads();
-  }
-
-  if (row0 >= rows) return;
-  l = sum32(sum16(l));
-  if (poison) l = __builtin_nanf("");
-  const float inv = l == 0.0f ? 0.0f : inverse_scale(vbits) / l;
-  float *const out = a.splits > 1 ? part : a.out + orow * D;
-  if (live) {
+      const int target = again ? tile : tile + 1;
+      const bool computes = tile >= t0 && !again && busy(0);
+      if (!V && computes) compute(tile, bad);
+      if (target < t1) {
+        f32x4 cur[8];
 #pragma unroll
-    for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4 *>(out + 16 * d + 4 * kq) = o[d] * inv;
-    if (a.splits > 1) {
-      if (kq == 0) *reinterpret_cast<float2 *>(part + D) = make_float2(m, l);
-    } else if (!(l > 0.0f) || l > 3.402823466e38f) {
-      atomicOr(a.err, kDevErrSoftmaxDenominator);
+        for (int i = 0; i < 8; ++i) cur[i] = raw[i];
+        if (target >= cached) finish(target, values, cur);
+        if (again && bad) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            bool wrong = false;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const bool fine = fabsf(cur[i][j]) < __builtin_inff();
+              cur[i][j] = fine ? cur[i][j] : 0.0f;
+              wrong |= !fine;
+            }
+            const int key = thread_key + step_key(i, values);
+            if (wrong) atomicOr(&bad_lds[key >> 5], 1u << (key & 31));
+          }
+        }
+        post(target & 1, cur);
+        if (tile < t0) {
+          __syncthreads();
+          kbits = scale_to(unbits(min(largest(t0 & 1, 4), kInfinite - 1)), 11);
+          vbits = scale_to(unbits(min(largest(t0 & 1, 0), kInfinite - 1)), 11);
+        }
+        write(target & 1, values, cur);
+      }
+      if (target + 1 < t1) {
+        load(target + 1, values);
+      } else {  // (what the registers hold is of no use: nothing to keep across the turn)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) asm volatile("" : "=v"(raw[i]));
+      }
+      if (V && computes) compute(tile, bad);
+      if (!again) {
+        bad = false;
+        ++tile;
+      }
+      __syncthreads();
+    }
+  };
+  if (values) turns(std::true_type{});
+  else turns(std::false_type{});
+
+  // The halves meet: waves 4..7 leave theirs in LDS.
+  constexpr int PER = 16 * D + 32;  // floats a block of rows: outputs, scores and sums
+  static_assert(KW == 1 || 4 * NB * PER * 4 <= (int)sizeof pieces_lds, "the halves' room");
+  float *const room = reinterpret_cast<float *>(pieces_lds);
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
+    if (!busy(n)) continue;
+    l[n] = sum32(sum16(l[n]));
+    if (poison[n]) l[n] = __builtin_nanf("");
+    if (KW == 2 && kw == 1) {
+      float *const mine = room + (rw * NB + n) * PER;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4 *>(mine + d * 256 + lane * 4) = o[n][d];
+      if (kq == 0) *reinterpret_cast<float2 *>(mine + 16 * D + 2 * col) = make_float2(m[n], l[n]);
     }
   }
+  if (KW == 2) {
+    __syncthreads();
+    if (kw == 1) return;
+  }
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
+    if (!busy(n)) continue;
+    if (KW == 2) {
+      const float *const other = room + (rw * NB + n) * PER;
+      const float2 ml = *reinterpret_cast<const float2 *>(other + 16 * D + 2 * col);
+      const float big = fmaxf(m[n], ml.x), mine = fast_exp2(m[n] - safe_max(big)), theirs = fast_exp2(ml.x - safe_max(big));
+      m[n] = big;
+      l[n] = l[n] * mine + ml.y * theirs;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) o[n][d] = o[n][d] * mine + *reinterpret_cast<const f32x4 *>(other + d * 256 + lane * 4) * theirs;
+    }
+    const float inv = l[n] == 0.0f ? 0.0f : inverse_scale(vbits) / l[n];
+    float *const out = a.splits > 1 ? part(n) : a.out + orow[n] * D;
+    if (live[n]) {
+#pragma unroll
+      for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4 *>(out + 16 * d + 4 * kq) = o[n][d] * inv;
+      if (a.splits > 1) {
+        if (kq == 0) *reinterpret_cast<float2 *>(out + D) = make_float2(m[n], l[n]);
+      } else if (!(l[n] > 0.0f) || l[n] > 3.402823466e38f) {
+        atomicOr(a.err, kDevErrSoftmaxDenominator);
+      }
+    }
+  }
+}
+
+// The bf16 prefill operands of the nodes' rows, from the cache's.
+// Grid: (blocks over nodes * D, KV heads, sequences), 256 threads.
+template <int MB>
+__global__ __launch_bounds__(256) void tree_operands_kernel(const TreeArgsOf<MB> a, int D) {
+  const int b = blockIdx.z, h = blockIdx.y, at = blockIdx.x * 256 + threadIdx.x, t = at / D, c = at - t * D;
+  bf16 *const kb = a.seq[b].kb, *const vt = a.seq[b].vt;
+  if (!kb || t >= a.seq[b].nodes) return;
+  const long row = a.seq[b].past + t, cap = a.seq[b].cap, from = (row * a.Hkv + h) * D + c;
+  kb[((long)h * cap + row) * D + c] = (bf16)a.seq[b].k[from];
+  vt[((long)h * D + c) * cap + vt_key_slot(row)] = (bf16)a.seq[b].v[from];
 }
 
 // The splits' outputs, each divided by its own sum, by their sums' shares. D / 4
@@ -559,7 +694,7 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(const TreeMerge a) {
 // start and its tiles, and the merge, which reads each split's output.
 TreePlan tree_plan(int D, int R, int Hkv, int window, const int *past, const int *nodes, int B, int cus) {
   const int BN = 8192 / D;
-  int tiles[kMaxDecodeBatch], blocks[kMaxDecodeBatch], most = 1;
+  int tiles[kMaxDecodeBatch], blocks[kMaxDecodeBatch], most = 1, most_rows = 1;
   long rows = 0;
   TreePlan p;
   for (int b = 0; b < B; ++b) {
@@ -567,10 +702,15 @@ TreePlan tree_plan(int D, int R, int Hkv, int window, const int *past, const int
     if (!nodes[b]) continue;
     const int lo = window > 0 ? std::max(0, past[b] + 1 - window) : 0;
     tiles[b] = (past[b] - lo + BN - 1) / BN + (nodes[b] + BN - 1) / BN;
-    blocks[b] = (nodes[b] * R + 127) / 128;
+    most_rows = std::max(most_rows, nodes[b] * R);
     most = std::max(most, tiles[b]);
-    p.blocks = std::max(p.blocks, blocks[b]);
     rows += (long)nodes[b] * R * Hkv;
+  }
+  p.kw = D < 256 && most_rows <= 64 ? 2 : 1;
+  const int per = 128 / p.kw;
+  for (int b = 0; b < B; ++b) {
+    blocks[b] = (nodes[b] * R + per - 1) / per;
+    p.blocks = std::max(p.blocks, blocks[b]);
   }
   constexpr double kStart = 6.0, kTile = 2.7;  // us
   double best = 0.0;
@@ -591,9 +731,9 @@ TreePlan tree_plan(int D, int R, int Hkv, int window, const int *past, const int
   return p;
 }
 
-template <int D, int MB>
+template <int D, int KW, int MB>
 static void run_tree(hipStream_t st, const TreeArgsOf<MB> &a, int B) {
-  hipLaunchKernelGGL((tree_attend_kernel<D, MB>), dim3(a.Hkv, a.splits, B * a.blocks), dim3(512), 0, st, a);
+  hipLaunchKernelGGL((tree_attend_kernel<D, KW, MB>), dim3(a.Hkv, a.splits, B * a.blocks), dim3(512), 0, st, a);
   if (a.splits > 1)
     hipLaunchKernelGGL(tree_merge_kernel<D>, dim3((unsigned)a.total), dim3(256), 0, st,
                        TreeMerge{a.part, a.out, a.err, a.splits, a.total});
@@ -601,9 +741,15 @@ static void run_tree(hipStream_t st, const TreeArgsOf<MB> &a, int B) {
 
 template <int MB>
 static hipError_t run_tree(hipStream_t st, const TreeArgsOf<MB> &a, int D, int B) {
-  if (D == 64) run_tree<64>(st, a, B);
-  else if (D == 128) run_tree<128>(st, a, B);
-  else run_tree<256>(st, a, B);
+  if (D == 64 && a.kw == 1) run_tree<64, 1>(st, a, B);
+  else if (D == 64) run_tree<64, 2>(st, a, B);
+  else if (D == 128 && a.kw == 1) run_tree<128, 1>(st, a, B);
+  else if (D == 128) run_tree<128, 2>(st, a, B);
+  else run_tree<256, 1>(st, a, B);
+  int most = 0;
+  for (int b = 0; b < B; ++b)
+    if (a.seq[b].kb) most = std::max(most, a.seq[b].nodes);
+  if (most) hipLaunchKernelGGL(tree_operands_kernel<MB>, dim3((most * D + 255) / 256, a.Hkv, B), dim3(256), 0, st, a, D);
   return hipGetLastError();
 }
 
