@@ -116,7 +116,7 @@ struct spissa_session {
   DevBuf amax;      // argmax partials
   DevBuf qstage;    // fused prefill step: bf16 Q operand
   DevBuf q4q;       // fused steps on a 4-bit cache: the rotated queries
-  DevBuf tree;      // tree steps: the key splits' outputs
+  DevBuf tree;      // tree steps: queries, visible nodes, outputs of parts of the keys
   float *lin = nullptr;  // partial sums of projections whose K is split over workgroups (linear_partials)
   std::mutex lin_mutex;  // held over the launches that write and read them
   DevBuf q4x;       // activations' pieces of projections of 4-bit weights (under lin_mutex)
@@ -2664,6 +2664,9 @@ static int validate_tree_config(const size_t *nodes, size_t batch, const spissa_
   if (total != cfg->query_len)
     return set_err(SPISSA_ERR_SHAPE, "the trees have %zu nodes, query_len is %zu", total, cfg->query_len);
   if (!cfg->causal) return set_err(SPISSA_ERR_SHAPE, "a tree step is causal");
+  if (cfg->kv_heads > 4096 || cfg->num_heads > 65535)
+    return set_err(SPISSA_ERR_SHAPE, "the tree step takes up to 4096 key/value heads and 65535 query heads, got %zu and %zu",
+                   cfg->kv_heads, cfg->num_heads);
   if (!decode_supported((int)std::min<size_t>(cfg->head_dim, 4096), 1))
     return set_err(SPISSA_ERR_SHAPE, "the tree step supports head_dim 64, 128 and 256, got %zu", cfg->head_dim);
   return SPISSA_OK;
@@ -2709,7 +2712,7 @@ static int run_tree_step(spissa_session *s, const spissa_rope_table *table, cons
   HIP_TRY(hipSetDevice(s->device));
   // (the workspace of every launch before the first: nothing is appended by a call that fails for want of it)
   std::vector<TreePlan> plans;
-  size_t bytes = 0;
+  size_t query_bytes = 0, mask_bytes = 0, part_bytes = 0;
   for (size_t b0 = 0; b0 < batch; b0 += kMaxDecodeBatch) {
     const int B = (int)std::min<size_t>(kMaxDecodeBatch, batch - b0);
     int past[kMaxDecodeBatch], count[kMaxDecodeBatch], n = 0;
@@ -2717,11 +2720,15 @@ static int run_tree_step(spissa_session *s, const spissa_rope_table *table, cons
       past[b] = (int)caches[b0 + b]->len;
       n += count[b] = (int)nodes[b0 + b];
     }
-    const TreePlan p = tree_plan(D, Hq / Hkv, Hkv, (int)cfg->window, past, count, B, s->cus);
+    TreePlan p;
+    if (!tree_plan(D, Hq / Hkv, Hkv, (int)cfg->window, past, count, B, s->cus, &p))
+      return set_err(SPISSA_ERR_SHAPE, "attention sizes exceed the device kernels' limits");
     plans.push_back(p);
-    if (p.splits > 1) bytes = std::max(bytes, (size_t)p.splits * n * Hq * (D + 4) * sizeof(float));
+    query_bytes = std::max(query_bytes, (size_t)p.groups * tree_query_bytes(D));
+    mask_bytes = std::max(mask_bytes, (size_t)n * (kTreeMaxNodes / 8));
+    if (p.splits > 1) part_bytes = std::max(part_bytes, (size_t)p.splits * n * Hq * (D + 4) * sizeof(float));
   }
-  if (bytes) ST_TRY(ensure_buf(s, s->tree, bytes));
+  ST_TRY(ensure_buf(s, s->tree, query_bytes + mask_bytes + part_bytes));
   size_t at = 0;
   for (size_t b0 = 0; b0 < batch; b0 += kMaxDecodeBatch) {
     const int B = (int)std::min<size_t>(kMaxDecodeBatch, batch - b0);
@@ -2729,7 +2736,7 @@ static int run_tree_step(spissa_session *s, const spissa_rope_table *table, cons
     int n = 0;
     for (int b = 0; b < B; ++b) {
       const spissa_kv_cache *c = caches[b0 + b];
-      a.seq[b] = TreeSeq{c->keys, c->values, c->kb, c->vt, (long)c->shadow_cap, (int)c->len, (int)nodes[b0 + b], n, 0};
+      a.seq[b] = TreeSeq{c->keys, c->values, c->kb, c->vt, (long)c->shadow_cap, (int)c->len, (int)nodes[b0 + b], n, 0, 0, 0, 0};
       n += (int)nodes[b0 + b];
     }
     if (n == 0) continue;
@@ -2739,7 +2746,9 @@ static int run_tree_step(spissa_session *s, const spissa_rope_table *table, cons
     a.out = d_out + at * Hq * D;
     a.parents = d_parents + at;
     at += n;
-    a.part = (float *)s->tree.p;
+    a.queries = (char *)s->tree.p;
+    a.mask = (unsigned *)((char *)s->tree.p + query_bytes);
+    a.part = (float *)((char *)s->tree.p + query_bytes + mask_bytes);
     a.cos = table ? table->cos : nullptr;
     a.sin = table ? table->sin : nullptr;
     a.prescale = 1.0f;
@@ -2755,13 +2764,9 @@ static int run_tree_step(spissa_session *s, const spissa_rope_table *table, cons
     a.R = Hq / Hkv;
     a.window = (int)cfg->window;
     a.qscale = (1.0f / sqrtf((float)D)) * 1.4426950408889634f;
-    const TreePlan &p = plans[b0 / kMaxDecodeBatch];
-    a.splits = p.splits;
-    a.tps = p.tps;
-    a.blocks = p.blocks;
-    a.kw = p.kw;
+    a.B = B;
     a.total = n * Hq;
-    HIP_TRY(launch_tree(s->stream, a, D, B));
+    HIP_TRY(launch_tree(s->stream, a, plans[b0 / kMaxDecodeBatch], D));
   }
   for (size_t b = 0; b < batch; ++b) caches[b]->len += nodes[b];
   return SPISSA_OK;

@@ -349,41 +349,46 @@ struct TreeSeq {
   bf16 *kb, *vt;     // its bf16 prefill operands, or null
   long cap;
   int past, nodes;   // cached rows; nodes, whose rows come after them
-  int first, pad;    // the sequence's first node among the launch's
+  int first;         // the sequence's first node among the launch's
+  int tiles, padded; // key tiles of one of its units, and the places they take (TreePlan)
+  int start;         // the place of its first unit
+  long group0;       // its first 16 rows' queries among the launch's
 };
 struct TreeBase {
   const float *q, *k, *v;        // [N, Hq, D], [N, Hkv, D]
   const int *parents;            // [N]
   float *out;
-  float *part;                   // [splits][N * Hq] entries of D + 4 floats: output, largest score, sum (splits > 1)
+  char *queries;                 // of 16 rows each: tree_query_bytes(D)
+  unsigned *mask;                // [N][kTreeMaxNodes / 32]: the nodes that a node sees
+  float *part;                   // [workgroups of a unit][N * Hq] entries of D + 4 floats: output, largest score, sum
   const float *cos, *sin;        // RoPE table rows by position, or null
   const float *q_norm, *k_norm;  // QK-norm, or null
   float eps, prescale;
   int *err;
-  int Hq, Hkv, R, window;
+  int B, Hq, Hkv, R, window;
   float qscale;                  // softmax scale * log2(e)
-  int splits, tps, blocks, kw;   // TreePlan
   int total;                     // N * Hq
+  int share, places, per;        // TreePlan's; rows of a block
 };
 template <int MB>
 struct TreeArgsOf : TreeBase {
   TreeSeq seq[MB];
 };
 typedef TreeArgsOf<kMaxDecodeBatch> TreeArgs;
-struct TreeMerge {
-  const float *part;
-  float *out;
-  int *err;
-  int splits, total;
-};
-// splits: workgroups of the longest sequence over its key tiles, each with up to tps of
-// them; blocks: of 128 / kw rows (nodes x query heads of a KV head) of the largest
-// tree; kw: waves that share a tile's keys.
+// A launch's work: units (a KV head of a block of 128 / kw rows, a row being a node and
+// a query head of the KV head) of key tiles at places one after the other, workgroups
+// with `share` places each, up to `splits` of them a unit; kw: waves that share a
+// tile's keys.
 struct TreePlan {
-  int splits = 1, tps = 1, blocks = 1, kw = 1;
+  int kw = 1, share = 1, splits = 1, places = 0;
+  long groups = 0;  // of 16 rows
+  int tiles[kMaxDecodeBatch], padded[kMaxDecodeBatch], start[kMaxDecodeBatch];
+  long group0[kMaxDecodeBatch];
 };
-TreePlan tree_plan(int D, int R, int Hkv, int window, const int *past, const int *nodes, int B, int cus);
-hipError_t launch_tree(hipStream_t st, const TreeArgs &a, int D, int B);
+bool tree_plan(int D, int R, int Hkv, int window, const int *past, const int *nodes, int B, int cus, TreePlan *plan);
+// The queries of 16 rows: two binary16 pieces, 16 inverse scales, 16 first keys.
+constexpr size_t tree_query_bytes(int D) { return 64 * (size_t)D + 128; }
+hipError_t launch_tree(hipStream_t st, TreeArgs &a, const TreePlan &p, int D);
 
 struct TreeAcceptArgs {
   const int *parents, *tokens, *sampled;
