@@ -79,14 +79,10 @@ __device__ __forceinline__ void load_pairs(const float *row, int l, f32x4 &lo, f
   lo = *reinterpret_cast<const f32x4 *>(row + 4 * l);
   hi = *reinterpret_cast<const f32x4 *>(row + D / 2 + 4 * l);
 }
-// The norm's weights times 1 / rms on such channels.
-template <int D>
-__device__ __forceinline__ void norm_pairs(f32x4 &lo, f32x4 &hi, const float *w, int l, float inv) {
+// The norm's weights times 1 / rms.
+__device__ __forceinline__ f32x4 norm4(f32x4 x, f32x4 w, float inv) {
 #pragma clang fp contract(off)
-  f32x4 a, b;
-  load_pairs<D>(w, l, a, b);
-  lo = lo * inv * a;
-  hi = hi * inv * b;
+  return x * inv * w;
 }
 __device__ __forceinline__ void rotate_pairs(f32x4 &lo, f32x4 &hi, const float *cos, const float *sin, long at) {
   const f32x4 c = *reinterpret_cast<const f32x4 *>(cos + at), s = *reinterpret_cast<const f32x4 *>(sin + at);
@@ -118,105 +114,135 @@ struct TreeQuery {
 
 }  // namespace
 
+// Up to 64 nodes, by each wave for itself: lane t's depth and nodes that it sees.
+struct SmallShape {
+  int depth;
+  unsigned lo, hi;
+};
+__device__ __forceinline__ SmallShape small_shape(int p, int nodes, int *err) {
+  const int t = threadIdx.x & 63;
+  if (p < -1 || p >= t) {
+    if (err && t < nodes) atomicOr(err, kDevErrTreeParent);
+    p = -1;
+  }
+  SmallShape s{p >= 0 ? 1 : 0, t < 32 ? 1u << t : 0u, t < 32 ? 0u : 1u << (t - 32)};
+  while (__any(p >= 0)) {
+    const int from = p < 0 ? t : p;
+    const int d = __shfl(s.depth, from), up = __shfl(p, from);
+    const unsigned l = (unsigned)__shfl((int)s.lo, from), h = (unsigned)__shfl((int)s.hi, from);
+    if (p >= 0) {
+      s.depth += d;
+      s.lo |= l;
+      s.hi |= h;
+      p = up;
+    }
+  }
+  return s;
+}
+
 // What the attention takes of the nodes, once each: the norm and the rotation of queries
 // and keys, keys and values into the cache (and its bf16 prefill operands), the queries
-// of 16 rows (a row: a node and one of the KV head's query heads) as the B operand of
-// the scores' product, two binary16 pieces of the query times a power of two, the
-// power's inverse, the first key that the row sees, and the nodes that a node sees.
-// Waves: one for the 16 rows of a KV head, then 64 / (D / 8) rows of keys or values.
-// Bound by latency: the parents, the rotation's rows, the stores.
-// Grid: (blocks of four waves of the longest sequence, sequences), 256 threads.
+// of 16 rows (a row: a node and one of the KV head's query heads; the last 16 are filled
+// up with the last row) as the B operand of the scores' product, two binary16 pieces of
+// the query times a power of two, the power's inverse, the first key that the row sees,
+// and the nodes that a node sees. D / 8 lanes a row, each with four channels and their
+// rotation's partners. Bound by latency: the parents, the rotation's rows, the stores.
+// Grid: (blocks of rows of the longest sequence, sequences), 256 threads.
 template <int D, int MB>
 __global__ __launch_bounds__(256) void tree_prepare_kernel(const TreeArgsOf<MB> a) {
-  constexpr int G = D / 32, TR = D / 8;
+  constexpr int G = D / 32, TR = D / 8, LINES = 256 / TR;
   __shared__ TreeShape shape;
   const int b = blockIdx.y, past = a.seq[b].past, nodes = a.seq[b].nodes, first = a.seq[b].first;
-  const int rows = nodes * a.R, groups = (rows + 15) / 16 * a.Hkv, jobs = groups + (nodes * a.Hkv * 2 * TR + 63) / 64;
-  const int tid = threadIdx.x, lane = tid & 63, job = blockIdx.x * 4 + (tid >> 6);
-  if ((int)blockIdx.x * 4 >= jobs) return;
-  const int parent = tid < nodes ? a.parents[first + tid] : -1;
-  // (what needs no position first)
-  f32x4 x[G], y[G];
-  const int kq = lane >> 4, h16 = job % a.Hkv, row = min(job / a.Hkv * 16 + (lane & 15), rows - 1), q_node = row / a.R;
-  const int line = (job - groups) * (64 / TR) + lane / TR, l = lane % TR;  // of keys, then of values: node by node
-  const bool key = line < nodes * a.Hkv;
-  const int in = key ? line : line - nodes * a.Hkv;
-  const bool mine = job >= groups && line < nodes * a.Hkv * 2;
-  if (job < groups) {
-    const float *const q = a.q + ((long)(first + q_node) * a.Hq + h16 * a.R + (row - q_node * a.R)) * D;
-#pragma unroll
-    for (int g = 0; g < G; ++g) load_pairs<D>(q, 4 * g + kq, x[g], y[g]);
-  } else if (mine) {
-    load_pairs<D>((key ? a.k : a.v) + ((long)first * a.Hkv + in) * D, l, x[0], y[0]);
-  }
-  if (blockIdx.x == 0) {
-    tree_shape<true>(parent, nodes, a.window, shape, a.err);
-    if (tid < nodes) {
-#pragma unroll
-      for (int w = 0; w < kMaskWords; ++w) a.mask[(long)(first + tid) * kMaskWords + w] = shape.mask[tid][w];
+  const int rows = nodes * a.R, padded = (rows + 15) & ~15;
+  const int queries = padded * a.Hkv, lines = queries + nodes * a.Hkv * 2;  // queries, keys, values
+  if ((int)blockIdx.x * LINES >= lines) return;
+  const int tid = threadIdx.x, lane = tid & 63, l = tid % TR, line = min((int)blockIdx.x * LINES + tid / TR, lines - 1);
+  const int parent = nodes <= 64 ? (lane < nodes ? a.parents[first + lane] : -1) : tid < nodes ? a.parents[first + tid] : -1;
+  const int kind = line < queries ? 0 : line < queries + nodes * a.Hkv ? 1 : 2;
+  const int in = kind == 0 ? line : kind == 1 ? line - queries : line - queries - nodes * a.Hkv;
+  // (a KV head's padded rows lie together, a node's heads do)
+  const int h = kind == 0 ? in / padded : in % a.Hkv, place = in - h * padded;
+  const int row = min(place, rows - 1), node = kind == 0 ? row / a.R : in / a.Hkv;
+  const float *const src = kind == 0 ? a.q + ((long)(first + node) * a.Hq + h * a.R + (row - node * a.R)) * D
+                                     : (kind == 1 ? +a.k : +a.v) + ((long)first * a.Hkv + in) * D;
+  f32x4 x, y, u, w;
+  load_pairs<D>(src, l, x, y);
+  if (a.q_norm && kind < 2) load_pairs<D>(kind == 0 ? +a.q_norm : +a.k_norm, l, u, w);
+  int *const err = blockIdx.x == 0 && tid < 64 ? a.err : nullptr;
+  int depth;
+  if (nodes <= 64 && !(a.window > 0 && a.window < nodes)) {
+    const SmallShape s = small_shape(parent, nodes, err);
+    depth = __shfl(s.depth, node);
+    if (blockIdx.x == 0 && tid < nodes) {
+      a.mask[(long)(first + tid) * kMaskWords] = s.lo;
+      a.mask[(long)(first + tid) * kMaskWords + 1] = s.hi;
     }
   } else {
-    tree_shape<false>(parent, nodes, a.window, shape, nullptr);
-  }
-  float minus_one = -1.0f;
-  asm volatile("" : "+s"(minus_one));
-  if (job < groups) {
-    const int pos = past + shape.depth[q_node];
-    if (a.q_norm) {
-      float sum = 0.0f;
+    const int mine = nodes <= 64 && tid >= 64 ? -1 : parent;
+    if (blockIdx.x == 0) {
+      tree_shape<true>(mine, nodes, a.window, shape, a.err);
+      if (tid < nodes) {
 #pragma unroll
-      for (int g = 0; g < G; ++g) sum += squares(x[g], y[g]);
-      const float inv = 1.0f / sqrtf(sum32(sum16(sum)) / (float)D + a.eps);
-#pragma unroll
-      for (int g = 0; g < G; ++g) norm_pairs<D>(x[g], y[g], a.q_norm, 4 * g + kq, inv);
+        for (int i = 0; i < kMaskWords; ++i) a.mask[(long)(first + tid) * kMaskWords + i] = shape.mask[tid][i];
+      }
+    } else {
+      tree_shape<false>(mine, nodes, a.window, shape, nullptr);
     }
+    depth = shape.depth[node];
+  }
+  if (kind < 2) {
+    if (a.q_norm) {
+      const float inv = 1.0f / sqrtf(group_sum<TR>(squares(x, y)) / (float)D + a.eps);
+      x = norm4(x, u, inv);
+      y = norm4(y, w, inv);
+    }
+    if (a.cos) rotate_pairs(x, y, a.cos, a.sin, (long)(past + depth) * (D / 2) + 4 * l);
+  }
+  if ((int)blockIdx.x * LINES + tid / TR >= lines) return;
+  if (kind == 0) {
+    float minus_one = -1.0f;
+    asm volatile("" : "+s"(minus_one));
+    x = x * a.prescale * a.qscale;
+    y = y * a.prescale * a.qscale;
     float most = 0.0f;
 #pragma unroll
-    for (int g = 0; g < G; ++g) {
-      if (a.cos) rotate_pairs(x[g], y[g], a.cos, a.sin, (long)pos * (D / 2) + 4 * (4 * g + kq));
-      x[g] = x[g] * a.prescale * a.qscale;
-      y[g] = y[g] * a.prescale * a.qscale;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float u = fabsf(x[g][i]), w = fabsf(y[g][i]);
-        most = fmaxf(most, fmaxf(u <= 3.402823466e38f ? u : 0.0f, w <= 3.402823466e38f ? w : 0.0f));
-      }
+    for (int i = 0; i < 4; ++i) {
+      const float p = fabsf(x[i]), q = fabsf(y[i]);
+      most = fmaxf(most, fmaxf(p <= 3.402823466e38f ? p : 0.0f, q <= 3.402823466e38f ? q : 0.0f));
     }
-    const unsigned bits = scale_to(max32(max16(most)), 9);
+    most = fmaxf(most, dpp<0xB1>(most));
+    most = fmaxf(most, dpp<0x4E>(most));
+    most = fmaxf(most, dpp<0x141>(most));
+    if constexpr (TR >= 16) most = fmaxf(most, dpp<0x140>(most));
+    if constexpr (TR >= 32) most = max16(most);
+    const unsigned bits = scale_to(most, 9);
     const float scale = unbits(bits);
-    const TreeQuery<D> out(a.queries, a.seq[b].group0 + job);
+    const float v[8] = {x[0] * scale, x[1] * scale, x[2] * scale, x[3] * scale, y[0] * scale, y[1] * scale, y[2] * scale, y[3] * scale};
+    half8 ph, pl;
+    split8(v, minus_one, &ph, &pl);
+    const TreeQuery<D> out(a.queries, a.seq[b].group0 + (place >> 4) * a.Hkv + h);
+    const int at = (l & 3) * 16 + (place & 15);
+    out.piece(0, l >> 2)[at] = ph;
+    out.piece(1, l >> 2)[at] = pl;
+    if (l == 0) {
+      out.inverse()[place & 15] = inverse_scale(bits);
+      out.from()[place & 15] = a.window > 0 ? max(0, past + depth + 1 - a.window) : 0;
+    }
+    return;
+  }
+  const long at = past + node;
+  const int head = in % a.Hkv;
+  float *const dst = (kind == 1 ? +a.seq[b].k : +a.seq[b].v) + (at * a.Hkv + head) * D + 4 * l;
+  *reinterpret_cast<f32x4 *>(dst) = x;
+  *reinterpret_cast<f32x4 *>(dst + D / 2) = y;
+  bf16 *const kb = a.seq[b].kb, *const vt = a.seq[b].vt;
+  if (kb) {
+    const long cap = a.seq[b].cap, step = kind == 1 ? 1 : cap;
+    bf16 *const to = kind == 1 ? kb + ((long)head * cap + at) * D + 4 * l : vt + ((long)head * D + 4 * l) * cap + vt_key_slot(at);
 #pragma unroll
-    for (int g = 0; g < G; ++g) {
-      const float v[8] = {x[g][0] * scale, x[g][1] * scale, x[g][2] * scale, x[g][3] * scale,
-                          y[g][0] * scale, y[g][1] * scale, y[g][2] * scale, y[g][3] * scale};
-      half8 ph, pl;
-      split8(v, minus_one, &ph, &pl);
-      out.piece(0, g)[lane] = ph;
-      out.piece(1, g)[lane] = pl;
-    }
-    if (kq == 0) {
-      out.inverse()[lane] = inverse_scale(bits);
-      out.from()[lane] = a.window > 0 ? max(0, pos + 1 - a.window) : 0;
-    }
-  } else if (mine) {
-    const int node = in / a.Hkv, h = in - node * a.Hkv;
-    const long at = past + node;
-    if (key) {
-      if (a.k_norm) norm_pairs<D>(x[0], y[0], a.k_norm, l, 1.0f / sqrtf(group_sum<TR>(squares(x[0], y[0])) / (float)D + a.eps));
-      if (a.cos) rotate_pairs(x[0], y[0], a.cos, a.sin, (past + shape.depth[node]) * (long)(D / 2) + 4 * l);
-    }
-    float *const dst = (key ? a.seq[b].k : a.seq[b].v) + (at * a.Hkv + h) * D + 4 * l;
-    *reinterpret_cast<f32x4 *>(dst) = x[0];
-    *reinterpret_cast<f32x4 *>(dst + D / 2) = y[0];
-    bf16 *const kb = a.seq[b].kb, *const vt = a.seq[b].vt;
-    if (kb) {
-      const long cap = a.seq[b].cap, step = key ? 1 : cap;
-      bf16 *const to = key ? kb + ((long)h * cap + at) * D + 4 * l : vt + ((long)h * D + 4 * l) * cap + vt_key_slot(at);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        to[i * step] = (bf16)x[0][i];
-        to[(D / 2 + i) * step] = (bf16)y[0][i];
-      }
+    for (int i = 0; i < 4; ++i) {
+      to[i * step] = (bf16)x[i];
+      to[(D / 2 + i) * step] = (bf16)y[i];
     }
   }
 }
@@ -726,12 +752,13 @@ static void run_merge(hipStream_t st, const TreeArgsOf<MB> &a, int splits) {
 
 template <int D, int KW, int MB>
 static void run_attend(hipStream_t st, const TreeArgsOf<MB> &a, const TreePlan &p) {
-  int jobs = 0;  // of the prepare kernel: queries, then keys and values
+  int lines = 0;  // of the prepare kernel: queries, keys and values
   for (int b = 0; b < a.B; ++b) {
     const int n = a.seq[b].nodes;
-    jobs = std::max(jobs, (n * a.R + 15) / 16 * a.Hkv + (n * a.Hkv * 2 * (D / 8) + 63) / 64);
+    lines = std::max(lines, (((n * a.R + 15) & ~15) + 2 * n) * a.Hkv);
   }
-  hipLaunchKernelGGL((tree_prepare_kernel<D, MB>), dim3((jobs + 3) / 4, a.B), dim3(256), 0, st, a);
+  constexpr int LINES = 2048 / D;
+  hipLaunchKernelGGL((tree_prepare_kernel<D, MB>), dim3((lines + LINES - 1) / LINES, a.B), dim3(256), 0, st, a);
   hipLaunchKernelGGL((tree_attend_kernel<D, KW, MB>), dim3((a.places + a.share - 1) / a.share), dim3(512), 0, st, a);
   if (p.splits > 1) run_merge<D>(st, a, p.splits);
 }
