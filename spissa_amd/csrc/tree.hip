@@ -150,7 +150,7 @@ __device__ __forceinline__ SmallShape small_shape(int p, int nodes, int *err) {
 // Grid: (blocks of rows of the longest sequence, sequences), 256 threads.
 template <int D, int MB>
 __global__ __launch_bounds__(256) void tree_prepare_kernel(const TreeArgsOf<MB> a) {
-  constexpr int G = D / 32, TR = D / 8, LINES = 256 / TR;
+  constexpr int TR = D / 8, LINES = 256 / TR;
   __shared__ TreeShape shape;
   const int b = blockIdx.y, past = a.seq[b].past, nodes = a.seq[b].nodes, first = a.seq[b].first;
   const int rows = nodes * a.R, padded = (rows + 15) & ~15;
@@ -294,6 +294,7 @@ __global__ __launch_bounds__(512, 2) void tree_attend_kernel(const TreeArgsOf<MB
   constexpr int BN = 8192 / D, G = D / 32, DT = D / 16, VB = BN / 32, KB = BN / 16, TR = D / 8;
   constexpr int RW = 8 / KW, ROWS = RW * 16;
   constexpr int KBW = KB / KW, VBW = VB / KW;  // a wave's 16 and 32 keys of a tile
+  constexpr int AHEAD = D == 256 ? 2 : 3;
   static_assert(KB * G == 16 && VB * DT == 16, "a tile has 8192 keys' and as many values' channels");
   __shared__ __attribute__((aligned(16))) half8 pieces_lds[2][2][2][1024];  // values, buffer, piece
   half8 (*const kp_lds)[2][1024] = pieces_lds[0], (*const vp_lds)[2][1024] = pieces_lds[1];
@@ -423,24 +424,49 @@ __global__ __launch_bounds__(512, 2) void tree_attend_kernel(const TreeArgsOf<MB
       const int buf = tile & 1;
       const bool own = tile >= cached;
       const int base = lo + tile * BN;
+      // Steps of two operands of either product, six instructions; their LDS reads run
+      // AHEAD - 1 steps before them. The scores' are two 16 keys of 32 channels each,
+      // the outputs' 32 keys of two 16 channels.
+      constexpr int KS = G * KBW / 2, VS = VBW * DT / 2;
+      half8 fh[AHEAD][2], fl[AHEAD][2];
+      auto read = [&](int step) __attribute__((always_inline)) {
+        half8 (&th)[2] = fh[step % AHEAD], (&tl)[2] = fl[step % AHEAD];
+        if (step < KS) {
+          const int g = step / (KBW / 2), k = step % (KBW / 2) * 2;
+          const int at = ((kw * KBW + k) * G + g) * 64 + kq * 16 + ((col ^ (4 * g + kq)) & 15);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            th[i] = kp_lds[buf][0][at + i * G * 64];
+            tl[i] = kp_lds[buf][1][at + i * G * 64];
+          }
+        } else if (step < KS + VS) {
+          const int v = (step - KS) / (DT / 2), d = (step - KS) % (DT / 2) * 2;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int at = ((kw * VBW + v) * DT + d + i) * 64 + kq * 16 + (col ^ ((d + i) & 3));
+            th[i] = vp_lds[buf][0][at];
+            tl[i] = vp_lds[buf][1][at];
+          }
+        }
+      };
       f32x4 sc[KBW];
 #pragma unroll
       for (int k = 0; k < KBW; ++k) sc[k] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int g = 0; g < G; ++g) {
-        const int at = (kw * KBW * G + g) * 64 + kq * 16 + ((col ^ (4 * g + kq)) & 15);
-        half8 fh[KBW], fl[KBW];
+      for (int i = 0; i < AHEAD - 1; ++i) read(i);
 #pragma unroll
-        for (int k = 0; k < KBW; ++k) {
-          fh[k] = kp_lds[buf][0][k * G * 64 + at];
-          fl[k] = kp_lds[buf][1][k * G * 64 + at];
-        }
+      for (int step = 0; step < KS; ++step) {
+        const int g = step / (KBW / 2), k = step % (KBW / 2) * 2;
+        read(step + AHEAD - 1);
+        __builtin_amdgcn_sched_barrier(0);
+        const half8 (&th)[2] = fh[step % AHEAD], (&tl)[2] = fl[step % AHEAD];
 #pragma unroll
-        for (int k = 0; k < KBW; ++k) sc[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fh[k], qh[g], sc[k], 0, 0, 0);
+        for (int i = 0; i < 2; ++i) sc[k + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(th[i], qh[g], sc[k + i], 0, 0, 0);
 #pragma unroll
-        for (int k = 0; k < KBW; ++k) sc[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fh[k], ql[g], sc[k], 0, 0, 0);
+        for (int i = 0; i < 2; ++i) sc[k + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(th[i], ql[g], sc[k + i], 0, 0, 0);
 #pragma unroll
-        for (int k = 0; k < KBW; ++k) sc[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fl[k], qh[g], sc[k], 0, 0, 0);
+        for (int i = 0; i < 2; ++i) sc[k + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(tl[i], qh[g], sc[k + i], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
       }
       // (finite and above 0: hidden scores stay -inf)
       const float f = fminf(fmaxf(inv_q * inverse_scale(kbits), 1.1754944e-38f), 3.402823466e38f);
@@ -488,23 +514,19 @@ __global__ __launch_bounds__(512, 2) void tree_attend_kernel(const TreeArgsOf<MB
         split8(p, minus_one, &ph[v], &pl[v]);
       }
 #pragma unroll
-      for (int v = 0; v < VBW; ++v)
+      for (int step = KS; step < KS + VS; ++step) {
+        const int v = (step - KS) / (DT / 2), d = (step - KS) % (DT / 2) * 2;
+        read(step + AHEAD - 1);
+        __builtin_amdgcn_sched_barrier(0);
+        const half8 (&th)[2] = fh[step % AHEAD], (&tl)[2] = fl[step % AHEAD];
 #pragma unroll
-        for (int d = 0; d < DT; d += 4) {
-          half8 fh[4], fl[4];
+        for (int i = 0; i < 2; ++i) o[d + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(th[i], ph[v], o[d + i], 0, 0, 0);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int at = ((kw * VBW + v) * DT + d + j) * 64 + kq * 16 + (col ^ j);
-            fh[j] = vp_lds[buf][0][at];
-            fl[j] = vp_lds[buf][1][at];
-          }
+        for (int i = 0; i < 2; ++i) o[d + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(th[i], pl[v], o[d + i], 0, 0, 0);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) o[d + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fh[j], ph[v], o[d + j], 0, 0, 0);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) o[d + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fh[j], pl[v], o[d + j], 0, 0, 0);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) o[d + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fl[j], ph[v], o[d + j], 0, 0, 0);
-        }
+        for (int i = 0; i < 2; ++i) o[d + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(tl[i], ph[v], o[d + i], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+      }
     };
 
     constexpr unsigned kInfinite = 0x7f800000u;
