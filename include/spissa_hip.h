@@ -571,7 +571,7 @@ int spissa_attention_sublayer_device(spissa_session *s, const spissa_attention_l
  * alone. Each setting is the struct's number, or, where the pointer is not
  * NULL, a device array of one number a row. */
 typedef struct {
-    size_t rows;
+    size_t rows;               /* up to 65535 (SHAPE otherwise) */
     size_t vocab;              /* up to 2^22 (SHAPE otherwise) */
     float temperature;         /* finite, >= 0 */
     size_t top_k;

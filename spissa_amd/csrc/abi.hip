@@ -116,6 +116,7 @@ struct spissa_session {
   DevBuf amax;      // argmax partials
   DevBuf qstage;    // fused prefill step: bf16 Q operand
   DevBuf q4q;       // fused steps on a 4-bit cache: the rotated queries
+  DevBuf sample;    // sampling: bins and lists of each row
   DevBuf tree;      // tree steps: queries, visible nodes, outputs of parts of the keys
   float *lin = nullptr;  // partial sums of projections whose K is split over workgroups (linear_partials)
   std::mutex lin_mutex;  // held over the launches that write and read them
@@ -235,6 +236,7 @@ static void session_free(spissa_session *s) {
   free_buf(s->qstage);
   free_buf(s->q4q);
   free_buf(s->tree);
+  free_buf(s->sample);
   free_buf(s->q4x);
   for (void *p : s->retired) (void)hipFree(p);
   if (s->d_err) (void)hipFree(s->d_err);
@@ -2619,8 +2621,8 @@ extern "C" int spissa_sample_device(spissa_session *s, const float *d_logits, co
   GUARD_BEGIN
   if (!cfg) return set_err(SPISSA_ERR_ARGUMENT, "config is null");
   if (cfg->rows && cfg->vocab == 0) return set_err(SPISSA_ERR_INVALID_TENSOR_DATA, "cannot sample from empty logits");
-  if (cfg->vocab > kSampleMaxVocab || cfg->rows > (size_t)INT32_MAX)
-    return set_err(SPISSA_ERR_SHAPE, "sampling takes up to %d rows of %zu logits, got %zu of %zu", INT32_MAX,
+  if (cfg->vocab > kSampleMaxVocab || cfg->rows > kSampleMaxRows)
+    return set_err(SPISSA_ERR_SHAPE, "sampling takes up to %zu rows of %zu logits, got %zu of %zu", kSampleMaxRows,
                    kSampleMaxVocab, cfg->rows, cfg->vocab);
   if (!(cfg->temperature >= 0.0f && std::isfinite(cfg->temperature)))
     return set_err(SPISSA_ERR_INVALID_TENSOR_DATA, "temperature %g is not a finite number >= 0", (double)cfg->temperature);
@@ -2647,7 +2649,8 @@ extern "C" int spissa_sample_device(spissa_session *s, const float *d_logits, co
   a.probs = d_probs;
   a.err = s->d_err;
   HIP_TRY(hipSetDevice(s->device));
-  HIP_TRY(launch_sample(s->stream, a));
+  ST_TRY(ensure_buf(s, s->sample, sample_workspace(a.rows, a.vocab)));
+  HIP_TRY(launch_sample(s->stream, a, s->sample.p));
   return SPISSA_OK;
   GUARD_END
 }

@@ -339,8 +339,9 @@ struct SampleArgs {
   float *probs;          // [rows] or null
   int *err;
 };
-constexpr size_t kSampleMaxVocab = (size_t)1 << 22;
-hipError_t launch_sample(hipStream_t st, const SampleArgs &a);
+constexpr size_t kSampleMaxVocab = (size_t)1 << 22, kSampleMaxRows = 65535;
+size_t sample_workspace(int rows, int vocab);
+hipError_t launch_sample(hipStream_t st, const SampleArgs &a, void *workspace);
 
 // ---- trees of drafted tokens (tree.hip) ----
 constexpr int kTreeMaxNodes = 256;
