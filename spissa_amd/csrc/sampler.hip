@@ -10,16 +10,17 @@
 //
 // A row's logits are read three times, by workgroups of a slice each:
 //   1. the slice's largest and smallest logit;
-//   2. counts and weights of 1024 bins of (max - x), fine enough that few tokens share
-//      the bin in which a filter ends;
-//   3. with those bins known: their tokens into a list, and the sum of the weights
-//      certain to be kept.
-// Between and after them a workgroup a row finds the bins, then sorts the list (of some
-// hundred tokens), finds the last kept one, draws, and walks the slice in which the draw
-// falls. A row whose list would not fit (thousands of tokens within a thousandth of the
-// logits' range) is done by bits of the logits instead, by a workgroup over the whole
-// row. Bound by latency for a few rows; for many by the reads and by the weights' 30
-// operations in 64 bits a token.
+//   2. the counts (for top-k) or else the weights (for top-p) of 1024 bins of (max - x),
+//      fine enough that few tokens share the bin in which the filter ends;
+//   3. with that bin known: into a list the tokens that have to be put in order (all of
+//      the top-k's bins, or those of the bin where top-p ends), and the sums of the
+//      weights certain to be kept, by granules of 256 logits.
+// Between and after them a workgroup a row finds the bin, then the last kept token in the
+// list (of some hundred), by bits of their order, draws, and walks the granule in which the
+// draw falls. A row whose list would not fit (thousands of tokens in a thousandth of the
+// logits' range, or a top-k of thousands) is done in the same way over the whole row.
+// Without filters the first, second and last steps are enough. Bound by latency for a
+// few rows; for many by the reads and by the weights' 30 operations in 64 bits a token.
 #include <algorithm>
 #include <climits>
 
@@ -32,7 +33,7 @@ namespace {
 
 typedef unsigned long long u64;
 
-constexpr int NT = 512, BINS = 1024, LIST = 4096;
+constexpr int NT = 512, BINS = 1024, LIST = 8192, GRANULE = 256;
 
 // Bits that rise with the value; both zeros alike.
 __device__ __forceinline__ unsigned sort_key(float x) {
@@ -40,6 +41,11 @@ __device__ __forceinline__ unsigned sort_key(float x) {
   return b ^ (b >> 31 ? 0xffffffffu : 0x80000000u);
 }
 __device__ __forceinline__ float key_value(unsigned k) { return __uint_as_float(k ^ (k >> 31 ? 0x80000000u : 0xffffffffu)); }
+
+// A token as a number that falls along the order: its logit's key, then its index.
+__device__ __forceinline__ u64 token_of(float x, int i) { return (u64)sort_key(x) << 32 | ~(unsigned)i; }
+__device__ __forceinline__ float logit_of(u64 token) { return key_value((unsigned)(token >> 32)); }
+__device__ __forceinline__ int index_of(u64 token) { return (int)~(unsigned)token; }
 
 // exp((x - max) / T) as 2^(n + r), |r| <= 1/2, by twelve terms of exp(r ln 2): off by at
 // most 2^-52 of itself.
@@ -81,15 +87,13 @@ struct Slice {
 };
 // What a row's later passes go by.
 struct Row {
-  u64 whole;            // weights of all
+  u64 whole, before;  // without top-k: weights of all, and of the bins before lo
   float top, per_bin;
   float temperature, top_p, min_p, u;
-  int top_k;            // 0: all
-  int state;            // kBad.. below
-  int lo, hi, k;        // bins of the list: lo..hi (where top-p may end) and k (where top-k ends); certain below lo
-  int need_k;           // tokens of bin k that top-k keeps
-  int first;            // the largest logit's first place
-  u64 before_lo, before_k;  // weights of the bins before lo and before k
+  int top_k;          // 0: all
+  int state;          // kBad..
+  int lo, hi;         // bins of the list; tokens of those before lo are certain of all but min_p
+  int first;          // the largest logit's first place
 };
 enum : int { kBad, kGreedy, kAll, kList };
 
@@ -115,24 +119,27 @@ __device__ __forceinline__ int bin_of(float x, float top, float per_bin) {
   return t < BINS - 1 ? (int)t : BINS - 1;
 }
 
-// f(index, logit) for a thread's logits of a slice, four in a row at a time.
-template <class F>
-__device__ __forceinline__ void each(const float *x, int from, int to, bool vec, F f) {
-  if (vec) {
-    for (int i = from + 4 * (int)threadIdx.x; i < to; i += 4 * NT) {
-      if (i + 4 <= to) {
-        const float4 v = *reinterpret_cast<const float4 *>(x + i);
-        f(i, v.x);
-        f(i + 1, v.y);
-        f(i + 2, v.z);
-        f(i + 3, v.w);
-      } else {
-        for (int j = i; j < to; ++j) f(j, x[j]);
-      }
+// The granules of a slice by waves: f(index, logit) for a lane's four, then done(granule).
+template <class F, class G>
+__device__ __forceinline__ void each(const float *x, int from, int to, F f, G done) {
+  const bool vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0;
+  for (int g = from + (int)(threadIdx.x >> 6) * GRANULE; g < to; g += NT / 64 * GRANULE) {
+    const int i = g + 4 * (int)(threadIdx.x & 63);
+    if (vec && i + 4 <= to) {
+      const float4 v = *reinterpret_cast<const float4 *>(x + i);
+      f(i, v.x);
+      f(i + 1, v.y);
+      f(i + 2, v.z);
+      f(i + 3, v.w);
+    } else {
+      for (int j = i; j < min(i + 4, to); ++j) f(j, x[j]);
     }
-  } else {
-    for (int i = from + (int)threadIdx.x; i < to; i += NT) f(i, x[i]);
+    done(g / GRANULE);
   }
+}
+__device__ __forceinline__ u64 wave_sum(u64 v) {
+  for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
+  return v;
 }
 
 template <class T>
@@ -170,42 +177,37 @@ __device__ T block_before(T v, T *part, T *all) {
 // A row's share of the workspace.
 struct Space {
   Row *row;
-  Slice *slices;
-  u64 *kept;        // [slices]: weights certain to be kept
-  u64 *weights;     // [slices][BINS]
-  unsigned *counts; // [slices][BINS]
   unsigned *listed; // tokens of the list (beyond LIST: not all of them there)
   u64 *list;        // [LIST]: key, and the index's complement
+  u64 *bins;        // [slices][BINS] weights or, half as long, counts
+  u64 *kept;        // [granules]: weights certain to be kept
+  Slice *slices;
 };
-__host__ __device__ inline size_t row_bytes(int slices) {
-  return ((sizeof(Row) + 15) & ~(size_t)15) + (size_t)slices * (sizeof(Slice) + 16 + BINS * 12) + 16 + LIST * 8;
+struct SampleWork {
+  char *space;
+  size_t row_bytes;
+  int slices, length;  // of a row; logits of a slice
+  int granules;
+  int shift;
+};
+constexpr size_t kRowHead = 80;
+static_assert(sizeof(Row) <= kRowHead && kRowHead % 16 == 0, "a row's head");
+inline size_t row_bytes(int slices, int granules) {
+  return kRowHead + 16 + LIST * 8 + (size_t)slices * (BINS * 8 + sizeof(Slice)) + ((size_t)granules * 8 + 15) / 16 * 16;
 }
-__device__ __forceinline__ Space space_of(char *workspace, int row, int slices) {
-  char *p = workspace + (size_t)row * row_bytes(slices);
+__device__ __forceinline__ Space space_of(const SampleWork &w, int row) {
+  char *const p = w.space + row * w.row_bytes;
   Space s;
   s.row = reinterpret_cast<Row *>(p);
-  p += (sizeof(Row) + 15) & ~(size_t)15;
-  s.listed = reinterpret_cast<unsigned *>(p);
-  p += 16;
-  s.list = reinterpret_cast<u64 *>(p);
-  p += LIST * 8;
-  s.weights = reinterpret_cast<u64 *>(p);
-  p += (size_t)slices * BINS * 8;
-  s.kept = reinterpret_cast<u64 *>(p);
-  p += (size_t)slices * 16;
-  s.slices = reinterpret_cast<Slice *>(p);
-  p += (size_t)slices * sizeof(Slice);
-  s.counts = reinterpret_cast<unsigned *>(p);
+  s.listed = reinterpret_cast<unsigned *>(p + kRowHead);
+  s.list = reinterpret_cast<u64 *>(p + kRowHead + 16);
+  s.bins = s.list + LIST;
+  s.slices = reinterpret_cast<Slice *>(s.bins + (size_t)w.slices * BINS);
+  s.kept = reinterpret_cast<u64 *>(s.slices + w.slices);
   return s;
 }
 
 }  // namespace
-
-struct SampleWork {
-  char *space;
-  int slices, length;  // of a row; logits of a slice
-  int shift;
-};
 
 // Grid: (slices, rows).
 __global__ __launch_bounds__(NT) void sample_ends_kernel(const SampleArgs a, const SampleWork w) {
@@ -213,14 +215,17 @@ __global__ __launch_bounds__(NT) void sample_ends_kernel(const SampleArgs a, con
   const int row = blockIdx.y, from = blockIdx.x * w.length, to = min(a.vocab, from + w.length);
   const float *const x = a.x + (long)row * a.vocab;
   Slice s{NEG_INF, __builtin_inff(), INT_MAX, 0};
-  each(x, from, to, (reinterpret_cast<uintptr_t>(x) & 15) == 0, [&](int i, float v) {
-    s.bad |= !(v < __builtin_inff());
-    if (v > s.most) {
-      s.most = v;
-      s.at = i;
-    }
-    s.least = fminf(s.least, v);
-  });
+  each(
+      x, from, to,
+      [&](int i, float v) {
+        s.bad |= !(v < __builtin_inff());
+        if (v > s.most) {
+          s.most = v;
+          s.at = i;
+        }
+        s.least = fminf(s.least, v);
+      },
+      [](int) {});
   auto join = [&](float most, float least, int at, int bad) {
     if (most > s.most || (most == s.most && at < s.at)) s.at = at;
     s.most = fmaxf(s.most, most);
@@ -232,12 +237,12 @@ __global__ __launch_bounds__(NT) void sample_ends_kernel(const SampleArgs a, con
   __syncthreads();
   if (threadIdx.x == 0) {
     for (int i = 1; i < NT / 64; ++i) join(part[i].most, part[i].least, part[i].at, part[i].bad);
-    space_of(w.space, row, w.slices).slices[blockIdx.x] = s;
+    space_of(w, row).slices[blockIdx.x] = s;
   }
 }
 
 // A row's ends from its slices', its settings, and what is to be done; every thread gets it.
-__device__ __forceinline__ Row row_of(const SampleArgs &a, const SampleWork &w, const Space &s, int row, int *first) {
+__device__ __forceinline__ Row row_of(const SampleArgs &a, const SampleWork &w, const Space &s, int row) {
   __shared__ Slice part[NT / 64];
   Slice e{NEG_INF, __builtin_inff(), INT_MAX, 0};
   auto join = [&](float most, float least, int at, int bad) {
@@ -251,6 +256,7 @@ __device__ __forceinline__ Row row_of(const SampleArgs &a, const SampleWork &w, 
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = e;
   __syncthreads();
   for (int i = 0; i < NT / 64; ++i) join(part[i].most, part[i].least, part[i].at, part[i].bad);
+  __syncthreads();
   Row r;
   const bool fine = settings(a, row, r);
   r.top = e.most;
@@ -261,183 +267,237 @@ __device__ __forceinline__ Row row_of(const SampleArgs &a, const SampleWork &w, 
             : r.temperature == 0.0f             ? kGreedy
             : r.top_k == 0 && r.top_p >= 1.0f   ? kAll
                                                 : kList;
-  *first = e.at;
+  r.first = e.at;
+  r.whole = r.before = 0;
+  r.lo = r.hi = 0;
   return r;
 }
 
-// Counts (for top-k) and weights (for top-p) of the slice's bins; without either filter
-// the sum of its kept weights. Grid: (slices, rows).
+// The counts or weights of the slice's bins; without a filter the sums of its granules'
+// kept weights. Grid: (slices, rows).
 __global__ __launch_bounds__(NT) void sample_bins_kernel(const SampleArgs a, const SampleWork w) {
-  __shared__ u64 weights[BINS], part[NT / 64];
-  __shared__ unsigned counts[BINS];
+  __shared__ u64 weights[BINS];
   const int row = blockIdx.y, from = blockIdx.x * w.length, to = min(a.vocab, from + w.length);
   const float *const x = a.x + (long)row * a.vocab;
-  const bool vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0;
-  const Space s = space_of(w.space, row, w.slices);
-  int first;
-  const Row r = row_of(a, w, s, row, &first);
-  if (blockIdx.x == 0 && threadIdx.x == 0) *s.listed = 0;
+  const Space s = space_of(w, row);
+  const Row r = row_of(a, w, s, row);
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    *s.listed = 0;
+    *s.row = r;
+  }
   if (r.state < kAll) return;
   const Weigh weigh = weigh_of(r, w.shift);
   if (r.state == kAll) {
     u64 sum = 0;
-    each(x, from, to, vec, [&](int, float v) { sum += weigh.least(v); });
-    sum = block_sum(sum, part);
-    if (threadIdx.x == 0) s.kept[blockIdx.x] = sum;
+    each(
+        x, from, to, [&](int, float v) { sum += weigh.least(v); },
+        [&](int g) {
+          sum = wave_sum(sum);
+          if ((threadIdx.x & 63) == 0) s.kept[g] = sum;
+          sum = 0;
+        });
     return;
   }
-  for (int i = threadIdx.x; i < BINS; i += NT) {
-    weights[i] = 0;
-    counts[i] = 0;
+  const bool by_count = r.top_k > 0;
+  unsigned *const counts = reinterpret_cast<unsigned *>(weights);
+  for (int i = threadIdx.x; i < BINS; i += NT) weights[i] = 0;
+  __syncthreads();
+  if (by_count) {
+    each(x, from, to, [&](int, float v) { atomicAdd(&counts[bin_of(v, r.top, r.per_bin)], 1u); }, [](int) {});
+  } else {
+    // (what has no weight, far down, would only meet in the last bin)
+    each(
+        x, from, to,
+        [&](int, float v) {
+          const u64 p = weigh(v);
+          if (p) atomicAdd(&weights[bin_of(v, r.top, r.per_bin)], p);
+        },
+        [](int) {});
   }
   __syncthreads();
-  const bool by_weight = r.top_p < 1.0f, by_count = r.top_k > 0;
-  each(x, from, to, vec, [&](int, float v) {
-    const int b = bin_of(v, r.top, r.per_bin);
-    if (by_count) atomicAdd(&counts[b], 1u);
-    if (by_weight && b < BINS - 1) atomicAdd(&weights[b], weigh(v));
-    else if (by_weight) {
-      const u64 p = weigh(v);
-      if (p) atomicAdd(&weights[b], p);
-    }
-  });
-  __syncthreads();
-  for (int i = threadIdx.x; i < BINS; i += NT) {
-    if (by_weight) s.weights[(long)blockIdx.x * BINS + i] = weights[i];
-    if (by_count) s.counts[(long)blockIdx.x * BINS + i] = counts[i];
-  }
+  u64 *const to_bins = s.bins + (size_t)blockIdx.x * BINS;
+  for (int i = threadIdx.x; i < (by_count ? BINS / 2 : BINS); i += NT) to_bins[i] = weights[i];
 }
 
-// The bins in which the filters end. Grid: rows.
+// The bin in which the filter ends. Grid: rows.
 __global__ __launch_bounds__(NT) void sample_cut_kernel(const SampleArgs a, const SampleWork w) {
-  __shared__ u64 part[NT / 64], before[BINS + 1];
-  __shared__ unsigned parts[NT / 64];
-  __shared__ int found[3];
-  __shared__ unsigned above_k;
+  __shared__ u64 part[NT / 64];
+  static_assert(BINS == 2 * NT, "a thread has two bins");
   const int row = blockIdx.x, t = threadIdx.x;
-  const Space s = space_of(w.space, row, w.slices);
-  int first;
-  Row r = row_of(a, w, s, row, &first);
-  constexpr int PER = BINS / NT;
-  if (r.state == kList) {
-    const bool by_weight = r.top_p < 1.0f, by_count = r.top_k > 0;
-    if (t < 3) found[t] = BINS - 1;
-    if (t == 0) above_k = 0;
-    u64 wt[PER] = {}, run = 0, total;
-    unsigned ct[PER] = {}, runs = 0, counted;
-    static_assert(PER == 2, "a thread's bins are one load");
-    if (by_weight) {
+  const Space s = space_of(w, row);
+  const Row r = *s.row;
+  if (r.state != kList) return;
+  u64 in[2] = {0, 0};
+  if (r.top_k > 0) {
+    const uint2 *const counts = reinterpret_cast<const uint2 *>(s.bins) + t;
 #pragma unroll 16
-      for (int i = 0; i < w.slices; ++i) {
-        const ulonglong2 v = reinterpret_cast<const ulonglong2 *>(s.weights + (long)i * BINS)[t];
-        wt[0] += v.x;
-        wt[1] += v.y;
-      }
+    for (int i = 0; i < w.slices; ++i) {
+      const uint2 v = counts[(size_t)i * BINS];
+      in[0] += v.x;
+      in[1] += v.y;
     }
-    if (by_count) {
+  } else {
+    const ulonglong2 *const weights = reinterpret_cast<const ulonglong2 *>(s.bins) + t;
 #pragma unroll 16
-      for (int i = 0; i < w.slices; ++i) {
-        const uint2 v = reinterpret_cast<const uint2 *>(s.counts + (long)i * BINS)[t];
-        ct[0] += v.x;
-        ct[1] += v.y;
-      }
+    for (int i = 0; i < w.slices; ++i) {
+      const ulonglong2 v = weights[(size_t)i * NT];
+      in[0] += v.x;
+      in[1] += v.y;
     }
-#pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      run += wt[j];
-      runs += ct[j];
-    }
-    u64 up = block_before(run, part, &total);
-    unsigned ups = block_before(runs, parts, &counted);
-#pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      before[t * PER + j] = up;
-      up += wt[j];
-      if (by_count && ups < (unsigned)r.top_k && ups + ct[j] >= (unsigned)r.top_k) {
-        found[2] = t * PER + j;
-        above_k = ups;
-      }
-      ups += ct[j];
-    }
-    if (t == NT - 1) before[BINS] = total;
-    __syncthreads();
-    int k = by_count ? found[2] : BINS;
-    // (the last bin of a range cut at 40 temperatures holds no weight: nothing to tell apart)
-    const bool cut_off = r.per_bin * (40.0f * r.temperature) <= BINS;
-    if (k == BINS - 1 && cut_off) k = BINS;
-    r.k = k;
-    r.need_k = k < BINS ? r.top_k - (int)above_k : 0;
-    r.before_k = k < BINS ? before[k] : 0;
-    r.whole = total;
-    r.lo = k;
-    r.hi = k;
-    if (by_weight) {
-      // the sum that top-p is of lies between those without and with all of bin k
-      const double least = (double)r.top_p * (double)before[k], most = (double)r.top_p * (double)before[k < BINS ? k + 1 : BINS];
-      const u64 want_lo = max((u64)1, (u64)__double2ll_ru(least)), want_hi = max((u64)1, (u64)__double2ll_ru(most));
-#pragma unroll
-      for (int j = 0; j < PER; ++j) {
-        const int b = t * PER + j;
-        if (before[b] < want_lo && before[b + 1] >= want_lo) found[0] = b;
-        if (before[b] < want_hi && before[b + 1] >= want_hi) found[1] = b;
-      }
-      __syncthreads();
-      r.lo = min(found[0], k);
-      r.hi = min(found[1], k);
-      r.before_lo = before[min(r.lo, BINS)];
-    }
-    if (k == BINS && !by_weight) r.state = kAll;  // (top-k takes all that has weight: its sums come in the next pass)
   }
-  if (t == 0) {
-    r.first = first;
-    *s.row = r;
+  u64 whole;
+  u64 up = block_before(in[0] + in[1], part, &whole);
+  // (the last bin of a range cut at 40 temperatures holds no weight: with fewer tokens
+  // before it than top-k keeps, those are all that count)
+  const bool far = r.per_bin * (40.0f * r.temperature) <= BINS;
+  const u64 want = r.top_k > 0 ? (u64)r.top_k : max((u64)1, (u64)__double2ll_ru((double)r.top_p * (double)whole));
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int b = 2 * t + j;
+    if (up < want && up + in[j] >= want) {
+      s.row->lo = r.top_k > 0 ? 0 : b;
+      s.row->hi = r.top_k > 0 && b == BINS - 1 && far ? BINS - 2 : b;
+      s.row->before = r.top_k > 0 ? 0 : up;
+      s.row->whole = whole;
+    }
+    up += in[j];
   }
 }
 
-// The tokens of the bins in which the filters end, and the sum of the certain ones.
-// Grid: (slices, rows).
+// The list's tokens, and the sums of the granules' certain ones. Grid: (slices, rows).
 __global__ __launch_bounds__(NT) void sample_list_kernel(const SampleArgs a, const SampleWork w) {
-  __shared__ u64 part[NT / 64], list[LIST];
+  constexpr unsigned HERE = 2048;
+  __shared__ u64 list[HERE];
   __shared__ unsigned listed, place;
   const int row = blockIdx.y, from = blockIdx.x * w.length, to = min(a.vocab, from + w.length);
   const float *const x = a.x + (long)row * a.vocab;
-  const Space s = space_of(w.space, row, w.slices);
+  const Space s = space_of(w, row);
   const Row r = *s.row;
-  if (r.state < kAll || (r.state == kAll && r.top_k == 0)) return;
+  if (r.state != kList) return;
   const Weigh weigh = weigh_of(r, w.shift);
-  const int lo = r.state == kAll ? BINS : r.lo;
   if (threadIdx.x == 0) listed = 0;
   __syncthreads();
   u64 sum = 0;
-  each(x, from, to, (reinterpret_cast<uintptr_t>(x) & 15) == 0, [&](int i, float v) {
-    const int b = bin_of(v, r.top, r.per_bin);
-    if (b < lo) {
-      sum += weigh.least(v);
-    } else if (b <= r.hi || b == r.k) {
-      const unsigned at = atomicAdd(&listed, 1u);
-      if (at < LIST) list[at] = (u64)sort_key(v) << 32 | ~(unsigned)i;
-    }
-  });
-  sum = block_sum(sum, part);
-  if (threadIdx.x == 0) {
-    s.kept[blockIdx.x] = sum;
-    place = listed ? atomicAdd(s.listed, listed) : 0;
-  }
+  each(
+      x, from, to,
+      [&](int i, float v) {
+        const int b = bin_of(v, r.top, r.per_bin);
+        if (b < r.lo) {
+          sum += weigh.least(v);
+        } else if (b <= r.hi) {
+          const u64 token = token_of(v, i);
+          unsigned at = atomicAdd(&listed, 1u);
+          if (at < HERE) {
+            list[at] = token;
+          } else if ((at = atomicAdd(s.listed, 1u)) < LIST) {
+            s.list[at] = token;
+          }
+        }
+      },
+      [&](int g) {
+        if (__any(sum != 0)) sum = wave_sum(sum);
+        if ((threadIdx.x & 63) == 0) s.kept[g] = sum;
+        sum = 0;
+      });
   __syncthreads();
-  for (unsigned i = threadIdx.x; i < min(listed, (unsigned)LIST); i += NT)
+  const unsigned here = min(listed, HERE);
+  if (threadIdx.x == 0) place = here ? atomicAdd(s.listed, here) : 0;
+  __syncthreads();
+  for (unsigned i = threadIdx.x; i < here; i += NT)
     if (place + i < LIST) s.list[place + i] = list[i];
 }
 
-// The last kept token from the list, the draw, and the token. Grid: rows.
+struct Select {
+  u64 sums[256], both[NT / 64][2], found, above;
+  unsigned counts[256], alone;
+};
+// The first token, from the largest down, at which the running sum of value(token), from
+// `base` on, reaches `want`. all(f): f(token) for the thread's tokens. Eight bits a
+// round, from the first in which any two differ, until one token is left.
+template <class All, class Value>
+__device__ u64 select(All all, Value value, u64 want, u64 base, Select &s) {
+  const int t = threadIdx.x;
+  u64 any = 0, every = ~0ull;
+  all([&](u64 e) {
+    any |= e;
+    every &= e;
+  });
+  for (int d = 32; d > 0; d >>= 1) {
+    any |= __shfl_xor(any, d);
+    every &= __shfl_xor(every, d);
+  }
+  __syncthreads();
+  if ((t & 63) == 0) {
+    s.both[t >> 6][0] = any;
+    s.both[t >> 6][1] = every;
+  }
+  __syncthreads();
+  for (int i = 0; i < NT / 64; ++i) {
+    any |= s.both[i][0];
+    every &= s.both[i][1];
+  }
+  int top = 64 - __clzll((long long)(any ^ every));  // undecided bits
+  if (any == every) return any;
+  u64 prefix = top == 64 ? 0 : any >> top;
+  while (top > 0) {
+    const int shift = max(0, top - 8);
+    const unsigned digits = (1u << (top - shift)) - 1;
+    if (t < 256) {
+      s.sums[t] = 0;
+      s.counts[t] = 0;
+    }
+    __syncthreads();
+    all([&](u64 e) {
+      if ((top == 64 ? 0 : e >> top) != prefix) return;
+      const unsigned d = (unsigned)(e >> shift) & digits;
+      const u64 v = value(e);
+      if (v) atomicAdd(&s.sums[d], v);
+      atomicAdd(&s.counts[d], 1u);
+    });
+    __syncthreads();
+    if (t < 64) {  // a lane's four digits, the largest in lane 0
+      u64 v[4], four = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) four += v[i] = s.sums[255 - 4 * t - i];
+      u64 up = four;
+      for (int d = 1; d < 64; d *= 2) {
+        const u64 o = __shfl_up(up, d);
+        if (t >= d) up += o;
+      }
+      u64 run = base + up - four;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (run < want && run + v[i] >= want) {
+          s.found = 255 - 4 * t - i;
+          s.above = run;
+          s.alone = s.counts[255 - 4 * t - i];
+        }
+        run += v[i];
+      }
+    }
+    __syncthreads();
+    prefix = prefix << (top - shift) | s.found;
+    base = s.above;
+    top = shift;
+    if (s.alone == 1) {
+      __syncthreads();
+      all([&](u64 e) {
+        if (e >> top == prefix) s.found = e;
+      });
+      __syncthreads();
+      return s.found;
+    }
+  }
+  return prefix;
+}
+
+// The last kept token, the draw, and the token. Grid: rows.
 __global__ __launch_bounds__(NT) void sample_draw_kernel(const SampleArgs a, const SampleWork w) {
-  __shared__ __attribute__((aligned(16))) u64 list[LIST];
-  __shared__ u64 part[NT / 64], hist[256];
-  __shared__ unsigned found;
-  __shared__ u64 above;
-  __shared__ u64 ends[2];
+  __shared__ u64 list[LIST], part[NT / 64], sums[NT], ends[2];
+  __shared__ Select choice;
   const int row = blockIdx.x, t = threadIdx.x, n = a.vocab;
   const float *const x = a.x + (long)row * n;
-  const Space s = space_of(w.space, row, w.slices);
+  const Space s = space_of(w, row);
   const Row r = *s.row;
   auto answer = [&](int token, float prob) {
     a.tokens[row] = token;
@@ -451,238 +511,146 @@ __global__ __launch_bounds__(NT) void sample_draw_kernel(const SampleArgs a, con
     return;
   }
   const Weigh weigh = weigh_of(r, w.shift);
-  unsigned last = 0;        // the last kept token's key,
-  unsigned last_at = UINT_MAX;  // and index: none of that key after it is kept
-  const unsigned listed = r.state == kList ? *s.listed : 0;
-  if (listed > LIST) {
-    // Eight bits of the keys a round, the highest first: the key at which the running
-    // sum from above (of `value` over keys above `floor`) reaches `want`, and what is above it.
-    auto select = [&](auto value, u64 want, unsigned floor, bool all, u64 *over) {
-      unsigned prefix = 0;
-      u64 sum = 0;
-      for (int at = 24; at >= 0; at -= 8) {
-        __syncthreads();
-        if (t < 256) hist[t] = 0;
-        __syncthreads();
-        for (int i = t; i < n; i += NT) {
-          const unsigned k = sort_key(x[i]);
-          if ((all || k > floor) && (at == 24 || k >> (at + 8) == prefix >> (at + 8))) atomicAdd(&hist[k >> at & 255], value(x[i]));
-        }
-        __syncthreads();
-        if (t == 0) {
-          u64 run = sum;
-          int b = 255;
-          while (b > 0 && run + hist[b] < want) run += hist[b--];
-          found = b;
-          above = run;
-        }
-        __syncthreads();
-        prefix |= found << at;
-        sum = above;
-      }
-      *over = sum;
-      return prefix;
-    };
-    u64 ties = ~0ull;  // tokens of the last key that stay
-    if (r.top_k > 0) {
-      u64 over;
-      last = select([](float) { return (u64)1; }, (u64)r.top_k, 0u, true, &over);
-      ties = (u64)r.top_k - over;
-    }
-    if (r.top_p < 1.0f) {
-      u64 wt = 0, same = 0;
-      for (int i = t; i < n; i += NT) {
-        const unsigned k = sort_key(x[i]);
-        if (k > last) wt += weigh(x[i]);
-        same += k == last;
-      }
-      const u64 over = block_sum(wt, part);
-      same = min(block_sum(same, part), ties);
-      const u64 one = last ? weigh(key_value(last)) : 0;
-      const u64 want = max((u64)1, (u64)__double2ll_ru((double)r.top_p * (double)(over + same * one)));
-      if (over < want) {
-        ties = min(same, one ? (want - over + one - 1) / one : same);
+  const int listed = r.state == kList ? (int)min(*s.listed, LIST + 1u) : 0;
+  const bool fits = listed <= LIST;
+  u64 last = 0;  // of the kept tokens
+  if (r.state == kList) {
+    if (fits)
+      for (int i = t; i < listed; i += NT) list[i] = s.list[i];
+    __syncthreads();
+    auto all = [&](auto f) {
+      if (fits) {
+        for (int i = t; i < listed; i += NT) f(list[i]);
       } else {
-        u64 before;
-        last = select([&](float v) { return weigh(v); }, want, last, false, &before);
-        const u64 each_one = max((u64)1, weigh(key_value(last)));
-        ties = (want - before + each_one - 1) / each_one;
+        for (int i = t; i < n; i += NT) f(token_of(x[i], i));
       }
-    }
-    // the index of the last of the ties
-    const int per = (n + NT - 1) / NT, from = min(n, t * per), to = min(n, from + per);
-    u64 same = 0, all;
-    for (int i = from; i < to; ++i) same += sort_key(x[i]) == last;
-    const u64 rank = block_before(same, part, &all);
-    if (t == 0) found = UINT_MAX;
-    __syncthreads();
-    if (rank < ties && rank + same >= ties) {
-      u64 left = ties - rank;
-      for (int i = from; i < to; ++i)
-        if (sort_key(x[i]) == last && --left == 0) found = (unsigned)i;
-    }
-    __syncthreads();
-    last_at = found;
-    // and the slices' sums, which the list would have had
-    for (int i = 0; i < w.slices; ++i) {
-      u64 sum = 0;
-      for (int j = i * w.length + t; j < min(n, (i + 1) * w.length); j += NT) {
-        const unsigned k = sort_key(x[j]);
-        if (k > last || (k == last && (unsigned)j <= last_at)) sum += weigh.least(x[j]);
-      }
-      sum = block_sum(sum, part);
-      if (t == 0) s.kept[i] = sum;
-    }
-    __syncthreads();
-    __threadfence_block();
-  } else if (listed > 0) {
-    // sorted: falling keys, rising indexes
-    int size = (int)listed;
-    if (size <= 2 * NT) {
-      // by each one's rank: none is there twice
-      u64 mine[2];
-      int rank[2] = {0, 0};
-#pragma unroll
-      for (int j = 0; j < 2; ++j) mine[j] = t + j * NT < size ? s.list[t + j * NT] : 0;
-#pragma unroll
-      for (int j = 0; j < 2; ++j) list[t + j * NT] = mine[j];
-      __syncthreads();
-      const ulonglong2 *const two = reinterpret_cast<const ulonglong2 *>(list);
-      for (int i = 0; i < (size + 1) / 2; ++i) {
-        const ulonglong2 v = two[i];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) rank[j] += (v.x > mine[j]) + (v.y > mine[j]);
-      }
-      __syncthreads();
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-        if (t + j * NT < size) list[rank[j]] = mine[j];
-    } else {
-      while (size & (size - 1)) size += size & -size;
-      for (int i = t; i < size; i += NT) list[i] = i < (int)listed ? s.list[i] : 0;
-      for (int k = 2; k <= size; k *= 2)
-        for (int j = k / 2; j > 0; j /= 2) {
-          __syncthreads();
-          for (int i = t; i < size / 2; i += NT) {
-            const int at = 2 * i - (i & (j - 1)), to = at + j;
-            const u64 p = list[at], q = list[to];
-            if ((p < q) == ((at & k) == 0)) {
-              list[at] = q;
-              list[to] = p;
-            }
-          }
-        }
-    }
-    __syncthreads();
-    // (a thread's run of the sorted list)
-    const int per = (size + NT - 1) / NT, from = min((int)listed, t * per), to = min((int)listed, from + per);
-    auto value_at = [&](int i) { return key_value((unsigned)(list[i] >> 32)); };
-    int end = (int)listed;  // tokens of the list that top-k keeps
-    if (r.k < BINS) {
-      // (those of bin k are the list's last)
-      u64 in = 0, all;
-      for (int i = from; i < to; ++i) in += bin_of(value_at(i), r.top, r.per_bin) == r.k;
-      block_before(in, part, &all);
-      end = (int)listed - (int)all + r.need_k;
-    }
-    int stop = end;
+    };
+    // (of fewer tokens with weight than top-k keeps, the last)
+    if (r.top_k > 0) last = select(all, [](u64) { return (u64)1; }, (u64)min(r.top_k, fits ? listed : n), 0, choice);
     if (r.top_p < 1.0f) {
-      // the sum that top-p is of: the bins before k, and what is kept of k (or all)
-      u64 in = 0, all, sum = 0;
-      for (int i = from; i < min(to, end); ++i) {
-        const u64 p = weigh(value_at(i));
-        sum += p;
-        if (r.k < BINS && bin_of(value_at(i), r.top, r.per_bin) == r.k) in += p;
+      auto left = [&](auto f) {
+        all([&](u64 e) {
+          if (e >= last) f(e);
+        });
+      };
+      auto value = [&](u64 e) { return weigh(logit_of(e)); };
+      u64 whole = r.whole;
+      if (r.top_k > 0 || !fits) {
+        whole = 0;
+        left([&](u64 e) { whole += value(e); });
+        whole = block_sum(whole, part);
       }
-      block_before(in, part, &all);
-      const u64 whole = r.k < BINS ? r.before_k + all : r.whole;
       const u64 want = max((u64)1, (u64)__double2ll_ru((double)r.top_p * (double)whole));
-      // (bins between hi and k are not in the list, nor does top-p end there)
-      u64 total;
-      const u64 up = block_before(sum, part, &total);
-      if (t == 0) found = (unsigned)end;
-      __syncthreads();
-      u64 run = r.before_lo + up;
-      for (int i = from; i < min(to, end); ++i) {
-        const u64 p = weigh(value_at(i));
-        if (run < want && run + p >= want) found = (unsigned)i + 1;
-        run += p;
-      }
-      __syncthreads();
-      stop = (int)found;
+      last = select(left, value, want, fits ? r.before : 0, choice);
     }
-    const u64 final = list[stop - 1];
-    last = (unsigned)(final >> 32);
-    last_at = ~(unsigned)final;
-    __syncthreads();
+    if (!fits) {  // the granules' sums, which the list would have completed
+      u64 sum = 0;
+      each(
+          x, 0, n,
+          [&](int i, float v) {
+            if (token_of(v, i) >= last) sum += weigh.least(v);
+          },
+          [&](int g) {
+            sum = wave_sum(sum);
+            if ((t & 63) == 0) s.kept[g] = sum;
+            sum = 0;
+          });
+      __threadfence_block();
+      __syncthreads();
+    }
   }
-  // The slices' sums with the list's kept tokens, and the draw.
-  u64 *const sums = hist;  // (up to 256 slices)
-  for (int i = t; i < w.slices; i += NT) sums[i] = s.kept[i];
+  // Threads' runs of granules, with the list's kept tokens, and the draw.
+  const int per = (w.granules + NT - 1) / NT, g0 = min(w.granules, t * per), g1 = min(w.granules, g0 + per);
+  u64 mine = 0;
+  for (int g = g0; g < g1; ++g) mine += s.kept[g];
+  sums[t] = mine;
   __syncthreads();
-  if (listed <= LIST)
-    for (int i = t; i < (int)listed; i += NT) {
-      const unsigned k = (unsigned)(list[i] >> 32), at = ~(unsigned)list[i];
-      if (k > last || (k == last && at <= last_at)) {
-        const u64 p = weigh.least(key_value(k));
-        if (p) atomicAdd(&sums[at / w.length], p);
+  auto each_listed = [&](auto see) {  // (in the list and kept)
+    for (int i = t; fits && i < listed; i += NT)
+      if (list[i] >= last) {
+        const u64 p = weigh.least(logit_of(list[i]));
+        if (p) see(index_of(list[i]) / GRANULE, p);
       }
-    }
+  };
+  each_listed([&](int g, u64 p) { atomicAdd(&sums[g / per], p); });
   __syncthreads();
   u64 total;
-  const u64 mine = t < w.slices ? sums[t] : 0, up = block_before(mine, part, &total);
+  mine = sums[t];
+  const u64 up = block_before(mine, part, &total);
   // (u times the sum rounds to what may be the sum itself: then the last of them)
   const u64 draw = min((u64)((double)r.u * (double)total), total - 1);
-  if (t < w.slices && draw >= up && draw < up + mine) {
+  if (draw >= up && draw < up + mine) {
     ends[0] = (u64)t;
     ends[1] = up;
   }
   __syncthreads();
-  const int begin = (int)ends[0] * w.length, finish = min(n, begin + w.length);
-  const int per = (w.length + NT - 1) / NT, from = min(finish, begin + t * per), to = min(finish, from + per);
-  auto kept = [&](int i) {
-    const float v = x[i];
-    const unsigned k = sort_key(v);
-    return k > last || (k == last && (unsigned)i <= last_at) ? weigh.least(v) : (u64)0;
-  };
-  u64 sum = 0, unused;
-  for (int i = from; i < to; ++i) sum += kept(i);
-  u64 run = ends[1] + block_before(sum, part, &unused);
-  if (draw < run || draw >= run + sum) return;
-  for (int i = from; i < to; ++i) {
-    const u64 p = kept(i);
-    run += p;
+  // The granule of that thread's.
+  const int first = (int)ends[0] * per;
+  u64 run = ends[1];
+  for (int i = t; i < per; i += NT) sums[i] = first + i < w.granules ? s.kept[first + i] : 0;
+  __syncthreads();
+  each_listed([&](int g, u64 p) {
+    if (g >= first && g < first + per) atomicAdd(&sums[g - first], p);
+  });
+  __syncthreads();
+  if (t >= 64) return;
+  int g = 0;
+  while (g + 1 < per && run + sums[g] <= draw) run += sums[g++];
+  // A lane's four of it.
+  const int from = (first + g) * GRANULE + 4 * t;
+  u64 p[4], four = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    p[i] = 0;
+    if (from + i < n) {
+      const float v = x[from + i];
+      if (token_of(v, from + i) >= last) p[i] = weigh.least(v);
+    }
+    four += p[i];
+  }
+  u64 sum = four;
+  for (int d = 1; d < 64; d *= 2) {
+    const u64 o = __shfl_up(sum, d);
+    if (t >= d) sum += o;
+  }
+  run += sum - four;
+  if (draw < run || draw >= run + four) return;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    run += p[i];
     if (run > draw) {
-      answer(i, (float)((double)p / (double)total));
+      answer(from + i, (float)((double)p[i] / (double)total));
       return;
     }
   }
 }
 
-// Slices of at least 4096 logits, for about two workgroups a CU.
-static void sample_slices(int rows, int vocab, int *slices, int *length) {
-  int n = std::max(1, std::min({(vocab + 4095) / 4096, (512 + rows - 1) / rows, 128}));
-  *length = ((vocab + n - 1) / n + 1023) & ~1023;
-  *slices = (vocab + *length - 1) / *length;
+// Rows of one round of launches: their workspaces take some hundred megabytes at most.
+constexpr int kRowsAtOnce = 1024;
+
+// Slices of at least 4096 logits, for up to four workgroups a CU.
+static SampleWork sample_work(int rows, int vocab) {
+  SampleWork w{};
+  rows = std::min(rows, kRowsAtOnce);
+  const int n = std::max(1, std::min({(vocab + 4095) / 4096, (1024 + rows - 1) / rows, 32}));
+  w.length = ((vocab + n - 1) / n + 1023) & ~1023;
+  w.slices = (vocab + w.length - 1) / w.length;
+  w.granules = (vocab + GRANULE - 1) / GRANULE;
+  w.row_bytes = row_bytes(w.slices, w.granules);
+  int bits = 0;
+  while (((long)1 << bits) < vocab) ++bits;
+  w.shift = std::min(62 - bits, 51);  // (sums stay below 2^62, weights below 2^52)
+  return w;
 }
 
-// Rows of one round of launches: their workspaces take some hundred megabytes at most.
-constexpr int kRowsAtOnce = 2048;
-
 size_t sample_workspace(int rows, int vocab) {
-  int slices, length;
-  sample_slices(std::min(rows, kRowsAtOnce), vocab, &slices, &length);
-  return (size_t)std::min(rows, kRowsAtOnce) * row_bytes(slices);
+  return (size_t)std::min(rows, kRowsAtOnce) * sample_work(rows, vocab).row_bytes;
 }
 
 hipError_t launch_sample(hipStream_t st, const SampleArgs &all, void *workspace) {
-  int bits = 0;
-  while (((long)1 << bits) < all.vocab) ++bits;
-  SampleWork w;
+  SampleWork w = sample_work(all.rows, all.vocab);
   w.space = (char *)workspace;
-  // (sums stay below 2^62, weights below 2^52)
-  w.shift = std::min(62 - bits, 51);
-  sample_slices(std::min(all.rows, kRowsAtOnce), all.vocab, &w.slices, &w.length);
+  const bool filters = all.d_top_k || all.d_top_p || all.top_p < 1.0f || (all.top_k > 0 && all.top_k < all.vocab);
   for (int first = 0; first < all.rows; first += kRowsAtOnce) {
     SampleArgs a = all;
     a.rows = std::min(kRowsAtOnce, all.rows - first);
@@ -697,8 +665,10 @@ hipError_t launch_sample(hipStream_t st, const SampleArgs &all, void *workspace)
     const dim3 grid(w.slices, a.rows);
     hipLaunchKernelGGL(sample_ends_kernel, grid, dim3(NT), 0, st, a, w);
     hipLaunchKernelGGL(sample_bins_kernel, grid, dim3(NT), 0, st, a, w);
-    hipLaunchKernelGGL(sample_cut_kernel, dim3(a.rows), dim3(NT), 0, st, a, w);
-    hipLaunchKernelGGL(sample_list_kernel, grid, dim3(NT), 0, st, a, w);
+    if (filters) {
+      hipLaunchKernelGGL(sample_cut_kernel, dim3(a.rows), dim3(NT), 0, st, a, w);
+      hipLaunchKernelGGL(sample_list_kernel, grid, dim3(NT), 0, st, a, w);
+    }
     hipLaunchKernelGGL(sample_draw_kernel, dim3(a.rows), dim3(NT), 0, st, a, w);
   }
   return hipGetLastError();
