@@ -33,7 +33,7 @@ namespace {
 
 typedef unsigned long long u64;
 
-constexpr int NT = 512, BINS = 1024, LIST = 8192, GRANULE = 256;
+constexpr int NT = 512, BINS = 1024, LIST = 8192, GRANULE = 256, FEW = 256;
 
 // Bits that rise with the value; both zeros alike.
 __device__ __forceinline__ unsigned sort_key(float x) {
@@ -70,13 +70,10 @@ struct Weigh {
     p = fma(p, r, 1.0);
     return __builtin_ldexp(p, (int)n + add);
   }
-  // The nearest whole number of 2^-shift (below 2^52: the sum's low bits are it).
-  __device__ __forceinline__ u64 operator()(float x) const {
-    return (u64)__double_as_longlong(real(x, shift) + 4503599627370496.0) & 0xfffffffffffffull;
-  }
-  __device__ __forceinline__ u64 least(float x) const {  // 0 below min_p
+  // The nearest whole number of 2^-shift (below 2^52: the sum's low bits are it), or 0 below `least`.
+  __device__ __forceinline__ u64 operator()(float x, double least) const {
     const double w = real(x, shift);
-    return w >= min_p ? (u64)__double_as_longlong(w + 4503599627370496.0) & 0xfffffffffffffull : 0;
+    return w >= least ? (u64)__double_as_longlong(w + 4503599627370496.0) & 0xfffffffffffffull : 0;
   }
 };
 
@@ -87,7 +84,7 @@ struct Slice {
 };
 // What a row's later passes go by.
 struct Row {
-  u64 whole, before;  // without top-k: weights of all, and of the bins before lo
+  u64 whole, before;  // weights of all, and of the bins before lo; for top-k counts, and those before hi
   float top, per_bin;
   float temperature, top_p, min_p, u;
   int top_k;          // 0: all
@@ -119,53 +116,82 @@ __device__ __forceinline__ int bin_of(float x, float top, float per_bin) {
   return t < BINS - 1 ? (int)t : BINS - 1;
 }
 
-// The granules of a slice by waves: f(index, logit) for a lane's four, then done(granule).
+// The sum of the lanes' values up to this one's, and of all.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ u64 dpp_of(u64 v) {
+  const unsigned lo = __builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
+  const unsigned hi = __builtin_amdgcn_update_dpp(0, (int)(v >> 32), CTRL, ROWS, 0xf, false);
+  return (u64)hi << 32 | lo;
+}
+__device__ __forceinline__ u64 wave_up_to(u64 v) {
+  v += dpp_of<0x111, 0xf>(v);  // within a row of 16 lanes, from 1, 2, 4 and 8 before
+  v += dpp_of<0x112, 0xf>(v);
+  v += dpp_of<0x114, 0xf>(v);
+  v += dpp_of<0x118, 0xf>(v);
+  v += dpp_of<0x142, 0xa>(v);  // a row's last to the next row
+  v += dpp_of<0x143, 0xc>(v);  // the first half's last to the second half
+  return v;
+}
+__device__ __forceinline__ u64 last_lane(u64 v) {
+  return (u64)(unsigned)__builtin_amdgcn_readlane((int)(v >> 32), 63) << 32 |
+         (unsigned)__builtin_amdgcn_readlane((int)v, 63);
+}
+__device__ __forceinline__ u64 wave_sum(u64 v) { return last_lane(wave_up_to(v)); }
+
+// The granules of a slice by waves: f(index, logit) for a lane's four, 64 apart, then
+// done(granule).
 template <class F, class G>
 __device__ __forceinline__ void each(const float *x, int from, int to, F f, G done) {
-  const bool vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0;
-  for (int g = from + (int)(threadIdx.x >> 6) * GRANULE; g < to; g += NT / 64 * GRANULE) {
-    const int i = g + 4 * (int)(threadIdx.x & 63);
-    if (vec && i + 4 <= to) {
-      const float4 v = *reinterpret_cast<const float4 *>(x + i);
-      f(i, v.x);
-      f(i + 1, v.y);
-      f(i + 2, v.z);
-      f(i + 3, v.w);
+  constexpr int STEP = NT / 64 * GRANULE;
+  const int lane = threadIdx.x & 63;
+  float next[4];
+  auto load = [&](int g) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) next[j] = x[min(g + 64 * j + lane, to - 1)];
+  };
+  int g = from + (int)(threadIdx.x >> 6) * GRANULE;
+  if (g < to) load(g);
+  for (; g < to; g += STEP) {
+    float v[4] = {next[0], next[1], next[2], next[3]};
+    if (g + STEP < to) load(g + STEP);
+    if (g + GRANULE <= to) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) f(g + 64 * j + lane, v[j]);
     } else {
-      for (int j = i; j < min(i + 4, to); ++j) f(j, x[j]);
+#pragma unroll 1
+      for (int i = g + lane; i < to; i += 64) {
+        f(i, v[0]);
+        v[0] = v[1];
+        v[1] = v[2];
+        v[2] = v[3];
+      }
     }
     done(g / GRANULE);
   }
 }
-__device__ __forceinline__ u64 wave_sum(u64 v) {
-  for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
+
+__device__ __forceinline__ u64 wave_least(u64 v) {
+  for (int d = 32; d > 0; d >>= 1) v = min(v, __shfl_xor(v, d));
   return v;
 }
 
-template <class T>
-__device__ T block_sum(T v, T *part) {
-  for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
+__device__ __forceinline__ u64 block_sum(u64 v, u64 *part) {
+  v = wave_sum(v);
   __syncthreads();
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
   __syncthreads();
-  T r = 0;
+  u64 r = 0;
   for (int i = 0; i < NT / 64; ++i) r += part[i];
   return r;
 }
 
 // The sum of the threads' values before this one's, and of all.
-template <class T>
-__device__ T block_before(T v, T *part, T *all) {
-  const int lane = threadIdx.x & 63;
-  T run = v;
-  for (int d = 1; d < 64; d *= 2) {
-    const T o = __shfl_up(run, d);
-    if (lane >= d) run += o;
-  }
+__device__ __forceinline__ u64 block_before(u64 v, u64 *part, u64 *all) {
+  const u64 run = wave_up_to(v);
   __syncthreads();
-  if (lane == 63) part[threadIdx.x >> 6] = run;
+  if ((threadIdx.x & 63) == 63) part[threadIdx.x >> 6] = run;
   __syncthreads();
-  T before = 0, total = 0;
+  u64 before = 0, total = 0;
   for (int i = 0; i < NT / 64; ++i) {
     if (i < (int)(threadIdx.x >> 6)) before += part[i];
     total += part[i];
@@ -215,17 +241,29 @@ __global__ __launch_bounds__(NT) void sample_ends_kernel(const SampleArgs a, con
   const int row = blockIdx.y, from = blockIdx.x * w.length, to = min(a.vocab, from + w.length);
   const float *const x = a.x + (long)row * a.vocab;
   Slice s{NEG_INF, __builtin_inff(), INT_MAX, 0};
-  each(
-      x, from, to,
-      [&](int i, float v) {
-        s.bad |= !(v < __builtin_inff());
-        if (v > s.most) {
-          s.most = v;
-          s.at = i;
-        }
-        s.least = fminf(s.least, v);
-      },
-      [](int) {});
+  auto see = [&](int i, float v) __attribute__((always_inline)) {
+    s.bad |= !(v < __builtin_inff());
+    if (v > s.most) {
+      s.most = v;
+      s.at = i;
+    }
+    s.least = fminf(s.least, v);
+  };
+  if ((reinterpret_cast<uintptr_t>(x) & 15) == 0) {
+#pragma unroll 2
+    for (int i = from + 4 * (int)threadIdx.x; i + 4 <= to; i += 4 * NT) {
+      const float4 v = *reinterpret_cast<const float4 *>(x + i);
+      see(i, v.x);
+      see(i + 1, v.y);
+      see(i + 2, v.z);
+      see(i + 3, v.w);
+    }
+    // (a lane's place of the last three)
+    const int i = (to & ~3) + (int)threadIdx.x;
+    if (i < to) see(i, x[i]);
+  } else {
+    for (int i = from + (int)threadIdx.x; i < to; i += NT) see(i, x[i]);
+  }
   auto join = [&](float most, float least, int at, int bad) {
     if (most > s.most || (most == s.most && at < s.at)) s.at = at;
     s.most = fmaxf(s.most, most);
@@ -287,32 +325,29 @@ __global__ __launch_bounds__(NT) void sample_bins_kernel(const SampleArgs a, con
   }
   if (r.state < kAll) return;
   const Weigh weigh = weigh_of(r, w.shift);
-  if (r.state == kAll) {
-    u64 sum = 0;
-    each(
-        x, from, to, [&](int, float v) { sum += weigh.least(v); },
-        [&](int g) {
-          sum = wave_sum(sum);
-          if ((threadIdx.x & 63) == 0) s.kept[g] = sum;
-          sum = 0;
-        });
-    return;
-  }
-  const bool by_count = r.top_k > 0;
+  const bool by_count = r.top_k > 0, sums = r.state == kAll;
   unsigned *const counts = reinterpret_cast<unsigned *>(weights);
   for (int i = threadIdx.x; i < BINS; i += NT) weights[i] = 0;
   __syncthreads();
   if (by_count) {
     each(x, from, to, [&](int, float v) { atomicAdd(&counts[bin_of(v, r.top, r.per_bin)], 1u); }, [](int) {});
   } else {
-    // (what has no weight, far down, would only meet in the last bin)
+    u64 sum = 0;
     each(
         x, from, to,
         [&](int, float v) {
-          const u64 p = weigh(v);
-          if (p) atomicAdd(&weights[bin_of(v, r.top, r.per_bin)], p);
+          const u64 p = weigh(v, sums ? weigh.min_p : 0.0);
+          sum += p;
+          // (what has no weight, far down, would only meet in the last bin)
+          if (!sums && p) atomicAdd(&weights[bin_of(v, r.top, r.per_bin)], p);
         },
-        [](int) {});
+        [&](int g) {
+          if (!sums) return;
+          sum = wave_sum(sum);
+          if ((threadIdx.x & 63) == 0) s.kept[g] = sum;
+          sum = 0;
+        });
+    if (sums) return;
   }
   __syncthreads();
   u64 *const to_bins = s.bins + (size_t)blockIdx.x * BINS;
@@ -357,7 +392,7 @@ __global__ __launch_bounds__(NT) void sample_cut_kernel(const SampleArgs a, cons
     if (up < want && up + in[j] >= want) {
       s.row->lo = r.top_k > 0 ? 0 : b;
       s.row->hi = r.top_k > 0 && b == BINS - 1 && far ? BINS - 2 : b;
-      s.row->before = r.top_k > 0 ? 0 : up;
+      s.row->before = up;
       s.row->whole = whole;
     }
     up += in[j];
@@ -383,7 +418,7 @@ __global__ __launch_bounds__(NT) void sample_list_kernel(const SampleArgs a, con
       [&](int i, float v) {
         const int b = bin_of(v, r.top, r.per_bin);
         if (b < r.lo) {
-          sum += weigh.least(v);
+          sum += weigh(v, weigh.min_p);
         } else if (b <= r.hi) {
           const u64 token = token_of(v, i);
           unsigned at = atomicAdd(&listed, 1u);
@@ -415,7 +450,7 @@ struct Select {
 // `base` on, reaches `want`. all(f): f(token) for the thread's tokens. Eight bits a
 // round, from the first in which any two differ, until one token is left.
 template <class All, class Value>
-__device__ u64 select(All all, Value value, u64 want, u64 base, Select &s) {
+__device__ __forceinline__ u64 select(All all, Value value, u64 want, u64 base, Select &s) {
   const int t = threadIdx.x;
   u64 any = 0, every = ~0ull;
   all([&](u64 e) {
@@ -459,12 +494,7 @@ __device__ u64 select(All all, Value value, u64 want, u64 base, Select &s) {
       u64 v[4], four = 0;
 #pragma unroll
       for (int i = 0; i < 4; ++i) four += v[i] = s.sums[255 - 4 * t - i];
-      u64 up = four;
-      for (int d = 1; d < 64; d *= 2) {
-        const u64 o = __shfl_up(up, d);
-        if (t >= d) up += o;
-      }
-      u64 run = base + up - four;
+      u64 run = base + wave_up_to(four) - four;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         if (run < want && run + v[i] >= want) {
@@ -491,14 +521,25 @@ __device__ u64 select(All all, Value value, u64 want, u64 base, Select &s) {
   return prefix;
 }
 
+// (a function of its own: a kernel that runs once waits for each line of its code)
+__device__ __attribute__((noinline)) u64 weigh_apart(Weigh weigh, float x, double least) { return weigh(x, least); }
+
 // The last kept token, the draw, and the token. Grid: rows.
 __global__ __launch_bounds__(NT) void sample_draw_kernel(const SampleArgs a, const SampleWork w) {
-  __shared__ u64 list[LIST], part[NT / 64], sums[NT], ends[2];
+  __shared__ u64 list[LIST], part[NT / 64], sums[NT], bins[BINS], few[FEW], values[FEW], runs[FEW], ends[2];
+  __shared__ unsigned ranks[FEW], many;
+  __shared__ int bin_found;
   __shared__ Select choice;
   const int row = blockIdx.x, t = threadIdx.x, n = a.vocab;
   const float *const x = a.x + (long)row * n;
   const Space s = space_of(w, row);
+  // (loads that wait for none: the row, the list's first tokens, a thread's run of granules)
   const Row r = *s.row;
+  const unsigned written = *s.listed;
+  const u64 token = s.list[t];
+  const int per = (w.granules + NT - 1) / NT, g0 = min(w.granules, t * per), g1 = min(w.granules, g0 + per);
+  u64 mine = 0;
+  for (int g = g0; g < g1; ++g) mine += s.kept[g];
   auto answer = [&](int token, float prob) {
     a.tokens[row] = token;
     if (a.probs) a.probs[row] = prob;
@@ -510,45 +551,140 @@ __global__ __launch_bounds__(NT) void sample_draw_kernel(const SampleArgs a, con
     }
     return;
   }
-  const Weigh weigh = weigh_of(r, w.shift);
-  const int listed = r.state == kList ? (int)min(*s.listed, LIST + 1u) : 0;
+  const Weigh weigher = weigh_of(r, w.shift);
+  auto weigh = [&](float v, double least) { return weigh_apart(weigher, v, least); };
+  const double min_p = weigher.min_p;
+  const int listed = r.state == kList ? (int)min(written, LIST + 1u) : 0;
   const bool fits = listed <= LIST;
   u64 last = 0;  // of the kept tokens
   if (r.state == kList) {
+    list[t] = token;
     if (fits)
-      for (int i = t; i < listed; i += NT) list[i] = s.list[i];
-    __syncthreads();
-    auto all = [&](auto f) {
-      if (fits) {
-        for (int i = t; i < listed; i += NT) f(list[i]);
-      } else {
-        for (int i = t; i < n; i += NT) f(token_of(x[i], i));
+      for (int i = t + NT; i < listed; i += NT) list[i] = s.list[i];
+    // The tokens of few[] before each of them, and their values' sum: a thread's share of
+    // the pairs, and what they come to for token t.
+    unsigned rank;
+    u64 run;
+    auto order = [&](int m) {
+      for (int c = t & 63; c < m; c += 64) {
+        const u64 e = few[c];
+        unsigned before = 0;
+        u64 sum = 0;
+#pragma unroll 4
+        for (int i = t >> 6; i < m; i += NT / 64) {
+          before += few[i] > e;
+          sum += few[i] > e ? values[i] : 0;
+        }
+        atomicAdd(&ranks[c], before);
+        atomicAdd(&runs[c], sum);
       }
+      __syncthreads();
+      rank = t < m ? ranks[t] : 0;
+      run = t < m ? runs[t] : 0;
     };
-    // (of fewer tokens with weight than top-k keeps, the last)
-    if (r.top_k > 0) last = select(all, [](u64) { return (u64)1; }, (u64)min(r.top_k, fits ? listed : n), 0, choice);
-    if (r.top_p < 1.0f) {
-      auto left = [&](auto f) {
-        all([&](u64 e) {
-          if (e >= last) f(e);
-        });
-      };
-      auto value = [&](u64 e) { return weigh(logit_of(e)); };
-      u64 whole = r.whole;
-      if (r.top_k > 0 || !fits) {
-        whole = 0;
-        left([&](u64 e) { whole += value(e); });
-        whole = block_sum(whole, part);
+    auto least_of = [&](u64 v) {
+      v = wave_least(v);
+      __syncthreads();
+      if ((t & 63) == 0) part[t >> 6] = v;
+      __syncthreads();
+      for (int i = 0; i < NT / 64; ++i) v = min(v, part[i]);
+      return v;
+    };
+    auto clear = [&]() {
+      if (t < FEW) {
+        ranks[t] = 0;
+        runs[t] = 0;
       }
-      const u64 want = max((u64)1, (u64)__double2ll_ru((double)r.top_p * (double)whole));
-      last = select(left, value, want, fits ? r.before : 0, choice);
+      if (t == 0) many = 0;
+    };
+    auto part_of = [&](u64 whole) { return max((u64)1, (u64)__double2ll_ru((double)r.top_p * (double)whole)); };
+    clear();
+    if (listed <= FEW) {  // both filters at once
+      u64 p = 0;
+      if (t < listed) {
+        few[t] = token;
+        values[t] = p = weigh(logit_of(token), 0.0);
+      }
+      __syncthreads();
+      order(listed);
+      const bool in = t < listed && (r.top_k == 0 || rank < (unsigned)r.top_k);
+      const u64 whole = r.top_k > 0 ? block_sum(in ? p : 0, part) : r.whole;
+      const bool kept = in && (r.top_p >= 1.0f || (r.top_k > 0 ? 0 : r.before) + run < part_of(whole));
+      last = least_of(kept ? token : ~0ull);
+    } else {
+      __syncthreads();
+      // Top-k's last token, then top-p's of what that leaves: each in a bin that is known
+      // or found, and of that bin's (of all, where the list is not whole) among few, or by
+      // bits of the order. (A list that top-k keeps all of has no last but all's.)
+      int bin = r.hi;
+      auto left = [&](auto f) __attribute__((always_inline)) {
+        const int count = fits ? listed : n;
+#pragma unroll 1
+        for (int i = t; i < count; i += NT) {
+          const u64 e = fits ? list[i] : token_of(x[i], i);
+          if (e >= last && (bin < 0 || bin_of(logit_of(e), r.top, r.per_bin) == bin)) f(e);
+        }
+      };
+      if (!fits) bin = -1;
+#pragma unroll 1
+      for (int filter = 0; filter < 2; ++filter) {
+        if (filter == 0 ? r.top_k == 0 || (fits && listed <= r.top_k) : r.top_p >= 1.0f) continue;
+        u64 want = (u64)r.top_k, base = fits ? r.before : 0;
+        if (filter == 1) {
+          u64 whole = r.whole;
+          if (!fits || r.top_k > 0) {
+            bin = -1;
+            base = whole = 0;
+            for (int i = t; i < BINS; i += NT) bins[i] = 0;
+            __syncthreads();
+            left([&](u64 e) {
+              const u64 p = weigh(logit_of(e), 0.0);
+              if (p) atomicAdd(&bins[bin_of(logit_of(e), r.top, r.per_bin)], p);
+            });
+            __syncthreads();
+            const u64 in[2] = {bins[2 * t], bins[2 * t + 1]};
+            u64 up = block_before(in[0] + in[1], part, &whole);
+            want = part_of(whole);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              if (up < want && up + in[j] >= want) {
+                bin_found = 2 * t + j;
+                ends[0] = up;
+              }
+              up += in[j];
+            }
+            __syncthreads();
+            bin = bin_found;
+            base = ends[0];
+          }
+          want = part_of(whole);
+        }
+        left([&](u64 e) {
+          const unsigned at = atomicAdd(&many, 1u);
+          if (at < FEW) {
+            few[at] = e;
+            values[at] = filter == 0 ? 1 : weigh(logit_of(e), 0.0);
+          }
+        });
+        __syncthreads();
+        const unsigned m = many;
+        if (m <= FEW) {
+          order((int)m);
+          last = least_of(t < (int)m && base + run < want ? few[t] : ~0ull);
+        } else {
+          last = select(left, [&](u64 e) { return filter == 0 ? 1 : weigh(logit_of(e), 0.0); }, want, base, choice);
+        }
+        __syncthreads();
+        clear();
+        __syncthreads();
+      }
     }
     if (!fits) {  // the granules' sums, which the list would have completed
       u64 sum = 0;
       each(
           x, 0, n,
           [&](int i, float v) {
-            if (token_of(v, i) >= last) sum += weigh.least(v);
+            if (token_of(v, i) >= last) sum += weigh(v, min_p);
           },
           [&](int g) {
             sum = wave_sum(sum);
@@ -557,18 +693,17 @@ __global__ __launch_bounds__(NT) void sample_draw_kernel(const SampleArgs a, con
           });
       __threadfence_block();
       __syncthreads();
+      mine = 0;
+      for (int g = g0; g < g1; ++g) mine += s.kept[g];
     }
   }
   // Threads' runs of granules, with the list's kept tokens, and the draw.
-  const int per = (w.granules + NT - 1) / NT, g0 = min(w.granules, t * per), g1 = min(w.granules, g0 + per);
-  u64 mine = 0;
-  for (int g = g0; g < g1; ++g) mine += s.kept[g];
   sums[t] = mine;
   __syncthreads();
   auto each_listed = [&](auto see) {  // (in the list and kept)
     for (int i = t; fits && i < listed; i += NT)
       if (list[i] >= last) {
-        const u64 p = weigh.least(logit_of(list[i]));
+        const u64 p = weigh(logit_of(list[i]), min_p);
         if (p) see(index_of(list[i]) / GRANULE, p);
       }
   };
@@ -587,41 +722,31 @@ __global__ __launch_bounds__(NT) void sample_draw_kernel(const SampleArgs a, con
   // The granule of that thread's.
   const int first = (int)ends[0] * per;
   u64 run = ends[1];
-  for (int i = t; i < per; i += NT) sums[i] = first + i < w.granules ? s.kept[first + i] : 0;
-  __syncthreads();
-  each_listed([&](int g, u64 p) {
-    if (g >= first && g < first + per) atomicAdd(&sums[g - first], p);
-  });
-  __syncthreads();
+  if (per > 1) {
+    for (int i = t; i < per; i += NT) sums[i] = first + i < w.granules ? s.kept[first + i] : 0;
+    __syncthreads();
+    each_listed([&](int g, u64 p) {
+      if (g >= first && g < first + per) atomicAdd(&sums[g - first], p);
+    });
+    __syncthreads();
+  }
   if (t >= 64) return;
   int g = 0;
   while (g + 1 < per && run + sums[g] <= draw) run += sums[g++];
-  // A lane's four of it.
-  const int from = (first + g) * GRANULE + 4 * t;
-  u64 p[4], four = 0;
+  // Its logits, 64 at a time.
+  const int from = (first + g) * GRANULE + t;
+  float v[GRANULE / 64];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    p[i] = 0;
-    if (from + i < n) {
-      const float v = x[from + i];
-      if (token_of(v, from + i) >= last) p[i] = weigh.least(v);
-    }
-    four += p[i];
-  }
-  u64 sum = four;
-  for (int d = 1; d < 64; d *= 2) {
-    const u64 o = __shfl_up(sum, d);
-    if (t >= d) sum += o;
-  }
-  run += sum - four;
-  if (draw < run || draw >= run + four) return;
+  for (int j = 0; j < GRANULE / 64; ++j) v[j] = x[min(from + 64 * j, n - 1)];
+#pragma unroll 1
+  for (int i = from, j = 0; j < GRANULE / 64; ++j, i += 64) {
+    const u64 p = i < n && token_of(v[0], i) >= last ? weigh(v[0], min_p) : 0;
+    const u64 sum = run + wave_up_to(p);
+    if (sum > draw && sum - p <= draw) answer(i, (float)((double)p / (double)total));
+    run = last_lane(sum);
+    if (run > draw) return;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    run += p[i];
-    if (run > draw) {
-      answer(from + i, (float)((double)p[i] / (double)total));
-      return;
-    }
+    for (int k = 1; k < GRANULE / 64; ++k) v[k - 1] = v[k];
   }
 }
 
