@@ -82,6 +82,11 @@ struct Slice {
   float most, least;
   int at, bad;
 };
+// (by value: the compiler puts what a choice takes by reference into scratch memory)
+__device__ __forceinline__ Slice joined(Slice a, Slice b) {
+  const int at = b.most > a.most ? +b.at : b.most == a.most ? min(a.at, b.at) : +a.at;
+  return Slice{fmaxf(a.most, b.most), fminf(a.least, b.least), at, a.bad | b.bad};
+}
 // What a row's later passes go by.
 struct Row {
   u64 whole, before;  // weights of all, and of the bins before lo; for top-k counts, and those before hi
@@ -233,13 +238,10 @@ __device__ __forceinline__ Space space_of(const SampleWork &w, int row) {
   return s;
 }
 
-}  // namespace
-
-// Grid: (slices, rows).
-__global__ __launch_bounds__(NT) void sample_ends_kernel(const SampleArgs a, const SampleWork w) {
+// The ends of x[from, to), for every thread; keep(index, logit) sees each once.
+template <class K>
+__device__ __forceinline__ Slice ends_of(const float *x, int from, int to, K keep) {
   __shared__ Slice part[NT / 64];
-  const int row = blockIdx.y, from = blockIdx.x * w.length, to = min(a.vocab, from + w.length);
-  const float *const x = a.x + (long)row * a.vocab;
   Slice s{NEG_INF, __builtin_inff(), INT_MAX, 0};
   auto see = [&](int i, float v) __attribute__((always_inline)) {
     s.bad |= !(v < __builtin_inff());
@@ -248,6 +250,7 @@ __global__ __launch_bounds__(NT) void sample_ends_kernel(const SampleArgs a, con
       s.at = i;
     }
     s.least = fminf(s.least, v);
+    keep(i, v);
   };
   if ((reinterpret_cast<uintptr_t>(x) & 15) == 0) {
 #pragma unroll 2
@@ -258,43 +261,23 @@ __global__ __launch_bounds__(NT) void sample_ends_kernel(const SampleArgs a, con
       see(i + 2, v.z);
       see(i + 3, v.w);
     }
-    // (a lane's place of the last three)
+    // (a lane's place of the last three; slices begin at multiples of four)
     const int i = (to & ~3) + (int)threadIdx.x;
     if (i < to) see(i, x[i]);
   } else {
+#pragma unroll 4
     for (int i = from + (int)threadIdx.x; i < to; i += NT) see(i, x[i]);
   }
-  auto join = [&](float most, float least, int at, int bad) {
-    if (most > s.most || (most == s.most && at < s.at)) s.at = at;
-    s.most = fmaxf(s.most, most);
-    s.least = fminf(s.least, least);
-    s.bad |= bad;
-  };
-  for (int d = 32; d > 0; d >>= 1) join(__shfl_xor(s.most, d), __shfl_xor(s.least, d), __shfl_xor(s.at, d), __shfl_xor(s.bad, d));
+  for (int d = 32; d > 0; d >>= 1)
+    s = joined(s, Slice{__shfl_xor(s.most, d), __shfl_xor(s.least, d), __shfl_xor(s.at, d), __shfl_xor(s.bad, d)});
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int i = 1; i < NT / 64; ++i) join(part[i].most, part[i].least, part[i].at, part[i].bad);
-    space_of(w, row).slices[blockIdx.x] = s;
-  }
+  for (int i = 0; i < NT / 64; ++i) s = joined(s, part[i]);
+  return s;
 }
 
-// A row's ends from its slices', its settings, and what is to be done; every thread gets it.
-__device__ __forceinline__ Row row_of(const SampleArgs &a, const SampleWork &w, const Space &s, int row) {
-  __shared__ Slice part[NT / 64];
-  Slice e{NEG_INF, __builtin_inff(), INT_MAX, 0};
-  auto join = [&](float most, float least, int at, int bad) {
-    if (most > e.most || (most == e.most && at < e.at)) e.at = at;
-    e.most = fmaxf(e.most, most);
-    e.least = fminf(e.least, least);
-    e.bad |= bad;
-  };
-  for (int i = threadIdx.x; i < w.slices; i += NT) join(s.slices[i].most, s.slices[i].least, s.slices[i].at, s.slices[i].bad);
-  for (int d = 32; d > 0; d >>= 1) join(__shfl_xor(e.most, d), __shfl_xor(e.least, d), __shfl_xor(e.at, d), __shfl_xor(e.bad, d));
-  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = e;
-  __syncthreads();
-  for (int i = 0; i < NT / 64; ++i) join(part[i].most, part[i].least, part[i].at, part[i].bad);
-  __syncthreads();
+// What is to be done for a row of these ends.
+__device__ __forceinline__ Row row_of(const SampleArgs &a, const Slice &e, int row) {
   Row r;
   const bool fine = settings(a, row, r);
   r.top = e.most;
@@ -311,6 +294,37 @@ __device__ __forceinline__ Row row_of(const SampleArgs &a, const SampleWork &w, 
   return r;
 }
 
+// The bins of the list, for r.lo and what follows from it: by the thread that holds, of
+// two bins each, the one where the filter ends.
+__device__ __forceinline__ void cut(const Row &r, const u64 (&in)[2], u64 *part, Row &to) {
+  u64 whole;
+  u64 up = block_before(in[0] + in[1], part, &whole);
+  // (the last bin of a range cut at 40 temperatures holds no weight: with fewer tokens
+  // before it than top-k keeps, those are all that count)
+  const bool far = r.per_bin * (40.0f * r.temperature) <= BINS;
+  const u64 want = r.top_k > 0 ? (u64)r.top_k : max((u64)1, (u64)__double2ll_ru((double)r.top_p * (double)whole));
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int b = 2 * (int)threadIdx.x + j;
+    if (up < want && up + in[j] >= want) {
+      to.lo = r.top_k > 0 ? 0 : b;
+      to.hi = r.top_k > 0 && b == BINS - 1 && far ? BINS - 2 : b;
+      to.before = up;
+      to.whole = whole;
+    }
+    up += in[j];
+  }
+}
+
+}  // namespace
+
+// Grid: (slices, rows).
+__global__ __launch_bounds__(NT) void sample_ends_kernel(const SampleArgs a, const SampleWork w) {
+  const int row = blockIdx.y, from = blockIdx.x * w.length, to = min(a.vocab, from + w.length);
+  const Slice s = ends_of(a.x + (long)row * a.vocab, from, to, [](int, float) {});
+  if (threadIdx.x == 0) space_of(w, row).slices[blockIdx.x] = s;
+}
+
 // The counts or weights of the slice's bins; without a filter the sums of its granules'
 // kept weights. Grid: (slices, rows).
 __global__ __launch_bounds__(NT) void sample_bins_kernel(const SampleArgs a, const SampleWork w) {
@@ -318,7 +332,13 @@ __global__ __launch_bounds__(NT) void sample_bins_kernel(const SampleArgs a, con
   const int row = blockIdx.y, from = blockIdx.x * w.length, to = min(a.vocab, from + w.length);
   const float *const x = a.x + (long)row * a.vocab;
   const Space s = space_of(w, row);
-  const Row r = row_of(a, w, s, row);
+  Slice e{NEG_INF, __builtin_inff(), INT_MAX, 0};
+  if ((int)(threadIdx.x & 63) < w.slices) e = s.slices[threadIdx.x & 63];
+  for (int d = 16; d > 0; d >>= 1)
+    e = joined(e, Slice{__shfl_xor(e.most, d), __shfl_xor(e.least, d), __shfl_xor(e.at, d), __shfl_xor(e.bad, d)});
+  // (the first half of the wave has them all)
+  e = Slice{__shfl(e.most, 0), __shfl(e.least, 0), __shfl(e.at, 0), __shfl(e.bad, 0)};
+  const Row r = row_of(a, e, row);
   if (blockIdx.x == 0 && threadIdx.x == 0) {
     *s.listed = 0;
     *s.row = r;
@@ -380,23 +400,7 @@ __global__ __launch_bounds__(NT) void sample_cut_kernel(const SampleArgs a, cons
       in[1] += v.y;
     }
   }
-  u64 whole;
-  u64 up = block_before(in[0] + in[1], part, &whole);
-  // (the last bin of a range cut at 40 temperatures holds no weight: with fewer tokens
-  // before it than top-k keeps, those are all that count)
-  const bool far = r.per_bin * (40.0f * r.temperature) <= BINS;
-  const u64 want = r.top_k > 0 ? (u64)r.top_k : max((u64)1, (u64)__double2ll_ru((double)r.top_p * (double)whole));
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int b = 2 * t + j;
-    if (up < want && up + in[j] >= want) {
-      s.row->lo = r.top_k > 0 ? 0 : b;
-      s.row->hi = r.top_k > 0 && b == BINS - 1 && far ? BINS - 2 : b;
-      s.row->before = up;
-      s.row->whole = whole;
-    }
-    up += in[j];
-  }
+  cut(r, in, part, *s.row);
 }
 
 // The list's tokens, and the sums of the granules' certain ones. Grid: (slices, rows).
@@ -524,12 +528,157 @@ __device__ __forceinline__ u64 select(All all, Value value, u64 want, u64 base, 
 // (a function of its own: a kernel that runs once waits for each line of its code)
 __device__ __attribute__((noinline)) u64 weigh_apart(Weigh weigh, float x, double least) { return weigh(x, least); }
 
+// What a workgroup needs to find the last kept token.
+struct Choice {
+  u64 part[NT / 64], bins[BINS], few[FEW], values[FEW], runs[FEW], ends[2];
+  unsigned ranks[FEW], many;
+  int bin;
+  Select select;
+};
+// The last kept token of a row from its list (in LDS, not yet waited for), or, where it is
+// not whole, from all of its logits, at(index).
+template <class W, class A>
+__device__ __forceinline__ u64 last_kept(const Row &r, W weigh, const u64 *list, int listed, bool fits, int n, A at,
+                                         Choice &c) {
+  const int t = threadIdx.x;
+  // The tokens of few[] before each of them, and their values' sum: a thread's share of
+  // the pairs, and what they come to for token t.
+  unsigned rank;
+  u64 run;
+  auto order = [&](int m) {
+    for (int j = t & 63; j < m; j += 64) {
+      const u64 e = c.few[j];
+      unsigned before = 0;
+      u64 sum = 0;
+#pragma unroll 4
+      for (int i = t >> 6; i < m; i += NT / 64) {
+        before += c.few[i] > e;
+        sum += c.few[i] > e ? c.values[i] : 0;
+      }
+      atomicAdd(&c.ranks[j], before);
+      atomicAdd(&c.runs[j], sum);
+    }
+    __syncthreads();
+    rank = t < m ? c.ranks[t] : 0;
+    run = t < m ? c.runs[t] : 0;
+  };
+  auto least_of = [&](u64 v) {
+    v = wave_least(v);
+    __syncthreads();
+    if ((t & 63) == 0) c.part[t >> 6] = v;
+    __syncthreads();
+    for (int i = 0; i < NT / 64; ++i) v = min(v, c.part[i]);
+    return v;
+  };
+  auto clear = [&]() {
+    if (t < FEW) {
+      c.ranks[t] = 0;
+      c.runs[t] = 0;
+    }
+    if (t == 0) c.many = 0;
+  };
+  auto part_of = [&](u64 whole) { return max((u64)1, (u64)__double2ll_ru((double)r.top_p * (double)whole)); };
+  clear();
+  __syncthreads();
+  if (listed <= FEW) {  // both filters at once
+    u64 p = 0, token = 0;
+    if (t < listed) {
+      c.few[t] = token = list[t];
+      c.values[t] = p = weigh(logit_of(token), 0.0);
+    }
+    __syncthreads();
+    order(listed);
+    const bool in = t < listed && (r.top_k == 0 || rank < (unsigned)r.top_k);
+    const u64 whole = r.top_k > 0 ? block_sum(in ? p : 0, c.part) : r.whole;
+    const bool kept = in && (r.top_p >= 1.0f || (r.top_k > 0 ? 0 : r.before) + run < part_of(whole));
+    return least_of(kept ? token : ~0ull);
+  }
+  // Top-k's last token, then top-p's of what that leaves: each in a bin that is known or
+  // found, and of that bin's (of all, where the list is not whole) among few, or by bits of
+  // the order. (A list that top-k keeps all of has no last but all's.)
+  u64 last = 0;
+  int bin = fits ? r.hi : -1;
+  auto left = [&](auto f) __attribute__((always_inline)) {
+    const int count = fits ? listed : n;
+#pragma unroll 1
+    for (int i = t; i < count; i += NT) {
+      const u64 e = fits ? list[i] : token_of(at(i), i);
+      if (e >= last && (bin < 0 || bin_of(logit_of(e), r.top, r.per_bin) == bin)) f(e);
+    }
+  };
+#pragma unroll 1
+  for (int filter = 0; filter < 2; ++filter) {
+    if (filter == 0 ? r.top_k == 0 || (fits && listed <= r.top_k) : r.top_p >= 1.0f) continue;
+    u64 want = (u64)r.top_k, base = fits ? r.before : 0;
+    if (filter == 1) {
+      u64 whole = r.whole;
+      if (!fits || r.top_k > 0) {
+        bin = -1;
+        for (int i = t; i < BINS; i += NT) c.bins[i] = 0;
+        __syncthreads();
+        left([&](u64 e) {
+          const u64 p = weigh(logit_of(e), 0.0);
+          if (p) atomicAdd(&c.bins[bin_of(logit_of(e), r.top, r.per_bin)], p);
+        });
+        __syncthreads();
+        const u64 in[2] = {c.bins[2 * t], c.bins[2 * t + 1]};
+        u64 up = block_before(in[0] + in[1], c.part, &whole);
+        want = part_of(whole);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          if (up < want && up + in[j] >= want) {
+            c.bin = 2 * t + j;
+            c.ends[0] = up;
+          }
+          up += in[j];
+        }
+        __syncthreads();
+        bin = c.bin;
+        base = c.ends[0];
+      }
+      want = part_of(whole);
+    }
+    left([&](u64 e) {
+      const unsigned place = atomicAdd(&c.many, 1u);
+      if (place < FEW) {
+        c.few[place] = e;
+        c.values[place] = filter == 0 ? 1 : weigh(logit_of(e), 0.0);
+      }
+    });
+    __syncthreads();
+    const unsigned m = c.many;
+    if (m <= FEW) {
+      order((int)m);
+      last = least_of(t < (int)m && base + run < want ? c.few[t] : ~0ull);
+    } else {
+      last = select(left, [&](u64 e) { return filter == 0 ? 1 : weigh(logit_of(e), 0.0); }, want, base, c.select);
+    }
+    __syncthreads();
+    clear();
+    __syncthreads();
+  }
+  return last;
+}
+
+// Whether a row is answered already.
+__device__ __forceinline__ bool answered(const SampleArgs &a, const Row &r, int row) {
+  if (r.state != kBad && r.state != kGreedy) return false;
+  if (threadIdx.x == 0) {
+    if (r.state == kBad) atomicOr(a.err, kDevErrSampling);
+    a.tokens[row] = r.state == kBad ? -1 : r.first;
+    if (a.probs) a.probs[row] = r.state == kBad ? 0.0f : 1.0f;
+  }
+  return true;
+}
+// (u times the sum rounds to what may be the sum itself: then the last of them)
+__device__ __forceinline__ u64 drawn(const Row &r, u64 total) {
+  return min((u64)((double)r.u * (double)total), total - 1);
+}
+
 // The last kept token, the draw, and the token. Grid: rows.
 __global__ __launch_bounds__(NT) void sample_draw_kernel(const SampleArgs a, const SampleWork w) {
-  __shared__ u64 list[LIST], part[NT / 64], sums[NT], bins[BINS], few[FEW], values[FEW], runs[FEW], ends[2];
-  __shared__ unsigned ranks[FEW], many;
-  __shared__ int bin_found;
-  __shared__ Select choice;
+  __shared__ u64 list[LIST], sums[NT];
+  __shared__ Choice choice;
   const int row = blockIdx.x, t = threadIdx.x, n = a.vocab;
   const float *const x = a.x + (long)row * n;
   const Space s = space_of(w, row);
@@ -540,17 +689,7 @@ __global__ __launch_bounds__(NT) void sample_draw_kernel(const SampleArgs a, con
   const int per = (w.granules + NT - 1) / NT, g0 = min(w.granules, t * per), g1 = min(w.granules, g0 + per);
   u64 mine = 0;
   for (int g = g0; g < g1; ++g) mine += s.kept[g];
-  auto answer = [&](int token, float prob) {
-    a.tokens[row] = token;
-    if (a.probs) a.probs[row] = prob;
-  };
-  if (r.state == kBad || r.state == kGreedy) {
-    if (t == 0) {
-      if (r.state == kBad) atomicOr(a.err, kDevErrSampling);
-      r.state == kBad ? answer(-1, 0.0f) : answer(r.first, 1.0f);
-    }
-    return;
-  }
+  if (answered(a, r, row)) return;
   const Weigh weigher = weigh_of(r, w.shift);
   auto weigh = [&](float v, double least) { return weigh_apart(weigher, v, least); };
   const double min_p = weigher.min_p;
@@ -561,124 +700,7 @@ __global__ __launch_bounds__(NT) void sample_draw_kernel(const SampleArgs a, con
     list[t] = token;
     if (fits)
       for (int i = t + NT; i < listed; i += NT) list[i] = s.list[i];
-    // The tokens of few[] before each of them, and their values' sum: a thread's share of
-    // the pairs, and what they come to for token t.
-    unsigned rank;
-    u64 run;
-    auto order = [&](int m) {
-      for (int c = t & 63; c < m; c += 64) {
-        const u64 e = few[c];
-        unsigned before = 0;
-        u64 sum = 0;
-#pragma unroll 4
-        for (int i = t >> 6; i < m; i += NT / 64) {
-          before += few[i] > e;
-          sum += few[i] > e ? values[i] : 0;
-        }
-        atomicAdd(&ranks[c], before);
-        atomicAdd(&runs[c], sum);
-      }
-      __syncthreads();
-      rank = t < m ? ranks[t] : 0;
-      run = t < m ? runs[t] : 0;
-    };
-    auto least_of = [&](u64 v) {
-      v = wave_least(v);
-      __syncthreads();
-      if ((t & 63) == 0) part[t >> 6] = v;
-      __syncthreads();
-      for (int i = 0; i < NT / 64; ++i) v = min(v, part[i]);
-      return v;
-    };
-    auto clear = [&]() {
-      if (t < FEW) {
-        ranks[t] = 0;
-        runs[t] = 0;
-      }
-      if (t == 0) many = 0;
-    };
-    auto part_of = [&](u64 whole) { return max((u64)1, (u64)__double2ll_ru((double)r.top_p * (double)whole)); };
-    clear();
-    if (listed <= FEW) {  // both filters at once
-      u64 p = 0;
-      if (t < listed) {
-        few[t] = token;
-        values[t] = p = weigh(logit_of(token), 0.0);
-      }
-      __syncthreads();
-      order(listed);
-      const bool in = t < listed && (r.top_k == 0 || rank < (unsigned)r.top_k);
-      const u64 whole = r.top_k > 0 ? block_sum(in ? p : 0, part) : r.whole;
-      const bool kept = in && (r.top_p >= 1.0f || (r.top_k > 0 ? 0 : r.before) + run < part_of(whole));
-      last = least_of(kept ? token : ~0ull);
-    } else {
-      __syncthreads();
-      // Top-k's last token, then top-p's of what that leaves: each in a bin that is known
-      // or found, and of that bin's (of all, where the list is not whole) among few, or by
-      // bits of the order. (A list that top-k keeps all of has no last but all's.)
-      int bin = r.hi;
-      auto left = [&](auto f) __attribute__((always_inline)) {
-        const int count = fits ? listed : n;
-#pragma unroll 1
-        for (int i = t; i < count; i += NT) {
-          const u64 e = fits ? list[i] : token_of(x[i], i);
-          if (e >= last && (bin < 0 || bin_of(logit_of(e), r.top, r.per_bin) == bin)) f(e);
-        }
-      };
-      if (!fits) bin = -1;
-#pragma unroll 1
-      for (int filter = 0; filter < 2; ++filter) {
-        if (filter == 0 ? r.top_k == 0 || (fits && listed <= r.top_k) : r.top_p >= 1.0f) continue;
-        u64 want = (u64)r.top_k, base = fits ? r.before : 0;
-        if (filter == 1) {
-          u64 whole = r.whole;
-          if (!fits || r.top_k > 0) {
-            bin = -1;
-            base = whole = 0;
-            for (int i = t; i < BINS; i += NT) bins[i] = 0;
-            __syncthreads();
-            left([&](u64 e) {
-              const u64 p = weigh(logit_of(e), 0.0);
-              if (p) atomicAdd(&bins[bin_of(logit_of(e), r.top, r.per_bin)], p);
-            });
-            __syncthreads();
-            const u64 in[2] = {bins[2 * t], bins[2 * t + 1]};
-            u64 up = block_before(in[0] + in[1], part, &whole);
-            want = part_of(whole);
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              if (up < want && up + in[j] >= want) {
-                bin_found = 2 * t + j;
-                ends[0] = up;
-              }
-              up += in[j];
-            }
-            __syncthreads();
-            bin = bin_found;
-            base = ends[0];
-          }
-          want = part_of(whole);
-        }
-        left([&](u64 e) {
-          const unsigned at = atomicAdd(&many, 1u);
-          if (at < FEW) {
-            few[at] = e;
-            values[at] = filter == 0 ? 1 : weigh(logit_of(e), 0.0);
-          }
-        });
-        __syncthreads();
-        const unsigned m = many;
-        if (m <= FEW) {
-          order((int)m);
-          last = least_of(t < (int)m && base + run < want ? few[t] : ~0ull);
-        } else {
-          last = select(left, [&](u64 e) { return filter == 0 ? 1 : weigh(logit_of(e), 0.0); }, want, base, choice);
-        }
-        __syncthreads();
-        clear();
-        __syncthreads();
-      }
-    }
+    last = last_kept(r, weigh, list, listed, fits, n, [&](int i) { return x[i]; }, choice);
     if (!fits) {  // the granules' sums, which the list would have completed
       u64 sum = 0;
       each(
@@ -711,17 +733,16 @@ __global__ __launch_bounds__(NT) void sample_draw_kernel(const SampleArgs a, con
   __syncthreads();
   u64 total;
   mine = sums[t];
-  const u64 up = block_before(mine, part, &total);
-  // (u times the sum rounds to what may be the sum itself: then the last of them)
-  const u64 draw = min((u64)((double)r.u * (double)total), total - 1);
+  const u64 up = block_before(mine, choice.part, &total);
+  const u64 draw = drawn(r, total);
   if (draw >= up && draw < up + mine) {
-    ends[0] = (u64)t;
-    ends[1] = up;
+    choice.ends[0] = (u64)t;
+    choice.ends[1] = up;
   }
   __syncthreads();
   // The granule of that thread's.
-  const int first = (int)ends[0] * per;
-  u64 run = ends[1];
+  const int first = (int)choice.ends[0] * per;
+  u64 run = choice.ends[1];
   if (per > 1) {
     for (int i = t; i < per; i += NT) sums[i] = first + i < w.granules ? s.kept[first + i] : 0;
     __syncthreads();
@@ -742,13 +763,107 @@ __global__ __launch_bounds__(NT) void sample_draw_kernel(const SampleArgs a, con
   for (int i = from, j = 0; j < GRANULE / 64; ++j, i += 64) {
     const u64 p = i < n && token_of(v[0], i) >= last ? weigh(v[0], min_p) : 0;
     const u64 sum = run + wave_up_to(p);
-    if (sum > draw && sum - p <= draw) answer(i, (float)((double)p / (double)total));
+    if (sum > draw && sum - p <= draw) {
+      a.tokens[row] = i;
+      if (a.probs) a.probs[row] = (float)((double)p / (double)total);
+    }
     run = last_lane(sum);
     if (run > draw) return;
 #pragma unroll
     for (int k = 1; k < GRANULE / 64; ++k) v[k - 1] = v[k];
   }
 }
+
+// All of it for rows of at most ROW logits, held in LDS, a workgroup each: the same steps
+// over the same numbers (granules are of 64 logits). Grid: rows.
+template <int ROW>
+__global__ __launch_bounds__(NT) void sample_row_kernel(const SampleArgs a, const int shift) {
+  constexpr int HERE = 1536;  // (with 8192 logits 61 KB: two workgroups a CU)
+  static_assert(ROW <= 64 * NT, "a granule a thread");
+  __shared__ float held[ROW];
+  __shared__ u64 list[HERE];
+  __shared__ Choice c;
+  __shared__ Row cut_row;
+  __shared__ unsigned written;
+  const int row = blockIdx.x, t = threadIdx.x, n = a.vocab;
+  for (int i = t; i < BINS; i += NT) c.bins[i] = 0;
+  if (t == 0) written = 0;
+  const Slice e = ends_of(a.x + (long)row * n, 0, n, [&](int i, float v) { held[i] = v; });
+  Row r = row_of(a, e, row);
+  if (answered(a, r, row)) return;
+  const Weigh weigher = weigh_of(r, shift);
+  auto weigh = [&](float v, double least) { return weigh_apart(weigher, v, least); };
+  u64 last = 0;
+  if (r.state == kList) {
+    unsigned *const counts = reinterpret_cast<unsigned *>(c.bins);
+    if (r.top_k > 0) {
+#pragma unroll 4
+      for (int i = t; i < n; i += NT) atomicAdd(&counts[bin_of(held[i], r.top, r.per_bin)], 1u);
+    } else {
+#pragma unroll 4
+      for (int i = t; i < n; i += NT) {
+        const u64 p = weigher(held[i], 0.0);
+        if (p) atomicAdd(&c.bins[bin_of(held[i], r.top, r.per_bin)], p);
+      }
+    }
+    __syncthreads();
+    u64 in[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) in[j] = r.top_k > 0 ? counts[2 * t + j] : c.bins[2 * t + j];
+    cut(r, in, c.part, cut_row);
+    __syncthreads();
+    r.lo = cut_row.lo;
+    r.hi = cut_row.hi;
+    r.before = cut_row.before;
+    r.whole = cut_row.whole;
+#pragma unroll 4
+    for (int i = t; i < n; i += NT) {
+      const int b = bin_of(held[i], r.top, r.per_bin);
+      if (b >= r.lo && b <= r.hi) {
+        const unsigned at = atomicAdd(&written, 1u);
+        if (at < HERE) list[at] = token_of(held[i], i);
+      }
+    }
+    __syncthreads();
+    const int listed = (int)written;
+    last = last_kept(r, weigh, list, listed, listed <= HERE, n, [&](int i) { return held[i]; }, c);
+  }
+  // The granules' sums, the draw and its granule.
+  u64 *const sums = c.bins;
+  __syncthreads();
+  sums[t] = 0;
+  __syncthreads();
+#pragma unroll 1
+  for (int i = t; i - (t & 63) < n; i += NT) {
+    u64 p = 0;
+    if (i < n && token_of(held[i], i) >= last) p = weigher(held[i], weigher.min_p);
+    if (__any(p != 0)) {
+      p = wave_sum(p);
+      if ((t & 63) == 0) sums[i >> 6] = p;
+    }
+  }
+  __syncthreads();
+  u64 total;
+  const u64 mine = sums[t], up = block_before(mine, c.part, &total), draw = drawn(r, total);
+  if (draw >= up && draw < up + mine) {
+    c.ends[0] = (u64)t;
+    c.ends[1] = up;
+  }
+  __syncthreads();
+  if (t >= 64) return;
+  const int i = 64 * (int)c.ends[0] + t;
+  const u64 p = i < n && token_of(held[min(i, n - 1)], i) >= last ? weigh(held[min(i, n - 1)], weigher.min_p) : 0;
+  const u64 sum = c.ends[1] + wave_up_to(p);
+  if (sum > draw && sum - p <= draw) {
+    a.tokens[row] = i;
+    if (a.probs) a.probs[row] = (float)((double)p / (double)total);
+  }
+}
+
+// Longest row that one workgroup takes. (One row of 1000, 4096, 8192 and 16000 logits with
+// all filters: 9, 12, 15 and 19 us against 17, 18, 19 and 20 in slices; by top-p alone 8, 12,
+// 18 and 28 us against 17, 19, 21 and 21.)
+constexpr int kRow = 8192;
 
 // Rows of one round of launches: their workspaces take some hundred megabytes at most.
 constexpr int kRowsAtOnce = 1024;
@@ -769,6 +884,7 @@ static SampleWork sample_work(int rows, int vocab) {
 }
 
 size_t sample_workspace(int rows, int vocab) {
+  if (vocab <= kRow) return 0;
   return (size_t)std::min(rows, kRowsAtOnce) * sample_work(rows, vocab).row_bytes;
 }
 
@@ -787,6 +903,10 @@ hipError_t launch_sample(hipStream_t st, const SampleArgs &all, void *workspace)
     if (a.d_min_p) a.d_min_p += first;
     a.tokens += first;
     if (a.probs) a.probs += first;
+    if (a.vocab <= kRow) {
+      hipLaunchKernelGGL((sample_row_kernel<kRow>), dim3(a.rows), dim3(NT), 0, st, a, w.shift);
+      continue;
+    }
     const dim3 grid(w.slices, a.rows);
     hipLaunchKernelGGL(sample_ends_kernel, grid, dim3(NT), 0, st, a, w);
     hipLaunchKernelGGL(sample_bins_kernel, grid, dim3(NT), 0, st, a, w);

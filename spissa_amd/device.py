@@ -62,11 +62,17 @@ def _dev_i32(t, name: str) -> int:
     return t.data_ptr()
 
 
+_i32 = None  # torch.int32, once such a device tensor has been seen
+
+
 def _many_i32(t, count: int, name: str) -> int:
-    p = _dev_i32(t, name)
-    if t is None or t.numel() < count or not t.is_contiguous():
+    global _i32
+    if _i32 is None:
+        _dev_i32(t, name)  # (the small calls are as long as their checks: no import in them)
+        _i32 = None if t is None else t.dtype
+    if not getattr(t, "is_cuda", False) or t.dtype is not _i32 or t.numel() < count or not t.is_contiguous():
         raise TypeError(f"{name} must be a contiguous int32 device tensor of {count} elements")
-    return p
+    return t.data_ptr()
 
 
 def _many_f32(t, count: int, name: str) -> int:
@@ -390,11 +396,10 @@ class Session:
         device tensors: path [sum(nodes)] and count, next_token [len(nodes)] from parents,
         tokens and sampled [sum(nodes)]."""
         n, b = sum(nodes), len(nodes)
-        ins = [_many_i32(t, n, name) if n else 0
-               for t, name in ((parents, "parents"), (tokens, "tokens"), (sampled, "sampled"), (path, "path"))]
         check(self._lib.spissa_tree_accept_device(
-            self.handle, *ins[:3], (_ffi.c_size * max(1, b))(*nodes), b, ins[3],
-            _many_i32(count, b, "count") if b else 0, _many_i32(next_token, b, "next_token") if b else 0))
+            self.handle, n and _many_i32(parents, n, "parents"), n and _many_i32(tokens, n, "tokens"),
+            n and _many_i32(sampled, n, "sampled"), (_ffi.c_size * max(1, b))(*nodes), b, n and _many_i32(path, n, "path"),
+            b and _many_i32(count, b, "count"), b and _many_i32(next_token, b, "next_token")))
 
     def keep_rows(self, caches: Sequence[KvCache], nodes: Sequence[int], path, count) -> None:
         """Moves the accepted nodes' rows together (spissa_kv_cache_keep_device): caches are those
