@@ -595,7 +595,7 @@ __device__ __forceinline__ u64 last_kept(const Row &r, W weigh, const u64 *list,
   }
   // Top-k's last token, then top-p's of what that leaves: each in a bin that is known or
   // found, and of that bin's (of all, where the list is not whole) among few, or by bits of
-  // the order. (A list that top-k keeps all of has no last but all's.)
+  // the order. (With fewer listed than top-k keeps, no other token has weight: see cut().)
   u64 last = 0;
   int bin = fits ? r.hi : -1;
   auto left = [&](auto f) __attribute__((always_inline)) {
@@ -608,7 +608,7 @@ __device__ __forceinline__ u64 last_kept(const Row &r, W weigh, const u64 *list,
   };
 #pragma unroll 1
   for (int filter = 0; filter < 2; ++filter) {
-    if (filter == 0 ? r.top_k == 0 || (fits && listed <= r.top_k) : r.top_p >= 1.0f) continue;
+    if (filter == 0 ? r.top_k == 0 || (fits && listed < r.top_k) : r.top_p >= 1.0f) continue;
     u64 want = (u64)r.top_k, base = fits ? r.before : 0;
     if (filter == 1) {
       u64 whole = r.whole;

@@ -250,3 +250,82 @@ def test_two_captured_calls_in_turn_with_eager_ones(gpu):
                 ses.sample(st["x"], st["u"], st["cfg"], eager)
                 ses.sync()
                 assert np.array_equal(eager.cpu().numpy(), got[0])
+
+
+HARD = [(1.0, 20000, 1.0, 0.0), (0.8, 20000, 0.9, 0.0), (0.8, 9000, 1.0, 0.001), (1.5, 1000, 0.7, 0.0), (50.0, 0, 0.3, 0.0),
+        (1.0, 300, 0.999, 0.0), (1e-4, 5000, 0.9, 0.0), (0.05, 257, 1.0, 0.0), (1.0, 256, 0.5, 0.0), (20.0, 12000, 0.99, 0.0)]
+
+
+@pytest.mark.parametrize("vocab", [300, 1537, 8191, 8192, 8193, 40001, 131073, 300001])
+@pytest.mark.parametrize("kind", ["plain", "ties", "flat", "equal"])
+def test_limits_among_thousands(s, vocab, kind):
+    """Lists that fill, overflow, or end among many equal tokens, on either side of the longest row of one workgroup."""
+    print(f"[case] sample vocab={vocab} {kind} limits among thousands", flush=True)
+    rng = np.random.default_rng(vocab + len(kind))
+    x = logits(rng, len(HARD), vocab, kind)
+    u = np.minimum(rng.random(len(HARD)), 1 - 2.0 ** -24).astype(np.float32)
+    compare(x, u, HARD, run(s, x, u, HARD))
+    s.sync()
+
+
+def test_the_longest_rows(s):
+    """2^22 logits a row: runs of several granules a thread."""
+    rng = np.random.default_rng(22)
+    x = logits(rng, 4, 1 << 22, "plain")
+    rows = [(1.0, 0, 1.0, 0.0), (0.9, 50, 0.95, 0.0), (1.2, 0, 0.9, 0.0), (3.0, 20000, 0.9, 0.0)]
+    for u in ([0.0, 0.25, 0.5, 0.999], [0.75, 0.9, 0.125, 0.3]):
+        compare(x, u, rows, run(s, x, u, rows))
+    s.sync()
+
+
+@pytest.mark.parametrize("n,vocab", [(1025, 9001), (2049, 1000), (65535, 5)])
+def test_more_rows_than_a_round_of_launches(s, n, vocab):
+    rng = np.random.default_rng(n)
+    x = logits(rng, 16, vocab, "plain")[np.arange(n) % 16]
+    u = np.minimum(rng.random(n), 1 - 2.0 ** -24).astype(np.float32)
+    rows = [ROWS[i % 7] for i in range(n)]
+    tokens, probs = run(s, x, u, rows)
+    at = np.unique(np.concatenate([[0, 1022, 1023, 1024, n - 1], rng.integers(0, n, 20)]))
+    compare(x[at], u[at], [rows[i] for i in at], (tokens[at], probs[at]))
+    assert (tokens >= 0).all() and (tokens < vocab).all()
+    s.sync()
+
+
+def test_two_sessions_at_once():
+    """Two sessions of two threads and streams: workspaces of their own, and the same tokens as alone."""
+    import threading
+
+    import torch
+
+    from spissa_amd.device import SamplingConfig, Session
+
+    rng = np.random.default_rng(6)
+    x = torch.as_tensor(logits(rng, 8, 50001, "plain"), device="cuda")
+    u = torch.as_tensor(rng.random(8).astype(np.float32), device="cuda")
+    cfgs = [SamplingConfig(0.9, 40, 0.9, 0.0), SamplingConfig(1.2, 0, 0.8, 0.01)]
+    torch.cuda.synchronize()
+    want, got, failed = [None] * 2, [[], []], []
+
+    def work(i, rounds):
+        try:
+            stream = torch.cuda.Stream()
+            ses = Session(0, stream=stream)
+            with torch.cuda.stream(stream):
+                for _ in range(rounds):
+                    t = torch.zeros(8, dtype=torch.int32, device="cuda")
+                    ses.sample(x, u, cfgs[i], t)
+                    got[i].append(t)
+                ses.sync()
+        except Exception as e:  # (shown by the main thread)
+            failed.append(e)
+
+    for i in range(2):
+        work(i, 1)
+        want[i] = got[i].pop().tolist()
+    threads = [threading.Thread(target=work, args=(i, 30)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
+    assert all(t.tolist() == want[i] for i in range(2) for t in got[i])
