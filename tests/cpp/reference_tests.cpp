@@ -833,6 +833,109 @@ TEST(fused_decode_step_matches_dropin_sequence) {
 
 }  // namespace
 
+// Decoding with drafted tokens: zero queries weigh what a node sees alike, and means of
+// whole numbers below 16 show which rows that was.
+TEST(drafted_tokens_on_device) {
+  const size_t Hq = 4, Hkv = 2, D = 64, P = 5, N = 4, W = Hkv * D;
+  auto session = ok(Session::create(0));
+  std::vector<float> k((P + N) * W), v(k.size());
+  for (size_t i = 0; i < k.size(); ++i) {
+    k[i] = (float)(i % 13);
+    v[i] = (float)((i * 5 + i / W) % 16);
+  }
+  auto cache = ok(session.kv_cache(Hkv, D, P + N));
+  ok(cache.append(slice(k, 0, P * W), slice(v, 0, P * W), P));
+  // node 0; 1 and 2 after it; 3 after 2
+  const std::vector<int32_t> parents{-1, 0, 0, 2}, tokens{9, 4, 7, 5}, sampled{7, 1, 5, 3};
+  float *dq = nullptr, *dk = nullptr, *dv = nullptr, *dout = nullptr;
+  int32_t *dp = nullptr, *dt = nullptr, *ds = nullptr, *path = nullptr, *count = nullptr, *next = nullptr;
+  CHECK(hipMalloc(&dq, N * Hq * D * 4) == hipSuccess && hipMalloc(&dk, N * W * 4) == hipSuccess &&
+        hipMalloc(&dv, N * W * 4) == hipSuccess && hipMalloc(&dout, N * Hq * D * 4) == hipSuccess);
+  for (int32_t **p : {&dp, &dt, &ds, &path, &count, &next}) CHECK(hipMalloc(p, N * 4) == hipSuccess);
+  CHECK(hipMemset(dq, 0, N * Hq * D * 4) == hipSuccess);
+  CHECK(hipMemcpy(dk, k.data() + P * W, N * W * 4, hipMemcpyHostToDevice) == hipSuccess);
+  CHECK(hipMemcpy(dv, v.data() + P * W, N * W * 4, hipMemcpyHostToDevice) == hipSuccess);
+  CHECK(hipMemcpy(dp, parents.data(), N * 4, hipMemcpyHostToDevice) == hipSuccess);
+  CHECK(hipMemcpy(dt, tokens.data(), N * 4, hipMemcpyHostToDevice) == hipSuccess);
+  CHECK(hipMemcpy(ds, sampled.data(), N * 4, hipMemcpyHostToDevice) == hipSuccess);
+  CHECK(hipDeviceSynchronize() == hipSuccess);
+  const KvAttentionConfig config{N, Hq, Hkv, D, true};
+  ok(session.tree_step(nullptr, dq, dk, dv, {&cache}, {N}, dp, config, dout));
+  ok(session.sync());
+  CHECK(cache.len() == P + N && cache.keys() == k && cache.values() == v);
+  std::vector<float> got(N * Hq * D), expected(got.size());
+  CHECK(hipMemcpy(got.data(), dout, got.size() * 4, hipMemcpyDeviceToHost) == hipSuccess);
+  for (size_t t = 0; t < N; ++t) {
+    std::vector<size_t> rows;
+    for (size_t i = 0; i < P; ++i) rows.push_back(i);
+    for (int a = (int)t; a >= 0; a = parents[a]) rows.push_back(P + a);
+    for (size_t h = 0; h < Hq; ++h)
+      for (size_t d = 0; d < D; ++d)
+        for (size_t i : rows)
+          expected[(t * Hq + h) * D + d] += v[i * W + h / (Hq / Hkv) * D + d] / (float)rows.size();
+  }
+  assert_close_vec(got, expected, 15.0f * 0x1p-20f);  // sixteen roundings of 2^-24 of 15
+
+  ok(session.tree_accept(dp, dt, ds, {N}, path, count, next));
+  ok(session.keep_rows({&cache}, {N}, path, count));
+  ok(session.sync());
+  std::vector<int32_t> ints(N);
+  CHECK(hipMemcpy(ints.data(), path, N * 4, hipMemcpyDeviceToHost) == hipSuccess);
+  CHECK((ints == std::vector<int32_t>{0, 2, 3, -1}));
+  int32_t one[2];
+  CHECK(hipMemcpy(one, count, 4, hipMemcpyDeviceToHost) == hipSuccess);
+  CHECK(hipMemcpy(one + 1, next, 4, hipMemcpyDeviceToHost) == hipSuccess);
+  CHECK(one[0] == 3 && one[1] == 3);
+  ok(cache.truncate(P + 3));
+  for (auto &rows : {std::pair(cache.keys(), k), std::pair(cache.values(), v)}) {
+    std::vector<float> kept = slice(rows.second, 0, (P + 1) * W);
+    for (size_t node : {2, 3}) kept.insert(kept.end(), rows.second.begin() + (P + node) * W, rows.second.begin() + (P + node + 1) * W);
+    CHECK(rows.first == kept);
+  }
+  CHECK(session.tree_step(nullptr, dq, dk, dv, {&cache}, {N, 1}, dp, config, dout).error().kind == ErrorKind::Shape);
+  CHECK(session.keep_rows({&cache, &cache}, {1}, path, count).error().kind == ErrorKind::Argument);
+  for (float *p : {dq, dk, dv, dout}) (void)hipFree(p);
+  for (int32_t *p : {dp, dt, ds, path, count, next}) (void)hipFree(p);
+}
+
+TEST(sampling_on_device) {
+  const size_t rows = 3, vocab = 5;
+  auto session = ok(Session::create(0));
+  // weights 1, 1/2, 0, 1/4, 1/4 of the largest
+  const float ln2 = std::log(2.0f), none = -INFINITY;
+  std::vector<float> logits;
+  for (size_t r = 0; r < rows; ++r) for (float x : {0.0f, -ln2, none, -2 * ln2, -2 * ln2}) logits.push_back(x);
+  const std::vector<float> u{0.0f, 0.6f, 0.99f};
+  float *dx = nullptr, *du = nullptr, *probs = nullptr;
+  int32_t *tokens = nullptr;
+  CHECK(hipMalloc(&dx, logits.size() * 4) == hipSuccess && hipMalloc(&du, rows * 4) == hipSuccess &&
+        hipMalloc(&probs, rows * 4) == hipSuccess && hipMalloc(&tokens, rows * 4) == hipSuccess);
+  CHECK(hipMemcpy(dx, logits.data(), logits.size() * 4, hipMemcpyHostToDevice) == hipSuccess);
+  CHECK(hipMemcpy(du, u.data(), rows * 4, hipMemcpyHostToDevice) == hipSuccess);
+  CHECK(hipDeviceSynchronize() == hipSuccess);
+  auto run = [&](float temperature, size_t top_k, float top_p, float min_p) {
+    const spissa_sampling_config cfg{rows, vocab, temperature, top_k, top_p, min_p, nullptr, nullptr, nullptr, nullptr};
+    ok(session.sample(dx, du, cfg, tokens, probs));
+    ok(session.sync());
+    std::vector<int32_t> got(rows);
+    CHECK(hipMemcpy(got.data(), tokens, rows * 4, hipMemcpyDeviceToHost) == hipSuccess);
+    return got;
+  };
+  typedef std::vector<int32_t> Ints;
+  CHECK((run(1.0f, 0, 1.0f, 0.0f) == Ints{0, 1, 4}));
+  std::vector<float> share(rows);
+  CHECK(hipMemcpy(share.data(), probs, rows * 4, hipMemcpyDeviceToHost) == hipSuccess);
+  assert_close_vec(share, {0.5f, 0.25f, 0.125f}, 0x1p-22f);  // logits and shares rounded to f32
+  CHECK((run(0.0f, 0, 1.0f, 0.0f) == Ints{0, 0, 0}));
+  CHECK((run(1.0f, 3, 1.0f, 0.0f) == Ints{0, 1, 3}));
+  CHECK((run(1.0f, 0, 0.7f, 0.0f) == Ints{0, 0, 1}));
+  CHECK((run(1.0f, 0, 1.0f, 0.4f) == Ints{0, 0, 1}));
+  const spissa_sampling_config bad{rows, vocab, -1.0f, 0, 1.0f, 0.0f, nullptr, nullptr, nullptr, nullptr};
+  CHECK(session.sample(dx, du, bad, tokens).error().kind == ErrorKind::InvalidTensorData);
+  for (float *p : {dx, du, probs}) (void)hipFree(p);
+  (void)hipFree(tokens);
+}
+
 int main(int argc, char **argv) {
   bool host_only = false, list = false;
   for (int i = 1; i < argc; ++i) {

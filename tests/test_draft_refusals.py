@@ -62,3 +62,10 @@ def test_null_handles():
     assert lib.spissa_kv_cache_keep_device(None, None, 1, counts, 1, None, None) == _ffi.ERR_SHAPE
     counts[0] = 3
     assert lib.spissa_kv_cache_keep_device(None, None, 1 << 63, (_ffi.c_size * 2)(3, 3), 2, None, None) == _ffi.ERR_SHAPE
+
+
+def test_the_rust_settings_follow_the_header():
+    from tests.test_integration_recipe import LIB_RS, c_struct_fields, rust_struct_fields
+
+    assert rust_struct_fields("spissa_sampling_config") == c_struct_fields("spissa_sampling_config")
+    assert "#[repr(C)]" in LIB_RS.split("pub struct spissa_sampling_config")[0][-80:]
