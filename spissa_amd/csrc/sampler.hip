@@ -8,19 +8,25 @@
 // single precision would move the borders of some hundred thousand tokens by 2^-24, and
 // one row in a hundred would come out another token).
 //
-// A row's logits are read three times, by workgroups of a slice each:
+// A row's logits are read three times, by workgroups of a slice each (sample_ends_kernel,
+// sample_bins_kernel, sample_list_kernel):
 //   1. the slice's largest and smallest logit;
 //   2. the counts (for top-k) or else the weights (for top-p) of 1024 bins of (max - x),
 //      fine enough that few tokens share the bin in which the filter ends;
 //   3. with that bin known: into a list the tokens that have to be put in order (all of
 //      the top-k's bins, or those of the bin where top-p ends), and the sums of the
 //      weights certain to be kept, by granules of 256 logits.
-// Between and after them a workgroup a row finds the bin, then the last kept token in the
-// list (of some hundred), by bits of their order, draws, and walks the granule in which the
-// draw falls. A row whose list would not fit (thousands of tokens in a thousandth of the
-// logits' range, or a top-k of thousands) is done in the same way over the whole row.
-// Without filters the first, second and last steps are enough. Bound by latency for a
-// few rows; for many by the reads and by the weights' 30 operations in 64 bits a token.
+// Then a workgroup a row (sample_draw_kernel) finds the last kept token in the list (of
+// some hundred), draws, and walks the granule in which the draw falls. A row whose list
+// would not fit (thousands of tokens in a thousandth of the logits' range, or a top-k of
+// thousands) is done in the same way over the whole row. Without filters the third launch
+// is left out, and up to 8192 logits are one workgroup's from start to end
+// (sample_row_kernel).
+//
+// Bound by latency for a few rows (one of 128256 logits, all filters: 19 us, four launches
+// of 4 to 6 us each); for many by reads and by the weights' 35 operations in 64 bits a
+// token: 64 rows of 128256 with settings of their own 48 us (9, 15, 14 and 15 us a launch;
+// 33 MB), five rows of 262144 without filters 15 us.
 #include <algorithm>
 #include <climits>
 
@@ -207,10 +213,10 @@ __device__ __forceinline__ u64 block_before(u64 v, u64 *part, u64 *all) {
 
 // A row's share of the workspace.
 struct Space {
-  Row *row;
+  Row *row, *cut;   // before and after the filters' bin is known
   unsigned *listed; // tokens of the list (beyond LIST: not all of them there)
   u64 *list;        // [LIST]: key, and the index's complement
-  u64 *bins;        // [slices][BINS] weights or, half as long, counts
+  u64 *bins;        // [BINS] weights or, half as long, counts
   u64 *kept;        // [granules]: weights certain to be kept
   Slice *slices;
 };
@@ -221,19 +227,20 @@ struct SampleWork {
   int granules;
   int shift;
 };
-constexpr size_t kRowHead = 80;
+constexpr size_t kRowHead = 80;  // of each of the two
 static_assert(sizeof(Row) <= kRowHead && kRowHead % 16 == 0, "a row's head");
 inline size_t row_bytes(int slices, int granules) {
-  return kRowHead + 16 + LIST * 8 + (size_t)slices * (BINS * 8 + sizeof(Slice)) + ((size_t)granules * 8 + 15) / 16 * 16;
+  return 2 * kRowHead + 16 + LIST * 8 + BINS * 8 + (size_t)slices * sizeof(Slice) + ((size_t)granules * 8 + 15) / 16 * 16;
 }
 __device__ __forceinline__ Space space_of(const SampleWork &w, int row) {
   char *const p = w.space + row * w.row_bytes;
   Space s;
   s.row = reinterpret_cast<Row *>(p);
-  s.listed = reinterpret_cast<unsigned *>(p + kRowHead);
-  s.list = reinterpret_cast<u64 *>(p + kRowHead + 16);
+  s.cut = reinterpret_cast<Row *>(p + kRowHead);
+  s.listed = reinterpret_cast<unsigned *>(p + 2 * kRowHead);
+  s.list = reinterpret_cast<u64 *>(p + 2 * kRowHead + 16);
   s.bins = s.list + LIST;
-  s.slices = reinterpret_cast<Slice *>(s.bins + (size_t)w.slices * BINS);
+  s.slices = reinterpret_cast<Slice *>(s.bins + BINS);
   s.kept = reinterpret_cast<u64 *>(s.slices + w.slices);
   return s;
 }
@@ -318,15 +325,19 @@ __device__ __forceinline__ void cut(const Row &r, const u64 (&in)[2], u64 *part,
 
 }  // namespace
 
+// The slices' ends; clears the bins. Reads at 4 TB/s (64 rows of 128256: 33 MB in 9 us).
 // Grid: (slices, rows).
 __global__ __launch_bounds__(NT) void sample_ends_kernel(const SampleArgs a, const SampleWork w) {
   const int row = blockIdx.y, from = blockIdx.x * w.length, to = min(a.vocab, from + w.length);
   const Slice s = ends_of(a.x + (long)row * a.vocab, from, to, [](int, float) {});
-  if (threadIdx.x == 0) space_of(w, row).slices[blockIdx.x] = s;
+  const Space space = space_of(w, row);
+  if (threadIdx.x == 0) space.slices[blockIdx.x] = s;
+  for (int i = blockIdx.x * NT + threadIdx.x; i < BINS; i += w.slices * NT) space.bins[i] = 0;
 }
 
 // The counts or weights of the slice's bins; without a filter the sums of its granules'
-// kept weights. Grid: (slices, rows).
+// kept weights. Slices' bins meet in memory (one array a slice and a launch a row that
+// summed them: 2.6 us more for one row, 1.4 for 64). Grid: (slices, rows).
 __global__ __launch_bounds__(NT) void sample_bins_kernel(const SampleArgs a, const SampleWork w) {
   __shared__ u64 weights[BINS];
   const int row = blockIdx.y, from = blockIdx.x * w.length, to = min(a.vocab, from + w.length);
@@ -342,6 +353,7 @@ __global__ __launch_bounds__(NT) void sample_bins_kernel(const SampleArgs a, con
   if (blockIdx.x == 0 && threadIdx.x == 0) {
     *s.listed = 0;
     *s.row = r;
+    *s.cut = r;
   }
   if (r.state < kAll) return;
   const Weigh weigh = weigh_of(r, w.shift);
@@ -370,49 +382,40 @@ __global__ __launch_bounds__(NT) void sample_bins_kernel(const SampleArgs a, con
     if (sums) return;
   }
   __syncthreads();
-  u64 *const to_bins = s.bins + (size_t)blockIdx.x * BINS;
-  for (int i = threadIdx.x; i < (by_count ? BINS / 2 : BINS); i += NT) to_bins[i] = weights[i];
-}
-
-// The bin in which the filter ends. Grid: rows.
-__global__ __launch_bounds__(NT) void sample_cut_kernel(const SampleArgs a, const SampleWork w) {
-  __shared__ u64 part[NT / 64];
-  static_assert(BINS == 2 * NT, "a thread has two bins");
-  const int row = blockIdx.x, t = threadIdx.x;
-  const Space s = space_of(w, row);
-  const Row r = *s.row;
-  if (r.state != kList) return;
-  u64 in[2] = {0, 0};
-  if (r.top_k > 0) {
-    const uint2 *const counts = reinterpret_cast<const uint2 *>(s.bins) + t;
-#pragma unroll 16
-    for (int i = 0; i < w.slices; ++i) {
-      const uint2 v = counts[(size_t)i * BINS];
-      in[0] += v.x;
-      in[1] += v.y;
-    }
-  } else {
-    const ulonglong2 *const weights = reinterpret_cast<const ulonglong2 *>(s.bins) + t;
-#pragma unroll 16
-    for (int i = 0; i < w.slices; ++i) {
-      const ulonglong2 v = weights[(size_t)i * NT];
-      in[0] += v.x;
-      in[1] += v.y;
+  // (whole numbers: the order of the slices changes nothing)
+  for (int i = threadIdx.x; i < BINS; i += NT) {
+    if (by_count) {
+      if (counts[i]) atomicAdd(reinterpret_cast<unsigned *>(s.bins) + i, counts[i]);
+    } else {
+      if (weights[i]) atomicAdd(&s.bins[i], weights[i]);
     }
   }
-  cut(r, in, part, *s.row);
 }
 
-// The list's tokens, and the sums of the granules' certain ones. Grid: (slices, rows).
+// The bin where the filter ends (by every workgroup for itself), the list's tokens, and the
+// sums of the granules' certain ones. Grid: (slices, rows).
 __global__ __launch_bounds__(NT) void sample_list_kernel(const SampleArgs a, const SampleWork w) {
   constexpr unsigned HERE = 2048;
-  __shared__ u64 list[HERE];
+  __shared__ u64 list[HERE], part[NT / 64];
   __shared__ unsigned listed, place;
+  __shared__ Row ends;
+  static_assert(BINS == 2 * NT, "a thread has two bins");
   const int row = blockIdx.y, from = blockIdx.x * w.length, to = min(a.vocab, from + w.length);
   const float *const x = a.x + (long)row * a.vocab;
   const Space s = space_of(w, row);
-  const Row r = *s.row;
+  // (counts lie in the first half of the bins)
+  const ulonglong2 weights = reinterpret_cast<const ulonglong2 *>(s.bins)[threadIdx.x];
+  const uint2 counts = reinterpret_cast<const uint2 *>(s.bins)[threadIdx.x];
+  Row r = *s.row;
   if (r.state != kList) return;
+  const u64 in[2] = {r.top_k > 0 ? (u64)counts.x : weights.x, r.top_k > 0 ? (u64)counts.y : weights.y};
+  cut(r, in, part, ends);
+  __syncthreads();
+  r.lo = ends.lo;
+  r.hi = ends.hi;
+  r.before = ends.before;
+  r.whole = ends.whole;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *s.cut = r;
   const Weigh weigh = weigh_of(r, w.shift);
   if (threadIdx.x == 0) listed = 0;
   __syncthreads();
@@ -660,7 +663,7 @@ __device__ __forceinline__ u64 last_kept(const Row &r, W weigh, const u64 *list,
   return last;
 }
 
-// Whether a row is answered already.
+// Whether a row is answered already (and, if so, its answer).
 __device__ __forceinline__ bool answered(const SampleArgs &a, const Row &r, int row) {
   if (r.state != kBad && r.state != kGreedy) return false;
   if (threadIdx.x == 0) {
@@ -675,7 +678,9 @@ __device__ __forceinline__ u64 drawn(const Row &r, u64 total) {
   return min((u64)((double)r.u * (double)total), total - 1);
 }
 
-// The last kept token, the draw, and the token. Grid: rows.
+// The last kept token, the draw, and the token. A chain of loads and sums over the
+// workgroup: 5.6 us with up to 256 listed, 15 with a thousand in an end bin of equal ones.
+// Grid: rows.
 __global__ __launch_bounds__(NT) void sample_draw_kernel(const SampleArgs a, const SampleWork w) {
   __shared__ u64 list[LIST], sums[NT];
   __shared__ Choice choice;
@@ -683,7 +688,7 @@ __global__ __launch_bounds__(NT) void sample_draw_kernel(const SampleArgs a, con
   const float *const x = a.x + (long)row * n;
   const Space s = space_of(w, row);
   // (loads that wait for none: the row, the list's first tokens, a thread's run of granules)
-  const Row r = *s.row;
+  const Row r = *s.cut;
   const unsigned written = *s.listed;
   const u64 token = s.list[t];
   const int per = (w.granules + NT - 1) / NT, g0 = min(w.granules, t * per), g1 = min(w.granules, g0 + per);
@@ -783,7 +788,7 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(const SampleArgs a, cons
   __shared__ float held[ROW];
   __shared__ u64 list[HERE];
   __shared__ Choice c;
-  __shared__ Row cut_row;
+  __shared__ Row found;
   __shared__ unsigned written;
   const int row = blockIdx.x, t = threadIdx.x, n = a.vocab;
   for (int i = t; i < BINS; i += NT) c.bins[i] = 0;
@@ -810,12 +815,12 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(const SampleArgs a, cons
     u64 in[2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) in[j] = r.top_k > 0 ? counts[2 * t + j] : c.bins[2 * t + j];
-    cut(r, in, c.part, cut_row);
+    cut(r, in, c.part, found);
     __syncthreads();
-    r.lo = cut_row.lo;
-    r.hi = cut_row.hi;
-    r.before = cut_row.before;
-    r.whole = cut_row.whole;
+    r.lo = found.lo;
+    r.hi = found.hi;
+    r.before = found.before;
+    r.whole = found.whole;
 #pragma unroll 4
     for (int i = t; i < n; i += NT) {
       const int b = bin_of(held[i], r.top, r.per_bin);
@@ -910,10 +915,7 @@ hipError_t launch_sample(hipStream_t st, const SampleArgs &all, void *workspace)
     const dim3 grid(w.slices, a.rows);
     hipLaunchKernelGGL(sample_ends_kernel, grid, dim3(NT), 0, st, a, w);
     hipLaunchKernelGGL(sample_bins_kernel, grid, dim3(NT), 0, st, a, w);
-    if (filters) {
-      hipLaunchKernelGGL(sample_cut_kernel, dim3(a.rows), dim3(NT), 0, st, a, w);
-      hipLaunchKernelGGL(sample_list_kernel, grid, dim3(NT), 0, st, a, w);
-    }
+    if (filters) hipLaunchKernelGGL(sample_list_kernel, grid, dim3(NT), 0, st, a, w);
     hipLaunchKernelGGL(sample_draw_kernel, dim3(a.rows), dim3(NT), 0, st, a, w);
   }
   return hipGetLastError();
