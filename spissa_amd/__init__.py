@@ -3,7 +3,8 @@
 The package mirrors crates/spissa-runtime/src/rotary.rs, the ops the path
 uses, the streaming linear projections either side of it and the LM head
 with greedy sampling after it, over the C ABI
-in include/spissa_hip.h (libspissa_hip.so). There is no
+in include/spissa_hip.h (libspissa_hip.so); spissa_amd.device adds the device
+tier, with steps of drafted tokens and sampling. There is no
 CPU fallback: every call runs the HIP kernels.
 """
 from .errors import (ArgumentError, DeviceError, InvalidTensorDataError, ShapeError,  # noqa: F401

@@ -376,12 +376,11 @@ struct TreeArgsOf : TreeBase {
   TreeSeq seq[MB];
 };
 typedef TreeArgsOf<kMaxDecodeBatch> TreeArgs;
-// A launch's work: units (a KV head of a block of 128 / kw rows, a row being a node and
-// a query head of the KV head) of key tiles at places one after the other, workgroups
-// with `share` places each, up to `splits` of them a unit; kw: waves that share a
-// tile's keys.
+// A launch's work: units (a KV head of a block of 128 rows, a row being a node and a
+// query head of the KV head) of key tiles at places one after the other, workgroups with
+// `share` places each, up to `splits` of them a unit.
 struct TreePlan {
-  int kw = 1, share = 1, splits = 1, places = 0;
+  int share = 1, splits = 1, places = 0;
   long groups = 0;  // of 16 rows
   int tiles[kMaxDecodeBatch], padded[kMaxDecodeBatch], start[kMaxDecodeBatch];
   long group0[kMaxDecodeBatch];

@@ -18,6 +18,7 @@ namespace spissa {
 namespace {
 
 constexpr int kMaskWords = kTreeMaxNodes / 32;
+constexpr int kTreeRows = 128;  // of a workgroup: a node and one of the KV head's query heads each
 
 // The nodes' depths and, with MASKS, the nodes that each sees (with a window those less
 // than it apart), by doubling: after k rounds a node knows the 2^k nodes above it. A
@@ -146,7 +147,9 @@ __device__ __forceinline__ SmallShape small_shape(int p, int nodes, int *err) {
 // up with the last row) as the B operand of the scores' product, two binary16 pieces of
 // the query times a power of two, the power's inverse, the first key that the row sees,
 // and the nodes that a node sees. D / 8 lanes a row, each with four channels and their
-// rotation's partners. Bound by latency: the parents, the rotation's rows, the stores.
+// rotation's partners. Bound by latency: the parents, the rotation's rows, the stores
+// (5 nodes of 32 + 2 x 8 rows of 64: 4 us; 256 of 4 + 2 x 1 of 256: 8 us; by each attention
+// workgroup for itself it cost 16 ragged sequences a quarter of their time).
 // Grid: (blocks of rows of the longest sequence, sequences), 256 threads.
 template <int D, int MB>
 __global__ __launch_bounds__(256) void tree_prepare_kernel(const TreeArgsOf<MB> a) {
@@ -266,10 +269,9 @@ __device__ __forceinline__ TreeUnit tree_unit(const Args &a, int at) {
   return u;
 }
 
-// Eight waves. A wave has 16 rows (a node and one of the KV head's query heads) and, of
-// each tile of 8192 / D keys, all or (KW 2, few rows) half: waves 0..3 the first, 4..7
-// the second, and the halves meet at the end. Tiles are first the cached rows from the
-// first that any node sees, then the nodes' own. A tile comes into registers while the
+// Eight waves of 16 rows (a node and one of the KV head's query heads) each, which take
+// tiles of 8192 / D keys. Tiles are first the cached rows from the first that any node
+// sees, then the nodes' own. A tile comes into registers while the
 // one before is computed; waves 0..3 take its values, waves 4..7 its keys, and write
 // them to LDS once for all rows as two binary16 pieces, in the order in which lanes take
 // the operands. S^T = K Q^T, so a lane has one row (column lane % 16) and four keys of
@@ -288,12 +290,19 @@ __device__ __forceinline__ TreeUnit tree_unit(const Args &a, int at) {
 // the other with their tiles, and a workgroup takes `share` of them in a row, of one
 // unit or of several; a unit of several workgroups' is merged by tree_merge_kernel.
 //
+// Bound by HBM with few rows (16 sequences of up to 8192 keys, 12 nodes, 24 heads on 8 of
+// 128: 135 us, 5.2 TB/s; one sequence, 26 nodes: 25 us, of which 6 fill and drain the
+// pipeline), by LDS reads beside the matrix instructions with many (256 nodes over 32768
+// keys, 4 heads on one of 256: 125 us, 275 TFLOP/s of plain products, three times that of
+// pieces). Two waves sharing
+// 16 rows' keys, where half the waves have no rows, came to the same (64 rows over 8192
+// keys of 8 heads of 128: 28.2 us a step against 27.2).
+//
 // Grid: workgroups.
-template <int D, int KW, int MB>
+template <int D, int MB>
 __global__ __launch_bounds__(512, 2) void tree_attend_kernel(const TreeArgsOf<MB> a) {
   constexpr int BN = 8192 / D, G = D / 32, DT = D / 16, VB = BN / 32, KB = BN / 16, TR = D / 8;
-  constexpr int RW = 8 / KW, ROWS = RW * 16;
-  constexpr int KBW = KB / KW, VBW = VB / KW;  // a wave's 16 and 32 keys of a tile
+  constexpr int ROWS = kTreeRows;
   constexpr int AHEAD = D == 256 ? 2 : 3;
   static_assert(KB * G == 16 && VB * DT == 16, "a tile has 8192 keys' and as many values' channels");
   __shared__ __attribute__((aligned(16))) half8 pieces_lds[2][2][2][1024];  // values, buffer, piece
@@ -311,7 +320,6 @@ __global__ __launch_bounds__(512, 2) void tree_attend_kernel(const TreeArgsOf<MB
     asm volatile("" : "+v"(tid));  // (what follows from it is formed in each turn: kept, it would not leave room for the rest)
     const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int col = lane & 15, kq = lane >> 4;
-    const int rw = wave % RW, kw = wave / RW;
     const bool values = wave < 4;
     const TreeUnit unit = tree_unit(a, place);
     const int t0 = place - unit.start, t1 = min(unit.tiles, t0 + (end - place));
@@ -322,7 +330,7 @@ __global__ __launch_bounds__(512, 2) void tree_attend_kernel(const TreeArgsOf<MB
     const int past = a.seq[unit.b].past, nodes = a.seq[unit.b].nodes, rows = nodes * a.R;
     const int lo = a.window > 0 ? max(0, past + 1 - a.window) : 0;
     const int cached = (past - lo + BN - 1) / BN;
-    const int row0 = unit.block * ROWS + rw * 16;
+    const int row0 = unit.block * ROWS + wave * 16;
     const bool busy = row0 < rows;
 
     // A thread's share of a tile: of values eight keys (4 q + 0..3 and 16 + 4 q + 0..3 of
@@ -427,13 +435,13 @@ __global__ __launch_bounds__(512, 2) void tree_attend_kernel(const TreeArgsOf<MB
       // Steps of two operands of either product, six instructions; their LDS reads run
       // AHEAD - 1 steps before them. The scores' are two 16 keys of 32 channels each,
       // the outputs' 32 keys of two 16 channels.
-      constexpr int KS = G * KBW / 2, VS = VBW * DT / 2;
+      constexpr int KS = G * KB / 2, VS = VB * DT / 2;
       half8 fh[AHEAD][2], fl[AHEAD][2];
       auto read = [&](int step) __attribute__((always_inline)) {
         half8 (&th)[2] = fh[step % AHEAD], (&tl)[2] = fl[step % AHEAD];
         if (step < KS) {
-          const int g = step / (KBW / 2), k = step % (KBW / 2) * 2;
-          const int at = ((kw * KBW + k) * G + g) * 64 + kq * 16 + ((col ^ (4 * g + kq)) & 15);
+          const int g = step / (KB / 2), k = step % (KB / 2) * 2;
+          const int at = (k * G + g) * 64 + kq * 16 + ((col ^ (4 * g + kq)) & 15);
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             th[i] = kp_lds[buf][0][at + i * G * 64];
@@ -443,20 +451,20 @@ __global__ __launch_bounds__(512, 2) void tree_attend_kernel(const TreeArgsOf<MB
           const int v = (step - KS) / (DT / 2), d = (step - KS) % (DT / 2) * 2;
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            const int at = ((kw * VBW + v) * DT + d + i) * 64 + kq * 16 + (col ^ ((d + i) & 3));
+            const int at = (v * DT + d + i) * 64 + kq * 16 + (col ^ ((d + i) & 3));
             th[i] = vp_lds[buf][0][at];
             tl[i] = vp_lds[buf][1][at];
           }
         }
       };
-      f32x4 sc[KBW];
+      f32x4 sc[KB];
 #pragma unroll
-      for (int k = 0; k < KBW; ++k) sc[k] = (f32x4){0.f, 0.f, 0.f, 0.f};
+      for (int k = 0; k < KB; ++k) sc[k] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < AHEAD - 1; ++i) read(i);
 #pragma unroll
       for (int step = 0; step < KS; ++step) {
-        const int g = step / (KBW / 2), k = step % (KBW / 2) * 2;
+        const int g = step / (KB / 2), k = step % (KB / 2) * 2;
         read(step + AHEAD - 1);
         __builtin_amdgcn_sched_barrier(0);
         const half8 (&th)[2] = fh[step % AHEAD], (&tl)[2] = fl[step % AHEAD];
@@ -472,8 +480,8 @@ __global__ __launch_bounds__(512, 2) void tree_attend_kernel(const TreeArgsOf<MB
       const float f = fminf(fmaxf(inv_q * inverse_scale(kbits), 1.1754944e-38f), 3.402823466e38f);
       if (own || bad || base + BN > past || base < wave_lo) {
 #pragma unroll
-        for (int v = 0; v < VBW; ++v) {
-          const int first = 32 * (kw * VBW + v);  // of the tile
+        for (int v = 0; v < VB; ++v) {
+          const int first = 32 * v;  // of the tile
           unsigned seen;
           if (own) {
             const int w = ((tile - cached) * BN + first) / 32;
@@ -484,7 +492,7 @@ __global__ __launch_bounds__(512, 2) void tree_attend_kernel(const TreeArgsOf<MB
             const int from = max(0, row_lo - base - first), to = min(32, past - base - first);
             seen = from >= 32 || to <= from ? 0u : (0xffffffffu << from) & (0xffffffffu >> (32 - to));
           }
-          if (bad) poison |= (seen & bad_lds[kw * VBW + v]) != 0;
+          if (bad) poison |= (seen & bad_lds[v]) != 0;
 #pragma unroll
           for (int i = 0; i < 8; ++i)
             if (!(seen >> ((i & 3) + 4 * kq + 16 * (i >> 2)) & 1u)) sc[2 * v + (i >> 2)][i & 3] = NEG_INF;
@@ -492,7 +500,7 @@ __global__ __launch_bounds__(512, 2) void tree_attend_kernel(const TreeArgsOf<MB
       }
       float big = NEG_INF;
 #pragma unroll
-      for (int k = 0; k < KBW; ++k) big = fmaxf(big, fmaxf(fmaxf(sc[k][0], sc[k][1]), fmaxf(sc[k][2], sc[k][3])));
+      for (int k = 0; k < KB; ++k) big = fmaxf(big, fmaxf(fmaxf(sc[k][0], sc[k][1]), fmaxf(sc[k][2], sc[k][3])));
       big = max32(max16(big)) * f;
       if (__any(big > m + 7.0f)) {
         const float next = big > m + 7.0f ? big : m, keep = fast_exp2(m - safe_max(next));
@@ -502,9 +510,9 @@ __global__ __launch_bounds__(512, 2) void tree_attend_kernel(const TreeArgsOf<MB
         for (int d = 0; d < DT; ++d) o[d] *= keep;
       }
       const float off = 8.0f - safe_max(m);  // weights times 2^8, up to 2^15
-      half8 ph[VBW], pl[VBW];
+      half8 ph[VB], pl[VB];
 #pragma unroll
-      for (int v = 0; v < VBW; ++v) {
+      for (int v = 0; v < VB; ++v) {
         float p[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -606,29 +614,9 @@ __global__ __launch_bounds__(512, 2) void tree_attend_kernel(const TreeArgsOf<MB
       __syncthreads();
     }
 
-    // The halves meet: waves 4..7 leave theirs in LDS.
-    constexpr int PER = 16 * D + 32;  // floats a wave: outputs, scores and sums
-    static_assert(KW == 1 || RW * PER * 4 <= (int)sizeof pieces_lds, "the halves' room");
-    float *const room = reinterpret_cast<float *>(pieces_lds) + rw * PER;
     l = sum32(sum16(l));
     if (poison) l = __builtin_nanf("");
-    if (KW == 2) {
-      if (kw == 1 && busy) {
-#pragma unroll
-        for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4 *>(room + d * 256 + lane * 4) = o[d];
-        if (kq == 0) *reinterpret_cast<float2 *>(room + 16 * D + 2 * col) = make_float2(m, l);
-      }
-      __syncthreads();
-    }
-    if (kw == 0 && busy) {
-      if (KW == 2) {
-        const float2 ml = *reinterpret_cast<const float2 *>(room + 16 * D + 2 * col);
-        const float big = fmaxf(m, ml.x), mine = fast_exp2(m - safe_max(big)), theirs = fast_exp2(ml.x - safe_max(big));
-        m = big;
-        l = l * mine + ml.y * theirs;
-#pragma unroll
-        for (int d = 0; d < DT; ++d) o[d] = o[d] * mine + *reinterpret_cast<const f32x4 *>(room + d * 256 + lane * 4) * theirs;
-      }
+    if (busy) {
       const float inv = l == 0.0f ? 0.0f : inverse_scale(vbits) / l;
       if (row0 + col < rows) {
         const int node = (row0 + col) / a.R;
@@ -649,7 +637,8 @@ __global__ __launch_bounds__(512, 2) void tree_attend_kernel(const TreeArgsOf<MB
 
 // The outputs of a unit's workgroups, each divided by its own sum, by their sums'
 // shares. D / 4 threads an output row and SL lanes over the workgroups, each with eight
-// loads in flight. Bound by latency.
+// loads in flight. Bound by latency (3 to 5 us), with many rows by the partial outputs'
+// reads (16 sequences: 8 us).
 // Grid: (blocks of rows), 256 threads.
 template <int D, int SL, int MB>
 __global__ __launch_bounds__(256) void tree_merge_kernel(const TreeArgsOf<MB> a) {
@@ -725,10 +714,7 @@ bool tree_plan(int D, int R, int Hkv, int window, const int *past, const int *no
   const int BN = 8192 / D;
   TreePlan &p = *plan;
   p = TreePlan{};
-  int most_rows = 1;
-  for (int b = 0; b < B; ++b) most_rows = std::max(most_rows, nodes[b] * R);
-  p.kw = D < 256 && most_rows <= 64 ? 2 : 1;
-  const int per = 128 / p.kw;
+  const int per = kTreeRows;
   long units[kMaxDecodeBatch], total = 0;
   for (int b = 0; b < B; ++b) {
     const int lo = window > 0 ? std::max(0, past[b] + 1 - window) : 0;
@@ -772,7 +758,7 @@ static void run_merge(hipStream_t st, const TreeArgsOf<MB> &a, int splits) {
   else run(std::integral_constant<int, 4>{});
 }
 
-template <int D, int KW, int MB>
+template <int D, int MB>
 static void run_attend(hipStream_t st, const TreeArgsOf<MB> &a, const TreePlan &p) {
   int lines = 0;  // of the prepare kernel: queries, keys and values
   for (int b = 0; b < a.B; ++b) {
@@ -781,22 +767,22 @@ static void run_attend(hipStream_t st, const TreeArgsOf<MB> &a, const TreePlan &
   }
   constexpr int LINES = 2048 / D;
   hipLaunchKernelGGL((tree_prepare_kernel<D, MB>), dim3((lines + LINES - 1) / LINES, a.B), dim3(256), 0, st, a);
-  hipLaunchKernelGGL((tree_attend_kernel<D, KW, MB>), dim3((a.places + a.share - 1) / a.share), dim3(512), 0, st, a);
+  hipLaunchKernelGGL((tree_attend_kernel<D, MB>), dim3((a.places + a.share - 1) / a.share), dim3(512), 0, st, a);
   if (p.splits > 1) run_merge<D>(st, a, p.splits);
 }
 
 template <int MB>
 static hipError_t run_tree(hipStream_t st, const TreeArgsOf<MB> &a, const TreePlan &p, int D) {
-  if (D == 64) p.kw == 1 ? run_attend<64, 1>(st, a, p) : run_attend<64, 2>(st, a, p);
-  else if (D == 128) p.kw == 1 ? run_attend<128, 1>(st, a, p) : run_attend<128, 2>(st, a, p);
-  else run_attend<256, 1>(st, a, p);
+  if (D == 64) run_attend<64>(st, a, p);
+  else if (D == 128) run_attend<128>(st, a, p);
+  else run_attend<256>(st, a, p);
   return hipGetLastError();
 }
 
 hipError_t launch_tree(hipStream_t st, TreeArgs &a, const TreePlan &p, int D) {
   a.share = p.share;
   a.places = p.places;
-  a.per = 128 / p.kw;
+  a.per = kTreeRows;
   for (int b = 0; b < a.B; ++b) {
     a.seq[b].start = p.start[b];
     a.seq[b].tiles = p.tiles[b];
@@ -812,7 +798,8 @@ hipError_t launch_tree(hipStream_t st, TreeArgs &a, const TreePlan &p, int D) {
 
 // The walk along confirmed nodes: every node that holds the token sampled at its
 // parent offers itself as the parent's next, the lowest one stays, and one thread
-// follows them. Bound by latency: a load, an LDS read a node of the path, a store.
+// follows them. Bound by latency: a load, an LDS read a node of the path, a store (5 nodes
+// 1.8 us, 64 trees of up to 64 nodes 3 us).
 // Grid: sequences; a wave each.
 __global__ __launch_bounds__(64) void tree_accept_kernel(const TreeAcceptArgs a) {
   __shared__ int sampled[kTreeMaxNodes], next[kTreeMaxNodes], path[kTreeMaxNodes];
@@ -892,7 +879,8 @@ __device__ __forceinline__ void move_rows(const int *path, int n, At at) {
 }  // namespace
 
 // Grid: (blocks over a row's pieces, caches, keys or values), 256 threads. Bound by
-// latency: the path, then one round of loads and one of stores.
+// latency: the path, then one round of loads and one of stores (28 caches, 4 rows of 8 x
+// 128: 3.6 us; 32 caches, 12 rows: 5.2 us).
 __global__ __launch_bounds__(256) void keep_kernel(const KeepArgs a) {
   __shared__ int path[kTreeMaxNodes], end;
   const KeepCache &c = a.cache[blockIdx.y];
