@@ -290,13 +290,13 @@ __device__ __forceinline__ TreeUnit tree_unit(const Args &a, int at) {
 // the other with their tiles, and a workgroup takes `share` of them in a row, of one
 // unit or of several; a unit of several workgroups' is merged by tree_merge_kernel.
 //
-// Bound by HBM with few rows (16 sequences of up to 8192 keys, 12 nodes, 24 heads on 8 of
-// 128: 135 us, 5.2 TB/s; one sequence, 26 nodes: 25 us, of which 6 fill and drain the
-// pipeline), by LDS reads beside the matrix instructions with many (256 nodes over 32768
-// keys, 4 heads on one of 256: 125 us, 275 TFLOP/s of plain products, three times that of
-// pieces). Two waves sharing
-// 16 rows' keys, where half the waves have no rows, came to the same (64 rows over 8192
-// keys of 8 heads of 128: 28.2 us a step against 27.2).
+// Bound by HBM with few rows (a step of 16 sequences of up to 8192 keys, 12 nodes each, 24
+// heads on 8 of 128: 143 us, 4.9 TB/s; of one sequence, 26 nodes: 32 us, of which 6 fill and
+// drain this pipeline and 7 are the other launches), by dependent chains of LDS reads and
+// matrix instructions at two waves a SIMD with many (256 nodes over 32768 keys, 4 heads on
+// one of 256: 133 us, 259 TFLOP/s of plain products, three times that of pieces). Two waves
+// sharing 16 rows' keys, where half the waves have no rows, came to the same (64 rows over
+// 8192 keys of 8 heads of 128: 28.2 us a step against 27.2).
 //
 // Grid: workgroups.
 template <int D, int MB>
