@@ -115,7 +115,8 @@ struct TreeQuery {
 
 }  // namespace
 
-// Up to 64 nodes, by each wave for itself: lane t's depth and nodes that it sees.
+// Up to 64 nodes, by each wave for itself: lane t's depth and nodes that it sees. (A step
+// of 26 nodes 32.4 us, with tree_shape 33.6.)
 struct SmallShape {
   int depth;
   unsigned lo, hi;
@@ -174,7 +175,7 @@ __global__ __launch_bounds__(256) void tree_prepare_kernel(const TreeArgsOf<MB> 
   int *const err = blockIdx.x == 0 && tid < 64 ? a.err : nullptr;
   int depth;
   if (nodes <= 64 && !(a.window > 0 && a.window < nodes)) {
-    const SmallShape s = small_shape(parent, nodes, err);
+    const SmallShape s = small_shape(parent, nodes, err);  // (a window that may part nodes takes the other)
     depth = __shfl(s.depth, node);
     if (blockIdx.x == 0 && tid < nodes) {
       a.mask[(long)(first + tid) * kMaskWords] = s.lo;
@@ -303,7 +304,7 @@ template <int D, int MB>
 __global__ __launch_bounds__(512, 2) void tree_attend_kernel(const TreeArgsOf<MB> a) {
   constexpr int BN = 8192 / D, G = D / 32, DT = D / 16, VB = BN / 32, KB = BN / 16, TR = D / 8;
   constexpr int ROWS = kTreeRows;
-  constexpr int AHEAD = D == 256 ? 2 : 3;
+  constexpr int AHEAD = 2;  // (three: the same with heads of 64 and 128, a tenth slower with heads of 256)
   static_assert(KB * G == 16 && VB * DT == 16, "a tile has 8192 keys' and as many values' channels");
   __shared__ __attribute__((aligned(16))) half8 pieces_lds[2][2][2][1024];  // values, buffer, piece
   half8 (*const kp_lds)[2][1024] = pieces_lds[0], (*const vp_lds)[2][1024] = pieces_lds[1];
@@ -708,8 +709,9 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(const TreeArgsOf<MB> a)
 
 // A workgroup's share of the tiles: a cus'th of them all. Units start with a
 // workgroup of their own, their tiles padded to whole shares, where that takes shares
-// at most an eighth larger; else they lie end to end, and a workgroup at a border takes
-// both sides (a start more). False where there are more places than an int has.
+// at most an eighth larger (26 nodes over 8192 rows: 32.4 us against 35.1 end to end, 256
+// over 32768: 135.5 against 145); else they lie end to end, and a workgroup at a border
+// takes both sides (a start more). False where there are more places than an int has.
 bool tree_plan(int D, int R, int Hkv, int window, const int *past, const int *nodes, int B, int cus, TreePlan *plan) {
   const int BN = 8192 / D;
   TreePlan &p = *plan;
@@ -753,8 +755,9 @@ static void run_merge(hipStream_t st, const TreeArgsOf<MB> &a, int splits) {
     constexpr int SL = decltype(lanes)::value, ROWS = 256 / (TR * SL);
     hipLaunchKernelGGL((tree_merge_kernel<D, SL, MB>), dim3((a.total + ROWS - 1) / ROWS), dim3(256), 0, st, a);
   };
+  // (a step with 26 or 33 workgroups a unit: 34.0 and 24.5 us with one lane a row, 32.8 and
+  // 22.8 with four; 16 sequences, 9 or fewer: 145.9 with one, 146.8 with four)
   if (splits <= 8) run(std::integral_constant<int, 1>{});
-  else if (splits <= 16) run(std::integral_constant<int, 2>{});
   else run(std::integral_constant<int, 4>{});
 }
 
@@ -790,7 +793,7 @@ hipError_t launch_tree(hipStream_t st, TreeArgs &a, const TreePlan &p, int D) {
     a.seq[b].group0 = p.group0[b];
   }
   if (a.B > 1) return run_tree(st, a, p, D);
-  TreeArgsOf<1> one;  // (a launch's arguments cost the host time)
+  TreeArgsOf<1> one;  // (a launch's arguments cost time: 16.2 us a step of five nodes, 17.2 with room for 16 sequences)
   static_cast<TreeBase &>(one) = a;
   one.seq[0] = a.seq[0];
   return run_tree(st, one, p, D);
