@@ -735,3 +735,72 @@ def test_drafted_decoding_writes_what_decoding_writes(s, settings):
         assert n == len(mine) - 1
         for x, y in zip(held(s, a, 0, n), held(s, b, 0, n)):
             assert np.abs(x - y).max() <= 1e-3
+
+
+@pytest.mark.parametrize("heads", [(24, 8, 128), (8, 2, 64), (4, 1, 256)])
+@pytest.mark.parametrize("what", [np.nan, np.inf, -np.inf])
+def test_a_query_that_is_not_finite_is_its_rows_alone(gpu, s, heads, what):
+    print(f"[case] {what} in a query {heads}", flush=True)
+    rng = np.random.default_rng(12)
+    dr = Draft(s, rng, heads, [333], [13])
+    dr.q[6, 1, 3] = what
+    out = dr.run(s).cpu().numpy()
+    with pytest.raises(gpu.InvalidTensorDataError):
+        s.sync()
+    s.sync()
+    assert not np.isfinite(out[6, 1]).any()
+    dr.q[6, 1] = 0
+    others = np.ones(out.shape[:2], bool)
+    others[6, 1] = False
+    want, _ = dr.plain()
+    assert rows_off(out[others], want[others]) <= ROW
+
+
+@pytest.mark.parametrize("scale", [1e-30, 1e-12, 1e4])
+def test_queries_of_any_size(s, scale):
+    """Small ones weigh all keys alike; large ones take one key, their scores' error 2^-22 of some 1e5: a weight that is
+    another's neighbour within 2^-22 * 1e5 = 0.03 could be off by that much, which N(0, 1) keys of 64 channels are not (the
+    two largest of 260 scores lie some 1e4 * 8 * 0.3 apart), so the row is the key's value to the pieces' 2^-23."""
+    rng = np.random.default_rng(13)
+    dr = Draft(s, rng, (4, 2, 64), [250], [10])
+    dr.q *= np.float32(scale)
+    out = dr.run(s).cpu().numpy()
+    s.sync()
+    assert rows_off(out, dr.plain()[0]) <= ROW
+
+
+def test_two_sessions_at_once(gpu):
+    """Two sessions of two threads and streams, each with caches and a workspace of its own: the same outputs as alone."""
+    import threading
+
+    import torch
+
+    from spissa_amd.device import Session
+
+    got, failed = [[], []], []
+
+    def work(i, rounds):
+        try:
+            stream = torch.cuda.Stream()
+            ses = Session(0, stream=stream)
+            with torch.cuda.stream(stream):
+                dr = Draft(ses, np.random.default_rng(20 + i), [(24, 8, 128), (8, 4, 256)][i], [[900], [40, 700]][i], [[12], [30, 3]][i])
+                for _ in range(rounds):
+                    got[i].append(dr.run(ses))
+                    for c, p in zip(dr.caches, dr.past):
+                        c.truncate(p)
+                ses.sync()
+        except Exception as e:  # (shown by the main thread)
+            failed.append(e)
+
+    want = []
+    for i in range(2):
+        work(i, 1)
+        want.append(got[i].pop())
+    threads = [threading.Thread(target=work, args=(i, 25)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
+    assert all(torch.equal(o, want[i]) for i in range(2) for o in got[i])
