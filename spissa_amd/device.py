@@ -9,6 +9,7 @@ rotary.rs:560-564 does).
 from __future__ import annotations
 
 import ctypes as C
+from array import array
 from dataclasses import dataclass
 from typing import Optional, Sequence
 
@@ -45,6 +46,13 @@ def _cache_array(caches, optional: bool = False):
     for i, c in enumerate(caches):
         arr[i] = None if optional and c is None else c.handle.value
     return arr
+
+
+def _sizes(counts):
+    """Counts as a C array of at least one."""
+    if len(counts) <= 8:
+        return (_ffi.c_size * max(1, len(counts)))(*counts)
+    return (_ffi.c_size * len(counts)).from_buffer(array("Q", counts))  # (64 of them: 1.4 us, not 6.4)
 
 
 _ONE_HANDLE = _ffi.c_void_p * 1
@@ -370,7 +378,7 @@ class Session:
         arr = _cache_array(caches)
         cfg = config._c()
         check(fn(self.handle, None if table is None else table.handle, _dev(q, "q"), _dev(k, "k"), _dev(v, "v"), arr,
-                 (_ffi.c_size * max(1, len(nodes)))(*nodes), len(caches), _many_i32(parents, n, "parents"),
+                 _sizes(nodes), len(caches), _many_i32(parents, n, "parents"),
                  C.byref(cfg), *more, _dev(out, "out")))
 
     def tree_step(self, table: Optional[RopeTable], q, k, v, caches: Sequence[KvCache], nodes: Sequence[int], parents,
@@ -398,7 +406,7 @@ class Session:
         n, b = sum(nodes), len(nodes)
         check(self._lib.spissa_tree_accept_device(
             self.handle, n and _many_i32(parents, n, "parents"), n and _many_i32(tokens, n, "tokens"),
-            n and _many_i32(sampled, n, "sampled"), (_ffi.c_size * max(1, b))(*nodes), b, n and _many_i32(path, n, "path"),
+            n and _many_i32(sampled, n, "sampled"), _sizes(nodes), b, n and _many_i32(path, n, "path"),
             b and _many_i32(count, b, "count"), b and _many_i32(next_token, b, "next_token")))
 
     def keep_rows(self, caches: Sequence[KvCache], nodes: Sequence[int], path, count) -> None:
@@ -410,7 +418,7 @@ class Session:
         if len(caches) % max(1, b) != 0 or (caches and not b):
             raise TypeError(f"{len(caches)} caches for {b} sequences")
         check(self._lib.spissa_kv_cache_keep_device(
-            self.handle, _cache_array(caches), len(caches) // max(1, b), (_ffi.c_size * max(1, b))(*nodes), b,
+            self.handle, _cache_array(caches), len(caches) // max(1, b), _sizes(nodes), b,
             _many_i32(path, n, "path") if n else 0, _many_i32(count, b, "count") if b else 0))
 
     def sample(self, logits, uniform, config: SamplingConfig, tokens, probs=None) -> None:
