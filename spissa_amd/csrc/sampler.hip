@@ -20,7 +20,7 @@
 // some hundred), draws, and walks the granule in which the draw falls. A row whose list
 // would not fit (thousands of tokens in a thousandth of the logits' range, or a top-k of
 // thousands) is done in the same way over the whole row. Without filters the third launch
-// is left out, and up to 8192 logits are one workgroup's from start to end
+// is left out, and up to 12288 logits are one workgroup's from start to end
 // (sample_row_kernel).
 //
 // Bound by latency for a few rows (one of 128256 logits, all filters: 19 us, four launches
@@ -780,37 +780,51 @@ __global__ __launch_bounds__(NT) void sample_draw_kernel(const SampleArgs a, con
 }
 
 // All of it for rows of at most ROW logits, held in LDS, a workgroup each: the same steps
-// over the same numbers (granules are of 64 logits). Grid: rows.
+// over the same numbers, four neighbours a thread at a time. Bound by latency and by one
+// CU's operations in 64 bits (kRow has the times). Grid: rows.
 template <int ROW>
 __global__ __launch_bounds__(NT) void sample_row_kernel(const SampleArgs a, const int shift) {
-  constexpr int HERE = 1536;  // (with 8192 logits 61 KB: two workgroups a CU)
-  static_assert(ROW <= 64 * NT, "a granule a thread");
-  __shared__ float held[ROW];
-  __shared__ u64 list[HERE];
+  constexpr int HERE = 1536;  // (with 12288 logits 79 KB: two workgroups a CU)
+  constexpr int WAVE = 256;   // logits of a wave's turn
+  static_assert(ROW <= 64 * WAVE, "a granule a lane");
+  __shared__ __attribute__((aligned(16))) float held[ROW];
+  __shared__ u64 list[HERE], sums[64];
   __shared__ Choice c;
   __shared__ Row found;
   __shared__ unsigned written;
   const int row = blockIdx.x, t = threadIdx.x, n = a.vocab;
   for (int i = t; i < BINS; i += NT) c.bins[i] = 0;
+  if (t < 64) sums[t] = 0;
   if (t == 0) written = 0;
   const Slice e = ends_of(a.x + (long)row * n, 0, n, [&](int i, float v) { held[i] = v; });
   Row r = row_of(a, e, row);
   if (answered(a, r, row)) return;
   const Weigh weigher = weigh_of(r, shift);
   auto weigh = [&](float v, double least) { return weigh_apart(weigher, v, least); };
+  // f(index, its four logits), of which those from n on do not count
+  auto fours = [&](int from, auto f) __attribute__((always_inline)) {
+    const f32x4 v = *reinterpret_cast<const f32x4 *>(held + from);
+    f(from, v);
+  };
   u64 last = 0;
   if (r.state == kList) {
     unsigned *const counts = reinterpret_cast<unsigned *>(c.bins);
-    if (r.top_k > 0) {
-#pragma unroll 4
-      for (int i = t; i < n; i += NT) atomicAdd(&counts[bin_of(held[i], r.top, r.per_bin)], 1u);
-    } else {
-#pragma unroll 4
-      for (int i = t; i < n; i += NT) {
-        const u64 p = weigher(held[i], 0.0);
-        if (p) atomicAdd(&c.bins[bin_of(held[i], r.top, r.per_bin)], p);
-      }
-    }
+#pragma unroll 1
+    for (int from = 4 * t; from < n; from += 4 * NT)
+      fours(from, [&](int i, f32x4 v) __attribute__((always_inline)) {
+        if (r.top_k > 0) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (i + j < n) atomicAdd(&counts[bin_of(v[j], r.top, r.per_bin)], 1u);
+        } else {
+          u64 p[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) p[j] = weigher(v[j], 0.0);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (i + j < n && p[j]) atomicAdd(&c.bins[bin_of(v[j], r.top, r.per_bin)], p[j]);
+        }
+      });
     __syncthreads();
     u64 in[2];
 #pragma unroll
@@ -821,54 +835,64 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(const SampleArgs a, cons
     r.hi = found.hi;
     r.before = found.before;
     r.whole = found.whole;
-#pragma unroll 4
-    for (int i = t; i < n; i += NT) {
-      const int b = bin_of(held[i], r.top, r.per_bin);
-      if (b >= r.lo && b <= r.hi) {
-        const unsigned at = atomicAdd(&written, 1u);
-        if (at < HERE) list[at] = token_of(held[i], i);
-      }
-    }
+#pragma unroll 1
+    for (int from = 4 * t; from < n; from += 4 * NT)
+      fours(from, [&](int i, f32x4 v) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int b = bin_of(v[j], r.top, r.per_bin);
+          if (i + j < n && b >= r.lo && b <= r.hi) {
+            const unsigned at = atomicAdd(&written, 1u);
+            if (at < HERE) list[at] = token_of(v[j], i + j);
+          }
+        }
+      });
     __syncthreads();
     const int listed = (int)written;
     last = last_kept(r, weigh, list, listed, listed <= HERE, n, [&](int i) { return held[i]; }, c);
   }
-  // The granules' sums, the draw and its granule.
-  u64 *const sums = c.bins;
-  __syncthreads();
-  sums[t] = 0;
-  __syncthreads();
-#pragma unroll 1
-  for (int i = t; i - (t & 63) < n; i += NT) {
-    u64 p = 0;
-    if (i < n && token_of(held[i], i) >= last) p = weigher(held[i], weigher.min_p);
-    if (__any(p != 0)) {
-      p = wave_sum(p);
-      if ((t & 63) == 0) sums[i >> 6] = p;
+  // The waves' sums of kept weights, the draw and its wave's turn.
+  auto kept = [&](int i, f32x4 v, u64 (&p)[4]) __attribute__((always_inline)) {
+    u64 sum = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      p[j] = i + j < n && token_of(v[j], i + j) >= last ? weigher(v[j], weigher.min_p) : 0;
+      sum += p[j];
     }
-  }
-  __syncthreads();
-  u64 total;
-  const u64 mine = sums[t], up = block_before(mine, c.part, &total), draw = drawn(r, total);
-  if (draw >= up && draw < up + mine) {
-    c.ends[0] = (u64)t;
-    c.ends[1] = up;
-  }
+    return sum;
+  };
+  u64 p[4];
+#pragma unroll 1
+  for (int from = 4 * t; from - 4 * (t & 63) < n; from += 4 * NT)
+    fours(from, [&](int i, f32x4 v) __attribute__((always_inline)) {
+      const u64 sum = kept(i, v, p);
+      if (!__any(sum != 0)) return;
+      const u64 all = wave_sum(sum);
+      if ((t & 63) == 0) sums[i / WAVE] = all;
+    });
   __syncthreads();
   if (t >= 64) return;
-  const int i = 64 * (int)c.ends[0] + t;
-  const u64 p = i < n && token_of(held[min(i, n - 1)], i) >= last ? weigh(held[min(i, n - 1)], weigher.min_p) : 0;
-  const u64 sum = c.ends[1] + wave_up_to(p);
-  if (sum > draw && sum - p <= draw) {
-    a.tokens[row] = i;
-    if (a.probs) a.probs[row] = (float)((double)p / (double)total);
-  }
+  const u64 mine = sums[t], up = wave_up_to(mine), total = last_lane(up), draw = drawn(r, total);
+  const int g = __ffsll((unsigned long long)__ballot(draw < up)) - 1;
+  const u64 before = __shfl(up - mine, g);
+  fours(WAVE * g + 4 * t, [&](int i, f32x4 v) __attribute__((always_inline)) {
+    u64 run = kept(i, v, p);
+    run = before + wave_up_to(run) - run;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (run <= draw && run + p[j] > draw) {
+        a.tokens[row] = i + j;
+        if (a.probs) a.probs[row] = (float)((double)p[j] / (double)total);
+      }
+      run += p[j];
+    }
+  });
 }
 
-// Longest row that one workgroup takes. (One row of 1000, 4096, 8192 and 16000 logits with
-// all filters: 9, 11, 15 and 19 us against 16, 17, 18 and 17 in slices; by top-p alone 8, 12,
-// 18 and 28 us against 16, 18, 20 and 19; 1024 rows of 8192: 34 us against 49.)
-constexpr int kRow = 8192;
+// Longest row that one workgroup takes. (One row of 1000, 4096, 8192 and 12288 logits with
+// all filters: 8, 10, 12 and 14 us against 15, 17, 18 and 17 in slices; by top-p alone 8, 11,
+// 15 and 19 us against 16, 19, 20 and 19; 1024 rows of 12288: 39 us against 56.)
+constexpr int kRow = 12288;
 
 // Rows of one round of launches: their workspaces take some hundred megabytes at most.
 constexpr int kRowsAtOnce = 1024;

@@ -329,3 +329,15 @@ def test_two_sessions_at_once():
         t.join()
     assert not failed
     assert all(t.tolist() == want[i] for i in range(2) for t in got[i])
+
+
+@pytest.mark.parametrize("vocab", [2047, 2049, 10007, 12287, 12288, 12289])
+@pytest.mark.parametrize("kind", ["plain", "ties", "banned", "equal", "wide"])
+def test_rows_about_the_longest_of_one_workgroup(s, vocab, kind):
+    print(f"[case] sample vocab={vocab} {kind} about the longest row of one workgroup", flush=True)
+    rng = np.random.default_rng(vocab * 3 + len(kind))
+    rows = ROWS + HARD
+    x = logits(rng, len(rows), vocab, kind)
+    u = np.minimum(rng.random(len(rows)), 1 - 2.0 ** -24).astype(np.float32)
+    compare(x, u, rows, run(s, x, u, rows))
+    s.sync()
