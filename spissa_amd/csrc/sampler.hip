@@ -182,8 +182,14 @@ __device__ __forceinline__ void each(const float *x, int from, int to, F f, G do
 }
 
 __device__ __forceinline__ u64 wave_least(u64 v) {
-  for (int d = 32; d > 0; d >>= 1) v = min(v, __shfl_xor(v, d));
-  return v;
+  v = ~v;  // (lane shifts bring zeros where there is no lane)
+  v = max(v, dpp_of<0x111, 0xf>(v));
+  v = max(v, dpp_of<0x112, 0xf>(v));
+  v = max(v, dpp_of<0x114, 0xf>(v));
+  v = max(v, dpp_of<0x118, 0xf>(v));
+  v = max(v, dpp_of<0x142, 0xa>(v));
+  v = max(v, dpp_of<0x143, 0xc>(v));
+  return ~last_lane(v);
 }
 
 __device__ __forceinline__ u64 block_sum(u64 v, u64 *part) {
@@ -532,8 +538,8 @@ __device__ __forceinline__ u64 select(All all, Value value, u64 want, u64 base, 
 __device__ __attribute__((noinline)) u64 weigh_apart(Weigh weigh, float x, double least) { return weigh(x, least); }
 
 // What a workgroup needs to find the last kept token.
-struct Choice {
-  u64 part[NT / 64], bins[BINS], few[FEW], values[FEW], runs[FEW], ends[2];
+struct alignas(16) Choice {
+  u64 part[NT / 64], bins[BINS], few[FEW + 32], values[FEW + 32], runs[FEW], ends[2];
   unsigned ranks[FEW], many;
   int bin;
   Select select;
@@ -549,14 +555,19 @@ __device__ __forceinline__ u64 last_kept(const Row &r, W weigh, const u64 *list,
   unsigned rank;
   u64 run;
   auto order = [&](int m) {
+    const int share = (m + 4 * NT / 64 - 1) / (4 * NT / 64) * 4, from = (t >> 6) * share;  // of a wave
+    if (t >= m && t < NT / 64 * share) c.few[t] = 0;  // (before none)
+    __syncthreads();
     for (int j = t & 63; j < m; j += 64) {
       const u64 e = c.few[j];
       unsigned before = 0;
       u64 sum = 0;
-#pragma unroll 4
-      for (int i = t >> 6; i < m; i += NT / 64) {
-        before += c.few[i] > e;
-        sum += c.few[i] > e ? c.values[i] : 0;
+#pragma unroll 2
+      for (int i = from; i < from + share; i += 4) {
+        const ulonglong2 a = *reinterpret_cast<const ulonglong2 *>(c.few + i), b = *reinterpret_cast<const ulonglong2 *>(c.few + i + 2);
+        const ulonglong2 x = *reinterpret_cast<const ulonglong2 *>(c.values + i), y = *reinterpret_cast<const ulonglong2 *>(c.values + i + 2);
+        before += (a.x > e) + (a.y > e) + (b.x > e) + (b.y > e);
+        sum += (a.x > e ? x.x : 0) + (a.y > e ? x.y : 0) + (b.x > e ? y.x : 0) + (b.y > e ? y.y : 0);
       }
       atomicAdd(&c.ranks[j], before);
       atomicAdd(&c.runs[j], sum);
