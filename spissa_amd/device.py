@@ -44,7 +44,9 @@ def _cache_array(caches, optional: bool = False):
             return _ONE_HANDLE(c.handle.value)
     arr = (_ffi.c_void_p * max(1, len(caches)))()
     for i, c in enumerate(caches):
-        arr[i] = None if optional and c is None else c.handle.value
+        if c is not None or not optional:
+            h = c._h  # (c.handle refuses a closed cache; asked for each of many it is a fifth of a short call)
+            arr[i] = h.value if h is not None else c.handle.value
     return arr
 
 

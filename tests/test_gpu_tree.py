@@ -804,3 +804,77 @@ def test_two_sessions_at_once(gpu):
         t.join()
     assert not failed
     assert all(torch.equal(o, want[i]) for i in range(2) for o in got[i])
+
+
+def test_a_closed_cache_is_refused(gpu, s):
+    dr = Draft(s, np.random.default_rng(0), (4, 2, 64), [5, 6, 7], [2, 1, 3])
+    dr.caches[1].close()
+    with pytest.raises(gpu.ArgumentError):
+        dr.run(s)
+    assert [len(dr.caches[0]), len(dr.caches[2])] == [5, 7]
+
+
+def test_a_whole_drafted_step_in_a_graph(gpu):
+    """Two layers' tree steps, sampling, the walk and the move captured as one graph: replayed with new inputs, with
+    eager calls of the same session between the replays, each replay equal to the same calls made eagerly."""
+    import torch
+
+    from spissa_amd.device import SamplingConfig, Session
+
+    rng = np.random.default_rng(31)
+    stream = torch.cuda.Stream()
+    ses = Session(0, stream=stream)
+    past, nodes, vocab, heads = [40, 333], [7, 12], 9001, (8, 2, 64)
+    n = sum(nodes)
+    with torch.cuda.stream(stream):
+        layers = [Draft(ses, rng, heads, past, nodes) for _ in range(2)]
+        twins = [[d.cache(ses, b) for b in range(2)] for d in layers]
+        ins = [{k: dev(getattr(d, k)) for k in "qkv"} for d in layers]
+        parents, drafted = layers[0].flat_parents(), torch.zeros(n, dtype=torch.int32, device="cuda")
+        logits, u = torch.zeros(n, vocab, device="cuda"), torch.zeros(n, device="cuda")
+        cfg = SamplingConfig(0.8, 3, 0.9, 0.0)
+
+        def step(caches):
+            """(outputs, sampled, path, count, next): new tensors."""
+            outs = [torch.zeros(n, 8, 64, device="cuda") for _ in layers]
+            ints = [torch.zeros(m, dtype=torch.int32, device="cuda") for m in (n, n, 2, 2)]
+            for i in range(2):
+                ses.tree_step(None, ins[i]["q"], ins[i]["k"], ins[i]["v"], caches[i], nodes, parents, layers[i].config(), outs[i])
+            ses.sample(logits, u, cfg, ints[0])
+            ses.tree_accept(parents, drafted, ints[0], nodes, *ints[1:])
+            ses.keep_rows([c for cs in caches for c in cs], nodes, ints[1], ints[2])
+            return outs + ints
+
+        def back(caches):
+            for cs in caches:
+                for c, p in zip(cs, past):
+                    c.truncate(p)
+
+        mine = [d.caches for d in layers]
+        step(mine)
+        back(mine)
+        ses.sync()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            got = step(mine)
+        walked = set()
+        for _ in range(4):
+            for i in ins:
+                for x in i.values():
+                    x.copy_(torch.as_tensor(rng.normal(size=tuple(x.shape)).astype(np.float32)))
+            logits.copy_(torch.as_tensor(rng.normal(size=(n, vocab)).astype(np.float32)))
+            u.copy_(torch.as_tensor(rng.random(n).astype(np.float32)))
+            # drafts that sampling often confirms: the largest logit after the parent
+            best = logits.argmax(1).int()
+            drafted.copy_(torch.where(parents >= 0, best[torch.cat([parents[:7].clamp(min=0), parents[7:].clamp(min=0) + 7]).long()], best))
+            graph.replay()
+            want = step(twins)
+            ses.sync()
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+            walked |= set(got[4].tolist())
+            for i in range(2):
+                for b in range(2):
+                    for x, y in zip(held(ses, mine[i][b], past[b], nodes[b]), held(ses, twins[i][b], past[b], nodes[b])):
+                        assert np.array_equal(x, y)
+            back(twins)
+        assert max(walked) > 1  # (some walks go on)
