@@ -45,7 +45,8 @@ def _cache_array(caches, optional: bool = False):
     arr = (_ffi.c_void_p * max(1, len(caches)))()
     for i, c in enumerate(caches):
         if c is not None or not optional:
-            h = c._h  # (c.handle refuses a closed cache; asked for each of many it is a fifth of a short call)
+            # (a call of the property for each of many is a fifth of a short step's host time)
+            h = getattr(c, "_h", None)
             arr[i] = h.value if h is not None else c.handle.value
     return arr
 
