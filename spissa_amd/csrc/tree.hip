@@ -564,12 +564,15 @@ __global__ __launch_bounds__(512, 2) void tree_attend_kernel(const TreeArgsOf<MB
           } else {
             rescale = false;
             kbits = scale_to(unbits(km), 11);
-            unsigned now = scale_to(unbits(vm), 11);
-            if (tile > t0) now = min(now, vbits);  // (the output so far only ever gets smaller)
-            const float keep = unbits(now) * inverse_scale(vbits);
-            vbits = now;
+            const unsigned now = scale_to(unbits(vm), 11);
+            if (tile == t0) {  // (there is no output yet, and a first scale may be 2^-116 where one above 2^11 is due)
+              vbits = now;
+            } else if (now < vbits) {  // (the output so far only ever gets smaller)
+              const float keep = unbits(now) * inverse_scale(vbits);
+              vbits = now;
 #pragma unroll
-            for (int d = 0; d < DT; ++d) o[d] *= keep;
+              for (int d = 0; d < DT; ++d) o[d] *= keep;
+            }
           }
           __syncthreads();  // (the tile's largest is read, its bad keys cleared)
         }

@@ -878,3 +878,51 @@ def test_a_whole_drafted_step_in_a_graph(gpu):
                         assert np.array_equal(x, y)
             back(twins)
         assert max(walked) > 1  # (some walks go on)
+
+
+@pytest.mark.parametrize("heads", [(24, 8, 128), (8, 2, 64), (4, 1, 256)])
+@pytest.mark.parametrize("where", ["key", "value"])
+@pytest.mark.parametrize("past,window", [([0, 0], 0), ([150, 40], 0), ([0, 0], 3), ([150, 40], 60)])
+@pytest.mark.parametrize("size", [0.01, 0.25, 0.0])
+def test_what_is_not_finite_beside_values_below_one(gpu, s, heads, where, past, window, size):
+    """As models' values are: the scale that the rest of a first tile takes is far above the one that a number
+    which is not finite leads to. (size 0: all other values nothing; then the outputs are nothing.)"""
+    print(f"[case] NaN in a drafted {where} {heads} past={past} window={window} size={size}", flush=True)
+    rng = np.random.default_rng(17)
+    dr = Draft(s, rng, heads, past, [40, 7], vscale=size)
+    bad = 11
+    (dr.k if where == "key" else dr.v)[bad, heads[1] - 1, 5] = np.nan
+    out = dr.run(s, window=window).cpu().numpy()
+    with pytest.raises(gpu.InvalidTensorDataError):
+        s.sync()
+    s.sync()
+    dr.k[bad] = dr.v[bad] = 0
+    want, _ = dr.plain(window=window)
+    sees = np.zeros(47, bool)
+    sees[:40] = drafts.seen(dr.parents[0], 0, window)[:, bad]
+    assert sees.any() and not sees.all()
+    if size:
+        assert rows_off(out[~sees], want[~sees]) <= ROW
+    else:
+        assert (out[~sees] == 0).all()
+    assert np.isnan(out[sees][:, -(heads[0] // heads[1]):]).all()
+
+
+@pytest.mark.parametrize("heads", [(24, 8, 128), (8, 2, 64), (4, 1, 256)])
+@pytest.mark.parametrize("what", [np.nan, np.inf])
+def test_a_cached_value_that_is_not_finite_and_that_deeper_nodes_do_not_see(gpu, s, heads, what):
+    rng = np.random.default_rng(18)
+    dr = Draft(s, rng, heads, [400], [30], vscale=0.01)
+    depth = np.array(drafts.depths(dr.parents[0]))
+    at = 400 + 4 + 1 - 100 - 1  # with a window of 100 seen by depths 0..3
+    dr.pv[0][at, 0, 3] = what
+    dr.caches = [dr.cache(s, 0)]
+    out = dr.run(s, window=100).cpu().numpy()
+    with pytest.raises(gpu.InvalidTensorDataError):
+        s.sync()
+    dr.pv[0][at] = 0
+    want, _ = dr.plain(window=100)
+    sees, group = depth <= 3, heads[0] // heads[1]
+    assert (~sees).any() and rows_off(out[~sees], want[~sees]) <= ROW and np.isnan(out[sees][:, :group]).all()
+    if heads[1] > 1:  # (the other KV heads' rows do not see it either)
+        assert np.isfinite(out[:, group:]).all()
