@@ -361,7 +361,7 @@ struct TreeBase {
   float *out;
   char *queries;                 // of 16 rows each: tree_query_bytes(D)
   unsigned *mask;                // [N][kTreeMaxNodes / 32]: the nodes that a node sees
-  float *part;                   // [workgroups of a unit][N * Hq] entries of D + 4 floats: output, largest score, sum
+  float *part;                   // [workgroups of a unit][N * Hq] entries of D + 4 floats: output, its weights' reference, sum
   const float *cos, *sin;        // RoPE table rows by position, or null
   const float *q_norm, *k_norm;  // QK-norm, or null
   float eps, prescale;

@@ -424,7 +424,9 @@ __global__ __launch_bounds__(512, 2) void tree_attend_kernel(const TreeArgsOf<MB
     }
 
     f32x4 o[DT];
-    float m = NEG_INF, l = 0.0f;  // m: the largest score so far, or up to 7 below it
+    // Weights are 2^(score - m): m is 8 below the largest score so far, or up to 15 below it;
+    // not less than 8 below where the numbers there are further apart, as 2^16 is no binary16.
+    float m = NEG_INF, l = 0.0f;
     bool poison = false;
 #pragma unroll
     for (int d = 0; d < DT; ++d) o[d] = (f32x4){0.f, 0.f, 0.f, 0.f};
@@ -503,14 +505,15 @@ __global__ __launch_bounds__(512, 2) void tree_attend_kernel(const TreeArgsOf<MB
 #pragma unroll
       for (int k = 0; k < KB; ++k) big = fmaxf(big, fmaxf(fmaxf(sc[k][0], sc[k][1]), fmaxf(sc[k][2], sc[k][3])));
       big = max32(max16(big)) * f;
-      if (__any(big > m + 7.0f)) {
-        const float next = big > m + 7.0f ? big : m, keep = fast_exp2(m - safe_max(next));
+      if (__any(big - m > 15.0f)) {
+        const float below = big - (big - (big - 8.0f) > 8.0f ? 0.0f : 8.0f);
+        const float next = big - m > 15.0f ? below : m, keep = fast_exp2(m - safe_max(next));
         m = next;
         l *= keep;
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[d] *= keep;
       }
-      const float off = 8.0f - safe_max(m);  // weights times 2^8, up to 2^15
+      const float off = -safe_max(m);
       half8 ph[VB], pl[VB];
 #pragma unroll
       for (int v = 0; v < VB; ++v) {

@@ -926,3 +926,18 @@ def test_a_cached_value_that_is_not_finite_and_that_deeper_nodes_do_not_see(gpu,
     assert (~sees).any() and rows_off(out[~sees], want[~sees]) <= ROW and np.isnan(out[sees][:, :group]).all()
     if heads[1] > 1:  # (the other KV heads' rows do not see it either)
         assert np.isfinite(out[:, group:]).all()
+
+
+@pytest.mark.parametrize("heads", [(24, 8, 128), (8, 2, 64), (4, 1, 256)])
+@pytest.mark.parametrize("past", [250, 3000])
+@pytest.mark.parametrize("scale", [1e6, 1e7, 1e8, 1e9, 1e10, 1e12, 1e30])
+def test_scores_of_any_size(s, heads, past, scale):
+    """Scores of 2^20 and more, between whose numbers in f32 lie 8, 16 and more: every row is the value of its largest
+    score, to the pieces' 2^-23, as the two largest of a row lie far more than 2^-20 of themselves apart."""
+    print(f"[case] queries of {scale} {heads} past={past}", flush=True)
+    rng = np.random.default_rng(28)
+    dr = Draft(s, rng, heads, [past], [10])
+    dr.q *= np.float32(scale)
+    out = dr.run(s).cpu().numpy()
+    s.sync()
+    assert rows_off(out, dr.plain()[0]) <= ROW
