@@ -280,12 +280,20 @@ __device__ __forceinline__ TreeUnit tree_unit(const Args &a, int at) {
 // the values' keys being stored in that order. Channels of the scores' product come as
 // 4 l..4 l + 3 beside D / 2 + 4 l..., as the rotation pairs them.
 //
-// Scales. Pieces hold 2^-23 of a number only between 2^-3 and 2^16. Keys and values
-// are multiplied by a power of two that takes the first tile's largest to 2^11..2^12.
-// Each tile's largest is known after it is written; one that does not fit (or is not
-// finite) is loaded and written again, with the scale that it needs, the output so
-// far following, or, where a number is not finite, with zeros in its place and its key
-// noted: rows that see such a key become NaN.
+// Scales. Pieces hold 2^-23 of a number only between 2^-3 and 2^16, and 2^-25 below. Keys
+// and values are multiplied by a power of two that takes the first tile's largest to
+// 2^11..2^12. Whether a tile's largest number is above 2^15, or four channels of one of its
+// rows all below 2^-2 (and not 0), is known after it is written. Such a tile is loaded and written again with a scale of its own; one whose rows no scale takes
+// together (more than 2^13 apart, or one not finite) in parts, from the largest keys
+// down, each with zeros in the place of the other rows, which nobody sees in that turn. So
+// every row is held to 2^-23 of its own largest, whatever stands beside it. A row with a
+// number that is not finite is in no part, but noted: nodes that see it become NaN.
+//
+// An output row is held times a power of two, its unit: the values' scale, as long as that
+// stays. Where it changes, a row takes the new one unless that costs it what it holds: one
+// whose weights are small (or nothing) beside larger values keeps its unit, and one that holds
+// large values keeps it where smaller ones follow; their weights are then multiplied by
+// what the two differ by.
 //
 // Work. The launch's units (a KV head of a block of rows of a sequence) lie one after
 // the other with their tiles, and a workgroup takes `share` of them in a row, of one
@@ -308,8 +316,12 @@ __global__ __launch_bounds__(512, 2) void tree_attend_kernel(const TreeArgsOf<MB
   static_assert(KB * G == 16 && VB * DT == 16, "a tile has 8192 keys' and as many values' channels");
   __shared__ __attribute__((aligned(16))) half8 pieces_lds[2][2][2][1024];  // values, buffer, piece
   half8 (*const kp_lds)[2][1024] = pieces_lds[0], (*const vp_lds)[2][1024] = pieces_lds[1];
-  __shared__ __attribute__((aligned(16))) unsigned most_lds[2][8];
-  __shared__ unsigned bad_lds[VB];
+  constexpr int kSpan = 13;  // powers of two between the largest rows of a part and its smallest
+  __shared__ __attribute__((aligned(16))) unsigned most_lds[2][8], least_lds[2][8];
+  __shared__ __attribute__((aligned(8))) unsigned char unfit_lds[2][8];
+  __shared__ unsigned size_lds[2 * BN];  // of a tile in parts: its keys' largest, then its values', as bits
+  __shared__ unsigned bad_lds[VB], left_lds[VB], take_lds[VB], scale_lds[3];
+  __shared__ int unit_lds[8][16];
 
   float minus_one = -1.0f;
   asm volatile("" : "+s"(minus_one));
@@ -356,16 +368,27 @@ __global__ __launch_bounds__(512, 2) void tree_attend_kernel(const TreeArgsOf<MB
         raw[i] = *reinterpret_cast<const f32x4 *>(src + at * 4u);
       }
     };
-    // The wave's largest magnitude, as bits (a NaN or an infinity is above the rest).
-    auto post = [&](int slot, const f32x4 (&cur)[8]) __attribute__((always_inline)) {
-      unsigned m = 0;
+    auto bits_of = [&](const f32x4 &x) __attribute__((always_inline)) {
+      return max(max(__float_as_uint(x[0]) & 0x7fffffffu, __float_as_uint(x[1]) & 0x7fffffffu),
+                 max(__float_as_uint(x[2]) & 0x7fffffffu, __float_as_uint(x[3]) & 0x7fffffffu));
+    };
+    // The wave's largest magnitude, as bits (a NaN or an infinity is above the rest), and
+    // the smallest of four channels' largest less 1 (four zeros are above the rest).
+    auto post = [&](int slot, const f32x4 (&cur)[8]) __attribute__((always_inline)) -> uint2 {
+      unsigned m = 0, s = ~0u;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        m = max(m, max(__float_as_uint(cur[i][0]) & 0x7fffffffu, __float_as_uint(cur[i][1]) & 0x7fffffffu));
-        m = max(m, max(__float_as_uint(cur[i][2]) & 0x7fffffffu, __float_as_uint(cur[i][3]) & 0x7fffffffu));
+        const unsigned of = bits_of(cur[i]);
+        m = max(m, of);
+        s = min(s, of - 1u);
       }
       m = wave_max_bits(m);
-      if (lane == 0) most_lds[slot][wave] = m;
+      s = ~wave_max_bits(~s);
+      if (lane == 0) {
+        most_lds[slot][wave] = m;
+        least_lds[slot][wave] = s;
+      }
+      return uint2{m, s};
     };
     unsigned kbits = 127u << 23, vbits = 127u << 23;  // the scales, as float bits
     auto write = [&](int buf, const f32x4 (&cur)[8]) __attribute__((always_inline)) {
@@ -400,7 +423,11 @@ __global__ __launch_bounds__(512, 2) void tree_attend_kernel(const TreeArgsOf<MB
     };
     auto largest = [&](int slot, int from) __attribute__((always_inline)) {
       const uint4 m = *reinterpret_cast<const uint4 *>(most_lds[slot] + from);
-      return max(max(m.x, m.y), max(m.z, m.w));
+      return __builtin_amdgcn_readfirstlane(max(max(m.x, m.y), max(m.z, m.w)));
+    };
+    auto smallest = [&](int slot, int from) __attribute__((always_inline)) {
+      const uint4 m = *reinterpret_cast<const uint4 *>(least_lds[slot] + from);
+      return __builtin_amdgcn_readfirstlane(min(min(m.x, m.y), min(m.z, m.w)));
     };
 
     half8 qh[G], ql[G];
@@ -428,10 +455,11 @@ __global__ __launch_bounds__(512, 2) void tree_attend_kernel(const TreeArgsOf<MB
     // not less than 8 below where the numbers there are further apart, as 2^16 is no binary16.
     float m = NEG_INF, l = 0.0f;
     bool poison = false;
+    int units = 0;  // the wave's rows' unit, as a float's exponent, or -1: each its own, in unit_lds
 #pragma unroll
     for (int d = 0; d < DT; ++d) o[d] = (f32x4){0.f, 0.f, 0.f, 0.f};
 
-    auto compute = [&](int tile, bool bad) __attribute__((always_inline)) {
+    auto compute = [&](int tile, bool parts) __attribute__((always_inline)) {
       const int buf = tile & 1;
       const bool own = tile >= cached;
       const int base = lo + tile * BN;
@@ -481,7 +509,7 @@ __global__ __launch_bounds__(512, 2) void tree_attend_kernel(const TreeArgsOf<MB
       }
       // (finite and above 0: hidden scores stay -inf)
       const float f = fminf(fmaxf(inv_q * inverse_scale(kbits), 1.1754944e-38f), 3.402823466e38f);
-      if (own || bad || base + BN > past || base < wave_lo) {
+      if (own || parts || base + BN > past || base < wave_lo) {
 #pragma unroll
         for (int v = 0; v < VB; ++v) {
           const int first = 32 * v;  // of the tile
@@ -495,7 +523,10 @@ __global__ __launch_bounds__(512, 2) void tree_attend_kernel(const TreeArgsOf<MB
             const int from = max(0, row_lo - base - first), to = min(32, past - base - first);
             seen = from >= 32 || to <= from ? 0u : (0xffffffffu << from) & (0xffffffffu >> (32 - to));
           }
-          if (bad) poison |= (seen & bad_lds[v]) != 0;
+          if (parts) {
+            poison |= (seen & bad_lds[v]) != 0;
+            seen &= take_lds[v];
+          }
 #pragma unroll
           for (int i = 0; i < 8; ++i)
             if (!(seen >> ((i & 3) + 4 * kq + 16 * (i >> 2)) & 1u)) sc[2 * v + (i >> 2)][i & 3] = NEG_INF;
@@ -514,6 +545,32 @@ __global__ __launch_bounds__(512, 2) void tree_attend_kernel(const TreeArgsOf<MB
         for (int d = 0; d < DT; ++d) o[d] *= keep;
       }
       const float off = -safe_max(m);
+      int lift = 0;  // what the row's unit is above the values' scale
+      const int scale = (int)(vbits >> 23);
+      if (units != scale) {
+        int unit = units >= 0 ? units : unit_lds[wave][col];
+        float most = 0.0f;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) most = fmaxf(fmaxf(most, fmaxf(fabsf(o[d][0]), fabsf(o[d][1]))), fmaxf(fabsf(o[d][2]), fabsf(o[d][3])));
+        most = max32(max16(most));
+        const int held = (int)(__float_as_uint(most) >> 23) - 127;
+        // (the largest weight of the tile is 2^weight; times the lift it stays below 2^15)
+        const int weight = (int)ceilf(fmaxf(big + off, -1000.0f)), room = 15 - weight;
+        int shift = scale - unit;
+        if (shift > 0 && most > 0.0f) shift = min(shift, max(0, 64 - held));
+        if (shift < 0 && weight < 0 && (most > 0.0f ? held + shift < 16 : weight > -1000)) shift = min(0, shift + room);
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[d][i] = __builtin_ldexpf(o[d][i], shift);
+        }
+        unit += shift;
+        unit_lds[wave][col] = unit;
+        lift = unit - scale;
+        const int first = __builtin_amdgcn_readfirstlane(unit);
+        units = __all(unit == first) ? first : -1;
+      }
+      const bool lifted = units != scale;
       half8 ph[VB], pl[VB];
 #pragma unroll
       for (int v = 0; v < VB; ++v) {
@@ -522,6 +579,10 @@ __global__ __launch_bounds__(512, 2) void tree_attend_kernel(const TreeArgsOf<MB
         for (int i = 0; i < 8; ++i) {
           p[i] = fast_exp2(fmaf(sc[2 * v + (i >> 2)][i & 3], f, off));
           l += p[i];
+        }
+        if (lifted) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) p[i] = __builtin_ldexpf(p[i], lift);
         }
         split8(p, minus_one, &ph[v], &pl[v]);
       }
@@ -542,68 +603,115 @@ __global__ __launch_bounds__(512, 2) void tree_attend_kernel(const TreeArgsOf<MB
     };
 
     constexpr unsigned kInfinite = 0x7f800000u;
-    constexpr unsigned kTop = (127u + 15u) << 23;  // 2^15
+    constexpr unsigned kTop = (127u + 15u) << 23, kLow = (2u * 127u - 2u) << 23;  // 2^15; 2^-2, biased twice
     // Between two barriers a wave writes its share of a tile and computes its part of the
     // one before. A tile that has to be written again takes a turn of its own, one in
-    // which something is not finite two, as the largest of the rest is not known before it
-    // is written. In the first turn there is nothing to compute, and the scales are set
-    // between reading the tile's largest and writing it.
-    bool bad = false, rescale = false;
+    // parts two for each but the last. In the first turn there is nothing to compute, and
+    // the scales are set between reading the tile's largest and writing it.
+    enum : int { kLook, kFits, kParts, kNextPart };  // (of the tile that is written: to be looked at, or why it was written again)
+    int mode = kLook;
 #pragma unroll 1
     for (int tile = t0 - 1; tile < t1;) {
       // (addresses anew each time)
       asm volatile("" : "+v"(thread_key), "+v"(thread_channel), "+v"(kl), "+v"(vl), "+v"(vb0), "+v"(vq), "+v"(col), "+v"(kq));
-      bool again = false;
-      if (tile >= t0) {
-        const unsigned km = largest(tile & 1, 4), vm = largest(tile & 1, 0);
-        const bool more = km >= kInfinite || vm >= kInfinite;
-        // (the largest times the scale, by exponents: bits of both less the bias)
-        again = more || rescale || km > kTop - kbits + (127u << 23) || vm > kTop - vbits + (127u << 23);
+      bool again = mode == kNextPart;
+      if (tile >= t0 && mode == kLook) {
+        const uint2 unfit = *reinterpret_cast<const uint2 *>(unfit_lds[tile & 1]);
+        again = __builtin_amdgcn_readfirstlane(unfit.x | unfit.y) != 0;
         if (again) {
-          load(tile);
-          if (more) {
-            bad = rescale = true;
+          const unsigned km = largest(tile & 1, 4), vm = largest(tile & 1, 0);
+          const unsigned ks = smallest(tile & 1, 4), vs = smallest(tile & 1, 0);
+          mode = kFits;
+          if (km >= kInfinite || vm >= kInfinite || (ks >> 23) + kSpan < km >> 23 || (vs >> 23) + kSpan < vm >> 23) {
+            mode = kParts;
+            for (int i = tid; i < 2 * BN; i += 512) size_lds[i] = 0;
             if (tid < VB) bad_lds[tid] = 0;
           } else {
-            rescale = false;
             kbits = scale_to(unbits(km), 11);
-            const unsigned now = scale_to(unbits(vm), 11);
-            if (tile == t0) {  // (there is no output yet, and a first scale may be 2^-116 where one above 2^11 is due)
-              vbits = now;
-            } else if (now < vbits) {  // (the output so far only ever gets smaller)
-              const float keep = unbits(now) * inverse_scale(vbits);
-              vbits = now;
-#pragma unroll
-              for (int d = 0; d < DT; ++d) o[d] *= keep;
-            }
+            vbits = scale_to(unbits(vm), 11);
           }
-          __syncthreads();  // (the tile's largest is read, its bad keys cleared)
         }
       }
-      const int target = again ? tile : tile + 1;
+      const bool hold = !again && mode == kParts && __builtin_amdgcn_readfirstlane(scale_lds[2]);  // (a part of the tile is still to be written)
+      const int target = again ? tile : hold ? t1 : tile + 1;
+      if (again) {
+        load(tile);
+        __syncthreads();  // (the tile's largest is read)
+      }
       if (target < t1) {
         f32x4 cur[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) cur[i] = raw[i];
-        if (again && bad) {
+        if (again && mode != kFits) {
+          if (mode == kParts) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int key = thread_key + step_key(i);
+              const unsigned of = bits_of(cur[i]);
+              if (of >= kInfinite) atomicOr(&bad_lds[key >> 5], 1u << (key & 31));
+              else atomicMax(&size_lds[(values ? BN : 0) + key], of);
+            }
+            __syncthreads();
+          }
+          if (wave == 0) {  // the next part: the largest keys left, and of those the largest values
+            constexpr int PER = (BN + 63) / 64;
+            unsigned key_size[PER], value_size[PER], km = 0, vm = 0;
+            bool in[PER];
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+              const int key = min(lane + 64 * i, BN - 1);
+              const unsigned words = mode == kParts ? ~bad_lds[key >> 5] : left_lds[key >> 5];
+              in[i] = lane + 64 * i < BN && (words >> (key & 31) & 1u);
+              key_size[i] = in[i] ? size_lds[key] : 0;
+              value_size[i] = size_lds[BN + key];
+              km = max(km, key_size[i]);
+            }
+            km = wave_max_bits(km);
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+              const bool near = in[i] && (key_size[i] == 0 || (key_size[i] >> 23) + kSpan >= km >> 23);
+              value_size[i] = near ? value_size[i] : kInfinite;
+              vm = max(vm, near ? value_size[i] : 0u);
+            }
+            vm = wave_max_bits(vm);
+            bool more = false;
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+              const bool now = value_size[i] == 0 || (value_size[i] < kInfinite && (value_size[i] >> 23) + kSpan >= vm >> 23);
+              const unsigned long long taken = __ballot(now), left = __ballot(in[i] && !now);
+              more |= left != 0;
+              if (lane < min(2, VB - 2 * i)) {
+                take_lds[2 * i + lane] = (unsigned)(taken >> (32 * lane));
+                left_lds[2 * i + lane] = (unsigned)(left >> (32 * lane));
+              }
+            }
+            if (lane == 0) {
+              scale_lds[0] = scale_to(unbits(km), 11);
+              scale_lds[1] = scale_to(unbits(vm), 11);
+              scale_lds[2] = more;
+            }
+          }
+          __syncthreads();
+          kbits = __builtin_amdgcn_readfirstlane(scale_lds[0]);
+          vbits = __builtin_amdgcn_readfirstlane(scale_lds[1]);
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            bool wrong = false;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const bool fine = fabsf(cur[i][j]) < __builtin_inff();
-              cur[i][j] = fine ? cur[i][j] : 0.0f;
-              wrong |= !fine;
-            }
             const int key = thread_key + step_key(i);
-            if (wrong) atomicOr(&bad_lds[key >> 5], 1u << (key & 31));
+            if (!(take_lds[key >> 5] >> (key & 31) & 1u)) cur[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
           }
+          mode = kParts;
         }
-        post(target & 1, cur);
+        uint2 ends;
+        if (!again) ends = post(target & 1, cur);
         if (tile < t0) {
           __syncthreads();
           kbits = scale_to(unbits(min(largest(t0 & 1, 4), kInfinite - 1)), 11);
           vbits = scale_to(unbits(min(largest(t0 & 1, 0), kInfinite - 1)), 11);
+          units = (int)(vbits >> 23);
+        }
+        if (!again && lane == 0) {  // (a number times the scale, by exponents: bits of both less the bias)
+          const unsigned of = values ? vbits : kbits;
+          unfit_lds[target & 1][wave] = ends.x >= kInfinite || ends.x > kTop + (127u << 23) - of || ends.y < kLow - min(of, kLow);
         }
         write(target & 1, cur);
       }
@@ -613,10 +721,10 @@ __global__ __launch_bounds__(512, 2) void tree_attend_kernel(const TreeArgsOf<MB
 #pragma unroll
         for (int i = 0; i < 8; ++i) asm volatile("" : "=v"(raw[i]));
       }
-      if (tile >= t0 && !again && busy) compute(tile, bad);
       if (!again) {
-        bad = false;
-        ++tile;
+        if (tile >= t0 && busy) compute(tile, mode == kParts);
+        mode = hold ? kNextPart : kLook;
+        if (!hold) ++tile;
       }
       __syncthreads();
     }
@@ -624,7 +732,7 @@ __global__ __launch_bounds__(512, 2) void tree_attend_kernel(const TreeArgsOf<MB
     l = sum32(sum16(l));
     if (poison) l = __builtin_nanf("");
     if (busy) {
-      const float inv = l == 0.0f ? 0.0f : inverse_scale(vbits) / l;
+      const float inv = l == 0.0f ? 0.0f : inverse_scale((unsigned)(units >= 0 ? units : unit_lds[wave][col]) << 23) / l;
       if (row0 + col < rows) {
         const int node = (row0 + col) / a.R;
         const long orow = (long)(a.seq[unit.b].first + node) * a.Hq + unit.h * a.R + (row0 + col - node * a.R);

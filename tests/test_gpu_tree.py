@@ -941,3 +941,159 @@ def test_scores_of_any_size(s, heads, past, scale):
     out = dr.run(s).cpu().numpy()
     s.sync()
     assert rows_off(out, dr.plain()[0]) <= ROW
+
+
+def with_rows(s, dr):
+    """The draft's caches from its rows as they are now."""
+    dr.caches = [dr.cache(s, i) for i in range(len(dr.past))]
+    return dr
+
+
+def by_scores(dr, window=0):
+    """What the scores' own errors may do to each output row, over the row's 2-norm. A score is a sum of D products
+    of pieces (off by 5 * 2^-24 of each) by 3 D / 32 instructions, off by half a step of their sum at most: for
+    huge keys far more than for the others. An output follows an error e_j of score j by p_j e_j (v_j - out);
+    twice that for errors up to 1."""
+    offs, at = [], 0
+    for p, parents, pk, pv in zip(dr.past, dr.parents, dr.pk, dr.pv):
+        n, r = len(parents), dr.hq // dr.hkv
+        k, v = (np.concatenate([a, b[at:at + n]]).astype(np.float64).repeat(r, 1) for a, b in ((pk, dr.k), (pv, dr.v)))
+        for t, seen in enumerate(drafts.seen(parents, p, window)):
+            q, kk, vv = dr.q[at + t].astype(np.float64), k[seen], v[seen]
+            sc = np.einsum("hd,mhd->mh", q, kk) / np.sqrt(dr.d)
+            w = np.exp(sc - sc.max(0))
+            w /= w.sum(0)
+            e = np.einsum("hd,mhd->mh", np.abs(q), np.abs(kk)) / np.sqrt(dr.d) * (5 + 3 * dr.d / 32) * 2.0 ** -24
+            out = np.einsum("mh,mhd->hd", w, vv)
+            offs.append(2 * np.einsum("mh,mh->h", w * e, np.linalg.norm(vv - out, axis=-1)) / np.linalg.norm(out, axis=-1))
+        at += n
+    return np.stack(offs)
+
+
+def each_off(got, want):
+    return np.linalg.norm(got.astype(np.float64) - want, axis=-1) / np.linalg.norm(want, axis=-1)
+
+
+OUTLIERS = [(24, 8, 128), (8, 2, 64), (4, 1, 256)]
+
+
+@pytest.mark.parametrize("heads", OUTLIERS)
+@pytest.mark.parametrize("where", ["key", "value", "both"])
+@pytest.mark.parametrize("size", [1e5, 1e8, 1e30])
+@pytest.mark.parametrize("past", [[0, 0], [150, 40]])
+def test_a_drafted_row_of_any_size_leaves_the_others(s, heads, where, size, past):
+    """Rows that do not see it are off by no more than without it; those that see it by what its score is off besides."""
+    print(f"[case] {where} of {size} {heads} past={past}", flush=True)
+    rng = np.random.default_rng(19)
+    dr = Draft(s, rng, heads, past, [40, 7])
+    for x, name in ((dr.k, "key"), (dr.v, "value")):
+        if where in (name, "both"):
+            x[11] *= np.float32(size)
+    out = dr.run(s).cpu().numpy()
+    s.sync()
+    want, _ = dr.plain()
+    sees = np.zeros(47, bool)
+    sees[:40] = drafts.seen(dr.parents[0], 0)[:, 11]
+    assert sees.any() and not sees.all()
+    assert rows_off(out[~sees], want[~sees]) <= ROW
+    assert (each_off(out, want) <= ROW + by_scores(dr))[sees].all()
+
+
+@pytest.mark.parametrize("heads", OUTLIERS)
+@pytest.mark.parametrize("where", ["key", "value"])
+@pytest.mark.parametrize("size", [1e8, 1e30])
+def test_a_cached_row_of_any_size_leaves_nodes_that_do_not_see_it(s, heads, where, size):
+    rng = np.random.default_rng(20)
+    dr = Draft(s, rng, heads, [400], [30])
+    at = 400 + 4 + 1 - 100 - 1  # with a window of 100 seen by depths 0..3
+    (dr.pk if where == "key" else dr.pv)[0][at] *= np.float32(size)
+    out = with_rows(s, dr).run(s, window=100).cpu().numpy()
+    s.sync()
+    want, _ = dr.plain(window=100)
+    deep = np.array(drafts.depths(dr.parents[0])) > 3
+    assert deep.any() and not deep.all()
+    assert rows_off(out[deep], want[deep]) <= ROW
+    assert (each_off(out, want) <= ROW + by_scores(dr, 100))[~deep].all()
+
+
+@pytest.mark.parametrize("heads", [(24, 8, 128), (16, 8, 64), (8, 4, 256)])
+@pytest.mark.parametrize("past", [600, 9000])
+@pytest.mark.parametrize("size", [1e5, 1e10, 1e30])
+def test_huge_values_of_no_weight(s, heads, past, size):
+    """Seen, but with scores some 100 below the others': in a first tile with more of them behind it in the same
+    workgroup, and in the middle."""
+    print(f"[case] values of {size} without weight {heads} past={past}", flush=True)
+    rng = np.random.default_rng(21)
+    dr = Draft(s, rng, heads, [past], [5])
+    dr.q = np.abs(dr.q)
+    for at in (0, 300):
+        dr.pk[0][at] = -20 * np.abs(dr.pk[0][at])
+        dr.pv[0][at] *= np.float32(size)
+    out = with_rows(s, dr).run(s).cpu().numpy()
+    s.sync()
+    assert rows_off(out, dr.plain()[0]) <= ROW
+
+
+@pytest.mark.parametrize("heads", OUTLIERS)
+@pytest.mark.parametrize("size", [1e5, 1e30])
+def test_huge_keys_of_no_weight(s, heads, size):
+    rng = np.random.default_rng(22)
+    dr = Draft(s, rng, heads, [5000], [21])
+    dr.q = np.abs(dr.q)
+    for at in (0, 333, 4999):
+        dr.pk[0][at] = -np.abs(dr.pk[0][at]) * np.float32(size)
+    out = with_rows(s, dr).run(s).cpu().numpy()
+    s.sync()
+    assert rows_off(out, dr.plain()[0]) <= ROW
+
+
+@pytest.mark.parametrize("heads", OUTLIERS)
+@pytest.mark.parametrize("at", [0, 250, 699])
+def test_a_huge_value_of_small_weight(s, heads, at):
+    """A weight of e^-28 of the others' and a value of 1e14: shares of the same size."""
+    rng = np.random.default_rng(23)
+    dr = Draft(s, rng, heads, [700], [9])
+    u = rng.normal(size=heads[2])
+    dr.q[:] = u
+    dr.pk[0][at] = u * (-28 * np.sqrt(heads[2]) / (u @ u))
+    dr.pv[0][at] *= np.float32(1e14)
+    out = with_rows(s, dr).run(s).cpu().numpy()
+    s.sync()
+    # (its score is the sum of 3 D / 32 matrix instructions, each off by half a step of 28 at most, and its weight by that share)
+    assert rows_off(out, dr.plain()[0]) <= ROW + 3 * heads[2] / 32 * 28 * 2.0 ** -24
+
+
+@pytest.mark.parametrize("heads", OUTLIERS)
+@pytest.mark.parametrize("past,nodes", [([0], [100]), ([1000], [30]), ([3000, 77], [40, 9])])
+@pytest.mark.parametrize("where", ["values", "small keys", "both"])
+def test_rows_of_all_sizes_in_a_tile(s, heads, past, nodes, where):
+    """Sizes from 2^-40 to 2^40 (keys: to 2^2) without order, a tile's rows held in many parts."""
+    print(f"[case] sizes without order: {where} {heads} past={past} nodes={nodes}", flush=True)
+    rng = np.random.default_rng(24)
+    dr = Draft(s, rng, heads, past, nodes)
+    for keys, rows in ((True, dr.pk + [dr.k]), (False, dr.pv + [dr.v])):
+        for x in rows:
+            if where in ("both", "small keys" if keys else "values"):
+                x *= np.float32(2) ** rng.integers(-40, 3 if keys else 41, (len(x), 1, 1)).astype(np.float32)
+    out = with_rows(s, dr).run(s).cpu().numpy()
+    s.sync()
+    assert rows_off(out, dr.plain()[0]) <= ROW
+
+
+@pytest.mark.parametrize("heads", OUTLIERS)
+def test_a_huge_row_beside_one_that_is_not_finite(gpu, s, heads):
+    rng = np.random.default_rng(25)
+    dr = Draft(s, rng, heads, [90], [40], vscale=0.01)
+    dr.v[11] *= np.float32(1e30)
+    dr.k[17] *= np.float32(-1e12)
+    dr.v[23, 0, 1], dr.k[31, 0, 2] = np.nan, -np.inf
+    out = dr.run(s).cpu().numpy()
+    with pytest.raises(gpu.InvalidTensorDataError):
+        s.sync()
+    s.sync()
+    seen = drafts.seen(dr.parents[0], 0)
+    poisoned = seen[:, 23] | seen[:, 31]
+    dr.v[23] = dr.k[31] = 0
+    want, _ = dr.plain()
+    assert poisoned.any() and rows_off(out[~poisoned], want[~poisoned]) <= ROW
+    assert np.isnan(out[poisoned][:, :heads[0] // heads[1]]).all()
