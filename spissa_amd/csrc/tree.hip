@@ -732,14 +732,15 @@ __global__ __launch_bounds__(512, 2) void tree_attend_kernel(const TreeArgsOf<MB
     l = sum32(sum16(l));
     if (poison) l = __builtin_nanf("");
     if (busy) {
-      const float inv = l == 0.0f ? 0.0f : inverse_scale((unsigned)(units >= 0 ? units : unit_lds[wave][col]) << 23) / l;
+      // (not their product: it would be below 2^-126 for the smallest values)
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l, down = inverse_scale((unsigned)(units >= 0 ? units : unit_lds[wave][col]) << 23);
       if (row0 + col < rows) {
         const int node = (row0 + col) / a.R;
         const long orow = (long)(a.seq[unit.b].first + node) * a.Hq + unit.h * a.R + (row0 + col - node * a.R);
         const bool whole = t0 == 0 && t1 == unit.tiles;
         float *const out = whole ? a.out + orow * D : a.part + ((long)slot_of * a.total + orow) * (D + 4);
 #pragma unroll
-        for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4 *>(out + 16 * d + 4 * kq) = o[d] * inv;
+        for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4 *>(out + 16 * d + 4 * kq) = o[d] * inv * down;
         if (!whole) {
           if (kq == 0) *reinterpret_cast<float2 *>(out + D) = make_float2(m, l);
         } else if (!(l > 0.0f) || l > 3.402823466e38f) {

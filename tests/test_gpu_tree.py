@@ -1097,3 +1097,16 @@ def test_a_huge_row_beside_one_that_is_not_finite(gpu, s, heads):
     want, _ = dr.plain()
     assert poisoned.any() and rows_off(out[~poisoned], want[~poisoned]) <= ROW
     assert np.isnan(out[poisoned][:, :heads[0] // heads[1]]).all()
+
+
+@pytest.mark.parametrize("heads", [(24, 8, 128), (8, 2, 64), (4, 1, 256)])
+@pytest.mark.parametrize("past", [0, 333])
+@pytest.mark.parametrize("scale,vscale", [(1.0, 1e-33), (1.0, 1e-36), (1e-34, 1e-36), (1e-34, 1.0)])
+def test_the_smallest_values(s, heads, past, scale, vscale):
+    """Down to outputs of 2^-126, whose last bit is 2^-149: 2^-24 of the larger half of a row of some 1e-37."""
+    rng = np.random.default_rng(27)
+    dr = Draft(s, rng, heads, [past], [21], scale=scale, vscale=vscale)
+    dr.q /= np.float32(scale)
+    out = dr.run(s).cpu().numpy()
+    s.sync()
+    assert rows_off(out, dr.plain()[0]) <= ROW
