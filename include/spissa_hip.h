@@ -584,12 +584,12 @@ typedef struct {
 } spissa_sampling_config;
 /* d_tokens[r] = the first index at which the running sum of row r's kept
  * weights, taken in index order, is above d_uniform[r] (0 <= u < 1) times their
- * sum; d_probs[r] (d_probs may be NULL) = its share of that sum. d_logits
- * [rows, vocab]. Weights are formed in 64 bits and summed as whole numbers of
- * 2^-51 (of 2^-62 times vocab's next power of two, where that is more), so a
- * row's token does not depend on the order of any sum, nor on the other rows; a
- * token whose weight rounds to 0 is never taken. A setting of the struct that is out of its range is
- * INVALID_TENSOR_DATA. A row with a NaN or +infinite logit, with none above
+ * sum; d_probs[r] (d_probs may be NULL) = its own weight, as formed, over that
+ * sum. d_logits [rows, vocab]. Weights are formed in 64 bits and summed as whole
+ * numbers of 2^-51 (of 2^-62 times vocab's next power of two, where that is
+ * more), so a row's token does not depend on the order of any sum, nor on the
+ * other rows; a token whose weight rounds to 0 is never taken. A setting of the
+ * struct that is out of its range is INVALID_TENSOR_DATA. A row with a NaN or +infinite logit, with none above
  * -infinity, or with a setting or uniform number out of its range gets token -1
  * and probability 0, and the next spissa_session_sync() reports it. The call uses
  * a workspace that grows with its sizes: under graph capture it must follow a

@@ -536,6 +536,11 @@ __device__ __forceinline__ u64 select(All all, Value value, u64 want, u64 base, 
 
 // (a function of its own: a kernel that runs once waits for each line of its code)
 __device__ __attribute__((noinline)) u64 weigh_apart(Weigh weigh, float x, double least) { return weigh(x, least); }
+// A token's share of the kept weights, its own as it was before it became a whole number (of
+// a token 27 temperatures down that is one or two of 2^-40 with 2^22 logits).
+__device__ __attribute__((noinline)) float share_of(Weigh weigh, float x, u64 total) {
+  return (float)(weigh.real(x, weigh.shift) / (double)total);
+}
 
 // What a workgroup needs to find the last kept token.
 struct alignas(16) Choice {
@@ -781,7 +786,7 @@ __global__ __launch_bounds__(NT) void sample_draw_kernel(const SampleArgs a, con
     const u64 sum = run + wave_up_to(p);
     if (sum > draw && sum - p <= draw) {
       a.tokens[row] = i;
-      if (a.probs) a.probs[row] = (float)((double)p / (double)total);
+      if (a.probs) a.probs[row] = share_of(weigher, v[0], total);
     }
     run = last_lane(sum);
     if (run > draw) return;
@@ -893,7 +898,7 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(const SampleArgs a, cons
     for (int j = 0; j < 4; ++j) {
       if (run <= draw && run + p[j] > draw) {
         a.tokens[row] = i + j;
-        if (a.probs) a.probs[row] = (float)((double)p[j] / (double)total);
+        if (a.probs) a.probs[row] = share_of(weigher, v[j], total);
       }
       run += p[j];
     }

@@ -341,3 +341,38 @@ def test_rows_about_the_longest_of_one_workgroup(s, vocab, kind):
     u = np.minimum(rng.random(len(rows)), 1 - 2.0 ** -24).astype(np.float32)
     compare(x, u, rows, run(s, x, u, rows))
     s.sync()
+
+
+def within(x, setting, tokens, probs):
+    """Each probability against the definition's of that token: weights off by (1 + 60) * 2^-52 of themselves in 64 bits
+    (logits up to 60 temperatures down), their sum by half a step of 2^-shift a token, one rounding to f32."""
+    for row, token, prob in zip(x.astype(np.float64), tokens, probs):
+        w = np.exp((row - row.max()) / np.float64(np.float32(setting[0])))
+        order = np.argsort(-row, kind="stable")[:setting[1] or None]
+        if setting[2] < 1:
+            run = np.cumsum(w[order])
+            order = order[:max(1, int(((run - w[order]) < np.float64(np.float32(setting[2])) * run[-1]).sum()))]
+        want = w[token] / w[order].sum()
+        lost = len(row) * 2.0 ** -(1 + min(51, 62 - int(np.ceil(np.log2(max(2, len(row)))))))
+        assert token in order and abs(prob - want) <= want * (2.0 ** -24 + 2.0 ** -45 + lost), (setting, token, prob, want)
+
+
+@pytest.mark.parametrize("vocab", [700, 12288, 12289, 262144, 1 << 22])
+@pytest.mark.parametrize("down", [18.0, 24.0, 27.0])
+@pytest.mark.parametrize("filters", [False, True])
+def test_probabilities_of_rare_tokens(s, vocab, down, filters):
+    """All but one logit `down` temperatures below it and the number above its share: one of them is drawn, with its own
+    probability (weights there are few steps of the whole numbers that are summed)."""
+    print(f"[case] sample vocab={vocab} rare tokens {down} down filters={filters}", flush=True)
+    rng = np.random.default_rng(vocab)
+    x = (np.float32(-down) + rng.uniform(-0.3, 0.3, (3, vocab))).astype(np.float32)
+    x[:, vocab // 3] = 0.0
+    x *= np.float32(0.75)
+    share = vocab * np.exp(-down)
+    # the largest token comes after a third of the others: numbers before and behind its share
+    u = np.array([0.0, 0.2 * share / (1 + share), 1 - 2.0 ** -24], np.float32)
+    setting = (0.75, 0, 1.0, 0.0) if not filters else (0.75, vocab - 1, 1.0, 0.0)
+    tokens, probs = run(s, x, u, [setting] * 3)
+    s.sync()
+    assert tokens[0] != vocab // 3
+    within(x, setting, tokens, probs)
