@@ -425,11 +425,13 @@ class Session:
             _many_i32(path, n, "path") if n else 0, _many_i32(count, b, "count") if b else 0))
 
     def sample(self, logits, uniform, config: SamplingConfig, tokens, probs=None) -> None:
-        """tokens[r] (int32) from each row of logits [rows, vocab] by the settings and the numbers
-        uniform [rows] in [0, 1), probs[r] (float32 or None) its probability (spissa_sample_device)."""
+        """tokens[r] (int32) from each row of logits [rows, vocab] (or all rows in one dimension) by the
+        settings and the numbers uniform [rows] in [0, 1), probs[r] (float32 or None) its probability
+        (spissa_sample_device)."""
         rows = uniform.numel()
-        if logits.numel() % max(1, rows) != 0:
-            raise TypeError(f"{logits.numel()} logits for {rows} rows")
+        shape = logits.shape
+        if len(shape) > 1 and shape[:-1].numel() != rows or logits.numel() % max(1, rows) != 0:
+            raise TypeError(f"logits {tuple(shape)} for {rows} rows")
         cfg = config._c(rows, logits.numel() // max(1, rows))
         check(self._lib.spissa_sample_device(
             self.handle, _dev(logits, "logits"), _dev(uniform, "uniform"), C.byref(cfg),

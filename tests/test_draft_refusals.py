@@ -69,3 +69,14 @@ def test_the_rust_settings_follow_the_header():
 
     assert rust_struct_fields("spissa_sampling_config") == c_struct_fields("spissa_sampling_config")
     assert "#[repr(C)]" in LIB_RS.split("pub struct spissa_sampling_config")[0][-80:]
+
+
+@pytest.mark.parametrize("shape,rows", [((4, 8), 2), ((4, 8), 8), ((2, 2, 8), 2), ((4, 8), 0), ((1, 8), 2), ((3, 0), 1), ((9,), 2)])
+def test_sampling_takes_one_number_a_row(shape, rows):
+    """Rows of logits are not joined or parted, also where their number divides."""
+    import torch
+
+    from spissa_amd.device import SamplingConfig, Session
+
+    with pytest.raises(TypeError, match="rows"):
+        Session.sample(None, torch.zeros(shape), torch.zeros(rows), SamplingConfig(), torch.zeros(rows, dtype=torch.int32))

@@ -376,3 +376,24 @@ def test_probabilities_of_rare_tokens(s, vocab, down, filters):
     s.sync()
     assert tokens[0] != vocab // 3
     within(x, setting, tokens, probs)
+
+
+def test_rows_by_the_logits_shape(s):
+    """[rows, vocab], further leading dimensions, or all in one: the same tokens; another number of rows is refused."""
+    import torch
+
+    from spissa_amd.device import SamplingConfig
+
+    rng = np.random.default_rng(14)
+    x, u = torch.as_tensor(logits(rng, 4, 1000, "plain"), device="cuda"), torch.as_tensor(rng.random(4).astype(np.float32), device="cuda")
+    got = []
+    for view in (x, x.view(2, 2, 1000), x.view(-1)):
+        t = torch.full((4,), -7, dtype=torch.int32, device="cuda")
+        s.sample(view, u, SamplingConfig(0.9, 40, 0.9, 0.0), t)
+        got.append(t.tolist())
+    s.sync()
+    assert got[0] == got[1] == got[2] and min(got[0]) >= 0
+    t = torch.full((4,), -7, dtype=torch.int32, device="cuda")
+    with pytest.raises(TypeError, match="rows"):
+        s.sample(x, u[:2], SamplingConfig(), t)
+    assert t.tolist() == [-7] * 4
