@@ -397,3 +397,169 @@ def test_rows_by_the_logits_shape(s):
     with pytest.raises(TypeError, match="rows"):
         s.sample(x, u[:2], SamplingConfig(), t)
     assert t.tolist() == [-7] * 4
+
+
+# ---- rows of several workgroups: the calls above, past the longest row of one
+
+
+def border(vocab):
+    """How far the sums of whole numbers may be off: half a step of each token's weight, and 2^-45 for the weights
+    themselves in 64 bits, over a sum of at least 1."""
+    return vocab * 2.0 ** -(1 + min(51, 62 - int(np.ceil(np.log2(max(2, vocab)))))) + 2.0 ** -45
+
+
+def same(x, u, rows, got):
+    left_out = 0
+    for i, (row, setting) in enumerate(zip(x, rows)):
+        token, prob, near = drafts.sample(row, u[i], *setting)
+        if near < border(len(row)):
+            left_out += 1
+            continue
+        assert got[0][i] == token, (i, setting, got[0][i], token, prob)
+        assert abs(got[1][i] - prob) <= prob * (2.0 ** -24 + border(len(row))), (i, setting)
+    assert left_out * 4 <= len(rows)
+
+
+@pytest.mark.parametrize("vocab", [12289, 32003, 262144])
+@pytest.mark.parametrize("setting", ROWS)
+def test_one_setting_for_all_long_rows(s, vocab, setting):
+    print(f"[case] sample vocab={vocab} by numbers {setting}", flush=True)
+    rng = np.random.default_rng(15)
+    x = logits(rng, 3, vocab, "plain")
+    u = rng.random(3).astype(np.float32)
+    a, b = run(s, x, u, [setting] * 3), run(s, x, u, [setting] * 3, per_row=False)
+    s.sync()
+    same(x, u, [setting] * 3, a)
+    assert np.array_equal(a[0], b[0]) and np.array_equal(a[1], b[1])
+
+
+@pytest.mark.parametrize("vocab", [32003, 128256])
+def test_long_rows_do_not_depend_on_their_neighbours(s, vocab):
+    rng = np.random.default_rng(16)
+    x = logits(rng, 48, vocab, "plain")
+    u = rng.random(48).astype(np.float32)
+    rows = [ROWS[i % len(ROWS)] for i in range(48)]
+    whole = run(s, x, u, rows)
+    for i in (0, 17, 31, 47):
+        one = run(s, x[i:i + 1], u[i:i + 1], rows[i:i + 1])
+        assert one[0][0] == whole[0][i] and one[1][0] == whole[1][i]
+    s.sync()
+
+
+@pytest.mark.parametrize("vocab", [12289, 40003])
+@pytest.mark.parametrize("setting", [(0.9, 40, 0.9, 0.0), (1.0, 0, 1.0, 0.0), (0.7, 0, 0.8, 0.01), (0.0, 0, 1.0, 0.0)])
+def test_long_rows_without_probabilities_in_an_offset_buffer(s, vocab, setting):
+    import torch
+
+    from spissa_amd.device import SamplingConfig
+
+    rng = np.random.default_rng(17)
+    x = logits(rng, 3, vocab, "plain")
+    u = rng.random(3).astype(np.float32)
+    buf = torch.full((3 * vocab + 9,), float("nan"), device="cuda")
+    buf[1:1 + 3 * vocab] = torch.as_tensor(x.reshape(-1), device="cuda")  # rows at no multiple of 16 bytes, none behind them
+    tokens = torch.full((5,), -7, dtype=torch.int32, device="cuda")
+    s.sample(buf[1:1 + 3 * vocab], torch.as_tensor(u, device="cuda"), SamplingConfig(*setting), tokens)
+    s.sync()
+    assert tokens.tolist() == [drafts.sample(x[i], u[i], *setting)[0] for i in range(3)] + [-7, -7]
+
+
+@pytest.mark.parametrize("filters", [False, True])
+@pytest.mark.parametrize("what", ["nan", "inf", "none", "u1", "u-", "unan", "t-", "tnan", "p", "m"])
+def test_bad_long_rows_are_reported_and_leave_the_others(gpu, s, what, filters):
+    """The bad number in a slice that is not the first, or in the settings."""
+    print(f"[case] bad long row {what} filters={filters}", flush=True)
+    rng = np.random.default_rng(18)
+    x = logits(rng, 3, 40001, "plain")
+    u = rng.random(3).astype(np.float32)
+    rows = [(0.8, 50, 0.95, 0.05) if filters else (0.8, 0, 1.0, 0.0)] * 3
+    if what == "nan":
+        x[1, 39999] = np.nan
+    elif what == "inf":
+        x[1, 20005] = np.inf
+    elif what == "none":
+        x[1] = -np.inf
+    elif what[0] == "u":
+        u[1] = {"u1": 1.0, "u-": -0.25, "unan": np.nan}[what]
+    else:
+        rows[1] = {"t-": (-1.0, 0, 1.0, 0.0), "tnan": (np.nan, 0, 1.0, 0.0), "p": (1.0, 0, 1.5, 0.0), "m": (1.0, 0, 1.0, -1.0)}[what]
+    tokens, probs = run(s, x, u, rows)
+    with pytest.raises(gpu.InvalidTensorDataError):
+        s.sync()
+    s.sync()
+    assert tokens[1] == -1 and probs[1] == 0
+    for i in (0, 2):
+        assert tokens[i] == drafts.sample(x[i], u[i], *rows[i])[0]
+
+
+@pytest.mark.parametrize("n,vocab", [(1025, 12289), (2051, 16001)])
+@pytest.mark.parametrize("per_row", [False, True])
+def test_more_long_rows_than_a_round_of_launches(s, n, vocab, per_row):
+    """The second round's workspace is the first's; its pointers go on where the first ended."""
+    print(f"[case] sample {n} x {vocab} per_row={per_row}", flush=True)
+    rng = np.random.default_rng(n)
+    x = logits(rng, 16, vocab, "plain")[np.arange(n) % 16]
+    u = np.minimum(rng.random(n), 1 - 2.0 ** -24).astype(np.float32)
+    for setting in [None] if per_row else [(1.0, 0, 1.0, 0.0), (0.8, 50, 0.95, 0.05)]:
+        rows = [ROWS[i % 7] for i in range(n)] if per_row else [setting] * n
+        tokens, probs = run(s, x, u, rows, per_row)
+        s.sync()
+        at = np.unique(np.concatenate([[0, 1022, 1023, 1024, n - 1], rng.integers(0, n, 12)]))
+        same(x[at], u[at], [rows[i] for i in at], (tokens[at], probs[at]))
+        assert (tokens >= 0).all() and (tokens < vocab).all()
+
+
+def test_captured_calls_of_long_rows_and_the_walk_behind_them(gpu):
+    """Two graphs of one session, each sampling long rows (by arrays, by numbers without filters) and walking a tree by what
+    came: replayed in turn with new inputs, eager calls between."""
+    import torch
+
+    from spissa_amd.device import SamplingConfig, Session
+
+    stream = torch.cuda.Stream()
+    ses = Session(0, stream=stream)
+    rng = np.random.default_rng(19)
+    parents = drafts.make_tree(rng, 12, 4)
+    with torch.cuda.stream(stream):
+        sets = []
+        for n, vocab, arrays in [(12, 20011, True), (12, 128256, False)]:
+            rows = [ROWS[i % len(ROWS)] if arrays else (0.02, 0, 1.0, 0.0) for i in range(n)]
+            cols = list(zip(*rows))
+            cfg = SamplingConfig(*(torch.tensor(c, dtype=torch.int32 if i == 1 else torch.float32, device="cuda") for i, c in enumerate(cols))
+                                 if arrays else rows[0])
+            i32 = lambda m: torch.zeros(m, dtype=torch.int32, device="cuda")  # noqa: E731
+            st = {"rows": rows, "x": torch.zeros(n, vocab, device="cuda"), "u": torch.zeros(n, device="cuda"), "p": torch.zeros(n, device="cuda"),
+                  "parents": torch.tensor(parents, dtype=torch.int32, device="cuda"), "drafted": i32(n), "t": i32(n), "walk": [i32(n), i32(1), i32(1)]}
+
+            def step(st=st, cfg=cfg, n=n):
+                ses.sample(st["x"], st["u"], cfg, st["t"], st["p"])
+                ses.tree_accept(st["parents"], st["drafted"], st["t"], [n], *st["walk"])
+
+            step()
+            sets.append((st, step))
+        ses.sync()
+        graphs = []
+        for st, step in sets:
+            graphs.append(torch.cuda.CUDAGraph())
+            with torch.cuda.graph(graphs[-1], stream=stream):
+                step()
+        walked = 0
+        for _ in range(3):
+            for (st, step), g in zip(sets, graphs):
+                n, vocab = st["x"].shape
+                x, u = logits(rng, n, vocab, "plain"), rng.random(n).astype(np.float32)
+                # drafts that sampling often confirms: the largest logit after the parent
+                drafted = np.array([x[max(0, p)].argmax() for p in parents], np.int32)
+                for name, v in (("x", x), ("u", u), ("drafted", drafted)):
+                    st[name].copy_(torch.as_tensor(v, device="cuda"))
+                st["t"].fill_(-9)
+                g.replay()
+                got = [v.cpu().numpy().copy() for v in (st["t"], st["p"], *st["walk"])]
+                same(x, u, st["rows"], got)
+                path, last = drafts.accept(parents, drafted, got[0])
+                assert got[2].tolist() == path + [-1] * (n - len(path)) and got[3][0] == len(path) and got[4][0] == last
+                walked = max(walked, len(path))
+                step()
+                ses.sync()
+                assert all(np.array_equal(a, b.cpu().numpy()) for a, b in zip(got, (st["t"], st["p"], *st["walk"])))
+        assert walked > 1
