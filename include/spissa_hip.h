@@ -587,8 +587,9 @@ typedef struct {
  * sum; d_probs[r] (d_probs may be NULL) = its own weight, as formed, over that
  * sum. d_logits [rows, vocab]. Weights are formed in 64 bits and summed as whole
  * numbers of 2^-51 (of 2^-62 times vocab's next power of two, where that is
- * more), so a row's token does not depend on the order of any sum, nor on the
- * other rows; a token whose weight rounds to 0 is never taken. A setting of the
+ * more; limits are off by half of that a token at most), so a row's token does
+ * not depend on the order of any sum, nor on the other rows; a token whose weight
+ * rounds to 0 is never taken. A setting of the
  * struct that is out of its range is INVALID_TENSOR_DATA. A row with a NaN or +infinite logit, with none above
  * -infinity, or with a setting or uniform number out of its range gets token -1
  * and probability 0, and the next spissa_session_sync() reports it. The call uses

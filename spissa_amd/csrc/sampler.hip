@@ -3,10 +3,12 @@
 //
 // All three filters keep the first tokens in the order of falling logits (equal ones
 // by index), so what is kept is known by its last token. Weights w = exp((x - max) / T)
-// are formed in 64 bits and held as whole numbers of 2^-shift: their sums are exact,
-// whatever the order, and the limits are met where the definition has them (sums in
-// single precision would move the borders of some hundred thousand tokens by 2^-24, and
-// one row in a hundred would come out another token).
+// are formed in 64 bits and held as the nearest whole numbers of 2^-shift: no sum adds an
+// error, whatever its order, and a limit lies off the definition's by the weights' own half
+// steps alone, n * 2^-(shift + 1) of the largest weight at most (n tokens: 2^-29 for 128256,
+// 2^-27 for 2^18, 2^-19 for 2^22, if all round the same way). (Sums in single precision
+// would move the borders of some hundred thousand tokens by 2^-24, and one row in a hundred
+// would come out another token.)
 //
 // A row's logits are read three times, by workgroups of a slice each (sample_ends_kernel,
 // sample_bins_kernel, sample_list_kernel):
@@ -53,8 +55,9 @@ __device__ __forceinline__ u64 token_of(float x, int i) { return (u64)sort_key(x
 __device__ __forceinline__ float logit_of(u64 token) { return key_value((unsigned)(token >> 32)); }
 __device__ __forceinline__ int index_of(u64 token) { return (int)~(unsigned)token; }
 
-// exp((x - max) / T) as 2^(n + r), |r| <= 1/2, by twelve terms of exp(r ln 2): off by at
-// most 2^-52 of itself.
+// exp((x - max) / T) as 2^y, y = n + r, |r| <= 1/2, by twelve terms of exp(r ln 2): off by
+// at most (1 + |y|) * 2^-51 of itself, as y and log2(e) / T are rounded (half of that the most
+// of 6000 formed on the host).
 struct Weigh {
   double top, inv, min_p;  // inv: log2(e) / T
   int shift;
