@@ -282,12 +282,15 @@ __device__ __forceinline__ TreeUnit tree_unit(const Args &a, int at) {
 //
 // Scales. Pieces hold 2^-23 of a number only between 2^-3 and 2^16, and 2^-25 below. Keys
 // and values are multiplied by a power of two that takes the first tile's largest to
-// 2^11..2^12. Whether a tile's largest number is above 2^15, or four channels of one of its
+// 2^11..2^12. Whether a tile's largest number is above 2^15, or eight channels of one of its
 // rows all below 2^-2 (and not 0), is known after it is written. Such a tile is loaded and written again with a scale of its own; one whose rows no scale takes
 // together (more than 2^13 apart, or one not finite) in parts, from the largest keys
 // down, each with zeros in the place of the other rows, which nobody sees in that turn. So
 // every row is held to 2^-23 of its own largest, whatever stands beside it. A row with a
-// number that is not finite is in no part, but noted: nodes that see it become NaN.
+// number that is not finite is in no part, but noted: nodes that see it become NaN. (The
+// step of 26 nodes below, 33 us: with one value of 1e6 43, with one in every tile 85, with
+// rows of 2^-40 to 2^40 182. With a key channel of 400 in every row it stays: of four
+// channels instead of eight, all small ones were common, 43 us.)
 //
 // An output row is held times a power of two, its unit: the values' scale, as long as that
 // stays. Where it changes, a row takes the new one unless that costs it what it holds: one
@@ -301,7 +304,7 @@ __device__ __forceinline__ TreeUnit tree_unit(const Args &a, int at) {
 //
 // Bound by HBM with few rows (a step of 16 sequences of up to 8192 keys, 12 nodes each, 24
 // heads on 8 of 128: 145 us, 4.8 TB/s; of one sequence, 26 nodes: 32 us, of which 6 fill and
-// drain this pipeline and 7 are the other launches), by dependent chains of LDS reads and
+// drain this pipeline and 7 are the other launches, and half a one the smallest channels), by dependent chains of LDS reads and
 // matrix instructions at two waves a SIMD with many (256 nodes over 32768 keys, 4 heads on
 // one of 256: 130 us, 265 TFLOP/s of plain products, three times that of pieces). Two waves
 // sharing 16 rows' keys, where half the waves have no rows, came to the same (64 rows over
@@ -373,15 +376,23 @@ __global__ __launch_bounds__(512, 2) void tree_attend_kernel(const TreeArgsOf<MB
                  max(__float_as_uint(x[2]) & 0x7fffffffu, __float_as_uint(x[3]) & 0x7fffffffu));
     };
     // The wave's largest magnitude, as bits (a NaN or an infinity is above the rest), and
-    // the smallest of four channels' largest less 1 (four zeros are above the rest).
+    // the smallest of eight channels' largest less 1 (eight zeros are above the rest).
     auto post = [&](int slot, const f32x4 (&cur)[8]) __attribute__((always_inline)) -> uint2 {
-      unsigned m = 0, s = ~0u;
+      unsigned m = 0, s = ~0u, of[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const unsigned of = bits_of(cur[i]);
-        m = max(m, of);
-        s = min(s, of - 1u);
+        of[i] = bits_of(cur[i]);
+        m = max(m, of[i]);
       }
+      if (values) {  // (the neighbour has the same keys' next four channels, or the ones before)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) of[i] = max(of[i], (unsigned)__builtin_amdgcn_update_dpp((int)of[i], (int)of[i], 0xB1, 0xf, 0xf, false));
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) of[i] = of[i + 1] = max(of[i], of[i + 1]);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s = min(s, of[i] - 1u);
       m = wave_max_bits(m);
       s = ~wave_max_bits(~s);
       if (lane == 0) {
@@ -523,7 +534,7 @@ __global__ __launch_bounds__(512, 2) void tree_attend_kernel(const TreeArgsOf<MB
             const int from = max(0, row_lo - base - first), to = min(32, past - base - first);
             seen = from >= 32 || to <= from ? 0u : (0xffffffffu << from) & (0xffffffffu >> (32 - to));
           }
-          if (parts) {
+          if (__builtin_expect(parts, 0)) {
             poison |= (seen & bad_lds[v]) != 0;
             seen &= take_lds[v];
           }
@@ -547,7 +558,7 @@ __global__ __launch_bounds__(512, 2) void tree_attend_kernel(const TreeArgsOf<MB
       const float off = -safe_max(m);
       int lift = 0;  // what the row's unit is above the values' scale
       const int scale = (int)(vbits >> 23);
-      if (units != scale) {
+      if (__builtin_expect(units != scale, 0)) {
         int unit = units >= 0 ? units : unit_lds[wave][col];
         float most = 0.0f;
 #pragma unroll
@@ -580,7 +591,7 @@ __global__ __launch_bounds__(512, 2) void tree_attend_kernel(const TreeArgsOf<MB
           p[i] = fast_exp2(fmaf(sc[2 * v + (i >> 2)][i & 3], f, off));
           l += p[i];
         }
-        if (lifted) {
+        if (__builtin_expect(lifted, 0)) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) p[i] = __builtin_ldexpf(p[i], lift);
         }
@@ -618,7 +629,7 @@ __global__ __launch_bounds__(512, 2) void tree_attend_kernel(const TreeArgsOf<MB
       if (tile >= t0 && mode == kLook) {
         const uint2 unfit = *reinterpret_cast<const uint2 *>(unfit_lds[tile & 1]);
         again = __builtin_amdgcn_readfirstlane(unfit.x | unfit.y) != 0;
-        if (again) {
+        if (__builtin_expect(again, 0)) {
           const unsigned km = largest(tile & 1, 4), vm = largest(tile & 1, 0);
           const unsigned ks = smallest(tile & 1, 4), vs = smallest(tile & 1, 0);
           mode = kFits;
@@ -634,7 +645,7 @@ __global__ __launch_bounds__(512, 2) void tree_attend_kernel(const TreeArgsOf<MB
       }
       const bool hold = !again && mode == kParts && __builtin_amdgcn_readfirstlane(scale_lds[2]);  // (a part of the tile is still to be written)
       const int target = again ? tile : hold ? t1 : tile + 1;
-      if (again) {
+      if (__builtin_expect(again, 0)) {
         load(tile);
         __syncthreads();  // (the tile's largest is read)
       }
@@ -642,7 +653,7 @@ __global__ __launch_bounds__(512, 2) void tree_attend_kernel(const TreeArgsOf<MB
         f32x4 cur[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) cur[i] = raw[i];
-        if (again && mode != kFits) {
+        if (__builtin_expect(again && mode != kFits, 0)) {
           if (mode == kParts) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
