@@ -25,9 +25,9 @@
 // is left out, and up to 12288 logits are one workgroup's from start to end
 // (sample_row_kernel).
 //
-// Bound by latency for a few rows (one of 128256 logits, all filters: 19 us, four launches
+// Bound by latency for a few rows (one of 128256 logits, all filters: 18 us, four launches
 // of 4 to 6 us each); for many by reads and by the weights' 35 operations in 64 bits a
-// token: 64 rows of 128256 with settings of their own 43 to 50 us (9, 15, 14, 15 us a launch;
+// token: 64 rows of 128256 with settings of their own 43 to 52 us (9, 15, 14, 15 us a launch;
 // 33 MB), five rows of 262144 without filters 15 us.
 #include <algorithm>
 #include <climits>

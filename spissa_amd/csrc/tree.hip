@@ -303,10 +303,10 @@ __device__ __forceinline__ TreeUnit tree_unit(const Args &a, int at) {
 // unit or of several; a unit of several workgroups' is merged by tree_merge_kernel.
 //
 // Bound by HBM with few rows (a step of 16 sequences of up to 8192 keys, 12 nodes each, 24
-// heads on 8 of 128: 145 us, 4.8 TB/s; of one sequence, 26 nodes: 32 us, of which 6 fill and
+// heads on 8 of 128: 145 us, 4.8 TB/s; of one sequence, 26 nodes: 32.5 us, of which 6 fill and
 // drain this pipeline and 7 are the other launches, and half a one the smallest channels), by dependent chains of LDS reads and
 // matrix instructions at two waves a SIMD with many (256 nodes over 32768 keys, 4 heads on
-// one of 256: 130 us, 265 TFLOP/s of plain products, three times that of pieces). Two waves
+// one of 256: 130 to 138 us, 250 to 265 TFLOP/s of plain products, three times that of pieces). Two waves
 // sharing 16 rows' keys, where half the waves have no rows, came to the same (64 rows over
 // 8192 keys of 8 heads of 128: 28.2 us a step against 27.2).
 //
