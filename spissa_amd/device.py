@@ -138,7 +138,7 @@ class SamplingConfig:
                 many = _many_i32 if name == "top_k" else _many_f32
                 setattr(c, "d_" + name, many(value, rows, name))
             elif name == "top_k":
-                c.top_k = max(0, int(value))
+                c.top_k = max(0, min(int(value), vocab))  # (all of them; no size_t holds any number)
             else:
                 setattr(c, name, float(value))
         return c

@@ -80,3 +80,10 @@ def test_sampling_takes_one_number_a_row(shape, rows):
 
     with pytest.raises(TypeError, match="rows"):
         Session.sample(None, torch.zeros(shape), torch.zeros(rows), SamplingConfig(), torch.zeros(rows, dtype=torch.int32))
+
+
+@pytest.mark.parametrize("top_k,kept", [(-3, 0), (0, 0), (7, 7), (100, 100), (1 << 40, 100), ((1 << 64) + 5, 100)])
+def test_a_top_k_of_any_size(top_k, kept):
+    from spissa_amd.device import SamplingConfig
+
+    assert SamplingConfig(top_k=top_k)._c(2, 100).top_k == kept
