@@ -1110,3 +1110,83 @@ def test_the_smallest_values(s, heads, past, scale, vscale):
     out = dr.run(s).cpu().numpy()
     s.sync()
     assert rows_off(out, dr.plain()[0]) <= ROW
+
+
+@pytest.mark.parametrize("heads", [(24, 8, 128), (8, 4, 256), (8, 2, 64)])
+@pytest.mark.parametrize("window,size", [(0, 1.0), (64, 1.0), (0, 1e6)])
+def test_a_gemma_chain_is_as_many_gemma_decode_steps(s, heads, window, size):
+    """With the norm, the prescale and a window; and with a value of 1e6 in the cache."""
+    from spissa_amd.rotary import KvAttentionConfig
+
+    rng = np.random.default_rng(29)
+    dr = Draft(s, rng, heads, [200], [6])
+    dr.pv[0][150] *= np.float32(size)
+    dr.parents = [[-1, 0, 1, 2, 3, 4]]
+    norm = [dev((1 + 0.25 * rng.normal(size=heads[2])).astype(np.float32)) for _ in range(2)]
+    table, *_ = tables(s, _ffi.ROPE_GEMMA, heads[2], 208)
+    with_rows(s, dr)
+    one = dr.cache(s, 0)
+    out = dev(np.zeros_like(dr.q))
+    s.gemma_tree_step(table, dev(dr.q), dev(dr.k), dev(dr.v), dr.caches, [6], dr.flat_parents(), dr.config(window), *norm, 1e-6, 0.75, out)
+    out = out.cpu().numpy()
+    cfg = KvAttentionConfig(1, *heads, True, window)
+    for t in range(6):
+        o = dev(np.zeros_like(dr.q[:1]))
+        s.gemma_decode_step(table, dev(dr.q[t:t + 1]), dev(dr.k[t:t + 1]), dev(dr.v[t:t + 1]), [one], cfg, *norm, 1e-6, 0.75, o)
+        # each side's own error, and 16 * 2^-24 of the rows of keys, whose norms are summed in different orders
+        assert rows_off(out[t:t + 1], o.cpu().numpy().astype(np.float64)) <= 2 * ROW + 16 * 2.0 ** -24 * np.sqrt(heads[2])
+    a, b = held(s, dr.caches[0], 0, 206), held(s, one, 0, 206)
+    assert rows_off(a[0], b[0].astype(np.float64)) <= 2 * 16 * 2.0 ** -24 and np.array_equal(a[1], b[1])
+    s.sync()
+
+
+@pytest.mark.parametrize("heads", OUTLIERS)
+def test_a_captured_step_replayed_with_huge_rows_and_such_as_are_not_finite(gpu, heads):
+    """Captured with ordinary rows; which tiles take turns of their own is found on the device in each replay."""
+    import torch
+
+    from spissa_amd.device import Session
+
+    rng = np.random.default_rng(30)
+    stream = torch.cuda.Stream()
+    ses = Session(0, stream=stream)
+    with torch.cuda.stream(stream):
+        dr = Draft(ses, rng, heads, [500, 70], [20, 9])
+        q, k, v, out = (torch.zeros(*x.shape, device="cuda") for x in (dr.q, dr.k, dr.v, dr.q))
+        args = (None, q, k, v, dr.caches, dr.nodes, dr.flat_parents(), dr.config(), out)
+        ses.tree_step(*args)
+        for c, p in zip(dr.caches, dr.past):
+            c.truncate(p)
+        ses.sync()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            ses.tree_step(*args)
+        sees = np.zeros(29, bool)
+        sees[:20] = drafts.seen(dr.parents[0], 0)[:, 7]
+        for size in (1.0, 1e8, np.nan, 1e-30, 1e30, 1.0):
+            dr.q, dr.k, dr.v = (rng.normal(size=x.shape).astype(np.float32) for x in (dr.q, dr.k, dr.v))
+            dr.v[7] *= np.float32(size)
+            for t, x in zip((q, k, v), (dr.q, dr.k, dr.v)):
+                t.copy_(dev(x))
+            out.fill_(np.nan)
+            graph.replay()
+            got = out.cpu().numpy()
+            if np.isnan(size):
+                with pytest.raises(gpu.InvalidTensorDataError):
+                    ses.sync()
+                dr.v[7] = 0
+                assert np.isnan(got[sees]).all()
+            else:
+                ses.sync()
+            want, _ = dr.plain()
+            at = ~sees if np.isnan(size) else np.ones(29, bool)
+            assert rows_off(got[at], want[at]) <= ROW, size
+            # and the call made eagerly has the same bits
+            for c, p in zip(dr.caches, dr.past):
+                c.truncate(p)
+            ses.tree_step(None, q, k, v, dr.caches, dr.nodes, dr.flat_parents(), dr.config(), out)
+            assert np.array_equal(out.cpu().numpy(), got, equal_nan=True)
+            if np.isnan(size):
+                with pytest.raises(gpu.InvalidTensorDataError):
+                    ses.sync()
+        ses.sync()
