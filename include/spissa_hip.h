@@ -614,9 +614,10 @@ int spissa_sample_device(spissa_session *s, const float *d_logits, const float *
  *
  * Products are f32's in all but name: queries, keys, values and softmax weights
  * as two nearest binary16 pieces (2^-23 of themselves, or, where that is more, of
- * the largest number of the same token's head; weights 2^-32 of the largest),
- * sums and softmax in f32. What other rows hold, of whatever size, changes
- * nothing of that.
+ * the largest number of the same token's head; weights, where that is more,
+ * 2^-32 of the row's largest: an output whose largest weights fall on values of
+ * 0 is off by 2^-32 of the others), sums and softmax in f32. What other rows
+ * hold, of whatever size, changes nothing of that.
  * A parent out of its range counts as -1 and is reported by the next
  * spissa_session_sync(); so is a key or value that is not finite, which makes
  * the outputs of the nodes that see it NaN, and those alone.
